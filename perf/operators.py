@@ -626,11 +626,8 @@ def _own_clip(s):
     if not hasattr(s, "views"):
         s.views = [s.view(g) for g in s.gradients]
         # side by side in one buffer, as the state of an optimizer is
-        flat, at = s.view(s.clipped), 0
-        s.into = []
-        for size in s.sizes:
-            s.into.append(tensor.subvector(flat, at, size))
-            at += size
+        flat, ends = s.view(s.clipped).buffer, np.cumsum(s.sizes).tolist()
+        s.into = [flat.sub_buffer(end - size, size) for end, size in zip(ends, s.sizes)]
         s.norm_view = s.view(s.norm)
         s.backend = optimize.Backend(tensor.check_stream(), s.case["datatype"])
     optimize.clip_gradients(s.backend, s.views, s.case["limit"], s.norm_view, s.into)
