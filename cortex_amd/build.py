@@ -44,6 +44,7 @@ SOURCES = [
     "ops_blas.cpp",
     "ops_gemm.hip",
     "ops_gemv.hip", "ops_pool.hip", "ops_conv.hip", "ops_conv_mfma.hip", "ops_lrn.hip",
+    "ops_norm.hip", "ops_experts.hip", "ops_grouped.hip", "ops_clip.hip",
 ]
 
 # -ffp-contract=off: the reference's CPU backend rounds after every JVM

@@ -32,6 +32,7 @@ TERNARY_OPS = {"select": 0}
 ACTIVATION_OPS = {"logistic": 0, "tanh": 1, "relu": 2}
 DISTRIBUTIONS = {"gaussian": 0, "flat": 1}
 POOL_OPS = {"max": 0, "avg": 1, "avg-exc-pad": 2}
+NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
 REDUCE_OPS = {"max": 0, "min": 1, "sum": 2, "mean": 3, "magnitude": 4, "magnitude-squared": 5}
 
 COPY_H2D, COPY_D2H, COPY_D2D = 0, 1, 2
@@ -169,6 +170,16 @@ PROTOTYPES = {
     "ct_gemv": [_P, _P, _L, _I, _D, _P, _L, _L, _L, _P, _L, _D, _I],
     "ct_rand": [_P, _P, _L, _I, _I, _D, _D, C.c_uint64, C.c_uint64],
     "ct_dropout_bernoulli_mask": [_P, _P, _I, _P, _L, _D, C.c_uint64, C.c_uint64],
+    "ct_norm_residual": [_P, _P, _DP, _P, _DP, _P, _P, _DP, _P, _DP, _P, _DP, _P, _P, _P, _P, _I, _I, _D, _D, _I],
+    "ct_norm_residual_gradient": [_P, _P, _DP, _P, _DP, _P, _P, _P, _P, _P, _P, _DP, _P, _DP, _P, _DP, _P, _DP, _P, _P, _DP, _P, _P,
+                                  _P, _I, _I, _D, _I],
+    "ct_route_experts": [_P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I],
+    "ct_route_experts_gradient": [_P, _P, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I],
+    "ct_grouped_gemm": [_P, _P, _L, _I, _D, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _D, _I],
+    "ct_grouped_gemm_weights": [_P, _P, _L, _L, _D, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _L, _L, _D, _I],
+    "ct_combine_experts": [_P, _P, _L, _P, _L, _L, _P, _P, _L, _L, _L, _I],
+    "ct_combine_experts_gradient": [_P, _P, _L, _P, _P, _L, _P, _L, _L, _P, _P, _L, _L, _L, _I],
+    "ct_clip_gradients": [_P, _P, _P, _P, _L, _D, _P, _I],
     "ct_adam_step": [_P, _I, _D, _D, _D, _D, _D, _D, _D, _P, _P, _P, _P, _L],
     "ct_adadelta_step": [_P, _I, _D, _D, _P, _P, _D, _P, _P, _L],
 }

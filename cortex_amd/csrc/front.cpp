@@ -314,7 +314,7 @@ bool convert(PyObject* o, T* out) {
       const unsigned long long v = PyLong_AsUnsignedLongLongMask(o);
       if (v == (unsigned long long)-1 && PyErr_Occurred()) return PyErr_Clear(), false;
       *out = reinterpret_cast<T>(v);
-      return std::is_void<typename std::remove_pointer<T>::type>::value;
+      return !std::is_same<T, const ct_dims*>::value;   // a struct is given as such
     }
     if (PyBytes_CheckExact(o) && std::is_same<T, const ct_dims*>::value && PyBytes_GET_SIZE(o) == sizeof(ct_dims)) {
       *out = reinterpret_cast<T>(PyBytes_AS_STRING(o));
@@ -368,7 +368,9 @@ Entry g_entries[] = {
     CT_ENTRY(ct_batch_normalize_update_and_apply_spatial), CT_ENTRY(ct_batch_normalize_gradients_eltwise),
     CT_ENTRY(ct_batch_normalize_gradients_spatial), CT_ENTRY(ct_gemm), CT_ENTRY(ct_gemv), CT_ENTRY(ct_rand),
     CT_ENTRY(ct_dropout_bernoulli_mask), CT_ENTRY(ct_adam_step), CT_ENTRY(ct_adadelta_step), CT_ENTRY(ct_lrn_forward),
-    CT_ENTRY(ct_lrn_backward)};
+    CT_ENTRY(ct_lrn_backward), CT_ENTRY(ct_norm_residual), CT_ENTRY(ct_norm_residual_gradient), CT_ENTRY(ct_route_experts),
+    CT_ENTRY(ct_route_experts_gradient), CT_ENTRY(ct_grouped_gemm), CT_ENTRY(ct_grouped_gemm_weights), CT_ENTRY(ct_combine_experts),
+    CT_ENTRY(ct_combine_experts_gradient), CT_ENTRY(ct_clip_gradients)};
 PyObject* g_index;     // name -> index of an entry whose address is known
 PyObject* g_library;   // the library that the addresses are of
 

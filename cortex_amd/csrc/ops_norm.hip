@@ -1,0 +1,850 @@
+// ops_norm.hip -- the norms after a block and before the next one, fused with the block's gate and residual
+// (ct_norm_residual), and their gradients.
+//
+// Forward, for a row z of the block and r of the residual:  zh = (z - m) s,  u = zh wp + bp,  out = c r + g u,
+// oh = (out - m') s',  h = oh wn + bn, s = 1 / sqrt(mean of (z - m)^2 + epsilon), m the mean or 0.
+// Backward, from dout and dh:  with the norm's transpose N^T(y) = s (y - [mean(y)] - xh mean(y xh)),
+//   d = dout + N'^T(dh wn),  dr = c d,  dg = d u,  du = d g,  dz = N^T(du wp),
+// and sums over the rows: S1 of du zh, S0 of du, T1 of dh oh, T0 of dh: the gradients of wp, bp, wn, bn.  A gate that is the
+// same for all rows is taken out of S1 and S0: its own gradient is wp S1 + bp S0, and wp's is g S1.
+//
+// A row is held in registers by LANES lanes, VPT pieces of 16 bytes to each, so that every operand is read once and every
+// result written once.  Rows that do not fit (more than 16384 floats) take the kernels at the end, which read again.
+#include <algorithm>
+#include <cmath>
+
+#include "elementwise.h"
+#include "rows.h"
+
+using namespace cthip;
+
+namespace {
+
+constexpr int kNormBlock = 256;
+
+enum GateKind { kNoGate, kScalarGate, kColumnGate, kRowGate, kFullGate };
+
+struct Matrix {
+  void* p;
+  int64_t ld;
+};
+
+struct NormArgs {
+  Matrix output, normalized, input, residual, gate;   // ld of the gate: of a full one
+  const void *post_scale, *post_bias, *pre_scale, *pre_bias;
+  void* statistics;
+  int64_t rows;
+  uint32_t width;
+  int post, pre, gate_kind;
+  double residual_scale, epsilon;
+};
+
+template <class T> __device__ __forceinline__ const T* row_of(const Matrix& m, int64_t row) { return static_cast<const T*>(m.p) + row * m.ld; }
+template <class T> __device__ __forceinline__ T* row_to(const Matrix& m, int64_t row) { return static_cast<T*>(m.p) + row * m.ld; }
+
+// The lanes that hold a row, and what each of them holds: piece t is elements N * (lane + t * LANES) and on.
+template <class T, int LANES, int VPT>
+struct Row {
+  static constexpr int N = Quad<T>::N, E = N * VPT;
+  uint32_t lane, width;
+  __device__ __forceinline__ uint32_t at(int t) const { return N * (lane + t * LANES); }
+  __device__ __forceinline__ bool has(int t, int e) const { return at(t) + e < width; }
+  __device__ __forceinline__ void load(const T* p, T (&x)[E], T absent = 0) const {
+#pragma unroll
+    for (int t = 0; t < VPT; ++t) {
+      if (at(t) + N <= width) {
+        const Quad<T> q = load_quad(p + at(t));
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[t * N + e] = q.v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[t * N + e] = has(t, e) ? p[at(t) + e] : absent;
+      }
+    }
+  }
+  // absent pointer: `fill` everywhere
+  __device__ __forceinline__ void load_or(const void* p, T fill, T (&x)[E]) const {
+    if (p) load(static_cast<const T*>(p), x);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = fill;
+    }
+  }
+  __device__ __forceinline__ void store(T* p, const T (&x)[E]) const {
+#pragma unroll
+    for (int t = 0; t < VPT; ++t) {
+      if (at(t) + N <= width) {
+        Quad<T> q;
+#pragma unroll
+        for (int e = 0; e < N; ++e) q.v[e] = x[t * N + e];
+        store_quad(p + at(t), q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (has(t, e)) p[at(t) + e] = x[t * N + e];
+      }
+    }
+  }
+};
+
+// Sums of K values over the LANES lanes of a row, in all of them.  A row of more than a wave is a whole block's; `lds` holds
+// K values to a wave, twice, used in turn so that one barrier a call is enough.
+template <class T, int LANES, int K>
+__device__ __forceinline__ void row_sum(T (&v)[K], T* lds, int& turn) {
+#pragma unroll
+  for (int m = (LANES < 64 ? LANES : 64) / 2; m > 0; m >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], m);
+  if constexpr (LANES > 64) {
+    constexpr int W = LANES / 64;
+    T* mine = lds + turn * (3 * W);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) mine[k * W + threadIdx.x / 64] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = mine[k * W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v[k] += mine[k * W + w];
+    }
+  }
+}
+
+template <class T> __device__ __forceinline__ T rate_of(T mean_square, T epsilon) { return T(1) / (T)sqrt(mean_square + epsilon); }
+
+template <class T, int LANES, int VPT>
+__global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_kernel(const NormArgs a) {
+  constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
+  using R = Row<T, LANES, VPT>;
+  constexpr int E = R::E, N = R::N;
+  __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
+  int turn = 0;
+  const R at{threadIdx.x % LANES, a.width};
+  const T inverse = T(1) / (T)a.width, epsilon = (T)a.epsilon;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * kRows) {
+    T x[E], y[E];
+    at.load(row_of<T>(a.input, row), x);
+    if (a.residual.p) at.load(row_of<T>(a.residual, row), y);
+    // the norm of x in place, its statistics to `place`
+    auto norm = [&](T (&x)[E], int kind, const void* scale, const void* bias, int place) {
+      T mean[1] = {0}, square[1] = {0};
+      T w[E], b[E];
+      at.load_or(scale, T(1), w);
+      if (bias) at.load(static_cast<const T*>(bias), b);
+      if (kind == CT_NORM_LAYER) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) mean[0] += x[i];
+        row_sum<T, LANES>(mean, lds, turn);
+        mean[0] *= inverse;
+#pragma unroll
+        for (int t = 0; t < VPT; ++t)
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[t * N + e] = at.has(t, e) ? x[t * N + e] - mean[0] : T(0);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) square[0] += x[i] * x[i];
+      row_sum<T, LANES>(square, lds, turn);
+      const T rate = rate_of(square[0] * inverse, epsilon);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = x[i] * rate * w[i];
+      if (bias) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] += b[i];
+      }
+      if (a.statistics && at.lane == 0) {
+        T* to = static_cast<T*>(a.statistics) + place * a.rows + row;
+        to[0] = mean[0];
+        to[a.rows] = rate;
+      }
+    };
+    auto no_norm = [&](int place) {
+      if (!a.statistics || at.lane != 0) return;
+      T* to = static_cast<T*>(a.statistics) + place * a.rows + row;
+      to[0] = 0;
+      to[a.rows] = 1;
+    };
+    if (a.post != CT_NORM_NONE) norm(x, a.post, a.post_scale, a.post_bias, 0);
+    else no_norm(0);
+    if (a.gate_kind == kScalarGate || a.gate_kind == kRowGate) {
+      const T g = static_cast<const T*>(a.gate.p)[a.gate_kind == kRowGate ? row * a.gate.ld : 0];
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] *= g;
+    } else if (a.gate_kind != kNoGate) {
+      T g[E];
+      at.load(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), g);
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] *= g[i];
+    }
+    if (a.residual.p) {
+      const T c = (T)a.residual_scale;
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = c * y[i] + x[i];
+    }
+#pragma unroll
+    for (int t = 0; t < VPT; ++t)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (!at.has(t, e)) x[t * N + e] = 0;   // a bias has no part beyond the row
+    at.store(row_to<T>(a.output, row), x);
+    if (a.pre == CT_NORM_NONE) {
+      no_norm(2);
+      continue;
+    }
+    norm(x, a.pre, a.pre_scale, a.pre_bias, 2);
+    at.store(row_to<T>(a.normalized, row), x);
+  }
+}
+
+// ------------------------------------------------------------------ gradient
+
+struct NormGradientArgs {
+  Matrix input_gradient, residual_gradient, gate_gradient, output_gradient, normalized_gradient, input, output, gate;
+  const void *post_scale, *post_bias, *pre_scale;
+  const void* statistics;
+  void* partial;             // [slots][blocks][width]
+  int64_t rows;
+  uint32_t width, blocks;
+  int post, pre, gate_kind;
+  int slot[4];               // of S1, S0, T1, T0 in partial; negative: not wanted
+  double residual_scale;
+};
+
+// Whether the gate is a factor of all rows' sums: then it is left out of them.
+__device__ __forceinline__ bool common_gate(int kind) { return kind == kNoGate || kind == kScalarGate || kind == kColumnGate; }
+
+template <class T, int LANES, int VPT, bool kSums, bool kBiases>
+__global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_gradient_kernel(const NormGradientArgs a) {
+  constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
+  using R = Row<T, LANES, VPT>;
+  constexpr int E = R::E, N = R::N;
+  __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
+  int turn = 0;
+  const R at{threadIdx.x % LANES, a.width};
+  const T inverse = T(1) / (T)a.width;
+  T s1[kSums ? E : 1] = {}, t1[kSums ? E : 1] = {}, s0[kBiases ? E : 1] = {}, t0[kBiases ? E : 1] = {};
+  const T* statistics = static_cast<const T*>(a.statistics);
+  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * kRows) {
+    T d[E];
+    if (a.output_gradient.p) at.load(row_of<T>(a.output_gradient, row), d);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] = 0;
+    }
+    T z[E];
+    at.load(row_of<T>(a.input, row), z);
+    if (a.pre != CT_NORM_NONE && a.normalized_gradient.p) {
+      T dh[E], oh[E], w[E];
+      at.load(row_of<T>(a.normalized_gradient, row), dh);
+      at.load(row_of<T>(a.output, row), oh);
+      at.load_or(a.pre_scale, T(1), w);
+      const T mean = statistics[2 * a.rows + row], rate = statistics[3 * a.rows + row];
+      T sums[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        oh[i] = (oh[i] - mean) * rate;
+        if constexpr (kSums) t1[i] += dh[i] * oh[i];
+        if constexpr (kBiases) t0[i] += dh[i];
+        const T y = dh[i] * w[i];   // zero beyond the row
+        sums[0] += y;
+        sums[1] += y * oh[i];
+        dh[i] = y;
+      }
+      row_sum<T, LANES>(sums, lds, turn);
+      const T first = a.pre == CT_NORM_LAYER ? sums[0] * inverse : T(0), second = sums[1] * inverse;
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] += rate * (dh[i] - first - oh[i] * second);
+    }
+#pragma unroll
+    for (int t = 0; t < VPT; ++t)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (!at.has(t, e)) d[t * N + e] = 0;
+    if (a.residual_gradient.p) {
+      T dr[E];
+      const T c = (T)a.residual_scale;
+#pragma unroll
+      for (int i = 0; i < E; ++i) dr[i] = c * d[i];
+      at.store(row_to<T>(a.residual_gradient, row), dr);
+    }
+    // zh; its sums; the gate's gradient; dz
+    const bool post = a.post != CT_NORM_NONE;
+    const T mean = post ? statistics[row] : T(0), rate = post ? statistics[a.rows + row] : T(1);
+    T w[E], b[E], g[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) z[i] = (z[i] - mean) * rate;
+    at.load_or(post ? a.post_scale : nullptr, T(1), w);
+    at.load_or(post ? a.post_bias : nullptr, T(0), b);
+    T row_gate = 1;
+    if (a.gate_kind == kScalarGate || a.gate_kind == kRowGate)
+      row_gate = static_cast<const T*>(a.gate.p)[a.gate_kind == kRowGate ? row * a.gate.ld : 0];
+    if (a.gate_kind == kColumnGate || a.gate_kind == kFullGate)
+      at.load(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), g);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) g[i] = row_gate;
+    }
+    if constexpr (kSums) {
+      if (common_gate(a.gate_kind)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s1[i] += d[i] * z[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s1[i] += g[i] * d[i] * z[i];
+      }
+    }
+    if constexpr (kBiases) {
+      if (common_gate(a.gate_kind)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s0[i] += d[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s0[i] += g[i] * d[i];
+      }
+    }
+    if (a.gate_kind == kFullGate && a.gate_gradient.p) {
+      T dg[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) dg[i] = d[i] * (z[i] * w[i] + b[i]);
+      at.store(row_to<T>(a.gate_gradient, row), dg);
+    }
+    const bool of_row = a.gate_kind == kRowGate && a.gate_gradient.p;
+    if (post || of_row) {
+      T sums[3] = {0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (of_row) sums[2] += d[i] * (z[i] * w[i] + b[i]);
+        d[i] *= g[i] * w[i];
+        sums[0] += d[i];
+        sums[1] += d[i] * z[i];
+      }
+      row_sum<T, LANES>(sums, lds, turn);
+      if (of_row && at.lane == 0) static_cast<T*>(a.gate_gradient.p)[row * a.gate_gradient.ld] = sums[2];
+      if (post) {
+        const T first = a.post == CT_NORM_LAYER ? sums[0] * inverse : T(0), second = sums[1] * inverse;
+#pragma unroll
+        for (int i = 0; i < E; ++i) d[i] = rate * (d[i] - first - z[i] * second);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] *= g[i];
+    }
+    if (a.input_gradient.p) at.store(row_to<T>(a.input_gradient, row), d);
+  }
+  if constexpr (kSums) {
+    // the sums of the block's rows, in the order of their groups of lanes
+    constexpr int kSumLds = kRows > 1 ? kRows * LANES * E : 1;
+    __shared__ T shared[kSumLds];
+    auto put = [&](int slot, const T (&of)[E]) {
+      if (slot < 0) return;
+      T* to = static_cast<T*>(a.partial) + ((int64_t)slot * a.blocks + blockIdx.x) * a.width;
+      if constexpr (kRows > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i) shared[(threadIdx.x / LANES * E + i) * LANES + at.lane] = of[i];
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < LANES * E; i += kThreads) {
+          const uint32_t lane = i % LANES, e = i / LANES, column = N * (lane + e / N * LANES) + e % N;
+          T sum = shared[i];
+#pragma unroll
+          for (int r = 1; r < kRows; ++r) sum += shared[r * LANES * E + i];
+          if (column < a.width) to[column] = sum;
+        }
+      } else {
+        at.store(to, of);
+      }
+    };
+    put(a.slot[0], s1);
+    put(a.slot[2], t1);
+    if constexpr (kBiases) {
+      put(a.slot[1], s0);
+      put(a.slot[3], t0);
+    }
+  }
+}
+
+struct NormFinishArgs {
+  const void* partial;
+  const void *post_scale, *post_bias;
+  const void* gate;
+  void *gate_gradient, *post_scale_gradient, *post_bias_gradient, *pre_scale_gradient, *pre_bias_gradient;
+  void* by_column;   // of a scalar gate's gradient: its part of each column
+  uint32_t width, blocks;
+  int slot[4];
+  int gate_kind;
+};
+
+// The blocks' sums of 16 columns, added in their order within each of 16 runs of blocks, in double.
+template <class T>
+__global__ void __launch_bounds__(256) norm_finish_kernel(const NormFinishArgs a) {
+  __shared__ double lds[4][16][16];
+  const uint32_t column = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    double sum = 0;
+    if (a.slot[s] >= 0 && column < a.width)
+      for (uint32_t b = run; b < a.blocks; b += 16)
+        sum += (double)static_cast<const T*>(a.partial)[((int64_t)a.slot[s] * a.blocks + b) * a.width + column];
+    lds[s][run][threadIdx.x % 16] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 || column >= a.width) return;
+  double sums[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    sums[s] = lds[s][0][threadIdx.x];
+    for (int r = 1; r < 16; ++r) sums[s] += lds[s][r][threadIdx.x];
+  }
+  double gate = 1;
+  if (a.gate_kind == kScalarGate) gate = (double)*static_cast<const T*>(a.gate);
+  if (a.gate_kind == kColumnGate) gate = (double)static_cast<const T*>(a.gate)[column];
+  auto store = [&](void* to, double v) {
+    if (to) static_cast<T*>(to)[column] = (T)v;
+  };
+  store(a.post_scale_gradient, gate * sums[0]);
+  store(a.post_bias_gradient, gate * sums[1]);
+  store(a.pre_scale_gradient, sums[2]);
+  store(a.pre_bias_gradient, sums[3]);
+  const double scale = a.post_scale ? (double)static_cast<const T*>(a.post_scale)[column] : 1.0;
+  const double bias = a.post_bias ? (double)static_cast<const T*>(a.post_bias)[column] : 0.0;
+  const double of_gate = scale * sums[0] + (a.slot[1] >= 0 ? bias * sums[1] : 0.0);
+  if (a.gate_kind == kColumnGate) store(a.gate_gradient, of_gate);
+  if (a.by_column) static_cast<double*>(a.by_column)[column] = of_gate;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) norm_scalar_gate_kernel(const double* by_column, uint32_t width, T* gradient) {
+  __shared__ double lds[4];
+  double sum = 0;
+  for (uint32_t c = threadIdx.x; c < width; c += 256) sum += by_column[c];
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) *gradient = (T)(lds[0] + lds[1] + lds[2] + lds[3]);
+}
+
+// ------------------------------------------------------------------ rows that do not fit registers
+
+constexpr int kLongBlock = 1024;
+
+template <int K> __device__ __forceinline__ void long_sum(double (&v)[K], double* lds) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) lds[k * 16 + threadIdx.x / 64] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = lds[k * 16];
+    for (int w = 1; w < 16; ++w) v[k] += lds[k * 16 + w];
+  }
+}
+
+template <class T> __device__ __forceinline__ T or_else(const void* p, int64_t i, T absent) { return p ? static_cast<const T*>(p)[i] : absent; }
+template <class T> __device__ __forceinline__ T gate_at(const Matrix& gate, int kind, int64_t row, uint32_t c) {
+  const T* g = static_cast<const T*>(gate.p);
+  return kind == kNoGate ? T(1) : kind == kScalarGate ? g[0] : kind == kColumnGate ? g[c] : kind == kRowGate ? g[row * gate.ld] : g[row * gate.ld + c];
+}
+
+template <class T>
+__global__ void __launch_bounds__(kLongBlock) norm_long_kernel(const NormArgs a) {
+  __shared__ double lds[16];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    auto statistics = [&](const T* x, int kind, int place, T* mean, T* rate) {
+      double m[1] = {0}, q[1] = {0};
+      *mean = 0;
+      *rate = 1;
+      if (kind == CT_NORM_LAYER) {
+        for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock) m[0] += (double)x[c];
+        long_sum(m, lds);
+        *mean = (T)(m[0] / a.width);
+      }
+      if (kind != CT_NORM_NONE) {
+        for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock) {
+          const double y = (double)x[c] - (kind == CT_NORM_LAYER ? m[0] / a.width : 0.0);
+          q[0] += y * y;
+        }
+        long_sum(q, lds);
+        *rate = (T)(1.0 / sqrt(q[0] / a.width + a.epsilon));
+      }
+      if (a.statistics && threadIdx.x == 0) {
+        T* to = static_cast<T*>(a.statistics) + place * a.rows + row;
+        to[0] = *mean;
+        to[a.rows] = *rate;
+      }
+    };
+    const T* z = row_of<T>(a.input, row);
+    T* out = row_to<T>(a.output, row);
+    T mean, rate;
+    statistics(z, a.post, 0, &mean, &rate);
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock) {
+      T u = z[c];
+      if (a.post != CT_NORM_NONE) u = (u - mean) * rate * or_else<T>(a.post_scale, c, 1) + or_else<T>(a.post_bias, c, 0);
+      u *= gate_at<T>(a.gate, a.gate_kind, row, c);
+      out[c] = a.residual.p ? (T)a.residual_scale * row_of<T>(a.residual, row)[c] + u : u;
+    }
+    __syncthreads();   // a lane reads again only what it wrote
+    statistics(out, a.pre, 2, &mean, &rate);
+    if (a.pre == CT_NORM_NONE) continue;
+    T* h = row_to<T>(a.normalized, row);
+    for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock)
+      h[c] = (out[c] - mean) * rate * or_else<T>(a.pre_scale, c, 1) + or_else<T>(a.pre_bias, c, 0);
+  }
+}
+
+// means [4][rows]: of y and y oh of the norm before the next block, of y and y zh of the one after this
+template <class T>
+struct LongRow {
+  const NormGradientArgs& a;
+  const double* means;
+  int64_t row;
+  T post_mean, post_rate, pre_mean, pre_rate;
+  __device__ __forceinline__ LongRow(const NormGradientArgs& a, const double* means, int64_t row) : a(a), means(means), row(row) {
+    const T* s = static_cast<const T*>(a.statistics);
+    post_mean = a.post != CT_NORM_NONE ? s[row] : T(0);
+    post_rate = a.post != CT_NORM_NONE ? s[a.rows + row] : T(1);
+    pre_mean = before() ? s[2 * a.rows + row] : T(0);
+    pre_rate = before() ? s[3 * a.rows + row] : T(1);
+  }
+  __device__ __forceinline__ bool before() const { return a.pre != CT_NORM_NONE && a.normalized_gradient.p; }
+  __device__ __forceinline__ T dh(uint32_t c) const { return row_of<T>(a.normalized_gradient, row)[c]; }
+  __device__ __forceinline__ T oh(uint32_t c) const { return (row_of<T>(a.output, row)[c] - pre_mean) * pre_rate; }
+  __device__ __forceinline__ T zh(uint32_t c) const { return (row_of<T>(a.input, row)[c] - post_mean) * post_rate; }
+  __device__ __forceinline__ T post_scale(uint32_t c) const { return a.post != CT_NORM_NONE ? or_else<T>(a.post_scale, c, 1) : T(1); }
+  __device__ __forceinline__ T u(uint32_t c) const {
+    return zh(c) * post_scale(c) + (a.post != CT_NORM_NONE ? or_else<T>(a.post_bias, c, 0) : T(0));
+  }
+  __device__ __forceinline__ T gate(uint32_t c) const { return gate_at<T>(a.gate, a.gate_kind, row, c); }
+  __device__ __forceinline__ double d(uint32_t c) const {
+    double v = a.output_gradient.p ? (double)row_of<T>(a.output_gradient, row)[c] : 0.0;
+    if (before()) {
+      const double y = (double)dh(c) * (double)or_else<T>(a.pre_scale, c, 1);
+      v += (double)pre_rate * (y - (a.pre == CT_NORM_LAYER ? means[row] : 0.0) - (double)oh(c) * means[a.rows + row]);
+    }
+    return v;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kLongBlock) norm_long_means_kernel(const NormGradientArgs a, double* means) {
+  __shared__ double lds[48];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const LongRow<T> r(a, means, row);
+    double p[2] = {0, 0}, q[3] = {0, 0, 0};
+    if (r.before()) {
+      for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock) {
+        const double y = (double)r.dh(c) * (double)or_else<T>(a.pre_scale, c, 1);
+        p[0] += y;
+        p[1] += y * (double)r.oh(c);
+      }
+      long_sum(p, lds);
+    }
+    if (threadIdx.x == 0) {
+      means[row] = p[0] / a.width;
+      means[a.rows + row] = p[1] / a.width;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.width; c += kLongBlock) {
+      const double d = r.d(c), y = d * (double)(r.gate(c) * r.post_scale(c));
+      q[0] += y;
+      q[1] += y * (double)r.zh(c);
+      q[2] += d * (double)r.u(c);
+    }
+    long_sum(q, lds);
+    if (threadIdx.x == 0) {
+      means[2 * a.rows + row] = q[0] / a.width;
+      means[3 * a.rows + row] = q[1] / a.width;
+      if (a.gate_kind == kRowGate && a.gate_gradient.p) static_cast<T*>(a.gate_gradient.p)[row * a.gate_gradient.ld] = (T)q[2];
+    }
+  }
+}
+
+// Block (x, y): 256 columns of every a.blocks-th row.
+template <class T>
+__global__ void __launch_bounds__(256) norm_long_sums_kernel(const NormGradientArgs a, const double* means) {
+  const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.width) return;
+  double sums[4] = {0, 0, 0, 0};
+  for (int64_t row = blockIdx.y; row < a.rows; row += a.blocks) {
+    const LongRow<T> r(a, means, row);
+    const double d = r.d(c) * (common_gate(a.gate_kind) ? 1.0 : (double)r.gate(c));
+    sums[0] += d * (double)r.zh(c);
+    sums[1] += d;
+    if (r.before()) {
+      sums[2] += (double)r.dh(c) * (double)r.oh(c);
+      sums[3] += (double)r.dh(c);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    if (a.slot[s] >= 0) static_cast<T*>(a.partial)[((int64_t)a.slot[s] * a.blocks + blockIdx.y) * a.width + c] = (T)sums[s];
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) norm_long_apply_kernel(const NormGradientArgs a, const double* means) {
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const LongRow<T> r(a, means, row);
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.width) continue;
+    const double d = r.d(c), gate = (double)r.gate(c);
+    double dz = d * gate;
+    const T u = r.u(c);
+    if (a.post != CT_NORM_NONE) {
+      dz *= (double)r.post_scale(c);
+      dz = (double)r.post_rate * (dz - (a.post == CT_NORM_LAYER ? means[2 * a.rows + row] : 0.0) - (double)r.zh(c) * means[3 * a.rows + row]);
+    }
+    if (a.gate_kind == kFullGate && a.gate_gradient.p) row_to<T>(a.gate_gradient, row)[c] = (T)(d * (double)u);
+    if (a.residual_gradient.p) row_to<T>(a.residual_gradient, row)[c] = (T)((double)(T)a.residual_scale * d);
+    if (a.input_gradient.p) row_to<T>(a.input_gradient, row)[c] = (T)dz;
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+// Calls f with the lanes of a row and the pieces to a lane that hold `width` elements; false if none do.
+template <class T, class F>
+bool with_shape(uint32_t width, F f) {
+  constexpr uint32_t N = Quad<T>::N;
+  const uint32_t pieces = (width + N - 1) / N;
+#define CT_SHAPE(L, V) \
+  if (pieces <= L * V) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>()), true
+  CT_SHAPE(16, 1); CT_SHAPE(16, 2); CT_SHAPE(16, 4);
+  CT_SHAPE(64, 2); CT_SHAPE(64, 4);
+  CT_SHAPE(256, 2); CT_SHAPE(256, 4);
+  CT_SHAPE(1024, 2); CT_SHAPE(1024, 4);
+#undef CT_SHAPE
+  return false;
+}
+
+constexpr int64_t kMostNormBlocks = 1 << 20;
+constexpr int64_t kMostSumBytes = int64_t(32) << 20;
+
+template <class T>
+int norm_typed(hipStream_t s, const NormArgs& a) {
+  const bool taken = with_shape<T>(a.width, [&](auto lanes, auto pieces) {
+    constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
+    const int64_t blocks = std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
+    hipLaunchKernelGGL((norm_kernel<T, L, V>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+  });
+  if (!taken) hipLaunchKernelGGL((norm_long_kernel<T>), dim3((uint32_t)std::min(a.rows, kMostNormBlocks)), dim3(kLongBlock), 0, s, a);
+  note_kernel(taken ? "norm_residual" : "norm_residual_long");
+  return after_launch(s);
+}
+
+template <class T>
+int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
+  const int slots = std::max({a.slot[0], a.slot[1], a.slot[2], a.slot[3]}) + 1;
+  const bool sums = slots > 0, biases = a.slot[1] >= 0 || a.slot[3] >= 0;
+  const bool fits = with_shape<T>(a.width, [](auto, auto) {});
+  int64_t rows_a_block = 1;
+  with_shape<T>(a.width, [&](auto lanes, auto) { rows_a_block = std::max(1, kNormBlock / decltype(lanes)::value); });
+  // whose sums the last launch adds
+  const int64_t most_blocks = std::max<int64_t>(1, std::min<int64_t>(512, kMostSumBytes / ((int64_t)std::max(slots, 1) * a.width * (int64_t)sizeof(T))));
+  a.blocks = f.blocks = (uint32_t)std::min((a.rows + rows_a_block - 1) / rows_a_block, most_blocks);
+  const size_t of_sums = (size_t)slots * a.blocks * a.width * sizeof(T), of_columns = (size_t)a.width * sizeof(double);
+  const size_t of_means = fits ? 0 : (size_t)4 * a.rows * sizeof(double);
+  void* scratch = nullptr;
+  if (int rc = stream_scratch(s, of_columns + of_means + of_sums, &scratch)) return rc;
+  double* by_column = static_cast<double*>(scratch);
+  double* means = by_column + a.width;
+  a.partial = means + (fits ? 0 : 4 * a.rows);
+  f.partial = a.partial;
+  if (f.by_column) f.by_column = by_column;
+  if (a.rows == 0) {
+    // sums of no rows
+  } else if (fits) {
+    with_shape<T>(a.width, [&](auto lanes, auto pieces) {
+      constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
+      const int64_t blocks = sums ? a.blocks : std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
+      if (biases) hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, true, true>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+      else if (sums) hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, true, false>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, false, false>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+    });
+  } else {
+    const uint32_t columns = (a.width + 255) / 256;
+    hipLaunchKernelGGL((norm_long_means_kernel<T>), dim3((uint32_t)std::min(a.rows, kMostNormBlocks)), dim3(kLongBlock), 0, s, a, means);
+    if (sums) hipLaunchKernelGGL((norm_long_sums_kernel<T>), dim3(columns, a.blocks), dim3(256), 0, s, a, means);
+    hipLaunchKernelGGL((norm_long_apply_kernel<T>), dim3(columns, (uint32_t)std::min<int64_t>(a.rows, 4096)), dim3(256), 0, s, a, means);
+  }
+  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 15) / 16), dim3(256), 0, s, f);
+  if (f.by_column) hipLaunchKernelGGL((norm_scalar_gate_kernel<T>), dim3(1), dim3(256), 0, s, by_column, a.width, static_cast<T*>(f.gate_gradient));
+  note_kernel(fits ? "norm_residual_gradient" : "norm_residual_gradient_long");
+  return after_launch(s);
+}
+
+// A [rows, width] operand; dimensions of one are a row.
+int read_matrix(const char* what, const void* p, const ct_dims* d, int64_t rows, int64_t width, Matrix* out) {
+  *out = Matrix{const_cast<void*>(p), 0};
+  if (!p) return CT_OK;
+  CT_REQUIRE(d && (d->ndim == 1 || d->ndim == 2), "%s: one or two dimensions are taken", what);
+  const int last = d->ndim - 1;
+  for (int i = 0; i <= last; ++i) CT_REQUIRE(!d->index[i], "%s: no indexed dimension is taken", what);
+  CT_REQUIRE((last ? d->shape[0] : 1) == rows && d->shape[last] == width, "%s is [%lld, %lld], [%lld, %lld] is needed", what,
+             (long long)(last ? d->shape[0] : 1), (long long)d->shape[last], (long long)rows, (long long)width);
+  CT_REQUIRE(width <= 1 || d->strides[last] == 1, "%s: the innermost stride must be 1", what);
+  out->ld = last ? d->strides[0] : width;
+  if (rows == 1) out->ld = std::max(out->ld, width);
+  CT_REQUIRE(out->ld >= width, "%s: column stride %lld below the row's length", what, (long long)out->ld);
+  return CT_OK;
+}
+
+int read_gate(const char* what, const void* p, const ct_dims* d, int64_t rows, int64_t width, Matrix* out, int* kind) {
+  *out = Matrix{const_cast<void*>(p), 0};
+  *kind = kNoGate;
+  if (!p) return CT_OK;
+  CT_REQUIRE(d && (d->ndim == 1 || d->ndim == 2), "%s: one or two dimensions are taken", what);
+  const int last = d->ndim - 1;
+  for (int i = 0; i <= last; ++i) CT_REQUIRE(!d->index[i], "%s: no indexed dimension is taken", what);
+  const int64_t r = last ? d->shape[0] : 1, w = d->shape[last];
+  CT_REQUIRE((r == rows || r == 1) && (w == width || w == 1), "%s is [%lld, %lld]: [%lld or 1, %lld or 1] is needed", what, (long long)r,
+             (long long)w, (long long)rows, (long long)width);
+  const bool by_row = r == rows && rows > 1, by_column = w == width && width > 1;
+  CT_REQUIRE(!by_column || d->strides[last] == 1, "%s: the innermost stride must be 1", what);
+  *kind = by_row ? (by_column ? kFullGate : kRowGate) : by_column ? kColumnGate : kScalarGate;
+  out->ld = by_row ? d->strides[0] : width;
+  CT_REQUIRE(!by_row || out->ld >= w, "%s: column stride %lld below the row's length", what, (long long)out->ld);
+  return CT_OK;
+}
+
+RowRange range_of(const Matrix& m, int64_t rows, int64_t width) { return {m.p, rows, width, m.ld}; }
+// Another matrix's elements, other than by being that matrix.
+bool meets_other(const Matrix& a, const Matrix& b, int64_t rows, int64_t width, int64_t size) {
+  return !(a.p == b.p && (a.ld == b.ld || rows == 1)) && rows_meet(range_of(a, rows, width), range_of(b, rows, width), size);
+}
+RowRange gate_range(const Matrix& m, int kind, int64_t rows, int64_t width) {
+  switch (kind) {
+    case kScalarGate: return {m.p, 1, 1, 1};
+    case kColumnGate: return {m.p, 1, width, width};
+    case kRowGate: return {m.p, rows, 1, m.ld};
+    case kFullGate: return {m.p, rows, width, m.ld};
+    default: return {nullptr, 0, 0, 1};
+  }
+}
+bool known_norm(int kind) { return kind == CT_NORM_NONE || kind == CT_NORM_RMS || kind == CT_NORM_LAYER; }
+constexpr int64_t kMostWidth = (int64_t(1) << 30);
+
+#define CT_TRY(expr) \
+  if (int rc__ = (expr)) return rc__
+
+}  // namespace
+
+extern "C" {
+
+int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, void* normalized, const ct_dims* normalized_dims,
+                     void* statistics, const void* input, const ct_dims* input_dims, const void* residual,
+                     const ct_dims* residual_dims, const void* gate, const ct_dims* gate_dims, const void* post_scale,
+                     const void* post_bias, const void* pre_scale, const void* pre_bias, int post_kind, int pre_kind,
+                     double residual_scale, double epsilon, int dtype) {
+  CT_REQUIRE(dtype == CT_F32 || dtype == CT_F64, "ct_norm_residual: datatype must be float or double");
+  CT_REQUIRE(known_norm(post_kind) && known_norm(pre_kind), "ct_norm_residual: unknown kind of norm");
+  CT_REQUIRE(epsilon >= 0, "ct_norm_residual: epsilon must not be negative");
+  CT_REQUIRE(output_dims && (output_dims->ndim == 1 || output_dims->ndim == 2), "output: one or two dimensions are taken");
+  const int64_t rows = output_dims->ndim == 2 ? output_dims->shape[0] : 1, width = output_dims->shape[output_dims->ndim - 1];
+  CT_REQUIRE(rows >= 0 && width >= 0 && width <= kMostWidth, "ct_norm_residual: bad extent");
+  if (rows == 0 || width == 0) return CT_OK;
+  CT_REQUIRE(output && input && (normalized || pre_kind == CT_NORM_NONE), "ct_norm_residual: null buffer");
+  NormArgs a{};
+  CT_TRY(read_matrix("output", output, output_dims, rows, width, &a.output));
+  CT_TRY(read_matrix("input", input, input_dims, rows, width, &a.input));
+  CT_TRY(read_matrix("residual", residual, residual_dims, rows, width, &a.residual));
+  CT_TRY(read_matrix("normalized", pre_kind == CT_NORM_NONE ? nullptr : normalized, normalized_dims, rows, width, &a.normalized));
+  CT_TRY(read_gate("gate", gate, gate_dims, rows, width, &a.gate, &a.gate_kind));
+  const int64_t size = dtype_size(dtype);
+  const RowRange of_gate = gate_range(a.gate, a.gate_kind, rows, width);
+  for (const Matrix* to : {&a.output, &a.normalized}) {
+    const RowRange range = range_of(*to, rows, width);
+    bool bad = meets_other(*to, a.input, rows, width, size) || meets_other(*to, a.residual, rows, width, size) || rows_meet(range, of_gate, size);
+    for (const void* p : {post_scale, post_bias, pre_scale, pre_bias}) bad = bad || rows_meet(range, {p, 1, width, width}, size);
+    bad = bad || rows_meet(range, {statistics, 1, 4 * rows, 4 * rows}, size);
+    CT_REQUIRE(!bad, "ct_norm_residual: a result overlaps an operand");
+  }
+  CT_REQUIRE(!rows_meet(range_of(a.output, rows, width), range_of(a.normalized, rows, width), size), "ct_norm_residual: the results overlap");
+  a.post_scale = post_scale; a.post_bias = post_bias; a.pre_scale = pre_scale; a.pre_bias = pre_bias;
+  a.statistics = statistics;
+  a.rows = rows; a.width = (uint32_t)width;
+  a.post = post_kind; a.pre = pre_kind;
+  a.residual_scale = residual_scale; a.epsilon = epsilon;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == CT_F32 ? norm_typed<float>(s, a) : norm_typed<double>(s, a);
+}
+
+int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims, void* residual_gradient,
+                              const ct_dims* residual_gradient_dims, void* gate_gradient, void* post_scale_gradient,
+                              void* post_bias_gradient, void* pre_scale_gradient, void* pre_bias_gradient,
+                              const void* output_gradient, const ct_dims* output_gradient_dims, const void* normalized_gradient,
+                              const ct_dims* normalized_gradient_dims, const void* input, const ct_dims* input_dims,
+                              const void* output, const ct_dims* output_dims, const void* statistics, const void* gate,
+                              const ct_dims* gate_dims, const void* post_scale, const void* post_bias, const void* pre_scale,
+                              int post_kind, int pre_kind, double residual_scale, int dtype) {
+  CT_REQUIRE(dtype == CT_F32 || dtype == CT_F64, "ct_norm_residual_gradient: datatype must be float or double");
+  CT_REQUIRE(known_norm(post_kind) && known_norm(pre_kind), "ct_norm_residual_gradient: unknown kind of norm");
+  CT_REQUIRE(input_dims && (input_dims->ndim == 1 || input_dims->ndim == 2), "input: one or two dimensions are taken");
+  const int64_t rows = input_dims->ndim == 2 ? input_dims->shape[0] : 1, width = input_dims->shape[input_dims->ndim - 1];
+  CT_REQUIRE(rows >= 0 && width >= 0 && width <= kMostWidth, "ct_norm_residual_gradient: bad extent");
+  if (width == 0) return CT_OK;
+  const bool before = pre_kind != CT_NORM_NONE && normalized_gradient;
+  CT_REQUIRE(rows == 0 || (input && (output || !before) && (statistics || (post_kind == CT_NORM_NONE && !before))),
+             "ct_norm_residual_gradient: null buffer");
+  CT_REQUIRE(!gate_gradient || gate, "ct_norm_residual_gradient: a gradient of no gate");
+  CT_REQUIRE(post_kind != CT_NORM_NONE || (!post_scale_gradient && !post_bias_gradient), "ct_norm_residual_gradient: gradients of no post norm");
+  CT_REQUIRE(pre_kind != CT_NORM_NONE || (!pre_scale_gradient && !pre_bias_gradient), "ct_norm_residual_gradient: gradients of no pre norm");
+  NormGradientArgs a{};
+  CT_TRY(read_matrix("input", input, input_dims, rows, width, &a.input));
+  CT_TRY(read_matrix("output", before ? output : nullptr, output_dims, rows, width, &a.output));
+  CT_TRY(read_matrix("output gradient", output_gradient, output_gradient_dims, rows, width, &a.output_gradient));
+  CT_TRY(read_matrix("normalized gradient", before ? normalized_gradient : nullptr, normalized_gradient_dims, rows, width, &a.normalized_gradient));
+  CT_TRY(read_matrix("input gradient", input_gradient, input_gradient_dims, rows, width, &a.input_gradient));
+  CT_TRY(read_matrix("residual gradient", residual_gradient, residual_gradient_dims, rows, width, &a.residual_gradient));
+  CT_TRY(read_gate("gate", gate, gate_dims, rows, width, &a.gate, &a.gate_kind));
+  // rows of a gate's gradient are packed as the gate's dimensions are
+  a.gate_gradient = Matrix{gate_gradient, a.gate_kind == kFullGate ? width : 1};
+  const int64_t size = dtype_size(dtype);
+  const RowRange of_gate = gate_range(a.gate, a.gate_kind, rows, width), of_gate_gradient = gate_range(a.gate_gradient, a.gate_kind, rows, width);
+  const Matrix* results[2] = {&a.input_gradient, &a.residual_gradient};
+  for (const Matrix* to : results) {
+    const RowRange range = range_of(*to, rows, width);
+    bool bad = meets_other(*to, a.output_gradient, rows, width, size) || meets_other(*to, a.normalized_gradient, rows, width, size) ||
+               rows_meet(range, range_of(a.input, rows, width), size) || rows_meet(range, range_of(a.output, rows, width), size) ||
+               rows_meet(range, of_gate, size) || rows_meet(range, of_gate_gradient, size) || rows_meet(range, {statistics, 1, 4 * rows, 4 * rows}, size);
+    for (const void* p : {post_scale, post_bias, pre_scale, (const void*)post_scale_gradient, (const void*)post_bias_gradient,
+                          (const void*)pre_scale_gradient, (const void*)pre_bias_gradient})
+      bad = bad || rows_meet(range, {p, 1, width, width}, size);
+    CT_REQUIRE(!bad, "ct_norm_residual_gradient: a result overlaps an operand");
+  }
+  for (const Matrix* m : {&a.input, &a.output, &a.output_gradient, &a.normalized_gradient})
+    CT_REQUIRE(!rows_meet(of_gate_gradient, range_of(*m, rows, width), size), "ct_norm_residual_gradient: the gate's gradient overlaps an operand");
+  CT_REQUIRE(!rows_meet(of_gate_gradient, of_gate, size), "ct_norm_residual_gradient: the gate's gradient overlaps the gate");
+  CT_REQUIRE(!rows_meet(range_of(a.input_gradient, rows, width), range_of(a.residual_gradient, rows, width), size),
+             "ct_norm_residual_gradient: the results overlap");
+  const bool of_columns = gate_gradient && (a.gate_kind == kColumnGate || a.gate_kind == kScalarGate);
+  a.post_scale = post_scale; a.post_bias = post_bias; a.pre_scale = pre_scale;
+  a.statistics = statistics;
+  a.rows = rows; a.width = (uint32_t)width;
+  a.post = post_kind; a.pre = pre_kind;
+  a.residual_scale = residual_scale;
+  const bool has_bias = post_kind != CT_NORM_NONE && post_bias;
+  const bool wanted[4] = {post_scale_gradient || of_columns, post_bias_gradient || (of_columns && has_bias), pre_scale_gradient != nullptr,
+                          pre_bias_gradient != nullptr};
+  NormFinishArgs f{};
+  for (int i = 0, slot = 0; i < 4; ++i) a.slot[i] = f.slot[i] = wanted[i] ? slot++ : -1;
+  f.post_scale = post_kind != CT_NORM_NONE ? post_scale : nullptr;
+  f.post_bias = has_bias ? post_bias : nullptr;
+  f.gate = gate; f.gate_kind = a.gate_kind;
+  f.gate_gradient = of_columns ? gate_gradient : nullptr;
+  f.post_scale_gradient = post_scale_gradient; f.post_bias_gradient = post_bias_gradient;
+  f.pre_scale_gradient = pre_scale_gradient; f.pre_bias_gradient = pre_bias_gradient;
+  f.by_column = of_columns && a.gate_kind == kScalarGate ? gate_gradient : nullptr;   // replaced by scratch
+  f.width = (uint32_t)width;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == CT_F32 ? norm_gradient_typed<float>(s, a, f) : norm_gradient_typed<double>(s, a, f);
+}
+
+}  // extern "C"

@@ -24,6 +24,7 @@ indirectly addressed dimension.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 from typing import Optional, Sequence
@@ -180,6 +181,14 @@ def _dims_ref(dims: dict):
 
 if capi.front is not None:
     _dims_ref = capi.front.stand_in(_dims_ref)   # for plain ints the struct's bytes (0.2 us; looking it up 0.4)
+
+
+def _ptr(buffer):
+    return None if buffer is None else buffer.ptr
+
+
+def _dims_or_none(dims):
+    return None if dims is None else _dims_ref(dims)
 
 
 def _arg_order_indexes(arg_order: Sequence[str]):
@@ -494,6 +503,75 @@ class HipStream:
         capi.call("ct_dropout_bernoulli_mask", self.handle, mult_buffer.ptr, capi.DTYPE_CODES[mult_buffer.datatype],
                   None if rand_buffer is None else rand_buffer.ptr, int(mult_buffer.ecount()), float(probability),
                   seed, offset)
+
+    # -- residual blocks with experts; no counterpart in the reference -----------
+    def norm_residual(self, output, output_dims, normalized, normalized_dims, statistics, input, input_dims, residual,
+                      residual_dims, gate, gate_dims, post_scale, post_bias, pre_scale, pre_bias, post_kind, pre_kind,
+                      residual_scale, epsilon) -> None:
+        capi.call("ct_norm_residual", self.handle, output.ptr, _dims_ref(output_dims), _ptr(normalized), _dims_or_none(normalized_dims),
+                  _ptr(statistics), input.ptr, _dims_ref(input_dims), _ptr(residual), _dims_or_none(residual_dims), _ptr(gate),
+                  _dims_or_none(gate_dims), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale), _ptr(pre_bias),
+                  capi.NORM_KINDS[post_kind], capi.NORM_KINDS[pre_kind], float(residual_scale), float(epsilon),
+                  capi.DTYPE_CODES[output.datatype])
+
+    def norm_residual_gradient(self, input_gradient, input_gradient_dims, residual_gradient, residual_gradient_dims, gate_gradient,
+                               post_scale_gradient, post_bias_gradient, pre_scale_gradient, pre_bias_gradient, output_gradient,
+                               output_gradient_dims, normalized_gradient, normalized_gradient_dims, input, input_dims, output,
+                               output_dims, statistics, gate, gate_dims, post_scale, post_bias, pre_scale, post_kind, pre_kind,
+                               residual_scale) -> None:
+        capi.call("ct_norm_residual_gradient", self.handle, _ptr(input_gradient), _dims_or_none(input_gradient_dims),
+                  _ptr(residual_gradient), _dims_or_none(residual_gradient_dims), _ptr(gate_gradient), _ptr(post_scale_gradient),
+                  _ptr(post_bias_gradient), _ptr(pre_scale_gradient), _ptr(pre_bias_gradient), _ptr(output_gradient),
+                  _dims_or_none(output_gradient_dims), _ptr(normalized_gradient), _dims_or_none(normalized_gradient_dims), input.ptr,
+                  _dims_ref(input_dims), _ptr(output), _dims_or_none(output_dims), _ptr(statistics), _ptr(gate),
+                  _dims_or_none(gate_dims), _ptr(post_scale), _ptr(post_bias), _ptr(pre_scale), capi.NORM_KINDS[post_kind],
+                  capi.NORM_KINDS[pre_kind], float(residual_scale), capi.DTYPE_CODES[input.datatype])
+
+    def route_experts(self, experts, weights, offsets, tokens, slots, logits, logits_colstride, n, n_experts, n_chosen,
+                      renormalize) -> None:
+        capi.call("ct_route_experts", self.handle, experts.ptr, weights.ptr, offsets.ptr, tokens.ptr, slots.ptr, logits.ptr,
+                  int(logits_colstride), int(n), int(n_experts), int(n_chosen), int(bool(renormalize)),
+                  capi.DTYPE_CODES[logits.datatype])
+
+    def route_experts_gradient(self, logits_gradient, logits_gradient_colstride, weights_gradient, weights, experts, logits,
+                               logits_colstride, n, n_experts, n_chosen, renormalize) -> None:
+        capi.call("ct_route_experts_gradient", self.handle, logits_gradient.ptr, int(logits_gradient_colstride),
+                  weights_gradient.ptr, weights.ptr, experts.ptr, _ptr(logits), int(logits_colstride), int(n), int(n_experts),
+                  int(n_chosen), int(bool(renormalize)), capi.DTYPE_CODES[logits_gradient.datatype])
+
+    def grouped_gemm(self, c, c_colstride, trans_b, alpha, a, a_row_count, a_col_count, a_colstride, index, b, b_col_count,
+                     b_colstride, b_stride, offsets, n_groups, row_count, beta) -> None:
+        capi.call("ct_grouped_gemm", self.handle, c.ptr, int(c_colstride), int(bool(trans_b)), float(alpha), a.ptr, int(a_row_count),
+                  int(a_col_count), int(a_colstride), _ptr(index), b.ptr, int(b_col_count), int(b_colstride), int(b_stride),
+                  offsets.ptr, int(n_groups), int(row_count), float(beta), capi.DTYPE_CODES[c.datatype])
+
+    def grouped_gemm_weights(self, c, c_colstride, c_stride, alpha, a, a_row_count, a_col_count, a_colstride, a_index, b,
+                             b_row_count, b_col_count, b_colstride, b_index, offsets, n_groups, row_count, beta) -> None:
+        capi.call("ct_grouped_gemm_weights", self.handle, c.ptr, int(c_colstride), int(c_stride), float(alpha), a.ptr,
+                  int(a_row_count), int(a_col_count), int(a_colstride), _ptr(a_index), b.ptr, int(b_row_count), int(b_col_count),
+                  int(b_colstride), _ptr(b_index), offsets.ptr, int(n_groups), int(row_count), float(beta),
+                  capi.DTYPE_CODES[c.datatype])
+
+    def combine_experts(self, output, output_colstride, rows, row_count, rows_colstride, weights, slots, n, n_chosen, width) -> None:
+        capi.call("ct_combine_experts", self.handle, output.ptr, int(output_colstride), rows.ptr, int(row_count), int(rows_colstride),
+                  _ptr(weights), slots.ptr, int(n), int(n_chosen), int(width), capi.DTYPE_CODES[output.datatype])
+
+    def combine_experts_gradient(self, rows_gradient, rows_gradient_colstride, weights_gradient, output_gradient,
+                                 output_gradient_colstride, rows, row_count, rows_colstride, weights, slots, n, n_chosen,
+                                 width) -> None:
+        capi.call("ct_combine_experts_gradient", self.handle, _ptr(rows_gradient), int(rows_gradient_colstride),
+                  _ptr(weights_gradient), output_gradient.ptr, int(output_gradient_colstride), _ptr(rows), int(row_count),
+                  int(rows_colstride), _ptr(weights), slots.ptr, int(n), int(n_chosen), int(width),
+                  capi.DTYPE_CODES[output_gradient.datatype])
+
+    def clip_gradients(self, gradients, outputs, max_norm, norm_and_factor) -> None:
+        """``gradients`` and ``outputs`` (or None) are lists of buffers."""
+        addresses = array.array("Q", [b.ptr for b in gradients])
+        into = None if outputs is None else array.array("Q", [b.ptr for b in outputs])
+        counts = array.array("q", [b._ecount for b in gradients])
+        capi.call("ct_clip_gradients", self.handle, addresses.buffer_info()[0], None if into is None else into.buffer_info()[0],
+                  counts.buffer_info()[0], len(addresses), float(max_norm), norm_and_factor.ptr,
+                  capi.DTYPE_CODES[norm_and_factor.datatype])
 
     # -- optimizers ---------------------------------------------------------
     def adam_step(self, alpha, beta1, beta2, epsilon, pow_beta1_t, pow_beta2_t, gradient_alpha, gradient, parameters,

@@ -48,6 +48,18 @@ def _buffer(x):
     return x.buffer if hasattr(x, "buffer") else x
 
 
+def _dense_buffer(x):
+    """The buffer of a tensor whose elements are all of it, or a buffer."""
+    if not hasattr(x, "buffer"):
+        return x
+    from . import tensor as ct
+
+    n = x.ecount()
+    if n != 1 and not ct.dense(x):
+        raise ValueError("clip_gradients: tensors must be dense")
+    return x.buffer if x.buffer.ecount() == n else x.buffer.sub_buffer(0, n)
+
+
 def _ensure_datatype(datatype, *buffers) -> None:
     actual = [b.get_datatype() for b in buffers]
     if any(a != datatype for a in actual):
@@ -129,6 +141,34 @@ class SGD:
             ct.binary_op(momentum_vals, 1.0, dxm, float(self.optimizer["learning-rate"]) * float(gradient_alpha), grad, "+")
             dx = ct.binary_op(temp, 1.0, dxm, 1 + momentum, momentum_vals, "-")
             ct.binary_op(params, 1.0, params, 1.0, dx, "+")
+
+
+def clip_gradients(backend: Backend, gradients, max_norm, norm_and_factor, outputs=None, in_place: bool = True) -> None:
+    """The norm over all ``gradients`` (buffers or dense tensors of the backend's datatype) and their clipping, ahead of
+    ``compute_parameters``: with norm = sqrt(sum of all squares),
+
+        factor = max_norm / max(norm, max_norm),   outputs = gradients * factor
+
+    into ``outputs`` or, without them, into the gradients themselves; with ``in_place`` false and no outputs only the norm
+    is formed.  ``norm_and_factor`` holds two values on the device, so that nothing waits for the host.  The reference's
+    gradients are sums over a batch that an optimizer multiplies by its gradient-alpha: a limit for their mean is the
+    batch's size times as much.  No counterpart in the reference."""
+    gradients = [_dense_buffer(g) for g in gradients]
+    if outputs is not None:
+        outputs = [_dense_buffer(o) for o in outputs]
+        if [o.ecount() for o in outputs] != [g.ecount() for g in gradients]:
+            raise ValueError("clip_gradients: outputs and gradients differ in their lengths")
+        if any(a.partially_alias(b) for a, b in zip(outputs, gradients)):
+            raise ValueError("clip_gradients: an output overlaps its gradient")
+    elif in_place:
+        outputs = gradients
+    result = _dense_buffer(norm_and_factor)
+    if result.ecount() != 2:
+        raise ValueError("clip_gradients: the norm and the factor are two values")
+    if not float(max_norm) > 0:
+        raise ValueError(f"clip_gradients: max_norm must be positive, got {max_norm}")
+    _ensure_datatype(backend.datatype, result, *gradients, *(outputs or ()))
+    backend.stream.clip_gradients(gradients, outputs, max_norm, result)
 
 
 def create_optimizer(backend: Backend, optimizer: dict):

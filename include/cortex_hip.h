@@ -547,6 +547,125 @@ int ct_lrn_backward(void* stream, void* input_gradient, const ct_dims* input_gra
                     const ct_dims* output_gradient_dims, int n, double k, double alpha, double beta,
                     int dtype);
 
+/* ------------------------------------------------- residual blocks with experts
+ * The operators that a feed-forward residual block of experts needs beside the calls above: the norms around the block
+ * with its gate and residual, the choice of experts and the order of rows that follows from it, products grouped by
+ * expert, the sum of a token's rows, and the norm of all gradients.  No counterpart in the reference.
+ *
+ * Matrices are row-major; a column stride is the distance in elements between two stored rows, at least the row's
+ * length.  dtype is CT_F32 or CT_F64; indexes are int32 in device memory.  An index outside its range is not followed:
+ * it is treated as the entry says (a row of zeros, a result that is not stored), so none reads or writes beyond a
+ * buffer.  Results are the same bits from call to call: no sum's order depends on timing. */
+
+/* The kind of a norm: NONE leaves a row as it is; RMS multiplies by 1 / sqrt(mean(x^2) + epsilon); LAYER takes the mean
+ * off first.  The population's mean in both. */
+typedef enum ct_norm_kind_t { CT_NORM_NONE = 0, CT_NORM_RMS = 1, CT_NORM_LAYER = 2 } ct_norm_kind_t;
+
+/* What leaves a block and enters the next, in one pass.  With N the norm of a row,
+ *   u          = N_post(input) * post_scale + post_bias     (input itself for CT_NORM_NONE)
+ *   output     = residual_scale * residual + gate * u
+ *   normalized = N_pre(output) * pre_scale + pre_bias       (not formed for CT_NORM_NONE)
+ * output, normalized, input and residual are [rows, width] with the column strides of the dimensions given; the
+ * innermost stride is 1.  gate is [rows, width], [1, width], [rows, 1] or [1, 1]; absent (NULL) it is 1.  A scale that
+ * is absent is 1, a bias 0, and so may residual be (then residual_scale is not read).  output may be residual or input
+ * itself and normalized may be input: each row is read before it is stored; other overlaps are refused.
+ * statistics [4, rows], or NULL: the mean and 1 / sqrt(...) of the post norm, then those of the pre norm, as the
+ * gradient needs them (0 and 1 where there is no norm).  Statistics are summed in the tensor's type, in double beyond
+ * the rows that fit registers (16384 values, half as many in double). */
+int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, void* normalized,
+                     const ct_dims* normalized_dims, void* statistics, const void* input,
+                     const ct_dims* input_dims, const void* residual, const ct_dims* residual_dims,
+                     const void* gate, const ct_dims* gate_dims, const void* post_scale,
+                     const void* post_bias, const void* pre_scale, const void* pre_bias, int post_kind,
+                     int pre_kind, double residual_scale, double epsilon, int dtype);
+
+/* Its gradient, from those of output and normalized (either may be NULL: zero).  input, output and statistics are those of
+ * the forward call.  Any result may be NULL: input_gradient, residual_gradient [rows, width], gate_gradient (the gate's
+ * shape; sums over what the gate was broadcast along), the gradients of the scales and biases [width].  All are
+ * overwritten.  input_gradient and residual_gradient may be output_gradient or normalized_gradient itself, but not one
+ * another, and no gradient may overlap an operand otherwise.  Column sums run over the rows in double once they leave a
+ * block's registers; the partial sums live in the stream's scratch memory (at most
+ * 32 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
+int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims,
+                              void* residual_gradient, const ct_dims* residual_gradient_dims,
+                              void* gate_gradient, void* post_scale_gradient, void* post_bias_gradient,
+                              void* pre_scale_gradient, void* pre_bias_gradient,
+                              const void* output_gradient, const ct_dims* output_gradient_dims,
+                              const void* normalized_gradient, const ct_dims* normalized_gradient_dims,
+                              const void* input, const ct_dims* input_dims, const void* output,
+                              const ct_dims* output_dims, const void* statistics, const void* gate,
+                              const ct_dims* gate_dims, const void* post_scale, const void* post_bias,
+                              const void* pre_scale, int post_kind, int pre_kind, double residual_scale,
+                              int dtype);
+
+/* The n_chosen experts of every token, their weights, and the order of rows by expert.  logits [n, n_experts]:
+ *   experts [n, n_chosen]  the largest logits, largest first, the lowest index first among equal ones (NaN counts as
+ *                          the largest); a logit of -infinity is never chosen: -1 where too few are left
+ *   weights [n, n_chosen]  softmax of the logits at those places: over the chosen ones if renormalize, else over all;
+ *                          0 where the expert is -1
+ *   offsets [n_experts + 1], tokens [n * n_chosen], slots [n, n_chosen]  the assignments (t, j) in order of their
+ *                          expert, and of (t, j) within one: expert e's are offsets[e] .. offsets[e + 1] - 1; tokens
+ *                          holds t at each of these places and -1 beyond offsets[n_experts]; slots holds the place of
+ *                          (t, j), -1 for an expert of -1
+ * 1 <= n_chosen <= min(32, n_experts), n_experts <= 1024, n * n_chosen < 2^31.  n = 0 writes the offsets only. */
+int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* offsets, int32_t* tokens,
+                     int32_t* slots, const void* logits, int64_t logits_colstride, int64_t n,
+                     int64_t n_experts, int64_t n_chosen, int renormalize, int dtype);
+
+/* The gradient of the weights with respect to the logits, overwritten: with p the softmax over the chosen experts if
+ * renormalize, else over all,  dlogit_e = p_e * (dw_e - sum over the chosen i of w_i dw_i), dw_e = 0 where e was not
+ * chosen (so 0 there under renormalize).  weights and experts as ct_route_experts stored them. */
+int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logits_gradient_colstride,
+                              const void* weights_gradient, const void* weights, const int32_t* experts,
+                              const void* logits, int64_t logits_colstride, int64_t n, int64_t n_experts,
+                              int64_t n_chosen, int renormalize, int dtype);
+
+/* Products of rows with the matrix of their group: for every group e and every row i in offsets[e] .. offsets[e + 1] - 1
+ *   c[i] = alpha * a[index[i]] * op(b_e) + beta * c[i]
+ * with op(b_e) [a_col_count, b_col_count], b_e = b + e * b_stride stored so, or transposed if trans_b.  index (NULL: i
+ * itself) selects rows of a [a_row_count, a_col_count]; one outside [0, a_row_count) is a row of zeros.  offsets
+ * [n_groups + 1] do not decrease and lie in [0, row_count]; rows of no group are not touched.  Groups of no rows cost
+ * nothing.  Float products are formed as ct_gemm's are; c overlaps no operand. */
+int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, double alpha, const void* a,
+                    int64_t a_row_count, int64_t a_col_count, int64_t a_colstride, const int32_t* index,
+                    const void* b, int64_t b_col_count, int64_t b_colstride, int64_t b_stride,
+                    const int32_t* offsets, int64_t n_groups, int64_t row_count, double beta, int dtype);
+
+/* Products over the rows of each group, as the gradients of those matrices are: for every group e
+ *   c_e = alpha * sum over i in offsets[e] .. offsets[e + 1] - 1 of a[a_index[i]]^T b[b_index[i]] + beta * c_e
+ * c_e = c + e * c_stride [a_col_count, b_col_count]; beta * c_e (zeros if beta is 0) for a group of no rows. */
+int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t c_stride, double alpha,
+                            const void* a, int64_t a_row_count, int64_t a_col_count, int64_t a_colstride,
+                            const int32_t* a_index, const void* b, int64_t b_row_count, int64_t b_col_count,
+                            int64_t b_colstride, const int32_t* b_index, const int32_t* offsets,
+                            int64_t n_groups, int64_t row_count, double beta, int dtype);
+
+/* output[t] = sum over j of weights[t, j] * rows[slots[t, j]], slots outside [0, row_count) left out; weights NULL: 1.
+ * rows [row_count, width], output [n, width], weights and slots [n, n_chosen] packed, n_chosen <= 32.  Sums run in the order of j,
+ * in the tensor's type. */
+int ct_combine_experts(void* stream, void* output, int64_t output_colstride, const void* rows,
+                       int64_t row_count, int64_t rows_colstride, const void* weights,
+                       const int32_t* slots, int64_t n, int64_t n_chosen, int64_t width, int dtype);
+
+/* Its gradient: rows_gradient[slots[t, j]] = weights[t, j] * output_gradient[t], rows that no slot names are not touched;
+ * weights_gradient[t, j] = output_gradient[t] . rows[slots[t, j]], 0 for a slot outside the range.  Either may be NULL
+ * (then so may rows, for weights_gradient's).  A row is named by one slot at most. */
+int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_gradient_colstride,
+                                void* weights_gradient, const void* output_gradient,
+                                int64_t output_gradient_colstride, const void* rows, int64_t row_count,
+                                int64_t rows_colstride, const void* weights, const int32_t* slots, int64_t n,
+                                int64_t n_chosen, int64_t width, int dtype);
+
+/* The norm over all of `count` gradients and their clipping: with norm = sqrt(sum of all squares), summed in double,
+ *   factor = max_norm / max(norm, max_norm),   outputs[i] = gradients[i] * factor.
+ * gradients, outputs and counts are HOST arrays (of device addresses and lengths), read before the call returns; an output may be
+ * its gradient (and overlaps nothing otherwise), and outputs may be NULL: then only the norm is formed.  norm_and_factor [2], in the tensors' type, in
+ * device memory, receives both.  max_norm > 0; infinity never clips.  A NaN among the gradients makes norm, factor and
+ * every output NaN; an infinity makes the factor 0. */
+int ct_clip_gradients(void* stream, const void* const* gradients, void* const* outputs,
+                      const int64_t* counts, int64_t count, double max_norm, void* norm_and_factor,
+                      int dtype);
+
 /* ------------------------------------------------- optimizers */
 
 /* Adam step (src/cortex/optimize/adam.clj:68-102, 116-134; resources/adam.cu).
