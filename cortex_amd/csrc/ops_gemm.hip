@@ -22,15 +22,11 @@
 
 #include "common.h"
 #include "gemm.h"
-#include "split_mfma.h"
+#include "split_tile.h"
 
 using namespace cthip;
 
 namespace {
-
-// Element `chunk` (of eight k) of row `row` of a tile in LDS, rows of 32 k: the chunks of a row are permuted so that eight
-// consecutive rows' reads of one chunk cover 128 bytes' worth of banks once.
-__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t chunk) { return row * 32 + ((chunk ^ (row >> 1)) & 3) * 8; }
 
 struct GemmArgs {
   const float* a;
@@ -68,39 +64,17 @@ __device__ __forceinline__ Place place_of(const GemmArgs& a, uint32_t unit) {
   return p;
 }
 
-// Eight consecutive k of one row of an operand: kRowMajor has them side by side, else a leading dimension apart.  `base` is
-// uniform and stays in scalar registers, `offset` is the lane's, in bytes.
-template <bool kRowMajor>
-__device__ __forceinline__ void load8(const float* base, uint32_t offset, int64_t ld, f32x4 (&to)[2]) {
-  uint64_t bits = reinterpret_cast<uint64_t>(base);
-  asm("" : "+s"(bits));   // or the loop keeps a 64-bit address per lane and load, for which there are no registers
-  typedef __attribute__((address_space(1))) const char* Global;
-  typedef f32x4 f32x4_at_4 __attribute__((aligned(4)));
-  const Global p = reinterpret_cast<Global>(bits);
-  if constexpr (kRowMajor) {
-    to[0] = *reinterpret_cast<__attribute__((address_space(1))) const f32x4_at_4*>(p + offset);
-    to[1] = *reinterpret_cast<__attribute__((address_space(1))) const f32x4_at_4*>(p + 16 + offset);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      to[e / 4][e % 4] = *reinterpret_cast<__attribute__((address_space(1))) const float*>(p + 4 * e * ld + offset);
-  }
-}
-
 // c = alpha * op(a) op(b) + beta * c over tiles of BM x BN, WM x WN waves to a group, KG groups to a block.  At least 32 k.
 // kA: a is stored [m][k], else [k][m]; kB: b is stored [n][k], else [k][n].
-// The floats are split once, on the way into LDS.  Groups take a run of k each and are added at the end: of results with
+// The tile is formed by split_tile (split_tile.h).  Groups take a run of k each and are added at the end: of results with
 // fewer tiles than compute units, whose blocks have a unit to themselves and wait for memory, a pair is formed in 0.87 us
 // for what takes one group 0.64 twice ([1024, 1024] over 1024 20.2 and 25.6 us); three groups gained nothing more.
 // Tried and not taken: tiles of 256 x 128 (no registers left beside their sums; 871 us where these take 741), prefetching
 // two tiles ahead (224 and 219 us), the order of instructions within a step left to the compiler (768 and 737).
 template <int BM, int BN, int WM, int WN, int KG, bool kA, bool kB>
 __global__ void __launch_bounds__(64 * WM * WN * KG, 2) gemm_kernel(const GemmArgs a) {
-  constexpr int BK = 32, T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, kChunks = BK / 8;
-  constexpr int UA = BM * kChunks / T, UB = BN * kChunks / T, U = UA + UB;   // runs of eight k that a lane stages
-  static_assert(UA * T == BM * kChunks && UB * T == BN * kChunks, "lanes share the tiles evenly");
-  constexpr int kLeft = 2 * kSplitPieces * BM * BK, kRight = 2 * kSplitPieces * BN * BK;
-  __shared__ __attribute__((aligned(16))) uint16_t all_lds[KG][kLeft + kRight];
+  constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, kTileLds = split_tile_lds(BM, BN);
+  __shared__ __attribute__((aligned(16))) uint16_t all_lds[KG][kTileLds];
   const uint32_t unit = unit_of_block(blockIdx.x, a.units);
   if (unit >= a.units) return;
   const Place place = place_of(a, unit);
@@ -109,189 +83,16 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) gemm_kernel(const GemmAr
   uint16_t* lds = all_lds[group];
   const uint32_t tiles = a.tiles_per_group, first = (place.split * KG + group) * tiles;
 
-  // Rows beyond the result repeat the last one and are not stored.
-  auto row_of = [&](int i) { return (i < UA ? kA : kB) ? ((i < UA ? i : i - UA) * T + tid) / kChunks
-                                                       : ((i < UA ? i : i - UA) * T + tid) % (i < UA ? BM : BN); };
-  auto chunk_of = [&](int i) { return (i < UA ? kA : kB) ? ((i < UA ? i : i - UA) * T + tid) % kChunks
-                                                         : ((i < UA ? i : i - UA) * T + tid) / (i < UA ? BM : BN); };
-  const float* base_a = a.a + (int64_t)(place.m_tile * BM) * (kA ? a.lda : 1);
-  const float* base_b = a.b + (int64_t)(place.n_tile * BN) * (kB ? a.ldb : 1);
-  uint32_t offset[U];
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const uint32_t last = i < UA ? a.m - 1 - place.m_tile * BM : a.n - 1 - place.n_tile * BN, r = min(row_of(i), last);
-    const uint32_t ld = (uint32_t)(i < UA ? a.lda : a.ldb);
-    offset[i] = 4 * ((i < UA ? kA : kB) ? r * ld + chunk_of(i) * 8 : chunk_of(i) * 8 * ld + r);
-  }
-  // The last tile of k, if it is a partial one, is loaded from 32 k before the end on; what an earlier tile had is set to
-  // zero, in both operands, before it is used.  Tiles beyond it are all zeros.
-  auto load = [&](int i, uint32_t tile, f32x4 (&to)[2]) {
-    const int64_t k0 = min((first + tile) * BK, a.k - BK);
-    if (i < UA) load8<kA>(base_a + (kA ? k0 : k0 * a.lda), offset[i], a.lda, to);
-    else load8<kB>(base_b + (kB ? k0 : k0 * a.ldb), offset[i], a.ldb, to);
-  };
-  auto drop_repeated = [&](int i, uint32_t tile, f32x4 (&r)[2]) {
-    const uint32_t k0 = (first + tile) * BK;
-    if (k0 + BK <= a.k) return;
-    asm volatile("");   // stays a branch: as selects it would cost every tile
-    const uint32_t repeated = k0 - (a.k - BK);   // of the tile's k; all of them beyond the last tile
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e / 4][e % 4] = chunk_of(i) * 8 + e < repeated ? 0.f : r[e / 4][e % 4];
-  };
-
-  f32x16 sums[2][MT][NT];   // the products of the leading pieces; all others
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int u = 0; u < NT; ++u) sums[s][t][u] = zero16();
-  const uint32_t wave_m = wave / WN * (MT * 32), wave_n = wave % WN * (NT * 32), row = lane & 31, half = lane >> 5;
-
-  {
-    const SplitWeights weights;
-    f32x4 raw[U][2];
-    u32x4 pieces[kSplitPieces];
-    auto piece_of = [&](int i, int buffer, int p) {
-      return i < UA ? &lds[(buffer * kSplitPieces + p) * BM * BK] : &lds[kLeft + (buffer * kSplitPieces + p) * BN * BK];
-    };
-    // half h of run i: the pieces go to LDS with the second one
-    auto stage = [&](int i, int h, int buffer, uint32_t tile) {
-      if (h == 0) drop_repeated(i, tile, raw[i]);
-      split4(raw[i][h], pieces, 4 * h, weights);
-      if (h == 0) return;
-#pragma unroll
-      for (int p = 0; p < kSplitPieces; ++p)
-        *reinterpret_cast<u32x4*>(piece_of(i, buffer, p) + tile_at(row_of(i), chunk_of(i))) = pieces[p];
-    };
-    bf16x8 left[2][MT][kSplitPieces], right[2][NT][kSplitPieces];
-    // piece p of an operand, k 16 * part .. + 15 of the tile
-    auto fetch_left = [&](int buffer, int part, int p) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-        left[part][t][p] = *reinterpret_cast<const bf16x8*>(piece_of(0, buffer, p) + tile_at(wave_m + t * 32 + row, part * 2 + half));
-    };
-    auto fetch_right = [&](int buffer, int part, int p) {
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-        right[part][u][p] = *reinterpret_cast<const bf16x8*>(piece_of(UA, buffer, p) + tile_at(wave_n + u * 32 + row, part * 2 + half));
-    };
-    auto multiply = [&](int part, int i) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          f32x16& to = sums[i + 1 < kSplitProducts][t][u];
-          to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(left[part][t][kSplitLeft[i]], right[part][u][kSplitRight[i]], to, 0, 0, 0);
-        }
-    };
-    // After product i of a half: pieces of the next half, those that its first product needs early, the others as the
-    // present half's last use frees their registers.
-    auto fetch_next = [&](int i, int buffer, int part) {
-      if (i == 0) {
-        fetch_left(buffer, part, 0);
-        fetch_right(buffer, part, 0);
-        fetch_right(buffer, part, 2);
-      }
-      if (i == 1) fetch_left(buffer, part, 2);
-      if (i == 3) fetch_right(buffer, part, 1);
-      if (i == 4) fetch_left(buffer, part, 1);
-    };
-    // One tile of k.  Its first half's fragments are in registers when it begins.  The products of that half run beside
-    // the splitting of the next tile into the other buffer, those of the second beside the reads of the next tile's first
-    // fragments: one barrier a tile, and no product waits for a read that was just issued.
-    auto step = [&](uint32_t tile, int buffer) {
-#pragma unroll
-      for (int i = 0; i < kSplitProducts; ++i) {
-        multiply(0, i);
-        fetch_next(i, buffer, 1);
-#pragma unroll
-        for (int j = i * 2 * U / kSplitProducts; j < (i + 1) * 2 * U / kSplitProducts; ++j) {
-          stage(j / 2, j % 2, buffer ^ 1, tile + 1);
-          if (j % 2) load(j / 2, tile + 2, raw[j / 2]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __syncthreads();
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < kSplitProducts; ++i) {
-        multiply(1, i);
-        fetch_next(i, buffer ^ 1, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < U; ++i) load(i, 0, raw[i]);
-#pragma unroll
-    for (int j = 0; j < 2 * U; ++j) stage(j / 2, j % 2, 0, 0);
-#pragma unroll
-    for (int i = 0; i < U; ++i) load(i, 1, raw[i]);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSplitProducts; ++i) fetch_next(i, 0, 0);
-    for (uint32_t tile = 0; tile < tiles; tile += 2) {
-      step(tile, 0);
-      step(tile + 1, 1);
-    }
-  }
-
-  bool found = false;
+  MatrixSource<BM, BN, T, kA, kB> source(a.a + (int64_t)(place.m_tile * BM) * (kA ? a.lda : 1), a.lda,
+                                         a.b + (int64_t)(place.n_tile * BN) * (kB ? a.ldb : 1), a.ldb,
+                                         a.m - 1 - place.m_tile * BM, a.n - 1 - place.n_tile * BN, a.k, first, tid);
   float result[MT][NT][16];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float sum = sums[0][t][u][r] + sums[1][t][u][r];
-        found |= not_finite(sum);
-        result[t][u][r] = sum * kSplitUnscale;
-      }
-  if (__syncthreads_or(found)) {
-    // In float: chains of a tile's 32 products, added up.
-    constexpr int LD = BK + 4;
-    float* left = reinterpret_cast<float*>(lds);
-    float* right = left + BM * LD;
-    static_assert((BM + BN) * LD * 4 <= (kLeft + kRight) * 2, "the floats fit where their pieces were");
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) result[t][u][r] = 0.f;
-    for (uint32_t tile = 0; tile < tiles; ++tile) {
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        f32x4 raw[2];
-        load(i, tile, raw);
-        drop_repeated(i, tile, raw);
-        float* to = (i < UA ? left : right) + row_of(i) * LD + chunk_of(i) * 8;
-        *reinterpret_cast<f32x4*>(to) = raw[0];
-        *reinterpret_cast<f32x4*>(to + 4) = raw[1];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          f32x16 sum = zero16();
-          for (int k = 0; k < BK; k += 8) {
-            const f32x4 l = *reinterpret_cast<const f32x4*>(left + (wave_m + t * 32 + row) * LD + k + 4 * half);
-            const f32x4 r = *reinterpret_cast<const f32x4*>(right + (wave_n + u * 32 + row) * LD + k + 4 * half);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_32x32x2f32(l[e], r[e], sum, 0, 0, 0);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) result[t][u][r] += sum[r];
-        }
-      __syncthreads();
-    }
-  }
+  split_tile<BM, BN, WM, WN>(source, tiles, lds, tid, result);
+  const uint32_t wave_m = wave / WN * (MT * 32), wave_n = wave % WN * (NT * 32), row = lane & 31, half = lane >> 5;
 
   if constexpr (KG > 1) {   // the groups' sums, added in their order
     constexpr int kCells = MT * NT * 16;
-    static_assert(T * kCells * 4 <= (kLeft + kRight) * 2, "a group's sums fit its LDS");
+    static_assert(T * kCells * 4 <= kTileLds * 2, "a group's sums fit its LDS");
     __syncthreads();
     if (group > 0) {
       float* to = reinterpret_cast<float*>(lds) + tid;

@@ -8,6 +8,7 @@
 
 #include "common.h"
 #include "rows.h"
+#include "split_tile.h"
 
 using namespace cthip;
 
@@ -139,6 +140,477 @@ __global__ void __launch_bounds__(256) grouped_weights_kernel(const GroupedArgs 
       });
 }
 
+// ------------------------------------------------------------------ float: the matrix cores, three pieces to a float
+
+// Tiles in bands of kBand rows, column after column, dealt to the dies in runs of kRun: what a die works on at a time is as
+// square as it can be and mostly of one group, and each die has a part of every group.
+constexpr uint32_t kBand = 8, kRun = 16;
+
+struct GroupedPlan {
+  uint32_t m_tiles, n_tiles, units;   // m_tiles: as many as there can be
+  FastDiv band_fd;
+};
+
+__device__ __forceinline__ bool place_of(const GroupedPlan& p, uint32_t* m_tile, uint32_t* n_tile) {
+  const uint32_t at = blockIdx.x / kXcds, unit = (at / kRun * kXcds + blockIdx.x % kXcds) * kRun + at % kRun;
+  if (unit >= p.units) return false;
+  uint32_t band, rest;
+  p.band_fd.divmod(unit, band, rest);
+  const uint32_t rows = min(kBand, p.m_tiles - band * kBand);
+  *n_tile = rest / rows;
+  *m_tile = band * kBand + rest - *n_tile * rows;
+  return true;
+}
+
+// Rows of a by their indexes, 32 k and more; the matrix of the group.  Rows beyond the group's last one repeat it.
+template <int BM, int BN, int T, bool kB>
+struct GroupedSource : TileShare<BM, BN, T, true, kB> {
+  using Share = TileShare<BM, BN, T, true, kB>;
+  using Share::BK;
+  using Share::U;
+  using Share::UA;
+  using Share::UB;
+  const float* row_a[UA];
+  bool absent[UA], any_absent;   // an index outside a: zeros in the place of its row
+  const float* base_b;
+  int64_t ldb;
+  uint32_t k;
+  uint32_t offset[UB];
+  __device__ __forceinline__ GroupedSource(const GroupedArgs& a, const Group& g, uint32_t row0, uint32_t col0, uint32_t tid)
+      : Share{tid}, any_absent(false), ldb(a.ldb), k(a.k) {
+#pragma unroll
+    for (int i = 0; i < UA; ++i) {
+      const uint32_t row = g.first + min(row0 + this->row_of(i), g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
+      absent[i] = from >= a.a_rows;
+      any_absent |= absent[i];
+      row_a[i] = static_cast<const float*>(a.a) + (int64_t)(absent[i] ? 0 : from) * a.lda + this->chunk_of(i) * 8;
+    }
+    any_absent = __ballot(any_absent) != 0;
+    base_b = static_cast<const float*>(a.b) + (int64_t)g.index * a.b_stride + (int64_t)col0 * (kB ? a.ldb : 1);
+#pragma unroll
+    for (int i = 0; i < UB; ++i) {
+      const uint32_t r = min(this->row_of(UA + i), a.n - 1 - col0), chunk = this->chunk_of(UA + i);
+      offset[i] = 4 * (kB ? r * (uint32_t)a.ldb + chunk * 8 : chunk * 8 * (uint32_t)a.ldb + r);
+    }
+  }
+  __device__ __forceinline__ void rewind() {}
+  __device__ __forceinline__ void load(int i, uint32_t tile, f32x4 (&to)[2]) const {
+    const int64_t k0 = min(tile * BK, k - BK);
+    if (i < UA) {
+      __builtin_memcpy(&to[0], row_a[i] + k0, 16);
+      __builtin_memcpy(&to[1], row_a[i] + k0 + 4, 16);
+    } else {
+      load8<kB>(base_b + (kB ? k0 : k0 * ldb), offset[i - UA], ldb, to);
+    }
+  }
+  __device__ __forceinline__ void drop(int i, uint32_t tile, f32x4 (&r)[2]) const {
+    if (i < UA && any_absent) {
+      asm volatile("");   // stays a branch
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e / 4][e % 4] = absent[i] ? 0.f : r[e / 4][e % 4];
+    }
+    const uint32_t k0 = tile * BK;
+    if (k0 + BK <= k) return;
+    asm volatile("");
+    const uint32_t repeated = k0 - (k - BK);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e / 4][e % 4] = this->chunk_of(i) * 8 + e < repeated ? 0.f : r[e / 4][e % 4];
+  }
+};
+
+template <int MT, int NT>
+__device__ __forceinline__ void store_tile(const GroupedArgs& a, float* c, uint32_t rows, uint32_t columns, uint32_t wave_m, uint32_t wave_n,
+                                           uint32_t lane, const float (&result)[MT][NT][16]) {
+  const uint32_t column = lane & 31, half = lane >> 5;
+  const float alpha = (float)a.alpha, beta = (float)a.beta;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const uint32_t n = wave_n + u * 32 + column;
+    if (n >= columns) continue;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t m = wave_m + t * 32 + 8 * (r / 4) + 4 * half + r % 4;
+        if (m >= rows) continue;
+        float& cell = c[(int64_t)m * a.ldc + n];
+        const float value = alpha * result[t][u][r];
+        cell = beta == 0.f ? value : value + beta * cell;
+      }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, bool kB>
+__global__ void __launch_bounds__(64 * WM * WN, 2) grouped_split_kernel(const GroupedArgs a, const GroupedPlan p) {
+  constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[split_tile_lds(BM, BN)];
+  uint32_t m_tile, n_tile;
+  Group g;
+  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, BM, &g)) return;
+  const uint32_t row0 = g.tile * BM, col0 = n_tile * BN, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  GroupedSource<BM, BN, T, kB> source(a, g, row0, col0, tid);
+  float result[MT][NT][16];
+  split_tile<BM, BN, WM, WN>(source, (a.k + 2 * kTileDepth - 1) / (2 * kTileDepth) * 2, lds, tid, result);
+  store_tile(a, static_cast<float*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0, g.rows - row0, a.n - col0, wave / WN * (MT * 32),
+             wave % WN * (NT * 32), tid & 63, result);
+}
+
+// Columns of the rows of a group, over which the products' sums run.  A wave loads eight rows at a time: its lanes 0 to 7
+// hold where they begin, read a tile ahead where there are indexes, and each load takes one as a scalar.  Rows beyond the
+// group's last one, and those of indexes outside the operand, are zeros.
+// kWide: operands of 4 GiB and more, with 64 bits to a row's place.  (Indexes read into scalar registers, and 64-bit scalar
+// addresses, took three times as long: 1500 and 470 us of 16 groups of 1024 rows, 2048 by 1024; the scalar loads were waited
+// for with all of LDS, and the addresses spilled.)
+template <int BM, int BN, int T, bool kWide>
+struct GroupedWeightsSource : TileShare<BM, BN, T, false, false> {
+  using Share = TileShare<BM, BN, T, false, false>;
+  using Share::BK;
+  using Share::U;
+  using Share::UA;
+  using Place = std::conditional_t<kWide, uint64_t, uint32_t>;
+  const float *base_a, *base_b;
+  const int32_t *index_a, *index_b;
+  uint32_t lda, ldb, rows_a, rows_b, first, rows;
+  uint32_t offset[U], chunk[U], absent[U], next[U];
+  __device__ __forceinline__ GroupedWeightsSource(const GroupedArgs& a, uint32_t first, uint32_t rows, uint32_t row0, uint32_t col0, uint32_t tid)
+      : Share{tid}, base_a(static_cast<const float*>(a.a) + row0), base_b(static_cast<const float*>(a.b) + col0), index_a(a.index_a),
+        index_b(a.index_b), lda((uint32_t)a.lda), ldb((uint32_t)a.ldb), rows_a(a.a_rows), rows_b(a.b_rows), first(first), rows(rows) {
+    static_assert(BM % 64 == 0 && BN % 64 == 0, "a wave's lanes are columns of one run");
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      offset[i] = 4 * min(this->row_of(i), i < UA ? a.m - 1 - row0 : a.n - 1 - col0);
+      chunk[i] = __builtin_amdgcn_readfirstlane(this->chunk_of(i));
+      absent[i] = 0;
+    }
+    rewind();
+  }
+  __device__ __forceinline__ uint32_t row_at(uint32_t i, uint32_t tile) const { return tile * BK + chunk[i] * 8 + (this->tid & 7); }
+  __device__ __forceinline__ void look_up(int i, uint32_t tile) {
+    const uint32_t row = first + min(row_at(i, tile), rows - 1);
+    const int32_t* index = i < UA ? index_a : index_b;
+    next[i] = index ? (uint32_t)index[row] : row;
+  }
+  __device__ __forceinline__ void rewind() {
+#pragma unroll
+    for (int i = 0; i < U; ++i) look_up(i, 0);
+  }
+  __device__ __forceinline__ void load(int i, uint32_t tile, f32x4 (&to)[2]) {
+    const bool outside = next[i] >= (i < UA ? rows_a : rows_b);
+    absent[i] = (uint32_t)__ballot(outside || row_at(i, tile) >= rows) & 0xff;
+    const Place begin = (Place)(outside ? 0 : next[i]) * (4 * (Place)(i < UA ? lda : ldb));
+    uint64_t base = reinterpret_cast<uint64_t>(i < UA ? base_a : base_b);
+    asm("" : "+s"(base));
+    typedef __attribute__((address_space(1))) const char* Global;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      Place at = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)begin, e);
+      if constexpr (kWide) at |= (Place)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(begin >> 32), e) << 32;
+      to[e / 4][e % 4] = *reinterpret_cast<__attribute__((address_space(1))) const float*>(reinterpret_cast<Global>(base) + (Place)(at + offset[i]));
+    }
+    look_up(i, tile + 1);
+  }
+  __device__ __forceinline__ void drop(int i, uint32_t, f32x4 (&r)[2]) const {
+    if (absent[i] == 0) return;
+    asm volatile("");   // stays a branch
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e / 4][e % 4] = absent[i] >> e & 1 ? 0.f : r[e / 4][e % 4];
+  }
+};
+
+template <int BM, int BN, int WM, int WN, bool kWide>
+__global__ void __launch_bounds__(64 * WM * WN, 2) grouped_weights_split_kernel(const GroupedArgs a, const GroupedPlan p) {
+  constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[split_tile_lds(BM, BN)];
+  uint32_t m_tile, n_tile;
+  if (!place_of(p, &m_tile, &n_tile)) return;
+  const uint32_t tiles = (a.m + BM - 1) / BM, group = m_tile / tiles, row0 = (m_tile - group * tiles) * BM, col0 = n_tile * BN;
+  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint2 rows = group_rows(a, group);
+  const uint32_t first = __builtin_amdgcn_readfirstlane(rows.x), count = __builtin_amdgcn_readfirstlane(rows.y);
+  float result[MT][NT][16] = {};
+  if (count > 0 && a.a_rows > 0 && a.b_rows > 0) {
+    GroupedWeightsSource<BM, BN, T, kWide> source(a, first, count, row0, col0, tid);
+    split_tile<BM, BN, WM, WN>(source, (count + 2 * kTileDepth - 1) / (2 * kTileDepth) * 2, lds, tid, result);
+  }
+  store_tile(a, static_cast<float*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0, a.m - row0, a.n - col0,
+             wave / WN * (MT * 32), wave % WN * (NT * 32), tid & 63, result);
+}
+
+// ------------------------------------------------------------------ float, a few rows to a group
+
+// What a few tokens ask of their experts is bound by reading the matrices: a block owns 16 rows by 64 columns, its W waves take
+// every W-th run of 32 k each, straight from memory into the fragments, and their sums are added in LDS in their order.  The
+// rows are split once for 64 columns.  Of a matrix stored [k][n] a lane takes four columns side by side.
+template <int W, bool kB>
+__global__ void __launch_bounds__(64 * W, 2) grouped_thin_kernel(const GroupedArgs a, const GroupedPlan p) {
+  constexpr uint32_t BM = 16, BN = 64, BK = 32, NT = BN / 16;
+  __shared__ float partial[W][BM * BN];
+  uint32_t m_tile, n_tile;
+  Group g;
+  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, BM, &g)) return;
+  const uint32_t row0 = g.tile * BM, col0 = n_tile * BN, lane = threadIdx.x & 63, at16 = lane % 16, quarter = lane / 16;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k_end = a.k;
+  const uint32_t row = g.first + min(row0 + at16, g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
+  const bool absent = from >= a.a_rows;
+  const float* left = static_cast<const float*>(a.a) + (int64_t)(absent ? 0 : from) * a.lda;
+  const float* b = static_cast<const float*>(a.b) + (int64_t)g.index * a.b_stride;
+  // column u of a lane's four
+  auto column_of = [&](uint32_t lane16, uint32_t u) { return col0 + (kB ? u * 16 + lane16 : lane16 * 4 + u); };
+  const float* right[kB ? NT : 1];
+#pragma unroll
+  for (uint32_t u = 0; u < (kB ? NT : 1); ++u) right[u] = b + (int64_t)(kB ? min(column_of(at16, u), a.n - 1) : col0) * (kB ? a.ldb : 1);
+  const bool whole = kB || column_of(at16, NT - 1) < a.n;
+  // eight k of the row and of each column, from k0 + 8 * quarter on
+  auto load = [&](uint32_t k0, f32x4 (&l)[2], f32x4 (&r)[NT][2]) {
+    const uint32_t k = k0 + quarter * 8;
+    if (k0 + BK <= k_end) {
+      __builtin_memcpy(&l[0], left + k, 16);
+      __builtin_memcpy(&l[1], left + k + 4, 16);
+      if constexpr (kB) {
+#pragma unroll
+        for (uint32_t u = 0; u < NT; ++u) {
+          __builtin_memcpy(&r[u][0], right[u] + k, 16);
+          __builtin_memcpy(&r[u][1], right[u] + k + 4, 16);
+        }
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+          const float* at = right[0] + (int64_t)(k + e) * a.ldb;
+          f32x4 four;
+          if (whole) __builtin_memcpy(&four, at + at16 * 4, 16);
+          else {
+#pragma unroll
+            for (uint32_t u = 0; u < NT; ++u) four[u] = at[min(column_of(at16, u), a.n - 1) - col0];
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < NT; ++u) r[u][e / 4][e % 4] = four[u];
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) {
+        const bool in = k + e < k_end;
+        const int64_t at = min(k + e, k_end - 1);
+        const float x = left[at];
+        l[e / 4][e % 4] = in ? x : 0.f;
+#pragma unroll
+        for (uint32_t u = 0; u < NT; ++u) {
+          const float y = kB ? right[kB ? u : 0][at] : right[0][at * a.ldb + min(column_of(at16, u), a.n - 1) - col0];
+          r[u][e / 4][e % 4] = in ? y : 0.f;
+        }
+      }
+    }
+    if (absent) l[0] = l[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  f32x4 sums[2][NT] = {};   // the products of the leading pieces; all others
+  bool found = k_end == 1;   // a product by itself: the floats' is rounded once
+  {
+    const SplitWeights weights;
+    f32x4 l[2], r[NT][2], l_next[2], r_next[NT][2];
+    const uint32_t mine = wave * BK;
+    if (mine < k_end) load(mine, l, r);
+    for (uint32_t k0 = mine; k0 < k_end; k0 += W * BK) {
+      const uint32_t next = k0 + W * BK;
+      if (next < k_end) load(next, l_next, r_next);
+      u32x4 lp[kSplitPieces];
+      split4(l[0], lp, 0, weights);
+      split4(l[1], lp, 4, weights);
+#pragma unroll
+      for (uint32_t u = 0; u < NT; ++u) {
+        u32x4 rp[kSplitPieces];
+        split4(r[u][0], rp, 0, weights);
+        split4(r[u][1], rp, 4, weights);
+#pragma unroll
+        for (int i = 0; i < kSplitProducts; ++i) {
+          f32x4& to = sums[i + 1 < kSplitProducts][u];
+          to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lp[kSplitLeft[i]]), __builtin_bit_cast(bf16x8, rp[kSplitRight[i]]), to, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] = l_next[h];
+#pragma unroll
+        for (uint32_t u = 0; u < NT; ++u) r[u][h] = r_next[u][h];
+      }
+    }
+  }
+  auto put_partial = [&](uint32_t u, int e, float value) { partial[wave][(quarter * 4 + e) * BN + column_of(at16, u) - col0] = value; };
+#pragma unroll
+  for (uint32_t u = 0; u < NT; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float sum = sums[0][u][e] + sums[1][u][e];
+      found |= not_finite(sum);
+      put_partial(u, e, sum * kSplitUnscale);
+    }
+  if (__syncthreads_or(found)) {
+    f32x4 total[NT] = {};
+    for (uint32_t k0 = wave * BK; k0 < k_end; k0 += W * BK) {
+      f32x4 l[2], r[NT][2];
+      load(k0, l, r);
+#pragma unroll
+      for (uint32_t u = 0; u < NT; ++u) {
+        f32x4 sum = {};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e / 4][e % 4], r[u][e / 4][e % 4], sum, 0, 0, 0);
+        total[u] += sum;
+      }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) put_partial(u, e, total[u][e]);
+    __syncthreads();
+  }
+  float* c = static_cast<float*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
+  const uint32_t rows = g.rows - row0, columns = a.n - col0;
+  for (uint32_t i = threadIdx.x; i < BM * BN; i += 64 * W) {
+    float sum = partial[0][i];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += partial[w][i];
+    if (i / BN < rows && i % BN < columns) put(c + (int64_t)(i / BN) * a.ldc + i % BN, sum, a.alpha, a.beta);
+  }
+}
+
+// ------------------------------------------------------------------ double: the matrix cores
+
+// A tile of S x S by four waves, S / 2 a side each, in products of 16 x 16 x 4: a wave's operands are 16 rows (or columns) by
+// lane % 16 of k lane / 16, its results rows lane / 16 + 4 r.  kDepth k are staged at a time, the next ones loaded meanwhile.
+// `left(row, k, to)` gives four k of a row if kA, else four rows of a k, from (row, k) on; `right` likewise with columns.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+template <int S, bool kA, bool kB, class Left, class Right, class Store>
+__device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right right, Store store) {
+  constexpr int BK = S == 64 ? 16 : 32, LD = S + 2, kQuads = S * BK / 4 / 256, MT = S / 32;
+  static_assert(kQuads == 1, "four elements of each operand to a lane");
+  __shared__ double lds_a[2][BK][LD], lds_b[2][BK][LD];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wave_m = wave / 2 * (S / 2), wave_n = wave % 2 * (S / 2);
+  auto row_of = [&](bool by_row) { return by_row ? tid / (BK / 4) : tid % (S / 4) * 4; };
+  auto k_of = [&](bool by_row) { return by_row ? tid % (BK / 4) * 4 : tid / (S / 4); };
+  double a[4], b[4];
+  auto put_in = [&](double (&lds)[BK][LD], bool by_row, const double (&x)[4]) {
+    const uint32_t r = row_of(by_row), k = k_of(by_row);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lds[by_row ? k + e : k][by_row ? r : r + e] = x[e];
+  };
+  f64x4 sum[MT][MT] = {};
+  left(row_of(kA), k_of(kA), a);
+  right(row_of(kB), k_of(kB), b);
+  put_in(lds_a[0], kA, a);
+  put_in(lds_b[0], kB, b);
+  __syncthreads();
+  int buffer = 0;
+  for (uint32_t k0 = 0; k0 < depth; k0 += BK, buffer ^= 1) {
+    const bool more = k0 + BK < depth;
+    if (more) {
+      left(row_of(kA), k0 + BK + k_of(kA), a);
+      right(row_of(kB), k0 + BK + k_of(kB), b);
+    }
+#pragma unroll
+    for (int k = 0; k < BK; k += 4) {
+      double l[MT], r[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        l[t] = lds_a[buffer][k + lane / 16][wave_m + t * 16 + lane % 16];
+        r[t] = lds_b[buffer][k + lane / 16][wave_n + t * 16 + lane % 16];
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(l[t], r[u], sum[t][u], 0, 0, 0);
+    }
+    if (more) {
+      put_in(lds_a[buffer ^ 1], kA, a);
+      put_in(lds_b[buffer ^ 1], kB, b);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) store(wave_m + t * 16 + lane / 16 + 4 * r, wave_n + u * 16 + lane % 16, sum[t][u][r]);
+}
+
+// Four elements from p[at] on, zeros from `end` on and where the row is absent.
+__device__ __forceinline__ void load4(const double* p, uint32_t at, uint32_t end, bool present, double (&to)[4]) {
+  if (present && at + 4 <= end) {
+    __builtin_memcpy(&to[0], p + at, 16);
+    __builtin_memcpy(&to[2], p + at + 2, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = present && at + e < end ? p[at + e] : 0.0;
+  }
+}
+
+template <int S, bool kB>
+__global__ void __launch_bounds__(256) grouped_double_kernel(const GroupedArgs a, const GroupedPlan p) {
+  uint32_t m_tile, n_tile;
+  Group g;
+  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, S, &g)) return;
+  const uint32_t row0 = g.tile * S, col0 = n_tile * S;
+  const double* b = static_cast<const double*>(a.b) + (int64_t)g.index * a.b_stride;
+  double* c = static_cast<double*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
+  const uint32_t my_row = row0 + threadIdx.x / (S == 64 ? 4 : 8);   // of a, the same for all k
+  uint32_t from = a.a_rows;
+  if (my_row < g.rows) from = a.index_a ? (uint32_t)a.index_a[g.first + my_row] : g.first + my_row;
+  const bool present = from < a.a_rows;
+  const double* left = static_cast<const double*>(a.a) + (int64_t)(present ? from : 0) * a.lda;
+  double_tile<S, true, kB>(
+      a.k, [&](uint32_t, uint32_t k, double (&to)[4]) { load4(left, k, a.k, present, to); },
+      [&](uint32_t n, uint32_t k, double (&to)[4]) {
+        if constexpr (kB) load4(b + (int64_t)(col0 + n) * a.ldb, k, a.k, col0 + n < a.n, to);
+        else load4(b + (int64_t)k * a.ldb, col0 + n, a.n, k < a.k, to);
+      },
+      [&](uint32_t r, uint32_t n, double sum) {
+        if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
+      });
+}
+
+template <int S>
+__global__ void __launch_bounds__(256) grouped_weights_double_kernel(const GroupedArgs a, const GroupedPlan p) {
+  uint32_t m_tile, n_tile;
+  if (!place_of(p, &m_tile, &n_tile)) return;
+  const uint32_t tiles = (a.m + S - 1) / S, group = m_tile / tiles, row0 = (m_tile - group * tiles) * S, col0 = n_tile * S;
+  const uint2 rows = group_rows(a, group);
+  double* c = static_cast<double*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0;
+  auto element = [&](const void* m, const int32_t* index, uint32_t count, int64_t ld, uint32_t k, uint32_t column, uint32_t width, double (&to)[4]) {
+    uint32_t from = count;
+    if (k < rows.y) from = index ? (uint32_t)index[rows.x + k] : rows.x + k;
+    const bool present = from < count;
+    load4(static_cast<const double*>(m) + (int64_t)(present ? from : 0) * ld, column, width, present, to);
+  };
+  double_tile<S, false, false>(
+      rows.y, [&](uint32_t r, uint32_t k, double (&to)[4]) { element(a.a, a.index_a, a.a_rows, a.lda, k, row0 + r, a.m, to); },
+      [&](uint32_t n, uint32_t k, double (&to)[4]) { element(a.b, a.index_b, a.b_rows, a.ldb, k, col0 + n, a.n, to); },
+      [&](uint32_t r, uint32_t n, double sum) {
+        if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
+      });
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+GroupedPlan plan_of(int64_t m_tiles, int64_t n_tiles) {
+  GroupedPlan p;
+  p.m_tiles = (uint32_t)m_tiles;
+  p.n_tiles = (uint32_t)n_tiles;
+  p.units = (uint32_t)(m_tiles * n_tiles);
+  p.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
+  return p;
+}
+
+// Microseconds of `blocks` tiles of 64 or of 128 a side over k_tiles of 32 k: the lines of ct_gemm's kernels.
+double time_of_medium(int64_t blocks, int64_t k_tiles) {
+  constexpr int64_t kUnits = 256;
+  const int64_t full = blocks / (3 * kUnits), rest = blocks - full * 3 * kUnits, shared = full * 3 + ceil_div(rest, kUnits);
+  return 3.3 + 1.3 * (double)shared + (double)k_tiles * (0.31 * (double)(full + (rest > 0)) + 0.33 * (double)shared);
+}
+double time_of_large(int64_t blocks, int64_t k_tiles) { return 1.8 + (double)ceil_div(blocks, 256) * (3.7 + 1.19 * (double)k_tiles); }
+
+constexpr int64_t kThinRows = 16;   // of a group, in the mean, that the thin kernel takes
+constexpr int64_t kMostUnits = int64_t(1) << 22, kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
+
 uint32_t tiles_of(int64_t n, int64_t side) { return (uint32_t)((n + side - 1) / side); }
 
 constexpr int64_t kMostExtent = (int64_t(1) << 31) - 1;
@@ -178,6 +650,55 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
   g.groups = (uint32_t)n_groups; g.rows = (uint32_t)row_count; g.a_rows = (uint32_t)a_row_count;
   g.n = (uint32_t)b_col_count; g.k = (uint32_t)a_col_count;
   g.trans_b = trans_b != 0;
+  const int64_t even_groups = std::min(n_groups, row_count);
+  auto grid_of = [](const GroupedPlan& p) { return dim3((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun)); };
+  if (dtype == CT_F64 && a_row_count > 0) {
+    const int64_t tiles64 = (row_count / 64 + even_groups / 2) * ceil_div(b_col_count, 64), side = tiles64 >= 1024 ? 64 : 32;
+    const int64_t m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
+    if (m_tiles * n_tiles <= kMostUnits) {
+      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), grid_of(p), dim3(256), 0, s, g, p);
+      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), grid_of(p), dim3(256), 0, s, g, p);
+      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), grid_of(p), dim3(256), 0, s, g, p);
+      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), grid_of(p), dim3(256), 0, s, g, p);
+      note_kernel("grouped_double");
+      return after_launch(s);
+    }
+  }
+  if (dtype == CT_F32 && a_row_count > 0 && a_col_count > 0 && (a_col_count < kTileDepth || row_count <= kThinRows * even_groups)) {
+    const int64_t m_tiles = row_count / 16 + even_groups, n_tiles = ceil_div(b_col_count, 64);
+    if (m_tiles * n_tiles <= kMostUnits) {
+      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      const bool few = a_col_count <= 256;
+      if (few && trans_b) hipLaunchKernelGGL((grouped_thin_kernel<4, true>), grid_of(p), dim3(256), 0, s, g, p);
+      else if (few) hipLaunchKernelGGL((grouped_thin_kernel<4, false>), grid_of(p), dim3(256), 0, s, g, p);
+      else if (trans_b) hipLaunchKernelGGL((grouped_thin_kernel<8, true>), grid_of(p), dim3(512), 0, s, g, p);
+      else hipLaunchKernelGGL((grouped_thin_kernel<8, false>), grid_of(p), dim3(512), 0, s, g, p);
+      note_kernel("grouped_thin");
+      return after_launch(s);
+    }
+  }
+  if (dtype == CT_F32 && a_col_count >= kTileDepth && a_row_count > 0 && b_colstride <= kMostSplitLd) {
+    // the tiles that there are if the groups are even
+    const int64_t even = std::min(n_groups, row_count), k_tiles = ceil_div(a_col_count, kTileDepth), side = row_count / even;
+    const double medium = time_of_medium(even * ceil_div(side, 64) * ceil_div(b_col_count, 64), k_tiles);
+    const double large = time_of_large(even * ceil_div(side, 128) * ceil_div(b_col_count, 128), k_tiles);
+    const int64_t height = large < medium ? 128 : 64;
+    const int64_t m_tiles = row_count / height + even, n_tiles = ceil_div(b_col_count, height);
+    if (m_tiles * n_tiles <= kMostUnits) {
+      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
+      if (height == 128) {
+        if (trans_b) hipLaunchKernelGGL((grouped_split_kernel<128, 128, 2, 4, true>), grid, dim3(512), 0, s, g, p);
+        else hipLaunchKernelGGL((grouped_split_kernel<128, 128, 2, 4, false>), grid, dim3(512), 0, s, g, p);
+      } else {
+        if (trans_b) hipLaunchKernelGGL((grouped_split_kernel<64, 64, 2, 2, true>), grid, dim3(256), 0, s, g, p);
+        else hipLaunchKernelGGL((grouped_split_kernel<64, 64, 2, 2, false>), grid, dim3(256), 0, s, g, p);
+      }
+      note_kernel(height == 128 ? "grouped_large" : "grouped_medium");
+      return after_launch(s);
+    }
+  }
   const int64_t tiles = row_count / kSide + std::min(n_groups, row_count);
   CT_REQUIRE(tiles <= 65535, "ct_grouped_gemm: %lld rows", (long long)row_count);
   const dim3 grid(tiles_of(b_col_count, kSide), (uint32_t)tiles);
@@ -215,6 +736,35 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
   g.alpha = alpha; g.beta = beta;
   g.groups = (uint32_t)n_groups; g.rows = (uint32_t)row_count; g.a_rows = (uint32_t)a_row_count; g.b_rows = (uint32_t)b_row_count;
   g.m = (uint32_t)a_col_count; g.n = (uint32_t)b_col_count;
+  if (dtype == CT_F32 && std::max(a_colstride, b_colstride) <= kMostWeightsLd) {
+    const int64_t k_tiles = ceil_div(std::max<int64_t>(row_count / n_groups, 1), kTileDepth);
+    const double medium = time_of_medium(n_groups * ceil_div(a_col_count, 64) * ceil_div(b_col_count, 64), k_tiles);
+    const double large = time_of_large(n_groups * ceil_div(a_col_count, 128) * ceil_div(b_col_count, 128), k_tiles);
+    const int64_t side = large < medium ? 128 : 64, m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
+    if (m_tiles * n_tiles <= kMostUnits) {
+      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
+      const bool wide = std::max(a_row_count * a_colstride, b_row_count * b_colstride) * size >= int64_t(1) << 32;
+      if (side == 128 && !wide) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, false>), grid, dim3(512), 0, s, g, p);
+      else if (side == 128) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, true>), grid, dim3(512), 0, s, g, p);
+      else if (!wide) hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, false>), grid, dim3(256), 0, s, g, p);
+      else hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, true>), grid, dim3(256), 0, s, g, p);
+      note_kernel(side == 128 ? "grouped_weights_large" : "grouped_weights_medium");
+      return after_launch(s);
+    }
+  }
+  if (dtype == CT_F64) {
+    const int64_t side = n_groups * ceil_div(a_col_count, 64) * ceil_div(b_col_count, 64) >= 1024 ? 64 : 32;
+    const int64_t m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
+    if (m_tiles * n_tiles <= kMostUnits) {
+      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
+      if (side == 64) hipLaunchKernelGGL((grouped_weights_double_kernel<64>), grid, dim3(256), 0, s, g, p);
+      else hipLaunchKernelGGL((grouped_weights_double_kernel<32>), grid, dim3(256), 0, s, g, p);
+      note_kernel("grouped_weights_double");
+      return after_launch(s);
+    }
+  }
   CT_REQUIRE(tiles_of(a_col_count, kSide) <= 65535, "ct_grouped_gemm_weights: %lld columns of a", (long long)a_col_count);
   const dim3 grid(tiles_of(b_col_count, kSide), tiles_of(a_col_count, kSide), (uint32_t)n_groups);
   if (dtype == CT_F32) hipLaunchKernelGGL((grouped_weights_kernel<float>), grid, dim3(256), 0, s, g);
