@@ -475,55 +475,138 @@ __global__ void __launch_bounds__(64 * W, 2) grouped_thin_kernel(const GroupedAr
 // ------------------------------------------------------------------ double: the matrix cores
 
 // A tile of S x S by four waves, S / 2 a side each, in products of 16 x 16 x 4: a wave's operands are 16 rows (or columns) by
-// lane % 16 of k lane / 16, its results rows lane / 16 + 4 r.  kDepth k are staged at a time, the next ones loaded meanwhile.
-// `left(row, k, to)` gives four k of a row if kA, else four rows of a k, from (row, k) on; `right` likewise with columns.
+// lane % 16 of k lane / 16, its results rows lane / 16 + 4 r.  BK k are staged in LDS at a time, the next two lots on their way
+// into registers meanwhile.  An operand gives a lane four elements of a lot.  Its loads have no branches that lanes take apart:
+// behind one, every load would be waited for before the next is used (30 us in place of 21, 2026 rows of 7 groups, 301 by 517).
 typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef f64x2 f64x2_at_8 __attribute__((aligned(8)));
 
-template <int S, bool kA, bool kB, class Left, class Right, class Store>
-__device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right right, Store store) {
-  constexpr int BK = S == 64 ? 16 : 32, LD = S + 2, kQuads = S * BK / 4 / 256, MT = S / 32;
-  static_assert(kQuads == 1, "four elements of each operand to a lane");
-  __shared__ double lds_a[2][BK][LD], lds_b[2][BK][LD];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wave_m = wave / 2 * (S / 2), wave_n = wave % 2 * (S / 2);
-  auto row_of = [&](bool by_row) { return by_row ? tid / (BK / 4) : tid % (S / 4) * 4; };
-  auto k_of = [&](bool by_row) { return by_row ? tid % (BK / 4) * 4 : tid / (S / 4); };
-  double a[4], b[4];
-  auto put_in = [&](double (&lds)[BK][LD], bool by_row, const double (&x)[4]) {
-    const uint32_t r = row_of(by_row), k = k_of(by_row);
+constexpr int double_depth(int side) { return side == 64 ? 16 : 32; }
+
+// Four k of a row, which is the same for all k; `end` k, at least one.
+template <int S>
+struct DoubleRow {
+  static constexpr int BK = double_depth(S);
+  static constexpr bool kByRow = true;
+  const double* p;
+  uint32_t end;
+  bool present;
+  static __device__ __forceinline__ uint32_t row() { return threadIdx.x / (BK / 4); }
+  static __device__ __forceinline__ uint32_t k() { return threadIdx.x % (BK / 4) * 4; }
+  __device__ __forceinline__ void load(uint32_t k0, f64x2 (&x)[2]) const {
+    if (k0 + BK <= end) {
+      x[0] = *reinterpret_cast<const f64x2_at_8*>(p + k0 + k());
+      x[1] = *reinterpret_cast<const f64x2_at_8*>(p + k0 + k() + 2);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) lds[by_row ? k + e : k][by_row ? r : r + e] = x[e];
+      for (int e = 0; e < 4; ++e) x[e / 2][e % 2] = p[min(k0 + k() + e, end - 1)];
+    }
+  }
+  __device__ __forceinline__ void mend(uint32_t k0, f64x2 (&x)[2]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e / 2][e % 2] = present && k0 + k() + e < end ? x[e / 2][e % 2] : 0.0;
+  }
+};
+
+// Four columns, from `column` on of `width`, of the rows that k goes over: row `first` + k, or the one that an index names there.
+template <int S>
+struct DoubleColumns {
+  static constexpr int BK = double_depth(S);
+  static constexpr bool kByRow = false;
+  const double* p;
+  int64_t ld;
+  const int32_t* index;
+  uint32_t first, end, rows;   // k below end, at least one; rows of p
+  uint32_t left;               // columns from the tile's first on
+  uint32_t next, absent;
+  static __device__ __forceinline__ uint32_t column() { return threadIdx.x % (S / 4) * 4; }
+  static __device__ __forceinline__ uint32_t k() { return threadIdx.x / (S / 4); }
+  __device__ __forceinline__ DoubleColumns(const double* p, int64_t ld, const int32_t* index, uint32_t first, uint32_t end, uint32_t rows, uint32_t left)
+      : p(p), ld(ld), index(index), first(first), end(end), rows(rows), left(left), absent(0) {
+    look_up(0);
+  }
+  __device__ __forceinline__ void look_up(uint32_t k0) {
+    const uint32_t row = first + min(k0 + k(), end - 1);
+    next = index ? (uint32_t)index[row] : row;
+  }
+  __device__ __forceinline__ void load(uint32_t k0, f64x2 (&x)[2]) {
+    const bool outside = next >= rows;
+    absent = absent << 1 | outside;   // of this lot, and of the one before
+    const double* row = p + (int64_t)(outside ? 0 : next) * ld;
+    if (left >= S) {
+      x[0] = *reinterpret_cast<const f64x2_at_8*>(row + column());
+      x[1] = *reinterpret_cast<const f64x2_at_8*>(row + column() + 2);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e / 2][e % 2] = row[min(column() + e, left - 1)];
+    }
+    look_up(k0 + BK);
+  }
+  // after the load of the next lot
+  __device__ __forceinline__ void mend(uint32_t k0, f64x2 (&x)[2]) const {
+    const bool zero = (absent >> 1 & 1) || k0 + k() >= end;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e / 2][e % 2] = zero ? 0.0 : x[e / 2][e % 2];
+  }
+};
+
+// Where an element of k lies in its row of S in LDS: half a wave's stores of one k of each of its rows, and its reads of 16
+// rows of two k, fall on different banks each.  Runs of four stay together.
+template <int S> __device__ __forceinline__ uint32_t double_at(uint32_t k, uint32_t row) {
+  if constexpr (S == 32) return row ^ ((k >> 2 & 3) << 2 | ((k ^ k >> 4) & 1) << 4);
+  else return row ^ ((k >> 2 & 1) << 3 | ((k ^ k >> 3) & 1) << 4);
+}
+
+template <int S, class Left, class Right, class Store>
+__device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right right, Store store) {
+  constexpr int BK = double_depth(S), MT = S / 32;
+  static_assert(S * BK / 4 == 256, "four elements of each operand to a lane");
+  __shared__ __attribute__((aligned(16))) double lds_a[BK][S], lds_b[BK][S];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave_m = wave / 2 * (S / 2), wave_n = wave % 2 * (S / 2);
+  auto put_in = [&](auto& operand, double (&lds)[BK][S], uint32_t k0, f64x2 (&x)[2]) {
+    using Operand = std::remove_reference_t<decltype(operand)>;
+    operand.mend(k0, x);
+    if constexpr (Operand::kByRow) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds[Operand::k() + e][double_at<S>(Operand::k() + e, Operand::row())] = x[e / 2][e % 2];
+    } else {
+      f64x2* to = reinterpret_cast<f64x2*>(&lds[Operand::k()][double_at<S>(Operand::k(), Operand::column())]);
+      to[0] = x[0];
+      to[1] = x[1];
+    }
   };
   f64x4 sum[MT][MT] = {};
-  left(row_of(kA), k_of(kA), a);
-  right(row_of(kB), k_of(kB), b);
-  put_in(lds_a[0], kA, a);
-  put_in(lds_b[0], kB, b);
-  __syncthreads();
-  int buffer = 0;
-  for (uint32_t k0 = 0; k0 < depth; k0 += BK, buffer ^= 1) {
-    const bool more = k0 + BK < depth;
-    if (more) {
-      left(row_of(kA), k0 + BK + k_of(kA), a);
-      right(row_of(kB), k0 + BK + k_of(kB), b);
-    }
+  f64x2 a[2][2], b[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    left.load(h * BK, a[h]);
+    right.load(h * BK, b[h]);
+  }
+  auto step = [&](uint32_t k0, int h) {
+    put_in(left, lds_a, k0, a[h]);
+    put_in(right, lds_b, k0, b[h]);
+    __syncthreads();
+    left.load(k0 + 2 * BK, a[h]);
+    right.load(k0 + 2 * BK, b[h]);
 #pragma unroll
     for (int k = 0; k < BK; k += 4) {
       double l[MT], r[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        l[t] = lds_a[buffer][k + lane / 16][wave_m + t * 16 + lane % 16];
-        r[t] = lds_b[buffer][k + lane / 16][wave_n + t * 16 + lane % 16];
+        l[t] = lds_a[k + lane / 16][double_at<S>(k + lane / 16, wave_m + t * 16 + lane % 16)];
+        r[t] = lds_b[k + lane / 16][double_at<S>(k + lane / 16, wave_n + t * 16 + lane % 16)];
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int u = 0; u < MT; ++u) sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(l[t], r[u], sum[t][u], 0, 0, 0);
     }
-    if (more) {
-      put_in(lds_a[buffer ^ 1], kA, a);
-      put_in(lds_b[buffer ^ 1], kB, b);
-    }
     __syncthreads();
+  };
+  for (uint32_t k0 = 0; k0 < depth; k0 += 2 * BK) {   // lots beyond the last one are zeros
+    step(k0, 0);
+    step(k0 + BK, 1);
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -533,60 +616,44 @@ __device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right rig
       for (int r = 0; r < 4; ++r) store(wave_m + t * 16 + lane / 16 + 4 * r, wave_n + u * 16 + lane % 16, sum[t][u][r]);
 }
 
-// Four elements from p[at] on, zeros from `end` on and where the row is absent.
-__device__ __forceinline__ void load4(const double* p, uint32_t at, uint32_t end, bool present, double (&to)[4]) {
-  if (present && at + 4 <= end) {
-    __builtin_memcpy(&to[0], p + at, 16);
-    __builtin_memcpy(&to[2], p + at + 2, 16);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = present && at + e < end ? p[at + e] : 0.0;
-  }
-}
-
 template <int S, bool kB>
-__global__ void __launch_bounds__(256) grouped_double_kernel(const GroupedArgs a, const GroupedPlan p) {
+__global__ void __launch_bounds__(256, 2) grouped_double_kernel(const GroupedArgs a, const GroupedPlan p) {
   uint32_t m_tile, n_tile;
   Group g;
   if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, S, &g)) return;
   const uint32_t row0 = g.tile * S, col0 = n_tile * S;
   const double* b = static_cast<const double*>(a.b) + (int64_t)g.index * a.b_stride;
   double* c = static_cast<double*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
-  const uint32_t my_row = row0 + threadIdx.x / (S == 64 ? 4 : 8);   // of a, the same for all k
-  uint32_t from = a.a_rows;
-  if (my_row < g.rows) from = a.index_a ? (uint32_t)a.index_a[g.first + my_row] : g.first + my_row;
+  const uint32_t row = g.first + min(row0 + DoubleRow<S>::row(), g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
   const bool present = from < a.a_rows;
-  const double* left = static_cast<const double*>(a.a) + (int64_t)(present ? from : 0) * a.lda;
-  double_tile<S, true, kB>(
-      a.k, [&](uint32_t, uint32_t k, double (&to)[4]) { load4(left, k, a.k, present, to); },
-      [&](uint32_t n, uint32_t k, double (&to)[4]) {
-        if constexpr (kB) load4(b + (int64_t)(col0 + n) * a.ldb, k, a.k, col0 + n < a.n, to);
-        else load4(b + (int64_t)k * a.ldb, col0 + n, a.n, k < a.k, to);
-      },
-      [&](uint32_t r, uint32_t n, double sum) {
-        if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
-      });
+  const DoubleRow<S> left{static_cast<const double*>(a.a) + (int64_t)(present ? from : 0) * a.lda, a.k, present};
+  auto store = [&](uint32_t r, uint32_t n, double sum) {
+    if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
+  };
+  if constexpr (kB) {
+    const uint32_t column = min(col0 + DoubleRow<S>::row(), a.n - 1);
+    double_tile<S>(a.k, left, DoubleRow<S>{b + (int64_t)column * a.ldb, a.k, true}, store);
+  } else {
+    double_tile<S>(a.k, left, DoubleColumns<S>(b + col0, a.ldb, nullptr, 0, a.k, a.k, a.n - col0), store);
+  }
 }
 
 template <int S>
-__global__ void __launch_bounds__(256) grouped_weights_double_kernel(const GroupedArgs a, const GroupedPlan p) {
+__global__ void __launch_bounds__(256, 2) grouped_weights_double_kernel(const GroupedArgs a, const GroupedPlan p) {
   uint32_t m_tile, n_tile;
   if (!place_of(p, &m_tile, &n_tile)) return;
   const uint32_t tiles = (a.m + S - 1) / S, group = m_tile / tiles, row0 = (m_tile - group * tiles) * S, col0 = n_tile * S;
   const uint2 rows = group_rows(a, group);
   double* c = static_cast<double*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0;
-  auto element = [&](const void* m, const int32_t* index, uint32_t count, int64_t ld, uint32_t k, uint32_t column, uint32_t width, double (&to)[4]) {
-    uint32_t from = count;
-    if (k < rows.y) from = index ? (uint32_t)index[rows.x + k] : rows.x + k;
-    const bool present = from < count;
-    load4(static_cast<const double*>(m) + (int64_t)(present ? from : 0) * ld, column, width, present, to);
+  auto store = [&](uint32_t r, uint32_t n, double sum) {
+    if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
   };
-  double_tile<S, false, false>(
-      rows.y, [&](uint32_t r, uint32_t k, double (&to)[4]) { element(a.a, a.index_a, a.a_rows, a.lda, k, row0 + r, a.m, to); },
-      [&](uint32_t n, uint32_t k, double (&to)[4]) { element(a.b, a.index_b, a.b_rows, a.ldb, k, col0 + n, a.n, to); },
-      [&](uint32_t r, uint32_t n, double sum) {
-        if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
-      });
+  if (rows.y > 0 && a.a_rows > 0 && a.b_rows > 0) {
+    double_tile<S>(rows.y, DoubleColumns<S>(static_cast<const double*>(a.a) + row0, a.lda, a.index_a, rows.x, rows.y, a.a_rows, a.m - row0),
+                   DoubleColumns<S>(static_cast<const double*>(a.b) + col0, a.ldb, a.index_b, rows.x, rows.y, a.b_rows, a.n - col0), store);
+  } else {
+    for (uint32_t i = threadIdx.x; i < S * S; i += 256) store(i / S, i % S, 0.0);
+  }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -652,7 +719,7 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
   g.trans_b = trans_b != 0;
   const int64_t even_groups = std::min(n_groups, row_count);
   auto grid_of = [](const GroupedPlan& p) { return dim3((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun)); };
-  if (dtype == CT_F64 && a_row_count > 0) {
+  if (dtype == CT_F64 && a_row_count > 0 && a_col_count > 0) {
     const int64_t tiles64 = (row_count / 64 + even_groups / 2) * ceil_div(b_col_count, 64), side = tiles64 >= 1024 ? 64 : 32;
     const int64_t m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
     if (m_tiles * n_tiles <= kMostUnits) {
