@@ -9,7 +9,8 @@
 // same for all rows is taken out of S1 and S0: its own gradient is wp S1 + bp S0, and wp's is g S1.
 //
 // A row is held in registers by LANES lanes, VPT pieces of 16 bytes to each, so that every operand is read once and every
-// result written once.  Rows that do not fit (more than 16384 floats) take the kernels at the end, which read again.
+// result written once.  Rows that do not fit (more than 16384 floats), and those shorter than a piece, take the kernels at
+// the end, which read again.
 #include <algorithm>
 #include <cmath>
 
@@ -42,50 +43,43 @@ struct NormArgs {
 template <class T> __device__ __forceinline__ const T* row_of(const Matrix& m, int64_t row) { return static_cast<const T*>(m.p) + row * m.ld; }
 template <class T> __device__ __forceinline__ T* row_to(const Matrix& m, int64_t row) { return static_cast<T*>(m.p) + row * m.ld; }
 
-// The lanes that hold a row, and what each of them holds: piece t is elements N * (lane + t * LANES) and on.
+// The lanes that hold a row of N elements or more, and what each of them holds: VPT pieces of N elements.  Piece t belongs at
+// element N * (lane + t * LANES); one that would pass the end of the row is the row's last N elements instead, of which the
+// lane owns what lies behind its place, perhaps nothing.  So loads have no branches, and none is waited for before the next.
 template <class T, int LANES, int VPT>
 struct Row {
   static constexpr int N = Quad<T>::N, E = N * VPT;
   uint32_t lane, width;
-  __device__ __forceinline__ uint32_t at(int t) const { return N * (lane + t * LANES); }
-  __device__ __forceinline__ bool has(int t, int e) const { return at(t) + e < width; }
-  __device__ __forceinline__ void load(const T* p, T (&x)[E], T absent = 0) const {
+  __device__ __forceinline__ uint32_t place(int t) const { return N * (lane + t * LANES); }
+  __device__ __forceinline__ uint32_t start(int t) const { return min(place(t), width - N); }
+  __device__ __forceinline__ bool owns(int t, int e) const { return start(t) + e >= place(t); }
+  __device__ __forceinline__ Quad<T> piece(const T* p, int t) const { return load_quad(p + start(t)); }
+  // of an operand that may be absent: `fill` then
+  __device__ __forceinline__ Quad<T> piece_or(const void* p, T fill, int t) const {
+    Quad<T> q;
+    if (p) return piece(static_cast<const T*>(p), t);
 #pragma unroll
-    for (int t = 0; t < VPT; ++t) {
-      if (at(t) + N <= width) {
-        const Quad<T> q = load_quad(p + at(t));
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[t * N + e] = q.v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[t * N + e] = has(t, e) ? p[at(t) + e] : absent;
-      }
-    }
+    for (int e = 0; e < N; ++e) q.v[e] = fill;
+    return q;
   }
-  // absent pointer: `fill` everywhere
-  __device__ __forceinline__ void load_or(const void* p, T fill, T (&x)[E]) const {
-    if (p) load(static_cast<const T*>(p), x);
-    else {
+  __device__ __forceinline__ void load(const T* p, Quad<T> (&x)[VPT]) const {
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = fill;
-    }
+    for (int t = 0; t < VPT; ++t) x[t] = piece(p, t);
   }
-  __device__ __forceinline__ void store(T* p, const T (&x)[E]) const {
+  __device__ __forceinline__ T owned(int t, int e, T x) const { return owns(t, e) ? x : T(0); }
+  __device__ __forceinline__ void store(T* p, int t, const Quad<T>& q) const {
+    if (place(t) + N <= width) {
+      store_quad(p + place(t), q);
+    } else {
 #pragma unroll
-    for (int t = 0; t < VPT; ++t) {
-      if (at(t) + N <= width) {
-        Quad<T> q;
-#pragma unroll
-        for (int e = 0; e < N; ++e) q.v[e] = x[t * N + e];
-        store_quad(p + at(t), q);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (has(t, e)) p[at(t) + e] = x[t * N + e];
-      }
+      for (int e = 0; e < N; ++e)
+        if (owns(t, e)) p[start(t) + e] = q.v[e];
     }
   }
 };
+
+#define CT_EACH                        \
+  _Pragma("unroll") for (int t = 0; t < VPT; ++t) _Pragma("unroll") for (int e = 0; e < N; ++e)
 
 // Sums of K values over the LANES lanes of a row, in all of them.  A row of more than a wave is a whole block's; `lds` holds
 // K values to a wave, twice, used in turn so that one barrier a call is enough.
@@ -118,40 +112,37 @@ template <class T, int LANES, int VPT>
 __global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_kernel(const NormArgs a) {
   constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
   using R = Row<T, LANES, VPT>;
-  constexpr int E = R::E, N = R::N;
+  constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
   int turn = 0;
   const R at{threadIdx.x % LANES, a.width};
   const T inverse = T(1) / (T)a.width, epsilon = (T)a.epsilon;
   for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * kRows) {
-    T x[E], y[E];
+    Quad<T> x[VPT], y[VPT];
     at.load(row_of<T>(a.input, row), x);
-    if (a.residual.p) at.load(row_of<T>(a.residual, row), y);
+    at.load(row_of<T>(a.residual.p ? a.residual : a.input, row), y);
     // the norm of x in place, its statistics to `place`
-    auto norm = [&](T (&x)[E], int kind, const void* scale, const void* bias, int place) {
+    auto norm = [&](int kind, const void* scale, const void* bias, int place) {
       T mean[1] = {0}, square[1] = {0};
-      T w[E], b[E];
-      at.load_or(scale, T(1), w);
-      if (bias) at.load(static_cast<const T*>(bias), b);
       if (kind == CT_NORM_LAYER) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) mean[0] += x[i];
+        CT_EACH mean[0] += at.owned(t, e, x[t].v[e]);
         row_sum<T, LANES>(mean, lds, turn);
         mean[0] *= inverse;
-#pragma unroll
-        for (int t = 0; t < VPT; ++t)
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[t * N + e] = at.has(t, e) ? x[t * N + e] - mean[0] : T(0);
+        CT_EACH x[t].v[e] -= mean[0];
       }
-#pragma unroll
-      for (int i = 0; i < E; ++i) square[0] += x[i] * x[i];
+      CT_EACH square[0] += at.owned(t, e, x[t].v[e] * x[t].v[e]);
       row_sum<T, LANES>(square, lds, turn);
       const T rate = rate_of(square[0] * inverse, epsilon);
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = x[i] * rate * w[i];
-      if (bias) {
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> w = at.piece_or(scale, T(1), t);
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] += b[i];
+        for (int e = 0; e < N; ++e) x[t].v[e] = x[t].v[e] * rate * w.v[e];
+        if (bias) {
+          const Quad<T> b = at.piece(static_cast<const T*>(bias), t);
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[t].v[e] += b.v[e];
+        }
       }
       if (a.statistics && at.lane == 0) {
         T* to = static_cast<T*>(a.statistics) + place * a.rows + row;
@@ -165,35 +156,32 @@ __global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_
       to[0] = 0;
       to[a.rows] = 1;
     };
-    if (a.post != CT_NORM_NONE) norm(x, a.post, a.post_scale, a.post_bias, 0);
+    if (a.post != CT_NORM_NONE) norm(a.post, a.post_scale, a.post_bias, 0);
     else no_norm(0);
     if (a.gate_kind == kScalarGate || a.gate_kind == kRowGate) {
       const T g = static_cast<const T*>(a.gate.p)[a.gate_kind == kRowGate ? row * a.gate.ld : 0];
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[i] *= g;
+      CT_EACH x[t].v[e] *= g;
     } else if (a.gate_kind != kNoGate) {
-      T g[E];
-      at.load(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), g);
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] *= g[i];
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> g = at.piece(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[t].v[e] *= g.v[e];
+      }
     }
     if (a.residual.p) {
       const T c = (T)a.residual_scale;
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = c * y[i] + x[i];
+      CT_EACH x[t].v[e] = c * y[t].v[e] + x[t].v[e];
     }
 #pragma unroll
-    for (int t = 0; t < VPT; ++t)
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (!at.has(t, e)) x[t * N + e] = 0;   // a bias has no part beyond the row
-    at.store(row_to<T>(a.output, row), x);
+    for (int t = 0; t < VPT; ++t) at.store(row_to<T>(a.output, row), t, x[t]);
     if (a.pre == CT_NORM_NONE) {
       no_norm(2);
       continue;
     }
-    norm(x, a.pre, a.pre_scale, a.pre_bias, 2);
-    at.store(row_to<T>(a.normalized, row), x);
+    norm(a.pre, a.pre_scale, a.pre_bias, 2);
+#pragma unroll
+    for (int t = 0; t < VPT; ++t) at.store(row_to<T>(a.normalized, row), t, x[t]);
   }
 }
 
@@ -207,159 +195,183 @@ struct NormGradientArgs {
   int64_t rows;
   uint32_t width, blocks;
   int post, pre, gate_kind;
-  int slot[4];               // of S1, S0, T1, T0 in partial; negative: not wanted
+  int slot[4], slots;        // of S1, S0, T1, T0 in partial; negative: not wanted
   double residual_scale;
 };
 
 // Whether the gate is a factor of all rows' sums: then it is left out of them.
 __device__ __forceinline__ bool common_gate(int kind) { return kind == kNoGate || kind == kScalarGate || kind == kColumnGate; }
 
-template <class T, int LANES, int VPT, bool kSums, bool kBiases>
+// The sums over the rows stay in LDS, a value to each lane and element, so that registers are left for what is on its way: the
+// next row's operands are loaded into the registers of this one's as those are used up.
+// kSums: 0 none, 1 S1 and T1, 2 all.  An absent gradient of the results is read from `input` and not used.
+template <class T, int LANES, int VPT, int kSums>
 __global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_gradient_kernel(const NormGradientArgs a) {
   constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
   using R = Row<T, LANES, VPT>;
-  constexpr int E = R::E, N = R::N;
+  constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
+  extern __shared__ __attribute__((aligned(16))) char sums_lds[];
   int turn = 0;
   const R at{threadIdx.x % LANES, a.width};
   const T inverse = T(1) / (T)a.width;
-  T s1[kSums ? E : 1] = {}, t1[kSums ? E : 1] = {}, s0[kBiases ? E : 1] = {}, t0[kBiases ? E : 1] = {};
-  const T* statistics = static_cast<const T*>(a.statistics);
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * kRows) {
-    T d[E];
-    if (a.output_gradient.p) at.load(row_of<T>(a.output_gradient, row), d);
-    else {
+  // the pieces of sum `slot` of a group of lanes, side by side
+  Quad<T>* const sums = reinterpret_cast<Quad<T>*>(sums_lds);
+  const uint32_t pieces = (a.width + N - 1) / N;
+  auto has = [&](int t) { return at.lane + t * LANES < pieces; };
+  auto sum_at = [&](int slot, int group, int t) -> Quad<T>& { return sums[(slot * kRows + group) * pieces + at.lane + t * LANES]; };
+  const int group = threadIdx.x / LANES;
+  // value(t, e) to every sum of a slot
+  auto add_to = [&](int slot, auto value) {
+    if (slot < 0) return;
 #pragma unroll
-      for (int i = 0; i < E; ++i) d[i] = 0;
+    for (int t = 0; t < VPT; ++t) {
+      if (!has(t)) continue;
+      Quad<T> q = sum_at(slot, group, t);
+#pragma unroll
+      for (int e = 0; e < N; ++e) q.v[e] += value(t, e);
+      sum_at(slot, group, t) = q;
     }
-    T z[E];
+  };
+  if constexpr (kSums > 0) {
+#pragma unroll
+    for (int slot = 0; slot < 2 * kSums; ++slot)
+      if (slot < a.slots) {
+#pragma unroll
+        for (int t = 0; t < VPT; ++t)
+          if (has(t)) sum_at(slot, group, t) = Quad<T>{};
+      }
+  }
+  const T* statistics = static_cast<const T*>(a.statistics);
+  const bool post = a.post != CT_NORM_NONE, pre = a.pre != CT_NORM_NONE && a.normalized_gradient.p;
+  const Matrix& of_d = a.output_gradient.p ? a.output_gradient : a.input;
+  const Matrix& of_dh = pre ? a.normalized_gradient : a.input;
+  const Matrix& of_oh = pre ? a.output : a.input;
+  const int64_t stride = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
+  Quad<T> d[VPT], z[VPT], dh[VPT], oh[VPT];
+  if (row < a.rows) {
+    at.load(row_of<T>(of_dh, row), dh);
+    at.load(row_of<T>(of_oh, row), oh);
+    at.load(row_of<T>(of_d, row), d);
     at.load(row_of<T>(a.input, row), z);
-    if (a.pre != CT_NORM_NONE && a.normalized_gradient.p) {
-      T dh[E], oh[E], w[E];
-      at.load(row_of<T>(a.normalized_gradient, row), dh);
-      at.load(row_of<T>(a.output, row), oh);
-      at.load_or(a.pre_scale, T(1), w);
+  }
+  for (; row < a.rows; row += stride) {
+    const int64_t next = min(row + stride, a.rows - 1);
+    if (!a.output_gradient.p) CT_EACH d[t].v[e] = 0;
+    if (pre) {
       const T mean = statistics[2 * a.rows + row], rate = statistics[3 * a.rows + row];
+      CT_EACH oh[t].v[e] = (oh[t].v[e] - mean) * rate;
+      if constexpr (kSums > 0) add_to(a.slot[2], [&](int t, int e) { return dh[t].v[e] * oh[t].v[e]; });
+      if constexpr (kSums > 1) add_to(a.slot[3], [&](int t, int e) { return dh[t].v[e]; });
       T sums[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        oh[i] = (oh[i] - mean) * rate;
-        if constexpr (kSums) t1[i] += dh[i] * oh[i];
-        if constexpr (kBiases) t0[i] += dh[i];
-        const T y = dh[i] * w[i];   // zero beyond the row
-        sums[0] += y;
-        sums[1] += y * oh[i];
-        dh[i] = y;
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> w = at.piece_or(a.pre_scale, T(1), t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          dh[t].v[e] *= w.v[e];
+          sums[0] += at.owned(t, e, dh[t].v[e]);
+          sums[1] += at.owned(t, e, dh[t].v[e] * oh[t].v[e]);
+        }
       }
       row_sum<T, LANES>(sums, lds, turn);
       const T first = a.pre == CT_NORM_LAYER ? sums[0] * inverse : T(0), second = sums[1] * inverse;
-#pragma unroll
-      for (int i = 0; i < E; ++i) d[i] += rate * (dh[i] - first - oh[i] * second);
+      CT_EACH d[t].v[e] += rate * (dh[t].v[e] - first - oh[t].v[e] * second);
     }
-#pragma unroll
-    for (int t = 0; t < VPT; ++t)
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (!at.has(t, e)) d[t * N + e] = 0;
+    at.load(row_of<T>(of_dh, next), dh);
+    at.load(row_of<T>(of_oh, next), oh);
     if (a.residual_gradient.p) {
-      T dr[E];
       const T c = (T)a.residual_scale;
 #pragma unroll
-      for (int i = 0; i < E; ++i) dr[i] = c * d[i];
-      at.store(row_to<T>(a.residual_gradient, row), dr);
+      for (int t = 0; t < VPT; ++t) {
+        Quad<T> q;
+#pragma unroll
+        for (int e = 0; e < N; ++e) q.v[e] = c * d[t].v[e];
+        at.store(row_to<T>(a.residual_gradient, row), t, q);
+      }
     }
     // zh; its sums; the gate's gradient; dz
-    const bool post = a.post != CT_NORM_NONE;
     const T mean = post ? statistics[row] : T(0), rate = post ? statistics[a.rows + row] : T(1);
-    T w[E], b[E], g[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) z[i] = (z[i] - mean) * rate;
-    at.load_or(post ? a.post_scale : nullptr, T(1), w);
-    at.load_or(post ? a.post_bias : nullptr, T(0), b);
-    T row_gate = 1;
-    if (a.gate_kind == kScalarGate || a.gate_kind == kRowGate)
-      row_gate = static_cast<const T*>(a.gate.p)[a.gate_kind == kRowGate ? row * a.gate.ld : 0];
-    if (a.gate_kind == kColumnGate || a.gate_kind == kFullGate)
-      at.load(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), g);
-    else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) g[i] = row_gate;
+    CT_EACH z[t].v[e] = (z[t].v[e] - mean) * rate;
+    const bool of_columns = common_gate(a.gate_kind), of_row = a.gate_kind == kRowGate && a.gate_gradient.p;
+    if (kSums > 0 && of_columns) {
+      add_to(a.slot[0], [&](int t, int e) { return d[t].v[e] * z[t].v[e]; });
+      if constexpr (kSums > 1) add_to(a.slot[1], [&](int t, int e) { return d[t].v[e]; });
     }
-    if constexpr (kSums) {
-      if (common_gate(a.gate_kind)) {
+    T sums[3] = {0, 0, 0};
+    if (of_row || (a.gate_kind == kFullGate && a.gate_gradient.p)) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) s1[i] += d[i] * z[i];
-      } else {
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> w = at.piece_or(post ? a.post_scale : nullptr, T(1), t);
+        Quad<T> u = at.piece_or(post ? a.post_bias : nullptr, T(0), t);
 #pragma unroll
-        for (int i = 0; i < E; ++i) s1[i] += g[i] * d[i] * z[i];
+        for (int e = 0; e < N; ++e) {
+          u.v[e] = d[t].v[e] * (z[t].v[e] * w.v[e] + u.v[e]);
+          sums[2] += at.owned(t, e, u.v[e]);
+        }
+        if (!of_row) at.store(row_to<T>(a.gate_gradient, row), t, u);
       }
     }
-    if constexpr (kBiases) {
-      if (common_gate(a.gate_kind)) {
+    if (a.gate_kind == kColumnGate || a.gate_kind == kFullGate) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) s0[i] += d[i];
-      } else {
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> g = at.piece(static_cast<const T*>(a.gate.p) + (a.gate_kind == kFullGate ? row * a.gate.ld : 0), t);
 #pragma unroll
-        for (int i = 0; i < E; ++i) s0[i] += g[i] * d[i];
+        for (int e = 0; e < N; ++e) d[t].v[e] *= g.v[e];
       }
+    } else if (a.gate_kind != kNoGate) {
+      const T g = static_cast<const T*>(a.gate.p)[a.gate_kind == kRowGate ? row * a.gate.ld : 0];
+      CT_EACH d[t].v[e] *= g;
     }
-    if (a.gate_kind == kFullGate && a.gate_gradient.p) {
-      T dg[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) dg[i] = d[i] * (z[i] * w[i] + b[i]);
-      at.store(row_to<T>(a.gate_gradient, row), dg);
+    if (kSums > 0 && !of_columns) {
+      add_to(a.slot[0], [&](int t, int e) { return d[t].v[e] * z[t].v[e]; });
+      if constexpr (kSums > 1) add_to(a.slot[1], [&](int t, int e) { return d[t].v[e]; });
     }
-    const bool of_row = a.gate_kind == kRowGate && a.gate_gradient.p;
     if (post || of_row) {
-      T sums[3] = {0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        if (of_row) sums[2] += d[i] * (z[i] * w[i] + b[i]);
-        d[i] *= g[i] * w[i];
-        sums[0] += d[i];
-        sums[1] += d[i] * z[i];
+      for (int t = 0; t < VPT; ++t) {
+        const Quad<T> w = at.piece_or(post ? a.post_scale : nullptr, T(1), t);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          d[t].v[e] *= w.v[e];
+          sums[0] += at.owned(t, e, d[t].v[e]);
+          sums[1] += at.owned(t, e, d[t].v[e] * z[t].v[e]);
+        }
       }
       row_sum<T, LANES>(sums, lds, turn);
       if (of_row && at.lane == 0) static_cast<T*>(a.gate_gradient.p)[row * a.gate_gradient.ld] = sums[2];
       if (post) {
         const T first = a.post == CT_NORM_LAYER ? sums[0] * inverse : T(0), second = sums[1] * inverse;
-#pragma unroll
-        for (int i = 0; i < E; ++i) d[i] = rate * (d[i] - first - z[i] * second);
+        CT_EACH d[t].v[e] = rate * (d[t].v[e] - first - z[t].v[e] * second);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) d[i] *= g[i];
     }
-    if (a.input_gradient.p) at.store(row_to<T>(a.input_gradient, row), d);
+    if (a.input_gradient.p) {
+#pragma unroll
+      for (int t = 0; t < VPT; ++t) at.store(row_to<T>(a.input_gradient, row), t, d[t]);
+    }
+    at.load(row_of<T>(of_d, next), d);
+    at.load(row_of<T>(a.input, next), z);
   }
-  if constexpr (kSums) {
-    // the sums of the block's rows, in the order of their groups of lanes
-    constexpr int kSumLds = kRows > 1 ? kRows * LANES * E : 1;
-    __shared__ T shared[kSumLds];
-    auto put = [&](int slot, const T (&of)[E]) {
-      if (slot < 0) return;
-      T* to = static_cast<T*>(a.partial) + ((int64_t)slot * a.blocks + blockIdx.x) * a.width;
-      if constexpr (kRows > 1) {
-        __syncthreads();
+  if constexpr (kSums > 0) {
+    // of the block's rows, in the order of their groups of lanes
+    __syncthreads();
+    if (threadIdx.x >= LANES) return;
 #pragma unroll
-        for (int i = 0; i < E; ++i) shared[(threadIdx.x / LANES * E + i) * LANES + at.lane] = of[i];
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < LANES * E; i += kThreads) {
-          const uint32_t lane = i % LANES, e = i / LANES, column = N * (lane + e / N * LANES) + e % N;
-          T sum = shared[i];
+    for (int s = 0; s < 4; ++s) {
+      if (a.slot[s] < 0 || (kSums == 1 && s % 2 == 1)) continue;
+      T* to = static_cast<T*>(a.partial) + ((int64_t)a.slot[s] * a.blocks + blockIdx.x) * a.width;
 #pragma unroll
-          for (int r = 1; r < kRows; ++r) sum += shared[r * LANES * E + i];
-          if (column < a.width) to[column] = sum;
+      for (int t = 0; t < VPT; ++t) {
+        if (!has(t)) continue;
+        Quad<T> q = sum_at(a.slot[s], 0, t);
+        for (int r = 1; r < kRows; ++r) {
+          const Quad<T> other = sum_at(a.slot[s], r, t);
+#pragma unroll
+          for (int e = 0; e < N; ++e) q.v[e] += other.v[e];
         }
-      } else {
-        at.store(to, of);
+        at.store(to, t, q);
       }
-    };
-    put(a.slot[0], s1);
-    put(a.slot[2], t1);
-    if constexpr (kBiases) {
-      put(a.slot[1], s0);
-      put(a.slot[3], t0);
     }
   }
 }
@@ -375,26 +387,28 @@ struct NormFinishArgs {
   int gate_kind;
 };
 
-// The blocks' sums of 16 columns, added in their order within each of 16 runs of blocks, in double.
+// The blocks' sums of 32 columns, added in their order within each of 32 runs of blocks, in double.
 template <class T>
-__global__ void __launch_bounds__(256) norm_finish_kernel(const NormFinishArgs a) {
-  __shared__ double lds[4][16][16];
-  const uint32_t column = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
+__global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs a) {
+  __shared__ double lds[4][32][32];
+  const uint32_t column = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     double sum = 0;
-    if (a.slot[s] >= 0 && column < a.width)
-      for (uint32_t b = run; b < a.blocks; b += 16)
-        sum += (double)static_cast<const T*>(a.partial)[((int64_t)a.slot[s] * a.blocks + b) * a.width + column];
-    lds[s][run][threadIdx.x % 16] = sum;
+    if (a.slot[s] >= 0 && column < a.width) {
+      const T* from = static_cast<const T*>(a.partial) + (int64_t)a.slot[s] * a.blocks * a.width + column;
+#pragma unroll 8
+      for (uint32_t b = run; b < a.blocks; b += 32) sum += (double)from[(int64_t)b * a.width];
+    }
+    lds[s][run][threadIdx.x % 32] = sum;
   }
   __syncthreads();
-  if (threadIdx.x >= 16 || column >= a.width) return;
+  if (threadIdx.x >= 32 || column >= a.width) return;
   double sums[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     sums[s] = lds[s][0][threadIdx.x];
-    for (int r = 1; r < 16; ++r) sums[s] += lds[s][r][threadIdx.x];
+    for (int r = 1; r < 32; ++r) sums[s] += lds[s][r][threadIdx.x];
   }
   double gate = 1;
   if (a.gate_kind == kScalarGate) gate = (double)*static_cast<const T*>(a.gate);
@@ -614,6 +628,7 @@ template <class T, class F>
 bool with_shape(uint32_t width, F f) {
   constexpr uint32_t N = Quad<T>::N;
   const uint32_t pieces = (width + N - 1) / N;
+  if (width < N) return false;
 #define CT_SHAPE(L, V) \
   if (pieces <= L * V) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>()), true
   CT_SHAPE(16, 1); CT_SHAPE(16, 2); CT_SHAPE(16, 4);
@@ -625,6 +640,7 @@ bool with_shape(uint32_t width, F f) {
 }
 
 constexpr int64_t kMostNormBlocks = 1 << 20;
+constexpr int64_t kMostSumLds = 128 << 10;   // of a block, for its sums
 constexpr int64_t kMostSumBytes = int64_t(32) << 20;
 
 template <class T>
@@ -643,9 +659,10 @@ template <class T>
 int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
   const int slots = std::max({a.slot[0], a.slot[1], a.slot[2], a.slot[3]}) + 1;
   const bool sums = slots > 0, biases = a.slot[1] >= 0 || a.slot[3] >= 0;
-  const bool fits = with_shape<T>(a.width, [](auto, auto) {});
+  a.slots = slots;
   int64_t rows_a_block = 1;
-  with_shape<T>(a.width, [&](auto lanes, auto) { rows_a_block = std::max(1, kNormBlock / decltype(lanes)::value); });
+  bool fits = with_shape<T>(a.width, [&](auto lanes, auto) { rows_a_block = std::max(1, kNormBlock / decltype(lanes)::value); });
+  fits = fits && (int64_t)slots * a.width * (int64_t)sizeof(T) <= kMostSumLds;
   // whose sums the last launch adds
   const int64_t most_blocks = std::max<int64_t>(1, std::min<int64_t>(512, kMostSumBytes / ((int64_t)std::max(slots, 1) * a.width * (int64_t)sizeof(T))));
   a.blocks = f.blocks = (uint32_t)std::min((a.rows + rows_a_block - 1) / rows_a_block, most_blocks);
@@ -664,9 +681,14 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
     with_shape<T>(a.width, [&](auto lanes, auto pieces) {
       constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
       const int64_t blocks = sums ? a.blocks : std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
-      if (biases) hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, true, true>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
-      else if (sums) hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, true, false>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((norm_gradient_kernel<T, L, V, false, false>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+      const size_t lds = (size_t)slots * kRows * ((a.width + Quad<T>::N - 1) / Quad<T>::N) * sizeof(Quad<T>);
+      auto launch = [&](auto kernel) {
+        if (lds > (48 << 10)) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kThreads), lds, s, a);
+      };
+      if (biases) launch(norm_gradient_kernel<T, L, V, 2>);
+      else if (sums) launch(norm_gradient_kernel<T, L, V, 1>);
+      else launch(norm_gradient_kernel<T, L, V, 0>);
     });
   } else {
     const uint32_t columns = (a.width + 255) / 256;
@@ -674,7 +696,7 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
     if (sums) hipLaunchKernelGGL((norm_long_sums_kernel<T>), dim3(columns, a.blocks), dim3(256), 0, s, a, means);
     hipLaunchKernelGGL((norm_long_apply_kernel<T>), dim3(columns, (uint32_t)std::min<int64_t>(a.rows, 4096)), dim3(256), 0, s, a, means);
   }
-  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 15) / 16), dim3(256), 0, s, f);
+  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 31) / 32), dim3(1024), 0, s, f);
   if (f.by_column) hipLaunchKernelGGL((norm_scalar_gate_kernel<T>), dim3(1), dim3(256), 0, s, by_column, a.width, static_cast<T*>(f.gate_gradient));
   note_kernel(fits ? "norm_residual_gradient" : "norm_residual_gradient_long");
   return after_launch(s);
