@@ -46,7 +46,7 @@ template <class T> __device__ __forceinline__ T* row_to(const Matrix& m, int64_t
 // The lanes that hold a row of N elements or more, and what each of them holds: VPT pieces of N elements.  Piece t belongs at
 // element N * (lane + t * LANES); one that would pass the end of the row is the row's last N elements instead, of which the
 // lane owns what lies behind its place, perhaps nothing.  So loads have no branches, and none is waited for before the next.
-template <class T, int LANES, int VPT>
+template <class T, int LANES, int VPT, bool kStreaming>
 struct Row {
   static constexpr int N = Quad<T>::N, E = N * VPT;
   uint32_t lane, width;
@@ -64,12 +64,12 @@ struct Row {
   }
   __device__ __forceinline__ void load(const T* p, Quad<T> (&x)[VPT]) const {
 #pragma unroll
-    for (int t = 0; t < VPT; ++t) x[t] = piece(p, t);
+    for (int t = 0; t < VPT; ++t) x[t] = load_quad<kStreaming>(p + start(t));
   }
   __device__ __forceinline__ T owned(int t, int e, T x) const { return owns(t, e) ? x : T(0); }
   __device__ __forceinline__ void store(T* p, int t, const Quad<T>& q) const {
     if (place(t) + N <= width) {
-      store_quad(p + place(t), q);
+      store_quad<kStreaming>(p + place(t), q);
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -108,10 +108,10 @@ __device__ __forceinline__ void row_sum(T (&v)[K], T* lds, int& turn) {
 
 template <class T> __device__ __forceinline__ T rate_of(T mean_square, T epsilon) { return T(1) / (T)sqrt(mean_square + epsilon); }
 
-template <class T, int LANES, int VPT>
+template <class T, int LANES, int VPT, bool kStreaming>
 __global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_kernel(const NormArgs a) {
   constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
-  using R = Row<T, LANES, VPT>;
+  using R = Row<T, LANES, VPT, kStreaming>;
   constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
   int turn = 0;
@@ -205,10 +205,10 @@ __device__ __forceinline__ bool common_gate(int kind) { return kind == kNoGate |
 // The sums over the rows stay in LDS, a value to each lane and element, so that registers are left for what is on its way: the
 // next row's operands are loaded into the registers of this one's as those are used up.
 // kSums: 0 none, 1 S1 and T1, 2 all.  An absent gradient of the results is read from `input` and not used.
-template <class T, int LANES, int VPT, int kSums>
+template <class T, int LANES, int VPT, int kSums, bool kStreaming>
 __global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_gradient_kernel(const NormGradientArgs a) {
   constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
-  using R = Row<T, LANES, VPT>;
+  using R = Row<T, LANES, VPT, kStreaming>;
   constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
   extern __shared__ __attribute__((aligned(16))) char sums_lds[];
@@ -390,13 +390,15 @@ struct NormFinishArgs {
 // The blocks' sums of 32 columns, added in their order within each of 32 runs of blocks, in double.
 template <class T>
 __global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs a) {
-  __shared__ double lds[4][32][32];
+  __shared__ double lds[2][32][32];
   const uint32_t column = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
+  // S1 and S0 by one half of the blocks, T1 and T0 by the other
+  const int half = 2 * blockIdx.y;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int s = 0; s < 2; ++s) {
     double sum = 0;
-    if (a.slot[s] >= 0 && column < a.width) {
-      const T* from = static_cast<const T*>(a.partial) + (int64_t)a.slot[s] * a.blocks * a.width + column;
+    if (a.slot[half + s] >= 0 && column < a.width) {
+      const T* from = static_cast<const T*>(a.partial) + (int64_t)a.slot[half + s] * a.blocks * a.width + column;
 #pragma unroll 8
       for (uint32_t b = run; b < a.blocks; b += 32) sum += (double)from[(int64_t)b * a.width];
     }
@@ -404,22 +406,25 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs 
   }
   __syncthreads();
   if (threadIdx.x >= 32 || column >= a.width) return;
-  double sums[4];
+  double sums[2];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int s = 0; s < 2; ++s) {
     sums[s] = lds[s][0][threadIdx.x];
     for (int r = 1; r < 32; ++r) sums[s] += lds[s][r][threadIdx.x];
+  }
+  auto store = [&](void* to, double v) {
+    if (to) static_cast<T*>(to)[column] = (T)v;
+  };
+  if (half) {
+    store(a.pre_scale_gradient, sums[0]);
+    store(a.pre_bias_gradient, sums[1]);
+    return;
   }
   double gate = 1;
   if (a.gate_kind == kScalarGate) gate = (double)*static_cast<const T*>(a.gate);
   if (a.gate_kind == kColumnGate) gate = (double)static_cast<const T*>(a.gate)[column];
-  auto store = [&](void* to, double v) {
-    if (to) static_cast<T*>(to)[column] = (T)v;
-  };
   store(a.post_scale_gradient, gate * sums[0]);
   store(a.post_bias_gradient, gate * sums[1]);
-  store(a.pre_scale_gradient, sums[2]);
-  store(a.pre_bias_gradient, sums[3]);
   const double scale = a.post_scale ? (double)static_cast<const T*>(a.post_scale)[column] : 1.0;
   const double bias = a.post_bias ? (double)static_cast<const T*>(a.post_bias)[column] : 0.0;
   const double of_gate = scale * sums[0] + (a.slot[1] >= 0 ? bias * sums[1] : 0.0);
@@ -643,12 +648,17 @@ constexpr int64_t kMostNormBlocks = 1 << 20;
 constexpr int64_t kMostSumLds = 128 << 10;   // of a block, for its sums
 constexpr int64_t kMostSumBytes = int64_t(32) << 20;
 
+// Operands and results that the last-level cache does not hold together go past the caches.
+bool streaming(int64_t rows, int64_t width, int64_t matrices, int64_t size) { return rows * width * matrices * size > int64_t(256) << 20; }
+
 template <class T>
 int norm_typed(hipStream_t s, const NormArgs& a) {
   const bool taken = with_shape<T>(a.width, [&](auto lanes, auto pieces) {
     constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
     const int64_t blocks = std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
-    hipLaunchKernelGGL((norm_kernel<T, L, V>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+    if (streaming(a.rows, a.width, 3 + (a.pre != CT_NORM_NONE), sizeof(T)))
+      hipLaunchKernelGGL((norm_kernel<T, L, V, true>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((norm_kernel<T, L, V, false>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
   });
   if (!taken) hipLaunchKernelGGL((norm_long_kernel<T>), dim3((uint32_t)std::min(a.rows, kMostNormBlocks)), dim3(kLongBlock), 0, s, a);
   note_kernel(taken ? "norm_residual" : "norm_residual_long");
@@ -686,9 +696,13 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
         if (lds > (48 << 10)) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kThreads), lds, s, a);
       };
-      if (biases) launch(norm_gradient_kernel<T, L, V, 2>);
-      else if (sums) launch(norm_gradient_kernel<T, L, V, 1>);
-      else launch(norm_gradient_kernel<T, L, V, 0>);
+      const bool past = streaming(a.rows, a.width, 6, sizeof(T));
+      if (biases && past) launch(norm_gradient_kernel<T, L, V, 2, true>);
+      else if (biases) launch(norm_gradient_kernel<T, L, V, 2, false>);
+      else if (sums && past) launch(norm_gradient_kernel<T, L, V, 1, true>);
+      else if (sums) launch(norm_gradient_kernel<T, L, V, 1, false>);
+      else if (past) launch(norm_gradient_kernel<T, L, V, 0, true>);
+      else launch(norm_gradient_kernel<T, L, V, 0, false>);
     });
   } else {
     const uint32_t columns = (a.width + 255) / 256;
@@ -696,7 +710,7 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
     if (sums) hipLaunchKernelGGL((norm_long_sums_kernel<T>), dim3(columns, a.blocks), dim3(256), 0, s, a, means);
     hipLaunchKernelGGL((norm_long_apply_kernel<T>), dim3(columns, (uint32_t)std::min<int64_t>(a.rows, 4096)), dim3(256), 0, s, a, means);
   }
-  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 31) / 32), dim3(1024), 0, s, f);
+  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 31) / 32, 2), dim3(1024), 0, s, f);
   if (f.by_column) hipLaunchKernelGGL((norm_scalar_gate_kernel<T>), dim3(1), dim3(256), 0, s, by_column, a.width, static_cast<T*>(f.gate_gradient));
   note_kernel(fits ? "norm_residual_gradient" : "norm_residual_gradient_long");
   return after_launch(s);

@@ -27,11 +27,25 @@ template <class T> struct Quad {
   static constexpr int N = 16 / sizeof(T);
   T v[N];
 };
-template <class T> __device__ __forceinline__ Quad<T> load_quad(const T* p) {
-  Quad<T> q;
-  __builtin_memcpy(&q, p, 16);
-  return q;
+template <class T> struct QuadBits {
+  typedef T Aligned __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef Aligned AtElement __attribute__((aligned(sizeof(T))));
+};
+// kStreaming: past the caches, for what is used once and does not fit them
+template <bool kStreaming = false, class T> __device__ __forceinline__ Quad<T> load_quad(const T* p) {
+  using Bits = QuadBits<T>;
+  const typename Bits::AtElement* from = reinterpret_cast<const typename Bits::AtElement*>(p);
+  typename Bits::Aligned v;
+  if constexpr (kStreaming) v = __builtin_nontemporal_load(from);
+  else v = *from;
+  return __builtin_bit_cast(Quad<T>, v);
 }
-template <class T> __device__ __forceinline__ void store_quad(T* p, const Quad<T>& q) { __builtin_memcpy(p, &q, 16); }
+template <bool kStreaming = false, class T> __device__ __forceinline__ void store_quad(T* p, const Quad<T>& q) {
+  using Bits = QuadBits<T>;
+  typename Bits::AtElement* to = reinterpret_cast<typename Bits::AtElement*>(p);
+  const typename Bits::Aligned v = __builtin_bit_cast(typename Bits::Aligned, q);
+  if constexpr (kStreaming) __builtin_nontemporal_store(v, to);
+  else *to = v;
+}
 
 }  // namespace cthip
