@@ -17,6 +17,7 @@ using namespace cthip;
 namespace {
 
 constexpr int kRouteBlock = 256;
+constexpr int64_t kCombineCacheBytes = int64_t(256) << 20;   // what the last-level cache holds
 constexpr int64_t kMostBlocks = 1 << 20;   // of a launch; blocks take more than one token each beyond
 constexpr int kMostExperts = 1024, kMostChosen = 32;
 
@@ -317,57 +318,169 @@ struct CombineArgs {
   uint32_t n, n_chosen, width;
 };
 
-template <class T>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+constexpr int kCombineBlock = 256;
+constexpr int kRowsAhead = 4;   // of a token, whose loads are on their way together
+
+// A wave to a part of a token's row: 16 bytes to a lane, kRowsAhead rows of the token at a time.  A lane that would pass the end of the
+// row takes its last 16 bytes and stores what lies behind its place.
+template <class T, bool kStreaming>
+__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const CombineArgs a, uint32_t parts, FastDiv parts_fd) {
+  constexpr uint32_t N = Quad<T>::N;
+  const uint32_t lane = threadIdx.x & 63, waves = gridDim.x * (kCombineBlock / 64);
   const T* rows = static_cast<const T*>(a.rows);
   const T* weights = static_cast<const T*>(a.weights);
-  for (uint32_t token = blockIdx.x; token < a.n; token += gridDim.x) {
-  T* out = static_cast<T*>(a.output) + (int64_t)token * a.output_colstride;
-  for (uint32_t c = threadIdx.x; c < a.width; c += 256) {
-    T sum = 0;
-    for (uint32_t j = 0; j < a.n_chosen; ++j) {
-      const int64_t at = (int64_t)token * a.n_chosen + j;
-      const int64_t slot = a.slots[at];
-      if (slot < 0 || slot >= a.row_count) continue;
-      const T x = rows[slot * a.rows_colstride + c];
-      sum += weights ? weights[at] * x : x;
+  for (uint64_t unit = (blockIdx.x * kCombineBlock + threadIdx.x) >> 6; unit < (uint64_t)a.n * parts; unit += waves) {
+    uint32_t token, part;
+    if (parts == 1) token = (uint32_t)unit, part = 0;
+    else if (unit < (uint64_t(1) << 31)) parts_fd.divmod((uint32_t)unit, token, part);
+    else token = (uint32_t)(unit / parts), part = (uint32_t)(unit % parts);
+    const uint32_t place = (part * 64 + lane) * N;
+    if (place >= a.width) continue;
+    const uint32_t c = a.width >= N ? min(place, a.width - N) : 0, count = min(N, a.width);
+    const int64_t first = (int64_t)token * a.n_chosen;
+    Quad<T> sum = {};
+    for (uint32_t j0 = 0; j0 < a.n_chosen; j0 += kRowsAhead) {
+      Quad<T> x[kRowsAhead];
+      T w[kRowsAhead];
+#pragma unroll
+      for (int r = 0; r < kRowsAhead; ++r) {
+        const uint32_t j = min(j0 + r, a.n_chosen - 1);
+        const int64_t slot = a.slots[first + j];
+        const bool in = j0 + r < a.n_chosen && slot >= 0 && slot < a.row_count;
+        w[r] = !in ? T(0) : weights ? weights[first + j] : T(1);
+        x[r] = Quad<T>{};
+        if (!in) continue;
+        const T* from = rows + slot * a.rows_colstride + c;
+        if (a.width >= N) x[r] = load_quad<kStreaming>(from);
+        else
+          for (uint32_t e = 0; e < count; ++e) x[r].v[e] = from[e];
+      }
+#pragma unroll
+      for (int r = 0; r < kRowsAhead; ++r)
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e) sum.v[e] += w[r] * x[r].v[e];
     }
-    out[c] = sum;
+    T* out = static_cast<T*>(a.output) + (int64_t)token * a.output_colstride;
+    if (place + N <= a.width) store_quad<kStreaming>(out + place, sum);
+    else {
+#pragma unroll
+      for (uint32_t e = 0; e < N; ++e)
+        if (e < count && c + e >= place) out[c + e] = sum.v[e];
+    }
   }
+}
+
+// WAVES waves to a token, and its rows kRowsAhead at a time: its gradient is read again from the caches for every such lot.
+template <class T, int WAVES, bool kStreaming>
+__global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const CombineArgs a) {
+  constexpr uint32_t N = Quad<T>::N;
+  constexpr int kTokens = kCombineBlock / 64 / WAVES;
+  __shared__ T lds[2][kCombineBlock / 64][kRowsAhead];
+  int turn = 0;
+  const uint32_t wave = threadIdx.x >> 6, of_token = threadIdx.x % (64 * WAVES), stride = 64 * WAVES * N;
+  const T* weights = static_cast<const T*>(a.weights);
+  // all of a block's waves go on together: a token beyond the last one is the last one, and not stored
+  for (uint32_t t0 = blockIdx.x * kTokens; t0 < a.n; t0 += gridDim.x * kTokens) {
+    const uint32_t token = min(t0 + wave / WAVES, a.n - 1);
+    const bool mine = t0 + wave / WAVES < a.n;
+    const int64_t first = (int64_t)token * a.n_chosen;
+    const T* dy = static_cast<const T*>(a.output_gradient) + (int64_t)token * a.gradient_colstride;
+    for (uint32_t j0 = 0; j0 < a.n_chosen; j0 += kRowsAhead) {
+      T dot[kRowsAhead], w[kRowsAhead];
+      int64_t slot[kRowsAhead];
+#pragma unroll
+      for (int r = 0; r < kRowsAhead; ++r) {
+        const uint32_t j = min(j0 + r, a.n_chosen - 1);
+        slot[r] = a.slots[first + j];
+        if (!mine || j0 + r >= a.n_chosen || slot[r] < 0 || slot[r] >= a.row_count) slot[r] = -1;
+        w[r] = weights ? weights[first + j] : T(1);
+        dot[r] = 0;
+      }
+      for (uint32_t place = of_token * N; place < a.width; place += stride) {
+        const uint32_t c = a.width >= N ? min(place, a.width - N) : 0, count = min(N, a.width);
+        Quad<T> g = {}, x[kRowsAhead];
+        if (a.width >= N) g = load_quad(dy + c);
+        else
+          for (uint32_t e = 0; e < count; ++e) g.v[e] = dy[c + e];
+#pragma unroll
+        for (int r = 0; r < kRowsAhead; ++r) {
+          x[r] = Quad<T>{};
+          if (slot[r] < 0 || !a.weights_gradient) continue;
+          const T* from = static_cast<const T*>(a.rows) + slot[r] * a.rows_colstride + c;
+          if (a.width >= N) x[r] = load_quad<kStreaming>(from);
+          else
+            for (uint32_t e = 0; e < count; ++e) x[r].v[e] = from[e];
+        }
+        const bool whole = place + N <= a.width;
+#pragma unroll
+        for (int r = 0; r < kRowsAhead; ++r) {
+          if (slot[r] < 0) continue;
+          if (a.output) {
+            T* to = static_cast<T*>(a.output) + slot[r] * a.output_colstride;
+            Quad<T> q;
+#pragma unroll
+            for (uint32_t e = 0; e < N; ++e) q.v[e] = w[r] * g.v[e];
+            if (whole) store_quad<kStreaming>(to + place, q);
+            else {
+#pragma unroll
+              for (uint32_t e = 0; e < N; ++e)
+                if (e < count && c + e >= place) to[c + e] = q.v[e];
+            }
+          }
+#pragma unroll
+          for (uint32_t e = 0; e < N; ++e) dot[r] += c + e >= place ? g.v[e] * x[r].v[e] : T(0);
+        }
+      }
+      if (!a.weights_gradient) continue;
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1)
+#pragma unroll
+        for (int r = 0; r < kRowsAhead; ++r) dot[r] += __shfl_xor(dot[r], m);
+      T* to = static_cast<T*>(a.weights_gradient) + first + j0;
+      const uint32_t j = threadIdx.x & 63;
+      if constexpr (WAVES == 1) {
+#pragma unroll
+        for (int r = 0; r < kRowsAhead; ++r)
+          if (mine && j == (uint32_t)r && j0 + r < a.n_chosen) to[r] = dot[r];
+      } else {
+        if (j == 0) {
+#pragma unroll
+          for (int r = 0; r < kRowsAhead; ++r) lds[turn][wave][r] = dot[r];
+        }
+        __syncthreads();
+        if (mine && wave % WAVES == 0 && j < kRowsAhead && j0 + j < a.n_chosen) {
+          T sum = lds[turn][wave][j];
+#pragma unroll
+          for (int v = 1; v < WAVES; ++v) sum += lds[turn][wave + v][j];
+          to[j] = sum;
+        }
+        turn ^= 1;   // written again only after another barrier
+      }
+    }
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) combine_gradient_kernel(const CombineArgs a) {
-  __shared__ T lds[4];
-  const T* rows = static_cast<const T*>(a.rows);
-  for (uint32_t token = blockIdx.x; token < a.n; token += gridDim.x) {
-  const T* dy = static_cast<const T*>(a.output_gradient) + (int64_t)token * a.gradient_colstride;
-  for (uint32_t j = 0; j < a.n_chosen; ++j) {
-    const int64_t at = (int64_t)token * a.n_chosen + j;
-    const int64_t slot = a.slots[at];
-    const bool in = slot >= 0 && slot < a.row_count;
-    T dot = 0;
-    if (in) {
-      const T w = a.weights ? static_cast<const T*>(a.weights)[at] : T(1);
-      T* to = static_cast<T*>(a.output) + slot * a.output_colstride;
-      const T* row = rows + slot * a.rows_colstride;
-      for (uint32_t c = threadIdx.x; c < a.width; c += 256) {
-        const T g = dy[c];
-        if (a.output) to[c] = w * g;
-        if (a.weights_gradient) dot += g * row[c];
-      }
-    }
-    if (a.weights_gradient) {
-#pragma unroll
-      for (int m = 32; m > 0; m >>= 1) dot += __shfl_xor(dot, m);
-      if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) static_cast<T*>(a.weights_gradient)[at] = lds[0] + lds[1] + lds[2] + lds[3];
-      __syncthreads();
-    }
-  }
-  }
+void combine_launch(hipStream_t s, const CombineArgs& a) {
+  constexpr int64_t kWaves = kCombineBlock / 64;
+  const uint32_t parts = (a.width + 64 * Quad<T>::N - 1) / (64 * Quad<T>::N);
+  const int64_t blocks = std::min<int64_t>(((int64_t)a.n * parts + kWaves - 1) / kWaves, kMostBlocks);
+  const bool past = (int64_t)a.n * (a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
+  if (past) hipLaunchKernelGGL((combine_kernel<T, true>), dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a, parts, FastDiv(parts));
+  else hipLaunchKernelGGL((combine_kernel<T, false>), dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a, parts, FastDiv(parts));
+}
+
+template <class T>
+void combine_gradient_launch(hipStream_t s, const CombineArgs& a) {
+  const bool past = (int64_t)a.n * (2 * a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
+  // a wave to a token, four where that leaves compute units without work
+  const bool few = a.n < 4096 && a.width > 256;
+  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, kMostBlocks);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a); };
+  if (few && past) launch(combine_gradient_kernel<T, 4, true>);
+  else if (few) launch(combine_gradient_kernel<T, 4, false>);
+  else if (past) launch(combine_gradient_kernel<T, 1, true>);
+  else launch(combine_gradient_kernel<T, 1, false>);
 }
 
 constexpr int64_t kMostRows = (int64_t(1) << 31) - 1;
@@ -448,8 +561,8 @@ int ct_combine_experts(void* stream, void* output, int64_t output_colstride, con
   a.output = output; a.rows = rows; a.weights = weights; a.slots = slots;
   a.output_colstride = output_colstride; a.rows_colstride = rows_colstride; a.row_count = row_count;
   a.n = (uint32_t)n; a.n_chosen = (uint32_t)n_chosen; a.width = (uint32_t)width;
-  if (dtype == CT_F32) hipLaunchKernelGGL((combine_kernel<float>), dim3((uint32_t)std::min(n, kMostBlocks)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((combine_kernel<double>), dim3((uint32_t)std::min(n, kMostBlocks)), dim3(256), 0, s, a);
+  if (dtype == CT_F32) combine_launch<float>(s, a);
+  else combine_launch<double>(s, a);
   note_kernel("combine");
   return after_launch(s);
 }
@@ -481,8 +594,8 @@ int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_
   a.output_colstride = rows_gradient_colstride; a.gradient_colstride = output_gradient_colstride; a.rows_colstride = rows_colstride;
   a.row_count = row_count;
   a.n = (uint32_t)n; a.n_chosen = (uint32_t)n_chosen; a.width = (uint32_t)width;
-  if (dtype == CT_F32) hipLaunchKernelGGL((combine_gradient_kernel<float>), dim3((uint32_t)std::min(n, kMostBlocks)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((combine_gradient_kernel<double>), dim3((uint32_t)std::min(n, kMostBlocks)), dim3(256), 0, s, a);
+  if (dtype == CT_F32) combine_gradient_launch<float>(s, a);
+  else combine_gradient_launch<double>(s, a);
   note_kernel("combine_gradient");
   return after_launch(s);
 }

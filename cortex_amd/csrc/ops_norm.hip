@@ -22,6 +22,8 @@ using namespace cthip;
 namespace {
 
 constexpr int kNormBlock = 256;
+// Lanes of a block: rows of a wave or less share one, others have one to themselves.
+constexpr int block_of(int lanes) { return lanes > 64 ? lanes : kNormBlock; }
 
 enum GateKind { kNoGate, kScalarGate, kColumnGate, kRowGate, kFullGate };
 
@@ -109,8 +111,8 @@ __device__ __forceinline__ void row_sum(T (&v)[K], T* lds, int& turn) {
 template <class T> __device__ __forceinline__ T rate_of(T mean_square, T epsilon) { return T(1) / (T)sqrt(mean_square + epsilon); }
 
 template <class T, int LANES, int VPT, bool kStreaming>
-__global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_kernel(const NormArgs a) {
-  constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
+__global__ void __launch_bounds__(block_of(LANES)) norm_kernel(const NormArgs a) {
+  constexpr int kThreads = block_of(LANES), kRows = kThreads / LANES;
   using R = Row<T, LANES, VPT, kStreaming>;
   constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
@@ -206,8 +208,8 @@ __device__ __forceinline__ bool common_gate(int kind) { return kind == kNoGate |
 // next row's operands are loaded into the registers of this one's as those are used up.
 // kSums: 0 none, 1 S1 and T1, 2 all.  An absent gradient of the results is read from `input` and not used.
 template <class T, int LANES, int VPT, int kSums, bool kStreaming>
-__global__ void __launch_bounds__(LANES > kNormBlock ? LANES : kNormBlock) norm_gradient_kernel(const NormGradientArgs a) {
-  constexpr int kThreads = LANES > kNormBlock ? LANES : kNormBlock, kRows = kThreads / LANES;
+__global__ void __launch_bounds__(block_of(LANES), VPT == 4 ? 3 : 4) norm_gradient_kernel(const NormGradientArgs a) {
+  constexpr int kThreads = block_of(LANES), kRows = kThreads / LANES;
   using R = Row<T, LANES, VPT, kStreaming>;
   constexpr int N = R::N;
   __shared__ T lds[LANES > 64 ? 2 * 3 * (LANES / 64) : 1];
@@ -645,6 +647,7 @@ bool with_shape(uint32_t width, F f) {
 }
 
 constexpr int64_t kMostNormBlocks = 1 << 20;
+constexpr int64_t kUnits = 256, kLdsOfAUnit = 160 << 10, kBytesAhead = 128 << 10;
 constexpr int64_t kMostSumLds = 128 << 10;   // of a block, for its sums
 constexpr int64_t kMostSumBytes = int64_t(32) << 20;
 
@@ -654,7 +657,7 @@ bool streaming(int64_t rows, int64_t width, int64_t matrices, int64_t size) { re
 template <class T>
 int norm_typed(hipStream_t s, const NormArgs& a) {
   const bool taken = with_shape<T>(a.width, [&](auto lanes, auto pieces) {
-    constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
+    constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = block_of(L), kRows = kThreads / L;
     const int64_t blocks = std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
     if (streaming(a.rows, a.width, 3 + (a.pre != CT_NORM_NONE), sizeof(T)))
       hipLaunchKernelGGL((norm_kernel<T, L, V, true>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, a);
@@ -665,36 +668,48 @@ int norm_typed(hipStream_t s, const NormArgs& a) {
   return after_launch(s);
 }
 
+// Blocks to a compute unit whose operands are on their way at the same time: 128 KiB in all.  (16384 x 2048 floats, three, four
+// and five blocks of 256 lanes: 157, 151 and 163 us; 8192 x 4096, two, three and four: 150, 155 and 177; more blocks also leave more sums.)
+int64_t blocks_of_a_unit(int64_t bytes_of_a_block, int waves, int pieces) {
+  const int64_t of_registers = (pieces == 4 ? 12 : pieces == 2 ? 16 : 24) / waves;
+  return std::max<int64_t>(1, std::min(kBytesAhead / bytes_of_a_block, of_registers));
+}
+
 template <class T>
 int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
   const int slots = std::max({a.slot[0], a.slot[1], a.slot[2], a.slot[3]}) + 1;
   const bool sums = slots > 0, biases = a.slot[1] >= 0 || a.slot[3] >= 0;
   a.slots = slots;
-  int64_t rows_a_block = 1;
-  bool fits = with_shape<T>(a.width, [&](auto lanes, auto) { rows_a_block = std::max(1, kNormBlock / decltype(lanes)::value); });
-  fits = fits && (int64_t)slots * a.width * (int64_t)sizeof(T) <= kMostSumLds;
-  // whose sums the last launch adds
-  const int64_t most_blocks = std::max<int64_t>(1, std::min<int64_t>(512, kMostSumBytes / ((int64_t)std::max(slots, 1) * a.width * (int64_t)sizeof(T))));
-  a.blocks = f.blocks = (uint32_t)std::min((a.rows + rows_a_block - 1) / rows_a_block, most_blocks);
-  const size_t of_sums = (size_t)slots * a.blocks * a.width * sizeof(T), of_columns = (size_t)a.width * sizeof(double);
-  const size_t of_means = fits ? 0 : (size_t)4 * a.rows * sizeof(double);
-  void* scratch = nullptr;
-  if (int rc = stream_scratch(s, of_columns + of_means + of_sums, &scratch)) return rc;
-  double* by_column = static_cast<double*>(scratch);
-  double* means = by_column + a.width;
-  a.partial = means + (fits ? 0 : 4 * a.rows);
-  f.partial = a.partial;
-  if (f.by_column) f.by_column = by_column;
+  const bool fits = with_shape<T>(a.width, [](auto, auto) {}) && (int64_t)slots * a.width * (int64_t)sizeof(T) <= kMostSumLds;
+  const size_t of_columns = (size_t)a.width * sizeof(double), of_means = fits ? 0 : (size_t)4 * a.rows * sizeof(double);
+  double *by_column = nullptr, *means = nullptr;
+  // Scratch for the sums of `blocks` blocks, which the last launch adds.
+  auto with_sums_of = [&](int64_t blocks) {
+    a.blocks = f.blocks = (uint32_t)blocks;
+    void* scratch = nullptr;
+    if (int rc = stream_scratch(s, of_columns + of_means + (size_t)slots * blocks * a.width * sizeof(T), &scratch)) return rc;
+    by_column = static_cast<double*>(scratch);
+    means = by_column + a.width;
+    a.partial = means + (fits ? 0 : 4 * a.rows);
+    f.partial = a.partial;
+    return (int)CT_OK;
+  };
+  const int64_t most_blocks = std::max<int64_t>(1, kMostSumBytes / ((int64_t)std::max(slots, 1) * a.width * (int64_t)sizeof(T)));
+  int rc = CT_OK;
   if (a.rows == 0) {
-    // sums of no rows
+    rc = with_sums_of(0);
   } else if (fits) {
     with_shape<T>(a.width, [&](auto lanes, auto pieces) {
-      constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = std::max(L, kNormBlock), kRows = kThreads / L;
-      const int64_t blocks = sums ? a.blocks : std::min((a.rows + kRows - 1) / kRows, kMostNormBlocks);
+      constexpr int L = decltype(lanes)::value, V = decltype(pieces)::value, kThreads = block_of(L), kRows = kThreads / L;
       const size_t lds = (size_t)slots * kRows * ((a.width + Quad<T>::N - 1) / Quad<T>::N) * sizeof(Quad<T>);
       auto launch = [&](auto kernel) {
+        // each block of as many rows as the others
+        const int64_t ahead = (int64_t)4 * kRows * a.width * sizeof(T), of_lds = lds ? std::max<int64_t>(1, kLdsOfAUnit / (int64_t)(lds + 1024)) : 32;
+        const int64_t at_once = kUnits * std::min(blocks_of_a_unit(ahead, kThreads / 64, V), of_lds), groups = (a.rows + kRows - 1) / kRows;
+        const int64_t turns = (groups + at_once - 1) / at_once;
+        if ((rc = with_sums_of(std::min((groups + turns - 1) / turns, most_blocks)))) return;
         if (lds > (48 << 10)) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kThreads), lds, s, a);
+        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), lds, s, a);
       };
       const bool past = streaming(a.rows, a.width, 6, sizeof(T));
       if (biases && past) launch(norm_gradient_kernel<T, L, V, 2, true>);
@@ -704,12 +719,14 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
       else if (past) launch(norm_gradient_kernel<T, L, V, 0, true>);
       else launch(norm_gradient_kernel<T, L, V, 0, false>);
     });
-  } else {
+  } else if (!(rc = with_sums_of(std::min<int64_t>({a.rows, most_blocks, 512})))) {
     const uint32_t columns = (a.width + 255) / 256;
     hipLaunchKernelGGL((norm_long_means_kernel<T>), dim3((uint32_t)std::min(a.rows, kMostNormBlocks)), dim3(kLongBlock), 0, s, a, means);
     if (sums) hipLaunchKernelGGL((norm_long_sums_kernel<T>), dim3(columns, a.blocks), dim3(256), 0, s, a, means);
     hipLaunchKernelGGL((norm_long_apply_kernel<T>), dim3(columns, (uint32_t)std::min<int64_t>(a.rows, 4096)), dim3(256), 0, s, a, means);
   }
+  if (rc) return rc;
+  if (f.by_column) f.by_column = by_column;
   if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 31) / 32, 2), dim3(1024), 0, s, f);
   if (f.by_column) hipLaunchKernelGGL((norm_scalar_gate_kernel<T>), dim3(1), dim3(256), 0, s, by_column, a.width, static_cast<T*>(f.gate_gradient));
   note_kernel(fits ? "norm_residual_gradient" : "norm_residual_gradient_long");
