@@ -319,140 +319,189 @@ struct CombineArgs {
 };
 
 constexpr int kCombineBlock = 256;
-constexpr int kRowsAhead = 4;   // of a token, whose loads are on their way together
 
-// A wave to a part of a token's row: 16 bytes to a lane, kRowsAhead rows of the token at a time.  A lane that would pass the end of the
-// row takes its last 16 bytes and stores what lies behind its place.
-template <class T, bool kStreaming>
-__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const CombineArgs a, uint32_t parts, FastDiv parts_fd) {
-  constexpr uint32_t N = Quad<T>::N;
-  const uint32_t lane = threadIdx.x & 63, waves = gridDim.x * (kCombineBlock / 64);
-  const T* rows = static_cast<const T*>(a.rows);
-  const T* weights = static_cast<const T*>(a.weights);
-  for (uint64_t unit = (blockIdx.x * kCombineBlock + threadIdx.x) >> 6; unit < (uint64_t)a.n * parts; unit += waves) {
-    uint32_t token, part;
-    if (parts == 1) token = (uint32_t)unit, part = 0;
-    else if (unit < (uint64_t(1) << 31)) parts_fd.divmod((uint32_t)unit, token, part);
-    else token = (uint32_t)(unit / parts), part = (uint32_t)(unit % parts);
-    const uint32_t place = (part * 64 + lane) * N;
-    if (place >= a.width) continue;
-    const uint32_t c = a.width >= N ? min(place, a.width - N) : 0, count = min(N, a.width);
-    const int64_t first = (int64_t)token * a.n_chosen;
-    Quad<T> sum = {};
-    for (uint32_t j0 = 0; j0 < a.n_chosen; j0 += kRowsAhead) {
-      Quad<T> x[kRowsAhead];
-      T w[kRowsAhead];
-#pragma unroll
-      for (int r = 0; r < kRowsAhead; ++r) {
-        const uint32_t j = min(j0 + r, a.n_chosen - 1);
-        const int64_t slot = a.slots[first + j];
-        const bool in = j0 + r < a.n_chosen && slot >= 0 && slot < a.row_count;
-        w[r] = !in ? T(0) : weights ? weights[first + j] : T(1);
-        x[r] = Quad<T>{};
-        if (!in) continue;
-        const T* from = rows + slot * a.rows_colstride + c;
-        if (a.width >= N) x[r] = load_quad<kStreaming>(from);
-        else
-          for (uint32_t e = 0; e < count; ++e) x[r].v[e] = from[e];
-      }
-#pragma unroll
-      for (int r = 0; r < kRowsAhead; ++r)
-#pragma unroll
-        for (uint32_t e = 0; e < N; ++e) sum.v[e] += w[r] * x[r].v[e];
-    }
-    T* out = static_cast<T*>(a.output) + (int64_t)token * a.output_colstride;
-    if (place + N <= a.width) store_quad<kStreaming>(out + place, sum);
-    else {
-#pragma unroll
-      for (uint32_t e = 0; e < N; ++e)
-        if (e < count && c + e >= place) out[c + e] = sum.v[e];
-    }
+template <class T> __device__ __forceinline__ T from_lane(T x, uint32_t lane) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+  } else {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint64_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, lane);
+    return __builtin_bit_cast(T, low | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane) << 32);
   }
 }
 
-// WAVES waves to a token, and its rows kRowsAhead at a time: its gradient is read again from the caches for every such lot.
+// 16 bytes of a row to a lane: the ones at its place, or the row's last ones if those would pass its end; rows shorter than
+// that element by element.
+template <class T>
+struct RowPart {
+  static constexpr uint32_t N = Quad<T>::N;
+  uint32_t place, start, width;
+  __device__ __forceinline__ RowPart(uint32_t place, uint32_t width) : place(place), start(width >= N ? min(place, width - N) : 0), width(width) {}
+  __device__ __forceinline__ bool owns(uint32_t e) const { return start + e >= place && (width >= N || e < width); }
+  template <bool kStreaming> __device__ __forceinline__ Quad<T> load(const T* row) const {
+    if (width >= N) return load_quad<kStreaming>(row + start);
+    Quad<T> q;
+#pragma unroll
+    for (uint32_t e = 0; e < N; ++e) q.v[e] = row[min(e, width - 1)];
+    return q;
+  }
+  template <bool kStreaming> __device__ __forceinline__ void store(T* row, const Quad<T>& q) const {
+    if (place + N <= width) {
+      store_quad<kStreaming>(row + place, q);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < N; ++e)
+        if (owns(e)) row[start + e] = q.v[e];
+    }
+  }
+};
+
+// A wave to a run of tokens and 64 x 16 bytes of their rows.  The slots and weights of up to 64 assignments are one load of the
+// wave's, and the rows of kRowsAhead assignments are on their way together, whichever tokens they are of: waves that took a
+// token each spent their time on two loads, one behind the other (65536 tokens of one row of 1 KiB 42 us).
+constexpr int kRowsAhead = 8;
+
+template <class T, bool kStreaming>
+__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const CombineArgs a, uint32_t parts, uint32_t run, uint32_t units) {
+  const uint32_t lane = threadIdx.x & 63, unit = __builtin_amdgcn_readfirstlane((blockIdx.x * kCombineBlock + threadIdx.x) >> 6);
+  if (unit >= units) return;
+  const uint32_t runs = unit / parts, part = unit - runs * parts, k = a.n_chosen;
+  const RowPart<T> at((part * 64 + lane) * Quad<T>::N, a.width);
+  const T* rows = static_cast<const T*>(a.rows);
+  T* out = static_cast<T*>(a.output);
+  const uint64_t begin = (uint64_t)runs * run;
+  const uint32_t tokens = (uint32_t)min((uint64_t)run, a.n - begin);
+  Quad<T> sum = {};
+  for (uint32_t t0 = 0; t0 < tokens;) {
+    const uint32_t now = min(64 / k, tokens - t0), count = now * k;   // tokens, assignments
+    const int64_t first = (int64_t)(begin + t0) * k;
+    const int64_t mine = first + min(lane, count - 1);
+    const int32_t slot = a.slots[mine];
+    const T weight = a.weights ? static_cast<const T*>(a.weights)[mine] : T(1);
+    uint32_t left = k, token = t0;
+    for (uint32_t i0 = 0; i0 < count; i0 += kRowsAhead) {
+      Quad<T> x[kRowsAhead];
+      bool in[kRowsAhead];
+#pragma unroll
+      for (uint32_t r = 0; r < kRowsAhead; ++r) {
+        const int32_t of = __builtin_amdgcn_readlane(slot, min(i0 + r, count - 1));
+        in[r] = i0 + r < count && of >= 0 && of < a.row_count;
+        if (in[r]) x[r] = at.template load<kStreaming>(rows + (int64_t)of * a.rows_colstride);
+      }
+#pragma unroll
+      for (uint32_t r = 0; r < kRowsAhead; ++r) {
+        if (i0 + r >= count) break;
+        if (in[r]) {
+          const T w = from_lane(weight, i0 + r);
+#pragma unroll
+          for (uint32_t e = 0; e < Quad<T>::N; ++e) sum.v[e] += w * x[r].v[e];
+        }
+        if (--left == 0) {
+          if (at.place < a.width) at.template store<kStreaming>(out + (int64_t)(begin + token) * a.output_colstride, sum);
+          sum = Quad<T>{};
+          left = k;
+          ++token;
+        }
+      }
+    }
+    t0 += now;
+  }
+}
+
+// WAVES waves to a token, whose rows are taken kRowsOfAToken at a time; the next piece of each is on its way while one is used, and the
+// next token's slots while a token is.  The token's gradient is read again, from the caches, for every such lot.
+constexpr int kRowsOfAToken = 4;
+
 template <class T, int WAVES, bool kStreaming>
 __global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const CombineArgs a) {
-  constexpr uint32_t N = Quad<T>::N;
+  constexpr uint32_t N = Quad<T>::N, R = kRowsOfAToken;
   constexpr int kTokens = kCombineBlock / 64 / WAVES;
-  __shared__ T lds[2][kCombineBlock / 64][kRowsAhead];
+  __shared__ T lds[2][kCombineBlock / 64][R];
   int turn = 0;
-  const uint32_t wave = threadIdx.x >> 6, of_token = threadIdx.x % (64 * WAVES), stride = 64 * WAVES * N;
-  const T* weights = static_cast<const T*>(a.weights);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = a.n_chosen;
+  const uint32_t of_token = threadIdx.x % (64 * WAVES), stride = 64 * WAVES * N, pieces = (a.width + stride - 1) / stride;
+  const bool dots = a.weights_gradient != nullptr;
   // all of a block's waves go on together: a token beyond the last one is the last one, and not stored
+  int32_t next_slot;
+  T next_weight;
+  auto look_up = [&](uint32_t token) {
+    const int64_t at = (int64_t)min(token, a.n - 1) * k + min(lane, k - 1);
+    next_slot = a.slots[at];
+    next_weight = a.weights ? static_cast<const T*>(a.weights)[at] : T(1);
+  };
+  look_up(blockIdx.x * kTokens + wave / WAVES);
   for (uint32_t t0 = blockIdx.x * kTokens; t0 < a.n; t0 += gridDim.x * kTokens) {
-    const uint32_t token = min(t0 + wave / WAVES, a.n - 1);
     const bool mine = t0 + wave / WAVES < a.n;
-    const int64_t first = (int64_t)token * a.n_chosen;
+    const uint32_t token = min(t0 + wave / WAVES, a.n - 1);
+    const int32_t slots = next_slot;
+    const T weights = next_weight;
+    look_up(t0 + gridDim.x * kTokens + wave / WAVES);
     const T* dy = static_cast<const T*>(a.output_gradient) + (int64_t)token * a.gradient_colstride;
-    for (uint32_t j0 = 0; j0 < a.n_chosen; j0 += kRowsAhead) {
-      T dot[kRowsAhead], w[kRowsAhead];
-      int64_t slot[kRowsAhead];
+    for (uint32_t j0 = 0; j0 < k; j0 += R) {
+      T dot[R], w[R];
+      bool in[R];
+      const T* row[R];
+      T* to[R];
 #pragma unroll
-      for (int r = 0; r < kRowsAhead; ++r) {
-        const uint32_t j = min(j0 + r, a.n_chosen - 1);
-        slot[r] = a.slots[first + j];
-        if (!mine || j0 + r >= a.n_chosen || slot[r] < 0 || slot[r] >= a.row_count) slot[r] = -1;
-        w[r] = weights ? weights[first + j] : T(1);
+      for (uint32_t r = 0; r < R; ++r) {
+        const uint32_t j = min(j0 + r, k - 1);
+        const int32_t slot = __builtin_amdgcn_readlane(slots, j);
+        in[r] = mine && j0 + r < k && slot >= 0 && slot < a.row_count;
+        w[r] = from_lane(weights, j);
         dot[r] = 0;
+        // one that is not used reads the gradient in its place
+        row[r] = in[r] && dots ? static_cast<const T*>(a.rows) + (int64_t)slot * a.rows_colstride : dy;
+        to[r] = static_cast<T*>(a.output) + (int64_t)(in[r] ? slot : 0) * a.output_colstride;
       }
-      for (uint32_t place = of_token * N; place < a.width; place += stride) {
-        const uint32_t c = a.width >= N ? min(place, a.width - N) : 0, count = min(N, a.width);
-        Quad<T> g = {}, x[kRowsAhead];
-        if (a.width >= N) g = load_quad(dy + c);
-        else
-          for (uint32_t e = 0; e < count; ++e) g.v[e] = dy[c + e];
+      Quad<T> g, x[R], g_next, x_next[R];
+      auto load = [&](uint32_t piece, Quad<T>& g, Quad<T> (&x)[R]) {
+        const RowPart<T> at(min(of_token * N + piece * stride, a.width), a.width);
+        g = at.template load<false>(dy);
 #pragma unroll
-        for (int r = 0; r < kRowsAhead; ++r) {
-          x[r] = Quad<T>{};
-          if (slot[r] < 0 || !a.weights_gradient) continue;
-          const T* from = static_cast<const T*>(a.rows) + slot[r] * a.rows_colstride + c;
-          if (a.width >= N) x[r] = load_quad<kStreaming>(from);
-          else
-            for (uint32_t e = 0; e < count; ++e) x[r].v[e] = from[e];
-        }
-        const bool whole = place + N <= a.width;
+        for (uint32_t r = 0; r < R; ++r) x[r] = at.template load<kStreaming>(row[r]);
+      };
+      if (pieces) load(0, g, x);
+      for (uint32_t piece = 0; piece < pieces; ++piece) {
+        load(piece + 1, g_next, x_next);
+        const RowPart<T> at(of_token * N + piece * stride, a.width);
+        const bool some = at.place < a.width;
 #pragma unroll
-        for (int r = 0; r < kRowsAhead; ++r) {
-          if (slot[r] < 0) continue;
-          if (a.output) {
-            T* to = static_cast<T*>(a.output) + slot[r] * a.output_colstride;
+        for (uint32_t r = 0; r < R; ++r) {
+          if (a.output && in[r] && some) {
             Quad<T> q;
 #pragma unroll
             for (uint32_t e = 0; e < N; ++e) q.v[e] = w[r] * g.v[e];
-            if (whole) store_quad<kStreaming>(to + place, q);
-            else {
-#pragma unroll
-              for (uint32_t e = 0; e < N; ++e)
-                if (e < count && c + e >= place) to[c + e] = q.v[e];
-            }
+            at.template store<kStreaming>(to[r], q);
           }
 #pragma unroll
-          for (uint32_t e = 0; e < N; ++e) dot[r] += c + e >= place ? g.v[e] * x[r].v[e] : T(0);
+          for (uint32_t e = 0; e < N; ++e) dot[r] += at.owns(e) ? g.v[e] * x[r].v[e] : T(0);
+          x[r] = x_next[r];
         }
+        g = g_next;
       }
-      if (!a.weights_gradient) continue;
+      if (!dots) continue;
 #pragma unroll
       for (int m = 32; m > 0; m >>= 1)
 #pragma unroll
-        for (int r = 0; r < kRowsAhead; ++r) dot[r] += __shfl_xor(dot[r], m);
-      T* to = static_cast<T*>(a.weights_gradient) + first + j0;
-      const uint32_t j = threadIdx.x & 63;
+        for (uint32_t r = 0; r < R; ++r) dot[r] += __shfl_xor(dot[r], m);
+#pragma unroll
+      for (uint32_t r = 0; r < R; ++r) dot[r] = in[r] ? dot[r] : T(0);
+      T* result = static_cast<T*>(a.weights_gradient) + (int64_t)token * k + j0;
       if constexpr (WAVES == 1) {
 #pragma unroll
-        for (int r = 0; r < kRowsAhead; ++r)
-          if (mine && j == (uint32_t)r && j0 + r < a.n_chosen) to[r] = dot[r];
+        for (uint32_t r = 0; r < R; ++r)
+          if (mine && lane == r && j0 + r < k) result[r] = dot[r];
       } else {
-        if (j == 0) {
+        if (lane == 0) {
 #pragma unroll
-          for (int r = 0; r < kRowsAhead; ++r) lds[turn][wave][r] = dot[r];
+          for (uint32_t r = 0; r < R; ++r) lds[turn][wave][r] = dot[r];
         }
         __syncthreads();
-        if (mine && wave % WAVES == 0 && j < kRowsAhead && j0 + j < a.n_chosen) {
-          T sum = lds[turn][wave][j];
+        if (mine && wave % WAVES == 0 && lane < R && j0 + lane < k) {
+          T sum = lds[turn][wave][lane];
 #pragma unroll
-          for (int v = 1; v < WAVES; ++v) sum += lds[turn][wave + v][j];
-          to[j] = sum;
+          for (int v = 1; v < WAVES; ++v) sum += lds[turn][wave + v][lane];
+          result[lane] = sum;
         }
         turn ^= 1;   // written again only after another barrier
       }
@@ -460,14 +509,19 @@ __global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const C
   }
 }
 
+constexpr int64_t kWavesOfTheChip = 256 * 32;
+
 template <class T>
 void combine_launch(hipStream_t s, const CombineArgs& a) {
-  constexpr int64_t kWaves = kCombineBlock / 64;
-  const uint32_t parts = (a.width + 64 * Quad<T>::N - 1) / (64 * Quad<T>::N);
-  const int64_t blocks = std::min<int64_t>(((int64_t)a.n * parts + kWaves - 1) / kWaves, kMostBlocks);
+  const int64_t parts = (a.width + 64 * Quad<T>::N - 1) / (64 * Quad<T>::N);
+  // tokens to a wave: no more than leave a wave to every place there is for one, unless there are more waves than a launch takes
+  int64_t run = std::max<int64_t>(1, std::min<int64_t>((int64_t)a.n * parts / kWavesOfTheChip, 64 / a.n_chosen));
+  run = std::max(run, ((int64_t)a.n * parts + kMostBlocks - 1) / kMostBlocks);
+  const int64_t units = (a.n + run - 1) / run * parts;
+  const dim3 grid((uint32_t)((units + kCombineBlock / 64 - 1) / (kCombineBlock / 64)));
   const bool past = (int64_t)a.n * (a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
-  if (past) hipLaunchKernelGGL((combine_kernel<T, true>), dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a, parts, FastDiv(parts));
-  else hipLaunchKernelGGL((combine_kernel<T, false>), dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a, parts, FastDiv(parts));
+  if (past) hipLaunchKernelGGL((combine_kernel<T, true>), grid, dim3(kCombineBlock), 0, s, a, (uint32_t)parts, (uint32_t)run, (uint32_t)units);
+  else hipLaunchKernelGGL((combine_kernel<T, false>), grid, dim3(kCombineBlock), 0, s, a, (uint32_t)parts, (uint32_t)run, (uint32_t)units);
 }
 
 template <class T>
@@ -475,7 +529,7 @@ void combine_gradient_launch(hipStream_t s, const CombineArgs& a) {
   const bool past = (int64_t)a.n * (2 * a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
   // a wave to a token, four where that leaves compute units without work
   const bool few = a.n < 4096 && a.width > 256;
-  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, kMostBlocks);
+  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, few ? kMostBlocks : 2048);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a); };
   if (few && past) launch(combine_gradient_kernel<T, 4, true>);
   else if (few) launch(combine_gradient_kernel<T, 4, false>);
