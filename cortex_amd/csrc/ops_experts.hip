@@ -408,96 +408,118 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const CombineArg
   }
 }
 
-// WAVES waves to a token, whose rows are taken kRowsOfAToken at a time; the next piece of each is on its way while one is used, and the
-// next token's slots while a token is.  The token's gradient is read again, from the caches, for every such lot.
-constexpr int kRowsOfAToken = 4;
-
-template <class T, int WAVES, bool kStreaming>
+// WAVES waves to a token, whose rows are taken R at a time, a lot.  What a wave uses next is on its way while it uses
+// a piece: the lot's next piece, or the first one of the next lot or token.  The token's gradient is read again, from the caches,
+// for every lot.
+template <class T, int WAVES, int R, bool kStreaming>
 __global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const CombineArgs a) {
-  constexpr uint32_t N = Quad<T>::N, R = kRowsOfAToken;
-  constexpr int kTokens = kCombineBlock / 64 / WAVES;
+  constexpr uint32_t N = Quad<T>::N, kTokens = kCombineBlock / 64 / WAVES;
   __shared__ T lds[2][kCombineBlock / 64][R];
   int turn = 0;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = a.n_chosen;
   const uint32_t of_token = threadIdx.x % (64 * WAVES), stride = 64 * WAVES * N, pieces = (a.width + stride - 1) / stride;
   const bool dots = a.weights_gradient != nullptr;
-  // all of a block's waves go on together: a token beyond the last one is the last one, and not stored
-  int32_t next_slot;
-  T next_weight;
+  struct Lot {
+    uint32_t token, j0;   // a token beyond the last one is read as that, and not stored: a block's waves go on together
+    const T* dy;
+    const T* row[R];
+    int32_t slot[R];      // negative: not used
+    T weight[R];
+  };
+  int32_t slots = 0, slots_ahead;   // of the lot's token and the next one, an assignment to a lane
+  T weights = T(0), weights_ahead;
   auto look_up = [&](uint32_t token) {
     const int64_t at = (int64_t)min(token, a.n - 1) * k + min(lane, k - 1);
-    next_slot = a.slots[at];
-    next_weight = a.weights ? static_cast<const T*>(a.weights)[at] : T(1);
+    slots_ahead = a.slots[at];
+    weights_ahead = a.weights ? static_cast<const T*>(a.weights)[at] : T(1);
   };
-  look_up(blockIdx.x * kTokens + wave / WAVES);
-  for (uint32_t t0 = blockIdx.x * kTokens; t0 < a.n; t0 += gridDim.x * kTokens) {
-    const bool mine = t0 + wave / WAVES < a.n;
-    const uint32_t token = min(t0 + wave / WAVES, a.n - 1);
-    const int32_t slots = next_slot;
-    const T weights = next_weight;
-    look_up(t0 + gridDim.x * kTokens + wave / WAVES);
-    const T* dy = static_cast<const T*>(a.output_gradient) + (int64_t)token * a.gradient_colstride;
-    for (uint32_t j0 = 0; j0 < k; j0 += R) {
-      T dot[R], w[R];
-      bool in[R];
-      const T* row[R];
-      T* to[R];
+  auto lot_of = [&](uint32_t token, uint32_t j0) {
+    Lot l;
+    l.token = token;
+    l.j0 = j0;
+    l.dy = static_cast<const T*>(a.output_gradient) + (int64_t)min(token, a.n - 1) * a.gradient_colstride;
 #pragma unroll
-      for (uint32_t r = 0; r < R; ++r) {
-        const uint32_t j = min(j0 + r, k - 1);
-        const int32_t slot = __builtin_amdgcn_readlane(slots, j);
-        in[r] = mine && j0 + r < k && slot >= 0 && slot < a.row_count;
-        w[r] = from_lane(weights, j);
-        dot[r] = 0;
-        // one that is not used reads the gradient in its place
-        row[r] = in[r] && dots ? static_cast<const T*>(a.rows) + (int64_t)slot * a.rows_colstride : dy;
-        to[r] = static_cast<T*>(a.output) + (int64_t)(in[r] ? slot : 0) * a.output_colstride;
-      }
-      Quad<T> g, x[R], g_next, x_next[R];
-      auto load = [&](uint32_t piece, Quad<T>& g, Quad<T> (&x)[R]) {
-        const RowPart<T> at(min(of_token * N + piece * stride, a.width), a.width);
-        g = at.template load<false>(dy);
+    for (int r = 0; r < R; ++r) {
+      const uint32_t j = min(j0 + r, k - 1u);
+      const int32_t slot = __builtin_amdgcn_readlane(slots, j);
+      const bool in = token < a.n && j0 + r < k && slot >= 0 && slot < a.row_count;
+      l.slot[r] = in ? slot : -1;
+      l.weight[r] = from_lane(weights, j);
+      // one that is not used reads the gradient in its place
+      l.row[r] = in && dots ? static_cast<const T*>(a.rows) + (int64_t)slot * a.rows_colstride : l.dy;
+    }
+    return l;
+  };
+  Quad<T> g, x[R], g_next, x_next[R];
+  auto load = [&](const Lot& l, uint32_t piece, Quad<T>& g, Quad<T> (&x)[R]) {
+    const RowPart<T> at(min(of_token * N + piece * stride, a.width), a.width);
+    g = at.template load<false>(l.dy);
 #pragma unroll
-        for (uint32_t r = 0; r < R; ++r) x[r] = at.template load<kStreaming>(row[r]);
-      };
-      if (pieces) load(0, g, x);
-      for (uint32_t piece = 0; piece < pieces; ++piece) {
-        load(piece + 1, g_next, x_next);
-        const RowPart<T> at(of_token * N + piece * stride, a.width);
-        const bool some = at.place < a.width;
-#pragma unroll
-        for (uint32_t r = 0; r < R; ++r) {
-          if (a.output && in[r] && some) {
-            Quad<T> q;
-#pragma unroll
-            for (uint32_t e = 0; e < N; ++e) q.v[e] = w[r] * g.v[e];
-            at.template store<kStreaming>(to[r], q);
-          }
-#pragma unroll
-          for (uint32_t e = 0; e < N; ++e) dot[r] += at.owns(e) ? g.v[e] * x[r].v[e] : T(0);
-          x[r] = x_next[r];
+    for (int r = 0; r < R; ++r) x[r] = at.template load<kStreaming>(l.row[r]);
+  };
+  const uint32_t step = gridDim.x * kTokens;
+  uint32_t first = blockIdx.x * kTokens;   // token of the block's first wave
+  auto next_token = [&] {
+    slots = slots_ahead;
+    weights = weights_ahead;
+    look_up(first + step + wave / WAVES);
+  };
+  look_up(first + wave / WAVES);
+  next_token();
+  Lot lot = lot_of(first + wave / WAVES, 0);
+  load(lot, 0, g, x);
+  while (first < a.n) {
+    T dot[R] = {};
+    Lot next = lot;
+    for (uint32_t piece = 0; piece < pieces; ++piece) {
+      uint32_t ahead = piece + 1;
+      if (ahead == pieces) {
+        ahead = 0;
+        if (lot.j0 + R < k) {
+          next = lot_of(lot.token, lot.j0 + R);
+        } else {
+          first += step;
+          next_token();
+          next = lot_of(first + wave / WAVES, 0);
         }
-        g = g_next;
       }
-      if (!dots) continue;
+      load(next, ahead, g_next, x_next);
+      const RowPart<T> at(of_token * N + piece * stride, a.width);
+      const bool some = at.place < a.width;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (a.output && lot.slot[r] >= 0 && some) {
+          Quad<T> q;
+#pragma unroll
+          for (uint32_t e = 0; e < N; ++e) q.v[e] = lot.weight[r] * g.v[e];
+          at.template store<kStreaming>(static_cast<T*>(a.output) + (int64_t)lot.slot[r] * a.output_colstride, q);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e) dot[r] += at.owns(e) ? g.v[e] * x[r].v[e] : T(0);
+        x[r] = x_next[r];
+      }
+      g = g_next;
+    }
+    if (dots) {
 #pragma unroll
       for (int m = 32; m > 0; m >>= 1)
 #pragma unroll
-        for (uint32_t r = 0; r < R; ++r) dot[r] += __shfl_xor(dot[r], m);
+        for (int r = 0; r < R; ++r) dot[r] += __shfl_xor(dot[r], m);
 #pragma unroll
-      for (uint32_t r = 0; r < R; ++r) dot[r] = in[r] ? dot[r] : T(0);
-      T* result = static_cast<T*>(a.weights_gradient) + (int64_t)token * k + j0;
+      for (int r = 0; r < R; ++r) dot[r] = lot.slot[r] >= 0 ? dot[r] : T(0);
+      T* result = static_cast<T*>(a.weights_gradient) + (int64_t)lot.token * k + lot.j0;
+      const bool stored = lot.token < a.n && lane < (uint32_t)R && lot.j0 + lane < k;
       if constexpr (WAVES == 1) {
 #pragma unroll
-        for (uint32_t r = 0; r < R; ++r)
-          if (mine && lane == r && j0 + r < k) result[r] = dot[r];
+        for (int r = 0; r < R; ++r)
+          if (stored && lane == (uint32_t)r) result[r] = dot[r];
       } else {
         if (lane == 0) {
 #pragma unroll
-          for (uint32_t r = 0; r < R; ++r) lds[turn][wave][r] = dot[r];
+          for (int r = 0; r < R; ++r) lds[turn][wave][r] = dot[r];
         }
         __syncthreads();
-        if (mine && wave % WAVES == 0 && lane < R && j0 + lane < k) {
+        if (stored && wave % WAVES == 0) {
           T sum = lds[turn][wave][lane];
 #pragma unroll
           for (int v = 1; v < WAVES; ++v) sum += lds[turn][wave + v][lane];
@@ -506,10 +528,12 @@ __global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const C
         turn ^= 1;   // written again only after another barrier
       }
     }
+    lot = next;
   }
 }
 
 constexpr int64_t kWavesOfTheChip = 256 * 32;
+constexpr int64_t kGradientBlocks = 256 * 4;   // that the chip holds
 
 template <class T>
 void combine_launch(hipStream_t s, const CombineArgs& a) {
@@ -529,12 +553,18 @@ void combine_gradient_launch(hipStream_t s, const CombineArgs& a) {
   const bool past = (int64_t)a.n * (2 * a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
   // a wave to a token, four where that leaves compute units without work
   const bool few = a.n < 4096 && a.width > 256;
-  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, few ? kMostBlocks : 2048);
+  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, few ? kMostBlocks : kGradientBlocks);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a); };
-  if (few && past) launch(combine_gradient_kernel<T, 4, true>);
-  else if (few) launch(combine_gradient_kernel<T, 4, false>);
-  else if (past) launch(combine_gradient_kernel<T, 1, true>);
-  else launch(combine_gradient_kernel<T, 1, false>);
+  auto of_rows = [&](auto rows) {
+    constexpr int R = decltype(rows)::value;
+    if (few && past) launch(combine_gradient_kernel<T, 4, R, true>);
+    else if (few) launch(combine_gradient_kernel<T, 4, R, false>);
+    else if (past) launch(combine_gradient_kernel<T, 1, R, true>);
+    else launch(combine_gradient_kernel<T, 1, R, false>);
+  };
+  if (a.n_chosen == 1) of_rows(std::integral_constant<int, 1>());
+  else if (a.n_chosen == 2) of_rows(std::integral_constant<int, 2>());
+  else of_rows(std::integral_constant<int, 4>());
 }
 
 constexpr int64_t kMostRows = (int64_t(1) << 31) - 1;
@@ -641,6 +671,7 @@ int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_
   CT_REQUIRE(!rows_meet(result, {output_gradient, n, width, output_gradient_colstride}, dtype_size(dtype)) &&
                  !rows_meet(result, {weights_gradient ? rows : nullptr, row_count, width, rows_colstride}, dtype_size(dtype)),
              "ct_combine_experts_gradient: rows_gradient overlaps an operand");
+  if (width == 0) return weights_gradient ? ct_memset(stream, weights_gradient, dtype, 0.0, n * n_chosen) : (int)CT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   CombineArgs a{};
   a.output = rows_gradient; a.weights_gradient = weights_gradient; a.output_gradient = output_gradient; a.rows = rows;

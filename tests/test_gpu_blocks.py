@@ -598,6 +598,15 @@ def test_combine_experts(D, size):
     assert np.array_equal(read(dw2), read(dw)) and np.array_equal(read(to2), read(to))
 
 
+def test_combine_of_rows_without_elements(D):
+    """Nothing to add up: the weights' gradient is zero, and nothing else is written."""
+    dw, ts = D.tensor(np.full((5, 2), 9.0)), D.tensor(np.arange(10).reshape(5, 2), "int")
+    empty = lambda n: D.tensor(np.zeros((n, 0)))
+    blocks.combine_experts(empty(5), empty(10), None, ts)
+    blocks.combine_experts_gradient(empty(10), dw, empty(5), empty(10), None, ts)
+    assert np.all(read(dw) == 0)
+
+
 # ------------------------------------------------------------------------------------------------- clipping
 
 @pytest.mark.parametrize("sizes", [[1], [3, 0, 5], [100352, 128, 1280, 10], [16384, 16385, 1, 32767, 40001], list(range(1, 260)),
