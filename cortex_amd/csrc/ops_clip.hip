@@ -3,9 +3,11 @@
 // norm = sqrt(sum over all tensors of g^2), factor = max_norm / max(norm, max_norm), out = g * factor.  Squares are formed and
 // summed in double: a float's square is exact there and no sum of floats overflows.
 //
-// Three launches: pieces of kPiece values sum their squares, one block adds the pieces' sums in their order, the pieces are
-// multiplied by the factor.  The tensors travel in the launch's arguments, kTensors to a launch: a table in device memory
-// would have to be copied there by every call.
+// The tensors are cut into pieces; a launch's blocks take every so manieth piece, form one sum of squares each, and the norm is
+// the sum of those in their order.  A few sums are added by every block that needs the factor, more by a launch of their own.
+// The pieces are multiplied by the factor last to first: what was read last is still in the last-level cache.
+// The tensors travel in the launch's arguments, kTensors to a launch: a table in device memory would have to be copied there
+// by every call.
 #include <algorithm>
 #include <cmath>
 
@@ -17,32 +19,47 @@ using namespace cthip;
 namespace {
 
 constexpr int kClipBlock = 256;
-constexpr int kPieceBytes = 64 << 10;
 constexpr int kTensors = 120;
+constexpr int64_t kMostClipBlocks = 2048;   // of a launch: what the chip holds
+constexpr int64_t kFewSums = 512;           // which every block adds by itself
+constexpr int64_t kLeastPiece = 4 << 10, kMostPiece = 64 << 10;   // bytes
+constexpr int64_t kClipCacheBytes = int64_t(256) << 20;
 
 struct ClipTable {
   const void* in[kTensors];
   void* out[kTensors];
   int64_t count[kTensors];
-  uint32_t first[kTensors];   // piece of the launch that begins a tensor
+  uint32_t first[kTensors + 1];   // piece of the launch that begins a tensor; all of them
   uint32_t tensors;
 };
 static_assert(sizeof(ClipTable) <= 3600, "with the other arguments within 4 KiB");
 
-// The tensor that a piece belongs to: the last one that begins at or before it.
-__device__ __forceinline__ uint32_t tensor_of(const ClipTable& t, uint32_t piece) {
-  uint32_t low = 0, high = t.tensors;
-  while (high - low > 1) {
-    const uint32_t mid = (low + high) / 2;
-    if (t.first[mid] <= piece) low = mid; else high = mid;
+template <class T> struct Piece {
+  const T* in;
+  T* out;
+  uint32_t n;
+};
+
+// The tensor that a piece belongs to is the last one that begins at or before it: a wave looks at 64 at a time.
+template <class T>
+__device__ __forceinline__ Piece<T> piece_of(const ClipTable& t, uint32_t piece, uint32_t piece_shift) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t i = 0;
+#pragma unroll
+  for (uint32_t i0 = 0; i0 < kTensors; i0 += 64) {
+    const uint32_t at = min(i0 + lane, (uint32_t)kTensors);
+    i += __popcll(__ballot(i0 + lane < t.tensors && t.first[at] <= piece));
   }
-  return low;
+  i = __builtin_amdgcn_readfirstlane(i) - 1;
+  const int64_t begin = (int64_t)(piece - t.first[i]) << piece_shift;
+  return {static_cast<const T*>(t.in[i]) + begin, static_cast<T*>(t.out[i]) + begin,
+          (uint32_t)min(int64_t(1) << piece_shift, t.count[i] - begin)};
 }
 
 __device__ __forceinline__ double block_sum(double x, double* lds) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) x += __shfl_xor(x, m);
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int wave = threadIdx.x >> 6, waves = kClipBlock >> 6;
   if ((threadIdx.x & 63) == 0) lds[wave] = x;
   __syncthreads();
   double sum = lds[0];
@@ -50,79 +67,103 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
   return sum;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kClipBlock) clip_squares_kernel(const ClipTable t, double* partial) {
-  constexpr int N = Quad<T>::N, kPiece = kPieceBytes / sizeof(T);
-  __shared__ double lds[kClipBlock / 64];
-  const uint32_t i = tensor_of(t, blockIdx.x);
-  const int64_t first = (int64_t)(blockIdx.x - t.first[i]) * kPiece;
-  const uint32_t n = (uint32_t)min((int64_t)kPiece, t.count[i] - first);
-  const T* in = static_cast<const T*>(t.in[i]) + first;
-  double sum = 0;
-  for (uint32_t at = threadIdx.x * N; at < n; at += kClipBlock * N) {
-    if (at + N <= n) {
-      const Quad<T> q = load_quad(in + at);
+constexpr int kQuads = 4;   // of a lane, whose loads are on their way together
+
+// Calls f(at, quad) for the quads of n elements, and g(at, element) for what is left.
+template <bool kStreaming, class T, class F, class G>
+__device__ __forceinline__ void for_piece(const T* in, uint32_t n, F f, G g) {
+  constexpr uint32_t N = Quad<T>::N, kStep = kClipBlock * N;
+  uint32_t at = threadIdx.x * N, done = 0;
+  for (; done + kQuads * kStep <= n; done += kQuads * kStep, at += kQuads * kStep) {
+    Quad<T> q[kQuads];
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += (double)q.v[e] * (double)q.v[e];
-    } else {
-      for (uint32_t e = at; e < n; ++e) sum += (double)in[e] * (double)in[e];
-    }
+    for (int i = 0; i < kQuads; ++i) q[i] = load_quad<kStreaming>(in + at + i * kStep);
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) f(at + i * kStep, q[i]);
+  }
+  for (; at < n; at += kStep) {
+    if (at + N <= n) f(at, load_quad<kStreaming>(in + at));
+    else
+      for (uint32_t e = at; e < n; ++e) g(e, in[e]);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kClipBlock) clip_squares_kernel(const ClipTable t, uint32_t pieces, uint32_t piece_shift, double* partial) {
+  __shared__ double lds[kClipBlock / 64];
+  double sum = 0;
+  for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
+    const Piece<T> piece = piece_of<T>(t, p, piece_shift);
+    for_piece<false>(
+        piece.in, piece.n,
+        [&](uint32_t, const Quad<T>& q) {
+#pragma unroll
+          for (int e = 0; e < Quad<T>::N; ++e) sum = fma((double)q.v[e], (double)q.v[e], sum);
+        },
+        [&](uint32_t, T x) { sum = fma((double)x, (double)x, sum); });
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
+// By the lanes of a block of kClipBlock, in every kernel: the same bits.
 template <class T>
-__global__ void __launch_bounds__(1024) clip_norm_kernel(const double* partial, uint32_t n, double max_norm, T* norm_and_factor) {
-  __shared__ double lds[16];
+__device__ __forceinline__ T factor_of(const double* partial, uint32_t n, double max_norm, T* norm_and_factor, double* lds) {
   double sum = 0;
-  for (uint32_t i = threadIdx.x; i < n; i += 1024) sum += partial[i];
-  sum = block_sum(sum, lds);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(sum);
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n; i += kClipBlock) sum += partial[i];
+  const double norm = sqrt(block_sum(sum, lds));
+  const T factor = (T)(norm <= max_norm ? 1.0 : max_norm / norm);   // NaN where the norm is
+  if (norm_and_factor && threadIdx.x == 0) {
     norm_and_factor[0] = (T)norm;
-    norm_and_factor[1] = (T)(norm <= max_norm ? 1.0 : max_norm / norm);   // NaN where the norm is
+    norm_and_factor[1] = factor;
   }
+  return factor;
 }
 
 template <class T>
-__global__ void __launch_bounds__(kClipBlock) clip_scale_kernel(const ClipTable t, const T* norm_and_factor) {
-  constexpr int N = Quad<T>::N, kPiece = kPieceBytes / sizeof(T);
-  const T factor = norm_and_factor[1];
-  const uint32_t i = tensor_of(t, blockIdx.x);
-  if (t.in[i] == t.out[i] && factor == (T)1) return;
-  const int64_t first = (int64_t)(blockIdx.x - t.first[i]) * kPiece;
-  const uint32_t n = (uint32_t)min((int64_t)kPiece, t.count[i] - first);
-  const T* in = static_cast<const T*>(t.in[i]) + first;
-  T* out = static_cast<T*>(t.out[i]) + first;
-  for (uint32_t at = threadIdx.x * N; at < n; at += kClipBlock * N) {
-    if (at + N <= n) {
-      Quad<T> q = load_quad(in + at);
+__global__ void __launch_bounds__(kClipBlock) clip_norm_kernel(const double* partial, uint32_t n, double max_norm, T* norm_and_factor) {
+  __shared__ double lds[kClipBlock / 64];
+  factor_of(partial, n, max_norm, norm_and_factor, lds);
+}
+
+// `sums` != 0: the factor is found from as many sums, and stored by the first block if `norm_and_factor` is to be; else read there.
+template <class T, bool kStreaming>
+__global__ void __launch_bounds__(kClipBlock) clip_scale_kernel(const ClipTable t, uint32_t pieces, uint32_t piece_shift, const double* partial,
+                                                                uint32_t sums, double max_norm, T* norm_and_factor, bool store) {
+  __shared__ double lds[kClipBlock / 64];
+  const T factor = sums ? factor_of(partial, sums, max_norm, store && blockIdx.x == 0 ? norm_and_factor : nullptr, lds) : norm_and_factor[1];
+  for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
+    const Piece<T> piece = piece_of<T>(t, pieces - 1 - p, piece_shift);
+    if (piece.in == piece.out && factor == (T)1) continue;
+    T* const out = piece.out;
+    for_piece<kStreaming>(
+        piece.in, piece.n,
+        [&](uint32_t at, Quad<T> q) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) q.v[e] *= factor;
-      store_quad(out + at, q);
-    } else {
-      for (uint32_t e = at; e < n; ++e) out[e] = in[e] * factor;
-    }
+          for (int e = 0; e < Quad<T>::N; ++e) q.v[e] *= factor;
+          store_quad<kStreaming>(out + at, q);
+        },
+        [&](uint32_t at, T x) { out[at] = x * factor; });
   }
 }
 
-// Calls `launch(table, pieces of the launch, pieces before it)` for tables that together hold every piece.
+// Calls `launch(table, pieces, blocks)` for tables that together hold every piece, of the tensors in their order or in the other.
 template <class F>
-void for_tables(const void* const* in, void* const* out, const int64_t* counts, int64_t count, int64_t piece, F launch) {
+void for_tables(const void* const* in, void* const* out, const int64_t* counts, int64_t count, uint32_t piece_shift, bool last_first, F launch) {
   ClipTable t;
   t.tensors = 0;
   uint32_t pieces = 0;
-  int64_t before = 0;
   auto flush = [&] {
-    if (t.tensors) launch(t, pieces, before);
-    before += pieces;
+    t.first[t.tensors] = pieces;
+    if (t.tensors) launch(t, pieces, (uint32_t)std::min<int64_t>(pieces, kMostClipBlocks));
     pieces = t.tensors = 0;
   };
-  for (int64_t i = 0; i < count; ++i) {
+  for (int64_t k = 0; k < count; ++k) {
+    const int64_t i = last_first ? count - 1 - k : k;
     if (counts[i] == 0) continue;
-    const int64_t of_this = (counts[i] + piece - 1) / piece;
-    if (t.tensors == kTensors || pieces + of_this > INT32_MAX / kClipBlock) flush();
+    const int64_t of_this = ((counts[i] - 1) >> piece_shift) + 1;
+    if (t.tensors == kTensors || pieces + of_this > INT32_MAX) flush();
     t.in[t.tensors] = in[i];
     t.out[t.tensors] = out ? out[i] : nullptr;
     t.count[t.tensors] = counts[i];
@@ -135,21 +176,39 @@ void for_tables(const void* const* in, void* const* out, const int64_t* counts, 
 template <class T>
 int clip_typed(hipStream_t s, const void* const* in, void* const* out, const int64_t* counts, int64_t count, double max_norm,
                T* norm_and_factor) {
-  constexpr int64_t kPiece = kPieceBytes / sizeof(T);
-  int64_t pieces = 0;
-  for (int64_t i = 0; i < count; ++i) pieces += (counts[i] + kPiece - 1) / kPiece;
-  CT_REQUIRE(pieces < INT32_MAX, "ct_clip_gradients: %lld pieces", (long long)pieces);
+  int64_t values = 0;
+  for (int64_t i = 0; i < count; ++i) values += counts[i];
+  // pieces small enough to give every block one
+  int64_t bytes = kLeastPiece;
+  while (bytes < kMostPiece && values * (int64_t)sizeof(T) > bytes * kMostClipBlocks) bytes *= 2;
+  uint32_t piece_shift = 0;
+  while ((int64_t(1) << piece_shift) * (int64_t)sizeof(T) < bytes) ++piece_shift;
+  int64_t sums = 0;
+  for_tables(in, out, counts, count, piece_shift, false, [&](const ClipTable&, uint32_t, uint32_t blocks) { sums += blocks; });
+  CT_REQUIRE(sums < INT32_MAX, "ct_clip_gradients: %lld tensors", (long long)count);
   void* scratch = nullptr;
-  if (int rc = stream_scratch(s, std::max<int64_t>(pieces, 1) * sizeof(double), &scratch)) return rc;
-  double* partial = static_cast<double*>(scratch);
-  for_tables(in, out, counts, count, kPiece, [&](const ClipTable& t, uint32_t n, int64_t before) {
-    hipLaunchKernelGGL((clip_squares_kernel<T>), dim3(n), dim3(kClipBlock), 0, s, t, partial + before);
+  if (int rc = stream_scratch(s, std::max<int64_t>(sums, 1) * sizeof(double), &scratch)) return rc;
+  double* const partial = static_cast<double*>(scratch);
+  double* to = partial;
+  for_tables(in, out, counts, count, piece_shift, false, [&](const ClipTable& t, uint32_t pieces, uint32_t blocks) {
+    hipLaunchKernelGGL((clip_squares_kernel<T>), dim3(blocks), dim3(kClipBlock), 0, s, t, pieces, piece_shift, to);
+    to += blocks;
   });
-  hipLaunchKernelGGL((clip_norm_kernel<T>), dim3(1), dim3(1024), 0, s, partial, (uint32_t)pieces, max_norm, norm_and_factor);
-  if (out)
-    for_tables(in, out, counts, count, kPiece, [&](const ClipTable& t, uint32_t n, int64_t) {
-      hipLaunchKernelGGL((clip_scale_kernel<T>), dim3(n), dim3(kClipBlock), 0, s, t, norm_and_factor);
+  const bool few = out && sums > 0 && sums <= kFewSums;
+  if (!few) hipLaunchKernelGGL((clip_norm_kernel<T>), dim3(1), dim3(kClipBlock), 0, s, partial, (uint32_t)sums, max_norm, norm_and_factor);
+  if (out) {
+    const bool past = 2 * values * (int64_t)sizeof(T) > kClipCacheBytes;
+    bool store = few;
+    for_tables(in, out, counts, count, piece_shift, true, [&](const ClipTable& t, uint32_t pieces, uint32_t blocks) {
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kClipBlock), 0, s, t, pieces, piece_shift, partial, few ? (uint32_t)sums : 0u, max_norm,
+                           norm_and_factor, store);
+      };
+      if (past) launch(clip_scale_kernel<T, true>);
+      else launch(clip_scale_kernel<T, false>);
+      store = false;
     });
+  }
   note_kernel("clip");
   return after_launch(s);
 }
