@@ -13,8 +13,14 @@ optimizers (:func:`cortex_amd.optimize.clip_gradients`).
 """
 from __future__ import annotations
 
+from . import capi
 from . import tensor as ct
 from .tensor import Tensor, TensorError, check_stream
+
+# What the operands of a call are, found in native code (csrc/front.cpp) where they are as they mostly are: each call checks
+# those numbers, and what does not pass there goes through the checks below, which say what is wrong.  (Some 10 us of Python a
+# call, for kernels of 3 to 5; 2 us so.)
+_operands = capi.front.operands if capi.front is not None else lambda kinds, tensors: None
 
 NORM_KINDS = ("none", "rms", "layer")
 
@@ -99,6 +105,23 @@ def norm_descriptor(*, post="rms", pre="rms", epsilon=1e-5, residual_scale=1.0) 
 
 
 _OF_COLUMNS = ("post-scale", "post-bias", "pre-scale", "pre-bias")
+_PARAMETERS = {*_OF_COLUMNS, "gate"}
+
+
+def _norm_fits(shape, matrices, gate, statistics, scales) -> bool:
+    """Whether matrices (rows, columns, distance; zeros if absent) are of ``shape`` and the other operands go with it."""
+    rows, columns = shape
+    for i in range(0, len(matrices), 3):
+        if matrices[i] and (matrices[i] != rows or matrices[i + 1] != columns):
+            return False
+    if gate[0] and not (gate[0] in (1, rows) and gate[1] in (1, columns)):
+        return False
+    if statistics[0] and statistics != (2, 4 * rows, rows):
+        return False
+    for i in range(0, len(scales), 3):
+        if scales[i] and (scales[i] != 1 or scales[i + 1] != columns):
+            return False
+    return True
 
 
 def _norm_parameters(name: str, first: Tensor, parameters: dict, shape):
@@ -128,8 +151,19 @@ def norm_residual(output: Tensor, normalized: Tensor, statistics: Tensor, input:
     ([4, rows], or None) is what :func:`norm_residual_gradient` needs.  ``output`` may be the residual or the input itself,
     ``normalized`` the input."""
     name = "norm-residual"
-    shape = _rows(name, "input", input)[:2]
+    p = parameters.get
     has_pre = descriptor["pre"] != "none"
+    if parameters.keys() <= _PARAMETERS and (normalized is not None or not has_pre):
+        normalized = normalized if has_pre else None
+        gate, scales = p("gate"), (p("post-scale"), p("post-bias"), p("pre-scale"), p("pre-bias"))
+        found = _operands("mmmmmppppp", (input, output, residual, normalized, gate, statistics, *scales))
+        if found is not None and _norm_fits(found[:2], found[3:12], found[12:15], found[15:18], found[18:]):
+            check_stream().norm_residual(output.buffer, output.dimensions, _buffer(normalized), _dims(normalized), _buffer(statistics),
+                                         input.buffer, input.dimensions, _buffer(residual), _dims(residual), _buffer(gate),
+                                         _dims(gate), *map(_buffer, scales), descriptor["post"], descriptor["pre"],
+                                         descriptor["residual-scale"], descriptor["epsilon"])
+            return output, normalized
+    shape = _rows(name, "input", input)[:2]
     if has_pre and normalized is None:
         raise TensorError(f"{name}: a norm before the next block needs a tensor to store to")
     normalized = normalized if has_pre else None
@@ -139,7 +173,6 @@ def norm_residual(output: Tensor, normalized: Tensor, statistics: Tensor, input:
             raise TensorError(f"{name}: shapes differ: {what} {list(t.shape())}, input {list(shape)}")
     _packed(name, "statistics", statistics, [4, shape[0]])
     gate = _norm_parameters(name, output, parameters, shape)
-    p = parameters.get
     check_stream().norm_residual(output.buffer, output.dimensions, _buffer(normalized), _dims(normalized), _buffer(statistics),
                                  input.buffer, input.dimensions, _buffer(residual), _dims(residual), _buffer(gate), _dims(gate),
                                  _buffer(p("post-scale")), _buffer(p("post-bias")), _buffer(p("pre-scale")),
@@ -154,6 +187,22 @@ def norm_residual_gradient(input_gradient: Tensor, residual_gradient: Tensor, pa
     """The gradients of :func:`norm_residual`, all overwritten, from those of its results (either may be None: zero).  Any
     gradient that is None, or not in ``parameter_gradients``, is not formed."""
     name = "norm-residual-gradient"
+    p, g = parameters.get, parameter_gradients.get
+    if parameters.keys() <= _PARAMETERS and parameter_gradients.keys() <= parameters.keys():
+        gate, scales = p("gate"), (p("post-scale"), p("post-bias"), p("pre-scale"), p("pre-bias"))
+        results = (g("post-scale"), g("post-bias"), g("pre-scale"), g("pre-bias"))
+        found = _operands("mmmmmmmmppppppppp", (input, input_gradient, residual_gradient, output_gradient, normalized_gradient,
+                                                output, gate, g("gate"), statistics, *scales, *results))
+        if (found is not None and _norm_fits(found[:2], found[3:18], found[18:21], found[24:27], found[27:]) and
+                (not found[21] or (found[21:23] == found[18:20] and found[23] == found[22])) and
+                not any(b and not a for a, b in zip(found[27:39:3], found[39::3]))):
+            check_stream().norm_residual_gradient(
+                _buffer(input_gradient), _dims(input_gradient), _buffer(residual_gradient), _dims(residual_gradient),
+                _buffer(g("gate")), *map(_buffer, results), _buffer(output_gradient), _dims(output_gradient),
+                _buffer(normalized_gradient), _dims(normalized_gradient), input.buffer, input.dimensions, _buffer(output),
+                _dims(output), _buffer(statistics), _buffer(gate), _dims(gate), *map(_buffer, scales[:3]), descriptor["post"],
+                descriptor["pre"], descriptor["residual-scale"])
+            return input_gradient, residual_gradient
     shape = _rows(name, "input", input)[:2]
     _floating(name, input, input_gradient, residual_gradient, output_gradient, normalized_gradient, output, statistics)
     for what, t in (("input gradient", input_gradient), ("residual gradient", residual_gradient),
@@ -169,7 +218,6 @@ def norm_residual_gradient(input_gradient: Tensor, residual_gradient: Tensor, pa
         if parameters.get(key) is None:
             raise TensorError(f"{name}: a gradient of {key!r}, which is no parameter")
         _packed(name, f"the gradient of {key}", t, parameters[key].shape())
-    p, g = parameters.get, parameter_gradients.get
     check_stream().norm_residual_gradient(
         _buffer(input_gradient), _dims(input_gradient), _buffer(residual_gradient), _dims(residual_gradient), _buffer(g("gate")),
         _buffer(g("post-scale")), _buffer(g("post-bias")), _buffer(g("pre-scale")), _buffer(g("pre-bias")),
@@ -193,6 +241,16 @@ def route_experts(experts: Tensor, weights: Tensor, offsets: Tensor, tokens: Ten
     expert e has the places offsets[e] to offsets[e + 1] - 1, ``tokens`` names the token at a place (-1 beyond the last
     one) and ``slots`` the place of an assignment (-1 where there is none)."""
     name = "route-experts"
+    found = _operands("mipiii", (logits, experts, weights, offsets, tokens, slots))
+    if found is not None:
+        n, n_experts, stride, dimensions, count, n_chosen = found[:6]
+        of_choice = (dimensions, count, n_chosen)
+        if (dimensions == 2 and count == n * n_chosen and n_chosen <= 32 and n_chosen <= n_experts <= 1024 and
+                found[6:9] == of_choice and found[9:12] == (1, n_experts + 1, n_experts + 1) and found[12:15] == (1, count, count) and
+                found[15:] == of_choice):
+            check_stream().route_experts(experts.buffer, weights.buffer, offsets.buffer, tokens.buffer, slots.buffer, logits.buffer,
+                                         stride, n, n_experts, n_chosen, renormalize)
+            return experts, weights
     n, n_experts, stride = _rows(name, "logits", logits)
     n_chosen = int(experts.shape()[-1])
     _floating(name, logits, weights)
@@ -211,6 +269,15 @@ def route_experts_gradient(logits_gradient: Tensor, weights_gradient: Tensor, we
                            renormalize: bool = True) -> Tensor:
     """The gradient of the weights with respect to the logits, overwritten.  ``logits`` may be None under ``renormalize``."""
     name = "route-experts-gradient"
+    found = _operands("mmppi", (logits_gradient, logits, weights_gradient, weights, experts))
+    if found is not None:
+        n, n_experts, gradient_stride, rows, columns, stride = found[:6]
+        of_choice = found[12:]
+        if ((found[3:5] == found[:2] or (logits is None and renormalize)) and of_choice[0] == 2 and of_choice[1] == n * of_choice[2] and
+                found[6:9] == of_choice == found[9:12]):
+            check_stream().route_experts_gradient(logits_gradient.buffer, gradient_stride, weights_gradient.buffer, weights.buffer,
+                                                  experts.buffer, _buffer(logits), stride, n, n_experts, of_choice[2], renormalize)
+            return logits_gradient
     n, n_experts, gradient_stride = _rows(name, "logits gradient", logits_gradient)
     n_chosen = int(experts.shape()[-1])
     _floating(name, logits_gradient, weights_gradient, weights, logits)
@@ -246,6 +313,14 @@ def grouped_gemm(C: Tensor, trans_b, alpha, A: Tensor, B: Tensor, beta, offsets:
     C[i] = alpha * A[index[i]] * (trans-b? B[e]) + beta * C[i].  Rows of no group are left as they are.  Without ``index``
     row i of A is row i; an index outside A is a row of zeros."""
     name = "grouped-gemm"
+    found = _operands("mmgii", (C, A, B, offsets, index))
+    if found is not None:
+        rows, columns, c_stride, a_rows, a_columns, a_stride, groups, b_rows, b_columns, b_row_stride, b_stride = found[:11]
+        if ((b_rows, b_columns) == ((columns, a_columns) if trans_b else (a_columns, columns)) and
+                found[11:14] == (1, groups + 1, groups + 1) and (found[14:] == (1, rows, rows) if index is not None else a_rows == rows)):
+            check_stream().grouped_gemm(C.buffer, c_stride, trans_b, alpha, A.buffer, a_rows, a_columns, a_stride, _buffer(index),
+                                        B.buffer, columns, b_row_stride, b_stride, offsets.buffer, groups, rows, beta)
+            return C
     _floating(name, C, A, B)
     rows, c_columns, c_stride = _rows(name, "C", C)
     a_rows, a_columns, a_stride = _rows(name, "A", A)
@@ -293,6 +368,15 @@ def combine_experts(output: Tensor, rows: Tensor, weights: Tensor, slots: Tensor
     """output[t] = sum over j of weights[t, j] * rows[slots[t, j]]; slots outside the rows are left out.  ``weights`` None
     means ones."""
     name = "combine-experts"
+    found = _operands("mmpi", (output, rows, weights, slots))
+    if found is not None:
+        n, width, stride, count, columns, rows_stride = found[:6]
+        of_choice = found[9:]
+        if (columns == width and of_choice[0] == 2 and of_choice[1] == n * of_choice[2] and
+                (weights is None or found[6:9] == of_choice)):
+            check_stream().combine_experts(output.buffer, stride, rows.buffer, count, rows_stride, _buffer(weights), slots.buffer, n,
+                                           of_choice[2], width)
+            return output
     _floating(name, output, rows, weights)
     _indexes(name, output, slots=slots)
     n, width, stride = _rows(name, "output", output)

@@ -465,8 +465,162 @@ PyObject* stand_in(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return result;
 }
 
+// ---------------------------------------------------------------- operands of the calls of blocks.py and optimize.py
+
+PyObject *s_device, *s_buffer, *s_datatype, *s_ptr, *s_ecount;
+
+// The datatype of a buffer: 'f', 'd', 'i' (float, double, int), 0 for another.
+char type_of(PyObject* buffer) {
+  PyObject* name = PyObject_GetAttr(buffer, s_datatype);
+  if (!name) return PyErr_Clear(), 0;
+  char type = 0;
+  if (PyUnicode_CheckExact(name))
+    type = PyUnicode_CompareWithASCIIString(name, "float") == 0 ? 'f' : PyUnicode_CompareWithASCIIString(name, "double") == 0 ? 'd' :
+           PyUnicode_CompareWithASCIIString(name, "int") == 0 ? 'i' : 0;
+  Py_DECREF(name);
+  return type;
+}
+
+// Whether the elements lie one behind the other in their order; none for tensors without elements.
+bool packed(const Plain& p, int64_t* count) {
+  *count = 1;
+  for (Py_ssize_t i = p.n; i-- > 0;) {
+    if (p.shape[i] < 1 || (p.shape[i] != 1 && p.strides[i] != *count) || !multiply(*count, p.shape[i], count)) return false;
+  }
+  return true;
+}
+
+struct Operands {
+  PyObject* device = nullptr;   // borrowed
+  char floating = 0;
+  int64_t values[128];
+  Py_ssize_t n = 0;
+};
+
+// Appends what an operand of a kind is; false for what Python decides.
+bool add_operand(PyObject* tensor, char kind, Operands* o) {
+  const Py_ssize_t fields = kind == 'm' ? 3 : kind == 'g' ? 5 : kind == 'p' || kind == 'i' ? 3 : -1;
+  if (fields < 0 || o->n + fields > 128) return false;
+  int64_t* to = o->values + o->n;
+  o->n += fields;
+  if (tensor == Py_None) {
+    for (Py_ssize_t i = 0; i < fields; ++i) to[i] = 0;
+    return true;
+  }
+  PyObject* device = PyObject_GetAttr(tensor, s_device);
+  PyObject* dims = device ? PyObject_GetAttr(tensor, s_dimensions) : nullptr;
+  PyObject* buffer = dims ? PyObject_GetAttr(tensor, s_buffer) : nullptr;
+  bool fine = buffer != nullptr;
+  if (!fine) PyErr_Clear();
+  Plain p;
+  if (fine && !o->device) o->device = device;
+  fine = fine && o->device == device && read_dims(dims, &p) && p.n >= 1;
+  const char type = fine ? type_of(buffer) : 0;
+  if (fine && kind == 'i') fine = type == 'i';
+  else if (fine) {
+    if (!o->floating) o->floating = type;
+    fine = (type == 'f' || type == 'd') && type == o->floating;
+  }
+  if (fine && kind == 'm') {
+    const int64_t rows = p.n == 2 ? p.shape[0] : 1, columns = p.shape[p.n - 1];
+    fine = p.n <= 2 && rows >= 1 && columns >= 1 && (columns == 1 || p.strides[p.n - 1] == 1);
+    const int64_t stride = !fine ? 0 : rows > 1 ? p.strides[0] : p.n == 2 && p.strides[0] > columns ? p.strides[0] : columns;
+    fine = fine && stride >= columns;
+    to[0] = rows, to[1] = columns, to[2] = stride;
+  } else if (fine && kind == 'g') {
+    fine = p.n == 3 && p.shape[0] >= 1 && p.shape[1] >= 1 && p.shape[2] >= 1 && (p.shape[2] == 1 || p.strides[2] == 1) &&
+           (p.shape[1] == 1 || p.strides[1] >= p.shape[2]);
+    if (fine) {
+      for (int i = 0; i < 3; ++i) to[i] = p.shape[i];
+      to[3] = p.strides[1] > p.shape[2] ? p.strides[1] : p.shape[2];
+      to[4] = p.strides[0];
+    }
+  } else if (fine) {
+    int64_t count = 0;
+    fine = packed(p, &count);
+    to[0] = p.n, to[1] = count, to[2] = p.shape[p.n - 1];
+  }
+  Py_XDECREF(buffer);
+  Py_XDECREF(dims);
+  Py_XDECREF(device);
+  return fine;
+}
+
+// operands(kinds, tensors): a tuple of numbers, some to each tensor (zeros for None), or None where one is not what its kind
+// asks for: 'm' rows of a matrix of floats (rows, columns, distance), 'g' a matrix to each group (groups, rows, columns, distance of rows,
+// of matrices), 'p' floats one behind the other and 'i' ints (dimensions, elements, the last dimension).  All floats of one type, all
+// tensors on one device.
+PyObject* operands(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Py_ssize_t length = 0;
+  const char* kinds = n == 2 && PyUnicode_Check(args[0]) && PyTuple_CheckExact(args[1]) ? PyUnicode_AsUTF8AndSize(args[0], &length) : nullptr;
+  if (!kinds || length != PyTuple_GET_SIZE(args[1])) return PyErr_SetString(PyExc_TypeError, "operands(kinds, tensors)"), nullptr;
+  Operands o;
+  for (Py_ssize_t i = 0; i < length; ++i)
+    if (!add_operand(PyTuple_GET_ITEM(args[1], i), kinds[i], &o)) Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(o.n);
+  for (Py_ssize_t i = 0; result && i < o.n; ++i) {
+    PyObject* value = PyLong_FromLongLong(o.values[i]);
+    if (!value) Py_CLEAR(result);
+    else PyTuple_SET_ITEM(result, i, value);
+  }
+  return result;
+}
+
+bool int_of(PyObject* object, PyObject* name, int64_t* out) {
+  PyObject* value = PyObject_GetAttr(object, name);
+  if (!value) return PyErr_Clear(), false;
+  int overflow = 0;
+  bool fine = PyLong_CheckExact(value);
+  if (fine) *out = PyLong_AsLongLongAndOverflow(value, &overflow);
+  Py_DECREF(value);
+  return fine && !overflow;
+}
+
+// addresses(list): (addresses, counts, datatype) of buffers, or of dense tensors that are all of their buffers, as bytes of
+// eight to each; None where Python decides.
+PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 1 || !PyList_CheckExact(args[0])) Py_RETURN_NONE;
+  const Py_ssize_t count = PyList_GET_SIZE(args[0]);
+  PyObject* at = PyBytes_FromStringAndSize(nullptr, 8 * count);
+  PyObject* counts = at ? PyBytes_FromStringAndSize(nullptr, 8 * count) : nullptr;
+  if (!counts) return Py_XDECREF(at), nullptr;
+  char type = 0;
+  bool fine = count > 0;
+  for (Py_ssize_t i = 0; fine && i < count; ++i) {
+    PyObject* item = PyList_GET_ITEM(args[0], i);
+    PyObject* buffer = PyObject_GetAttr(item, s_buffer);
+    int64_t elements = -1, address = 0, length = 0;
+    if (buffer) {
+      PyObject* dims = PyObject_GetAttr(item, s_dimensions);
+      Plain p;
+      fine = dims && read_dims(dims, &p) && packed(p, &elements);
+      if (!dims) PyErr_Clear();
+      Py_XDECREF(dims);
+    } else {
+      PyErr_Clear();
+      Py_INCREF(item);
+      buffer = item;
+    }
+    const char own = fine ? type_of(buffer) : 0;
+    if (!type) type = own;
+    fine = fine && (own == 'f' || own == 'd') && own == type && int_of(buffer, s_ptr, &address) && int_of(buffer, s_ecount, &length) &&
+           (elements < 0 || elements == length);
+    reinterpret_cast<int64_t*>(PyBytes_AS_STRING(at))[i] = address;
+    reinterpret_cast<int64_t*>(PyBytes_AS_STRING(counts))[i] = length;
+    Py_DECREF(buffer);
+  }
+  PyObject* result = nullptr;
+  if (fine) result = Py_BuildValue("OOs", at, counts, type == 'f' ? "float" : "double");
+  Py_DECREF(at);
+  Py_DECREF(counts);
+  if (result || PyErr_Occurred()) return result;
+  Py_RETURN_NONE;
+}
+
 PyMethodDef g_module_methods[] = {{"stand_in", as_method(stand_in), METH_FASTCALL, nullptr},
                                   {"bind", as_method(bind), METH_FASTCALL, nullptr},
+                                  {"operands", as_method(operands), METH_FASTCALL, nullptr},
+                                  {"addresses", as_method(addresses), METH_FASTCALL, nullptr},
                                   {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, g_module_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -478,6 +632,11 @@ PyMODINIT_FUNC PyInit__front() {
   s_max_shape = PyUnicode_InternFromString("max-shape");
   s_dimensions = PyUnicode_InternFromString("dimensions");
   s_lib = PyUnicode_InternFromString("_lib");
+  s_device = PyUnicode_InternFromString("device");
+  s_buffer = PyUnicode_InternFromString("buffer");
+  s_datatype = PyUnicode_InternFromString("datatype");
+  s_ptr = PyUnicode_InternFromString("ptr");
+  s_ecount = PyUnicode_InternFromString("_ecount");
   g_index = PyDict_New();
-  return s_shape && s_strides && s_max_shape && s_dimensions && s_lib && g_index ? PyModule_Create(&g_module) : nullptr;
+  return s_device && s_buffer && s_datatype && s_ptr && s_ecount && s_shape && s_strides && s_max_shape && s_dimensions && s_lib && g_index ? PyModule_Create(&g_module) : nullptr;
 }

@@ -47,6 +47,32 @@ template <class T> __device__ __forceinline__ T of_key(typename KeyOf<T>::Key k)
 // Of -infinity: this and all below it are never chosen.
 template <class T> __device__ __forceinline__ typename KeyOf<T>::Key closed_key() { return key_of<T>(-__builtin_inf()); }
 
+// ------------------------------------------------------------------ reductions over the lanes of a token
+
+// The value `step` lanes further on in a row of 16, around its end: no trip through LDS.
+template <int step> __device__ __forceinline__ uint32_t rotated(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + step, 0xf, 0xf, true);
+}
+template <int step> __device__ __forceinline__ uint64_t rotated(uint64_t x) {
+  return (uint64_t)rotated<step>((uint32_t)x) | (uint64_t)rotated<step>((uint32_t)(x >> 32)) << 32;
+}
+template <int step> __device__ __forceinline__ float rotated(float x) { return __builtin_bit_cast(float, rotated<step>(__builtin_bit_cast(uint32_t, x))); }
+template <int step> __device__ __forceinline__ double rotated(double x) { return __builtin_bit_cast(double, rotated<step>(__builtin_bit_cast(uint64_t, x))); }
+
+// f over the LANES (16 or 64) lanes of a token, in all of them.
+template <int LANES, class X, class F>
+__device__ __forceinline__ X over_lanes(X x, F f) {
+  x = f(x, rotated<8>(x));
+  x = f(x, rotated<4>(x));
+  x = f(x, rotated<2>(x));
+  x = f(x, rotated<1>(x));
+  if constexpr (LANES == 64) {
+    x = f(x, __shfl_xor(x, 16));
+    x = f(x, __shfl_xor(x, 32));
+  }
+  return x;
+}
+
 struct RouteArgs {
   int32_t* experts;
   void* weights;
@@ -57,7 +83,7 @@ struct RouteArgs {
   int64_t colstride;
   uint32_t n, n_experts, n_chosen, tokens_per_block, blocks;
   bool renormalize;
-  int32_t* counts;   // [blocks][n_experts + 1]; then, in place, of all blocks before
+  int32_t* counts;   // [n_experts + 1][blocks]; then, in place, of all blocks before
   int32_t* totals;   // [n_experts + 1]
 };
 
@@ -65,40 +91,33 @@ struct RouteArgs {
 template <class T, int LANES, int V>
 __device__ __forceinline__ void choose(const RouteArgs& a, uint32_t token, uint32_t lane, uint32_t* counts) {
   using Key = typename KeyOf<T>::Key;
+  constexpr int kMine = kMostChosen / LANES + (kMostChosen % LANES > 0);   // choices that a lane keeps: j % LANES is its own
   const T* row = static_cast<const T*>(a.logits) + (int64_t)token * a.colstride;
   T x[V];
   Key key[V];
 #pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = row[min(lane + v * LANES, a.n_experts - 1)];
+#pragma unroll
   for (int v = 0; v < V; ++v) {
-    const uint32_t e = lane + v * LANES;
-    x[v] = e < a.n_experts ? row[e] : -__builtin_inf();
+    if (lane + v * LANES >= a.n_experts) x[v] = -__builtin_inf();
     key[v] = key_of<T>(x[v]);
     if (key[v] <= closed_key<T>()) key[v] = 0;
   }
   T top = 0, sum = 0;
   uint32_t found = 0;
-  T mine[kMostChosen / LANES + 1];   // value j of the chosen ones, in lane j % LANES
+  T power_of[kMine] = {};
+  int32_t expert_of[kMine];
 #pragma unroll
-  for (auto& m : mine) m = 0;
-  const int64_t at = (int64_t)token * a.n_chosen;
+  for (int q = 0; q < kMine; ++q) expert_of[q] = -1;
   for (uint32_t j = 0; j < a.n_chosen; ++j) {
-    Key best = 0;
-    uint32_t index = 0xffffffffu;
+    Key best = key[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > best) {
-        best = key[v];
-        index = lane + v * LANES;
-      }
+    for (int v = 1; v < V; ++v) best = max(best, key[v]);
+    best = over_lanes<LANES>(best, [](Key x, Key y) { return x > y ? x : y; });
+    uint32_t index = 0xffffffffu;   // the lowest that has it
 #pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) {
-      const Key k = __shfl_xor(best, m);
-      const uint32_t i = __shfl_xor(index, m);
-      if (k > best || (k == best && i < index)) {
-        best = k;
-        index = i;
-      }
-    }
+    for (int v = V - 1; v >= 0; --v) index = key[v] == best ? lane + v * LANES : index;
+    index = over_lanes<LANES>(index, [](uint32_t x, uint32_t y) { return min(x, y); });
     const bool any = best != 0;
     const T value = of_key<T>(best);
     if (j == 0) top = value;
@@ -106,42 +125,29 @@ __device__ __forceinline__ void choose(const RouteArgs& a, uint32_t token, uint3
     sum += power;
     found += any;
 #pragma unroll
-    for (int q = 0; q < (int)(sizeof(mine) / sizeof(T)); ++q)
-      if (j == lane + q * LANES) mine[q] = power;
-    if (lane == 0) {
-      a.experts[at + j] = any ? (int32_t)index : -1;
-      atomicAdd(&counts[any ? index : a.n_experts], 1u);
-    }
+    for (int q = 0; q < kMine; ++q)
+      if (j == lane + q * LANES) {
+        power_of[q] = power;
+        expert_of[q] = any ? (int32_t)index : -1;
+      }
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (index == lane + v * LANES) key[v] = 0;
+    for (int v = 0; v < V; ++v) key[v] = index == lane + v * LANES ? Key(0) : key[v];
   }
   if (!a.renormalize) {
     sum = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) sum += (T)exp(x[v] - top);   // of a row without an open expert: not used
-#pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
+    sum = over_lanes<LANES>(sum, [](T x, T y) { return x + y; });
   }
-  T* weights = static_cast<T*>(a.weights) + at;
+  const int64_t at = (int64_t)token * a.n_chosen;
 #pragma unroll
-  for (int q = 0; q < (int)(sizeof(mine) / sizeof(T)); ++q) {
+  for (int q = 0; q < kMine; ++q) {
     const uint32_t j = lane + q * LANES;
-    if (j < a.n_chosen) weights[j] = j < found ? mine[q] / sum : T(0);
+    if (j >= a.n_chosen) continue;
+    a.experts[at + j] = expert_of[q];
+    static_cast<T*>(a.weights)[at + j] = j < found ? power_of[q] / sum : T(0);
+    atomicAdd(&counts[expert_of[q] < 0 ? a.n_experts : (uint32_t)expert_of[q]], 1u);
   }
-}
-
-template <class T, int LANES, int V>
-__global__ void __launch_bounds__(kRouteBlock) route_choose_kernel(const RouteArgs a) {
-  __shared__ uint32_t counts[kMostExperts + 1];
-  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) counts[e] = 0;
-  __syncthreads();
-  const uint32_t first = blockIdx.x * a.tokens_per_block, end = min(a.n, first + a.tokens_per_block);
-  for (uint32_t t = first + threadIdx.x / LANES; t < end; t += kRouteBlock / LANES)
-    choose<T, LANES, V>(a, t, threadIdx.x % LANES, counts);
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock)
-    a.counts[(int64_t)blockIdx.x * (a.n_experts + 1) + e] = counts[e];
 }
 
 __device__ __forceinline__ uint32_t wave_inclusive(uint32_t x) {
@@ -153,55 +159,53 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t x) {
   return x;
 }
 
-// Block e: the counts of expert e in the blocks before each.
-__global__ void __launch_bounds__(64) route_scan_kernel(const RouteArgs a) {
-  const uint32_t e = blockIdx.x, pitch = a.n_experts + 1, lane = threadIdx.x;
+constexpr int kRouteWaves = kRouteBlock / 64;
+
+// What a block keeps in LDS to place its assignments: where each expert's begin, and where a wave's next one of each goes.
+struct PlaceLds {
+  uint32_t start[kMostExperts + 1];
+  uint32_t cursor[kRouteWaves][kMostExperts + 1];
+};
+
+// The assignments of each expert begin where those of the ones before end.  By the first wave; `offsets` where they are stored.
+template <class Total>
+__device__ __forceinline__ void begin_experts(const RouteArgs& a, PlaceLds& lds, Total total, bool store) {
+  const uint32_t lane = threadIdx.x & 63, buckets = a.n_experts + 1;
+  if (threadIdx.x >= 64) return;
   uint32_t before = 0;
-  for (uint32_t b0 = 0; b0 < a.blocks; b0 += 64) {
-    const uint32_t b = b0 + lane;
-    const uint32_t count = b < a.blocks ? a.counts[(int64_t)b * pitch + e] : 0;
-    const uint32_t upto = wave_inclusive(count);
-    if (b < a.blocks) a.counts[(int64_t)b * pitch + e] = before + upto - count;
+  for (uint32_t e0 = 0; e0 < buckets; e0 += 64) {
+    const uint32_t e = e0 + lane, count = e < buckets ? total(e) : 0, upto = wave_inclusive(count);
+    if (e < buckets) {
+      lds.start[e] = before + upto - count;
+      if (store) a.offsets[e] = (int32_t)lds.start[e];
+    }
     before += __shfl(upto, 63);
   }
-  if (lane == 0) a.totals[e] = before;
 }
 
-// tokens and slots of a block's assignments, each wave a run of them in its order.
-__global__ void __launch_bounds__(kRouteBlock) route_place_kernel(const RouteArgs a) {
-  constexpr int kWaves = kRouteBlock / 64;
-  __shared__ uint32_t start[kMostExperts + 1];
-  __shared__ uint32_t cursor[kWaves][kMostExperts + 1];   // where a wave's next assignment of an expert goes
+// tokens and slots of assignments first .. end - 1, each wave a run of them in its order; before(e): those of expert e ahead of
+// `first`.
+template <class Before>
+__device__ __forceinline__ void place(const RouteArgs& a, PlaceLds& lds, uint32_t first, uint32_t end, Before before) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, buckets = a.n_experts + 1;
-  for (uint32_t e = threadIdx.x; e < kWaves * (kMostExperts + 1); e += kRouteBlock) (&cursor[0][0])[e] = 0;
-  if (wave == 0) {
-    uint32_t before = 0;
-    for (uint32_t e0 = 0; e0 < buckets; e0 += 64) {
-      const uint32_t e = e0 + lane, count = e < buckets ? a.totals[e] : 0, upto = wave_inclusive(count);
-      if (e < buckets) {
-        start[e] = before + upto - count;
-        if (blockIdx.x == 0) a.offsets[e] = start[e];
-      }
-      before += __shfl(upto, 63);
-    }
-  }
+  for (uint32_t e = threadIdx.x; e < buckets; e += kRouteBlock)
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) lds.cursor[w][e] = 0;
   __syncthreads();
-  const uint32_t first = blockIdx.x * a.tokens_per_block * a.n_chosen;
-  const uint32_t end = min(a.n, (blockIdx.x + 1) * a.tokens_per_block) * a.n_chosen;
-  const uint32_t run = ((end - first + kWaves - 1) / kWaves + 63) / 64 * 64;
+  const uint32_t run = ((end - first + kRouteWaves - 1) / kRouteWaves + 63) / 64 * 64;
   const uint32_t mine = min(end, first + wave * run), mine_end = min(end, mine + run);
   auto bucket_of = [&](uint32_t i) {
     const int32_t e = a.experts[i];
     return e < 0 ? a.n_experts : (uint32_t)e;
   };
-  for (uint32_t i = mine + lane; i < mine_end; i += 64) atomicAdd(&cursor[wave][bucket_of(i)], 1u);
+  for (uint32_t i = mine + lane; i < mine_end; i += 64) atomicAdd(&lds.cursor[wave][bucket_of(i)], 1u);
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < buckets; e += kRouteBlock) {
-    uint32_t at = start[e] + a.counts[(int64_t)blockIdx.x * buckets + e];
+    uint32_t at = lds.start[e] + before(e);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t count = cursor[w][e];
-      cursor[w][e] = at;
+    for (int w = 0; w < kRouteWaves; ++w) {
+      const uint32_t count = lds.cursor[w][e];
+      lds.cursor[w][e] = at;
       at += count;
     }
   }
@@ -218,10 +222,10 @@ __global__ void __launch_bounds__(kRouteBlock) route_place_kernel(const RouteArg
     }
     const uint32_t rank = __popcll(same & ((uint64_t(1) << lane) - 1));
     uint32_t at = 0;
-    if (in) at = cursor[wave][bucket] + rank;
+    if (in) at = lds.cursor[wave][bucket] + rank;
     __threadfence_block();   // read by all lanes before one of them moves it
     __builtin_amdgcn_wave_barrier();
-    if (in && rank == 0) cursor[wave][bucket] = at + __popcll(same);
+    if (in && rank == 0) lds.cursor[wave][bucket] = at + __popcll(same);
     __threadfence_block();
     __builtin_amdgcn_wave_barrier();
     if (in) {
@@ -233,25 +237,97 @@ __global__ void __launch_bounds__(kRouteBlock) route_place_kernel(const RouteArg
 }
 
 template <class T, int LANES, int V>
+__global__ void __launch_bounds__(kRouteBlock) route_choose_kernel(const RouteArgs a) {
+  __shared__ uint32_t counts[kMostExperts + 1];
+  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) counts[e] = 0;
+  __syncthreads();
+  const uint32_t first = blockIdx.x * a.tokens_per_block, end = min(a.n, first + a.tokens_per_block);
+  for (uint32_t t = first + threadIdx.x / LANES; t < end; t += kRouteBlock / LANES)
+    choose<T, LANES, V>(a, t, threadIdx.x % LANES, counts);
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) a.counts[(int64_t)e * a.blocks + blockIdx.x] = counts[e];
+}
+
+// Block e: the counts of expert e in the blocks before each.
+__global__ void __launch_bounds__(kRouteBlock) route_scan_kernel(const RouteArgs a) {
+  __shared__ uint32_t of_waves[kRouteWaves];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t* counts = a.counts + (int64_t)blockIdx.x * a.blocks;
+  constexpr uint32_t kEach = 4;
+  uint32_t before = 0;
+  for (uint32_t b0 = 0; b0 < a.blocks; b0 += kRouteBlock * kEach) {
+    const uint32_t b = b0 + threadIdx.x * kEach;
+    uint32_t count[kEach], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+      count[i] = b + i < a.blocks ? counts[b + i] : 0;
+      sum += count[i];
+    }
+    const uint32_t upto = wave_inclusive(sum);
+    __syncthreads();
+    if (lane == 63) of_waves[wave] = upto;
+    __syncthreads();
+    uint32_t at = before + upto - sum;
+#pragma unroll
+    for (uint32_t w = 0; w < kRouteWaves; ++w) {
+      if (w < wave) at += of_waves[w];
+      before += of_waves[w];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+      if (b + i < a.blocks) counts[b + i] = (int32_t)at;
+      at += count[i];
+    }
+  }
+  if (threadIdx.x == 0) a.totals[blockIdx.x] = (int32_t)before;
+}
+
+__global__ void __launch_bounds__(kRouteBlock) route_place_kernel(const RouteArgs a) {
+  __shared__ PlaceLds lds;
+  begin_experts(a, lds, [&](uint32_t e) { return (uint32_t)a.totals[e]; }, blockIdx.x == 0);
+  const uint32_t first = blockIdx.x * a.tokens_per_block * a.n_chosen;
+  const uint32_t end = min(a.n, (blockIdx.x + 1) * a.tokens_per_block) * a.n_chosen;
+  place(a, lds, first, end, [&](uint32_t e) { return (uint32_t)a.counts[(int64_t)e * a.blocks + blockIdx.x]; });
+}
+
+// A few tokens: all of it in one block.
+template <class T, int LANES, int V>
+__global__ void __launch_bounds__(kRouteBlock) route_few_kernel(const RouteArgs a) {
+  __shared__ uint32_t counts[kMostExperts + 1];
+  __shared__ PlaceLds lds;
+  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) counts[e] = 0;
+  __syncthreads();
+  for (uint32_t t = threadIdx.x / LANES; t < a.n; t += kRouteBlock / LANES) choose<T, LANES, V>(a, t, threadIdx.x % LANES, counts);
+  __threadfence_block();   // the experts are read again by other lanes
+  __syncthreads();
+  begin_experts(a, lds, [&](uint32_t e) { return counts[e]; }, true);
+  place(a, lds, 0, a.n * a.n_chosen, [](uint32_t) { return 0u; });
+}
+
+// What one block does in less time than three launches take.
+constexpr uint32_t kFewTokens = 128;
+
+template <class T, int LANES, int V>
 void route_launch(hipStream_t s, const RouteArgs& a) {
-  hipLaunchKernelGGL((route_choose_kernel<T, LANES, V>), dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
+  if (a.n <= kFewTokens) hipLaunchKernelGGL((route_few_kernel<T, LANES, V>), dim3(1), dim3(kRouteBlock), 0, s, a);
+  else hipLaunchKernelGGL((route_choose_kernel<T, LANES, V>), dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
 }
 
 template <class T>
 int route_typed(hipStream_t s, RouteArgs a) {
-  if (a.n > 0) {
-    const uint32_t e = a.n_experts;
-    if (e <= 16) route_launch<T, 16, 1>(s, a);
-    else if (e <= 32) route_launch<T, 16, 2>(s, a);
-    else if (e <= 64) route_launch<T, 16, 4>(s, a);
-    else if (e <= 128) route_launch<T, 16, 8>(s, a);
-    else if (e <= 256) route_launch<T, 64, 4>(s, a);
-    else if (e <= 512) route_launch<T, 64, 8>(s, a);
-    else route_launch<T, 64, 16>(s, a);
+  const uint32_t e = a.n_experts;
+  if (e <= 16) route_launch<T, 16, 1>(s, a);
+  else if (e <= 32) route_launch<T, 16, 2>(s, a);
+  else if (e <= 64) route_launch<T, 16, 4>(s, a);
+  else if (e <= 128) route_launch<T, 16, 8>(s, a);
+  else if (e <= 256) route_launch<T, 64, 4>(s, a);
+  else if (e <= 512) route_launch<T, 64, 8>(s, a);
+  else route_launch<T, 64, 16>(s, a);
+  if (a.n > kFewTokens) {
+    hipLaunchKernelGGL(route_scan_kernel, dim3(a.n_experts + 1), dim3(kRouteBlock), 0, s, a);
+    hipLaunchKernelGGL(route_place_kernel, dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
   }
-  hipLaunchKernelGGL(route_scan_kernel, dim3(a.n_experts + 1), dim3(64), 0, s, a);
-  hipLaunchKernelGGL(route_place_kernel, dim3(std::max(a.blocks, 1u)), dim3(kRouteBlock), 0, s, a);
-  note_kernel("route");
+  note_kernel(a.n <= kFewTokens ? "route_few" : "route");
   return after_launch(s);
 }
 
@@ -268,40 +344,92 @@ struct RouteGradientArgs {
   bool renormalize;
 };
 
-// A wave to a token: lane j holds its j-th choice.
+// 16 bytes of a row to a lane: the ones at its place, or the row's last ones if those would pass its end; rows shorter than
+// that element by element.
 template <class T>
-__global__ void __launch_bounds__(kRouteBlock) route_gradient_kernel(const RouteGradientArgs a) {
-  const uint32_t lane = threadIdx.x & 63, waves = gridDim.x * (kRouteBlock / 64);
-  for (uint32_t token = (blockIdx.x * kRouteBlock + threadIdx.x) >> 6; token < a.n; token += waves) {
-  const int64_t at = (int64_t)token * a.n_chosen + lane;
-  const bool in = lane < a.n_chosen;
-  const int32_t expert = in ? a.experts[at] : -1;
-  const T weight = in ? static_cast<const T*>(a.weights)[at] : T(0);
-  const T dw = in ? static_cast<const T*>(a.weights_gradient)[at] : T(0);
-  T common = expert >= 0 ? weight * dw : T(0);
+struct RowPart {
+  static constexpr uint32_t N = Quad<T>::N;
+  uint32_t place, start, width;
+  __device__ __forceinline__ RowPart(uint32_t place, uint32_t width) : place(place), start(width >= N ? min(place, width - N) : 0), width(width) {}
+  __device__ __forceinline__ bool owns(uint32_t e) const { return start + e >= place && (width >= N || e < width); }
+  template <bool kStreaming> __device__ __forceinline__ Quad<T> load(const T* row) const {
+    if (width >= N) return load_quad<kStreaming>(row + start);
+    Quad<T> q;
 #pragma unroll
-  for (int m = 32; m > 0; m >>= 1) common += __shfl_xor(common, m);
-  const T taken = a.renormalize ? weight * (dw - common) : weight * dw;
-  T* to = static_cast<T*>(a.logits_gradient) + (int64_t)token * a.gradient_colstride;
-  const T* row = static_cast<const T*>(a.logits) + (int64_t)token * a.colstride;
-  const int32_t first = __shfl(expert, 0);
-  const T first_weight = __shfl(weight, 0);
-  const bool any = first >= 0 && (uint32_t)first < a.n_experts;
-  const T top = any && !a.renormalize ? row[first] : T(0);
-  for (uint32_t e0 = 0; e0 < a.n_experts; e0 += 64) {
-    const uint32_t e = e0 + lane;
-    const bool is = e < a.n_experts;
-    T d = 0;
-    // the largest logit's weight is one over the sum of all powers
-    if (!a.renormalize && any && is) d = -common * (first_weight * (T)exp(row[e] - top));
-    for (uint32_t j = 0; j < a.n_chosen; ++j) {
-      const int32_t chosen = __shfl(expert, j);
-      const T of = __shfl(taken, j);
-      if (chosen == (int32_t)e) d += of;
+    for (uint32_t e = 0; e < N; ++e) q.v[e] = row[min(e, width - 1)];
+    return q;
+  }
+  template <bool kStreaming> __device__ __forceinline__ void store(T* row, const Quad<T>& q) const {
+    if (place + N <= width) {
+      store_quad<kStreaming>(row + place, q);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < N; ++e)
+        if (owns(e)) row[start + e] = q.v[e];
     }
-    if (is) to[e] = d;
   }
+};
+
+// LANES lanes to a token, as many as it has choices or more; lane j holds its j-th choice.  The chosen ones' gradients reach the lanes
+// that store them through a row in LDS, zeros elsewhere.
+template <class T, int LANES>
+__global__ void __launch_bounds__(kRouteBlock) route_gradient_kernel(const RouteGradientArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char row_lds[];
+  const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = kRouteBlock / LANES;
+  T* taken_of = reinterpret_cast<T*>(row_lds) + group * a.n_experts;
+  for (uint32_t e = lane; e < a.n_experts; e += LANES) taken_of[e] = 0;
+  const uint32_t rounds = (a.n + gridDim.x * groups - 1) / (gridDim.x * groups);
+  for (uint32_t i = 0; i < rounds; ++i) {
+    const uint32_t unit = (i * gridDim.x + blockIdx.x) * groups + group, token = min(unit, a.n - 1);   // beyond the last one: not stored
+    const int64_t at = (int64_t)token * a.n_chosen + min(lane, a.n_chosen - 1);
+    const int32_t expert = a.experts[at];
+    const bool in = lane < a.n_chosen && expert >= 0 && (uint32_t)expert < a.n_experts;
+    const T weight = static_cast<const T*>(a.weights)[at];
+    const T dw = static_cast<const T*>(a.weights_gradient)[at];
+    T common = in ? weight * dw : T(0);
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) common += __shfl_xor(common, m);
+    if (in) taken_of[expert] = a.renormalize ? weight * (dw - common) : weight * dw;
+    __threadfence_block();
+    __builtin_amdgcn_wave_barrier();   // a token's lanes are one wave's
+    const int32_t first = __shfl(expert, 0, LANES);
+    const T first_weight = __shfl(weight, 0, LANES);
+    const bool any = first >= 0 && (uint32_t)first < a.n_experts;
+    const T* row = static_cast<const T*>(a.logits) + (int64_t)token * a.colstride;
+    const T top = any && !a.renormalize ? row[first] : T(0);
+    T* to = static_cast<T*>(a.logits_gradient) + (int64_t)token * a.gradient_colstride;
+    for (uint32_t place = lane * Quad<T>::N; place < a.n_experts; place += LANES * Quad<T>::N) {
+      const RowPart<T> part(place, a.n_experts);
+      Quad<T> q;
+#pragma unroll
+      for (uint32_t e = 0; e < Quad<T>::N; ++e) q.v[e] = taken_of[min(part.start + e, a.n_experts - 1)];
+      if (!a.renormalize && any) {
+        const Quad<T> x = part.template load<false>(row);
+        // the largest logit's weight is one over the sum of all powers
+#pragma unroll
+        for (uint32_t e = 0; e < Quad<T>::N; ++e) q.v[e] -= common * (first_weight * (T)exp(x.v[e] - top));
+      }
+      if (unit < a.n) part.template store<false>(to, q);
+    }
+    __threadfence_block();
+    __builtin_amdgcn_wave_barrier();
+    if (in) taken_of[expert] = 0;
   }
+}
+
+template <class T>
+void route_gradient_launch(hipStream_t s, const RouteGradientArgs& a) {
+  constexpr uint32_t N = Quad<T>::N;
+  const uint32_t lanes = std::max((a.n_experts + N - 1) / N, a.n_chosen);
+  auto launch = [&](auto of_lanes) {
+    constexpr uint32_t L = decltype(of_lanes)::value, kGroups = kRouteBlock / L;
+    const uint32_t blocks = (uint32_t)std::min<int64_t>((a.n + kGroups - 1) / kGroups, 2048);
+    hipLaunchKernelGGL((route_gradient_kernel<T, L>), dim3(blocks), dim3(kRouteBlock), kGroups * a.n_experts * sizeof(T), s, a);
+  };
+  if (lanes <= 8) launch(std::integral_constant<uint32_t, 8>());
+  else if (lanes <= 16) launch(std::integral_constant<uint32_t, 16>());
+  else if (lanes <= 32) launch(std::integral_constant<uint32_t, 32>());
+  else launch(std::integral_constant<uint32_t, 64>());
 }
 
 // ------------------------------------------------------------------ combining
@@ -329,32 +457,6 @@ template <class T> __device__ __forceinline__ T from_lane(T x, uint32_t lane) {
     return __builtin_bit_cast(T, low | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane) << 32);
   }
 }
-
-// 16 bytes of a row to a lane: the ones at its place, or the row's last ones if those would pass its end; rows shorter than
-// that element by element.
-template <class T>
-struct RowPart {
-  static constexpr uint32_t N = Quad<T>::N;
-  uint32_t place, start, width;
-  __device__ __forceinline__ RowPart(uint32_t place, uint32_t width) : place(place), start(width >= N ? min(place, width - N) : 0), width(width) {}
-  __device__ __forceinline__ bool owns(uint32_t e) const { return start + e >= place && (width >= N || e < width); }
-  template <bool kStreaming> __device__ __forceinline__ Quad<T> load(const T* row) const {
-    if (width >= N) return load_quad<kStreaming>(row + start);
-    Quad<T> q;
-#pragma unroll
-    for (uint32_t e = 0; e < N; ++e) q.v[e] = row[min(e, width - 1)];
-    return q;
-  }
-  template <bool kStreaming> __device__ __forceinline__ void store(T* row, const Quad<T>& q) const {
-    if (place + N <= width) {
-      store_quad<kStreaming>(row + place, q);
-    } else {
-#pragma unroll
-      for (uint32_t e = 0; e < N; ++e)
-        if (owns(e)) row[start + e] = q.v[e];
-    }
-  }
-};
 
 // A wave to a run of tokens and 64 x 16 bytes of their rows.  The slots and weights of up to 64 assignments are one load of the
 // wave's, and the rows of kRowsAhead assignments are on their way together, whichever tokens they are of: waves that took a
@@ -595,14 +697,16 @@ int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* off
   a.colstride = logits_colstride;
   a.n = (uint32_t)n; a.n_experts = (uint32_t)n_experts; a.n_chosen = (uint32_t)n_chosen;
   a.renormalize = renormalize != 0;
-  // 64 tokens to a block, more where the blocks' counts would take more than 8 MiB
-  const int64_t most_blocks = std::max<int64_t>(1, (int64_t(2) << 20) / (n_experts + 1));
-  a.tokens_per_block = (uint32_t)std::max<int64_t>(64, (n + most_blocks - 1) / most_blocks);
-  a.blocks = (uint32_t)((n + a.tokens_per_block - 1) / a.tokens_per_block);
-  void* scratch = nullptr;
-  if (int rc = stream_scratch(s, ((size_t)a.blocks + 1) * (n_experts + 1) * sizeof(int32_t), &scratch)) return rc;
-  a.totals = static_cast<int32_t*>(scratch);
-  a.counts = a.totals + n_experts + 1;
+  if (n > kFewTokens) {
+    // 64 tokens to a block, more where the blocks' counts would take more than 8 MiB
+    const int64_t most_blocks = std::max<int64_t>(1, (int64_t(2) << 20) / (n_experts + 1));
+    a.tokens_per_block = (uint32_t)std::max<int64_t>(64, (n + most_blocks - 1) / most_blocks);
+    a.blocks = (uint32_t)((n + a.tokens_per_block - 1) / a.tokens_per_block);
+    void* scratch = nullptr;
+    if (int rc = stream_scratch(s, ((size_t)a.blocks + 1) * (n_experts + 1) * sizeof(int32_t), &scratch)) return rc;
+    a.totals = static_cast<int32_t*>(scratch);
+    a.counts = a.totals + n_experts + 1;
+  }
   return dtype == CT_F32 ? route_typed<float>(s, a) : route_typed<double>(s, a);
 }
 
@@ -623,9 +727,8 @@ int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logit
   hipStream_t s = static_cast<hipStream_t>(stream);
   const RouteGradientArgs a{logits_gradient, weights_gradient, weights, experts, logits, logits_gradient_colstride,
                             logits_colstride, (uint32_t)n, (uint32_t)n_experts, (uint32_t)n_chosen, renormalize != 0};
-  const dim3 grid((uint32_t)std::min<int64_t>((n + kRouteBlock / 64 - 1) / (kRouteBlock / 64), kMostBlocks));
-  if (dtype == CT_F32) hipLaunchKernelGGL((route_gradient_kernel<float>), grid, dim3(kRouteBlock), 0, s, a);
-  else hipLaunchKernelGGL((route_gradient_kernel<double>), grid, dim3(kRouteBlock), 0, s, a);
+  if (dtype == CT_F32) route_gradient_launch<float>(s, a);
+  else route_gradient_launch<double>(s, a);
   note_kernel("route_gradient");
   return after_launch(s);
 }

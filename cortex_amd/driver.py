@@ -24,7 +24,6 @@ indirectly addressed dimension.
 """
 from __future__ import annotations
 
-import array
 import ctypes as C
 import os
 from typing import Optional, Sequence
@@ -564,14 +563,10 @@ class HipStream:
                   int(rows_colstride), _ptr(weights), slots.ptr, int(n), int(n_chosen), int(width),
                   capi.DTYPE_CODES[output_gradient.datatype])
 
-    def clip_gradients(self, gradients, outputs, max_norm, norm_and_factor) -> None:
-        """``gradients`` and ``outputs`` (or None) are lists of buffers."""
-        addresses = array.array("Q", [b.ptr for b in gradients])
-        into = None if outputs is None else array.array("Q", [b.ptr for b in outputs])
-        counts = array.array("q", [b._ecount for b in gradients])
-        capi.call("ct_clip_gradients", self.handle, addresses.buffer_info()[0], None if into is None else into.buffer_info()[0],
-                  counts.buffer_info()[0], len(addresses), float(max_norm), norm_and_factor.ptr,
-                  capi.DTYPE_CODES[norm_and_factor.datatype])
+    def clip_gradients(self, gradients, counts, outputs, max_norm, norm_and_factor) -> None:
+        """``gradients`` and ``outputs`` (or None) hold device addresses, ``counts`` lengths: bytes of eight to each."""
+        capi.call("ct_clip_gradients", self.handle, gradients, outputs, counts, len(counts) // 8, float(max_norm),
+                  norm_and_factor.ptr, capi.DTYPE_CODES[norm_and_factor.datatype])
 
     # -- optimizers ---------------------------------------------------------
     def adam_step(self, alpha, beta1, beta2, epsilon, pow_beta1_t, pow_beta2_t, gradient_alpha, gradient, parameters,

@@ -11,7 +11,10 @@ four calls of the tensor API.
 """
 from __future__ import annotations
 
+import array
 import dataclasses
+
+from . import capi
 
 
 def adam(**kwargs) -> dict:
@@ -153,22 +156,34 @@ def clip_gradients(backend: Backend, gradients, max_norm, norm_and_factor, outpu
     is formed.  ``norm_and_factor`` holds two values on the device, so that nothing waits for the host.  The reference's
     gradients are sums over a batch that an optimizer multiplies by its gradient-alpha: a limit for their mean is the
     batch's size times as much.  No counterpart in the reference."""
-    gradients = [_dense_buffer(g) for g in gradients]
-    if outputs is not None:
-        outputs = [_dense_buffer(o) for o in outputs]
-        if [o.ecount() for o in outputs] != [g.ecount() for g in gradients]:
-            raise ValueError("clip_gradients: outputs and gradients differ in their lengths")
-        if any(a.partially_alias(b) for a, b in zip(outputs, gradients)):
-            raise ValueError("clip_gradients: an output overlaps its gradient")
-    elif in_place:
-        outputs = gradients
     result = _dense_buffer(norm_and_factor)
     if result.ecount() != 2:
         raise ValueError("clip_gradients: the norm and the factor are two values")
     if not float(max_norm) > 0:
         raise ValueError(f"clip_gradients: max_norm must be positive, got {max_norm}")
-    _ensure_datatype(backend.datatype, result, *gradients, *(outputs or ()))
-    backend.stream.clip_gradients(gradients, outputs, max_norm, result)
+    at, counts, datatype = _addresses(gradients, backend.datatype)
+    into = at if in_place else None
+    if outputs is not None:
+        into, of_outputs, other = _addresses(outputs, backend.datatype)
+        if of_outputs != counts:
+            raise ValueError("clip_gradients: outputs and gradients differ in their lengths")
+        if other != datatype:
+            raise TypeError(f"Buffer datatype mismatch: expected {backend.datatype}, got {[datatype, other]}")
+    _ensure_datatype(backend.datatype, result)
+    if datatype != backend.datatype:
+        raise TypeError(f"Buffer datatype mismatch: expected {backend.datatype}, got {datatype}")
+    backend.stream.clip_gradients(at, counts, into, max_norm, result)
+
+
+def _addresses(tensors, datatype):
+    """(device addresses, lengths, datatype) of buffers or dense tensors: bytes of eight to each of the first two."""
+    if capi.front is not None:
+        found = capi.front.addresses(tensors)    # 0.2 us to a tensor, 1 us here
+        if found is not None:
+            return found
+    buffers = [_dense_buffer(x) for x in tensors]
+    _ensure_datatype(datatype, *buffers)
+    return (array.array("Q", [b.ptr for b in buffers]).tobytes(), array.array("q", [b.ecount() for b in buffers]).tobytes(), datatype)
 
 
 def create_optimizer(backend: Backend, optimizer: dict):
