@@ -338,12 +338,15 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) grouped_weights_split_kernel(
 
 // ------------------------------------------------------------------ float, a few rows to a group
 
-// What a few tokens ask of their experts is bound by reading the matrices: a block owns 16 rows by 64 columns, its W waves take
-// every W-th run of 32 k each, straight from memory into the fragments, and their sums are added in LDS in their order.  The
-// rows are split once for 64 columns.  Of a matrix stored [k][n] a lane takes four columns side by side.
-template <int W, bool kB>
-__global__ void __launch_bounds__(64 * W, 2) grouped_thin_kernel(const GroupedArgs a, const GroupedPlan p) {
-  constexpr uint32_t BM = 16, BN = 64, BK = 32, NT = BN / 16;
+// What a few tokens ask of their experts is bound by reading the matrices: a block owns 16 rows by 16 NT columns, its W waves
+// take every W-th run of 32 k each, straight from memory into the operands of v_mfma_f32_16x16x4_f32, and their sums are added in LDS in
+// their order.  That instruction is a sixteenth as fast as those of the split products, but takes the floats as they are: 537 MB
+// of 32 matrices, 4096 by 1024, one row each, in 128 us with split products, of which the splitting took what reading left (94 us with
+// nothing but the loads).  Of a matrix stored [k][n] a lane takes its NT columns side by side.
+template <int W, int NT, bool kB>
+__global__ void __launch_bounds__(64 * W, 4) grouped_thin_kernel(const GroupedArgs a, const GroupedPlan p) {
+  constexpr uint32_t BM = 16, BN = 16 * NT, BK = 32;
+  static_assert(NT == 1 || NT == 4, "loads of one column or four");
   __shared__ float partial[W][BM * BN];
   uint32_t m_tile, n_tile;
   Group g;
@@ -351,117 +354,88 @@ __global__ void __launch_bounds__(64 * W, 2) grouped_thin_kernel(const GroupedAr
   const uint32_t row0 = g.tile * BM, col0 = n_tile * BN, lane = threadIdx.x & 63, at16 = lane % 16, quarter = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k_end = a.k;
   const uint32_t row = g.first + min(row0 + at16, g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
-  const bool absent = from >= a.a_rows;
+  const bool absent = from >= a.a_rows, any_absent = __ballot(absent) != 0;   // an index outside a: zeros in the place of its row
   const float* left = static_cast<const float*>(a.a) + (int64_t)(absent ? 0 : from) * a.lda;
   const float* b = static_cast<const float*>(a.b) + (int64_t)g.index * a.b_stride;
-  // column u of a lane's four
-  auto column_of = [&](uint32_t lane16, uint32_t u) { return col0 + (kB ? u * 16 + lane16 : lane16 * 4 + u); };
+  // column u of a lane's
+  auto column_of = [&](uint32_t lane16, uint32_t u) { return col0 + (kB ? u * 16 + lane16 : lane16 * NT + u); };
   const float* right[kB ? NT : 1];
 #pragma unroll
-  for (uint32_t u = 0; u < (kB ? NT : 1); ++u) right[u] = b + (int64_t)(kB ? min(column_of(at16, u), a.n - 1) : col0) * (kB ? a.ldb : 1);
+  for (int u = 0; u < (kB ? NT : 1); ++u) right[u] = b + (int64_t)(kB ? min(column_of(at16, u), a.n - 1) : col0) * (kB ? a.ldb : 1);
   const bool whole = kB || column_of(at16, NT - 1) < a.n;
-  // eight k of the row and of each column, from k0 + 8 * quarter on
-  auto load = [&](uint32_t k0, f32x4 (&l)[2], f32x4 (&r)[NT][2]) {
+  // eight k from k0 + 8 * quarter on: of a row, of a column, of all columns where they are side by side
+  auto load_eight = [&](const float* from, uint32_t k0, f32x4 (&x)[2]) {
     const uint32_t k = k0 + quarter * 8;
     if (k0 + BK <= k_end) {
-      __builtin_memcpy(&l[0], left + k, 16);
-      __builtin_memcpy(&l[1], left + k + 4, 16);
-      if constexpr (kB) {
-#pragma unroll
-        for (uint32_t u = 0; u < NT; ++u) {
-          __builtin_memcpy(&r[u][0], right[u] + k, 16);
-          __builtin_memcpy(&r[u][1], right[u] + k + 4, 16);
-        }
-      } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-          const float* at = right[0] + (int64_t)(k + e) * a.ldb;
-          f32x4 four;
-          if (whole) __builtin_memcpy(&four, at + at16 * 4, 16);
-          else {
-#pragma unroll
-            for (uint32_t u = 0; u < NT; ++u) four[u] = at[min(column_of(at16, u), a.n - 1) - col0];
-          }
-#pragma unroll
-          for (uint32_t u = 0; u < NT; ++u) r[u][e / 4][e % 4] = four[u];
-        }
-      }
+      __builtin_memcpy(&x[0], from + k, 16);
+      __builtin_memcpy(&x[1], from + k + 4, 16);
     } else {
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) {
-        const bool in = k + e < k_end;
-        const int64_t at = min(k + e, k_end - 1);
-        const float x = left[at];
-        l[e / 4][e % 4] = in ? x : 0.f;
-#pragma unroll
-        for (uint32_t u = 0; u < NT; ++u) {
-          const float y = kB ? right[kB ? u : 0][at] : right[0][at * a.ldb + min(column_of(at16, u), a.n - 1) - col0];
-          r[u][e / 4][e % 4] = in ? y : 0.f;
-        }
+      for (int e = 0; e < 8; ++e) {
+        const float y = from[min(k + e, k_end - 1)];
+        x[e / 4][e % 4] = k + e < k_end ? y : 0.f;
       }
     }
-    if (absent) l[0] = l[1] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  f32x4 sums[2][NT] = {};   // the products of the leading pieces; all others
-  bool found = k_end == 1;   // a product by itself: the floats' is rounded once
-  {
-    const SplitWeights weights;
-    f32x4 l[2], r[NT][2], l_next[2], r_next[NT][2];
-    const uint32_t mine = wave * BK;
-    if (mine < k_end) load(mine, l, r);
-    for (uint32_t k0 = mine; k0 < k_end; k0 += W * BK) {
-      const uint32_t next = k0 + W * BK;
-      if (next < k_end) load(next, l_next, r_next);
-      u32x4 lp[kSplitPieces];
-      split4(l[0], lp, 0, weights);
-      split4(l[1], lp, 4, weights);
+  auto load_columns = [&](uint32_t k0, f32x4 (&r)[NT][2]) {
+    const uint32_t k = k0 + quarter * 8;
 #pragma unroll
-      for (uint32_t u = 0; u < NT; ++u) {
-        u32x4 rp[kSplitPieces];
-        split4(r[u][0], rp, 0, weights);
-        split4(r[u][1], rp, 4, weights);
+    for (int e = 0; e < 8; ++e) {
+      const float* at = right[0] + (int64_t)min(k + e, k_end - 1) * a.ldb;
+      if constexpr (NT == 1) {
+        r[0][e / 4][e % 4] = at[min(column_of(at16, 0), a.n - 1) - col0];
+      } else {
+        f32x4 four;
+        if (whole) __builtin_memcpy(&four, at + at16 * 4, 16);
+        else {
 #pragma unroll
-        for (int i = 0; i < kSplitProducts; ++i) {
-          f32x4& to = sums[i + 1 < kSplitProducts][u];
-          to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lp[kSplitLeft[i]]), __builtin_bit_cast(bf16x8, rp[kSplitRight[i]]), to, 0, 0, 0);
+          for (int u = 0; u < NT; ++u) four[u] = at[min(column_of(at16, u), a.n - 1) - col0];
         }
-      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] = l_next[h];
-#pragma unroll
-        for (uint32_t u = 0; u < NT; ++u) r[u][h] = r_next[u][h];
+        for (int u = 0; u < NT; ++u) r[u][e / 4][e % 4] = four[u];
       }
+    }
+    if (k0 + BK > k_end) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) r[u][e / 4][e % 4] = k + e < k_end ? r[u][e / 4][e % 4] : 0.f;
+    }
+  };
+  auto load_left = [&](uint32_t k0, f32x4 (&l)[2]) {
+    load_eight(left, k0, l);
+    if (any_absent && absent) l[0] = l[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  f32x4 sums[NT] = {}, l[2], l_next[2], r[NT][2];
+  const uint32_t mine = wave * BK;
+  if (mine < k_end) {
+    load_left(mine, l);
+    if constexpr (kB) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) load_eight(right[u], mine, r[u]);
+    } else {
+      load_columns(mine, r);
     }
   }
-  auto put_partial = [&](uint32_t u, int e, float value) { partial[wave][(quarter * 4 + e) * BN + column_of(at16, u) - col0] = value; };
+  for (uint32_t k0 = mine; k0 < k_end; k0 += W * BK) {
+    const uint32_t next = k0 + W * BK;
+    if (next < k_end) load_left(next, l_next);
 #pragma unroll
-  for (uint32_t u = 0; u < NT; ++u)
+    for (int u = 0; u < NT; ++u) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float sum = sums[0][u][e] + sums[1][u][e];
-      found |= not_finite(sum);
-      put_partial(u, e, sum * kSplitUnscale);
+      for (int e = 0; e < 8; ++e) sums[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e / 4][e % 4], r[u][e / 4][e % 4], sums[u], 0, 0, 0);
+      // the column's next run into the registers of this one
+      if (kB && next < k_end) load_eight(right[kB ? u : 0], next, r[u]);
     }
-  if (__syncthreads_or(found)) {
-    f32x4 total[NT] = {};
-    for (uint32_t k0 = wave * BK; k0 < k_end; k0 += W * BK) {
-      f32x4 l[2], r[NT][2];
-      load(k0, l, r);
-#pragma unroll
-      for (uint32_t u = 0; u < NT; ++u) {
-        f32x4 sum = {};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e / 4][e % 4], r[u][e / 4][e % 4], sum, 0, 0, 0);
-        total[u] += sum;
-      }
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < NT; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) put_partial(u, e, total[u][e]);
-    __syncthreads();
+    if (!kB && next < k_end) load_columns(next, r);
+    l[0] = l_next[0];
+    l[1] = l_next[1];
   }
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) partial[wave][(quarter * 4 + e) * BN + column_of(at16, u) - col0] = sums[u][e];
+  __syncthreads();
   float* c = static_cast<float*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
   const uint32_t rows = g.rows - row0, columns = a.n - col0;
   for (uint32_t i = threadIdx.x; i < BM * BN; i += 64 * W) {
@@ -668,14 +642,19 @@ GroupedPlan plan_of(int64_t m_tiles, int64_t n_tiles) {
 }
 
 // Microseconds of `blocks` tiles of 64 or of 128 a side over k_tiles of 32 k: the lines of ct_gemm's kernels.
+constexpr int64_t kUnits = 256;
 double time_of_medium(int64_t blocks, int64_t k_tiles) {
-  constexpr int64_t kUnits = 256;
   const int64_t full = blocks / (3 * kUnits), rest = blocks - full * 3 * kUnits, shared = full * 3 + ceil_div(rest, kUnits);
   return 3.3 + 1.3 * (double)shared + (double)k_tiles * (0.31 * (double)(full + (rest > 0)) + 0.33 * (double)shared);
 }
 double time_of_large(int64_t blocks, int64_t k_tiles) { return 1.8 + (double)ceil_div(blocks, 256) * (3.7 + 1.19 * (double)k_tiles); }
+// Of the kernel for a few rows, blocks of 64 and of 16 columns.
+double time_of_thin64(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, kUnits) * (0.5 + 0.28 * (double)k_tiles); }
+double time_of_thin16(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, 2 * kUnits) * (0.5 + 0.22 * (double)k_tiles); }
 
-constexpr int64_t kThinRows = 16;   // of a group, in the mean, that the thin kernel takes
+// Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
+// from 1024 on eight or sixteen are as fast or faster.
+constexpr int64_t kFewK = 768;
 constexpr int64_t kMostUnits = int64_t(1) << 22, kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
 
 uint32_t tiles_of(int64_t n, int64_t side) { return (uint32_t)((n + side - 1) / side); }
@@ -732,37 +711,34 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
       return after_launch(s);
     }
   }
-  if (dtype == CT_F32 && a_row_count > 0 && a_col_count > 0 && (a_col_count < kTileDepth || row_count <= kThinRows * even_groups)) {
-    const int64_t m_tiles = row_count / 16 + even_groups, n_tiles = ceil_div(b_col_count, 64);
+  if (dtype == CT_F32 && a_row_count > 0 && a_col_count > 0) {
+    // The tiles that there are if the groups are even, and the kernel that takes them soonest.  With 4096 by 1024 [n][k] and 8 groups,
+    // us with 16 columns to a block, 64, and tiles of 64 and 128 a side: of one row 28, 34, 88 and 151; of 32 rows 60, 40, 88 and 153; of
+    // 128 rows 228, 145, 89 and 150; with 32 groups of 128 rows 910, 568, 286 and 217.
+    const int64_t k_tiles = ceil_div(a_col_count, kTileDepth), mean = row_count / even_groups;
+    const int64_t thin_tiles = even_groups * ceil_div(mean, 16);
+    const double thin64 = time_of_thin64(thin_tiles * ceil_div(b_col_count, 64), k_tiles);
+    const double thin16 = time_of_thin16(thin_tiles * ceil_div(b_col_count, 16), k_tiles);
+    const double medium = time_of_medium(even_groups * ceil_div(mean, 64) * ceil_div(b_col_count, 64), k_tiles);
+    const double large = time_of_large(even_groups * ceil_div(mean, 128) * ceil_div(b_col_count, 128), k_tiles);
+    const bool split = a_col_count >= kTileDepth && b_colstride <= kMostSplitLd;
+    const bool thin = !split || std::min(thin64, thin16) < std::min(medium, large);
+    const int64_t height = thin ? 16 : large < medium ? 128 : 64, width = !thin ? height : thin16 < thin64 ? 16 : 64;
+    const int64_t m_tiles = row_count / height + even_groups, n_tiles = ceil_div(b_col_count, width);
     if (m_tiles * n_tiles <= kMostUnits) {
       const GroupedPlan p = plan_of(m_tiles, n_tiles);
-      const bool few = a_col_count <= 256;
-      if (few && trans_b) hipLaunchKernelGGL((grouped_thin_kernel<4, true>), grid_of(p), dim3(256), 0, s, g, p);
-      else if (few) hipLaunchKernelGGL((grouped_thin_kernel<4, false>), grid_of(p), dim3(256), 0, s, g, p);
-      else if (trans_b) hipLaunchKernelGGL((grouped_thin_kernel<8, true>), grid_of(p), dim3(512), 0, s, g, p);
-      else hipLaunchKernelGGL((grouped_thin_kernel<8, false>), grid_of(p), dim3(512), 0, s, g, p);
-      note_kernel("grouped_thin");
-      return after_launch(s);
-    }
-  }
-  if (dtype == CT_F32 && a_col_count >= kTileDepth && a_row_count > 0 && b_colstride <= kMostSplitLd) {
-    // the tiles that there are if the groups are even
-    const int64_t even = std::min(n_groups, row_count), k_tiles = ceil_div(a_col_count, kTileDepth), side = row_count / even;
-    const double medium = time_of_medium(even * ceil_div(side, 64) * ceil_div(b_col_count, 64), k_tiles);
-    const double large = time_of_large(even * ceil_div(side, 128) * ceil_div(b_col_count, 128), k_tiles);
-    const int64_t height = large < medium ? 128 : 64;
-    const int64_t m_tiles = row_count / height + even, n_tiles = ceil_div(b_col_count, height);
-    if (m_tiles * n_tiles <= kMostUnits) {
-      const GroupedPlan p = plan_of(m_tiles, n_tiles);
-      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
-      if (height == 128) {
-        if (trans_b) hipLaunchKernelGGL((grouped_split_kernel<128, 128, 2, 4, true>), grid, dim3(512), 0, s, g, p);
-        else hipLaunchKernelGGL((grouped_split_kernel<128, 128, 2, 4, false>), grid, dim3(512), 0, s, g, p);
-      } else {
-        if (trans_b) hipLaunchKernelGGL((grouped_split_kernel<64, 64, 2, 2, true>), grid, dim3(256), 0, s, g, p);
-        else hipLaunchKernelGGL((grouped_split_kernel<64, 64, 2, 2, false>), grid, dim3(256), 0, s, g, p);
-      }
-      note_kernel(height == 128 ? "grouped_large" : "grouped_medium");
+      auto launch = [&](auto of_b, auto of_not_b, int waves) {
+        if (trans_b) hipLaunchKernelGGL(of_b, grid_of(p), dim3(64 * waves), 0, s, g, p);
+        else hipLaunchKernelGGL(of_not_b, grid_of(p), dim3(64 * waves), 0, s, g, p);
+      };
+      const bool few = a_col_count <= kFewK;
+      if (thin && width == 64 && few) launch(grouped_thin_kernel<4, 4, true>, grouped_thin_kernel<4, 4, false>, 4);
+      else if (thin && width == 64) launch(grouped_thin_kernel<8, 4, true>, grouped_thin_kernel<8, 4, false>, 8);
+      else if (thin && few) launch(grouped_thin_kernel<4, 1, true>, grouped_thin_kernel<4, 1, false>, 4);
+      else if (thin) launch(grouped_thin_kernel<16, 1, true>, grouped_thin_kernel<16, 1, false>, 16);
+      else if (height == 128) launch(grouped_split_kernel<128, 128, 2, 4, true>, grouped_split_kernel<128, 128, 2, 4, false>, 8);
+      else launch(grouped_split_kernel<64, 64, 2, 2, true>, grouped_split_kernel<64, 64, 2, 2, false>, 4);
+      note_kernel(thin ? "grouped_thin" : height == 128 ? "grouped_large" : "grouped_medium");
       return after_launch(s);
     }
   }
