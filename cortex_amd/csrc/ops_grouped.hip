@@ -5,6 +5,7 @@
 // tiles of all rows and one more to each group.  A block finds its group by adding up the groups' tiles; blocks beyond the
 // last tile end.  Offsets are clamped as they are read, so that no content of theirs leads outside a buffer.
 #include <algorithm>
+#include <optional>
 
 #include "common.h"
 #include "rows.h"
@@ -21,9 +22,10 @@ struct GroupedArgs {
   const int32_t* index_a;
   const int32_t* index_b;
   const int32_t* offsets;
-  int64_t lda, ldb, ldc, b_stride, c_stride;
+  int64_t lda, ldb, ldc, b_stride, c_stride, c_split;   // c_split: between the results of a launch's parts of k
   double alpha, beta;
   uint32_t groups, rows, a_rows, b_rows, m, n, k;   // m, k: of the weights' products only where rows are not
+  uint32_t part;   // k of a part
   bool trans_b;
 };
 
@@ -142,23 +144,30 @@ __global__ void __launch_bounds__(256) grouped_weights_kernel(const GroupedArgs 
 
 // ------------------------------------------------------------------ float: the matrix cores, three pieces to a float
 
-// Tiles in bands of kBand rows, column after column, dealt to the dies in runs of kRun: what a die works on at a time is as
-// square as it can be and mostly of one group, and each die has a part of every group.
+// Tiles in bands of kBand rows, column after column, part of k after part, dealt to the dies in runs: what a die works on at a
+// time is as square as it can be and mostly of one group, and each die has a part of every group.  Runs of kRun, or as many as
+// give every die one (64 tiles in runs of 16 would leave four dies idle).
 constexpr uint32_t kBand = 8, kRun = 16;
 
 struct GroupedPlan {
-  uint32_t m_tiles, n_tiles, units;   // m_tiles: as many as there can be
-  FastDiv band_fd;
+  uint32_t m_tiles, n_tiles, units, parts, run_shift;   // m_tiles: as many as there can be; units: of all parts
+  FastDiv part_fd, band_fd;
 };
 
-__device__ __forceinline__ bool place_of(const GroupedPlan& p, uint32_t* m_tile, uint32_t* n_tile) {
-  const uint32_t at = blockIdx.x / kXcds, unit = (at / kRun * kXcds + blockIdx.x % kXcds) * kRun + at % kRun;
+struct TilePlace {
+  uint32_t m_tile, n_tile, part;
+};
+
+__device__ __forceinline__ bool place_of(const GroupedPlan& p, TilePlace* out) {
+  const uint32_t at = blockIdx.x / kXcds, run = at >> p.run_shift;
+  uint32_t unit = ((run * kXcds + blockIdx.x % kXcds) << p.run_shift) + (at - (run << p.run_shift));
   if (unit >= p.units) return false;
   uint32_t band, rest;
+  p.part_fd.divmod(unit, out->part, unit);
   p.band_fd.divmod(unit, band, rest);
   const uint32_t rows = min(kBand, p.m_tiles - band * kBand);
-  *n_tile = rest / rows;
-  *m_tile = band * kBand + rest - *n_tile * rows;
+  out->n_tile = rest / rows;
+  out->m_tile = band * kBand + rest - out->n_tile * rows;
   return true;
 }
 
@@ -174,10 +183,10 @@ struct GroupedSource : TileShare<BM, BN, T, true, kB> {
   bool absent[UA], any_absent;   // an index outside a: zeros in the place of its row
   const float* base_b;
   int64_t ldb;
-  uint32_t k;
+  uint32_t k, begin;
   uint32_t offset[UB];
-  __device__ __forceinline__ GroupedSource(const GroupedArgs& a, const Group& g, uint32_t row0, uint32_t col0, uint32_t tid)
-      : Share{tid}, any_absent(false), ldb(a.ldb), k(a.k) {
+  __device__ __forceinline__ GroupedSource(const GroupedArgs& a, const Group& g, uint32_t row0, uint32_t col0, uint32_t begin, uint32_t tid)
+      : Share{tid}, any_absent(false), ldb(a.ldb), k(a.k), begin(begin) {
 #pragma unroll
     for (int i = 0; i < UA; ++i) {
       const uint32_t row = g.first + min(row0 + this->row_of(i), g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
@@ -195,7 +204,7 @@ struct GroupedSource : TileShare<BM, BN, T, true, kB> {
   }
   __device__ __forceinline__ void rewind() {}
   __device__ __forceinline__ void load(int i, uint32_t tile, f32x4 (&to)[2]) const {
-    const int64_t k0 = min(tile * BK, k - BK);
+    const int64_t k0 = min(begin + tile * BK, k - BK);
     if (i < UA) {
       __builtin_memcpy(&to[0], row_a[i] + k0, 16);
       __builtin_memcpy(&to[1], row_a[i] + k0 + 4, 16);
@@ -209,7 +218,7 @@ struct GroupedSource : TileShare<BM, BN, T, true, kB> {
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[e / 4][e % 4] = absent[i] ? 0.f : r[e / 4][e % 4];
     }
-    const uint32_t k0 = tile * BK;
+    const uint32_t k0 = begin + tile * BK;
     if (k0 + BK <= k) return;
     asm volatile("");
     const uint32_t repeated = k0 - (k - BK);
@@ -244,15 +253,23 @@ template <int BM, int BN, int WM, int WN, bool kB>
 __global__ void __launch_bounds__(64 * WM * WN, 2) grouped_split_kernel(const GroupedArgs a, const GroupedPlan p) {
   constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
   __shared__ __attribute__((aligned(16))) uint16_t lds[split_tile_lds(BM, BN)];
-  uint32_t m_tile, n_tile;
+  TilePlace at;
   Group g;
-  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, BM, &g)) return;
-  const uint32_t row0 = g.tile * BM, col0 = n_tile * BN, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  GroupedSource<BM, BN, T, kB> source(a, g, row0, col0, tid);
+  if (!place_of(p, &at) || !find_group(a, at.m_tile, BM, &g)) return;
+  const uint32_t row0 = g.tile * BM, col0 = at.n_tile * BN, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t begin = at.part * a.part, count = min(a.part, a.k - begin);
+  GroupedSource<BM, BN, T, kB> source(a, g, row0, col0, begin, tid);
   float result[MT][NT][16];
-  split_tile<BM, BN, WM, WN>(source, (a.k + 2 * kTileDepth - 1) / (2 * kTileDepth) * 2, lds, tid, result);
-  store_tile(a, static_cast<float*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0, g.rows - row0, a.n - col0, wave / WN * (MT * 32),
+  split_tile<BM, BN, WM, WN>(source, (count + 2 * kTileDepth - 1) / (2 * kTileDepth) * 2, lds, tid, result);
+  store_tile(a, static_cast<float*>(a.c) + at.part * a.c_split + (int64_t)(g.first + row0) * a.ldc + col0, g.rows - row0, a.n - col0, wave / WN * (MT * 32),
              wave % WN * (NT * 32), tid & 63, result);
+}
+
+// The rows of a group whose products a block adds up: an even share, of whole tiles, for each of the parts.
+__device__ __forceinline__ uint2 part_of(uint2 rows, uint32_t part, uint32_t parts) {
+  if (parts == 1) return rows;
+  const uint32_t each = ((rows.y + parts - 1) / parts + 2 * kTileDepth - 1) / (2 * kTileDepth) * (2 * kTileDepth), from = min(part * each, rows.y);
+  return make_uint2(rows.x + from, min(each, rows.y - from));
 }
 
 // Columns of the rows of a group, over which the products' sums run.  A wave loads eight rows at a time: its lanes 0 to 7
@@ -321,18 +338,18 @@ template <int BM, int BN, int WM, int WN, bool kWide>
 __global__ void __launch_bounds__(64 * WM * WN, 2) grouped_weights_split_kernel(const GroupedArgs a, const GroupedPlan p) {
   constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
   __shared__ __attribute__((aligned(16))) uint16_t lds[split_tile_lds(BM, BN)];
-  uint32_t m_tile, n_tile;
-  if (!place_of(p, &m_tile, &n_tile)) return;
-  const uint32_t tiles = (a.m + BM - 1) / BM, group = m_tile / tiles, row0 = (m_tile - group * tiles) * BM, col0 = n_tile * BN;
+  TilePlace at;
+  if (!place_of(p, &at)) return;
+  const uint32_t tiles = (a.m + BM - 1) / BM, group = at.m_tile / tiles, row0 = (at.m_tile - group * tiles) * BM, col0 = at.n_tile * BN;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint2 rows = group_rows(a, group);
+  const uint2 rows = part_of(group_rows(a, group), at.part, p.parts);
   const uint32_t first = __builtin_amdgcn_readfirstlane(rows.x), count = __builtin_amdgcn_readfirstlane(rows.y);
   float result[MT][NT][16] = {};
   if (count > 0 && a.a_rows > 0 && a.b_rows > 0) {
     GroupedWeightsSource<BM, BN, T, kWide> source(a, first, count, row0, col0, tid);
     split_tile<BM, BN, WM, WN>(source, (count + 2 * kTileDepth - 1) / (2 * kTileDepth) * 2, lds, tid, result);
   }
-  store_tile(a, static_cast<float*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0, a.m - row0, a.n - col0,
+  store_tile(a, static_cast<float*>(a.c) + at.part * a.c_split + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0, a.m - row0, a.n - col0,
              wave / WN * (MT * 32), wave % WN * (NT * 32), tid & 63, result);
 }
 
@@ -348,10 +365,10 @@ __global__ void __launch_bounds__(64 * W, 4) grouped_thin_kernel(const GroupedAr
   constexpr uint32_t BM = 16, BN = 16 * NT, BK = 32;
   static_assert(NT == 1 || NT == 4, "loads of one column or four");
   __shared__ float partial[W][BM * BN];
-  uint32_t m_tile, n_tile;
+  TilePlace at;
   Group g;
-  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, BM, &g)) return;
-  const uint32_t row0 = g.tile * BM, col0 = n_tile * BN, lane = threadIdx.x & 63, at16 = lane % 16, quarter = lane / 16;
+  if (!place_of(p, &at) || !find_group(a, at.m_tile, BM, &g)) return;
+  const uint32_t row0 = g.tile * BM, col0 = at.n_tile * BN, lane = threadIdx.x & 63, at16 = lane % 16, quarter = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k_end = a.k;
   const uint32_t row = g.first + min(row0 + at16, g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
   const bool absent = from >= a.a_rows, any_absent = __ballot(absent) != 0;   // an index outside a: zeros in the place of its row
@@ -592,10 +609,10 @@ __device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right rig
 
 template <int S, bool kB>
 __global__ void __launch_bounds__(256, 2) grouped_double_kernel(const GroupedArgs a, const GroupedPlan p) {
-  uint32_t m_tile, n_tile;
+  TilePlace at;
   Group g;
-  if (!place_of(p, &m_tile, &n_tile) || !find_group(a, m_tile, S, &g)) return;
-  const uint32_t row0 = g.tile * S, col0 = n_tile * S;
+  if (!place_of(p, &at) || !find_group(a, at.m_tile, S, &g)) return;
+  const uint32_t row0 = g.tile * S, col0 = at.n_tile * S;
   const double* b = static_cast<const double*>(a.b) + (int64_t)g.index * a.b_stride;
   double* c = static_cast<double*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
   const uint32_t row = g.first + min(row0 + DoubleRow<S>::row(), g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
@@ -614,11 +631,11 @@ __global__ void __launch_bounds__(256, 2) grouped_double_kernel(const GroupedArg
 
 template <int S>
 __global__ void __launch_bounds__(256, 2) grouped_weights_double_kernel(const GroupedArgs a, const GroupedPlan p) {
-  uint32_t m_tile, n_tile;
-  if (!place_of(p, &m_tile, &n_tile)) return;
-  const uint32_t tiles = (a.m + S - 1) / S, group = m_tile / tiles, row0 = (m_tile - group * tiles) * S, col0 = n_tile * S;
-  const uint2 rows = group_rows(a, group);
-  double* c = static_cast<double*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0;
+  TilePlace at;
+  if (!place_of(p, &at)) return;
+  const uint32_t tiles = (a.m + S - 1) / S, group = at.m_tile / tiles, row0 = (at.m_tile - group * tiles) * S, col0 = at.n_tile * S;
+  const uint2 rows = part_of(group_rows(a, group), at.part, p.parts);
+  double* c = static_cast<double*>(a.c) + at.part * a.c_split + (int64_t)group * a.c_stride + (int64_t)row0 * a.ldc + col0;
   auto store = [&](uint32_t r, uint32_t n, double sum) {
     if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
   };
@@ -630,15 +647,96 @@ __global__ void __launch_bounds__(256, 2) grouped_weights_double_kernel(const Gr
   }
 }
 
+// ------------------------------------------------------------------ the parts of k brought together
+
+// partial [parts][c's cells, dense], added in their order: of rows of c (those from the first group's to the last one's only),
+// or of matrices.
+template <class T, bool kWeights>
+__global__ void __launch_bounds__(256) grouped_sum_kernel(const GroupedArgs a, const T* partial, uint32_t parts, uint32_t cells, FastDiv n_fd, FastDiv m_fd) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= cells) return;
+  uint32_t row, column, group = 0;
+  n_fd.divmod(i, row, column);
+  if constexpr (kWeights) {
+    m_fd.divmod(row, group, row);
+  } else {
+    const uint2 last = group_rows(a, a.groups - 1);
+    if (row < group_rows(a, 0).x || row >= last.x + last.y) return;
+  }
+  double sum = 0.0;
+  for (uint32_t s0 = 0; s0 < parts; s0 += 8) {   // loads of eight parts on their way
+    T x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = partial[(int64_t)min(s0 + s, parts - 1) * cells + i];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) sum += s0 + s < parts ? x[s] : T(0);
+  }
+  put(static_cast<T*>(a.c) + (int64_t)group * a.c_stride + (int64_t)row * a.ldc + column, (T)sum, a.alpha, a.beta);
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-GroupedPlan plan_of(int64_t m_tiles, int64_t n_tiles) {
-  GroupedPlan p;
-  p.m_tiles = (uint32_t)m_tiles;
-  p.n_tiles = (uint32_t)n_tiles;
-  p.units = (uint32_t)(m_tiles * n_tiles);
-  p.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
-  return p;
+struct Launch {
+  GroupedPlan plan;
+  dim3 grid;
+};
+
+Launch launch_of(int64_t m_tiles, int64_t n_tiles, int64_t parts) {
+  Launch l;
+  l.plan.m_tiles = (uint32_t)m_tiles;
+  l.plan.n_tiles = (uint32_t)n_tiles;
+  l.plan.units = (uint32_t)(m_tiles * n_tiles * parts);
+  l.plan.parts = (uint32_t)parts;
+  l.plan.run_shift = 0;
+  while ((uint32_t(2) << l.plan.run_shift) <= std::min(kRun, l.plan.units / kXcds)) ++l.plan.run_shift;
+  l.plan.part_fd = FastDiv((uint32_t)(m_tiles * n_tiles));
+  l.plan.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
+  const int64_t round = (int64_t)kXcds << l.plan.run_shift;
+  l.grid = dim3((uint32_t)(ceil_div(l.plan.units, round) * round));
+  return l;
+}
+
+// Sums whose k is divided among blocks: their products go to scratch, and a second launch adds them up.
+template <class T>
+class Parts {
+ public:
+  // As many as asked for, or one where no scratch is to be had: while the stream is being captured, or for want of memory.
+  Parts(hipStream_t s, int64_t parts, int64_t cells) : stream_(s), cells_(cells), count_(1) {
+    if (parts == 1) return;
+    scratch_.emplace(s, (size_t)(parts * cells) * sizeof(T));
+    partial_ = static_cast<T*>(scratch_->get());
+    if (partial_) count_ = parts;
+  }
+  int64_t count() const { return count_; }
+  // Of the first launch; matrices of `m` rows, or none.
+  GroupedArgs args(GroupedArgs a, int64_t m) const {
+    if (!partial_) return a;
+    a.c = partial_;
+    a.ldc = a.n;
+    a.c_stride = m * a.n;
+    a.c_split = cells_;
+    a.alpha = 1.0;
+    a.beta = 0.0;
+    return a;
+  }
+  template <bool kWeights>
+  void add_up(const GroupedArgs& a) const {
+    if (!partial_) return;
+    hipLaunchKernelGGL((grouped_sum_kernel<T, kWeights>), dim3((uint32_t)ceil_div(cells_, 256)), dim3(256), 0, stream_, a, partial_, (uint32_t)count_,
+                       (uint32_t)cells_, FastDiv(a.n), FastDiv(kWeights ? a.m : 1));
+  }
+
+ private:
+  hipStream_t stream_;
+  std::optional<ProductScratch> scratch_;   // until both launches are made
+  T* partial_ = nullptr;
+  int64_t cells_, count_;
+};
+
+// The second launch, and its bytes at 3.3 TB/s; no more than the scratch there may be.
+double time_of_sum(int64_t parts, int64_t cells, int64_t size) {
+  if (parts == 1) return 0.0;
+  return parts * cells * size > (int64_t)kMostProductScratch ? 1e9 : 4.5 + 0.3e-6 * (double)((parts + 1) * cells * size);
 }
 
 // Microseconds of `blocks` tiles of 64 or of 128 a side over k_tiles of 32 k: the lines of ct_gemm's kernels.
@@ -651,6 +749,45 @@ double time_of_large(int64_t blocks, int64_t k_tiles) { return 1.8 + (double)cei
 // Of the kernel for a few rows, blocks of 64 and of 16 columns.
 double time_of_thin64(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, kUnits) * (0.5 + 0.28 * (double)k_tiles); }
 double time_of_thin16(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, 2 * kUnits) * (0.5 + 0.22 * (double)k_tiles); }
+
+struct Choice {
+  int64_t height, width, parts;
+  double us;
+};
+
+// Of k_tiles tiles of k, divided evenly and in pairs of tiles: those of a part.
+int64_t tiles_of_part(int64_t k_tiles, int64_t parts) { return ceil_div(ceil_div(k_tiles, parts), 2) * 2; }
+
+// Tiles of 64 and 128 a side, with k in one part or several, against the best so far.  The times of 64 products of 2 and 8 even groups,
+// 64 to 1024 rows each, k 1024 to 4096: 5 % above the best plan's of each.  Us of one part and of what is chosen: 2 groups of 128 rows,
+// k 4096, n 1024: 89 and 29; 8 groups of 64, k 4096, n 1024: 88 and 52; of the weights' products 8 groups of 4096 rows, 128 by 128: 110 and 47.
+// Blocks of 128 a side write their parts at once, 6 us a round.
+constexpr int64_t kMostParts = 32;
+void consider_parts(Choice* best, int64_t blocks64, int64_t blocks128, int64_t k_tiles, int64_t cells, int64_t most_parts) {
+  for (int64_t parts = 1; parts <= most_parts; parts *= 2) {
+    const int64_t tiles = parts == 1 ? k_tiles : tiles_of_part(k_tiles, parts);
+    if (parts > 1 && tiles * (parts - 1) >= k_tiles) break;   // the last part would have none
+    const double sum = time_of_sum(parts, cells, sizeof(float));
+    const double medium = time_of_medium(blocks64 * parts, tiles) + sum, large = time_of_large(blocks128 * parts, tiles) + sum + (parts > 1 ? 6.0 * (double)ceil_div(blocks128 * parts, kUnits) : 0.0);
+    if (medium < best->us) *best = {64, 64, parts, medium};
+    if (large < best->us) *best = {128, 128, parts, large};
+  }
+}
+
+// The same of double, tiles of 32 and 64 a side: one block's steps over twice the mean k, for groups are seldom even (7 groups of 290
+// rows in the mean, 301 by 517: 35 us in tiles of 32, 56 in tiles of 64, which take 18 where they are even), or those of all blocks.
+double time_of_double(int64_t side, int64_t blocks, int64_t k) {
+  const double b = (double)blocks;
+  return 4.0 + 0.001 * (double)k * (side == 32 ? std::max(2 * 20.0, 13.0 + 0.046 * b) : std::max(2 * 54.0, 15.0 + 0.145 * b));
+}
+void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks64, int64_t k, int64_t cells, int64_t most_parts) {
+  for (int64_t parts = 1; parts <= most_parts && k >= parts * 64; parts *= 2) {
+    const double sum = time_of_sum(parts, cells, sizeof(double));
+    const double small = time_of_double(32, blocks32 * parts, ceil_div(k, parts)) + sum, large = time_of_double(64, blocks64 * parts, ceil_div(k, parts)) + sum;
+    if (small < best->us) *best = {32, 32, parts, small};
+    if (large < best->us) *best = {64, 64, parts, large};
+  }
+}
 
 // Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
 // from 1024 on eight or sixteen are as fast or faster.
@@ -697,16 +834,15 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
   g.n = (uint32_t)b_col_count; g.k = (uint32_t)a_col_count;
   g.trans_b = trans_b != 0;
   const int64_t even_groups = std::min(n_groups, row_count);
-  auto grid_of = [](const GroupedPlan& p) { return dim3((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun)); };
   if (dtype == CT_F64 && a_row_count > 0 && a_col_count > 0) {
     const int64_t tiles64 = (row_count / 64 + even_groups / 2) * ceil_div(b_col_count, 64), side = tiles64 >= 1024 ? 64 : 32;
     const int64_t m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
     if (m_tiles * n_tiles <= kMostUnits) {
-      const GroupedPlan p = plan_of(m_tiles, n_tiles);
-      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), grid_of(p), dim3(256), 0, s, g, p);
-      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), grid_of(p), dim3(256), 0, s, g, p);
-      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), grid_of(p), dim3(256), 0, s, g, p);
-      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), grid_of(p), dim3(256), 0, s, g, p);
+      const Launch l = launch_of(m_tiles, n_tiles, 1);
+      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), l.grid, dim3(256), 0, s, g, l.plan);
+      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), l.grid, dim3(256), 0, s, g, l.plan);
+      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), l.grid, dim3(256), 0, s, g, l.plan);
+      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), l.grid, dim3(256), 0, s, g, l.plan);
       note_kernel("grouped_double");
       return after_launch(s);
     }
@@ -715,30 +851,39 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
     // The tiles that there are if the groups are even, and the kernel that takes them soonest.  With 4096 by 1024 [n][k] and 8 groups,
     // us with 16 columns to a block, 64, and tiles of 64 and 128 a side: of one row 28, 34, 88 and 151; of 32 rows 60, 40, 88 and 153; of
     // 128 rows 228, 145, 89 and 150; with 32 groups of 128 rows 910, 568, 286 and 217.
-    const int64_t k_tiles = ceil_div(a_col_count, kTileDepth), mean = row_count / even_groups;
-    const int64_t thin_tiles = even_groups * ceil_div(mean, 16);
-    const double thin64 = time_of_thin64(thin_tiles * ceil_div(b_col_count, 64), k_tiles);
-    const double thin16 = time_of_thin16(thin_tiles * ceil_div(b_col_count, 16), k_tiles);
-    const double medium = time_of_medium(even_groups * ceil_div(mean, 64) * ceil_div(b_col_count, 64), k_tiles);
-    const double large = time_of_large(even_groups * ceil_div(mean, 128) * ceil_div(b_col_count, 128), k_tiles);
-    const bool split = a_col_count >= kTileDepth && b_colstride <= kMostSplitLd;
-    const bool thin = !split || std::min(thin64, thin16) < std::min(medium, large);
-    const int64_t height = thin ? 16 : large < medium ? 128 : 64, width = !thin ? height : thin16 < thin64 ? 16 : 64;
-    const int64_t m_tiles = row_count / height + even_groups, n_tiles = ceil_div(b_col_count, width);
+    const int64_t k_tiles = ceil_div(a_col_count, kTileDepth), cells = row_count * b_col_count;
+    auto tiles_of = [&](int64_t height) { return even_groups * ceil_div(row_count / even_groups, height); };
+    const double thin64 = time_of_thin64(tiles_of(16) * ceil_div(b_col_count, 64), k_tiles);
+    const double thin16 = time_of_thin16(tiles_of(16) * ceil_div(b_col_count, 16), k_tiles);
+    auto blocks_of = [&](int64_t side) { return tiles_of(side) * ceil_div(b_col_count, side); };
+    auto choose = [&](int64_t most_parts) {
+      Choice best{16, thin16 < thin64 ? 16 : 64, 1, std::min(thin64, thin16)};
+      if (a_col_count >= kTileDepth && b_colstride <= kMostSplitLd) consider_parts(&best, blocks_of(64), blocks_of(128), k_tiles, cells, most_parts);
+      return best;
+    };
+    Choice best = choose(kMostParts);
+    const Parts<float> parts(s, best.parts, cells);
+    if (parts.count() < best.parts) best = choose(1);
+    const bool thin = best.height == 16;
+    const int64_t m_tiles = row_count / best.height + even_groups, n_tiles = ceil_div(b_col_count, best.width);
     if (m_tiles * n_tiles <= kMostUnits) {
-      const GroupedPlan p = plan_of(m_tiles, n_tiles);
+      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
+      GroupedArgs of_parts = parts.args(g, 0);
+      of_parts.part = (uint32_t)(tiles_of_part(k_tiles, parts.count()) * kTileDepth);
       auto launch = [&](auto of_b, auto of_not_b, int waves) {
-        if (trans_b) hipLaunchKernelGGL(of_b, grid_of(p), dim3(64 * waves), 0, s, g, p);
-        else hipLaunchKernelGGL(of_not_b, grid_of(p), dim3(64 * waves), 0, s, g, p);
+        if (trans_b) hipLaunchKernelGGL(of_b, l.grid, dim3(64 * waves), 0, s, of_parts, l.plan);
+        else hipLaunchKernelGGL(of_not_b, l.grid, dim3(64 * waves), 0, s, of_parts, l.plan);
       };
       const bool few = a_col_count <= kFewK;
-      if (thin && width == 64 && few) launch(grouped_thin_kernel<4, 4, true>, grouped_thin_kernel<4, 4, false>, 4);
-      else if (thin && width == 64) launch(grouped_thin_kernel<8, 4, true>, grouped_thin_kernel<8, 4, false>, 8);
+      if (thin && best.width == 64 && few) launch(grouped_thin_kernel<4, 4, true>, grouped_thin_kernel<4, 4, false>, 4);
+      else if (thin && best.width == 64) launch(grouped_thin_kernel<8, 4, true>, grouped_thin_kernel<8, 4, false>, 8);
       else if (thin && few) launch(grouped_thin_kernel<4, 1, true>, grouped_thin_kernel<4, 1, false>, 4);
       else if (thin) launch(grouped_thin_kernel<16, 1, true>, grouped_thin_kernel<16, 1, false>, 16);
-      else if (height == 128) launch(grouped_split_kernel<128, 128, 2, 4, true>, grouped_split_kernel<128, 128, 2, 4, false>, 8);
+      else if (best.height == 128) launch(grouped_split_kernel<128, 128, 2, 4, true>, grouped_split_kernel<128, 128, 2, 4, false>, 8);
       else launch(grouped_split_kernel<64, 64, 2, 2, true>, grouped_split_kernel<64, 64, 2, 2, false>, 4);
-      note_kernel(thin ? "grouped_thin" : height == 128 ? "grouped_large" : "grouped_medium");
+      parts.add_up<false>(g);
+      static const char* const kNames[] = {"grouped_medium", "grouped_large", "grouped_medium+grouped_sum", "grouped_large+grouped_sum"};
+      note_kernel(thin ? "grouped_thin" : kNames[(best.height == 128) + 2 * (parts.count() > 1)]);
       return after_launch(s);
     }
   }
@@ -779,32 +924,49 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
   g.alpha = alpha; g.beta = beta;
   g.groups = (uint32_t)n_groups; g.rows = (uint32_t)row_count; g.a_rows = (uint32_t)a_row_count; g.b_rows = (uint32_t)b_row_count;
   g.m = (uint32_t)a_col_count; g.n = (uint32_t)b_col_count;
+  const int64_t cells = n_groups * a_col_count * b_col_count, mean = std::max<int64_t>(row_count / n_groups, 1);
+  auto blocks_of = [&](int64_t side) { return n_groups * ceil_div(a_col_count, side) * ceil_div(b_col_count, side); };
   if (dtype == CT_F32 && std::max(a_colstride, b_colstride) <= kMostWeightsLd) {
-    const int64_t k_tiles = ceil_div(std::max<int64_t>(row_count / n_groups, 1), kTileDepth);
-    const double medium = time_of_medium(n_groups * ceil_div(a_col_count, 64) * ceil_div(b_col_count, 64), k_tiles);
-    const double large = time_of_large(n_groups * ceil_div(a_col_count, 128) * ceil_div(b_col_count, 128), k_tiles);
-    const int64_t side = large < medium ? 128 : 64, m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
+    auto choose = [&](int64_t most_parts) {
+      Choice best{0, 0, 1, 1e12};
+      consider_parts(&best, blocks_of(64), blocks_of(128), ceil_div(mean, kTileDepth), cells, most_parts);
+      return best;
+    };
+    Choice best = choose(kMostParts);
+    const Parts<float> parts(s, best.parts, cells);
+    if (parts.count() < best.parts) best = choose(1);
+    const int64_t m_tiles = n_groups * ceil_div(a_col_count, best.height), n_tiles = ceil_div(b_col_count, best.width);
     if (m_tiles * n_tiles <= kMostUnits) {
-      const GroupedPlan p = plan_of(m_tiles, n_tiles);
-      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
-      const bool wide = std::max(a_row_count * a_colstride, b_row_count * b_colstride) * size >= int64_t(1) << 32;
-      if (side == 128 && !wide) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, false>), grid, dim3(512), 0, s, g, p);
-      else if (side == 128) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, true>), grid, dim3(512), 0, s, g, p);
-      else if (!wide) hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, false>), grid, dim3(256), 0, s, g, p);
-      else hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, true>), grid, dim3(256), 0, s, g, p);
-      note_kernel(side == 128 ? "grouped_weights_large" : "grouped_weights_medium");
+      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
+      const GroupedArgs of_parts = parts.args(g, a_col_count);
+      const bool wide = std::max(a_row_count * a_colstride, b_row_count * b_colstride) * size >= int64_t(1) << 32, large = best.height == 128;
+      if (large && !wide) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, false>), l.grid, dim3(512), 0, s, of_parts, l.plan);
+      else if (large) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, true>), l.grid, dim3(512), 0, s, of_parts, l.plan);
+      else if (!wide) hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      else hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      parts.add_up<true>(g);
+      static const char* const kNames[] = {"grouped_weights_medium", "grouped_weights_large", "grouped_weights_medium+grouped_sum", "grouped_weights_large+grouped_sum"};
+      note_kernel(kNames[large + 2 * (parts.count() > 1)]);
       return after_launch(s);
     }
   }
   if (dtype == CT_F64) {
-    const int64_t side = n_groups * ceil_div(a_col_count, 64) * ceil_div(b_col_count, 64) >= 1024 ? 64 : 32;
-    const int64_t m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
+    auto choose = [&](int64_t most_parts) {
+      Choice best{32, 32, 1, 1e12};
+      consider_double_parts(&best, blocks_of(32), blocks_of(64), mean, cells, most_parts);
+      return best;
+    };
+    Choice best = choose(kMostParts);
+    const Parts<double> parts(s, best.parts, cells);
+    if (parts.count() < best.parts) best = choose(1);
+    const int64_t side = best.height, m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
     if (m_tiles * n_tiles <= kMostUnits) {
-      const GroupedPlan p = plan_of(m_tiles, n_tiles);
-      const dim3 grid((uint32_t)(ceil_div(p.units, kXcds * kRun) * kXcds * kRun));
-      if (side == 64) hipLaunchKernelGGL((grouped_weights_double_kernel<64>), grid, dim3(256), 0, s, g, p);
-      else hipLaunchKernelGGL((grouped_weights_double_kernel<32>), grid, dim3(256), 0, s, g, p);
-      note_kernel("grouped_weights_double");
+      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
+      const GroupedArgs of_parts = parts.args(g, a_col_count);
+      if (side == 64) hipLaunchKernelGGL((grouped_weights_double_kernel<64>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      else hipLaunchKernelGGL((grouped_weights_double_kernel<32>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      parts.add_up<true>(g);
+      note_kernel(parts.count() > 1 ? "grouped_weights_double+grouped_sum" : "grouped_weights_double");
       return after_launch(s);
     }
   }

@@ -521,6 +521,89 @@ def test_grouped_gemm_weights(D, size):
                 close(got[e], want, abs(alpha) * (np.abs(x).T @ np.abs(y)) + np.abs(beta * c[e]), (len(x) + 4) * D.u, f"{kind} {capi.last_kernel()}")
 
 
+@pytest.mark.parametrize("trans_b", [True, False])
+@pytest.mark.parametrize("size", [(2, 300, 4100, 200), (1, 260, 2081, 65), (1, 900, 4129, 65), (8, 1100, 3000, 260)], ids=str)
+def test_grouped_gemm_whose_sums_are_divided(stream, size, trans_b):
+    """Few tiles and long sums: blocks take parts of k, and a second launch adds them up, in the groups' rows alone (not of 260
+    rows by 65, which the kernel for a few rows takes)."""
+    D = Owned("float")
+    groups, rows, k, n = size
+    for turn, (kind, whole, alpha, beta) in enumerate((("any", True, 1.0, 0.0), ("short", False, 1.5, 0.0), ("one", False, -0.5, 0.75))):
+        rng = np.random.default_rng(rows + k + turn)
+        make = (lambda *s: rng.integers(-7, 8, s).astype(np.float32)) if whole else (lambda *s: rng.standard_normal(s).astype(np.float32))
+        offsets = offsets_of(rng, groups, rows, kind)
+        index = rng.integers(0, rows, rows)
+        index[::7] = rng.choice([-1, rows, 1 << 30], len(index[::7]))
+        a, c = make(rows, k), make(rows, n)
+        b = make(groups, n, k) if trans_b else make(groups, k, n)
+        tc = D.block(c, turn)
+        blocks.grouped_gemm(tc, trans_b, alpha, D.block(a, turn), D.tensor(b), beta, D.tensor(offsets, "int"), index=D.tensor(index, "int"))
+        assert capi.last_kernel() == "grouped_thin" if rows == 260 else capi.last_kernel().endswith("+grouped_sum")
+        want, scale = grouped64(a, index, b, trans_b, offsets, c, alpha, beta)
+        got = read(tc)
+        inside = np.zeros(rows, bool)
+        inside[offsets[0]:offsets[-1]] = True
+        assert np.array_equal(got[~inside], c[~inside]), "rows of no group were written"
+        if whole:
+            assert np.array_equal(got.astype(np.float64), want)
+        else:
+            close(got, want, scale, (k + 4) * 2.0 ** -24, kind)
+    D.free()
+
+
+@pytest.mark.parametrize("size", [(2, 9000, 130, 70), (3, 7001, 33, 65), (1, 5000, 64, 64)], ids=str)
+def test_grouped_gemm_weights_whose_sums_are_divided(D, size):
+    groups, rows, m, n = size
+    for turn, (kind, whole, alpha, beta) in enumerate((("any", True, 1.0, 0.0), ("short", False, 1.5, 0.0), ("one", False, -0.5, 0.75))):
+        rng = np.random.default_rng(rows + m + turn)
+        make = (lambda *s: rng.integers(-7, 8, s).astype(D.type)) if whole else (lambda *s: rng.standard_normal(s).astype(D.type))
+        offsets = offsets_of(rng, groups, rows, kind)
+        ia = rng.integers(0, rows, rows)
+        ia[::9] = -1
+        a, b, c = make(rows, m), make(rows, n), make(groups, m, n)
+        tc = D.tensor(c)
+        blocks.grouped_gemm_weights(tc, alpha, D.block(a, turn), D.block(b, 1), beta, D.tensor(offsets, "int"), a_index=D.tensor(ia, "int"))
+        assert capi.last_kernel().endswith("+grouped_sum")
+        got, x_all = read(tc), np.where((ia >= 0)[:, None], a[ia], 0).astype(np.float64)
+        for e in range(groups):
+            x, y = x_all[offsets[e]:offsets[e + 1]], b[offsets[e]:offsets[e + 1]].astype(np.float64)
+            want = alpha * (x.T @ y) + beta * c[e].astype(np.float64)
+            if whole:
+                assert np.array_equal(got[e].astype(np.float64), want), (kind, e)
+            else:
+                close(got[e], want, abs(alpha) * (np.abs(x).T @ np.abs(y)) + np.abs(beta * c[e]), (len(x) + 4) * D.u, kind)
+
+
+def test_grouped_gemm_weights_of_an_operand_beyond_four_gib(stream):
+    """Rows that begin past 2^32 bytes are found: whole numbers, every sum exact."""
+    D = Owned("float")
+    rng = np.random.default_rng(35)
+    ld, a_rows = 1 << 16, (1 << 14) + 40                      # 4.01 GiB of which 200 columns of a few rows are looked at
+    rows, m, n = 300, 200, 70
+    whole = ct.new_tensor([a_rows * ld], datatype="float")
+    D.kept.append(whole)
+    index = np.concatenate([rng.integers(0, 40, rows // 2), rng.integers(a_rows - 40, a_rows, rows - rows // 2)])
+    small = rng.integers(-7, 8, (a_rows, m)).astype(np.float32)
+    for r in np.unique(index):
+        row = D.tensor(small[r])
+        capi.call("ct_memcpy_async", whole.buffer.ptr + 4 * ld * int(r), row.buffer.ptr, 4 * m, capi.COPY_D2D, stream.handle)
+    a = ct.Tensor(whole.device, {"shape": [a_rows, m], "strides": [ld, 1]}, whole.buffer)
+    b = rng.integers(-7, 8, (rows, n)).astype(np.float32)
+    offsets = np.array([0, 120, 120, rows])
+    tc = D.tensor(np.zeros((3, m, n)))
+    blocks.grouped_gemm_weights(tc, 1.0, a, D.tensor(b), 0.0, D.tensor(offsets, "int"), a_index=D.tensor(index, "int"))
+    x = small[index].astype(np.float64)
+    for e in range(3):
+        i = slice(offsets[e], offsets[e + 1])
+        assert np.array_equal(read(tc)[e].astype(np.float64), x[i].T @ b[i])
+    # the same operand's rows in the products
+    weights, c = rng.integers(-7, 8, (3, n, m)).astype(np.float32), D.tensor(np.zeros((rows, n)))
+    blocks.grouped_gemm(c, True, 1.0, a, D.tensor(weights), 0.0, D.tensor(offsets, "int"), index=D.tensor(index, "int"))
+    want, _ = grouped64(small, index, weights, True, offsets, np.zeros((rows, n), np.float32), 1.0, 0.0)
+    assert np.array_equal(read(c).astype(np.float64), want)
+    D.free()
+
+
 def test_grouped_offsets_that_make_no_sense_stay_inside(D):
     """Offsets that decrease or lie outside the rows are clamped: whatever is computed, nothing beside the result changes."""
     rng = np.random.default_rng(31)
@@ -666,6 +749,188 @@ def test_clip_gradients_that_are_not_finite(D, stream):
             assert np.isnan(norm) and np.isnan(factor) and np.all(np.isnan(got))
         else:
             assert np.isinf(norm) and factor == 0 and got[0] == 0 and got[2] == 0 and np.isnan(got[1])
+
+
+# ------------------------------------------------------------------------------------------------- the checks in Python
+
+def test_operands_that_only_the_checks_in_python_take(stream, monkeypatch):
+    """Every call comes out the same whether its operands are found in native code or by the checks behind it."""
+    D = Owned("float")
+    n, width, experts, chosen = 37, 24, 6, 2
+
+    def run():
+        random = np.random.default_rng(48)
+        make = lambda *s: D.tensor(random.standard_normal(s))
+        empty, whole = (lambda *s: D.tensor(np.zeros(s))), (lambda *s: D.tensor(np.zeros(s), "int"))
+        x, residual, h, out, statistics = make(n, width), make(n, width), empty(n, width), empty(n, width), empty(4, n)
+        p = {"pre-scale": make(width), "post-scale": make(width), "gate": make(1, width)}
+        g = {k: empty(*t.shape()) for k, t in p.items()}
+        d = blocks.norm_descriptor(post="rms", pre="rms")
+        blocks.norm_residual(out, h, statistics, x, residual, p, d)
+        dx, dr = empty(n, width), empty(n, width)
+        blocks.norm_residual_gradient(dx, dr, g, make(n, width), make(n, width), x, out, statistics, p, d)
+        at, w, offsets, tokens, slots = whole(n, chosen), empty(n, chosen), whole(experts + 1), whole(n * chosen), whole(n, chosen)
+        logits, dl = make(n, experts), empty(n, experts)
+        blocks.route_experts(at, w, offsets, tokens, slots, logits)
+        blocks.route_experts_gradient(dl, make(n, chosen), w, at, logits)
+        rows, dw = empty(n * chosen, width), empty(experts, width, width)
+        blocks.grouped_gemm(rows, True, 1.0, h, make(experts, width, width), 0.0, offsets, index=tokens)
+        blocks.grouped_gemm_weights(dw, 1.0, rows, h, 0.0, offsets, b_index=tokens)
+        y, drows, dweights = empty(n, width), empty(n * chosen, width), empty(n, chosen)
+        blocks.combine_experts(y, rows, w, slots)
+        blocks.combine_experts_gradient(drows, dweights, make(n, width), rows, w, slots)
+        norm = empty(2)
+        optimize.clip_gradients(optimize.Backend(stream), [dw, drows], 1.0, norm)
+        return [read(t) for t in (out, h, dx, dr, *g.values(), at, w, offsets, tokens, slots, dl, rows, dw, y, drows, dweights, norm)]
+
+    found = run()
+    monkeypatch.setattr(blocks, "_operands", lambda kinds, tensors: None)
+    for a, b in zip(found, run()):
+        assert np.array_equal(a, b)
+    D.free()
+
+
+# ------------------------------------------------------------------------------------------------- graphs
+
+def test_calls_recorded_into_a_graph():
+    """A step of every operator, recorded with the scratch that the stream holds and replayed with new inputs, eager calls of
+    the same step in between: each replay's results are the eager ones, bit for bit."""
+    import ctypes as C
+    rt = C.CDLL("libamdhip64.so")
+    capi.call("ct_set_device", 0)
+    capi.call("ct_set_debug_sync", 0)
+    stream = drv.HipDriver().default_device().create_stream()
+    D = Owned("float")
+    rng = np.random.default_rng(43)
+    width, experts, chosen, inner = 200, 6, 2, 2100
+    with ct.tensor_context(stream, "float"):
+        make = lambda *s: D.tensor(rng.standard_normal(s))
+        sides = []
+        p = {"pre-scale": make(width), "pre-bias": make(width), "post-scale": make(width), "post-bias": make(width), "gate": make(1, width)}
+        inputs = {n: {"x": make(n, width), "r": make(n, width), "do": make(n, width), "dh": make(n, width), "logits": make(n, experts),
+                      "dw": make(n, chosen), "y": make(n * chosen, inner), "dy": make(n, width)} for n in (100, 1300)}
+        first, second = make(experts, inner, width), make(experts, width, inner)
+        for _ in range(2):
+            side = {"norm": D.tensor(np.zeros(2))}
+            for n in inputs:
+                empty, whole = (lambda *s: D.tensor(np.zeros(s))), (lambda *s: D.tensor(np.zeros(s), "int"))
+                side[n] = dict(out=empty(n, width), h=empty(n, width), statistics=empty(4, n), dx=empty(n, width), dr=empty(n, width),
+                               g={k: empty(*t.shape()) for k, t in p.items()}, at=whole(n, chosen), w=empty(n, chosen), offsets=whole(experts + 1),
+                               tokens=whole(n * chosen), slots=whole(n, chosen), dl=empty(n, experts), rows=empty(n * chosen, inner),
+                               back=empty(n * chosen, width), d_first=empty(experts, inner, width), y=empty(n, width),
+                               d_back=empty(n * chosen, width), d_weights=empty(n, chosen))
+            sides.append(side)
+
+        d = blocks.norm_descriptor(post="layer", pre="layer", residual_scale=0.5)
+
+        def step(side):
+            for n, i in inputs.items():
+                o = side[n]
+                blocks.norm_residual(o["out"], o["h"], o["statistics"], i["x"], i["r"], p, d)
+                blocks.norm_residual_gradient(o["dx"], o["dr"], o["g"], i["do"], i["dh"], i["x"], o["out"], o["statistics"], p, d)
+                blocks.route_experts(o["at"], o["w"], o["offsets"], o["tokens"], o["slots"], i["logits"])
+                blocks.route_experts_gradient(o["dl"], i["dw"], o["w"], o["at"], i["logits"])
+                blocks.grouped_gemm(o["rows"], True, 1.0, o["h"], first, 0.0, o["offsets"], index=o["tokens"])
+                blocks.grouped_gemm(o["back"], True, 1.0, i["y"], second, 0.0, o["offsets"])
+                blocks.grouped_gemm_weights(o["d_first"], 1.0, o["rows"], o["h"], 0.0, o["offsets"], b_index=o["tokens"])
+                blocks.combine_experts(o["y"], o["back"], o["w"], o["slots"])
+                blocks.combine_experts_gradient(o["d_back"], o["d_weights"], i["dy"], o["back"], o["w"], o["slots"])
+            optimize.clip_gradients(optimize.Backend(stream), [t for n in inputs for t in side[n]["g"].values()] + [side[n]["d_first"] for n in inputs],
+                                    1.0, side["norm"])
+
+        def results(side):
+            out = [read(side["norm"])]
+            for n in inputs:
+                for t in side[n].values():
+                    out += [read(v) for v in (t.values() if isinstance(t, dict) else [t])]
+            return out
+
+        step(sides[1])      # kernels are loaded and scratch is in place
+        capi.call("ct_stream_sync", stream.handle)
+        graph, graph_exec = C.c_void_p(), C.c_void_p()
+        rt.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+        rt.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+        rt.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+        rt.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+        rt.hipGraphExecDestroy.argtypes = rt.hipGraphDestroy.argtypes = [C.c_void_p]
+        assert rt.hipStreamBeginCapture(stream.handle, 1) == 0
+        try:
+            step(sides[1])
+        finally:
+            ended = rt.hipStreamEndCapture(stream.handle, C.byref(graph))
+        assert ended == 0 and graph.value
+        assert rt.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+        for replay in range(4):
+            for n, i in inputs.items():
+                for t in i.values():
+                    new = D.tensor(rng.standard_normal(t.shape()))
+                    capi.call("ct_memcpy_async", t.buffer.ptr, new.buffer.ptr, t.ecount() * 4, capi.COPY_D2D, stream.handle)
+            step(sides[0])
+            want = results(sides[0])
+            assert rt.hipGraphLaunch(graph_exec, stream.handle) == 0
+            for a, b in zip(results(sides[1]), want):
+                assert np.all(np.isfinite(b)) and np.array_equal(a, b), replay
+        capi.call("ct_stream_sync", stream.handle)
+        assert rt.hipGraphExecDestroy(graph_exec) == 0 and rt.hipGraphDestroy(graph) == 0
+        D.free()
+    stream.release()
+    capi.call("ct_set_debug_sync", 1)
+
+
+def test_divided_sums_recorded_without_scratch_do_without():
+    """A capture that finds no scratch for the parts: one launch, and the same whole numbers."""
+    import ctypes as C
+    rt = C.CDLL("libamdhip64.so")
+    rt.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    rt.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    rt.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    rt.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    rt.hipGraphExecDestroy.argtypes = rt.hipGraphDestroy.argtypes = [C.c_void_p]
+    capi.call("ct_set_device", 0)
+    capi.call("ct_set_debug_sync", 0)
+    rng = np.random.default_rng(45)
+    for datatype in ("float", "double"):
+        D = Owned(datatype)
+        device = drv.HipDriver().default_device()
+        stream, loader = device.create_stream(), device.create_stream()
+        make = lambda *s: rng.integers(-7, 8, s).astype(NUMPY[datatype])
+        a, b, x = make(300, 4100), make(2, 200, 4100), make(300, 64)
+        offsets = np.array([0, 140, 300])
+        with ct.tensor_context(loader, datatype):
+            ta, tb, tx, to = D.tensor(a), D.tensor(b), D.tensor(x), D.tensor(offsets, "int")
+            tc, tw = D.tensor(np.zeros((300, 200))), D.tensor(np.zeros((2, 64, 64)))
+            long, wide = D.tensor(make(9000, 64)), D.tensor(np.array([0, 5000, 9000]), "int")
+            blocks.grouped_gemm(tc, True, 1.0, ta, tb, 0.0, to)        # the kernels are loaded
+            blocks.grouped_gemm_weights(tw, 1.0, long, long, 0.0, wide)
+            assert capi.last_kernel().endswith("+grouped_sum")
+            capi.call("ct_stream_sync", loader.handle)
+        kernels = []
+        with ct.tensor_context(stream, datatype):
+            graph, graph_exec = C.c_void_p(), C.c_void_p()
+            assert rt.hipStreamBeginCapture(stream.handle, 1) == 0
+            try:
+                blocks.grouped_gemm(tc, True, 1.0, ta, tb, 0.0, to)
+                kernels.append(capi.last_kernel())
+                blocks.grouped_gemm_weights(tw, 1.0, long, long, 0.0, wide)
+                kernels.append(capi.last_kernel())
+            finally:
+                ended = rt.hipStreamEndCapture(stream.handle, C.byref(graph))
+            assert ended == 0 and graph.value and not any(k.endswith("+grouped_sum") for k in kernels), kernels
+            assert rt.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+            host = read(long).astype(np.float64)
+            for _ in range(2):
+                assert rt.hipGraphLaunch(graph_exec, stream.handle) == 0
+                got, weights = read(tc).astype(np.float64), read(tw).astype(np.float64)
+                for e in range(2):
+                    i, j = slice(offsets[e], offsets[e + 1]), slice(*((0, 5000), (5000, 9000))[e])
+                    assert np.array_equal(got[i], a[i].astype(np.float64) @ b[e].T.astype(np.float64))
+                    assert np.array_equal(weights[e], host[j].T @ host[j])
+            capi.call("ct_stream_sync", stream.handle)
+            assert rt.hipGraphExecDestroy(graph_exec) == 0 and rt.hipGraphDestroy(graph) == 0
+            D.free()
+        stream.release()
+        loader.release()
+    capi.call("ct_set_debug_sync", 1)
 
 
 # ------------------------------------------------------------------------------------------------- streams
