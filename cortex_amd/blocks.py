@@ -38,6 +38,12 @@ def _floating(name: str, first: Tensor, *others) -> None:
             raise TensorError("Tensor arguments are not all on same device")
 
 
+def _needed(name: str, **tensors) -> None:
+    for what, t in tensors.items():
+        if t is None:
+            raise TensorError(f"{name}: {what.replace('_', ' ')} is needed")
+
+
 def _is_packed(t: Tensor) -> bool:
     shape, expected = t.dimensions["shape"], 1
     if not all(type(n) is int for n in shape):
@@ -153,7 +159,7 @@ def norm_residual(output: Tensor, normalized: Tensor, statistics: Tensor, input:
     name = "norm-residual"
     p = parameters.get
     has_pre = descriptor["pre"] != "none"
-    if parameters.keys() <= _PARAMETERS and (normalized is not None or not has_pre):
+    if output is not None and parameters.keys() <= _PARAMETERS and (normalized is not None or not has_pre):
         normalized = normalized if has_pre else None
         gate, scales = p("gate"), (p("post-scale"), p("post-bias"), p("pre-scale"), p("pre-bias"))
         found = _operands("mmmmmppppp", (input, output, residual, normalized, gate, statistics, *scales))
@@ -163,6 +169,7 @@ def norm_residual(output: Tensor, normalized: Tensor, statistics: Tensor, input:
                                          _dims(gate), *map(_buffer, scales), descriptor["post"], descriptor["pre"],
                                          descriptor["residual-scale"], descriptor["epsilon"])
             return output, normalized
+    _needed(name, input=input, output=output)
     shape = _rows(name, "input", input)[:2]
     if has_pre and normalized is None:
         raise TensorError(f"{name}: a norm before the next block needs a tensor to store to")
@@ -203,6 +210,7 @@ def norm_residual_gradient(input_gradient: Tensor, residual_gradient: Tensor, pa
                 _dims(output), _buffer(statistics), _buffer(gate), _dims(gate), *map(_buffer, scales[:3]), descriptor["post"],
                 descriptor["pre"], descriptor["residual-scale"])
             return input_gradient, residual_gradient
+    _needed(name, input=input)
     shape = _rows(name, "input", input)[:2]
     _floating(name, input, input_gradient, residual_gradient, output_gradient, normalized_gradient, output, statistics)
     for what, t in (("input gradient", input_gradient), ("residual gradient", residual_gradient),
@@ -251,6 +259,7 @@ def route_experts(experts: Tensor, weights: Tensor, offsets: Tensor, tokens: Ten
             check_stream().route_experts(experts.buffer, weights.buffer, offsets.buffer, tokens.buffer, slots.buffer, logits.buffer,
                                          stride, n, n_experts, n_chosen, renormalize)
             return experts, weights
+    _needed(name, logits=logits, experts=experts, weights=weights, offsets=offsets, tokens=tokens, slots=slots)
     n, n_experts, stride = _rows(name, "logits", logits)
     n_chosen = int(experts.shape()[-1])
     _floating(name, logits, weights)
@@ -278,6 +287,7 @@ def route_experts_gradient(logits_gradient: Tensor, weights_gradient: Tensor, we
             check_stream().route_experts_gradient(logits_gradient.buffer, gradient_stride, weights_gradient.buffer, weights.buffer,
                                                   experts.buffer, _buffer(logits), stride, n, n_experts, of_choice[2], renormalize)
             return logits_gradient
+    _needed(name, logits_gradient=logits_gradient, weights_gradient=weights_gradient, weights=weights, experts=experts)
     n, n_experts, gradient_stride = _rows(name, "logits gradient", logits_gradient)
     n_chosen = int(experts.shape()[-1])
     _floating(name, logits_gradient, weights_gradient, weights, logits)
@@ -321,6 +331,7 @@ def grouped_gemm(C: Tensor, trans_b, alpha, A: Tensor, B: Tensor, beta, offsets:
             check_stream().grouped_gemm(C.buffer, c_stride, trans_b, alpha, A.buffer, a_rows, a_columns, a_stride, _buffer(index),
                                         B.buffer, columns, b_row_stride, b_stride, offsets.buffer, groups, rows, beta)
             return C
+    _needed(name, C=C, A=A, B=B, offsets=offsets)
     _floating(name, C, A, B)
     rows, c_columns, c_stride = _rows(name, "C", C)
     a_rows, a_columns, a_stride = _rows(name, "A", A)
@@ -345,6 +356,17 @@ def grouped_gemm_weights(C: Tensor, alpha, A: Tensor, B: Tensor, beta, offsets: 
     """For every group e: C[e] = alpha * sum over its rows i of A[a-index[i]]^T B[b-index[i]] + beta * C[e]; beta * C[e]
     where it has none."""
     name = "grouped-gemm-weights"
+    found = _operands("mmgiii", (A, B, C, offsets, a_index, b_index))
+    if found is not None:
+        a_rows, a_columns, a_stride, b_rows, b_columns, b_stride, groups, c_rows, c_columns, c_row_stride, c_stride = found[:11]
+        rows = found[15] if a_index is not None else a_rows
+        if ((a_columns, b_columns) == (c_rows, c_columns) and found[11:14] == (1, groups + 1, groups + 1) and
+                rows == (found[18] if b_index is not None else b_rows)):
+            check_stream().grouped_gemm_weights(C.buffer, c_row_stride, c_stride, alpha, A.buffer, a_rows, a_columns, a_stride,
+                                                _buffer(a_index), B.buffer, b_rows, b_columns, b_stride, _buffer(b_index),
+                                                offsets.buffer, groups, rows, beta)
+            return C
+    _needed(name, C=C, A=A, B=B, offsets=offsets)
     _floating(name, C, A, B)
     groups, c_rows, c_columns, c_row_stride, c_stride = _matrices(name, "C", C)
     a_rows, a_columns, a_stride = _rows(name, "A", A)
@@ -377,6 +399,7 @@ def combine_experts(output: Tensor, rows: Tensor, weights: Tensor, slots: Tensor
             check_stream().combine_experts(output.buffer, stride, rows.buffer, count, rows_stride, _buffer(weights), slots.buffer, n,
                                            of_choice[2], width)
             return output
+    _needed(name, output=output, rows=rows, slots=slots)
     _floating(name, output, rows, weights)
     _indexes(name, output, slots=slots)
     n, width, stride = _rows(name, "output", output)
@@ -396,6 +419,18 @@ def combine_experts_gradient(rows_gradient: Tensor, weights_gradient: Tensor, ou
     """rows-gradient[slots[t, j]] = weights[t, j] * output-gradient[t] (rows that no slot names are left as they are) and
     weights-gradient[t, j] = output-gradient[t] . rows[slots[t, j]].  Either may be None."""
     name = "combine-experts-gradient"
+    found = _operands("mmmppi", (output_gradient, rows_gradient, rows, weights_gradient, weights, slots))
+    if found is not None:
+        n, width, stride, to_count, to_columns, to_stride, count, columns, rows_stride = found[:9]
+        of_choice = found[15:]
+        if (of_choice[0] == 2 and of_choice[1] == n * of_choice[2] and (rows_gradient is None or to_columns == width) and
+                (columns == width if rows is not None else weights_gradient is None) and (not to_count or not count or to_count == count) and
+                (weights_gradient is None or found[9:12] == of_choice) and (weights is None or found[12:15] == of_choice)):
+            check_stream().combine_experts_gradient(_buffer(rows_gradient), to_stride or width, _buffer(weights_gradient), output_gradient.buffer,
+                                                    stride, _buffer(rows), to_count or count, rows_stride or width, _buffer(weights),
+                                                    slots.buffer, n, of_choice[2], width)
+            return
+    _needed(name, output_gradient=output_gradient, slots=slots)
     _floating(name, output_gradient, rows_gradient, weights_gradient, rows, weights)
     _indexes(name, output_gradient, slots=slots)
     n, width, stride = _rows(name, "output gradient", output_gradient)

@@ -260,3 +260,111 @@ def test_tensor_api(message, call):
         with pytest.raises((ValueError, TypeError)) as e:
             call()
     assert message in str(e.value), str(e.value)
+
+
+# ---------------------------------------------------------------- operands found in native code
+
+class Recorder:
+    """A stream that notes the calls it gets."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        plain = lambda a: (tuple(a["shape"]), tuple(a["strides"])) if isinstance(a, dict) else a.key if isinstance(a, Keyed) else a
+        return lambda *args: self.calls.append((name, [plain(a) for a in args]))
+
+
+class Keyed(Stub):
+    """A buffer that is told apart from others."""
+
+
+def operand(rng, shape, datatype, key):
+    """A tensor of this shape, or of one near it, in rows that may lie apart; now and then of another type, or none."""
+    shape = list(shape)
+    if rng.random() < 0.06:
+        shape[rng.randrange(len(shape))] += rng.choice([-1, 1, 3])
+    if rng.random() < 0.04:
+        shape = rng.choice([[1] + shape, shape[1:] or [1], shape + [1], [0] + shape[1:]])
+    if rng.random() < 0.04:
+        return None
+    if rng.random() < 0.05:
+        datatype = rng.choice(["float", "double", "int", "byte"])
+    strides = dims.dimensions(shape)["strides"] if all(shape) else [1] * len(shape)
+    if len(shape) > 1 and rng.random() < 0.3:
+        pad = rng.choice([1, 5, -1])
+        strides = [s + pad for s in strides[:-1]] + strides[-1:]
+    if rng.random() < 0.04:
+        strides = strides[:-1] + [2]
+    n = 1
+    for s in shape:
+        n *= s
+    buffer = Keyed(n, datatype)
+    buffer.key = (key, datatype)
+    return ct.Tensor(DEVICE if rng.random() < 0.97 else "another", {"shape": shape, "strides": strides}, buffer)
+
+
+def drawn_call(rng):
+    n, width, experts, chosen = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 4), rng.randint(1, 3)
+    columns, rows, real = rng.randint(1, 5), rng.randint(1, 6), rng.choice(["float", "double"])
+    count = iter(range(100))
+    f, j = (lambda *s: operand(rng, s, real, next(count))), (lambda *s: operand(rng, s, "int", next(count)))
+    maybe = lambda x: x if rng.random() < 0.7 else None
+    kind = rng.randrange(7)
+    if kind < 2:
+        d = blocks.norm_descriptor(post=rng.choice(blocks.NORM_KINDS), pre=rng.choice(blocks.NORM_KINDS))
+        p = {k: maybe(f(width)) for k in ("post-scale", "post-bias", "pre-scale", "pre-bias")}
+        p["gate"] = maybe(f(rng.choice([1, n]), rng.choice([1, width])))
+        if kind == 0:
+            args = f(n, width), f(n, width), maybe(f(4, n)), f(n, width), maybe(f(n, width)), p, d
+            return lambda: blocks.norm_residual(*args)
+        g = {k: maybe(f(*t.shape())) for k, t in p.items() if t is not None and all(s >= 0 for s in t.shape())}
+        args = f(n, width), maybe(f(n, width)), g, maybe(f(n, width)), maybe(f(n, width)), f(n, width), f(n, width), f(4, n), p, d
+        return lambda: blocks.norm_residual_gradient(*args)
+    if kind == 2:
+        args = j(n, chosen), f(n, chosen), j(experts + 1), j(n * chosen), j(n, chosen), f(n, experts)
+        return lambda: blocks.route_experts(*args)
+    if kind == 3:
+        args, renormalize = (f(n, experts), f(n, chosen), f(n, chosen), j(n, chosen), maybe(f(n, experts))), rng.random() < 0.5
+        return lambda: blocks.route_experts_gradient(*args, renormalize=renormalize)
+    if kind == 4:
+        trans, index = rng.random() < 0.5, maybe(j(rows))
+        args = (f(rows, columns), trans, 1.0, f(rows if index is None else n, width), f(experts, *((columns, width) if trans else (width, columns))),
+                0.0, j(experts + 1))
+        return lambda: blocks.grouped_gemm(*args, index=index)
+    if kind == 5:
+        ia, ib = maybe(j(rows)), maybe(j(rows))
+        args = f(experts, width, columns), 1.0, f(rows if ia is None else n, width), f(rows if ib is None else n + 1, columns), 0.0, j(experts + 1), ia, ib
+        return lambda: blocks.grouped_gemm_weights(*args)
+    if rng.random() < 0.5:
+        args = f(n, width), f(rows, width), maybe(f(n, chosen)), j(n, chosen)
+        return lambda: blocks.combine_experts(*args)
+    args = maybe(f(rows, width)), maybe(f(n, chosen)), f(n, width), maybe(f(rows, width)), maybe(f(n, chosen)), j(n, chosen)
+    return lambda: blocks.combine_experts_gradient(*args)
+
+
+@pytest.mark.skipif(capi.front is None, reason="the native front is not built")
+def test_native_operands_are_those_of_the_checks(monkeypatch):
+    """Calls drawn with operands that fit, or nearly: with the operands found in native code and without, the same call
+    reaches the stream, or the same error is raised."""
+    import random
+    reached = refused = 0
+    for seed in range(8000):
+        outcomes = []
+        for native in (True, False):
+            with monkeypatch.context() as m:
+                if not native:
+                    m.setattr(blocks, "_operands", lambda kinds, tensors: None)
+                stream = Recorder()
+                call = drawn_call(random.Random(seed))
+                with ct.tensor_context(stream, "float"):
+                    try:
+                        call()
+                        outcomes.append(stream.calls)
+                    except (ValueError, TypeError) as e:
+                        assert not stream.calls
+                        outcomes.append((type(e), str(e)))
+        assert outcomes[0] == outcomes[1], seed
+        reached += isinstance(outcomes[0], list)
+        refused += not isinstance(outcomes[0], list)
+    assert reached > 1000 and refused > 1000, (reached, refused)
