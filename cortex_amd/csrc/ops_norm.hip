@@ -126,6 +126,17 @@ __global__ void __launch_bounds__(block_of(LANES)) norm_kernel(const NormArgs a)
     // the norm of x in place, its statistics to `place`
     auto norm = [&](int kind, const void* scale, const void* bias, int place) {
       T mean[1] = {0}, square[1] = {0};
+      // The parameters are on their way while the sums are formed: rows of 256, layer norms before and after, 43 us a 65536, were 61; of
+      // 1531 doubles 45 us a 5003, were 51.  Not with 1024 lanes, which have no registers for them (rows of 16384 134 us, and 97 so).
+      constexpr bool kAhead = LANES <= 256;
+      Quad<T> w_ahead[kAhead ? VPT : 1], b_ahead[kAhead ? VPT : 1];
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int t = 0; t < VPT; ++t) {
+          w_ahead[t] = at.piece_or(scale, T(1), t);
+          b_ahead[t] = at.piece_or(bias, T(0), t);
+        }
+      }
       if (kind == CT_NORM_LAYER) {
         CT_EACH mean[0] += at.owned(t, e, x[t].v[e]);
         row_sum<T, LANES>(mean, lds, turn);
@@ -137,11 +148,11 @@ __global__ void __launch_bounds__(block_of(LANES)) norm_kernel(const NormArgs a)
       const T rate = rate_of(square[0] * inverse, epsilon);
 #pragma unroll
       for (int t = 0; t < VPT; ++t) {
-        const Quad<T> w = at.piece_or(scale, T(1), t);
+        const Quad<T> w = kAhead ? w_ahead[kAhead ? t : 0] : at.piece_or(scale, T(1), t);
 #pragma unroll
         for (int e = 0; e < N; ++e) x[t].v[e] = x[t].v[e] * rate * w.v[e];
         if (bias) {
-          const Quad<T> b = at.piece(static_cast<const T*>(bias), t);
+          const Quad<T> b = kAhead ? b_ahead[kAhead ? t : 0] : at.piece(static_cast<const T*>(bias), t);
 #pragma unroll
           for (int e = 0; e < N; ++e) x[t].v[e] += b.v[e];
         }
@@ -208,7 +219,7 @@ __device__ __forceinline__ bool common_gate(int kind) { return kind == kNoGate |
 // next row's operands are loaded into the registers of this one's as those are used up.
 // kSums: 0 none, 1 S1 and T1, 2 all.  An absent gradient of the results is read from `input` and not used.
 template <class T, int LANES, int VPT, int kSums, bool kStreaming>
-__global__ void __launch_bounds__(block_of(LANES), VPT == 4 ? 3 : 4) norm_gradient_kernel(const NormGradientArgs a) {
+__global__ void __launch_bounds__(block_of(LANES), VPT >= 3 ? 3 : 4) norm_gradient_kernel(const NormGradientArgs a) {
   constexpr int kThreads = block_of(LANES), kRows = kThreads / LANES;
   using R = Row<T, LANES, VPT, kStreaming>;
   constexpr int N = R::N;
@@ -630,7 +641,8 @@ __global__ void __launch_bounds__(256) norm_long_apply_kernel(const NormGradient
 
 // ------------------------------------------------------------------ host
 
-// Calls f with the lanes of a row and the pieces to a lane that hold `width` elements; false if none do.
+// Calls f with the lanes of a row and the pieces to a lane that hold `width` elements; false if none do.  (Three pieces beside two and
+// four: 32768 x 768 floats 75 us and 116 of the gradient, with four 87 and 121; 3000 x 5000 doubles 99 and 289, with four 145 and 389.)
 template <class T, class F>
 bool with_shape(uint32_t width, F f) {
   constexpr uint32_t N = Quad<T>::N;
@@ -638,10 +650,10 @@ bool with_shape(uint32_t width, F f) {
   if (width < N) return false;
 #define CT_SHAPE(L, V) \
   if (pieces <= L * V) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>()), true
-  CT_SHAPE(16, 1); CT_SHAPE(16, 2); CT_SHAPE(16, 4);
-  CT_SHAPE(64, 2); CT_SHAPE(64, 4);
-  CT_SHAPE(256, 2); CT_SHAPE(256, 4);
-  CT_SHAPE(1024, 2); CT_SHAPE(1024, 4);
+  CT_SHAPE(16, 1); CT_SHAPE(16, 2); CT_SHAPE(16, 3); CT_SHAPE(16, 4);
+  CT_SHAPE(64, 2); CT_SHAPE(64, 3); CT_SHAPE(64, 4);
+  CT_SHAPE(256, 2); CT_SHAPE(256, 3); CT_SHAPE(256, 4);
+  CT_SHAPE(1024, 2); CT_SHAPE(1024, 3); CT_SHAPE(1024, 4);
 #undef CT_SHAPE
   return false;
 }
@@ -671,7 +683,7 @@ int norm_typed(hipStream_t s, const NormArgs& a) {
 // Blocks to a compute unit whose operands are on their way at the same time: 128 KiB in all.  (16384 x 2048 floats, three, four
 // and five blocks of 256 lanes: 157, 151 and 163 us; 8192 x 4096, two, three and four: 150, 155 and 177; more blocks also leave more sums.)
 int64_t blocks_of_a_unit(int64_t bytes_of_a_block, int waves, int pieces) {
-  const int64_t of_registers = (pieces == 4 ? 12 : pieces == 2 ? 16 : 24) / waves;
+  const int64_t of_registers = (pieces >= 3 ? 12 : pieces == 2 ? 16 : 24) / waves;
   return std::max<int64_t>(1, std::min(kBytesAhead / bytes_of_a_block, of_registers));
 }
 

@@ -219,6 +219,14 @@ def test_norm_residual(D, shape, kinds):
         check_norm(D, *shape, *kinds, gate, biases=(i + n) % 2 == 0, residual=(i + n) % 3 != 0, pad=i % 3, seed=i)
 
 
+@pytest.mark.parametrize("kinds", [("rms", "rms"), ("layer", "layer")], ids="-".join)
+@pytest.mark.parametrize("shape", [(37, 70), (37, 95), (300, 150), (13, 191), (9, 300), (9, 383), (200, 700), (7, 767), (5, 1100), (5, 1535), (40, 2500),
+                                   (3, 4500), (3, 6143), (4, 9001)], ids=str)
+def test_norm_residual_of_three_pieces_to_a_lane(D, shape, kinds):
+    """Rows between two and four pieces of 16 bytes to each of the lanes that hold them."""
+    check_norm(D, *shape, *kinds, "column", kinds[0] == "layer", True, 1, sum(shape))
+
+
 @pytest.mark.parametrize("gate", ["column", "row", "full", "scalar", None])
 @pytest.mark.parametrize("shape", [(2100, 40), (1111, 300), (600, 1500)], ids=str)
 def test_norm_residual_sums_over_many_rows(D, shape, gate):
