@@ -467,14 +467,16 @@ PyObject* stand_in(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------- operands of the calls of blocks.py and optimize.py
 
-PyObject *s_device, *s_buffer, *s_datatype, *s_ptr, *s_ecount;
+PyObject *s_device, *s_buffer, *s_datatype, *s_ptr, *s_ecount, *s_float, *s_double, *s_int;
 
 // The datatype of a buffer: 'f', 'd', 'i' (float, double, int), 0 for another.
 char type_of(PyObject* buffer) {
   PyObject* name = PyObject_GetAttr(buffer, s_datatype);
   if (!name) return PyErr_Clear(), 0;
   char type = 0;
-  if (PyUnicode_CheckExact(name))
+  if (name == s_float || name == s_double || name == s_int)   // names are mostly interned
+    type = name == s_float ? 'f' : name == s_double ? 'd' : 'i';
+  else if (PyUnicode_CheckExact(name))
     type = PyUnicode_CompareWithASCIIString(name, "float") == 0 ? 'f' : PyUnicode_CompareWithASCIIString(name, "double") == 0 ? 'd' :
            PyUnicode_CompareWithASCIIString(name, "int") == 0 ? 'i' : 0;
   Py_DECREF(name);
@@ -586,9 +588,10 @@ PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!counts) return Py_XDECREF(at), nullptr;
   char type = 0;
   bool fine = count > 0;
+  const PyTypeObject* of_buffers = nullptr;   // the type of an item that had no buffer of its own: to find that out again costs as much as the rest
   for (Py_ssize_t i = 0; fine && i < count; ++i) {
     PyObject* item = PyList_GET_ITEM(args[0], i);
-    PyObject* buffer = PyObject_GetAttr(item, s_buffer);
+    PyObject* buffer = Py_TYPE(item) == of_buffers ? nullptr : PyObject_GetAttr(item, s_buffer);
     int64_t elements = -1, address = 0, length = 0;
     if (buffer) {
       PyObject* dims = PyObject_GetAttr(item, s_dimensions);
@@ -598,6 +601,7 @@ PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_XDECREF(dims);
     } else {
       PyErr_Clear();
+      of_buffers = Py_TYPE(item);
       Py_INCREF(item);
       buffer = item;
     }
@@ -637,6 +641,9 @@ PyMODINIT_FUNC PyInit__front() {
   s_datatype = PyUnicode_InternFromString("datatype");
   s_ptr = PyUnicode_InternFromString("ptr");
   s_ecount = PyUnicode_InternFromString("_ecount");
+  s_float = PyUnicode_InternFromString("float");
+  s_double = PyUnicode_InternFromString("double");
+  s_int = PyUnicode_InternFromString("int");
   g_index = PyDict_New();
-  return s_device && s_buffer && s_datatype && s_ptr && s_ecount && s_shape && s_strides && s_max_shape && s_dimensions && s_lib && g_index ? PyModule_Create(&g_module) : nullptr;
+  return s_device && s_buffer && s_datatype && s_ptr && s_ecount && s_float && s_double && s_int && s_shape && s_strides && s_max_shape && s_dimensions && s_lib && g_index ? PyModule_Create(&g_module) : nullptr;
 }
