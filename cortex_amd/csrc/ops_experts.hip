@@ -16,7 +16,8 @@ using namespace cthip;
 
 namespace {
 
-constexpr int kRouteBlock = 256;
+constexpr int kRouteBlock = 256, kFewBlock = 1024;
+constexpr uint32_t kFewBlocks = 64;   // whose counts each adds up itself, rather than a launch between (1024 tokens of 128 experts: 9.7 us, were 12.5)
 constexpr int64_t kCombineCacheBytes = int64_t(256) << 20;   // what the last-level cache holds
 constexpr int64_t kMostBlocks = 1 << 20;   // of a launch; blocks take more than one token each beyond
 constexpr int kMostExperts = 1024, kMostChosen = 32;
@@ -185,22 +186,22 @@ __device__ __forceinline__ void begin_experts(const RouteArgs& a, PlaceLds& lds,
 
 // tokens and slots of assignments first .. end - 1, each wave a run of them in its order; before(e): those of expert e ahead of
 // `first`.
-template <class Before>
+template <int kThreads, class Before>
 __device__ __forceinline__ void place(const RouteArgs& a, PlaceLds& lds, uint32_t first, uint32_t end, Before before) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, buckets = a.n_experts + 1;
-  for (uint32_t e = threadIdx.x; e < buckets; e += kRouteBlock)
+  const uint32_t lane = threadIdx.x & 63, wave = min(threadIdx.x >> 6, (uint32_t)kRouteWaves), buckets = a.n_experts + 1;   // later waves: no run
+  for (uint32_t e = threadIdx.x; e < buckets; e += kThreads)
 #pragma unroll
     for (int w = 0; w < kRouteWaves; ++w) lds.cursor[w][e] = 0;
   __syncthreads();
   const uint32_t run = ((end - first + kRouteWaves - 1) / kRouteWaves + 63) / 64 * 64;
-  const uint32_t mine = min(end, first + wave * run), mine_end = min(end, mine + run);
+  const uint32_t mine = min(end, first + wave * run), mine_end = wave < kRouteWaves ? min(end, mine + run) : mine;
   auto bucket_of = [&](uint32_t i) {
     const int32_t e = a.experts[i];
     return e < 0 ? a.n_experts : (uint32_t)e;
   };
   for (uint32_t i = mine + lane; i < mine_end; i += 64) atomicAdd(&lds.cursor[wave][bucket_of(i)], 1u);
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < buckets; e += kRouteBlock) {
+  for (uint32_t e = threadIdx.x; e < buckets; e += kThreads) {
     uint32_t at = lds.start[e] + before(e);
 #pragma unroll
     for (int w = 0; w < kRouteWaves; ++w) {
@@ -282,52 +283,80 @@ __global__ void __launch_bounds__(kRouteBlock) route_scan_kernel(const RouteArgs
   if (threadIdx.x == 0) a.totals[blockIdx.x] = (int32_t)before;
 }
 
+// kScan: a block adds up the counts of all blocks itself, and of those before it.
+template <bool kScan>
 __global__ void __launch_bounds__(kRouteBlock) route_place_kernel(const RouteArgs a) {
   __shared__ PlaceLds lds;
-  begin_experts(a, lds, [&](uint32_t e) { return (uint32_t)a.totals[e]; }, blockIdx.x == 0);
+  __shared__ uint32_t totals[kScan ? kMostExperts + 1 : 1], befores[kScan ? kMostExperts + 1 : 1];
+  if constexpr (kScan) {
+    for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) {
+      const int32_t* counts = a.counts + (int64_t)e * a.blocks;
+      uint32_t total = 0, before = 0;
+#pragma unroll 8
+      for (uint32_t b = 0; b < a.blocks; ++b) {
+        const uint32_t count = (uint32_t)counts[b];
+        total += count;
+        before += b < blockIdx.x ? count : 0;
+      }
+      totals[e] = total;
+      befores[e] = before;
+    }
+    __syncthreads();
+  }
+  begin_experts(a, lds, [&](uint32_t e) { return kScan ? totals[e] : (uint32_t)a.totals[e]; }, blockIdx.x == 0);
   const uint32_t first = blockIdx.x * a.tokens_per_block * a.n_chosen;
   const uint32_t end = min(a.n, (blockIdx.x + 1) * a.tokens_per_block) * a.n_chosen;
-  place(a, lds, first, end, [&](uint32_t e) { return (uint32_t)a.counts[(int64_t)e * a.blocks + blockIdx.x]; });
+  place<kRouteBlock>(a, lds, first, end, [&](uint32_t e) { return kScan ? befores[e] : (uint32_t)a.counts[(int64_t)e * a.blocks + blockIdx.x]; });
 }
 
 // A few tokens: all of it in one block.
 template <class T, int LANES, int V>
-__global__ void __launch_bounds__(kRouteBlock) route_few_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kFewBlock) route_few_kernel(const RouteArgs a) {
   __shared__ uint32_t counts[kMostExperts + 1];
   __shared__ PlaceLds lds;
-  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kRouteBlock) counts[e] = 0;
+  for (uint32_t e = threadIdx.x; e <= a.n_experts; e += kFewBlock) counts[e] = 0;
   __syncthreads();
-  for (uint32_t t = threadIdx.x / LANES; t < a.n; t += kRouteBlock / LANES) choose<T, LANES, V>(a, t, threadIdx.x % LANES, counts);
+  for (uint32_t t = threadIdx.x / LANES; t < a.n; t += kFewBlock / LANES) choose<T, LANES, V>(a, t, threadIdx.x % LANES, counts);
   __threadfence_block();   // the experts are read again by other lanes
   __syncthreads();
   begin_experts(a, lds, [&](uint32_t e) { return counts[e]; }, true);
-  place(a, lds, 0, a.n * a.n_chosen, [](uint32_t) { return 0u; });
+  place<kFewBlock>(a, lds, 0, a.n * a.n_chosen, [](uint32_t) { return 0u; });
 }
 
-// What one block does in less time than three launches take.
-constexpr uint32_t kFewTokens = 128;
+// What one block does in less time than two launches take.  Us of one block, and of two launches: 32 tokens, 8 of 128 experts, 6.3 and
+// 8.0; 64 tokens, 8 of 128, 9.2 and 8.3; 8 tokens, 8 of 506, 8.3 and 12.7; 32 tokens, 8 of 506, 16.0 and 14.0.
+bool is_few(int64_t n, int64_t n_experts, int64_t n_chosen, int64_t size) {
+  return n_experts <= (size == 8 ? 128 : 256) ? n <= 64 && n * n_chosen <= 256 : n <= 32 && n * n_chosen <= 64;
+}
 
 template <class T, int LANES, int V>
-void route_launch(hipStream_t s, const RouteArgs& a) {
-  if (a.n <= kFewTokens) hipLaunchKernelGGL((route_few_kernel<T, LANES, V>), dim3(1), dim3(kRouteBlock), 0, s, a);
+void route_launch(hipStream_t s, const RouteArgs& a, bool few) {
+  if (few) hipLaunchKernelGGL((route_few_kernel<T, LANES, V>), dim3(1), dim3(kFewBlock), 0, s, a);
   else hipLaunchKernelGGL((route_choose_kernel<T, LANES, V>), dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
 }
 
+// The lanes of a token: 16, so that a wave works on four, as long as they have registers for its logits; a block of 1024 has fewer.
+// (65536 tokens, 8 of 256: 48 us, with 64 lanes 88; 4096 tokens 16 and 57.)
 template <class T>
 int route_typed(hipStream_t s, RouteArgs a) {
   const uint32_t e = a.n_experts;
-  if (e <= 16) route_launch<T, 16, 1>(s, a);
-  else if (e <= 32) route_launch<T, 16, 2>(s, a);
-  else if (e <= 64) route_launch<T, 16, 4>(s, a);
-  else if (e <= 128) route_launch<T, 16, 8>(s, a);
-  else if (e <= 256) route_launch<T, 64, 4>(s, a);
-  else if (e <= 512) route_launch<T, 64, 8>(s, a);
-  else route_launch<T, 64, 16>(s, a);
-  if (a.n > kFewTokens) {
+  const bool few = is_few(a.n, e, a.n_chosen, sizeof(T));
+  if (e <= 16) route_launch<T, 16, 1>(s, a, few);
+  else if (e <= 32) route_launch<T, 16, 2>(s, a, few);
+  else if (e <= 64) route_launch<T, 16, 4>(s, a, few);
+  else if (e <= 128) route_launch<T, 16, 8>(s, a, few);
+  else if (e <= 256 && few && sizeof(T) == 8) hipLaunchKernelGGL((route_few_kernel<T, 64, 4>), dim3(1), dim3(kFewBlock), 0, s, a);
+  else if (e <= 256) route_launch<T, 16, 16>(s, a, few);
+  else if (e <= 512 && few) hipLaunchKernelGGL((route_few_kernel<T, 64, 8>), dim3(1), dim3(kFewBlock), 0, s, a);
+  else if (e <= 512) hipLaunchKernelGGL((route_choose_kernel<T, 16, 32>), dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
+  else route_launch<T, 64, 16>(s, a, few);
+  if (!few && a.blocks <= kFewBlocks) {
+    hipLaunchKernelGGL(route_place_kernel<true>, dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
+  } else if (!few) {
     hipLaunchKernelGGL(route_scan_kernel, dim3(a.n_experts + 1), dim3(kRouteBlock), 0, s, a);
-    hipLaunchKernelGGL(route_place_kernel, dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
+    hipLaunchKernelGGL(route_place_kernel<false>, dim3(a.blocks), dim3(kRouteBlock), 0, s, a);
   }
-  note_kernel(a.n <= kFewTokens ? "route_few" : "route");
+  note_kernel(few ? "route_few" : "route");
   return after_launch(s);
 }
 
@@ -697,10 +726,10 @@ int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* off
   a.colstride = logits_colstride;
   a.n = (uint32_t)n; a.n_experts = (uint32_t)n_experts; a.n_chosen = (uint32_t)n_chosen;
   a.renormalize = renormalize != 0;
-  if (n > kFewTokens) {
-    // 64 tokens to a block, more where the blocks' counts would take more than 8 MiB
+  if (!is_few(n, n_experts, n_chosen, dtype_size(dtype))) {
+    // 16 tokens to a block, 64 where there are blocks enough, more where the blocks' counts would take more than 8 MiB
     const int64_t most_blocks = std::max<int64_t>(1, (int64_t(2) << 20) / (n_experts + 1));
-    a.tokens_per_block = (uint32_t)std::max<int64_t>(64, (n + most_blocks - 1) / most_blocks);
+    a.tokens_per_block = (uint32_t)std::max<int64_t>(n <= 8192 ? 16 : 64, (n + most_blocks - 1) / most_blocks);
     a.blocks = (uint32_t)((n + a.tokens_per_block - 1) / a.tokens_per_block);
     void* scratch = nullptr;
     if (int rc = stream_scratch(s, ((size_t)a.blocks + 1) * (n_experts + 1) * sizeof(int32_t), &scratch)) return rc;

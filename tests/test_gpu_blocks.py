@@ -366,7 +366,8 @@ def run_route(D, logits, k, renormalize, pad=0):
 
 
 ROUTES = [(1, 1, 1), (1, 2, 2), (3, 7, 3), (16, 64, 8), (63, 16, 1), (64, 17, 4), (65, 33, 2), (200, 128, 8), (1000, 129, 6),
-          (700, 256, 32), (130, 300, 5), (90, 1000, 32), (257, 1024, 3), (5000, 8, 2), (9001, 60, 4)]
+          (700, 256, 32), (130, 300, 5), (90, 1000, 32), (257, 1024, 3), (5000, 8, 2), (9001, 60, 4),
+          (20, 300, 2), (32, 512, 2), (16, 200, 8), (60, 250, 4), (33, 257, 1), (31, 700, 2), (300, 400, 5), (1024, 130, 3), (1025, 500, 3), (8193, 513, 2)]
 
 
 @pytest.mark.parametrize("renormalize", [True, False])
