@@ -614,18 +614,19 @@ __global__ void __launch_bounds__(256, 2) grouped_double_kernel(const GroupedArg
   if (!place_of(p, &at) || !find_group(a, at.m_tile, S, &g)) return;
   const uint32_t row0 = g.tile * S, col0 = at.n_tile * S;
   const double* b = static_cast<const double*>(a.b) + (int64_t)g.index * a.b_stride;
-  double* c = static_cast<double*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
+  double* c = static_cast<double*>(a.c) + at.part * a.c_split + (int64_t)(g.first + row0) * a.ldc + col0;
+  const uint32_t begin = at.part * a.part, count = min(a.part, a.k - begin);
   const uint32_t row = g.first + min(row0 + DoubleRow<S>::row(), g.rows - 1), from = a.index_a ? (uint32_t)a.index_a[row] : row;
   const bool present = from < a.a_rows;
-  const DoubleRow<S> left{static_cast<const double*>(a.a) + (int64_t)(present ? from : 0) * a.lda, a.k, present};
+  const DoubleRow<S> left{static_cast<const double*>(a.a) + (int64_t)(present ? from : 0) * a.lda + begin, count, present};
   auto store = [&](uint32_t r, uint32_t n, double sum) {
     if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
   };
   if constexpr (kB) {
     const uint32_t column = min(col0 + DoubleRow<S>::row(), a.n - 1);
-    double_tile<S>(a.k, left, DoubleRow<S>{b + (int64_t)column * a.ldb, a.k, true}, store);
+    double_tile<S>(count, left, DoubleRow<S>{b + (int64_t)column * a.ldb + begin, count, true}, store);
   } else {
-    double_tile<S>(a.k, left, DoubleColumns<S>(b + col0, a.ldb, nullptr, 0, a.k, a.k, a.n - col0), store);
+    double_tile<S>(count, left, DoubleColumns<S>(b + (int64_t)begin * a.ldb + col0, a.ldb, nullptr, 0, count, count, a.n - col0), store);
   }
 }
 
@@ -758,32 +759,36 @@ struct Choice {
 // Of k_tiles tiles of k, divided evenly and in pairs of tiles: those of a part.
 int64_t tiles_of_part(int64_t k_tiles, int64_t parts) { return ceil_div(ceil_div(k_tiles, parts), 2) * 2; }
 
+constexpr int64_t kMostParts = 32;
+// Large tiles of parts, a round of blocks at a time, are written at once.
+double write_of_parts(int64_t parts, int64_t blocks) { return parts > 1 ? 6.0 * (double)ceil_div(blocks * parts, kUnits) : 0.0; }
+
 // Tiles of 64 and 128 a side, with k in one part or several, against the best so far.  The times of 64 products of 2 and 8 even groups,
 // 64 to 1024 rows each, k 1024 to 4096: 5 % above the best plan's of each.  Us of one part and of what is chosen: 2 groups of 128 rows,
 // k 4096, n 1024: 89 and 29; 8 groups of 64, k 4096, n 1024: 88 and 52; of the weights' products 8 groups of 4096 rows, 128 by 128: 110 and 47.
-// Blocks of 128 a side write their parts at once, 6 us a round.
-constexpr int64_t kMostParts = 32;
 void consider_parts(Choice* best, int64_t blocks64, int64_t blocks128, int64_t k_tiles, int64_t cells, int64_t most_parts) {
   for (int64_t parts = 1; parts <= most_parts; parts *= 2) {
     const int64_t tiles = parts == 1 ? k_tiles : tiles_of_part(k_tiles, parts);
     if (parts > 1 && tiles * (parts - 1) >= k_tiles) break;   // the last part would have none
     const double sum = time_of_sum(parts, cells, sizeof(float));
-    const double medium = time_of_medium(blocks64 * parts, tiles) + sum, large = time_of_large(blocks128 * parts, tiles) + sum + (parts > 1 ? 6.0 * (double)ceil_div(blocks128 * parts, kUnits) : 0.0);
+    const double medium = time_of_medium(blocks64 * parts, tiles) + sum, large = time_of_large(blocks128 * parts, tiles) + sum + write_of_parts(parts, blocks128);
     if (medium < best->us) *best = {64, 64, parts, medium};
     if (large < best->us) *best = {128, 128, parts, large};
   }
 }
 
-// The same of double, tiles of 32 and 64 a side: one block's steps over twice the mean k, for groups are seldom even (7 groups of 290
-// rows in the mean, 301 by 517: 35 us in tiles of 32, 56 in tiles of 64, which take 18 where they are even), or those of all blocks.
-double time_of_double(int64_t side, int64_t blocks, int64_t k) {
-  const double b = (double)blocks;
-  return 4.0 + 0.001 * (double)k * (side == 32 ? std::max(2 * 20.0, 13.0 + 0.046 * b) : std::max(2 * 54.0, 15.0 + 0.145 * b));
+// The same of double, tiles of 32 and 64 a side: one block's steps over the longest sum, or those of all blocks over the mean one.  Of
+// the weights' products the longest is taken to be twice the mean, for groups are seldom even (7 groups of 290 rows in the mean, 301 by
+// 517: 35 us in tiles of 32, 56 in tiles of 64, which take 18 where they are even).
+double time_of_double(int64_t side, int64_t blocks, double mean_k, double longest_k) {
+  const double one = side == 32 ? 0.020 : 0.054;
+  const double all = side == 32 ? 0.010 + 0.0000475 * (double)blocks : 0.015 + 0.037 * (double)ceil_div(blocks, kUnits);
+  return 4.0 + std::max(longest_k * one, mean_k * all);
 }
-void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks64, int64_t k, int64_t cells, int64_t most_parts) {
-  for (int64_t parts = 1; parts <= most_parts && k >= parts * 64; parts *= 2) {
-    const double sum = time_of_sum(parts, cells, sizeof(double));
-    const double small = time_of_double(32, blocks32 * parts, ceil_div(k, parts)) + sum, large = time_of_double(64, blocks64 * parts, ceil_div(k, parts)) + sum;
+void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks64, int64_t mean_k, int64_t longest_k, int64_t cells, int64_t most_parts) {
+  for (int64_t parts = 1; parts <= most_parts && (parts == 1 || mean_k >= parts * 64); parts *= 2) {
+    const double sum = time_of_sum(parts, cells, sizeof(double)), mean = (double)mean_k / (double)parts, longest = (double)longest_k / (double)parts;
+    const double small = time_of_double(32, blocks32 * parts, mean, longest) + sum, large = time_of_double(64, blocks64 * parts, mean, longest) + sum + write_of_parts(parts, blocks64);
     if (small < best->us) *best = {32, 32, parts, small};
     if (large < best->us) *best = {64, 64, parts, large};
   }
@@ -834,16 +839,29 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
   g.n = (uint32_t)b_col_count; g.k = (uint32_t)a_col_count;
   g.trans_b = trans_b != 0;
   const int64_t even_groups = std::min(n_groups, row_count);
+  const int64_t cells = row_count * b_col_count;
+  auto row_tiles_of = [&](int64_t height) { return even_groups * ceil_div(row_count / even_groups, height); };   // if the groups are even
+  auto blocks_of = [&](int64_t side) { return row_tiles_of(side) * ceil_div(b_col_count, side); };
   if (dtype == CT_F64 && a_row_count > 0 && a_col_count > 0) {
-    const int64_t tiles64 = (row_count / 64 + even_groups / 2) * ceil_div(b_col_count, 64), side = tiles64 >= 1024 ? 64 : 32;
-    const int64_t m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
+    auto choose = [&](int64_t most_parts) {
+      Choice best{32, 32, 1, 1e12};
+      consider_double_parts(&best, blocks_of(32), blocks_of(64), a_col_count, a_col_count, cells, most_parts);
+      return best;
+    };
+    Choice best = choose(kMostParts);
+    const Parts<double> parts(s, best.parts, cells);
+    if (parts.count() < best.parts) best = choose(1);
+    const int64_t side = best.height, m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
     if (m_tiles * n_tiles <= kMostUnits) {
-      const Launch l = launch_of(m_tiles, n_tiles, 1);
-      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), l.grid, dim3(256), 0, s, g, l.plan);
-      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), l.grid, dim3(256), 0, s, g, l.plan);
-      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), l.grid, dim3(256), 0, s, g, l.plan);
-      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), l.grid, dim3(256), 0, s, g, l.plan);
-      note_kernel("grouped_double");
+      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
+      GroupedArgs of_parts = parts.args(g, 0);
+      of_parts.part = (uint32_t)ceil_div(a_col_count, parts.count());
+      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
+      parts.add_up<false>(g);
+      note_kernel(parts.count() > 1 ? "grouped_double+grouped_sum" : "grouped_double");
       return after_launch(s);
     }
   }
@@ -851,11 +869,9 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
     // The tiles that there are if the groups are even, and the kernel that takes them soonest.  With 4096 by 1024 [n][k] and 8 groups,
     // us with 16 columns to a block, 64, and tiles of 64 and 128 a side: of one row 28, 34, 88 and 151; of 32 rows 60, 40, 88 and 153; of
     // 128 rows 228, 145, 89 and 150; with 32 groups of 128 rows 910, 568, 286 and 217.
-    const int64_t k_tiles = ceil_div(a_col_count, kTileDepth), cells = row_count * b_col_count;
-    auto tiles_of = [&](int64_t height) { return even_groups * ceil_div(row_count / even_groups, height); };
-    const double thin64 = time_of_thin64(tiles_of(16) * ceil_div(b_col_count, 64), k_tiles);
-    const double thin16 = time_of_thin16(tiles_of(16) * ceil_div(b_col_count, 16), k_tiles);
-    auto blocks_of = [&](int64_t side) { return tiles_of(side) * ceil_div(b_col_count, side); };
+    const int64_t k_tiles = ceil_div(a_col_count, kTileDepth);
+    const double thin64 = time_of_thin64(row_tiles_of(16) * ceil_div(b_col_count, 64), k_tiles);
+    const double thin16 = time_of_thin16(row_tiles_of(16) * ceil_div(b_col_count, 16), k_tiles);
     auto choose = [&](int64_t most_parts) {
       Choice best{16, thin16 < thin64 ? 16 : 64, 1, std::min(thin64, thin16)};
       if (a_col_count >= kTileDepth && b_colstride <= kMostSplitLd) consider_parts(&best, blocks_of(64), blocks_of(128), k_tiles, cells, most_parts);
@@ -953,7 +969,7 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
   if (dtype == CT_F64) {
     auto choose = [&](int64_t most_parts) {
       Choice best{32, 32, 1, 1e12};
-      consider_double_parts(&best, blocks_of(32), blocks_of(64), mean, cells, most_parts);
+      consider_double_parts(&best, blocks_of(32), blocks_of(64), mean, 2 * mean, cells, most_parts);
       return best;
     };
     Choice best = choose(kMostParts);

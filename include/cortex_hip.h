@@ -165,8 +165,9 @@ int ct_stream_destroy(void* stream);
  * allocates a new one.  A caller that wants no allocation and no synchronisation inside later
  * calls (a latency-critical loop, a stream about to be captured into a graph) reserves once:
  * partial_bytes for the partial results of split reductions, matrix-vector products, convolution
- * passes and batch-normalization statistics (reductions never need more than 16 MiB), and as much
- * again, up to 256 MiB, for those of float matrix products (ct_gemm), which have blocks of their own:
+ * passes, batch-normalization statistics and the calls of residual blocks that say so (reductions never
+ * need more than 16 MiB), and as much again, up to 256 MiB, for those of float matrix products (ct_gemm)
+ * and of products by group (ct_grouped_gemm, ct_grouped_gemm_weights), which have blocks of their own:
  * those grow without synchronising, and the smaller ones stay until the stream is destroyed;
  * accumulate_bytes for each of the two blocks that accumulations into a broadcast or indexed
  * destination stage their temporaries through (at most the destination's size times the updates'
@@ -607,7 +608,8 @@ int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims*
  *                          expert, and of (t, j) within one: expert e's are offsets[e] .. offsets[e + 1] - 1; tokens
  *                          holds t at each of these places and -1 beyond offsets[n_experts]; slots holds the place of
  *                          (t, j), -1 for an expert of -1
- * 1 <= n_chosen <= min(32, n_experts), n_experts <= 1024, n * n_chosen < 2^31.  n = 0 writes the offsets only. */
+ * 1 <= n_chosen <= min(32, n_experts), n_experts <= 1024, n * n_chosen < 2^31.  n = 0 writes the offsets only.  More than a
+ * few tokens need scratch memory of the stream, up to 8 MiB. */
 int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* offsets, int32_t* tokens,
                      int32_t* slots, const void* logits, int64_t logits_colstride, int64_t n,
                      int64_t n_experts, int64_t n_chosen, int renormalize, int dtype);
@@ -625,7 +627,9 @@ int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logit
  * with op(b_e) [a_col_count, b_col_count], b_e = b + e * b_stride stored so, or transposed if trans_b.  index (NULL: i
  * itself) selects rows of a [a_row_count, a_col_count]; one outside [0, a_row_count) is a row of zeros.  offsets
  * [n_groups + 1] do not decrease and lie in [0, row_count]; rows of no group are not touched.  Groups of no rows cost
- * nothing.  Float products are formed as ct_gemm's are; c overlaps no operand. */
+ * nothing.  Float products are formed as ct_gemm's are, or by float instructions where groups have few rows; c overlaps no
+ * operand.  Few results of long sums are summed in parts that a second launch adds up, here and below, in scratch memory of the
+ * stream; a captured stream that has none does without, which may differ in the last bits. */
 int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, double alpha, const void* a,
                     int64_t a_row_count, int64_t a_col_count, int64_t a_colstride, const int32_t* index,
                     const void* b, int64_t b_col_count, int64_t b_colstride, int64_t b_stride,
@@ -661,7 +665,8 @@ int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_
  * gradients, outputs and counts are HOST arrays (of device addresses and lengths), read before the call returns; an output may be
  * its gradient (and overlaps nothing otherwise), and outputs may be NULL: then only the norm is formed.  norm_and_factor [2], in the tensors' type, in
  * device memory, receives both.  max_norm > 0; infinity never clips.  A NaN among the gradients makes norm, factor and
- * every output NaN; an infinity makes the factor 0. */
+ * every output NaN; an infinity makes the factor 0.  Scratch memory of the stream: 8 bytes to a piece of 4 KiB or more, 16 KiB
+ * to 120 gradients at most. */
 int ct_clip_gradients(void* stream, const void* const* gradients, void* const* outputs,
                       const int64_t* counts, int64_t count, double max_norm, void* norm_and_factor,
                       int dtype);

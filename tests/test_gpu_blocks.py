@@ -560,6 +560,34 @@ def test_grouped_gemm_whose_sums_are_divided(stream, size, trans_b):
     D.free()
 
 
+@pytest.mark.parametrize("trans_b", [True, False])
+@pytest.mark.parametrize("size", [(2, 9, 2500, 55), (29, 11, 2532, 55), (1, 40, 1031, 33), (3, 200, 4100, 70)], ids=str)
+def test_grouped_gemm_in_double_whose_sums_are_divided(stream, size, trans_b):
+    D = Owned("double")
+    groups, rows, k, n = size
+    for turn, (kind, whole, alpha, beta) in enumerate((("any", True, 1.0, 0.0), ("short", False, 1.5, 0.0), ("one", False, -0.5, 0.75))):
+        rng = np.random.default_rng(rows + k + turn)
+        make = (lambda *s: rng.integers(-7, 8, s).astype(np.float64)) if whole else (lambda *s: rng.standard_normal(s))
+        offsets = offsets_of(rng, groups, rows, kind)
+        index = rng.integers(0, rows, rows)
+        index[::7] = rng.choice([-1, rows, 1 << 30], len(index[::7]))
+        a, c = make(rows, k), make(rows, n)
+        b = make(groups, n, k) if trans_b else make(groups, k, n)
+        tc = D.block(c, turn)
+        blocks.grouped_gemm(tc, trans_b, alpha, D.block(a, turn), D.tensor(b), beta, D.tensor(offsets, "int"), index=D.tensor(index, "int"))
+        assert capi.last_kernel() == "grouped_double+grouped_sum"
+        want, scale = grouped64(a, index, b, trans_b, offsets, c, alpha, beta)
+        got = read(tc)
+        inside = np.zeros(rows, bool)
+        inside[offsets[0]:offsets[-1]] = True
+        assert np.array_equal(got[~inside], c[~inside]), "rows of no group were written"
+        if whole:
+            assert np.array_equal(got, want)
+        else:
+            close(got, want, scale, (k + 4) * 2.0 ** -53, kind)
+    D.free()
+
+
 @pytest.mark.parametrize("size", [(2, 9000, 130, 70), (3, 7001, 33, 65), (1, 5000, 64, 64)], ids=str)
 def test_grouped_gemm_weights_whose_sums_are_divided(D, size):
     groups, rows, m, n = size
