@@ -5,7 +5,8 @@
 //
 // The tensors are cut into pieces; a launch's blocks take every so manieth piece, form one sum of squares each, and the norm is
 // the sum of those in their order.  A few sums are added by every block that needs the factor, more by a launch of their own.
-// The pieces are multiplied by the factor last to first: what was read last is still in the last-level cache.
+// The pieces are multiplied by the factor last to first: what was read last is still in the last-level cache.  Memory bounds it: 171
+// million floats in 300 tensors 377 us, two reads and a write at 5.5 TB/s (first to last 436).
 // The tensors travel in the launch's arguments, kTensors to a launch: a table in device memory would have to be copied there
 // by every call.
 #include <algorithm>
@@ -21,7 +22,7 @@ namespace {
 constexpr int kClipBlock = 256;
 constexpr int kTensors = 120;
 constexpr int64_t kMostClipBlocks = 2048;   // of a launch: what the chip holds
-constexpr int64_t kFewSums = 512;           // which every block adds by itself
+constexpr int64_t kFewSums = 2048;          // which every block adds by itself (19 tensors, 4.9 million floats: 15.9 us, with a launch for them 18.5)
 constexpr int64_t kLeastPiece = 4 << 10, kMostPiece = 64 << 10;   // bytes
 constexpr int64_t kClipCacheBytes = int64_t(256) << 20;
 
