@@ -32,6 +32,15 @@ def stream():
     s.release()
 
 
+@pytest.fixture()
+def as_released():
+    """Debug-sync mode off, as a user runs, and on again for the other tests."""
+    capi.call("ct_set_device", 0)
+    capi.call("ct_set_debug_sync", 0)
+    yield
+    capi.call("ct_set_debug_sync", 1)
+
+
 class Owned:
     """Tensors on the device, freed together; a matrix may be a block of a wider one, whose rest must stay as it is."""
 
@@ -829,13 +838,11 @@ def test_operands_that_only_the_checks_in_python_take(stream, monkeypatch):
 
 # ------------------------------------------------------------------------------------------------- graphs
 
-def test_calls_recorded_into_a_graph():
+def test_calls_recorded_into_a_graph(as_released):
     """A step of every operator, recorded with the scratch that the stream holds and replayed with new inputs, eager calls of
     the same step in between: each replay's results are the eager ones, bit for bit."""
     import ctypes as C
     rt = C.CDLL("libamdhip64.so")
-    capi.call("ct_set_device", 0)
-    capi.call("ct_set_debug_sync", 0)
     stream = drv.HipDriver().default_device().create_stream()
     D = Owned("float")
     rng = np.random.default_rng(43)
@@ -911,10 +918,9 @@ def test_calls_recorded_into_a_graph():
         assert rt.hipGraphExecDestroy(graph_exec) == 0 and rt.hipGraphDestroy(graph) == 0
         D.free()
     stream.release()
-    capi.call("ct_set_debug_sync", 1)
 
 
-def test_divided_sums_recorded_without_scratch_do_without():
+def test_divided_sums_recorded_without_scratch_do_without(as_released):
     """A capture that finds no scratch for the parts: one launch, and the same whole numbers."""
     import ctypes as C
     rt = C.CDLL("libamdhip64.so")
@@ -923,8 +929,6 @@ def test_divided_sums_recorded_without_scratch_do_without():
     rt.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
     rt.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
     rt.hipGraphExecDestroy.argtypes = rt.hipGraphDestroy.argtypes = [C.c_void_p]
-    capi.call("ct_set_device", 0)
-    capi.call("ct_set_debug_sync", 0)
     rng = np.random.default_rng(45)
     for datatype in ("float", "double"):
         D = Owned(datatype)
@@ -967,15 +971,12 @@ def test_divided_sums_recorded_without_scratch_do_without():
             D.free()
         stream.release()
         loader.release()
-    capi.call("ct_set_debug_sync", 1)
 
 
 # ------------------------------------------------------------------------------------------------- streams
 
-def test_calls_on_two_streams_do_not_meet():
+def test_calls_on_two_streams_do_not_meet(as_released):
     """Each stream has its own scratch memory: the same calls on two streams at once give what each gives alone."""
-    capi.call("ct_set_device", 0)
-    capi.call("ct_set_debug_sync", 0)
     device = drv.HipDriver().default_device()
     rng = np.random.default_rng(41)
     results = []

@@ -12,6 +12,15 @@ from cortex_amd import tensor as ct
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture()
+def as_released():
+    """Debug-sync mode off, as a user runs, and on again for the other tests."""
+    capi.call("ct_set_device", 0)
+    capi.call("ct_set_debug_sync", 0)
+    yield
+    capi.call("ct_set_debug_sync", 1)
+
+
 def made(rng, tokens, width, hidden, experts, datatype, biases):
     shapes = {"router": ([experts, width], 1.0), "first": ([experts, hidden, width], width ** -0.5),
               "second": ([experts, width, hidden], hidden ** -0.5)}
@@ -63,10 +72,8 @@ def test_a_block_s_gradients_are_the_differences(kinds, renormalize):
     stream.release()
 
 
-def test_a_few_training_steps_lower_the_loss():
+def test_a_few_training_steps_lower_the_loss(as_released):
     """Mean squared distance from the results of another block of the same kind: forward, backward, clipping, Adam."""
-    capi.call("ct_set_device", 0)
-    capi.call("ct_set_debug_sync", 0)
     stream = drv.HipDriver().default_device().create_stream()
     rng = np.random.default_rng(4)
     tokens, width, hidden, experts, chosen = 256, 64, 96, 8, 2
