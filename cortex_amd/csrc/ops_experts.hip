@@ -7,7 +7,7 @@
 // instructions, some hundred to a choice of a wave's four tokens: 65536 tokens, 8 of 128 experts, 28 us of 41; 14 for the gradient, which is bound by memory.
 //
 // Combining reads the rows of a token once and writes its sum; its gradient reads the token's gradient and its rows once and
-// writes as many.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us (4.8 TB/s) and 120 (4.9).
+// writes as many.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us (4.8 TB/s) and 108 (5.4).
 #include <algorithm>
 
 #include "elementwise.h"
@@ -540,132 +540,7 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const CombineArg
   }
 }
 
-// WAVES waves to a token, whose rows are taken R at a time, a lot.  What a wave uses next is on its way while it uses
-// a piece: the lot's next piece, or the first one of the next lot or token.  The token's gradient is read again, from the caches,
-// for every lot.
-template <class T, int WAVES, int R, bool kStreaming>
-__global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const CombineArgs a) {
-  constexpr uint32_t N = Quad<T>::N, kTokens = kCombineBlock / 64 / WAVES;
-  __shared__ T lds[2][kCombineBlock / 64][R];
-  int turn = 0;
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = a.n_chosen;
-  const uint32_t of_token = threadIdx.x % (64 * WAVES), stride = 64 * WAVES * N, pieces = (a.width + stride - 1) / stride;
-  const bool dots = a.weights_gradient != nullptr;
-  struct Lot {
-    uint32_t token, j0;   // a token beyond the last one is read as that, and not stored: a block's waves go on together
-    const T* dy;
-    const T* row[R];
-    int32_t slot[R];      // negative: not used
-    T weight[R];
-  };
-  int32_t slots = 0, slots_ahead;   // of the lot's token and the next one, an assignment to a lane
-  T weights = T(0), weights_ahead;
-  auto look_up = [&](uint32_t token) {
-    const int64_t at = (int64_t)min(token, a.n - 1) * k + min(lane, k - 1);
-    slots_ahead = a.slots[at];
-    weights_ahead = a.weights ? static_cast<const T*>(a.weights)[at] : T(1);
-  };
-  auto lot_of = [&](uint32_t token, uint32_t j0) {
-    Lot l;
-    l.token = token;
-    l.j0 = j0;
-    l.dy = static_cast<const T*>(a.output_gradient) + (int64_t)min(token, a.n - 1) * a.gradient_colstride;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const uint32_t j = min(j0 + r, k - 1u);
-      const int32_t slot = __builtin_amdgcn_readlane(slots, j);
-      const bool in = token < a.n && j0 + r < k && slot >= 0 && slot < a.row_count;
-      l.slot[r] = in ? slot : -1;
-      l.weight[r] = from_lane(weights, j);
-      // one that is not used reads the gradient in its place
-      l.row[r] = in && dots ? static_cast<const T*>(a.rows) + (int64_t)slot * a.rows_colstride : l.dy;
-    }
-    return l;
-  };
-  Quad<T> g, x[R], g_next, x_next[R];
-  auto load = [&](const Lot& l, uint32_t piece, Quad<T>& g, Quad<T> (&x)[R]) {
-    const RowPart<T> at(min(of_token * N + piece * stride, a.width), a.width);
-    g = at.template load<false>(l.dy);
-#pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = at.template load<kStreaming>(l.row[r]);
-  };
-  const uint32_t step = gridDim.x * kTokens;
-  uint32_t first = blockIdx.x * kTokens;   // token of the block's first wave
-  auto next_token = [&] {
-    slots = slots_ahead;
-    weights = weights_ahead;
-    look_up(first + step + wave / WAVES);
-  };
-  look_up(first + wave / WAVES);
-  next_token();
-  Lot lot = lot_of(first + wave / WAVES, 0);
-  load(lot, 0, g, x);
-  while (first < a.n) {
-    T dot[R] = {};
-    Lot next = lot;
-    for (uint32_t piece = 0; piece < pieces; ++piece) {
-      uint32_t ahead = piece + 1;
-      if (ahead == pieces) {
-        ahead = 0;
-        if (lot.j0 + R < k) {
-          next = lot_of(lot.token, lot.j0 + R);
-        } else {
-          first += step;
-          next_token();
-          next = lot_of(first + wave / WAVES, 0);
-        }
-      }
-      load(next, ahead, g_next, x_next);
-      const RowPart<T> at(of_token * N + piece * stride, a.width);
-      const bool some = at.place < a.width;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (a.output && lot.slot[r] >= 0 && some) {
-          Quad<T> q;
-#pragma unroll
-          for (uint32_t e = 0; e < N; ++e) q.v[e] = lot.weight[r] * g.v[e];
-          at.template store<kStreaming>(static_cast<T*>(a.output) + (int64_t)lot.slot[r] * a.output_colstride, q);
-        }
-#pragma unroll
-        for (uint32_t e = 0; e < N; ++e) dot[r] += at.owns(e) ? g.v[e] * x[r].v[e] : T(0);
-        x[r] = x_next[r];
-      }
-      g = g_next;
-    }
-    if (dots) {
-#pragma unroll
-      for (int m = 32; m > 0; m >>= 1)
-#pragma unroll
-        for (int r = 0; r < R; ++r) dot[r] += __shfl_xor(dot[r], m);
-#pragma unroll
-      for (int r = 0; r < R; ++r) dot[r] = lot.slot[r] >= 0 ? dot[r] : T(0);
-      T* result = static_cast<T*>(a.weights_gradient) + (int64_t)lot.token * k + lot.j0;
-      const bool stored = lot.token < a.n && lane < (uint32_t)R && lot.j0 + lane < k;
-      if constexpr (WAVES == 1) {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (stored && lane == (uint32_t)r) result[r] = dot[r];
-      } else {
-        if (lane == 0) {
-#pragma unroll
-          for (int r = 0; r < R; ++r) lds[turn][wave][r] = dot[r];
-        }
-        __syncthreads();
-        if (stored && wave % WAVES == 0) {
-          T sum = lds[turn][wave][lane];
-#pragma unroll
-          for (int v = 1; v < WAVES; ++v) sum += lds[turn][wave + v][lane];
-          result[lane] = sum;
-        }
-        turn ^= 1;   // written again only after another barrier
-      }
-    }
-    lot = next;
-  }
-}
-
 constexpr int64_t kWavesOfTheChip = 256 * 32;
-constexpr int64_t kGradientBlocks = 256 * 4;   // that the chip holds
 
 template <class T>
 void combine_launch(hipStream_t s, const CombineArgs& a) {
@@ -680,25 +555,72 @@ void combine_launch(hipStream_t s, const CombineArgs& a) {
   else hipLaunchKernelGGL((combine_kernel<T, false>), grid, dim3(kCombineBlock), 0, s, a, (uint32_t)parts, (uint32_t)run, (uint32_t)units);
 }
 
+// LANES lanes to an assignment, each by itself: its row's gradient, and the product of its row with the token's gradient.  That is read
+// again for each of its rows, out of the caches, and nothing waits for another row.  (A wave to a token, two or four rows at a time with the
+// next ones on their way, was as fast for 16384 tokens of 4 rows of 1000 floats, 125 us, and slower elsewhere: 60000 tokens of 8 rows of 64
+// floats 113 us and 48 so; one token of 8 rows of 4096 doubles 19 and 6.)
+template <class T, int LANES, bool kStreaming>
+__global__ void __launch_bounds__(kCombineBlock) combine_gradient_kernel(const CombineArgs a, uint32_t assignments, FastDiv k_fd) {
+  constexpr uint32_t N = Quad<T>::N, kGroups = kCombineBlock / LANES;
+  __shared__ T lds[2][kCombineBlock / 64];
+  int turn = 0;
+  const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const bool dots = a.weights_gradient != nullptr;
+  for (uint32_t unit0 = blockIdx.x * kGroups; unit0 < assignments; unit0 += gridDim.x * kGroups) {
+    const uint32_t unit = min(unit0 + group, assignments - 1);
+    const int32_t slot = a.slots[unit];
+    const bool in = slot >= 0 && slot < a.row_count;
+    const T weight = a.weights ? static_cast<const T*>(a.weights)[unit] : T(1);
+    const T* dy = static_cast<const T*>(a.output_gradient) + (int64_t)k_fd.div(unit) * a.gradient_colstride;
+    const T* row = in && dots ? static_cast<const T*>(a.rows) + (int64_t)slot * a.rows_colstride : dy;
+    T* to = static_cast<T*>(a.output) + (int64_t)(in ? slot : 0) * a.output_colstride;
+    T dot = 0;
+#pragma unroll 4
+    for (uint32_t place = lane * N; place < a.width; place += LANES * N) {
+      const RowPart<T> at(place, a.width);
+      Quad<T> g = at.template load<false>(dy);
+      const Quad<T> x = at.template load<kStreaming>(row);
+#pragma unroll
+      for (uint32_t e = 0; e < N; ++e) {
+        dot += at.owns(e) ? g.v[e] * x.v[e] : T(0);
+        g.v[e] *= weight;
+      }
+      if (a.output && in && unit0 + group < assignments) at.template store<kStreaming>(to, g);
+    }
+    if (!dots) continue;
+#pragma unroll
+    for (int m = (LANES < 64 ? LANES : 64) / 2; m > 0; m >>= 1) dot += __shfl_xor(dot, m);
+    if constexpr (LANES > 64) {
+      T* mine = lds[turn];
+      turn ^= 1;
+      if (threadIdx.x % 64 == 0) mine[threadIdx.x / 64] = dot;
+      __syncthreads();
+      dot = mine[0];
+#pragma unroll
+      for (int w = 1; w < LANES / 64; ++w) dot += mine[w];
+    }
+    if (lane == 0 && unit0 + group < assignments) static_cast<T*>(a.weights_gradient)[unit] = in ? dot : T(0);
+  }
+}
+
 template <class T>
 void combine_gradient_launch(hipStream_t s, const CombineArgs& a) {
   const bool past = (int64_t)a.n * (2 * a.n_chosen + 1) * a.width * (int64_t)sizeof(T) > kCombineCacheBytes;
-  // a wave to a token, four where that leaves compute units without work
-  const bool few = a.n < 4096 && a.width > 256;
-  const int64_t blocks = std::min<int64_t>(few ? a.n : (a.n + 3) / 4, few ? kMostBlocks : kGradientBlocks);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kCombineBlock), 0, s, a); };
-  // four rows at a time where the caches hold them (4096 tokens of 4 rows of 1024 floats: 25 us, two at a time 27), two where they
-  // do not (16384 tokens: 118 us, four 139: fewer registers, more waves)
-  auto of_rows = [&](auto rows) {
-    constexpr int R = decltype(rows)::value;
-    if (few && past) launch(combine_gradient_kernel<T, 4, R, true>);
-    else if (few) launch(combine_gradient_kernel<T, 4, R, false>);
-    else if (past) launch(combine_gradient_kernel<T, 1, R, true>);
-    else launch(combine_gradient_kernel<T, 1, R, false>);
-  };
-  if (a.n_chosen == 1) of_rows(std::integral_constant<int, 1>());
-  else if (a.n_chosen == 2 || past) of_rows(std::integral_constant<int, 2>());
-  else of_rows(std::integral_constant<int, 4>());
+  const int64_t assignments = (int64_t)a.n * a.n_chosen, pieces = (a.width + Quad<T>::N - 1) / Quad<T>::N;
+  // Lanes by the length of a row, and all of a block where there are too few rows for the chip, or where the caches do not hold long ones.  Us with
+  // 16, 64 and 256: 60000 tokens of 4 rows of 64 floats 25, 67 and 222; 2000 of 4 of 1024 15.5, 14.0 and 19.3; 500 of one of 4096 38, 11.8 and
+  // 6.0; 8192 of 4 of 2048 160, 156 and 123.
+  const int lanes = pieces <= 64 ? 16 : assignments <= 1024 || (past && pieces >= 512 && a.n_chosen > 2) ? 256 : 64;
+  const int64_t groups = kCombineBlock / lanes;
+  const dim3 grid((uint32_t)std::min((assignments + groups - 1) / groups, kMostBlocks));
+  const FastDiv k_fd(a.n_chosen);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kCombineBlock), 0, s, a, (uint32_t)assignments, k_fd); };
+  if (lanes == 16 && past) launch(combine_gradient_kernel<T, 16, true>);
+  else if (lanes == 16) launch(combine_gradient_kernel<T, 16, false>);
+  else if (lanes == 64 && past) launch(combine_gradient_kernel<T, 64, true>);
+  else if (lanes == 64) launch(combine_gradient_kernel<T, 64, false>);
+  else if (past) launch(combine_gradient_kernel<T, 256, true>);
+  else launch(combine_gradient_kernel<T, 256, false>);
 }
 
 constexpr int64_t kMostRows = (int64_t(1) << 31) - 1;
