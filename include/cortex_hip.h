@@ -586,7 +586,7 @@ int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, voi
  * overwritten.  input_gradient and residual_gradient may be output_gradient or normalized_gradient itself, but not one
  * another, and no gradient may overlap an operand otherwise.  Column sums run over the rows in double once they leave a
  * block's registers; the partial sums live in the stream's scratch memory (at most
- * 32 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
+ * 64 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
 int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims,
                               void* residual_gradient, const ct_dims* residual_gradient_dims,
                               void* gate_gradient, void* post_scale_gradient, void* post_bias_gradient,

@@ -243,6 +243,34 @@ def test_norm_residual_sums_over_many_rows(D, shape, gate):
     check_norm(D, *shape, "rms", "rms", gate, biases=False, residual=True, pad=1, seed=4)
 
 
+@pytest.mark.parametrize("gate", ["column", "row", "full", "scalar", None])
+@pytest.mark.parametrize("shape", [(40, 4500), (7, 8192), (300, 9001), (5, 16384)], ids=str)
+def test_norm_residual_whose_sums_take_two_passes(D, shape, gate):
+    """The sums of scales and of biases, which LDS does not hold together."""
+    check_norm(D, *shape, "layer", "layer", gate, biases=True, residual=True, pad=1, seed=6)
+
+
+def test_norm_gradient_in_place_of_two_passes(D):
+    """The gradients of the results overwritten: the same bits as into memory of their own."""
+    rng = np.random.default_rng(49)
+    rows, width = 30, 8192 if D.datatype == "double" else 12000
+    make = lambda *s: rng.standard_normal(s)
+    d = blocks.norm_descriptor(post="layer", pre="layer")
+    p = {k: D.tensor(make(width)) for k in ("post-scale", "post-bias", "pre-scale", "pre-bias")}
+    z, out, h, statistics = D.tensor(make(rows, width)), D.tensor(np.zeros((rows, width))), D.tensor(np.zeros((rows, width))), D.tensor(np.zeros((4, rows)))
+    blocks.norm_residual(out, h, statistics, z, D.tensor(make(rows, width)), p, d)
+    dout, dh = make(rows, width), make(rows, width)
+    results = []
+    for in_place in (False, True):
+        tout, th = D.tensor(dout), D.tensor(dh)
+        dz, dr = (th, tout) if in_place else (D.tensor(np.zeros((rows, width))), D.tensor(np.zeros((rows, width))))
+        g = {k: D.tensor(np.zeros(width)) for k in p}
+        blocks.norm_residual_gradient(dz, dr, g, tout, th, z, out, statistics, p, d)
+        results.append([read(t) for t in (dz, dr, *g.values())])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b) and np.any(a != 0)
+
+
 @pytest.mark.parametrize("kinds", [("rms", "rms"), ("layer", "layer"), ("none", "layer")], ids="-".join)
 @pytest.mark.parametrize("shape", LONG, ids=str)
 def test_norm_residual_of_long_rows(D, shape, kinds):
