@@ -799,7 +799,8 @@ void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks64, int
 // Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
 // from 1024 on eight or sixteen are as fast or faster.
 constexpr int64_t kFewK = 768;
-constexpr int64_t kMostUnits = int64_t(1) << 22, kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
+// Tiles of a launch: 2^32 lanes or more are refused, and a block has up to 1024.
+constexpr int64_t kMostUnits = int64_t(1) << 21, kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
 
 uint32_t tiles_of(int64_t n, int64_t side) { return (uint32_t)((n + side - 1) / side); }
 

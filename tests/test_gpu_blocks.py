@@ -678,6 +678,58 @@ def test_grouped_gemm_weights_of_an_operand_beyond_four_gib(stream):
     D.free()
 
 
+def test_grouped_products_without_terms_or_rows(D, stream):
+    """Sums of no terms, and operands without rows, whose indexes all lie outside: beta times what was there, in the groups' rows."""
+    code = capi.DTYPE_CODES[D.datatype]
+    rows, k, n = 9, 5, 6
+    offsets, index = D.tensor([0, 4, 7], "int"), D.tensor(np.arange(rows), "int")
+    b = D.tensor(np.ones((2, n, k)))
+    for a_rows, terms in ((rows, 0), (0, k)):
+        for beta in (0.0, 0.5):
+            c = np.arange(rows * n, dtype=D.type).reshape(rows, n) + 1
+            tc = D.tensor(c)
+            capi.call("ct_grouped_gemm", stream.handle, tc.buffer.ptr, n, 1, 1.0, None, a_rows, terms, k, index.buffer.ptr, b.buffer.ptr, n, k,
+                      n * k, offsets.buffer.ptr, 2, rows, beta, code)
+            assert np.array_equal(read(tc), np.concatenate([beta * c[:7], c[7:]]))
+    y = D.tensor(np.ones((rows, n)))
+    for beta in (0.0, 0.5):
+        w = np.arange(2 * k * n, dtype=D.type).reshape(2, k, n) + 1
+        tw = D.tensor(w)
+        capi.call("ct_grouped_gemm_weights", stream.handle, tw.buffer.ptr, n, k * n, 1.0, None, 0, k, k, index.buffer.ptr, y.buffer.ptr, rows, n, n,
+                  None, offsets.buffer.ptr, 2, rows, beta, code)
+        assert np.array_equal(read(tw), beta * w)
+
+
+def test_grouped_products_of_rows_far_apart(stream):
+    """Further than the tiles' 32-bit offsets reach: a matrix's rows 2^22 floats and more apart, and operands of the weights' products
+    2^30 and more.  Whole numbers: every sum exact."""
+    D = Owned("float")
+    rng = np.random.default_rng(53)
+    rows, k, n, ld = 200, 64, 5, (1 << 22) + 3
+    a, b = rng.integers(-7, 8, (rows, k)).astype(np.float32), rng.integers(-7, 8, (n, k)).astype(np.float32)
+    far = ct.new_tensor([n * ld], datatype="float")
+    D.kept.append(far)
+    for r in range(n):
+        row = D.tensor(b[r])
+        capi.call("ct_memcpy_async", far.buffer.ptr + 4 * ld * r, row.buffer.ptr, 4 * k, capi.COPY_D2D, stream.handle)
+    offsets, c = D.tensor([0, rows], "int"), D.tensor(np.zeros((rows, n)))
+    capi.call("ct_grouped_gemm", stream.handle, c.buffer.ptr, n, 1, 1.0, D.tensor(a).buffer.ptr, rows, k, k, None, far.buffer.ptr, n, ld, n * ld,
+              offsets.buffer.ptr, 1, rows, 0.0, capi.F32)
+    assert np.array_equal(read(c), a @ b.T)
+    ld = (1 << 30) + 5
+    x, y = rng.integers(-7, 8, (2, 70)).astype(np.float32), rng.integers(-7, 8, (2, 33)).astype(np.float32)
+    far = ct.new_tensor([ld + 70], datatype="float")
+    D.kept.append(far)
+    for r in range(2):
+        row = D.tensor(x[r])
+        capi.call("ct_memcpy_async", far.buffer.ptr + 4 * ld * r, row.buffer.ptr, 4 * 70, capi.COPY_D2D, stream.handle)
+    offsets, w = D.tensor([0, 2], "int"), D.tensor(np.zeros((1, 70, 33)))
+    capi.call("ct_grouped_gemm_weights", stream.handle, w.buffer.ptr, 33, 70 * 33, 1.0, far.buffer.ptr, 2, 70, ld, None, D.tensor(y).buffer.ptr, 2, 33, 33,
+              None, offsets.buffer.ptr, 1, 2, 0.0, capi.F32)
+    assert np.array_equal(read(w)[0], x.T @ y)
+    D.free()
+
+
 def test_grouped_offsets_that_make_no_sense_stay_inside(D):
     """Offsets that decrease or lie outside the rows are clamped: whatever is computed, nothing beside the result changes."""
     rng = np.random.default_rng(31)
