@@ -7,7 +7,7 @@
 // instructions, some hundred to a choice of a wave's four tokens: 65536 tokens, 8 of 128 experts, 28 us of 41; 14 for the gradient, which is bound by memory.
 //
 // Combining reads the rows of a token once and writes its sum; its gradient reads the token's gradient and its rows once and
-// writes as many.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us (4.8 TB/s) and 108 (5.4).
+// writes as many.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us (4.8 TB/s) and 115 (5.1).
 #include <algorithm>
 
 #include "elementwise.h"
