@@ -793,7 +793,8 @@ int read_gate(const char* what, const void* p, const ct_dims* d, int64_t rows, i
   const int64_t r = last ? d->shape[0] : 1, w = d->shape[last];
   CT_REQUIRE((r == rows || r == 1) && (w == width || w == 1), "%s is [%lld, %lld]: [%lld or 1, %lld or 1] is needed", what, (long long)r,
              (long long)w, (long long)rows, (long long)width);
-  const bool by_row = r == rows && rows > 1, by_column = w == width && width > 1;
+  // of no rows, [0, ..] is a gate by row too: its gradient has no elements, a column sum would be stored behind it
+  const bool by_row = r == rows && rows != 1, by_column = w == width && width > 1;
   CT_REQUIRE(!by_column || d->strides[last] == 1, "%s: the innermost stride must be 1", what);
   *kind = by_row ? (by_column ? kFullGate : kRowGate) : by_column ? kColumnGate : kScalarGate;
   out->ld = by_row ? d->strides[0] : width;

@@ -1,0 +1,41 @@
+"""The operators of residual blocks with experts where a call has next to nothing to do, where operands alias, and where sizes
+pass a threshold between kernels; beside tests/test_gpu_blocks.py, whose formulas and bars they use."""
+import numpy as np
+import pytest
+
+from cortex_amd import blocks
+from cortex_amd import tensor as ct
+from test_gpu_blocks import D, Owned, read, stream, strides_of  # noqa: F401  (fixtures among them)
+
+pytestmark = pytest.mark.gpu
+
+
+def part(D, whole, at, shape):
+    """A dense tensor of `shape` whose elements are those of the vector `whole` from `at` on; perhaps none."""
+    return ct.Tensor(whole.device, {"shape": list(shape), "strides": strides_of(shape)}, whole.buffer.sub_buffer(at, int(np.prod(shape))))
+
+
+# ------------------------------------------------------------------------------------------------- norms of nothing
+
+@pytest.mark.parametrize("biases", [False, True])
+@pytest.mark.parametrize("gate", [(0, 50), (0, 1), (1, 50), (1, 1)], ids=str)
+def test_norm_gradient_of_no_rows_stays_inside_its_gradients(D, gate, biases):
+    """The gradients are parts of one buffer, as those of a network often are: those that have elements are zeros, and what lies
+    behind one that has none is not written."""
+    width = 50
+    shapes = {"post-scale": (width,), "pre-scale": (width,), "gate": gate}
+    if biases:
+        shapes.update({"post-bias": (width,), "pre-bias": (width,)})
+    guard = 64
+    total = sum(int(np.prod(s)) + guard for s in shapes.values())
+    values, flat, want = D.tensor(np.ones(total)), D.tensor(np.full(total, 7.25)), np.full(total, 7.25)
+    p, g, at = {}, {}, 0
+    for k, s in shapes.items():
+        p[k], g[k] = part(D, values, at, s), part(D, flat, at, s)
+        want[at:at + int(np.prod(s))] = 0
+        at += int(np.prod(s)) + guard
+    empty = [D.tensor(np.zeros((0, width))) for _ in range(4)]
+    d = blocks.norm_descriptor(post="layer", pre="rms")
+    blocks.norm_residual(empty[0], empty[1], None, empty[2], empty[3], p, d)
+    blocks.norm_residual_gradient(empty[0], empty[1], g, empty[2], empty[3], empty[0], empty[1], None, p, d)
+    assert np.array_equal(read(flat), want)
