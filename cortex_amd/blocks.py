@@ -48,6 +48,8 @@ def _is_packed(t: Tensor) -> bool:
     shape, expected = t.dimensions["shape"], 1
     if not all(type(n) is int for n in shape):
         return False
+    if 0 in shape:    # whatever its strides
+        return True
     for n, stride in zip(reversed(shape), reversed(t.dimensions["strides"])):
         if n != 1 and stride != expected:
             return False

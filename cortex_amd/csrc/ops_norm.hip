@@ -877,11 +877,17 @@ int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims*
   CT_REQUIRE(input_dims && (input_dims->ndim == 1 || input_dims->ndim == 2), "input: one or two dimensions are taken");
   const int64_t rows = input_dims->ndim == 2 ? input_dims->shape[0] : 1, width = input_dims->shape[input_dims->ndim - 1];
   CT_REQUIRE(rows >= 0 && width >= 0 && width <= kMostWidth, "ct_norm_residual_gradient: bad extent");
-  if (width == 0) return CT_OK;
+  CT_REQUIRE(!gate_gradient || gate, "ct_norm_residual_gradient: a gradient of no gate");
+  if (width == 0) {   // a gate by row or of one value has a gradient all the same: a sum of nothing
+    if (!gate_gradient) return CT_OK;
+    Matrix of_gate;
+    int kind;
+    CT_TRY(read_gate("gate", gate, gate_dims, rows, width, &of_gate, &kind));
+    return ct_memset(stream, gate_gradient, dtype, 0.0, (gate_dims->ndim == 2 ? gate_dims->shape[0] : 1) * gate_dims->shape[gate_dims->ndim - 1]);
+  }
   const bool before = pre_kind != CT_NORM_NONE && normalized_gradient;
   CT_REQUIRE(rows == 0 || (input && (output || !before) && (statistics || (post_kind == CT_NORM_NONE && !before))),
              "ct_norm_residual_gradient: null buffer");
-  CT_REQUIRE(!gate_gradient || gate, "ct_norm_residual_gradient: a gradient of no gate");
   CT_REQUIRE(post_kind != CT_NORM_NONE || (!post_scale_gradient && !post_bias_gradient), "ct_norm_residual_gradient: gradients of no post norm");
   CT_REQUIRE(pre_kind != CT_NORM_NONE || (!pre_scale_gradient && !pre_bias_gradient), "ct_norm_residual_gradient: gradients of no pre norm");
   NormGradientArgs a{};

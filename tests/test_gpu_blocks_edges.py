@@ -39,3 +39,16 @@ def test_norm_gradient_of_no_rows_stays_inside_its_gradients(D, gate, biases):
     blocks.norm_residual(empty[0], empty[1], None, empty[2], empty[3], p, d)
     blocks.norm_residual_gradient(empty[0], empty[1], g, empty[2], empty[3], empty[0], empty[1], None, p, d)
     assert np.array_equal(read(flat), want)
+
+
+@pytest.mark.parametrize("gate", [(7, 1), (1, 1), (7, 0), (1, 0)], ids=str)
+def test_norm_gradient_of_rows_without_elements(D, gate):
+    """A gate's gradient that has elements is a sum of nothing: zeros, and no more of them than it has."""
+    rows, n = 7, int(np.prod(gate))
+    flat, empty = D.tensor(np.full(20, 7.25)), [D.tensor(np.zeros((rows, 0))) for _ in range(4)]
+    p, g = {"gate": part(D, D.tensor(np.ones(20)), 0, gate)}, {"gate": part(D, flat, 2, gate)}
+    d = blocks.norm_descriptor(post="rms", pre="none")
+    blocks.norm_residual_gradient(empty[0], empty[1], g, empty[2], None, empty[3], empty[3], D.tensor(np.zeros((4, rows))), p, d)
+    want = np.full(20, 7.25)
+    want[2:2 + n] = 0
+    assert np.array_equal(read(flat), want)
