@@ -52,15 +52,20 @@ def _buffer(x):
 
 
 def _dense_buffer(x):
-    """The buffer of a tensor whose elements are all of it, or a buffer."""
+    """(a buffer, the order of its elements) of a buffer, or of a tensor whose elements are all of it.  The order is None where
+    they lie as they are counted; else (extent, stride) of every dimension but those of one element."""
     if not hasattr(x, "buffer"):
-        return x
-    from . import tensor as ct
-
+        return x, None
+    shape, strides = x.dimensions["shape"], x.dimensions["strides"]
     n = x.ecount()
-    if n != 1 and not ct.dense(x):
-        raise ValueError("clip_gradients: tensors must be dense")
-    return x.buffer if x.buffer.ecount() == n else x.buffer.sub_buffer(0, n)
+    order = [(extent, stride) for extent, stride in zip(shape, strides) if extent != 1] if n else []
+    expected = 1
+    for extent, stride in sorted(order, key=lambda d: d[1]):
+        if type(extent) is not int or stride != expected:
+            raise ValueError("clip_gradients: tensors must be dense")
+        expected *= extent
+    as_counted = all(a[1] > b[1] for a, b in zip(order, order[1:]))
+    return x.buffer if x.buffer.ecount() == n else x.buffer.sub_buffer(0, n), None if as_counted else order
 
 
 def _ensure_datatype(datatype, *buffers) -> None:
@@ -152,21 +157,23 @@ def clip_gradients(backend: Backend, gradients, max_norm, norm_and_factor, outpu
 
         factor = max_norm / max(norm, max_norm),   outputs = gradients * factor
 
-    into ``outputs`` or, without them, into the gradients themselves; with ``in_place`` false and no outputs only the norm
+    into ``outputs`` (each in the order of its gradient, where that is not the order of its elements) or, without them, into the gradients themselves; with ``in_place`` false and no outputs only the norm
     is formed.  ``norm_and_factor`` holds two values on the device, so that nothing waits for the host.  The reference's
     gradients are sums over a batch that an optimizer multiplies by its gradient-alpha: a limit for their mean is the
     batch's size times as much.  No counterpart in the reference."""
-    result = _dense_buffer(norm_and_factor)
+    result, _ = _dense_buffer(norm_and_factor)
     if result.ecount() != 2:
         raise ValueError("clip_gradients: the norm and the factor are two values")
     if not float(max_norm) > 0:
         raise ValueError(f"clip_gradients: max_norm must be positive, got {max_norm}")
-    at, counts, datatype = _addresses(gradients, backend.datatype)
+    at, counts, datatype, orders = _addresses(gradients, backend.datatype)
     into = at if in_place else None
     if outputs is not None:
-        into, of_outputs, other = _addresses(outputs, backend.datatype)
+        into, of_outputs, other, into_orders = _addresses(outputs, backend.datatype)
         if of_outputs != counts:
             raise ValueError("clip_gradients: outputs and gradients differ in their lengths")
+        if into_orders != orders:
+            raise ValueError("clip_gradients: the elements of an output lie in another order than its gradient's")
         if other != datatype:
             raise TypeError(f"Buffer datatype mismatch: expected {backend.datatype}, got {[datatype, other]}")
     _ensure_datatype(backend.datatype, result)
@@ -176,14 +183,17 @@ def clip_gradients(backend: Backend, gradients, max_norm, norm_and_factor, outpu
 
 
 def _addresses(tensors, datatype):
-    """(device addresses, lengths, datatype) of buffers or dense tensors: bytes of eight to each of the first two."""
+    """(device addresses, lengths, datatype, orders) of buffers or dense tensors: bytes of eight to each of the first two; the
+    orders are None where all lie as they are counted, which is what native code takes."""
     if capi.front is not None:
         found = capi.front.addresses(tensors)    # 0.2 us to a tensor, 1 us here
         if found is not None:
-            return found
-    buffers = [_dense_buffer(x) for x in tensors]
+            return (*found, None)
+    found = [_dense_buffer(x) for x in tensors]
+    buffers, orders = [b for b, _ in found], [order for _, order in found]
     _ensure_datatype(datatype, *buffers)
-    return (array.array("Q", [b.ptr for b in buffers]).tobytes(), array.array("q", [b.ecount() for b in buffers]).tobytes(), datatype)
+    return (array.array("Q", [b.ptr for b in buffers]).tobytes(), array.array("q", [b.ecount() for b in buffers]).tobytes(), datatype,
+            orders if any(order is not None for order in orders) else None)
 
 
 def create_optimizer(backend: Backend, optimizer: dict):
