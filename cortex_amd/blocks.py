@@ -503,22 +503,27 @@ class ExpertBlock:
 
     def backward(self, parameters: dict, x: Tensor, output: Tensor, x_gradient: Tensor, residual_gradient: Tensor,
                  output_gradient: Tensor, normalized_gradient: Tensor):
-        """The gradients of x and of the residual and of every parameter that has one, from those of the results."""
+        """The gradients of x and of the residual and of every parameter that has one, from those of the results.  A parameter whose
+        "gradient" is None or absent is held as it is: nothing is formed for it alone."""
         p = {k: v["buffer"] for k, v in parameters.items()}
+        router, first, second = (parameters[k].get("gradient") for k in ("router", "first", "second"))
         norm_residual_gradient(self.combined_gradient, residual_gradient, self._norms(parameters, "gradient"), output_gradient,
                                normalized_gradient, self.combined, output, self.statistics, self._norms(parameters, "buffer"),
                                self.descriptor)
         combine_experts_gradient(self.outer_gradient, self.weights_gradient, self.combined_gradient, self.outer, self.weights,
                                  self.slots)
-        grouped_gemm_weights(parameters["second"]["gradient"], 1.0, self.outer_gradient, self.inner, 0.0, self.offsets)
+        if second is not None:
+            grouped_gemm_weights(second, 1.0, self.outer_gradient, self.inner, 0.0, self.offsets)
         grouped_gemm(self.inner_gradient, False, 1.0, self.outer_gradient, p["second"], 0.0, self.offsets)
         ct.activation_gradient(self.inner_gradient, self.inner_gradient, self.inner, "relu")
-        grouped_gemm_weights(parameters["first"]["gradient"], 1.0, self.inner_gradient, x, 0.0, self.offsets, b_index=self.tokens)
+        if first is not None:
+            grouped_gemm_weights(first, 1.0, self.inner_gradient, x, 0.0, self.offsets, b_index=self.tokens)
         # the gradient of x: of its rows among the experts, and of the router's
         grouped_gemm(self.outer_gradient, False, 1.0, self.inner_gradient, p["first"], 0.0, self.offsets)
         combine_experts(x_gradient, self.outer_gradient, None, self.slots)
         route_experts_gradient(self.logits_gradient, self.weights_gradient, self.weights, self.experts, self.logits,
                                renormalize=self.renormalize)
-        ct.gemm(parameters["router"]["gradient"], True, False, 1.0, self.logits_gradient, x, 0.0)
+        if router is not None:
+            ct.gemm(router, True, False, 1.0, self.logits_gradient, x, 0.0)
         ct.gemm(x_gradient, False, False, 1.0, self.logits_gradient, p["router"], 1.0)
         return x_gradient, residual_gradient

@@ -52,3 +52,33 @@ def test_norm_gradient_of_rows_without_elements(D, gate):
     want = np.full(20, 7.25)
     want[2:2 + n] = 0
     assert np.array_equal(read(flat), want)
+
+
+# ------------------------------------------------------------------------------------------------- the layer
+
+@pytest.mark.parametrize("held", [("router",), ("first",), ("second",), ("gate", "post-scale"), ("router", "first", "second", "pre-scale")], ids="-".join)
+def test_a_block_with_parameters_that_are_held(D, held):
+    """Parameters without a gradient, by None or by its absence: all other gradients are the same bits as with it."""
+    rng = np.random.default_rng(61)
+    tokens, width, hidden, experts, chosen = 20, 24, 36, 5, 2
+    shapes = {"router": (experts, width), "first": (experts, hidden, width), "second": (experts, width, hidden), "post-scale": (width,),
+              "pre-scale": (width,), "gate": (1, width)}
+    values = {k: D.tensor(rng.standard_normal(s)) for k, s in shapes.items()}
+    make = lambda: D.tensor(rng.standard_normal((tokens, width)))
+    x, residual, to_output, to_normalized = (make() for _ in range(4))
+    results = []
+    for how in ("all", "none", "absent"):
+        p = {k: {"buffer": v, "gradient": D.tensor(np.full(shapes[k], 3.0))} for k, v in values.items()}
+        for k in held if how != "all" else ():
+            if how == "none":
+                p[k]["gradient"] = None
+            else:
+                del p[k]["gradient"]
+        block = blocks.ExpertBlock(tokens, width, hidden, experts, chosen, datatype=D.datatype)
+        output, normalized, dx, dr = (D.tensor(np.zeros((tokens, width))) for _ in range(4))
+        block.forward(p, x, residual, output, normalized)
+        block.backward(p, x, output, dx, dr, to_output, to_normalized)
+        results.append([read(dx), read(dr)] + [read(p[k]["gradient"]) for k in shapes if k not in held])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert np.array_equal(a, b) and np.any(a != 0)
