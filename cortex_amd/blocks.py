@@ -156,8 +156,8 @@ def norm_residual(output: Tensor, normalized: Tensor, statistics: Tensor, input:
 
     ``parameters`` may hold "post-scale", "post-bias", "pre-scale", "pre-bias" ([width]) and "gate" ([rows, width], or 1 in
     either place); ``residual`` may be None, ``normalized`` too without a norm before the next block.  ``statistics``
-    ([4, rows], or None) is what :func:`norm_residual_gradient` needs.  ``output`` may be the residual or the input itself,
-    ``normalized`` the input."""
+    ([4, rows], or None) is what :func:`norm_residual_gradient` needs.  ``output`` and ``normalized`` may each be the residual or
+    the input itself."""
     name = "norm-residual"
     p = parameters.get
     has_pre = descriptor["pre"] != "none"

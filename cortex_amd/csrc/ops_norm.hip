@@ -847,13 +847,18 @@ int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, voi
   CT_TRY(read_gate("gate", gate, gate_dims, rows, width, &a.gate, &a.gate_kind));
   const int64_t size = dtype_size(dtype);
   const RowRange of_gate = gate_range(a.gate, a.gate_kind, rows, width);
+  const Run of_statistics{statistics, 4 * rows * size};
   for (const Matrix* to : {&a.output, &a.normalized}) {
     const RowRange range = range_of(*to, rows, width);
     bool bad = meets_other(*to, a.input, rows, width, size) || meets_other(*to, a.residual, rows, width, size) || rows_meet(range, of_gate, size);
-    for (const void* p : {post_scale, post_bias, pre_scale, pre_bias}) bad = bad || rows_meet(range, {p, 1, width, width}, size);
-    bad = bad || rows_meet(range, {statistics, 1, 4 * rows, 4 * rows}, size);
+    for (const void* p : {post_scale, post_bias, pre_scale, pre_bias}) bad = bad || run_meets({p, width * size}, range, size);
+    bad = bad || run_meets(of_statistics, range, size);
     CT_REQUIRE(!bad, "ct_norm_residual: a result overlaps an operand");
   }
+  bool of_operands = run_meets(of_statistics, range_of(a.input, rows, width), size) || run_meets(of_statistics, range_of(a.residual, rows, width), size) ||
+                     run_meets(of_statistics, of_gate, size);
+  for (const void* p : {post_scale, post_bias, pre_scale, pre_bias}) of_operands = of_operands || runs_meet(of_statistics, {p, width * size});
+  CT_REQUIRE(!of_operands, "ct_norm_residual: the statistics overlap an operand");
   CT_REQUIRE(!rows_meet(range_of(a.output, rows, width), range_of(a.normalized, rows, width), size), "ct_norm_residual: the results overlap");
   a.post_scale = post_scale; a.post_bias = post_bias; a.pre_scale = pre_scale; a.pre_bias = pre_bias;
   a.statistics = statistics;
@@ -902,20 +907,29 @@ int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims*
   a.gate_gradient = Matrix{gate_gradient, a.gate_kind == kFullGate ? width : 1};
   const int64_t size = dtype_size(dtype);
   const RowRange of_gate = gate_range(a.gate, a.gate_kind, rows, width), of_gate_gradient = gate_range(a.gate_gradient, a.gate_kind, rows, width);
-  const Matrix* results[2] = {&a.input_gradient, &a.residual_gradient};
-  for (const Matrix* to : results) {
+  // of what is read, and of the gradients that are no matrices
+  const RowRange matrices[] = {range_of(a.input, rows, width), range_of(a.output, rows, width), range_of(a.output_gradient, rows, width),
+                               range_of(a.normalized_gradient, rows, width), of_gate};
+  const Run vectors[] = {{post_kind != CT_NORM_NONE ? post_scale : nullptr, width * size}, {post_kind != CT_NORM_NONE ? post_bias : nullptr, width * size},
+                         {before ? pre_scale : nullptr, width * size}, {statistics, 4 * rows * size}};
+  const Run gradients[] = {{post_scale_gradient, width * size}, {post_bias_gradient, width * size}, {pre_scale_gradient, width * size},
+                           {pre_bias_gradient, width * size}, {gate_gradient, of_gate_gradient.rows * of_gate_gradient.width * size}};
+  for (const Matrix* to : {&a.input_gradient, &a.residual_gradient}) {
     const RowRange range = range_of(*to, rows, width);
     bool bad = meets_other(*to, a.output_gradient, rows, width, size) || meets_other(*to, a.normalized_gradient, rows, width, size) ||
-               rows_meet(range, range_of(a.input, rows, width), size) || rows_meet(range, range_of(a.output, rows, width), size) ||
-               rows_meet(range, of_gate, size) || rows_meet(range, of_gate_gradient, size) || rows_meet(range, {statistics, 1, 4 * rows, 4 * rows}, size);
-    for (const void* p : {post_scale, post_bias, pre_scale, (const void*)post_scale_gradient, (const void*)post_bias_gradient,
-                          (const void*)pre_scale_gradient, (const void*)pre_bias_gradient})
-      bad = bad || rows_meet(range, {p, 1, width, width}, size);
+               rows_meet(range, matrices[0], size) || rows_meet(range, matrices[1], size) || rows_meet(range, of_gate, size);
+    for (const Run& run : vectors) bad = bad || run_meets(run, range, size);
+    for (const Run& run : gradients) bad = bad || run_meets(run, range, size);
     CT_REQUIRE(!bad, "ct_norm_residual_gradient: a result overlaps an operand");
   }
-  for (const Matrix* m : {&a.input, &a.output, &a.output_gradient, &a.normalized_gradient})
-    CT_REQUIRE(!rows_meet(of_gate_gradient, range_of(*m, rows, width), size), "ct_norm_residual_gradient: the gate's gradient overlaps an operand");
-  CT_REQUIRE(!rows_meet(of_gate_gradient, of_gate, size), "ct_norm_residual_gradient: the gate's gradient overlaps the gate");
+  for (int i = 0; i < 5; ++i) {
+    bool bad = false, results = false;
+    for (const RowRange& m : matrices) bad = bad || run_meets(gradients[i], m, size);
+    for (const Run& run : vectors) bad = bad || runs_meet(gradients[i], run);
+    for (int j = 0; j < i; ++j) results = results || runs_meet(gradients[i], gradients[j]);
+    CT_REQUIRE(!bad, "ct_norm_residual_gradient: %s overlaps an operand", i == 4 ? "the gate's gradient" : "the gradient of a scale or bias");
+    CT_REQUIRE(!results, "ct_norm_residual_gradient: the results overlap");
+  }
   CT_REQUIRE(!rows_meet(range_of(a.input_gradient, rows, width), range_of(a.residual_gradient, rows, width), size),
              "ct_norm_residual_gradient: the results overlap");
   const bool of_columns = gate_gradient && (a.gate_kind == kColumnGate || a.gate_kind == kScalarGate);

@@ -11,10 +11,30 @@ struct RowRange {
   int64_t rows, width, ld;
 };
 
-// Whether two of them have an element in common.  Column blocks of one wider matrix do not; where the leading dimensions
-// differ, ranges of bytes decide.
+// Bytes one behind the other.
+struct Run {
+  const void* p;
+  int64_t bytes;
+};
+
+inline bool runs_meet(const Run& a, const Run& b) {
+  const int64_t x = (int64_t)(uintptr_t)a.p, y = (int64_t)(uintptr_t)b.p;
+  return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
+
+// Whether a run has a byte of one of the rows; what lies between rows is none.
+inline bool run_meets(const Run& run, const RowRange& m, int64_t size) {
+  if (m.rows < 1 || m.width < 1 || !runs_meet(run, {m.p, ((m.rows - 1) * m.ld + m.width) * size})) return false;
+  const int64_t off = (int64_t)(uintptr_t)run.p - (int64_t)(uintptr_t)m.p;
+  return off < 0 || off % (m.ld * size) < m.width * size || off % (m.ld * size) + run.bytes > m.ld * size;
+}
+
+// Whether two of them have an element in common.  Column blocks of one wider matrix do not, nor does a single row, or one of rows
+// without gaps, that lies between the other's; else, where the leading dimensions differ, ranges of bytes decide.
 inline bool rows_meet(const RowRange& a, const RowRange& b, int64_t size) {
   if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+  if (a.rows == 1 || a.ld == a.width) return run_meets({a.p, a.rows * a.width * size}, b, size);
+  if (b.rows == 1 || b.ld == b.width) return run_meets({b.p, b.rows * b.width * size}, a, size);
   const int64_t x = (int64_t)(uintptr_t)a.p, y = (int64_t)(uintptr_t)b.p;
   if (y >= x + ((a.rows - 1) * a.ld + a.width) * size || x >= y + ((b.rows - 1) * b.ld + b.width) * size) return false;
   if (a.ld != b.ld || (y - x) % size) return true;

@@ -569,7 +569,7 @@ typedef enum ct_norm_kind_t { CT_NORM_NONE = 0, CT_NORM_RMS = 1, CT_NORM_LAYER =
  * output, normalized, input and residual are [rows, width] with the column strides of the dimensions given; the
  * innermost stride is 1.  gate is [rows, width], [1, width], [rows, 1] or [1, 1]; absent (NULL) it is 1.  A scale that
  * is absent is 1, a bias 0, and so may residual be (then residual_scale is not read).  output may be residual or input
- * itself and normalized may be input: each row is read before it is stored; other overlaps are refused.
+ * itself and normalized may be either: each row is read before it is stored; other overlaps are refused.
  * statistics [4, rows], or NULL: the mean and 1 / sqrt(...) of the post norm, then those of the pre norm, as the
  * gradient needs them (0 and 1 where there is no norm).  Statistics are summed in the tensor's type, in double beyond
  * the rows that fit registers (16384 values, half as many in double). */
@@ -584,9 +584,8 @@ int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, voi
  * the forward call.  Any result may be NULL: input_gradient, residual_gradient [rows, width], gate_gradient (the gate's
  * shape; sums over what the gate was broadcast along), the gradients of the scales and biases [width].  All are
  * overwritten.  input_gradient and residual_gradient may be output_gradient or normalized_gradient itself, but not one
- * another, and no gradient may overlap an operand otherwise.  Column sums run over the rows in double once they leave a
- * block's registers; the partial sums live in the stream's scratch memory (at most
- * 64 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
+ * another; other overlaps of a gradient with an operand or another gradient are refused.  Column sums run over the rows in
+ * double once they leave a block's registers; the partial sums live in the stream's scratch memory (at most 64 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
 int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims,
                               void* residual_gradient, const ct_dims* residual_gradient_dims,
                               void* gate_gradient, void* post_scale_gradient, void* post_bias_gradient,

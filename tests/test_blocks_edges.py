@@ -7,7 +7,7 @@ import pytest
 from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
-from test_blocks_refusals import Recorder, t
+from test_blocks_refusals import A, Recorder, d, norm, norm_gradient, refuses, t
 
 
 # ---------------------------------------------------------------- clipping: the order of elements
@@ -73,3 +73,38 @@ def test_clipping_takes_tensors_that_fill_their_memory(native, monkeypatch):
     for shape, strides in (([4, 4], [4, 0]), ([4, 4], [8, 1]), ([2, 3], [3, 2])):
         with pytest.raises(ValueError, match="must be dense"):
             clipped([at(4096, *shape, strides=strides, count=100)])
+
+
+# ---------------------------------------------------------------- overlaps
+#
+# Every operand is at an address of its own, 1 MiB from the next one (test_blocks_refusals).  What is moved here meets another
+# one's elements in one place at least: the call would read what it has stored, or store twice to one place.
+
+LAST = 4 * (4 * 8 - 1)      # bytes from the first element of 4 rows of 8 floats to their last
+
+
+@pytest.mark.parametrize("change", [
+    {"statistics": A[3]}, {"statistics": A[3] + LAST}, {"statistics": A[4] - 4 * 15}, {"statistics": A[5] + 28}, {"statistics": A[6] + 28},
+    {"statistics": A[7] - 60}, {"post_bias": A[2] + 60}, {"pre_bias": A[2] - 28}], ids=str)
+def test_norm_statistics_that_overlap(change):
+    refuses("the statistics overlap an operand", "ct_norm_residual", *norm(**change))
+
+
+@pytest.mark.parametrize("message,change", [
+    ("scale or bias overlaps", {"post_scale_gradient": A[11]}), ("scale or bias overlaps", {"post_scale_gradient": A[7] + LAST}),
+    ("scale or bias overlaps", {"post_bias_gradient": A[5]}), ("scale or bias overlaps", {"post_bias_gradient": A[6] - 28}),
+    ("scale or bias overlaps", {"pre_scale_gradient": A[12]}), ("scale or bias overlaps", {"pre_bias_gradient": A[8] + 4}),
+    ("scale or bias overlaps", {"pre_scale_gradient": A[9] + 60}), ("scale or bias overlaps", {"pre_bias_gradient": A[10]}),
+    ("gate's gradient overlaps", {"gate_gradient": A[9] + 60}), ("gate's gradient overlaps", {"gate_gradient": A[11] - 28}),
+    ("results overlap", {"post_bias_gradient": A[3] + 28}), ("results overlap", {"pre_bias_gradient": A[4] - 28}),
+    ("results overlap", {"gate_gradient": A[3]}), ("results overlap", {"pre_scale_gradient": A[3]}),
+    ("overlaps an operand", {"pre_scale_gradient": A[0] + LAST}), ("overlaps an operand", {"gate_gradient": A[1] - 28})], ids=str)
+def test_norm_gradients_that_overlap(message, change):
+    refuses(message, "ct_norm_residual_gradient", *norm_gradient(**change))
+
+
+@pytest.mark.parametrize("change", [{"post_scale_gradient": A[7] + 4 * 57}, {"pre_scale_gradient": A[8] + 4 * 7},
+                                    {"gate_gradient": A[7] + 4 * (3 * 64 - 7)}], ids=str)
+def test_vectors_that_reach_from_a_gap_into_a_row(change):
+    apart = d(4, 8, strides=[64, 1])
+    refuses("overlaps an operand", "ct_norm_residual_gradient", *norm_gradient(input_dims=apart, output_dims=apart, **change))

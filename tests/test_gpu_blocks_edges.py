@@ -54,6 +54,26 @@ def test_norm_gradient_of_rows_without_elements(D, gate):
     assert np.array_equal(read(flat), want)
 
 
+def test_norm_gradients_between_the_rows_of_an_operand(D):
+    """Vectors in the columns that a wider matrix has beside the operand overlap nothing of it, and are taken."""
+    rng = np.random.default_rng(62)
+    rows, width, wide = 5, 24, 100
+    whole = D.tensor(rng.standard_normal(rows * wide))
+    z = ct.Tensor(whole.device, {"shape": [rows, width], "strides": [wide, 1]}, whole.buffer)
+    p = {k: D.tensor(rng.standard_normal(width)) for k in ("post-scale", "post-bias", "pre-scale")}
+    d = blocks.norm_descriptor(post="layer", pre="rms")
+    out, h, stats, dout, dh = (D.tensor(rng.standard_normal(s)) for s in ([(rows, width)] * 2 + [(4, rows)] + [(rows, width)] * 2))
+    blocks.norm_residual(out, h, stats, z, None, p, d)
+    results = []
+    for between in (False, True):
+        g = {k: part(D, whole, wide * i + width + 3 * i, (width,)) if between else D.tensor(np.zeros(width)) for i, k in enumerate(p)}
+        dz = D.tensor(np.zeros((rows, width)))
+        blocks.norm_residual_gradient(dz, None, g, dout, dh, z, out, stats, p, d)
+        results.append([read(dz)] + [read(t) for t in g.values()])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b) and np.any(a != 0)
+
+
 # ------------------------------------------------------------------------------------------------- the layer
 
 @pytest.mark.parametrize("held", [("router",), ("first",), ("second",), ("gate", "post-scale"), ("router", "first", "second", "pre-scale")], ids="-".join)
