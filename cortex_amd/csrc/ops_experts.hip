@@ -643,13 +643,19 @@ int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* off
   CT_REQUIRE(n <= kMostRows / n_chosen, "ct_route_experts: %lld tokens", (long long)n);
   CT_REQUIRE(offsets && (n == 0 || (experts && weights && tokens && slots && logits)), "ct_route_experts: null buffer");
   CT_REQUIRE(logits_colstride >= n_experts, "ct_route_experts: column stride %lld below the row's length", (long long)logits_colstride);
+  const int64_t size = dtype_size(dtype), choices = n * n_chosen;
+  const Run results[] = {{experts, choices * 4}, {weights, choices * size}, {offsets, (n_experts + 1) * 4}, {tokens, choices * 4}, {slots, choices * 4}};
+  for (int i = 0; i < 5; ++i) {
+    CT_REQUIRE(!run_meets(results[i], {logits, n, n_experts, logits_colstride}, size), "ct_route_experts: a result overlaps the logits");
+    for (int j = 0; j < i; ++j) CT_REQUIRE(!runs_meet(results[i], results[j]), "ct_route_experts: the results overlap");
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   RouteArgs a{};
   a.experts = experts; a.weights = weights; a.offsets = offsets; a.tokens = tokens; a.slots = slots; a.logits = logits;
   a.colstride = logits_colstride;
   a.n = (uint32_t)n; a.n_experts = (uint32_t)n_experts; a.n_chosen = (uint32_t)n_chosen;
   a.renormalize = renormalize != 0;
-  if (!is_few(n, n_experts, n_chosen, dtype_size(dtype))) {
+  if (!is_few(n, n_experts, n_chosen, size)) {
     // 16 tokens to a block, 64 where there are blocks enough, more where the blocks' counts would take more than 8 MiB
     const int64_t most_blocks = std::max<int64_t>(1, (int64_t(2) << 20) / (n_experts + 1));
     a.tokens_per_block = (uint32_t)std::max<int64_t>(n <= 8192 ? 16 : 64, (n + most_blocks - 1) / most_blocks);
@@ -676,6 +682,13 @@ int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logit
              "ct_route_experts_gradient: null buffer");
   CT_REQUIRE(logits_gradient_colstride >= n_experts && (renormalize || logits_colstride >= n_experts),
              "ct_route_experts_gradient: a column stride below the row's length");
+  const int64_t size = dtype_size(dtype), choices = n * n_chosen;
+  const RowRange result{logits_gradient, n, n_experts, logits_gradient_colstride};
+  const bool in_place = logits_gradient == logits && (logits_gradient_colstride == logits_colstride || n == 1);   // a token's lanes read its row piece by piece ahead of storing it
+  CT_REQUIRE(!run_meets({weights_gradient, choices * size}, result, size) && !run_meets({weights, choices * size}, result, size) &&
+                 !run_meets({experts, choices * 4}, result, size) &&
+                 (renormalize || in_place || !rows_meet(result, {logits, n, n_experts, logits_colstride}, size)),
+             "ct_route_experts_gradient: logits_gradient overlaps an operand");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const RouteGradientArgs a{logits_gradient, weights_gradient, weights, experts, logits, logits_gradient_colstride,
                             logits_colstride, (uint32_t)n, (uint32_t)n_experts, (uint32_t)n_chosen, renormalize != 0};

@@ -607,7 +607,8 @@ int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims*
  *                          expert, and of (t, j) within one: expert e's are offsets[e] .. offsets[e + 1] - 1; tokens
  *                          holds t at each of these places and -1 beyond offsets[n_experts]; slots holds the place of
  *                          (t, j), -1 for an expert of -1
- * 1 <= n_chosen <= min(32, n_experts), n_experts <= 1024, n * n_chosen < 2^31.  n = 0 writes the offsets only.  More than a
+ * 1 <= n_chosen <= min(32, n_experts), n_experts <= 1024, n * n_chosen < 2^31.  n = 0 writes the offsets only.  The results
+ * overlap neither one another nor the logits.  More than a
  * few tokens need scratch memory of the stream, up to 8 MiB. */
 int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* offsets, int32_t* tokens,
                      int32_t* slots, const void* logits, int64_t logits_colstride, int64_t n,
@@ -615,7 +616,8 @@ int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* off
 
 /* The gradient of the weights with respect to the logits, overwritten: with p the softmax over the chosen experts if
  * renormalize, else over all,  dlogit_e = p_e * (dw_e - sum over the chosen i of w_i dw_i), dw_e = 0 where e was not
- * chosen (so 0 there under renormalize).  weights and experts as ct_route_experts stored them. */
+ * chosen (so 0 there under renormalize).  weights and experts as ct_route_experts stored them.  logits_gradient may be logits
+ * itself, and overlaps no operand otherwise; logits are not read under renormalize. */
 int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logits_gradient_colstride,
                               const void* weights_gradient, const void* weights, const int32_t* experts,
                               const void* logits, int64_t logits_colstride, int64_t n, int64_t n_experts,

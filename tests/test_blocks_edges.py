@@ -7,7 +7,7 @@ import pytest
 from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
-from test_blocks_refusals import A, Recorder, d, norm, norm_gradient, refuses, t
+from test_blocks_refusals import A, Recorder, d, norm, norm_gradient, refuses, route, route_gradient, t
 
 
 # ---------------------------------------------------------------- clipping: the order of elements
@@ -108,3 +108,20 @@ def test_norm_gradients_that_overlap(message, change):
 def test_vectors_that_reach_from_a_gap_into_a_row(change):
     apart = d(4, 8, strides=[64, 1])
     refuses("overlaps an operand", "ct_norm_residual_gradient", *norm_gradient(input_dims=apart, output_dims=apart, **change))
+
+
+@pytest.mark.parametrize("message,change", [
+    ("results overlap", {"weights": A[0] + 4 * 39}), ("results overlap", {"offsets": A[0] - 4 * 16}), ("results overlap", {"tokens": A[2] + 4 * 16}),
+    ("results overlap", {"slots": A[3]}), ("results overlap", {"slots": A[1] + 8 * 39, "dtype": capi.F64}),
+    ("the logits", {"experts": A[5] + 4 * 159}), ("the logits", {"weights": A[5]}), ("the logits", {"offsets": A[5] - 4 * 16}),
+    ("the logits", {"tokens": A[5] + 4 * 32}), ("the logits", {"slots": A[5] + 4 * (9 * 40 + 15), "logits_colstride": 40})], ids=str)
+def test_routing_into_what_overlaps(message, change):
+    refuses(message, "ct_route_experts", *route(**change))
+
+
+@pytest.mark.parametrize("change", [
+    {"weights_gradient": A[0]}, {"weights": A[0] + 4 * 159}, {"experts": A[0] - 4 * 39}, {"logits": A[0] + 4},
+    {"logits": A[0], "logits_colstride": 17}, {"weights": A[0] + 4 * 159, "renormalize": 1},
+    {"weights": A[0] + 4 * 17, "logits_gradient_colstride": 60, "n_chosen": 5}], ids=str)
+def test_routing_gradients_that_overlap(change):
+    refuses("overlaps an operand", "ct_route_experts_gradient", *route_gradient(**change))

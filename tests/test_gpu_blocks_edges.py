@@ -5,7 +5,7 @@ import pytest
 
 from cortex_amd import blocks
 from cortex_amd import tensor as ct
-from test_gpu_blocks import D, Owned, read, stream, strides_of  # noqa: F401  (fixtures among them)
+from test_gpu_blocks import D, Owned, read, run_route, stream, strides_of  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -72,6 +72,24 @@ def test_norm_gradients_between_the_rows_of_an_operand(D):
         results.append([read(dz)] + [read(t) for t in g.values()])
     for a, b in zip(*results):
         assert np.array_equal(a, b) and np.any(a != 0)
+
+
+# ------------------------------------------------------------------------------------------------- routing
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("size", [(1, 3, 2), (50, 7, 3), (40, 30, 2), (33, 61, 8), (21, 130, 4), (9, 1021, 5), (3000, 257, 2)], ids=str)
+def test_route_gradient_in_place_of_the_logits(D, size, renormalize):
+    """The same bits as into memory of its own, rows apart and with widths that end inside a piece."""
+    n, e, k = size
+    rng = np.random.default_rng(63)
+    logits = rng.standard_normal((n, e))
+    logits[rng.random((n, e)) < 0.2] = -np.inf
+    apart, to = D.block(logits, 3), D.block(np.zeros((n, e)), 3)
+    t, (experts, weights, *_) = run_route(D, logits, k, renormalize)
+    dw = D.tensor(rng.standard_normal((n, k)))
+    blocks.route_experts_gradient(to, dw, weights, experts, apart, renormalize=renormalize)
+    blocks.route_experts_gradient(apart, dw, weights, experts, apart, renormalize=renormalize)
+    assert np.array_equal(read(apart), read(to)) and np.any(read(to) != 0)
 
 
 # ------------------------------------------------------------------------------------------------- the layer
