@@ -708,8 +708,11 @@ int ct_combine_experts(void* stream, void* output, int64_t output_colstride, con
   if (n == 0 || width == 0) return CT_OK;
   CT_REQUIRE(output && slots && (rows || row_count == 0), "ct_combine_experts: null buffer");
   CT_REQUIRE(output_colstride >= width && rows_colstride >= width, "ct_combine_experts: a column stride below the row's length");
-  CT_REQUIRE(!rows_meet({output, n, width, output_colstride}, {rows, row_count, width, rows_colstride}, dtype_size(dtype)),
-             "ct_combine_experts: output and rows overlap");
+  const int64_t size = dtype_size(dtype);
+  const RowRange result{output, n, width, output_colstride};
+  CT_REQUIRE(!rows_meet(result, {rows, row_count, width, rows_colstride}, size), "ct_combine_experts: output and rows overlap");
+  CT_REQUIRE(!run_meets({weights, n * n_chosen * size}, result, size) && !run_meets({slots, n * n_chosen * 4}, result, size),
+             "ct_combine_experts: output overlaps the weights or the slots");
   hipStream_t s = static_cast<hipStream_t>(stream);
   CombineArgs a{};
   a.output = output; a.rows = rows; a.weights = weights; a.slots = slots;
@@ -738,9 +741,17 @@ int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_
                  (!weights_gradient || rows_colstride >= width),
              "ct_combine_experts_gradient: a column stride below the row's length");
   const RowRange result{rows_gradient, row_count, width, rows_gradient_colstride};
-  CT_REQUIRE(!rows_meet(result, {output_gradient, n, width, output_gradient_colstride}, dtype_size(dtype)) &&
-                 !rows_meet(result, {weights_gradient ? rows : nullptr, row_count, width, rows_colstride}, dtype_size(dtype)),
+  const int64_t size = dtype_size(dtype);
+  const RowRange of_output{output_gradient, n, width, output_gradient_colstride}, of_rows{weights_gradient ? rows : nullptr, row_count, width, rows_colstride};
+  const Run of_weights{weights, n * n_chosen * size}, of_slots{slots, n * n_chosen * 4}, to_weights{weights_gradient, n * n_chosen * size};
+  CT_REQUIRE(!rows_meet(result, of_output, size) && !rows_meet(result, of_rows, size) && !run_meets(of_weights, result, size) &&
+                 !run_meets(of_slots, result, size),
              "ct_combine_experts_gradient: rows_gradient overlaps an operand");
+  // a weight is read by the lanes that store its gradient, ahead of that
+  CT_REQUIRE(!run_meets(to_weights, of_output, size) && !run_meets(to_weights, of_rows, size) && !runs_meet(to_weights, of_slots) &&
+                 (weights_gradient == weights || !runs_meet(to_weights, of_weights)),
+             "ct_combine_experts_gradient: weights_gradient overlaps an operand");
+  CT_REQUIRE(!run_meets(to_weights, result, size), "ct_combine_experts_gradient: the results overlap");
   if (width == 0) return weights_gradient ? ct_memset(stream, weights_gradient, dtype, 0.0, n * n_chosen) : (int)CT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   CombineArgs a{};

@@ -647,14 +647,15 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
 
 /* output[t] = sum over j of weights[t, j] * rows[slots[t, j]], slots outside [0, row_count) left out; weights NULL: 1.
  * rows [row_count, width], output [n, width], weights and slots [n, n_chosen] packed, n_chosen <= 32.  Sums run in the order of j,
- * in the tensor's type. */
+ * in the tensor's type.  output overlaps no operand. */
 int ct_combine_experts(void* stream, void* output, int64_t output_colstride, const void* rows,
                        int64_t row_count, int64_t rows_colstride, const void* weights,
                        const int32_t* slots, int64_t n, int64_t n_chosen, int64_t width, int dtype);
 
 /* Its gradient: rows_gradient[slots[t, j]] = weights[t, j] * output_gradient[t], rows that no slot names are not touched;
  * weights_gradient[t, j] = output_gradient[t] . rows[slots[t, j]], 0 for a slot outside the range.  Either may be NULL
- * (then so may rows, for weights_gradient's).  A row is named by one slot at most. */
+ * (then so may rows, for weights_gradient's).  A row is named by one slot at most.  weights_gradient may be weights itself; the
+ * results overlap neither one another nor an operand otherwise. */
 int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_gradient_colstride,
                                 void* weights_gradient, const void* output_gradient,
                                 int64_t output_gradient_colstride, const void* rows, int64_t row_count,

@@ -7,7 +7,7 @@ import pytest
 from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
-from test_blocks_refusals import A, Recorder, d, norm, norm_gradient, refuses, route, route_gradient, t
+from test_blocks_refusals import A, Recorder, combine, combine_gradient, d, norm, norm_gradient, refuses, route, route_gradient, t
 
 
 # ---------------------------------------------------------------- clipping: the order of elements
@@ -125,3 +125,21 @@ def test_routing_into_what_overlaps(message, change):
     {"weights": A[0] + 4 * 17, "logits_gradient_colstride": 60, "n_chosen": 5}], ids=str)
 def test_routing_gradients_that_overlap(change):
     refuses("overlaps an operand", "ct_route_experts_gradient", *route_gradient(**change))
+
+
+@pytest.mark.parametrize("message,change", [
+    ("weights or the slots", {"weights": A[0] + 4 * 79}), ("weights or the slots", {"weights": A[0] - 4 * 19}), ("weights or the slots", {"slots": A[0]}),
+    ("weights or the slots", {"slots": A[0] + 4 * (9 * 30 + 7), "output_colstride": 30}),
+    ("weights or the slots", {"weights": A[0] - 8 * 19, "dtype": capi.F64})], ids=str)
+def test_combining_into_what_overlaps(message, change):
+    refuses(message, "ct_combine_experts", *combine(**change))
+
+
+@pytest.mark.parametrize("message,change", [
+    ("rows_gradient overlaps", {"weights": A[0] + 4 * 159}), ("rows_gradient overlaps", {"slots": A[0] - 4 * 19}),
+    ("weights_gradient overlaps", {"weights_gradient": A[2]}), ("weights_gradient overlaps", {"weights_gradient": A[3] + 4 * 159}),
+    ("weights_gradient overlaps", {"weights_gradient": A[5] + 4 * 19}), ("weights_gradient overlaps", {"weights_gradient": A[4] + 4}),
+    ("weights_gradient overlaps", {"weights_gradient": A[4] - 4 * 19}), ("results overlap", {"weights_gradient": A[0] + 4 * 159}),
+    ("weights_gradient overlaps", {"weights_gradient": A[5], "rows_gradient": None})], ids=str)
+def test_combining_gradients_that_overlap(message, change):
+    refuses(message, "ct_combine_experts_gradient", *combine_gradient(**change))

@@ -92,6 +92,22 @@ def test_route_gradient_in_place_of_the_logits(D, size, renormalize):
     assert np.array_equal(read(apart), read(to)) and np.any(read(to) != 0)
 
 
+# ------------------------------------------------------------------------------------------------- combining
+
+@pytest.mark.parametrize("size", [(1, 1, 1), (40, 3, 33), (700, 2, 1000), (3, 4, 4100), (300, 4, 2050)], ids=str)
+def test_combine_gradient_in_place_of_the_weights(D, size):
+    """The same bits as into memory of its own, with 16, 64 and 256 lanes to an assignment."""
+    n, k, width = size
+    rng = np.random.default_rng(64)
+    rows, dy = D.tensor(rng.standard_normal((n * k, width))), D.tensor(rng.standard_normal((n, width)))
+    slots, weights = D.tensor(rng.permutation(n * k).reshape(n, k), "int"), D.tensor(rng.standard_normal((n, k)))
+    to = [D.tensor(np.zeros((n * k, width))) for _ in range(2)]
+    apart = D.tensor(np.zeros((n, k)))
+    blocks.combine_experts_gradient(to[0], apart, dy, rows, weights, slots)
+    blocks.combine_experts_gradient(to[1], weights, dy, rows, weights, slots)
+    assert np.array_equal(read(weights), read(apart)) and np.array_equal(read(to[0]), read(to[1])) and np.any(read(apart) != 0)
+
+
 # ------------------------------------------------------------------------------------------------- the layer
 
 @pytest.mark.parametrize("held", [("router",), ("first",), ("second",), ("gate", "post-scale"), ("router", "first", "second", "pre-scale")], ids="-".join)
