@@ -831,8 +831,10 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
   const int64_t size = dtype_size(dtype);
   const RowRange result{c, row_count, b_col_count, c_colstride};
   CT_REQUIRE(!rows_meet(result, {a_col_count ? a : nullptr, a_row_count, a_col_count, a_colstride}, size) &&
-                 !rows_meet(result, {a_col_count ? b : nullptr, 1, (n_groups - 1) * b_stride + (b_rows - 1) * b_colstride + b_cols, 1}, size),
+                 !run_meets({a_col_count ? b : nullptr, ((n_groups - 1) * b_stride + (b_rows - 1) * b_colstride + b_cols) * size}, result, size),
              "ct_grouped_gemm: c overlaps an operand");
+  CT_REQUIRE(!run_meets({offsets, (n_groups + 1) * 4}, result, size) && !run_meets({index, row_count * 4}, result, size),
+             "ct_grouped_gemm: c overlaps the offsets or the index");
   hipStream_t s = static_cast<hipStream_t>(stream);
   GroupedArgs g{};
   g.a = a; g.b = b; g.c = c; g.index_a = index; g.offsets = offsets;
@@ -933,9 +935,11 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
              "ct_grouped_gemm_weights: a column stride below the row's length");
   CT_REQUIRE(n_groups == 1 || c_stride >= (a_col_count - 1) * c_colstride + b_col_count, "ct_grouped_gemm_weights: results overlap one another");
   const int64_t size = dtype_size(dtype);
-  const RowRange result{c, 1, (n_groups - 1) * c_stride + (a_col_count - 1) * c_colstride + b_col_count, 1};
-  CT_REQUIRE(!rows_meet(result, {a, a_row_count, a_col_count, a_colstride}, size) && !rows_meet(result, {b, b_row_count, b_col_count, b_colstride}, size),
+  const Run result{c, ((n_groups - 1) * c_stride + (a_col_count - 1) * c_colstride + b_col_count) * size};
+  CT_REQUIRE(!run_meets(result, {a, a_row_count, a_col_count, a_colstride}, size) && !run_meets(result, {b, b_row_count, b_col_count, b_colstride}, size),
              "ct_grouped_gemm_weights: c overlaps an operand");
+  CT_REQUIRE(!runs_meet(result, {offsets, (n_groups + 1) * 4}) && !runs_meet(result, {a_index, row_count * 4}) && !runs_meet(result, {b_index, row_count * 4}),
+             "ct_grouped_gemm_weights: c overlaps the offsets or an index");
   hipStream_t s = static_cast<hipStream_t>(stream);
   GroupedArgs g{};
   g.a = a; g.b = b; g.c = c; g.index_a = a_index; g.index_b = b_index; g.offsets = offsets;

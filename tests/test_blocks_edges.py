@@ -7,7 +7,7 @@ import pytest
 from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
-from test_blocks_refusals import A, Recorder, combine, combine_gradient, d, norm, norm_gradient, refuses, route, route_gradient, t
+from test_blocks_refusals import A, Recorder, combine, combine_gradient, d, grouped, norm, norm_gradient, refuses, route, route_gradient, t, weights
 
 
 # ---------------------------------------------------------------- clipping: the order of elements
@@ -143,3 +143,14 @@ def test_combining_into_what_overlaps(message, change):
     ("weights_gradient overlaps", {"weights_gradient": A[5], "rows_gradient": None})], ids=str)
 def test_combining_gradients_that_overlap(message, change):
     refuses(message, "ct_combine_experts_gradient", *combine_gradient(**change))
+
+
+@pytest.mark.parametrize("change", [{"offsets": A[0] + 4 * 639}, {"offsets": A[0] - 4 * 3}, {"index": A[0] - 4 * 19}, {"index": A[0] + 4 * 320},
+                                    {"index": A[0] + 8 * 90 * 3 - 4 * 19, "c_colstride": 90, "dtype": capi.F64}], ids=str)
+def test_products_into_their_offsets_or_index(change):
+    refuses("offsets or the index", "ct_grouped_gemm", *grouped(**change))
+
+
+@pytest.mark.parametrize("change", [{"offsets": A[0] + 4 * 1535}, {"offsets": A[0] - 4 * 3}, {"a_index": A[0] - 4 * 19}, {"b_index": A[0] + 4 * 512}], ids=str)
+def test_products_over_rows_into_their_offsets_or_indexes(change):
+    refuses("offsets or an index", "ct_grouped_gemm_weights", *weights(**change))
