@@ -11,6 +11,8 @@
 // by every call.
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "elementwise.h"
 #include "rows.h"
@@ -214,6 +216,36 @@ int clip_typed(hipStream_t s, const void* const* in, void* const* out, const int
   return after_launch(s);
 }
 
+// The memory of a tensor that has elements.
+struct Extent {
+  uintptr_t begin, end;
+  int64_t tensor;
+};
+
+// Whether no output meets another one or another tensor's gradient; `by_place` has room for all outputs.
+bool outputs_apart(const void* const* in, void* const* out, const int64_t* counts, int64_t count, int64_t size, Extent* by_place, int64_t* bad) {
+  int64_t n = 0;
+  bool in_order = true, in_place = true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (counts[i] == 0) continue;
+    const uintptr_t at = (uintptr_t)out[i];
+    in_order = in_order && (n == 0 || by_place[n - 1].begin <= at);
+    in_place = in_place && out[i] == in[i];
+    by_place[n++] = {at, at + (uintptr_t)(counts[i] * size), i};
+  }
+  if (!in_order) std::sort(by_place, by_place + n, [](const Extent& a, const Extent& b) { return a.begin < b.begin; });
+  for (int64_t k = 1; k < n; ++k)
+    if (by_place[k].begin < by_place[k - 1].end) return *bad = by_place[k].tensor, false;
+  if (in_place) return true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (counts[i] == 0) continue;
+    const uintptr_t begin = (uintptr_t)in[i], end = begin + (uintptr_t)(counts[i] * size);
+    const Extent* const o = std::upper_bound(by_place, by_place + n, begin, [](uintptr_t at, const Extent& e) { return at < e.end; });
+    if (o != by_place + n && o->begin < end && !(o->tensor == i && out[i] == in[i])) return *bad = o->tensor, false;
+  }
+  return true;
+}
+
 }  // namespace
 
 extern "C" int ct_clip_gradients(void* stream, const void* const* gradients, void* const* outputs, const int64_t* counts,
@@ -223,14 +255,25 @@ extern "C" int ct_clip_gradients(void* stream, const void* const* gradients, voi
   CT_REQUIRE(max_norm > 0, "ct_clip_gradients: max_norm must be positive");
   CT_REQUIRE(norm_and_factor && (count == 0 || (gradients && counts)), "ct_clip_gradients: null argument");
   const int64_t size = dtype_size(dtype), most = int64_t(1) << 40;
+  const Run of_norm{norm_and_factor, 2 * size};
   for (int64_t i = 0; i < count; ++i) {
     CT_REQUIRE(counts[i] >= 0 && counts[i] <= most, "ct_clip_gradients: tensor %lld has %lld values", (long long)i, (long long)counts[i]);
     if (counts[i] == 0) continue;
     CT_REQUIRE(gradients[i] && (!outputs || outputs[i]), "ct_clip_gradients: null buffer");
+    CT_REQUIRE(!runs_meet(of_norm, {gradients[i], counts[i] * size}) && !(outputs && runs_meet(of_norm, {outputs[i], counts[i] * size})),
+               "ct_clip_gradients: the norm and the factor overlap tensor %lld", (long long)i);
     if (outputs && outputs[i] != gradients[i]) {
       const uintptr_t a = (uintptr_t)gradients[i], b = (uintptr_t)outputs[i], bytes = (uintptr_t)(counts[i] * size);
       CT_REQUIRE(a + bytes <= b || b + bytes <= a, "ct_clip_gradients: output %lld overlaps its gradient", (long long)i);
     }
+  }
+  if (outputs) {
+    Extent few[kTensors];
+    const std::unique_ptr<Extent[]> many(count > kTensors ? new (std::nothrow) Extent[count] : nullptr);
+    CT_REQUIRE(count <= kTensors || many, "ct_clip_gradients: no memory for a list of %lld tensors", (long long)count);
+    int64_t bad = 0;
+    CT_REQUIRE(outputs_apart(gradients, outputs, counts, count, size, many ? many.get() : few, &bad),
+               "ct_clip_gradients: output %lld overlaps another tensor", (long long)bad);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == CT_F32) return clip_typed<float>(s, gradients, outputs, counts, count, max_norm, static_cast<float*>(norm_and_factor));

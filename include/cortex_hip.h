@@ -664,9 +664,9 @@ int ct_combine_experts_gradient(void* stream, void* rows_gradient, int64_t rows_
 
 /* The norm over all of `count` gradients and their clipping: with norm = sqrt(sum of all squares), summed in double,
  *   factor = max_norm / max(norm, max_norm),   outputs[i] = gradients[i] * factor.
- * gradients, outputs and counts are HOST arrays (of device addresses and lengths), read before the call returns; an output may be
- * its gradient (and overlaps nothing otherwise), and outputs may be NULL: then only the norm is formed.  norm_and_factor [2], in the tensors' type, in
- * device memory, receives both.  max_norm > 0; infinity never clips.  A NaN among the gradients makes norm, factor and
+ * gradients, outputs and counts are HOST arrays (of device addresses and lengths), read before the call returns.  An output may be
+ * its gradient and overlaps nothing otherwise, no other output or gradient either; outputs may be NULL: then only the norm is
+ * formed.  norm_and_factor [2], in the tensors' type, in device memory apart from all of them, receives both.  max_norm > 0; infinity never clips.  A NaN among the gradients makes norm, factor and
  * every output NaN; an infinity makes the factor 0.  Scratch memory of the stream: 8 bytes to a piece of 4 KiB or more, 16 KiB
  * to 120 gradients at most. */
 int ct_clip_gradients(void* stream, const void* const* gradients, void* const* outputs,

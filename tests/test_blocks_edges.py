@@ -1,5 +1,7 @@
 """Calls of the operators of residual blocks with experts that are refused, or that reach the stream, by how their operands lie
 in memory.  Nothing here needs a GPU."""
+import ctypes as C
+import random
 import struct
 
 import pytest
@@ -154,3 +156,46 @@ def test_products_into_their_offsets_or_index(change):
 @pytest.mark.parametrize("change", [{"offsets": A[0] + 4 * 1535}, {"offsets": A[0] - 4 * 3}, {"a_index": A[0] - 4 * 19}, {"b_index": A[0] + 4 * 512}], ids=str)
 def test_products_over_rows_into_their_offsets_or_indexes(change):
     refuses("offsets or an index", "ct_grouped_gemm_weights", *weights(**change))
+
+
+# ---------------------------------------------------------------- clipping: outputs and other tensors
+
+def clip(gradients, outputs, counts, result=A[20], dtype=capi.F32):
+    n = len(gradients)
+    addresses = lambda x: None if x is None else (C.c_void_p * n)(*x)
+    return None, addresses(gradients), addresses(outputs), (C.c_int64 * n)(*counts), n, 1.0, result, dtype
+
+
+@pytest.mark.parametrize("message,gradients,outputs,counts", [
+    ("overlaps another", [A[0], A[1]], [A[1], A[2]], [8, 8]), ("overlaps another", [A[0], A[1]], [A[2], A[0] + 28], [8, 8]),
+    ("overlaps another", [A[0], A[1]], [A[1] - 28, A[1]], [8, 8]), ("overlaps another", [A[0], A[1]], [A[2], A[2] + 28], [8, 8]),
+    ("overlaps another", [A[0], A[0]], [A[0], A[0]], [8, 8]), ("overlaps another", [A[0], A[1]], [A[1], A[0]], [8, 8]),
+    ("overlaps another", [A[0], A[5], A[1]], [A[0], A[1] - 4 * 7, A[1]], [8, 8, 8]),
+    ("norm and the factor overlap tensor 1", [A[0], A[20] - 28], None, [8, 8]), ("norm and the factor overlap tensor 0", [A[0], A[1]], [A[20] + 4, A[2]], [8, 8])])
+def test_clipping_into_another_tensor(message, gradients, outputs, counts):
+    refuses(message, "ct_clip_gradients", *clip(gradients, outputs, counts))
+
+
+def test_clipping_long_lists_into_another_tensor():
+    """Lists drawn at random, in any order, whose tensors touch but do not meet, but for one output: that one is named, or the tensor
+    that it meets."""
+    for seed in range(200):
+        rng = random.Random(seed)
+        n = rng.choice([2, 3, 50, 119, 120, 121, 300])
+        counts = [rng.randint(0, 9) for _ in range(n)]
+        places, at = {}, 1 << 20
+        for slot in rng.sample(range(2 * n), 2 * n):
+            places[slot] = at
+            at += 4 * counts[slot % n]
+        gradients = [places[i] for i in range(n)]
+        outputs = [g if rng.random() < 0.5 else places[n + i] for i, g in enumerate(gradients)]
+        some = [i for i in range(n) if counts[i]]
+        if len(some) < 2:
+            continue
+        i, j = rng.sample(some, 2)
+        meets = rng.choice([gradients[j], outputs[j]])
+        # from its last byte before the other's end to its first after the other's beginning
+        outputs[i] = meets + 4 * rng.randint(1 - counts[i], counts[j] - 1)
+        with pytest.raises(capi.CortexHipError) as e:
+            capi.call("ct_clip_gradients", *clip(gradients, outputs, counts, result=1 << 30))
+        assert e.value.status == 1 and "overlaps" in e.value.message, (seed, e.value.message)

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from cortex_amd import blocks
+from cortex_amd import optimize
 from cortex_amd import tensor as ct
 from test_gpu_blocks import D, Owned, read, run_route, stream, strides_of  # noqa: F401  (fixtures among them)
 
@@ -106,6 +107,33 @@ def test_combine_gradient_in_place_of_the_weights(D, size):
     blocks.combine_experts_gradient(to[0], apart, dy, rows, weights, slots)
     blocks.combine_experts_gradient(to[1], weights, dy, rows, weights, slots)
     assert np.array_equal(read(weights), read(apart)) and np.array_equal(read(to[0]), read(to[1])) and np.any(read(apart) != 0)
+
+
+# ------------------------------------------------------------------------------------------------- clipping
+
+@pytest.mark.parametrize("n", [2, 50, 120, 121, 300])
+def test_clip_gradients_of_tensors_that_touch_in_any_order(D, stream, n):
+    """Gradients and outputs side by side in one buffer, shuffled, some in place: nothing overlaps, and each goes where it belongs."""
+    rng = np.random.default_rng(n)
+    counts = rng.integers(0, 40, n)
+    counts[0] = 7
+    order = rng.permutation(2 * n)
+    ends = np.cumsum(counts[order % n])
+    places = np.empty(2 * n, np.int64)
+    places[order] = ends - counts[order % n]
+    host = rng.standard_normal(int(ends[-1])).astype(D.type)
+    flat, result = D.tensor(host), D.tensor(np.zeros(2))
+    piece = lambda slot: flat.buffer.sub_buffer(int(places[slot]), int(counts[slot % n]))
+    into = [i if rng.random() < 0.5 else n + i for i in range(n)]
+    optimize.clip_gradients(optimize.Backend(stream, D.datatype), [piece(i) for i in range(n)], 0.5, result, [piece(i) for i in into])
+    norm, factor = read(result)
+    values = [host[places[i]:places[i] + counts[i]] for i in range(n)]
+    want64 = np.sqrt(sum((v.astype(np.float64) ** 2).sum() for v in values))
+    assert abs(float(norm) - want64) <= (4 * D.u + host.size * 2.0 ** -53) * want64
+    want = host.copy()
+    for i, slot in enumerate(into):
+        want[places[slot]:places[slot] + counts[i]] = values[i] * factor
+    assert np.array_equal(read(flat), want)
 
 
 # ------------------------------------------------------------------------------------------------- the layer
