@@ -1,7 +1,7 @@
 // ops_grouped.hip -- products of rows with the matrix of their group (ct_grouped_gemm), and the products over the rows of
 // each group that are those matrices' gradients (ct_grouped_gemm_weights).
 //
-// Groups are runs of rows between offsets in device memory.  A launch has as many blocks as the tiles can be at most: the
+// Groups are runs of rows between offsets in device memory.  A call launches as many blocks as the tiles can be at most: the
 // tiles of all rows and one more to each group.  A block finds its group by adding up the groups' tiles; blocks beyond the
 // last tile end.  Offsets are clamped as they are read, so that no content of theirs leads outside a buffer.
 #include <algorithm>
@@ -101,45 +101,51 @@ __device__ __forceinline__ void put(T* cell, T sum, double alpha, double beta) {
   *cell = beta == 0 ? value : value + (T)beta * *cell;
 }
 
+// Of operands without rows, and of sums without terms.  A block takes every so manieth tile of rows and of columns, here and below.
 template <class T>
 __global__ void __launch_bounds__(256) grouped_kernel(const GroupedArgs a) {
   Group g;
-  if (!find_group(a, blockIdx.y, kSide, &g)) return;
-  const uint32_t row0 = g.tile * kSide, col0 = blockIdx.x * kSide;
-  const T* b = static_cast<const T*>(a.b) + (int64_t)g.index * a.b_stride;
-  T* c = static_cast<T*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
-  tile_product<T>(
-      a.k,
-      [&](uint32_t r, uint32_t k) -> T {
-        if (row0 + r >= g.rows || k >= a.k) return 0;
-        const uint32_t i = g.first + row0 + r, from = a.index_a ? (uint32_t)a.index_a[i] : i;
-        return from < a.a_rows ? static_cast<const T*>(a.a)[(int64_t)from * a.lda + k] : T(0);
-      },
-      [&](uint32_t k, uint32_t n) -> T {
-        if (k >= a.k || col0 + n >= a.n) return 0;
-        return a.trans_b ? b[(int64_t)(col0 + n) * a.ldb + k] : b[(int64_t)k * a.ldb + col0 + n];
-      },
-      [&](uint32_t r, uint32_t n, T sum) {
-        if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
-      });
+  for (uint32_t tile = blockIdx.y; find_group(a, tile, kSide, &g); tile += gridDim.y) {
+    const uint32_t row0 = g.tile * kSide;
+    const T* b = static_cast<const T*>(a.b) + (int64_t)g.index * a.b_stride;
+    for (uint32_t col0 = blockIdx.x * kSide; col0 < a.n; col0 += gridDim.x * kSide) {
+      T* c = static_cast<T*>(a.c) + (int64_t)(g.first + row0) * a.ldc + col0;
+      tile_product<T>(
+          a.k,
+          [&](uint32_t r, uint32_t k) -> T {
+            if (row0 + r >= g.rows || k >= a.k) return 0;
+            const uint32_t i = g.first + row0 + r, from = a.index_a ? (uint32_t)a.index_a[i] : i;
+            return from < a.a_rows ? static_cast<const T*>(a.a)[(int64_t)from * a.lda + k] : T(0);
+          },
+          [&](uint32_t k, uint32_t n) -> T {
+            if (k >= a.k || col0 + n >= a.n) return 0;
+            return a.trans_b ? b[(int64_t)(col0 + n) * a.ldb + k] : b[(int64_t)k * a.ldb + col0 + n];
+          },
+          [&](uint32_t r, uint32_t n, T sum) {
+            if (row0 + r < g.rows && col0 + n < a.n) put(c + (int64_t)r * a.ldc + n, sum, a.alpha, a.beta);
+          });
+    }
+  }
 }
 
-template <class T>
+// Of floats whose rows lie further apart than the tiles' offsets reach.
 __global__ void __launch_bounds__(256) grouped_weights_kernel(const GroupedArgs a) {
-  const uint32_t group = blockIdx.z, row0 = blockIdx.y * kSide, col0 = blockIdx.x * kSide;
+  const uint32_t group = blockIdx.z;
   const uint2 rows = group_rows(a, group);
-  T* c = static_cast<T*>(a.c) + (int64_t)group * a.c_stride;
-  auto element = [&](const void* p, const int32_t* index, uint32_t count, int64_t ld, uint32_t k, uint32_t column, uint32_t width) -> T {
+  float* c = static_cast<float*>(a.c) + (int64_t)group * a.c_stride;
+  auto element = [&](const void* p, const int32_t* index, uint32_t count, int64_t ld, uint32_t k, uint32_t column, uint32_t width) -> float {
     if (k >= rows.y || column >= width) return 0;
     const uint32_t i = rows.x + k, from = index ? (uint32_t)index[i] : i;
-    return from < count ? static_cast<const T*>(p)[(int64_t)from * ld + column] : T(0);
+    return from < count ? static_cast<const float*>(p)[(int64_t)from * ld + column] : 0.f;
   };
-  tile_product<T>(
-      rows.y, [&](uint32_t r, uint32_t k) { return element(a.a, a.index_a, a.a_rows, a.lda, k, row0 + r, a.m); },
-      [&](uint32_t k, uint32_t n) { return element(a.b, a.index_b, a.b_rows, a.ldb, k, col0 + n, a.n); },
-      [&](uint32_t r, uint32_t n, T sum) {
-        if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)(row0 + r) * a.ldc + col0 + n, sum, a.alpha, a.beta);
-      });
+  for (uint32_t row0 = blockIdx.y * kSide; row0 < a.m; row0 += gridDim.y * kSide)
+    for (uint32_t col0 = blockIdx.x * kSide; col0 < a.n; col0 += gridDim.x * kSide)
+      tile_product<float>(
+          rows.y, [&](uint32_t r, uint32_t k) { return element(a.a, a.index_a, a.a_rows, a.lda, k, row0 + r, a.m); },
+          [&](uint32_t k, uint32_t n) { return element(a.b, a.index_b, a.b_rows, a.ldb, k, col0 + n, a.n); },
+          [&](uint32_t r, uint32_t n, float sum) {
+            if (row0 + r < a.m && col0 + n < a.n) put(c + (int64_t)(row0 + r) * a.ldc + col0 + n, sum, a.alpha, a.beta);
+          });
 }
 
 // ------------------------------------------------------------------ float: the matrix cores, three pieces to a float
@@ -151,6 +157,7 @@ constexpr uint32_t kBand = 8, kRun = 16;
 
 struct GroupedPlan {
   uint32_t m_tiles, n_tiles, units, parts, run_shift;   // m_tiles: as many as there can be; units: of all parts
+  uint32_t first;                                       // unit of this launch
   FastDiv part_fd, band_fd;
 };
 
@@ -160,7 +167,7 @@ struct TilePlace {
 
 __device__ __forceinline__ bool place_of(const GroupedPlan& p, TilePlace* out) {
   const uint32_t at = blockIdx.x / kXcds, run = at >> p.run_shift;
-  uint32_t unit = ((run * kXcds + blockIdx.x % kXcds) << p.run_shift) + (at - (run << p.run_shift));
+  uint32_t unit = p.first + ((run * kXcds + blockIdx.x % kXcds) << p.run_shift) + (at - (run << p.run_shift));
   if (unit >= p.units) return false;
   uint32_t band, rest;
   p.part_fd.divmod(unit, out->part, unit);
@@ -679,24 +686,27 @@ __global__ void __launch_bounds__(256) grouped_sum_kernel(const GroupedArgs a, c
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-struct Launch {
-  GroupedPlan plan;
-  dim3 grid;
-};
+// A launch of 2^32 lanes or more is refused, and a block has up to 1024: more tiles than this take several launches.
+constexpr int64_t kMostUnits = int64_t(1) << 21, kMostTiles = (int64_t(1) << 31) - 1;
+static_assert(kMostUnits % (kXcds * kRun) == 0, "a launch ends with a round of runs");
 
-Launch launch_of(int64_t m_tiles, int64_t n_tiles, int64_t parts) {
-  Launch l;
-  l.plan.m_tiles = (uint32_t)m_tiles;
-  l.plan.n_tiles = (uint32_t)n_tiles;
-  l.plan.units = (uint32_t)(m_tiles * n_tiles * parts);
-  l.plan.parts = (uint32_t)parts;
-  l.plan.run_shift = 0;
-  while ((uint32_t(2) << l.plan.run_shift) <= std::min(kRun, l.plan.units / kXcds)) ++l.plan.run_shift;
-  l.plan.part_fd = FastDiv((uint32_t)(m_tiles * n_tiles));
-  l.plan.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
-  const int64_t round = (int64_t)kXcds << l.plan.run_shift;
-  l.grid = dim3((uint32_t)(ceil_div(l.plan.units, round) * round));
-  return l;
+// Calls `launch(grid, plan)` for launches that together have a block for every unit.
+template <class F>
+void for_launches(int64_t m_tiles, int64_t n_tiles, int64_t parts, F launch) {
+  GroupedPlan p;
+  p.m_tiles = (uint32_t)m_tiles;
+  p.n_tiles = (uint32_t)n_tiles;
+  p.units = (uint32_t)(m_tiles * n_tiles * parts);
+  p.parts = (uint32_t)parts;
+  p.run_shift = 0;
+  while ((uint32_t(2) << p.run_shift) <= std::min(kRun, p.units / kXcds)) ++p.run_shift;
+  p.part_fd = FastDiv((uint32_t)(m_tiles * n_tiles));
+  p.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
+  const int64_t round = (int64_t)kXcds << p.run_shift;
+  for (int64_t first = 0; first < p.units; first += kMostUnits) {
+    p.first = (uint32_t)first;
+    launch(dim3((uint32_t)(ceil_div(std::min(p.units - first, kMostUnits), round) * round)), p);
+  }
 }
 
 // Sums whose k is divided among blocks: their products go to scratch, and a second launch adds them up.
@@ -799,10 +809,12 @@ void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks64, int
 // Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
 // from 1024 on eight or sixteen are as fast or faster.
 constexpr int64_t kFewK = 768;
-// Tiles of a launch: 2^32 lanes or more are refused, and a block has up to 1024.
-constexpr int64_t kMostUnits = int64_t(1) << 21, kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
+constexpr int64_t kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
 
-uint32_t tiles_of(int64_t n, int64_t side) { return (uint32_t)((n + side - 1) / side); }
+// Of the kernels whose blocks walk over tiles: as many as one launch may have along each side.
+dim3 plain_grid(int64_t columns, int64_t row_tiles, int64_t groups) {
+  return dim3((uint32_t)std::min(ceil_div(columns, kSide), kMostUnits), (uint32_t)std::min<int64_t>(row_tiles, 65535), (uint32_t)groups);
+}
 
 constexpr int64_t kMostExtent = (int64_t(1) << 31) - 1;
 bool extent(int64_t n) { return n >= 0 && n <= kMostExtent; }
@@ -857,18 +869,18 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
     const Parts<double> parts(s, best.parts, cells);
     if (parts.count() < best.parts) best = choose(1);
     const int64_t side = best.height, m_tiles = row_count / side + even_groups, n_tiles = ceil_div(b_col_count, side);
-    if (m_tiles * n_tiles <= kMostUnits) {
-      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
-      GroupedArgs of_parts = parts.args(g, 0);
-      of_parts.part = (uint32_t)ceil_div(a_col_count, parts.count());
-      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      parts.add_up<false>(g);
-      note_kernel(parts.count() > 1 ? "grouped_double+grouped_sum" : "grouped_double");
-      return after_launch(s);
-    }
+    CT_REQUIRE(m_tiles <= kMostTiles / parts.count() / n_tiles, "ct_grouped_gemm: %lld rows of %lld columns", (long long)row_count, (long long)b_col_count);
+    GroupedArgs of_parts = parts.args(g, 0);
+    of_parts.part = (uint32_t)ceil_div(a_col_count, parts.count());
+    for_launches(m_tiles, n_tiles, parts.count(), [&](dim3 grid, const GroupedPlan& plan) {
+      if (side == 64 && trans_b) hipLaunchKernelGGL((grouped_double_kernel<64, true>), grid, dim3(256), 0, s, of_parts, plan);
+      else if (side == 64) hipLaunchKernelGGL((grouped_double_kernel<64, false>), grid, dim3(256), 0, s, of_parts, plan);
+      else if (trans_b) hipLaunchKernelGGL((grouped_double_kernel<32, true>), grid, dim3(256), 0, s, of_parts, plan);
+      else hipLaunchKernelGGL((grouped_double_kernel<32, false>), grid, dim3(256), 0, s, of_parts, plan);
+    });
+    parts.add_up<false>(g);
+    note_kernel(parts.count() > 1 ? "grouped_double+grouped_sum" : "grouped_double");
+    return after_launch(s);
   }
   if (dtype == CT_F32 && a_row_count > 0 && a_col_count > 0) {
     // The tiles that there are if the groups are even, and the kernel that takes them soonest.  With 4096 by 1024 [n][k] and 8 groups,
@@ -887,30 +899,28 @@ int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, dou
     if (parts.count() < best.parts) best = choose(1);
     const bool thin = best.height == 16;
     const int64_t m_tiles = row_count / best.height + even_groups, n_tiles = ceil_div(b_col_count, best.width);
-    if (m_tiles * n_tiles <= kMostUnits) {
-      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
-      GroupedArgs of_parts = parts.args(g, 0);
-      of_parts.part = (uint32_t)(tiles_of_part(k_tiles, parts.count()) * kTileDepth);
-      auto launch = [&](auto of_b, auto of_not_b, int waves) {
-        if (trans_b) hipLaunchKernelGGL(of_b, l.grid, dim3(64 * waves), 0, s, of_parts, l.plan);
-        else hipLaunchKernelGGL(of_not_b, l.grid, dim3(64 * waves), 0, s, of_parts, l.plan);
-      };
-      const bool few = a_col_count <= kFewK;
-      if (thin && best.width == 64 && few) launch(grouped_thin_kernel<4, 4, true>, grouped_thin_kernel<4, 4, false>, 4);
-      else if (thin && best.width == 64) launch(grouped_thin_kernel<8, 4, true>, grouped_thin_kernel<8, 4, false>, 8);
-      else if (thin && few) launch(grouped_thin_kernel<4, 1, true>, grouped_thin_kernel<4, 1, false>, 4);
-      else if (thin) launch(grouped_thin_kernel<16, 1, true>, grouped_thin_kernel<16, 1, false>, 16);
-      else if (best.height == 128) launch(grouped_split_kernel<128, 128, 2, 4, true>, grouped_split_kernel<128, 128, 2, 4, false>, 8);
-      else launch(grouped_split_kernel<64, 64, 2, 2, true>, grouped_split_kernel<64, 64, 2, 2, false>, 4);
-      parts.add_up<false>(g);
-      static const char* const kNames[] = {"grouped_medium", "grouped_large", "grouped_medium+grouped_sum", "grouped_large+grouped_sum"};
-      note_kernel(thin ? "grouped_thin" : kNames[(best.height == 128) + 2 * (parts.count() > 1)]);
-      return after_launch(s);
-    }
+    CT_REQUIRE(m_tiles <= kMostTiles / parts.count() / n_tiles, "ct_grouped_gemm: %lld rows of %lld columns", (long long)row_count, (long long)b_col_count);
+    GroupedArgs of_parts = parts.args(g, 0);
+    of_parts.part = (uint32_t)(tiles_of_part(k_tiles, parts.count()) * kTileDepth);
+    auto launch = [&](auto of_b, auto of_not_b, int waves) {
+      for_launches(m_tiles, n_tiles, parts.count(), [&](dim3 grid, const GroupedPlan& plan) {
+        if (trans_b) hipLaunchKernelGGL(of_b, grid, dim3(64 * waves), 0, s, of_parts, plan);
+        else hipLaunchKernelGGL(of_not_b, grid, dim3(64 * waves), 0, s, of_parts, plan);
+      });
+    };
+    const bool few = a_col_count <= kFewK;
+    if (thin && best.width == 64 && few) launch(grouped_thin_kernel<4, 4, true>, grouped_thin_kernel<4, 4, false>, 4);
+    else if (thin && best.width == 64) launch(grouped_thin_kernel<8, 4, true>, grouped_thin_kernel<8, 4, false>, 8);
+    else if (thin && few) launch(grouped_thin_kernel<4, 1, true>, grouped_thin_kernel<4, 1, false>, 4);
+    else if (thin) launch(grouped_thin_kernel<16, 1, true>, grouped_thin_kernel<16, 1, false>, 16);
+    else if (best.height == 128) launch(grouped_split_kernel<128, 128, 2, 4, true>, grouped_split_kernel<128, 128, 2, 4, false>, 8);
+    else launch(grouped_split_kernel<64, 64, 2, 2, true>, grouped_split_kernel<64, 64, 2, 2, false>, 4);
+    parts.add_up<false>(g);
+    static const char* const kNames[] = {"grouped_medium", "grouped_large", "grouped_medium+grouped_sum", "grouped_large+grouped_sum"};
+    note_kernel(thin ? "grouped_thin" : kNames[(best.height == 128) + 2 * (parts.count() > 1)]);
+    return after_launch(s);
   }
-  const int64_t tiles = row_count / kSide + std::min(n_groups, row_count);
-  CT_REQUIRE(tiles <= 65535, "ct_grouped_gemm: %lld rows", (long long)row_count);
-  const dim3 grid(tiles_of(b_col_count, kSide), (uint32_t)tiles);
+  const dim3 grid = plain_grid(b_col_count, row_count / kSide + std::min(n_groups, row_count), 1);
   if (dtype == CT_F32) hipLaunchKernelGGL((grouped_kernel<float>), grid, dim3(256), 0, s, g);
   else hipLaunchKernelGGL((grouped_kernel<double>), grid, dim3(256), 0, s, g);
   note_kernel("grouped");
@@ -959,19 +969,20 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
     const Parts<float> parts(s, best.parts, cells);
     if (parts.count() < best.parts) best = choose(1);
     const int64_t m_tiles = n_groups * ceil_div(a_col_count, best.height), n_tiles = ceil_div(b_col_count, best.width);
-    if (m_tiles * n_tiles <= kMostUnits) {
-      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
-      const GroupedArgs of_parts = parts.args(g, a_col_count);
-      const bool wide = std::max(a_row_count * a_colstride, b_row_count * b_colstride) * size >= int64_t(1) << 32, large = best.height == 128;
-      if (large && !wide) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, false>), l.grid, dim3(512), 0, s, of_parts, l.plan);
-      else if (large) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, true>), l.grid, dim3(512), 0, s, of_parts, l.plan);
-      else if (!wide) hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, false>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      else hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, true>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      parts.add_up<true>(g);
-      static const char* const kNames[] = {"grouped_weights_medium", "grouped_weights_large", "grouped_weights_medium+grouped_sum", "grouped_weights_large+grouped_sum"};
-      note_kernel(kNames[large + 2 * (parts.count() > 1)]);
-      return after_launch(s);
-    }
+    CT_REQUIRE(m_tiles <= kMostTiles / parts.count() / n_tiles, "ct_grouped_gemm_weights: %lld by %lld results of %lld groups", (long long)a_col_count,
+               (long long)b_col_count, (long long)n_groups);
+    const GroupedArgs of_parts = parts.args(g, a_col_count);
+    const bool wide = std::max(a_row_count * a_colstride, b_row_count * b_colstride) * size >= int64_t(1) << 32, large = best.height == 128;
+    for_launches(m_tiles, n_tiles, parts.count(), [&](dim3 grid, const GroupedPlan& plan) {
+      if (large && !wide) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, false>), grid, dim3(512), 0, s, of_parts, plan);
+      else if (large) hipLaunchKernelGGL((grouped_weights_split_kernel<128, 128, 2, 4, true>), grid, dim3(512), 0, s, of_parts, plan);
+      else if (!wide) hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, false>), grid, dim3(256), 0, s, of_parts, plan);
+      else hipLaunchKernelGGL((grouped_weights_split_kernel<64, 64, 2, 2, true>), grid, dim3(256), 0, s, of_parts, plan);
+    });
+    parts.add_up<true>(g);
+    static const char* const kNames[] = {"grouped_weights_medium", "grouped_weights_large", "grouped_weights_medium+grouped_sum", "grouped_weights_large+grouped_sum"};
+    note_kernel(kNames[large + 2 * (parts.count() > 1)]);
+    return after_launch(s);
   }
   if (dtype == CT_F64) {
     auto choose = [&](int64_t most_parts) {
@@ -983,20 +994,18 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
     const Parts<double> parts(s, best.parts, cells);
     if (parts.count() < best.parts) best = choose(1);
     const int64_t side = best.height, m_tiles = n_groups * ceil_div(a_col_count, side), n_tiles = ceil_div(b_col_count, side);
-    if (m_tiles * n_tiles <= kMostUnits) {
-      const Launch l = launch_of(m_tiles, n_tiles, parts.count());
-      const GroupedArgs of_parts = parts.args(g, a_col_count);
-      if (side == 64) hipLaunchKernelGGL((grouped_weights_double_kernel<64>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      else hipLaunchKernelGGL((grouped_weights_double_kernel<32>), l.grid, dim3(256), 0, s, of_parts, l.plan);
-      parts.add_up<true>(g);
-      note_kernel(parts.count() > 1 ? "grouped_weights_double+grouped_sum" : "grouped_weights_double");
-      return after_launch(s);
-    }
+    CT_REQUIRE(m_tiles <= kMostTiles / parts.count() / n_tiles, "ct_grouped_gemm_weights: %lld by %lld results of %lld groups", (long long)a_col_count,
+               (long long)b_col_count, (long long)n_groups);
+    const GroupedArgs of_parts = parts.args(g, a_col_count);
+    for_launches(m_tiles, n_tiles, parts.count(), [&](dim3 grid, const GroupedPlan& plan) {
+      if (side == 64) hipLaunchKernelGGL((grouped_weights_double_kernel<64>), grid, dim3(256), 0, s, of_parts, plan);
+      else hipLaunchKernelGGL((grouped_weights_double_kernel<32>), grid, dim3(256), 0, s, of_parts, plan);
+    });
+    parts.add_up<true>(g);
+    note_kernel(parts.count() > 1 ? "grouped_weights_double+grouped_sum" : "grouped_weights_double");
+    return after_launch(s);
   }
-  CT_REQUIRE(tiles_of(a_col_count, kSide) <= 65535, "ct_grouped_gemm_weights: %lld columns of a", (long long)a_col_count);
-  const dim3 grid(tiles_of(b_col_count, kSide), tiles_of(a_col_count, kSide), (uint32_t)n_groups);
-  if (dtype == CT_F32) hipLaunchKernelGGL((grouped_weights_kernel<float>), grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL((grouped_weights_kernel<double>), grid, dim3(256), 0, s, g);
+  hipLaunchKernelGGL(grouped_weights_kernel, plain_grid(b_col_count, ceil_div(a_col_count, kSide), n_groups), dim3(256), 0, s, g);
   note_kernel("grouped_weights");
   return after_launch(s);
 }

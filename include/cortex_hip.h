@@ -630,7 +630,8 @@ int ct_route_experts_gradient(void* stream, void* logits_gradient, int64_t logit
  * [n_groups + 1] do not decrease and lie in [0, row_count]; rows of no group are not touched.  Groups of no rows cost
  * nothing.  Float products are formed as ct_gemm's are, or by float instructions where groups have few rows.  Here and below
  * c overlaps no operand, offsets and indexes among them, and few results of long sums are summed in parts that a second launch
- * adds up, in scratch memory of the stream; a captured stream that has none does without, which may differ in the last bits. */
+ * adds up, in scratch memory of the stream; a captured stream that has none does without, which may differ in the last bits.
+ * Results of 2^31 tiles, of 16 rows by 16 columns or more each, are refused. */
 int ct_grouped_gemm(void* stream, void* c, int64_t c_colstride, int trans_b, double alpha, const void* a,
                     int64_t a_row_count, int64_t a_col_count, int64_t a_colstride, const int32_t* index,
                     const void* b, int64_t b_col_count, int64_t b_colstride, int64_t b_stride,

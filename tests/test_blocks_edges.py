@@ -199,3 +199,17 @@ def test_clipping_long_lists_into_another_tensor():
         with pytest.raises(capi.CortexHipError) as e:
             capi.call("ct_clip_gradients", *clip(gradients, outputs, counts, result=1 << 30))
         assert e.value.status == 1 and "overlaps" in e.value.message, (seed, e.value.message)
+
+
+@pytest.mark.parametrize("change", [dict(n_groups=65535, row_count=(1 << 31) - 1, a_row_count=(1 << 31) - 1, b_col_count=1 << 20, c_colstride=1 << 20),
+                                    dict(row_count=(1 << 31) - 1, a_row_count=(1 << 31) - 1, b_col_count=1 << 20, c_colstride=1 << 20, dtype=capi.F64)], ids=str)
+def test_products_of_more_tiles_than_can_be_counted(change):
+    far = 1 << 61
+    refuses("rows of", "ct_grouped_gemm", *grouped(**{**change, "c": 1 << 62, "a": 1 << 30, "b": far, "offsets": 1 << 20}))
+
+
+def test_products_over_rows_of_more_tiles_than_can_be_counted():
+    side = 1 << 22
+    refuses("by 4194304 results", "ct_grouped_gemm_weights",
+            *weights(c=1 << 62, c_colstride=side, c_stride=side * side, a=1 << 40, a_col_count=side, a_colstride=side, b=1 << 41, b_col_count=side,
+                     b_colstride=side))

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from cortex_amd import blocks
+from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
 from test_gpu_blocks import D, Owned, read, run_route, stream, strides_of  # noqa: F401  (fixtures among them)
@@ -91,6 +92,64 @@ def test_route_gradient_in_place_of_the_logits(D, size, renormalize):
     blocks.route_experts_gradient(to, dw, weights, experts, apart, renormalize=renormalize)
     blocks.route_experts_gradient(apart, dw, weights, experts, apart, renormalize=renormalize)
     assert np.array_equal(read(apart), read(to)) and np.any(read(to) != 0)
+
+
+# ------------------------------------------------------------------------------------------------- products of very many tiles
+
+def test_products_of_more_tiles_than_a_launch_takes(D, stream):
+    """Over 2^21 tiles of 16 rows (32 of doubles), k below a tile's and a single column.  Whole numbers: every sum exact."""
+    rng = np.random.default_rng(65)
+    rows, k = ((1 << 25) + 37, 2) if D.datatype == "float" else ((1 << 26) + 100, 1)
+    cuts = [5, 5 + (1 << 20), rows - 3]
+    a, b = rng.integers(-7, 8, (rows, k), np.int8).astype(D.type), rng.integers(1, 8, (3, 1, k)).astype(D.type)
+    c = D.tensor(np.full((rows, 1), 7.25))
+    blocks.grouped_gemm(c, True, 1.0, D.tensor(a), D.tensor(b), 0.0, D.tensor([cuts[0], cuts[1], cuts[1], cuts[2]], "int"))
+    got = read(c)
+    assert np.all(got[:cuts[0]] == 7.25) and np.all(got[cuts[2]:] == 7.25)
+    for e, i in ((0, slice(cuts[0], cuts[1])), (2, slice(cuts[1], cuts[2]))):
+        assert np.array_equal(got[i, 0], a[i] @ b[e, 0])
+
+
+def test_products_over_rows_of_more_tiles_than_a_launch_takes(D):
+    """65535 groups of 33 tiles, most of them without rows: the products of those that have some, zeros in all others."""
+    rng = np.random.default_rng(66)
+    groups, rows, n = 65535, 300, 2049 if D.datatype == "float" else 1025
+    group_of = np.sort(rng.integers(0, groups, rows))
+    group_of[-1] = groups - 1
+    offsets = np.searchsorted(group_of, np.arange(groups + 1))
+    a, b = rng.integers(-7, 8, (rows, 1)).astype(D.type), rng.integers(-7, 8, (rows, n)).astype(D.type)
+    c = D.tensor(np.full((groups, 1, n), 7.25))
+    blocks.grouped_gemm_weights(c, 1.0, D.tensor(a), D.tensor(b), 0.0, D.tensor(offsets, "int"))
+    want = np.zeros((groups, n), D.type)
+    np.add.at(want, group_of, a * b)
+    assert np.array_equal(read(c)[:, 0], want)
+
+
+def test_products_without_terms_over_very_many_rows(D, stream):
+    """More row tiles than a launch has rows of blocks: beta times what was there, in the groups' rows."""
+    rows, n, code = 5_000_000, 3, capi.DTYPE_CODES[D.datatype]
+    c = np.arange(rows * n, dtype=np.int64).reshape(rows, n) % 1021 + 1.0
+    offsets, tc = D.tensor([7, 4_500_000, rows - 9], "int"), D.tensor(c)
+    capi.call("ct_grouped_gemm", stream.handle, tc.buffer.ptr, n, 1, 1.0, None, rows, 0, 4, None, None, n, 4, 0, offsets.buffer.ptr, 2, rows, 0.5, code)
+    c[7:rows - 9] *= 0.5
+    assert np.array_equal(read(tc), c.astype(D.type))
+
+
+def test_products_over_rows_far_apart_of_very_many_columns(stream):
+    D = Owned("float")
+    rng = np.random.default_rng(67)
+    m, ld = 65535 * 64 + 100, (1 << 30) + 5
+    x, y = rng.integers(-7, 8, (2, m)).astype(np.float32), np.array([[2], [-3]], np.float32)
+    far = ct.new_tensor([ld + m], datatype="float")
+    D.kept.append(far)
+    for r in range(2):
+        row = D.tensor(x[r])
+        capi.call("ct_memcpy_async", far.buffer.ptr + 4 * ld * r, row.buffer.ptr, 4 * m, capi.COPY_D2D, stream.handle)
+    w = D.tensor(np.zeros((1, m, 1)))
+    capi.call("ct_grouped_gemm_weights", stream.handle, w.buffer.ptr, 1, m, 1.0, far.buffer.ptr, 2, m, ld, None, D.tensor(y).buffer.ptr, 2, 1, 1, None,
+              D.tensor([0, 2], "int").buffer.ptr, 1, 2, 0.0, capi.F32)
+    assert np.array_equal(read(w)[0], x.T @ y)
+    D.free()
 
 
 # ------------------------------------------------------------------------------------------------- combining
