@@ -76,6 +76,28 @@ def test_norm_gradients_between_the_rows_of_an_operand(D):
         assert np.array_equal(a, b) and np.any(a != 0)
 
 
+@pytest.mark.parametrize("shape", [(6, 3), (37, 70), (300, 300), (9, 5003), (2, 17000)], ids=str)
+@pytest.mark.parametrize("by_column", [False, True])
+def test_norms_with_a_gate_whose_rows_lie_apart(D, shape, by_column):
+    """A full gate, or one of a value to a row, that is a block of a wider matrix: the same bits as of one by itself."""
+    rows, width = shape
+    rng = np.random.default_rng(68)
+    gate = rng.standard_normal((rows, width if by_column else 1))
+    z, dout, dh = (D.tensor(rng.standard_normal((rows, width))) for _ in range(3))
+    p = {"post-scale": D.tensor(rng.standard_normal(width)), "post-bias": D.tensor(rng.standard_normal(width))}
+    d = blocks.norm_descriptor(post="rms", pre="layer")
+    results = []
+    for given in (D.tensor(gate), D.block(gate, 5)):
+        q = {**p, "gate": given}
+        out, h, dz, dr = (D.tensor(np.zeros((rows, width))) for _ in range(4))
+        stats, g = D.tensor(np.zeros((4, rows))), {k: D.tensor(np.full(t.shape(), 3.0)) for k, t in q.items()}
+        blocks.norm_residual(out, h, stats, z, None, q, d)
+        blocks.norm_residual_gradient(dz, dr, g, dout, dh, z, out, stats, q, d)
+        results.append([read(t) for t in (out, h, stats, dz, dr, *g.values())])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b) and np.any(a != 0)
+
+
 # ------------------------------------------------------------------------------------------------- routing
 
 @pytest.mark.parametrize("renormalize", [True, False])
