@@ -4,10 +4,12 @@
 // index.  Logits are compared as integers that order as they do, NaN above all, -infinity below every one that may be chosen.
 // The order of rows is a stable counting sort of the assignments (t, j) by expert: blocks of consecutive tokens count their
 // assignments, one block to an expert adds the blocks' counts up, and each block then knows the place of its own.  The choice is bound by its
-// instructions, some hundred to a choice of a wave's four tokens: 65536 tokens, 8 of 128 experts, 28 us of 41; 14 for the gradient, which is bound by memory.
+// instructions, some hundred to a choice of a wave's four tokens: 65536 tokens, 8 of 128 experts, 28 us of 41 (57 in double); 14 for the gradient, which is
+// bound by memory.
 //
-// Combining reads the rows of a token once and writes its sum; its gradient reads the token's gradient and its rows once and
-// writes as many.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us (4.8 TB/s) and 115 (5.1).
+// Combining reads the rows of a token once and writes its sum; its gradient reads each row once, the token's gradient once for each of
+// them, out of the caches from the second time on, and writes as many rows.  Memory bounds both: 16384 tokens of 4 rows of 1000 floats 69 us
+// (4.8 TB/s) and 109 to 118 (5.0 to 5.4).
 #include <algorithm>
 
 #include "elementwise.h"

@@ -584,8 +584,10 @@ int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, voi
  * the forward call.  Any result may be NULL: input_gradient, residual_gradient [rows, width], gate_gradient (the gate's
  * shape; sums over what the gate was broadcast along), the gradients of the scales and biases [width].  All are
  * overwritten.  input_gradient and residual_gradient may be output_gradient or normalized_gradient itself, but not one
- * another; other overlaps of a gradient with an operand or another gradient are refused.  Column sums run over the rows in
- * double once they leave a block's registers; the partial sums live in the stream's scratch memory (at most 64 MiB and, for rows that do not fit registers, 32 bytes to each and 8 to a column). */
+ * another; other overlaps of a gradient with an operand or another gradient are refused.  Column sums run over a block's
+ * rows in the tensor's type (in double for rows that do not fit registers) and over the blocks in double; the blocks' sums,
+ * in the tensor's type, live in the stream's scratch memory (at most 64 MiB and, for rows that do not fit registers, 32 bytes
+ * to each and 8 to a column). */
 int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims,
                               void* residual_gradient, const ct_dims* residual_gradient_dims,
                               void* gate_gradient, void* post_scale_gradient, void* post_bias_gradient,
