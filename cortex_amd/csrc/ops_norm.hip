@@ -403,9 +403,8 @@ struct NormFinishArgs {
 
 // The blocks' sums of 32 columns, added in their order within each of 32 runs of blocks, in double.
 template <class T>
-__global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs a) {
-  __shared__ double lds[2][32][32];
-  const uint32_t column = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
+__device__ __forceinline__ void finish_columns(const NormFinishArgs& a, uint32_t column0, double (&lds)[2][32][32]) {
+  const uint32_t column = column0 + threadIdx.x % 32, run = threadIdx.x / 32;
   // S1 and S0 by one half of the blocks, T1 and T0 by the other
   const int half = 2 * blockIdx.y;
 #pragma unroll
@@ -444,6 +443,17 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs 
   const double of_gate = scale * sums[0] + (a.slot[1] >= 0 ? bias * sums[1] : 0.0);
   if (a.gate_kind == kColumnGate) store(a.gate_gradient, of_gate);
   if (a.by_column) static_cast<double*>(a.by_column)[column] = of_gate;
+}
+
+// A launch of 2^32 lanes is refused: blocks take more than one run of columns of rows that long.
+constexpr int64_t kMostFinishBlocks = int64_t(1) << 21;
+template <class T>
+__global__ void __launch_bounds__(1024) norm_finish_kernel(const NormFinishArgs a) {
+  __shared__ double lds[2][32][32];
+  for (uint32_t column0 = blockIdx.x * 32; column0 < a.width; column0 += gridDim.x * 32) {
+    finish_columns<T>(a, column0, lds);
+    __syncthreads();
+  }
 }
 
 template <class T>
@@ -761,7 +771,7 @@ int norm_gradient_typed(hipStream_t s, NormGradientArgs a, NormFinishArgs f) {
   }
   if (rc) return rc;
   if (f.by_column) f.by_column = by_column;
-  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((a.width + 31) / 32, 2), dim3(1024), 0, s, f);
+  if (sums) hipLaunchKernelGGL((norm_finish_kernel<T>), dim3((uint32_t)std::min<int64_t>((a.width + 31) / 32, kMostFinishBlocks), 2), dim3(1024), 0, s, f);
   if (f.by_column) hipLaunchKernelGGL((norm_scalar_gate_kernel<T>), dim3(1), dim3(256), 0, s, by_column, a.width, static_cast<T*>(f.gate_gradient));
   note_kernel(fits ? "norm_residual_gradient" : "norm_residual_gradient_long");
   return after_launch(s);

@@ -76,6 +76,22 @@ def test_norm_gradients_between_the_rows_of_an_operand(D):
         assert np.array_equal(a, b) and np.any(a != 0)
 
 
+def test_norm_gradient_of_a_row_of_more_columns_than_a_launch_s_lanes(stream):
+    """The columns' sums of a row of over 2^27 floats.  All ones by a scale of ones and an epsilon of 3: the rate is exactly a half, the
+    sum over the row of y zh is its length over 2, and the row's gradient (1 - 1 / 4) / 2."""
+    D = Owned("float")
+    width = (1 << 27) + 33
+    ones = np.ones((1, width), np.float32)
+    d = blocks.norm_descriptor(post="rms", pre="none", epsilon=3.0)
+    z, out, scale, dz, dr = (D.tensor(x) for x in (ones, ones, ones[0], 0 * ones, 0 * ones))
+    stats, g = D.tensor(np.zeros((4, 1))), {"post-scale": D.tensor(np.full(width, 3.0, np.float32))}
+    blocks.norm_residual(out, None, stats, z, None, {"post-scale": scale}, d)
+    assert np.array_equal(read(stats)[:, 0], [0, 0.5, 0, 1]) and np.all(read(out) == 0.5)
+    blocks.norm_residual_gradient(dz, dr, g, z, None, z, out, stats, {"post-scale": scale}, d)
+    assert np.all(read(g["post-scale"]) == 0.5) and np.all(read(dz) == 0.375) and np.all(read(dr) == 1)
+    D.free()
+
+
 @pytest.mark.parametrize("shape", [(6, 3), (37, 70), (300, 300), (9, 5003), (2, 17000)], ids=str)
 @pytest.mark.parametrize("by_column", [False, True])
 def test_norms_with_a_gate_whose_rows_lie_apart(D, shape, by_column):
