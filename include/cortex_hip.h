@@ -586,8 +586,8 @@ int ct_norm_residual(void* stream, void* output, const ct_dims* output_dims, voi
  * overwritten.  input_gradient and residual_gradient may be output_gradient or normalized_gradient itself, but not one
  * another; other overlaps of a gradient with an operand or another gradient are refused.  Column sums run over a block's
  * rows in the tensor's type (in double for rows that do not fit registers) and over the blocks in double; the blocks' sums,
- * in the tensor's type, live in the stream's scratch memory (at most 64 MiB and, for rows that do not fit registers, 32 bytes
- * to each and 8 to a column). */
+ * in the tensor's type, live in the stream's scratch memory (at most 64 MiB, or four values to a column if that is more, and 8
+ * bytes to a column; for rows that do not fit registers 32 bytes to each). */
 int ct_norm_residual_gradient(void* stream, void* input_gradient, const ct_dims* input_gradient_dims,
                               void* residual_gradient, const ct_dims* residual_gradient_dims,
                               void* gate_gradient, void* post_scale_gradient, void* post_bias_gradient,
