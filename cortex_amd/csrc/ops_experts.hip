@@ -658,8 +658,8 @@ int ct_route_experts(void* stream, int32_t* experts, void* weights, int32_t* off
   a.n = (uint32_t)n; a.n_experts = (uint32_t)n_experts; a.n_chosen = (uint32_t)n_chosen;
   a.renormalize = renormalize != 0;
   if (!is_few(n, n_experts, n_chosen, size)) {
-    // 16 tokens to a block, 64 where there are blocks enough, more where the blocks' counts would take more than 8 MiB
-    const int64_t most_blocks = std::max<int64_t>(1, (int64_t(2) << 20) / (n_experts + 1));
+    // 16 tokens to a block, 64 where there are blocks enough, more where the blocks' counts and their totals would take more than 8 MiB
+    const int64_t most_blocks = (int64_t(2) << 20) / (n_experts + 1) - 1;
     a.tokens_per_block = (uint32_t)std::max<int64_t>(n <= 8192 ? 16 : 64, (n + most_blocks - 1) / most_blocks);
     a.blocks = (uint32_t)((n + a.tokens_per_block - 1) / a.tokens_per_block);
     void* scratch = nullptr;

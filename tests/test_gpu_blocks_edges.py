@@ -5,9 +5,10 @@ import pytest
 
 from cortex_amd import blocks
 from cortex_amd import capi
+from cortex_amd import driver as drv
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
-from test_gpu_blocks import D, Owned, read, run_route, stream, strides_of  # noqa: F401  (fixtures among them)
+from test_gpu_blocks import D, Owned, as_released, read, run_route, stream, strides_of  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -130,6 +131,50 @@ def test_route_gradient_in_place_of_the_logits(D, size, renormalize):
     blocks.route_experts_gradient(to, dw, weights, experts, apart, renormalize=renormalize)
     blocks.route_experts_gradient(apart, dw, weights, experts, apart, renormalize=renormalize)
     assert np.array_equal(read(apart), read(to)) and np.any(read(to) != 0)
+
+
+def test_routing_is_recorded_with_the_scratch_that_it_is_said_to_need(as_released):
+    """8 MiB reserved ahead: the most counts that there are, and their totals, fit; nothing is allocated while the stream is captured."""
+    import ctypes as C
+    rt = C.CDLL("libamdhip64.so")
+    rt.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    rt.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    rt.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    rt.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    rt.hipGraphExecDestroy.argtypes = rt.hipGraphDestroy.argtypes = [C.c_void_p]
+    device = drv.HipDriver().default_device()
+    stream, loader = device.create_stream(), device.create_stream()
+    capi.call("ct_stream_reserve_scratch", stream.handle, 8 << 20, 0)
+    n, e = 64 * 2048, 1023
+    D = Owned("float")
+    with ct.tensor_context(loader, "float"):
+        logits = ct.new_tensor([n, e])
+        D.kept.append(logits)
+        results = [D.tensor(np.full(s, 77), kind) for s, kind in (((n, 1), "int"), ((n, 1), "float"), ((e + 1,), "int"), ((n,), "int"), ((n, 1), "int"))]
+        blocks.route_experts(*results, logits)     # the kernels are loaded
+        want = [read(t) for t in results]
+        assert np.all(want[0] == 0) and np.all(want[1] == 1) and want[2].tolist() == [0] + [n] * e and np.array_equal(want[3], np.arange(n))
+        for t in results:
+            capi.call("ct_memset", loader.handle, t.buffer.ptr, capi.DTYPE_CODES[t.get_datatype()], 77.0, t.ecount())
+        capi.call("ct_stream_sync", loader.handle)
+    with ct.tensor_context(stream, "float"):
+        graph, graph_exec = C.c_void_p(), C.c_void_p()
+        assert rt.hipStreamBeginCapture(stream.handle, 1) == 0
+        try:
+            blocks.route_experts(*results, logits)
+        finally:
+            ended = rt.hipStreamEndCapture(stream.handle, C.byref(graph))
+        assert ended == 0 and graph.value
+        assert rt.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+        for _ in range(2):
+            assert rt.hipGraphLaunch(graph_exec, stream.handle) == 0
+            for a, b in zip(want, results):
+                assert np.array_equal(a, read(b))
+        capi.call("ct_stream_sync", stream.handle)
+        assert rt.hipGraphExecDestroy(graph_exec) == 0 and rt.hipGraphDestroy(graph) == 0
+        D.free()
+    stream.release()
+    loader.release()
 
 
 # ------------------------------------------------------------------------------------------------- products of very many tiles
