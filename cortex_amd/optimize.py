@@ -15,6 +15,7 @@ import array
 import dataclasses
 
 from . import capi
+from . import dimensions as dims
 
 
 def adam(**kwargs) -> dict:
@@ -57,13 +58,13 @@ def _dense_buffer(x):
     if not hasattr(x, "buffer"):
         return x, None
     shape, strides = x.dimensions["shape"], x.dimensions["strides"]
-    n = x.ecount()
-    order = [(extent, stride) for extent, stride in zip(shape, strides) if extent != 1] if n else []
-    expected = 1
+    n, dense, expected = x.ecount(), dims.direct_shape(shape), 1
+    order = [(int(extent), int(stride)) for extent, stride in zip(shape, strides) if extent != 1] if n and dense else []
     for extent, stride in sorted(order, key=lambda d: d[1]):
-        if type(extent) is not int or stride != expected:
-            raise ValueError("clip_gradients: tensors must be dense")
+        dense = dense and stride == expected
         expected *= extent
+    if not dense:
+        raise ValueError("clip_gradients: tensors must be dense")
     as_counted = all(a[1] > b[1] for a, b in zip(order, order[1:]))
     return x.buffer if x.buffer.ecount() == n else x.buffer.sub_buffer(0, n), None if as_counted else order
 

@@ -4,6 +4,7 @@ import ctypes as C
 import random
 import struct
 
+import numpy as np
 import pytest
 
 from cortex_amd import capi
@@ -65,6 +66,24 @@ def test_clipping_takes_results_in_the_order_of_their_gradients(native, monkeypa
                                ([plain, turned], [turned, plain]), ([at(4096, 3, 2, strides=[1, 3])], [at(12288, 2, 3, strides=[1, 2])])):
         with pytest.raises(ValueError, match="order"):
             clipped(gradients, outputs)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_clipping_takes_extents_of_any_whole_number(native, monkeypatch):
+    """A shape of numpy's numbers, as other calls take it; an index tensor in its place is refused."""
+    if not native:
+        monkeypatch.setattr(capi, "front", None)
+    x, turned = at(4096, 2, 3), at(8192, 2, 3)
+    x.dimensions = {"shape": [np.int64(2), np.int32(3)], "strides": [np.int64(3), 1]}
+    turned.dimensions = {"shape": [np.int64(2), 3], "strides": [1, np.int64(2)]}
+    assert clipped([x, turned]) == ((4096, 8192), (6, 6), (4096, 8192))
+    assert clipped([x], [at(12288, 6)]) == ((4096,), (6,), (12288,))
+    with pytest.raises(ValueError, match="order"):
+        clipped([turned], [at(12288, 6)])
+    indexed = at(4096, 2, 3, count=100)
+    indexed.dimensions = {"shape": [t(2, datatype="int"), 3], "strides": [3, 1]}
+    with pytest.raises(ValueError, match="must be dense"):
+        clipped([indexed])
 
 
 @pytest.mark.parametrize("native", [True, False])
