@@ -14,6 +14,7 @@ optimizers (:func:`cortex_amd.optimize.clip_gradients`).
 from __future__ import annotations
 
 from . import capi
+from . import dimensions as dims
 from . import tensor as ct
 from .tensor import Tensor, TensorError, check_stream
 
@@ -46,7 +47,7 @@ def _needed(name: str, **tensors) -> None:
 
 def _is_packed(t: Tensor) -> bool:
     shape, expected = t.dimensions["shape"], 1
-    if not all(type(n) is int for n in shape):
+    if not dims.direct_shape(shape):
         return False
     if 0 in shape:    # whatever its strides
         return True
@@ -78,10 +79,11 @@ def _packed(name: str, what: str, t: Tensor, shape) -> Tensor:
 def _rows(name: str, what: str, t: Tensor):
     """(rows, columns, distance of rows) of a matrix whose rows are contiguous; a vector is one row."""
     shape, strides = t.dimensions["shape"], t.dimensions["strides"]
+    if not 1 <= len(shape) <= 2 or not dims.direct_shape(shape):
+        raise TensorError(f"{name}: {what} must be a matrix")
+    shape, strides = [int(n) for n in shape], [int(n) for n in strides]
     if len(shape) == 1:
         shape, strides = [1, shape[0]], [shape[0], strides[0]]
-    if len(shape) != 2 or not all(type(n) is int for n in shape):
-        raise TensorError(f"{name}: {what} must be a matrix")
     rows, columns = shape
     if columns > 1 and strides[1] != 1:
         raise TensorError(f"{name}: the rows of {what} must be contiguous")
@@ -313,8 +315,9 @@ def route_experts_gradient(logits_gradient: Tensor, weights_gradient: Tensor, we
 def _matrices(name: str, what: str, t: Tensor):
     """(groups, rows, columns, distance of rows, distance of matrices) of a tensor of one matrix to a group."""
     shape, strides = t.dimensions["shape"], t.dimensions["strides"]
-    if len(shape) != 3 or not all(type(n) is int for n in shape):
+    if len(shape) != 3 or not dims.direct_shape(shape):
         raise TensorError(f"{name}: {what} must hold a matrix to each group")
+    shape, strides = [int(n) for n in shape], [int(n) for n in strides]
     if (shape[2] > 1 and strides[2] != 1) or (shape[1] > 1 and strides[1] < shape[2]):
         raise TensorError(f"{name}: the rows of {what} must be contiguous")
     return (*shape, max(strides[1], shape[2]), strides[0])

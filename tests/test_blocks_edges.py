@@ -7,6 +7,7 @@ import struct
 import numpy as np
 import pytest
 
+from cortex_amd import blocks
 from cortex_amd import capi
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
@@ -232,3 +233,34 @@ def test_products_over_rows_of_more_tiles_than_can_be_counted():
     refuses("by 4194304 results", "ct_grouped_gemm_weights",
             *weights(c=1 << 62, c_colstride=side, c_stride=side * side, a=1 << 40, a_col_count=side, a_colstride=side, b=1 << 41, b_col_count=side,
                      b_colstride=side))
+
+
+# ---------------------------------------------------------------- extents
+
+def whole(*shape, datatype="float"):
+    """A tensor whose extents and strides are numpy's whole numbers."""
+    x = t(*shape, datatype=datatype)
+    x.dimensions = {k: [np.int64(n) for n in x.dimensions[k]] for k in ("shape", "strides")}
+    return x
+
+
+def test_extents_of_any_whole_number():
+    """Every call reaches the stream with the numbers that plain ints give."""
+    d = blocks.norm_descriptor()
+    calls = []
+    for f, i in ((t, lambda *s: t(*s, datatype="int")), (whole, lambda *s: whole(*s, datatype="int"))):
+        stream = Recorder()
+        with ct.tensor_context(stream, "float"):
+            p = {"post-scale": f(8), "pre-scale": f(8), "gate": f(4, 1)}
+            blocks.norm_residual(f(4, 8), f(4, 8), f(4, 4), f(4, 8), f(4, 8), p, d)
+            blocks.norm_residual_gradient(f(4, 8), f(4, 8), {"gate": f(4, 1), "pre-scale": f(8)}, f(4, 8), f(4, 8), f(4, 8), f(4, 8), f(4, 4), p, d)
+            blocks.route_experts(i(4, 2), f(4, 2), i(6), i(8), i(4, 2), f(4, 5))
+            blocks.route_experts_gradient(f(4, 5), f(4, 2), f(4, 2), i(4, 2), f(4, 5), renormalize=False)
+            blocks.grouped_gemm(f(8, 3), True, 1.0, f(4, 8), f(5, 3, 8), 0.0, i(6), index=i(8))
+            blocks.grouped_gemm_weights(f(5, 3, 8), 1.0, f(8, 3), f(4, 8), 0.0, i(6), b_index=i(8))
+            blocks.combine_experts(f(4, 8), f(8, 8), f(4, 2), i(4, 2))
+            blocks.combine_experts_gradient(f(8, 8), f(4, 2), f(4, 8), f(8, 8), f(4, 2), i(4, 2))
+        calls.append([(name, [a if isinstance(a, (int, float, str, tuple)) else None for a in args]) for name, args in stream.calls])
+    assert calls[0] == calls[1] and len(calls[0]) == 8
+    numbers = [a for _, args in calls[1][2:] for a in args if a is not None and not isinstance(a, (float, str))]
+    assert all(type(a) in (int, bool) for a in numbers), numbers
