@@ -10,6 +10,7 @@
               the parameter buffer's offset inside the flat optimizer state (adam.clj:132-133)
     Adadelta  both accumulators addressed at the parameter offset (AdadeltaOptimizer.java:42-43)
     SGD       four tensor calls (sgd.clj:16-40), so the :cuda method's body serves unchanged
+    Muon      no counterpart in the reference: the momentum of a matrix made orthogonal by Newton-Schulz products
   UNEXERCISED (no JVM in the build image)."
   (:require [cortex.optimize :refer [PGradientOptimizer create-optimizer]]
             [cortex.optimize.sgd]
@@ -18,7 +19,10 @@
             [cortex.compute.nn.backend :as compute-backend]
             [cortex.compute.hip.ffi :as ffi :refer [call!]]
             [cortex.compute.hip.driver :refer [->ptr]]
-            [think.datatype.core :as dtype]))
+            [clojure.core.matrix :as m]
+            [think.datatype.core :as dtype])
+  (:import [com.sun.jna Memory]
+           [com.sun.jna.ptr LongByReference]))
 
 (set! *warn-on-reflection* true)
 
@@ -85,3 +89,62 @@
 (defmethod create-optimizer [:hip :sgd]
   [backend optimizer]
   ((get-method create-optimizer [:cuda :sgd]) backend optimizer))
+
+(defn orthogonalize-workspace
+  "Bytes of device memory with which all launches of orthogonalize! fill the chip; fewer serve, down to those of one matrix."
+  ^long [datatype n-matrices rows columns]
+  (let [result (LongByReference.)]
+    (call! "ct_orthogonalize_workspace" (long n-matrices) (long rows) (long columns) (int (ffi/datatype->code datatype)) result)
+    (.getValue result)))
+
+(defn- triples->native
+  "Three doubles to a step."
+  ^Memory [triples]
+  (let [values (vec (apply concat triples))
+        mem (Memory. (* 8 (count values)))]
+    (doseq [[^long i x] (map-indexed vector values)]
+      (.setDouble mem (* 8 i) (double x)))
+    mem))
+
+(defn orthogonalize!
+  "output = alpha * (input made orthogonal) + beta * output, of n-matrices matrices [rows columns].  `triples` holds the three
+  coefficients of each step; `workspace` is a device buffer of bytes that no other call uses meanwhile."
+  [stream output output-colstride output-stride alpha input input-colstride input-stride beta n-matrices rows columns triples
+   epsilon workspace]
+  (select-device! stream)
+  (let [coefficients (triples->native triples)]
+    (call! "ct_orthogonalize" (:handle stream) (->ptr output) (long output-colstride) (long output-stride) (double alpha)
+           (->ptr input) (long input-colstride) (long input-stride) (double beta) (long n-matrices) (long rows) (long columns)
+           coefficients (int (count triples)) (double epsilon) (->ptr workspace) (long (dtype/ecount workspace))
+           (ffi/dtype-code output))))
+
+(defrecord HipMuon [backend optimizer workspaces]
+  PGradientOptimizer
+  (batch-update [this _] this)
+  (compute-parameters! [this {:keys [momentum-vals]} gradient-alpha offset gradient parameters]
+    (let [{:keys [alpha momentum nesterov steps coefficients epsilon weight-decay]} optimizer
+          datatype (dtype/get-datatype backend)
+          stream (compute-backend/get-stream)
+          [rows columns :as shape] (m/shape parameters)
+          triples (triples->native (repeat steps coefficients))]
+      (when-not (= 2 (count shape))
+        (throw (ex-info "Muon is for matrices" {:shape shape})))
+      (ensure-datatype datatype gradient parameters momentum-vals)
+      (select-device! stream)
+      (let [need (orthogonalize-workspace datatype 1 rows columns)
+            ;; kept, the smaller ones too: a recorded graph may still write to them
+            workspace (or (first (filter #(>= (long (dtype/ecount %)) need) @workspaces))
+                          (let [fresh (drv/allocate-device-buffer need :byte)]
+                            (swap! workspaces conj fresh)
+                            fresh))]
+        (call! "ct_muon_step" (:handle stream) (int (ffi/datatype->code datatype)) (double alpha) (double momentum)
+               (ffi/bool->int nesterov) (double weight-decay) (double gradient-alpha) triples (int steps) (double epsilon)
+               (->ptr (->buffer gradient)) (->ptr (->buffer parameters)) (->ptr (->buffer momentum-vals (long offset)))
+               (long 1) (long rows) (long columns) (->ptr workspace) (long (dtype/ecount workspace)))))))
+
+(defmethod create-optimizer [:hip :muon]
+  [backend optimizer]
+  (->HipMuon backend (merge {:alpha 0.02 :momentum 0.95 :nesterov true :steps 5 :coefficients [3.4445 -4.7750 2.0315]
+                             :epsilon 1e-7 :weight-decay 0.0}
+                            optimizer)
+             (atom [])))

@@ -182,6 +182,9 @@ PROTOTYPES = {
     "ct_clip_gradients": [_P, _P, _P, _P, _L, _D, _P, _I],
     "ct_adam_step": [_P, _I, _D, _D, _D, _D, _D, _D, _D, _P, _P, _P, _P, _L],
     "ct_adadelta_step": [_P, _I, _D, _D, _P, _P, _D, _P, _P, _L],
+    "ct_orthogonalize_workspace": [_L, _L, _L, _I, C.POINTER(C.c_int64)],
+    "ct_orthogonalize": [_P, _P, _L, _L, _D, _P, _L, _L, _D, _L, _L, _L, _P, _I, _D, _P, _L, _I],
+    "ct_muon_step": [_P, _I, _D, _D, _I, _D, _D, _P, _I, _D, _P, _P, _P, _L, _L, _L, _P, _L],
 }
 STRING_FUNCTIONS = ("ct_last_error", "ct_last_kernel")
 

@@ -1,0 +1,761 @@
+// ops_ortho.hip -- matrices made orthogonal by Newton-Schulz products (ct_orthogonalize) and the optimizer step that is made of
+// it (ct_muon_step).
+//
+// With X = G / (|G| + epsilon), |G| the root of the sum of all squares, each step takes
+//   A = X X^T,   B = a I + b A + c A A,   X = B X
+// on the side of the matrix that is shorter (X^T X, and X B, of a tall one).  A step maps every singular value s of X to
+// s (a + b s^2 + c s^4) and leaves the singular vectors, so after a few of them all that are not tiny are near one.
+//
+// What bounds it: the products.  A and A A are symmetric: tiles below the diagonal are computed and stored twice.  Nothing is
+// done between the products: a I + b A + c A A is formed from the sums as they are stored, and a product stores its results as
+// the next one reads them.
+//
+// Float.  The singular values have a bound that the coefficients give, 1 at first and the largest s (a + b s^2 + c s^4) below the
+// last bound then, and no element of a matrix is larger than its largest singular value.  So the products are those of
+// pair_tile.h, two halves to a float, with scales from these bounds, and matrices lie in pieces between them: X by rows and by
+// columns, for one product's sums run along the rows and the other's along the columns.
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "double_tile.h"
+#include "pair_tile.h"
+#include "rows.h"
+
+using namespace cthip;
+
+namespace {
+
+// Consecutive units of work on one die: neighbouring tiles share operands in its L2.
+__device__ __forceinline__ uint32_t unit_of_block(uint32_t b, uint32_t units) {
+  const uint32_t per_die = (units + kXcds - 1) / kXcds;
+  return (b % kXcds) * per_die + b / kXcds;
+}
+
+// Tiles of one product in bands of kBand rows, column after column; of a symmetric one those at and below the diagonal, row
+// after row.
+constexpr uint32_t kBand = 8;
+
+struct TileOrder {
+  uint32_t units, tiles, m_tiles, n_tiles;   // tiles of a matrix; units: of all of them
+  FastDiv tiles_fd, band_fd;
+};
+
+struct TilePlace {
+  uint32_t matrix, m_tile, n_tile;
+};
+
+template <bool kSymmetric>
+__device__ __forceinline__ bool place_of(const TileOrder& o, TilePlace* p) {
+  const uint32_t unit = unit_of_block(blockIdx.x, o.units);
+  if (unit >= o.units) return false;
+  uint32_t tile, band, rest;
+  o.tiles_fd.divmod(unit, p->matrix, tile);
+  if constexpr (kSymmetric) {
+    uint32_t i = (uint32_t)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);   // may be one off
+    if (i * (i + 1) / 2 > tile) --i;
+    if ((i + 1) * (i + 2) / 2 <= tile) ++i;
+    p->m_tile = i;
+    p->n_tile = tile - i * (i + 1) / 2;
+  } else {
+    o.band_fd.divmod(tile, band, rest);
+    const uint32_t rows = min(kBand, o.m_tiles - band * kBand);
+    p->n_tile = rest / rows;
+    p->m_tile = band * kBand + rest - p->n_tile * rows;
+  }
+  return true;
+}
+
+enum Product { kGram, kSquare, kUpdate, kLast };
+constexpr bool is_symmetric(Product p) { return p == kGram || p == kSquare; }
+
+// ------------------------------------------------------------------ the norm, and the matrix divided by it
+
+// What a step begins with: of ct_orthogonalize a matrix x; of ct_muon_step the momentum x, which takes up the gradient.
+struct StartArgs {
+  const void* x;
+  const void* gradient;      // of a step, else null
+  void* momentum;            // x itself, of a step
+  double* partial;           // [matrix][kParts]
+  int64_t ld, stride;
+  uint32_t rows, columns;
+  double gradient_alpha, decay, epsilon;   // decay: of the momentum
+  bool nesterov;
+};
+
+constexpr uint32_t kParts = 256;
+
+// What is made orthogonal: the matrix, the momentum, or what it will be after another such gradient.
+template <class T>
+__device__ __forceinline__ T start_value(const StartArgs& a, int64_t at) {
+  const T x = static_cast<const T*>(a.x)[at];
+  if (!a.gradient || !a.nesterov) return x;
+  return (T)a.gradient_alpha * static_cast<const T*>(a.gradient)[at] + (T)a.decay * x;
+}
+
+__device__ __forceinline__ double sum_of_block(double x, double* lds) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) x += __shfl_down(x, d);
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// The sums of squares of parts of a matrix, in double; of a step, the momentum before them.  One read of what there is, a write of the
+// momentum: bound by memory.
+template <class T>
+__global__ void __launch_bounds__(256) start_norm_kernel(const StartArgs a, uint32_t parts, uint64_t each, bool dense) {
+  __shared__ double lds[4];
+  const int64_t base = (int64_t)blockIdx.y * a.stride;
+  const uint64_t cells = (uint64_t)a.rows * a.columns, first = blockIdx.x * each, end = min(first + each, cells);
+  double sum = 0.0;
+  for (uint64_t i0 = first + threadIdx.x; i0 < end; i0 += 4 * 256) {
+    T x[4], g[4];
+    int64_t at[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t i = min(i0 + e * 256, end - 1);
+      at[e] = base + (dense ? (int64_t)i : (int64_t)(i / a.columns) * a.ld + (int64_t)(i % a.columns));
+      x[e] = static_cast<const T*>(a.x)[at[e]];
+      if (a.gradient) g[e] = static_cast<const T*>(a.gradient)[at[e]];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i0 + e * 256 >= end) continue;
+      if (a.gradient) {
+        const T step = (T)a.gradient_alpha * g[e];
+        x[e] = (T)a.decay * x[e] + step;
+        static_cast<T*>(a.momentum)[at[e]] = x[e];
+        if (a.nesterov) x[e] = step + (T)a.decay * x[e];
+      }
+      sum += (double)x[e] * (double)x[e];
+    }
+  }
+  const double total = sum_of_block(sum, lds);
+  if (threadIdx.x == 0) a.partial[(int64_t)blockIdx.y * kParts + blockIdx.x] = total;
+}
+
+__device__ __forceinline__ double inverse_norm(const StartArgs& a, uint32_t matrix, uint32_t parts, double* lds) {
+  const double x = threadIdx.x < parts ? a.partial[(int64_t)matrix * kParts + threadIdx.x] : 0.0;
+  return 1.0 / (sqrt(sum_of_block(x, lds)) + a.epsilon);
+}
+
+// 64 x 64 elements as pieces, by rows and by columns.  The scale is a power of two.
+__global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, uint32_t parts, double scale, char* by_rows, char* by_columns,
+                                                           int64_t stride_rows, int64_t stride_columns) {
+  __shared__ double lds[4];
+  __shared__ uint32_t cells[64][65];
+  const uint32_t matrix = blockIdx.z, row0 = blockIdx.y * 64, column0 = blockIdx.x * 64;
+  const double factor = inverse_norm(a, matrix, parts, lds) * scale;
+  const int64_t base = (int64_t)matrix * a.stride;
+  const uint32_t c = threadIdx.x % 64;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t r = i * 4 + threadIdx.x / 64;
+    float x = 0.f;
+    if (row0 + r < a.rows && column0 + c < a.columns)
+      x = (float)((double)start_value<float>(a, base + (int64_t)(row0 + r) * a.ld + column0 + c) * factor);
+    _Float16 hi, lo;
+    split_pair(x, &hi, &lo);
+    cells[r][c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+  }
+  __syncthreads();
+  // eight k of a row to a lane, both pieces: 64 rows of two runs
+  const uint32_t row_runs = (a.columns + kPairRun - 1) / kPairRun, column_runs = (a.rows + kPairRun - 1) / kPairRun;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t at = i * 256 + threadIdx.x, r = at / 8, k = at % 8 * 8, run = k / 32;
+    auto put = [&](char* to, uint32_t row, uint32_t rows, uint32_t run0, uint32_t runs, bool turned) {
+      if (row >= rows || run0 + run >= runs) return;
+      pair_u32x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = turned ? cells[k + 2 * e][r] : cells[r][k + 2 * e], y = turned ? cells[k + 2 * e + 1][r] : cells[r][k + 2 * e + 1];
+        hi[e] = (x & 0xffff) | y << 16;
+        lo[e] = x >> 16 | (y & 0xffff0000u);
+      }
+      char* p = to + ((int64_t)row * runs + run0 + run) * kPairRunBytes + k % 32 * 2;
+      *reinterpret_cast<pair_u32x4*>(p) = hi;
+      *reinterpret_cast<pair_u32x4*>(p + 64) = lo;
+    };
+    put(by_rows + matrix * stride_rows, row0 + r, a.rows, column0 / 32, row_runs, false);
+    put(by_columns + matrix * stride_columns, column0 + r, a.columns, row0 / 32, column_runs, true);
+  }
+}
+
+__global__ void __launch_bounds__(256) start_double_kernel(const StartArgs a, uint32_t parts, double* to, int64_t stride, FastDiv columns_fd,
+                                                           uint32_t cells) {
+  __shared__ double lds[4];
+  const double factor = inverse_norm(a, blockIdx.y, parts, lds);
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < cells; i += gridDim.x * 256) {
+    uint32_t row, column;
+    columns_fd.divmod(i, row, column);
+    to[blockIdx.y * stride + i] = start_value<double>(a, (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld + column) * factor;
+  }
+}
+
+// ------------------------------------------------------------------ float
+
+struct PairArgs {
+  const char *left, *right;           // pieces, k along the rows
+  int64_t left_stride, right_stride;  // between matrices, bytes
+  TileOrder order;
+  uint32_t m, n, runs;
+  float unscale;
+  // results as pieces, [m][n] and [n][m]; of a symmetric product only the first
+  char *by_rows, *by_columns;
+  int64_t rows_stride, columns_stride;
+  float scale;
+  // of kSquare: a I + b A + c (sums), A as it is on the left
+  float a, b, c, a_unscale;
+  // of kLast: out = alpha * (sums) + beta * out
+  float* out;
+  int64_t ldo, out_stride;
+  float alpha, beta;
+};
+
+template <int S> struct PairShape;
+template <> struct PairShape<64> { static constexpr int kM = 2, kN = 2; };
+template <> struct PairShape<128> { static constexpr int kM = 2, kN = 2; };
+template <> struct PairShape<256> { static constexpr int kM = 2, kN = 4; };
+
+template <int S, Product kProduct>
+__global__ void __launch_bounds__(64 * PairShape<S>::kM * PairShape<S>::kN, 2) pair_kernel(const PairArgs a) {
+  constexpr int WM = PairShape<S>::kM, WN = PairShape<S>::kN, MT = S / WM / 32, NT = S / WN / 32;
+  __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(S, S)];
+  TilePlace at;
+  if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
+  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const uint32_t row0 = at.m_tile * S, column0 = at.n_tile * S, row_bytes = a.runs * kPairRunBytes;
+  const char* left = a.left + at.matrix * a.left_stride;
+  pair_f32x16 sum[MT][NT];
+  pair_tile<S, S, WM, WN>(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
+                          a.n - 1 - column0, row_bytes, 0, a.runs, lds, tid, sum);
+  const uint32_t wave_m = row0 + wave / WN * (MT * 32) + 4 * (lane >> 5), wave_n = column0 + wave % WN * (NT * 32) + (lane & 31);
+  if constexpr (kProduct == kLast) {
+    float* out = a.out + at.matrix * a.out_stride;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const uint32_t n = wave_n + u * 32;
+      if (n >= a.n) continue;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t m = wave_m + t * 32 + 8 * (r / 4) + r % 4;
+          if (m >= a.m) continue;
+          float& cell = out[(int64_t)m * a.ldo + n];
+          const float value = a.alpha * (sum[t][u][r] * a.unscale);
+          cell = a.beta == 0.f ? value : value + a.beta * cell;
+        }
+    }
+  } else {
+    // k along the columns of these results, and along the rows
+    const uint32_t runs_n = (a.n + kPairRun - 1) / kPairRun, runs_m = (a.m + kPairRun - 1) / kPairRun;
+    char* by_rows = a.by_rows + at.matrix * a.rows_stride;
+    char* by_columns = is_symmetric(kProduct) ? by_rows : a.by_columns + at.matrix * a.columns_stride;
+    const bool diagonal = is_symmetric(kProduct) && at.m_tile == at.n_tile;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t n = wave_n + u * 32, m = wave_m + t * 32 + 8 * q;
+          const int64_t turned = ((int64_t)n * runs_m + m / 32) * kPairRunBytes + m % 32 * 2;   // (n, m .. m + 3)
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = sum[t][u][4 * q + e] * a.unscale;
+          if constexpr (kProduct == kSquare) {
+            if (n < a.n && m < runs_m * kPairRun) {
+              const f16x4 hi = *reinterpret_cast<const f16x4*>(left + turned), lo = *reinterpret_cast<const f16x4*>(left + turned + 64);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[e] = a.c * x[e] + a.b * (((float)hi[e] + (float)lo[e]) * a.a_unscale) + (m + e == n ? a.a : 0.f);
+            }
+          }
+          f16x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            _Float16 h, l;
+            split_pair(m + e < a.m && n < a.n ? x[e] * a.scale : 0.f, &h, &l);
+            hi[e] = h;
+            lo[e] = l;
+          }
+          if (n < a.n && m < runs_m * kPairRun) {
+            *reinterpret_cast<f16x4*>(by_columns + turned) = hi;
+            *reinterpret_cast<f16x4*>(by_columns + turned + 64) = lo;
+          }
+          if (!diagonal && n < runs_n * kPairRun) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (m + e >= a.m) continue;
+              char* p = by_rows + ((int64_t)(m + e) * runs_n + n / 32) * kPairRunBytes + n % 32 * 2;
+              *reinterpret_cast<_Float16*>(p) = hi[e];
+              *reinterpret_cast<_Float16*>(p + 64) = lo[e];
+            }
+          }
+        }
+  }
+}
+
+// ------------------------------------------------------------------ double
+
+// Matrices lie as they are given, wide ([m][n], m <= n) or tall ([n][m]).
+struct DoubleArgs {
+  const double* x;
+  const double* square;   // A, or B
+  double* out;
+  int64_t x_stride, square_stride, out_stride, ldo;
+  TileOrder order;
+  uint32_t m, n;          // rows and columns of the results
+  uint32_t depth, ldx;
+  double a, b, c, alpha, beta;
+};
+
+template <int S, Product kProduct, bool kTall>
+__global__ void __launch_bounds__(256, 2) ortho_double_kernel(const DoubleArgs a) {
+  using Row = DoubleRow<S>;
+  using Columns = DoubleColumns<S>;
+  TilePlace at;
+  if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
+  const uint32_t row0 = at.m_tile * S, column0 = at.n_tile * S;
+  const double* x = a.x + at.matrix * a.x_stride;
+  const double* square = a.square + at.matrix * a.square_stride;
+  double* out = a.out + at.matrix * a.out_stride;
+  auto row_of = [&](const double* p, uint32_t ld, uint32_t first, uint32_t rows) {
+    return Row{p + (int64_t)min(first + Row::row(), rows - 1) * ld, a.depth, true};
+  };
+  auto columns_of = [&](const double* p, uint32_t ld, uint32_t first, uint32_t columns) {
+    return Columns(p + first, ld, nullptr, 0, a.depth, a.depth, columns - first);
+  };
+  if constexpr (is_symmetric(kProduct)) {
+    auto store = [&](uint32_t r, uint32_t n, double sum) {
+      r += row0;
+      n += column0;
+      if (r >= a.m || n >= a.n || r < n) return;
+      if constexpr (kProduct == kSquare) sum = a.c * sum + a.b * square[(int64_t)r * a.m + n] + (r == n ? a.a : 0.0);
+      out[(int64_t)r * a.m + n] = sum;
+      out[(int64_t)n * a.m + r] = sum;
+    };
+    if constexpr (kProduct == kSquare) double_tile<S>(a.depth, row_of(square, a.m, row0, a.m), row_of(square, a.m, column0, a.n), store);
+    else if constexpr (kTall) double_tile<S>(a.depth, columns_of(x, a.ldx, row0, a.m), columns_of(x, a.ldx, column0, a.n), store);
+    else double_tile<S>(a.depth, row_of(x, a.ldx, row0, a.m), row_of(x, a.ldx, column0, a.n), store);
+  } else {
+    auto store = [&](uint32_t r, uint32_t n, double sum) {
+      if (row0 + r >= a.m || column0 + n >= a.n) return;
+      double& cell = out[(int64_t)(row0 + r) * a.ldo + column0 + n];
+      if constexpr (kProduct == kUpdate) cell = sum;
+      else cell = a.beta == 0.0 ? a.alpha * sum : a.alpha * sum + a.beta * cell;
+    };
+    if constexpr (kTall) double_tile<S>(a.depth, row_of(x, a.ldx, row0, a.m), row_of(square, a.depth, column0, a.n), store);
+    else double_tile<S>(a.depth, row_of(square, a.depth, row0, a.m), columns_of(x, a.ldx, column0, a.n), store);
+  }
+}
+
+// ------------------------------------------------------------------ the host's side
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t aligned(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
+
+constexpr int64_t kMostSide = int64_t(1) << 21, kMostCount = 65535, kMostStride = int64_t(1) << 40;
+constexpr int kMostSteps = 64;
+
+// Where the matrices between the products lie in the workspace: bytes of a matrix each.
+struct Layout {
+  int64_t m, n;                                  // the shorter side and the longer one
+  int64_t x, turned, square, partial, matrix;   // matrix: of all that belongs to one
+  Layout(int64_t rows, int64_t columns, int dtype) : m(std::min(rows, columns)), n(std::max(rows, columns)) {
+    if (dtype == CT_F32) {
+      x = aligned(m * ceil_div(n, kPairRun) * kPairRunBytes);
+      turned = aligned(n * ceil_div(m, kPairRun) * kPairRunBytes);
+      square = aligned(m * ceil_div(m, kPairRun) * kPairRunBytes);
+    } else {
+      x = turned = aligned(m * n * 8);
+      square = aligned(m * m * 8);
+    }
+    partial = kParts * 8;
+    matrix = (dtype == CT_F32 ? x : 0) + 2 * turned + 2 * square + partial;
+  }
+};
+
+// Matrices beyond this many cells take turns: by then each launch fills the chip.
+constexpr int64_t kCellsAtOnce = int64_t(1) << 26;
+
+TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) {
+  TileOrder o;
+  const int64_t mt = ceil_div(m, side), nt = ceil_div(n, side), tiles = symmetric ? mt * (mt + 1) / 2 : mt * nt;
+  o.m_tiles = (uint32_t)mt;
+  o.n_tiles = (uint32_t)nt;
+  o.tiles = (uint32_t)tiles;
+  o.units = (uint32_t)(count * tiles);
+  o.tiles_fd = FastDiv(o.tiles);
+  o.band_fd = FastDiv((uint32_t)(kBand * nt));
+  return o;
+}
+
+dim3 grid_of(const TileOrder& o) { return dim3((uint32_t)(ceil_div(o.units, kXcds) * kXcds)); }
+
+int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) {
+  const int64_t mt = ceil_div(m, side), nt = ceil_div(n, side);
+  return count * (symmetric ? mt * (mt + 1) / 2 : mt * nt);
+}
+
+constexpr int64_t kUnits = 256;
+
+int64_t pair_side(int64_t count, int64_t m, int64_t n, int64_t runs, bool symmetric) {
+  if (tiles_of(count, m, n, 256, symmetric) >= kUnits) return 256;
+  return tiles_of(count, m, n, 128, symmetric) >= kUnits ? 128 : 64;
+}
+
+template <Product kProduct>
+void launch_pair(hipStream_t s, PairArgs a, int64_t count) {
+  constexpr bool kSymmetric = is_symmetric(kProduct);
+  const int64_t side = pair_side(count, a.m, a.n, a.runs, kSymmetric);
+  a.order = order_of(count, a.m, a.n, side, kSymmetric);
+  if (side == 256) hipLaunchKernelGGL((pair_kernel<256, kProduct>), grid_of(a.order), dim3(512), 0, s, a);
+  else if (side == 128) hipLaunchKernelGGL((pair_kernel<128, kProduct>), grid_of(a.order), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((pair_kernel<64, kProduct>), grid_of(a.order), dim3(256), 0, s, a);
+}
+
+template <Product kProduct>
+void launch_double(hipStream_t s, DoubleArgs a, int64_t count, bool tall) {
+  constexpr bool kSymmetric = is_symmetric(kProduct);
+  const int64_t side = tiles_of(count, a.m, a.n, 64, kSymmetric) >= kUnits ? 64 : 32;
+  a.order = order_of(count, a.m, a.n, side, kSymmetric);
+  const dim3 grid = grid_of(a.order);
+  if (side == 64 && tall) hipLaunchKernelGGL((ortho_double_kernel<64, kProduct, true>), grid, dim3(256), 0, s, a);
+  else if (side == 64) hipLaunchKernelGGL((ortho_double_kernel<64, kProduct, false>), grid, dim3(256), 0, s, a);
+  else if (tall) hipLaunchKernelGGL((ortho_double_kernel<32, kProduct, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((ortho_double_kernel<32, kProduct, false>), grid, dim3(256), 0, s, a);
+}
+
+// The largest |a + b s + c s^2| for s of 0 to `most`, and the largest |v (a + b v^2 + c v^4)| for v of 0 to the root of it.
+double most_of_factor(double a, double b, double c, double most) {
+  double found = std::max(std::abs(a), std::abs(a + (b + c * most) * most));
+  const double turn = c != 0 ? -b / (2 * c) : -1.0;
+  if (turn > 0 && turn < most) found = std::max(found, std::abs(a + (b + c * turn) * turn));
+  return found;
+}
+double most_of_step(double a, double b, double c, double most) {
+  auto value = [&](double s) { return std::abs(std::sqrt(s) * (a + (b + c * s) * s)); };
+  double found = value(most);
+  // a + 3 b s + 5 c s^2 = 0
+  const double root = 9 * b * b - 20 * a * c;
+  if (c == 0) {
+    const double s = b != 0 ? -a / (3 * b) : -1.0;
+    if (s > 0 && s < most) found = std::max(found, value(s));
+  } else if (root >= 0) {
+    for (double sign : {-1.0, 1.0}) {
+      const double s = (-3 * b + sign * std::sqrt(root)) / (10 * c);
+      if (s > 0 && s < most) found = std::max(found, value(s));
+    }
+  }
+  return found;
+}
+
+// The power of two that takes `bound`, and what rounding adds, to 2^kPairTop at most.
+float scale_for(double bound) {
+  int exponent;
+  std::frexp(std::max(1.02 * bound, 0x1p-40), &exponent);   // 1.02 bound <= 2^exponent
+  return std::ldexp(1.f, kPairTop - exponent);
+}
+
+struct Request {
+  StartArgs start;
+  void* out;
+  int64_t ldo, out_stride;
+  double alpha, beta;
+  const double* coefficients;
+  int steps;
+  int64_t count, rows, columns;
+  void* workspace;
+  int64_t workspace_bytes;
+  int dtype;
+};
+
+constexpr double kMostValue = 0x1p40;
+
+int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once) {
+  const bool tall = r.rows > r.columns;
+  char* const base = static_cast<char*>(r.workspace);
+  char* const x = base;
+  char* turned[2] = {x + at_once * l.x, x + at_once * (l.x + l.turned)};
+  char* const gram = turned[1] + at_once * l.turned;
+  char* const factor = gram + at_once * l.square;
+  double* const partial = reinterpret_cast<double*>(factor + at_once * l.square);
+  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 2048));
+  const uint64_t each = (uint64_t)ceil_div(cells, parts);
+  for (int64_t first = 0; first < r.count; first += at_once) {
+    const int64_t count = std::min(at_once, r.count - first);
+    StartArgs start = r.start;
+    const int64_t offset = first * start.stride * 4;
+    start.x = static_cast<const char*>(start.x) + offset;
+    if (start.gradient) start.gradient = static_cast<const char*>(start.gradient) + offset;
+    if (start.momentum) start.momentum = static_cast<char*>(start.momentum) + offset;
+    start.partial = partial;
+    hipLaunchKernelGGL((start_norm_kernel<float>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
+                       start.ld == r.columns);
+    double most = 1.0;
+    float x_scale = scale_for(most);
+    hipLaunchKernelGGL(start_pieces_kernel, dim3((uint32_t)ceil_div(r.columns, 64), (uint32_t)ceil_div(r.rows, 64), (uint32_t)count), dim3(256), 0, s,
+                       start, (uint32_t)parts, (double)x_scale, tall ? turned[0] : x, tall ? x : turned[0], tall ? l.turned : l.x, tall ? l.x : l.turned);
+    for (int step = 0; step < r.steps; ++step) {
+      const double *k = r.coefficients + 3 * step, ca = k[0], cb = k[1], cc = k[2];
+      const double most_factor = most_of_factor(ca, cb, cc, most * most), next = most_of_step(ca, cb, cc, most * most);
+      const float a_scale = scale_for(most * most), b_scale = scale_for(most_factor), next_scale = scale_for(next);
+      PairArgs g{};
+      g.left = g.right = x;
+      g.left_stride = g.right_stride = l.x;
+      g.m = g.n = (uint32_t)l.m;
+      g.runs = (uint32_t)ceil_div(l.n, kPairRun);
+      g.unscale = 1.f / (x_scale * x_scale);
+      g.by_rows = gram;
+      g.rows_stride = l.square;
+      g.scale = a_scale;
+      launch_pair<kGram>(s, g, count);
+      g.left = g.right = gram;
+      g.left_stride = g.right_stride = l.square;
+      g.runs = (uint32_t)ceil_div(l.m, kPairRun);
+      g.unscale = 1.f / (a_scale * a_scale);
+      g.by_rows = factor;
+      g.scale = b_scale;
+      g.a = (float)ca;
+      g.b = (float)cb;
+      g.c = (float)cc;
+      g.a_unscale = 1.f / a_scale;
+      launch_pair<kSquare>(s, g, count);
+      const bool last = step + 1 == r.steps;
+      PairArgs u{};
+      u.left = factor;
+      u.left_stride = l.square;
+      u.right = turned[step & 1];
+      u.right_stride = l.turned;
+      u.m = (uint32_t)l.m;
+      u.n = (uint32_t)l.n;
+      u.runs = (uint32_t)ceil_div(l.m, kPairRun);
+      u.unscale = 1.f / (b_scale * x_scale);
+      if (!last) {
+        u.by_rows = x;
+        u.rows_stride = l.x;
+        u.by_columns = turned[(step + 1) & 1];
+        u.columns_stride = l.turned;
+        u.scale = next_scale;
+        launch_pair<kUpdate>(s, u, count);
+      } else {
+        if (tall) {   // the rows of the result are those of X^T
+          std::swap(u.left, u.right);
+          std::swap(u.left_stride, u.right_stride);
+          std::swap(u.m, u.n);
+        }
+        u.out = static_cast<float*>(r.out) + first * r.out_stride;
+        u.ldo = r.ldo;
+        u.out_stride = r.out_stride;
+        u.alpha = (float)r.alpha;
+        u.beta = (float)r.beta;
+        launch_pair<kLast>(s, u, count);
+      }
+      most = next;
+      x_scale = next_scale;
+    }
+  }
+  note_kernel("orthogonalize_pair");
+  return after_launch(s);
+}
+
+int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once) {
+  const bool tall = r.rows > r.columns;
+  char* const base = static_cast<char*>(r.workspace);
+  double* x[2] = {reinterpret_cast<double*>(base), reinterpret_cast<double*>(base + at_once * l.x)};
+  double* const gram = reinterpret_cast<double*>(base + 2 * at_once * l.x);
+  double* const factor = reinterpret_cast<double*>(base + 2 * at_once * l.x + at_once * l.square);
+  double* const partial = reinterpret_cast<double*>(base + 2 * at_once * (l.x + l.square));
+  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 2048));
+  const uint64_t each = (uint64_t)ceil_div(cells, parts);
+  for (int64_t first = 0; first < r.count; first += at_once) {
+    const int64_t count = std::min(at_once, r.count - first);
+    StartArgs start = r.start;
+    const int64_t offset = first * start.stride * 8;
+    start.x = static_cast<const char*>(start.x) + offset;
+    if (start.gradient) start.gradient = static_cast<const char*>(start.gradient) + offset;
+    if (start.momentum) start.momentum = static_cast<char*>(start.momentum) + offset;
+    start.partial = partial;
+    hipLaunchKernelGGL((start_norm_kernel<double>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
+                       start.ld == r.columns);
+    hipLaunchKernelGGL(start_double_kernel, dim3((uint32_t)std::min<int64_t>(ceil_div(cells, 256), 4096), (uint32_t)count), dim3(256), 0, s, start,
+                       (uint32_t)parts, x[0], l.x / 8, FastDiv((uint32_t)r.columns), (uint32_t)cells);
+    for (int step = 0; step < r.steps; ++step) {
+      const double* k = r.coefficients + 3 * step;
+      DoubleArgs g{};
+      g.x = x[step & 1];
+      g.x_stride = l.x / 8;
+      g.ldx = (uint32_t)r.columns;
+      g.square_stride = g.out_stride = l.square / 8;
+      g.m = g.n = (uint32_t)l.m;
+      g.out = gram;
+      g.square = gram;
+      g.depth = (uint32_t)l.n;
+      launch_double<kGram>(s, g, count, tall);
+      g.out = factor;
+      g.depth = (uint32_t)l.m;
+      g.a = k[0];
+      g.b = k[1];
+      g.c = k[2];
+      launch_double<kSquare>(s, g, count, false);
+      g.square = factor;
+      g.m = (uint32_t)r.rows;
+      g.n = (uint32_t)r.columns;
+      if (step + 1 < r.steps) {
+        g.out = x[(step + 1) & 1];
+        g.out_stride = l.x / 8;
+        g.ldo = r.columns;
+        launch_double<kUpdate>(s, g, count, tall);
+      } else {
+        g.out = static_cast<double*>(r.out) + first * r.out_stride;
+        g.out_stride = r.out_stride;
+        g.ldo = r.ldo;
+        g.alpha = r.alpha;
+        g.beta = r.beta;
+        launch_double<kLast>(s, g, count, tall);
+      }
+    }
+  }
+  note_kernel("orthogonalize_double");
+  return after_launch(s);
+}
+
+int check_extents(const char* name, int64_t count, int64_t rows, int64_t columns) {
+  CT_REQUIRE(count >= 0 && rows >= 0 && columns >= 0, "%s: negative extent", name);
+  CT_REQUIRE(rows <= kMostSide && columns <= kMostSide && count <= kMostCount, "%s: %lld matrices of %lld by %lld, at most %lld of %lld a side are taken",
+             name, (long long)count, (long long)rows, (long long)columns, (long long)kMostCount, (long long)kMostSide);
+  CT_REQUIRE(rows * columns < int64_t(1) << 31, "%s: a matrix of %lld by %lld, 2^31 - 1 elements are taken", name, (long long)rows, (long long)columns);
+  return CT_OK;
+}
+
+// What both entry points check, and the products.
+int run(const char* name, hipStream_t s, Request r) {
+  const int64_t size = dtype_size(r.dtype);
+  CT_REQUIRE(r.steps >= 1 && r.steps <= kMostSteps, "%s: %d steps, 1 to %d are taken", name, r.steps, kMostSteps);
+  CT_REQUIRE(r.coefficients, "%s: null coefficients", name);
+  CT_REQUIRE(r.start.epsilon >= 0, "%s: epsilon must not be negative", name);
+  double bound = 1.0;
+  for (int step = 0; step < r.steps; ++step) {
+    const double* k = r.coefficients + 3 * step;
+    CT_REQUIRE(std::isfinite(k[0]) && std::isfinite(k[1]) && std::isfinite(k[2]), "%s: coefficients must be finite", name);
+    const double factor = most_of_factor(k[0], k[1], k[2], bound * bound);
+    bound = most_of_step(k[0], k[1], k[2], bound * bound);
+    CT_REQUIRE(factor <= kMostValue && bound <= kMostValue, "%s: with these coefficients singular values grow beyond 2^40", name);
+  }
+  if (r.count == 0 || r.rows == 0 || r.columns == 0) return CT_OK;
+  const Layout l(r.rows, r.columns, r.dtype);
+  CT_REQUIRE(r.workspace && (reinterpret_cast<uintptr_t>(r.workspace) & 15) == 0, "%s: the workspace must be a buffer, aligned to 16 bytes", name);
+  CT_REQUIRE(r.workspace_bytes >= l.matrix, "%s: a workspace of %lld bytes, a matrix takes %lld", name, (long long)r.workspace_bytes, (long long)l.matrix);
+  // a launch of 2^32 lanes or more is refused, and a block has up to 512
+  const int64_t most = (int64_t(1) << 22) / tiles_of(1, r.rows, r.columns, 32, false);
+  const int64_t at_once = std::min({r.count, r.workspace_bytes / l.matrix, std::max<int64_t>(1, most)});
+  const Run work{r.workspace, r.workspace_bytes};
+  auto run_of = [&](const void* p, int64_t ld, int64_t stride) { return Run{p, ((r.count - 1) * stride + (r.rows - 1) * ld + r.columns) * size}; };
+  const Run x = run_of(r.start.x, r.start.ld, r.start.stride), gradient = run_of(r.start.gradient, r.start.ld, r.start.stride);
+  const Run out = run_of(r.out, r.ldo, r.out_stride);
+  CT_REQUIRE(!runs_meet(work, x) && !runs_meet(work, gradient) && !runs_meet(work, out), "%s: the workspace overlaps an operand", name);
+  return r.dtype == CT_F32 ? run_float(s, r, l, at_once) : run_double(s, r, l, at_once);
+}
+
+}  // namespace
+
+#define CT_ORTHO_FLOATING(name) CT_REQUIRE(dtype == CT_F32 || dtype == CT_F64, name ": datatype must be float or double")
+
+extern "C" {
+
+int ct_orthogonalize_workspace(int64_t count, int64_t rows, int64_t columns, int dtype, int64_t* bytes) {
+  CT_ORTHO_FLOATING("ct_orthogonalize_workspace");
+  CT_REQUIRE(bytes, "ct_orthogonalize_workspace: null result");
+  CT_REQUIRE(count >= 0 && rows >= 0 && columns >= 0 && rows <= kMostSide && columns <= kMostSide && rows * columns < int64_t(1) << 31,
+             "ct_orthogonalize_workspace: bad extent");
+  *bytes = 0;
+  if (count == 0 || rows == 0 || columns == 0) return CT_OK;
+  *bytes = std::min(count, std::max<int64_t>(1, kCellsAtOnce / (rows * columns))) * Layout(rows, columns, dtype).matrix;
+  return CT_OK;
+}
+
+int ct_orthogonalize(void* stream, void* output, int64_t output_colstride, int64_t output_stride, double alpha, const void* input,
+                     int64_t input_colstride, int64_t input_stride, double beta, int64_t count, int64_t rows, int64_t columns,
+                     const double* coefficients, int steps, double epsilon, void* workspace, int64_t workspace_bytes, int dtype) {
+  CT_ORTHO_FLOATING("ct_orthogonalize");
+  if (int rc = check_extents("ct_orthogonalize", count, rows, columns)) return rc;
+  if (count > 0 && rows > 0 && columns > 0) {
+    CT_REQUIRE(output && input, "ct_orthogonalize: null buffer");
+    CT_REQUIRE(output_colstride >= columns && input_colstride >= columns, "ct_orthogonalize: a column stride below the row's length");
+    CT_REQUIRE(std::max({output_colstride, input_colstride, output_stride, input_stride}) <= kMostStride, "ct_orthogonalize: a stride beyond 2^40");
+    CT_REQUIRE(count == 1 || input_stride >= 0, "ct_orthogonalize: negative stride of matrices");
+    CT_REQUIRE(count == 1 || output_stride >= (rows - 1) * output_colstride + columns, "ct_orthogonalize: results overlap one another");
+    const int64_t size = dtype_size(dtype);
+    const bool in_place = output == input && output_colstride == input_colstride && (count == 1 || output_stride == input_stride);
+    CT_REQUIRE(in_place || !runs_meet({output, ((count - 1) * output_stride + (rows - 1) * output_colstride + columns) * size},
+                                      {input, ((count - 1) * input_stride + (rows - 1) * input_colstride + columns) * size}),
+               "ct_orthogonalize: output overlaps the input");
+  }
+  Request r{};
+  r.start.x = input;
+  r.start.ld = input_colstride;
+  r.start.stride = count > 1 ? input_stride : 0;
+  r.start.rows = (uint32_t)rows;
+  r.start.columns = (uint32_t)columns;
+  r.start.epsilon = epsilon;
+  r.out = output;
+  r.ldo = output_colstride;
+  r.out_stride = count > 1 ? output_stride : 0;
+  r.alpha = alpha;
+  r.beta = beta;
+  r.coefficients = coefficients;
+  r.steps = steps;
+  r.count = count;
+  r.rows = rows;
+  r.columns = columns;
+  r.workspace = workspace;
+  r.workspace_bytes = workspace_bytes;
+  r.dtype = dtype;
+  return run("ct_orthogonalize", static_cast<hipStream_t>(stream), r);
+}
+
+int ct_muon_step(void* stream, int dtype, double alpha, double momentum, int nesterov, double weight_decay, double gradient_alpha,
+                 const double* coefficients, int steps, double epsilon, const void* gradient, void* parameters, void* momentum_vals,
+                 int64_t count, int64_t rows, int64_t columns, void* workspace, int64_t workspace_bytes) {
+  CT_ORTHO_FLOATING("ct_muon_step");
+  if (int rc = check_extents("ct_muon_step", count, rows, columns)) return rc;
+  if (count > 0 && rows > 0 && columns > 0) {
+    CT_REQUIRE(gradient && parameters && momentum_vals, "ct_muon_step: null buffer");
+    const int64_t bytes = count * rows * columns * dtype_size(dtype);
+    CT_REQUIRE(!runs_meet({gradient, bytes}, {parameters, bytes}) && !runs_meet({gradient, bytes}, {momentum_vals, bytes}) &&
+                   !runs_meet({parameters, bytes}, {momentum_vals, bytes}),
+               "ct_muon_step: the gradient, the parameters and the momentum overlap");
+  }
+  Request r{};
+  r.start.x = momentum_vals;
+  r.start.gradient = gradient;
+  r.start.momentum = momentum_vals;
+  r.start.ld = columns;
+  r.start.stride = rows * columns;
+  r.start.rows = (uint32_t)rows;
+  r.start.columns = (uint32_t)columns;
+  r.start.gradient_alpha = gradient_alpha;
+  r.start.decay = momentum;
+  r.start.epsilon = epsilon;
+  r.start.nesterov = nesterov != 0;
+  r.out = parameters;
+  r.ldo = columns;
+  r.out_stride = rows * columns;
+  r.alpha = columns > 0 ? -alpha * std::sqrt(std::max(1.0, (double)rows / (double)columns)) : 0.0;
+  r.beta = 1.0 - alpha * weight_decay;
+  r.coefficients = coefficients;
+  r.steps = steps;
+  r.count = count;
+  r.rows = rows;
+  r.columns = columns;
+  r.workspace = workspace;
+  r.workspace_bytes = workspace_bytes;
+  r.dtype = dtype;
+  return run("ct_muon_step", static_cast<hipStream_t>(stream), r);
+}
+
+}  // extern "C"

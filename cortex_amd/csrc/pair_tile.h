@@ -1,0 +1,109 @@
+// pair_tile.h -- products of matrices with bounded elements on the half-precision matrix cores, two pieces to a float.
+//
+// v_mfma_f32_32x32x16_f16 takes as long as its bfloat16 form, and a half has eleven significant bits in place of eight: of a
+// float x, hi = x rounded to a half and lo = x - hi rounded to a half leave at most 2^-23 of the power of two below x, the last
+// of the float's bits, and
+//   a * b = hi hi + (hi lo + lo hi) + lo lo
+// without its last term (at most 2^-22 of the product, 2^-24.6 in the root mean square, of either sign) is three products where
+// three bfloat16 pieces take six.  What a half lacks is range, 2^-24 to 2^16, so this is for matrices whose elements have a known
+// bound: they are multiplied by a power of two that takes the bound to 2^14 at most, and what is below the least half is then
+// 2^-39 of the bound.  Sums are held in float.
+//
+// A matrix of pieces is stored in rows of runs of 32 k, 128 bytes to a run: the 32 leading pieces, then the 32 others.  Beyond its
+// columns a row is zeros up to a whole run.
+#pragma once
+
+#include "common.h"
+
+namespace cthip {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float pair_f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t pair_u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kPairRun = 32, kPairRunBytes = 128;
+// 2^kPairTop is the most that a bound is taken to.
+constexpr int kPairTop = 14;
+
+__device__ __forceinline__ void split_pair(float x, _Float16* hi, _Float16* lo) {
+  *hi = (_Float16)x;
+  *lo = (_Float16)(x - (float)*hi);
+}
+
+constexpr int pair_tile_lds(int bm, int bn) { return 2 * (bm + bn) * kPairRunBytes; }
+
+// The sums of runs first .. first + runs - 1 (of k) of BM rows of `a` with BN rows of `b`, over WM x WN waves of 64 lanes: a lane's
+// results of 32 x 32 cells, [.][.][r] row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.  Rows beyond the last ones repeat them.  All
+// of a block's waves call it, each group of them with an LDS of its own and as many runs.
+//
+// Chunks of 16 bytes of a row are permuted by the row's number, so that eight rows' reads of one chunk cover the banks once.
+template <int BM, int BN, int WM, int WN, int MT = BM / WM / 32, int NT = BN / WN / 32>
+__device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const char* b, uint32_t last_b, uint32_t row_bytes, uint32_t first,
+                                          uint32_t runs, char* lds, uint32_t tid, pair_f32x16 (&sum)[MT][NT]) {
+  constexpr int T = 64 * WM * WN, UA = BM * 8 / T, UB = BN * 8 / T, U = UA + UB, kBuffer = (BM + BN) * kPairRunBytes;
+  static_assert(UA * T == BM * 8 && UB * T == BN * 8 && T % 64 == 0, "lanes share the tiles evenly");
+  const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t wave_m = wave / WN * (MT * 32), wave_n = wave % WN * (NT * 32), row = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[t][u][r] = 0.f;
+  if (runs == 0) return;
+  uint32_t offset[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t r = min(((i < UA ? i : i - UA) * T + tid) / 8, i < UA ? last_a : last_b);
+    offset[i] = r * row_bytes + tid % 8 * 16;
+  }
+  const uint32_t put = tid / 8 * kPairRunBytes + ((tid ^ tid / 8) & 7) * 16;
+  pair_u32x4 raw[U];
+  auto load = [&](uint32_t run) {
+    const int64_t at = (int64_t)(first + min(run, runs - 1)) * kPairRunBytes;
+#pragma unroll
+    for (int i = 0; i < U; ++i) raw[i] = *reinterpret_cast<const pair_u32x4*>((i < UA ? a : b) + at + offset[i]);
+  };
+  auto stage = [&](uint32_t buffer) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      *reinterpret_cast<pair_u32x4*>(lds + buffer * kBuffer + (i < UA ? 0 : BM * kPairRunBytes) + (i < UA ? i : i - UA) * (T / 8 * kPairRunBytes) + put) = raw[i];
+  };
+  // piece p of 16 k of a run, of 32 rows
+  auto fetch = [&](uint32_t buffer, uint32_t base, uint32_t r, int part, int p) {
+    const uint32_t chunk = p * 4 + part * 2 + half;
+    return *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + base + r * kPairRunBytes + ((chunk ^ r) & 7) * 16);
+  };
+  auto multiply = [&](uint32_t buffer, int part) {
+    f16x8 left[MT][2], right[NT][2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) right[u][p] = fetch(buffer, BM * kPairRunBytes, wave_n + u * 32 + row, part, p);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) left[t][p] = fetch(buffer, 0, wave_m + t * 32 + row, part, p);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)   // the smaller products first
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+          sum[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[t][i == 0], right[u][i == 1], sum[t][u], 0, 0, 0);
+  };
+  load(0);
+  stage(0);
+  load(1);
+  __syncthreads();
+  for (uint32_t run = 0; run < runs; ++run) {
+    const uint32_t buffer = run & 1;
+    multiply(buffer, 0);
+    stage(buffer ^ 1);
+    load(run + 2);
+    multiply(buffer, 1);
+    __syncthreads();
+  }
+}
+
+}  // namespace cthip

@@ -580,6 +580,26 @@ class HipStream:
                   grad_accum.ptr, dx_accum.ptr, float(gradient_alpha), gradient.ptr, parameters.ptr, int(n))
 
 
+    # -- matrices made orthogonal; no counterpart in the reference -----------
+    def orthogonalize_workspace(self, count, rows, columns, datatype) -> int:
+        need = C.c_int64()
+        capi.call("ct_orthogonalize_workspace", int(count), int(rows), int(columns), capi.DTYPE_CODES[datatype], C.byref(need))
+        return need.value
+
+    def orthogonalize(self, output, output_colstride, output_stride, alpha, input, input_colstride, input_stride, beta, count, rows, columns,
+                      coefficients, epsilon, workspace) -> None:
+        """``coefficients`` are bytes of three doubles to a step."""
+        capi.call("ct_orthogonalize", self.handle, output.ptr, int(output_colstride), int(output_stride), float(alpha), input.ptr,
+                  int(input_colstride), int(input_stride), float(beta), int(count), int(rows), int(columns), coefficients, len(coefficients) // 24,
+                  float(epsilon), workspace.ptr, workspace.nbytes, capi.DTYPE_CODES[output.datatype])
+
+    def muon_step(self, alpha, momentum, nesterov, weight_decay, gradient_alpha, coefficients, epsilon, gradient, parameters, momentum_vals,
+                  count, rows, columns, workspace) -> None:
+        capi.call("ct_muon_step", self.handle, capi.DTYPE_CODES[gradient.datatype], float(alpha), float(momentum), int(bool(nesterov)),
+                  float(weight_decay), float(gradient_alpha), coefficients, len(coefficients) // 24, float(epsilon), gradient.ptr, parameters.ptr,
+                  momentum_vals.ptr, int(count), int(rows), int(columns), workspace.ptr, workspace.nbytes)
+
+
 class HipDevice:
     def __init__(self, driver: "HipDriver", index: int):
         self.driver = driver

@@ -7,7 +7,9 @@ called once per batch, ``compute_parameters`` once per parameter buffer with
 the running ``offset`` of that buffer inside the flat optimizer state
 (``src/cortex/nn/compute_binding.clj:817-854``).  The Adam and Adadelta steps
 are one fused kernel each on the backend's stream; SGD is, as in the reference,
-four calls of the tensor API.
+four calls of the tensor API.  Muon, which the reference has not, is one call of
+products between which nothing is done; it makes the momentum of a matrix
+orthogonal (:func:`orthogonalize`).
 """
 from __future__ import annotations
 
@@ -16,6 +18,10 @@ import dataclasses
 
 from . import capi
 from . import dimensions as dims
+
+# Of a step of :func:`orthogonalize`: odd polynomials of fifth degree whose slope at zero is large, so that small singular values
+# grow soonest; what is above them ends between 0.7 and 1.2.
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 def adam(**kwargs) -> dict:
@@ -35,6 +41,15 @@ def adadelta(**kwargs) -> dict:
 def sgd(**kwargs) -> dict:
     """Default SGD description (``sgd.clj:74-80``)."""
     out = {"type": "sgd", "learning-rate": 0.001, "momentum": 0.9}
+    out.update(kwargs)
+    return out
+
+
+def muon(**kwargs) -> dict:
+    """Default Muon description: momentum whose matrices are made orthogonal before they are taken off the parameters (:class:`Muon`).
+    No counterpart in the reference."""
+    out = {"type": "muon", "alpha": 0.02, "momentum": 0.95, "nesterov": True, "steps": 5, "coefficients": NEWTON_SCHULZ_COEFFICIENTS,
+           "epsilon": 1e-7, "weight-decay": 0.0}
     out.update(kwargs)
     return out
 
@@ -152,6 +167,116 @@ class SGD:
             ct.binary_op(params, 1.0, params, 1.0, dx, "+")
 
 
+def _matrices(name: str, what: str, x):
+    """(matrices, rows, columns, distance of rows, distance of matrices) of a tensor of one matrix or of several."""
+    if not hasattr(x, "buffer"):
+        raise ValueError(f"{name}: {what} must be a tensor, whose shape says what its matrices are")
+    shape, strides = x.dimensions["shape"], x.dimensions["strides"]
+    if not 2 <= len(shape) <= 3 or not dims.direct_shape(shape):
+        raise ValueError(f"{name}: {what} must be a matrix or matrices, got the shape {list(x.shape())}")
+    shape, strides = [int(n) for n in shape], [int(n) for n in strides]
+    if len(shape) == 2:
+        shape, strides = [1, *shape], [0, *strides]
+    count, rows, columns = shape
+    if (columns > 1 and strides[2] != 1) or (rows > 1 and strides[1] < columns):
+        raise ValueError(f"{name}: the rows of {what} must be contiguous and apart from one another")
+    return count, rows, columns, max(strides[1], columns) if rows > 1 else columns, strides[0] if count > 1 else 0
+
+
+def _packed_matrices(name: str, what: str, x, shape):
+    found = _matrices(name, what, x)
+    if found[:3] != shape or (0 not in shape and (found[3] != shape[2] or (shape[0] > 1 and found[4] != shape[1] * shape[2]))):
+        raise ValueError(f"{name}: {what} must be dense and of shape {list(shape)}, got {list(x.shape())}")
+    return x.buffer
+
+
+def _steps_of(coefficients, steps: int) -> bytes:
+    """Three doubles to a step: of one triple for all steps, or of one to each."""
+    triples = [tuple(map(float, c)) for c in coefficients] if hasattr(coefficients[0], "__len__") else [tuple(map(float, coefficients))] * int(steps)
+    if len(triples) != int(steps) or any(len(c) != 3 for c in triples):
+        raise ValueError(f"coefficients: three numbers, or three to each of {steps} steps")
+    return array.array("d", [x for c in triples for x in c]).tobytes()
+
+
+def orthogonalize_workspace(backend: Backend, input):
+    """A buffer for :func:`orthogonalize` of such a tensor, as large as makes all of its launches fill the chip.  Calls that may
+    overlap in time (on two streams, or of two recorded graphs) need one each; its owner releases it."""
+    _ensure_datatype(backend.datatype, _buffer(input))
+    need = backend.stream.orthogonalize_workspace(*_matrices("orthogonalize", "input", input)[:3], backend.datatype)
+    return backend.stream.get_device().allocate_device_buffer(max(1, need), "byte")
+
+
+def orthogonalize(backend: Backend, output, input, *, alpha=1.0, beta=0.0, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
+                  epsilon=1e-7, workspace=None) -> None:
+    """output = alpha * (input made orthogonal) + beta * output, of a matrix or of each of several ([count, rows, columns]):
+
+        X = input / (|input| + epsilon);   steps times, on the shorter side:  A = X X^T,  X = (a I + b A + c A A) X
+
+    with |.| the root of the sum of squares and (a, b, c) the coefficients, one triple or one to a step.  Rows are contiguous and any
+    distance apart; ``output`` may be ``input``.  ``workspace`` is of :func:`orthogonalize_workspace`; a smaller one serves as long as
+    one matrix fits.  Without it one is allocated and released, which waits for the stream.  No counterpart in the reference."""
+    name = "orthogonalize"
+    of_input, of_output = _matrices(name, "input", input), _matrices(name, "output", output)
+    if of_input[:3] != of_output[:3]:
+        raise ValueError(f"{name}: output {list(output.shape())} and input {list(input.shape())} differ")
+    _ensure_datatype(backend.datatype, output.buffer, input.buffer)
+    if output.buffer.device is not input.buffer.device:
+        raise ValueError(f"{name}: buffers are not all on the same device")
+    steps_of = _steps_of(coefficients, steps)
+    own = workspace is None
+    if own:
+        workspace = orthogonalize_workspace(backend, input)
+    try:
+        backend.stream.orthogonalize(output.buffer, *of_output[3:], alpha, input.buffer, *of_input[3:], beta, *of_input[:3], steps_of, epsilon,
+                                     _buffer(workspace))
+        if own:
+            backend.stream.sync()
+    finally:
+        if own:
+            workspace.release()
+
+
+@dataclasses.dataclass
+class Muon:
+    """Momentum for matrices, made orthogonal before it is taken off the parameters: of a matrix [rows, columns]
+
+        v = momentum * v + gradient-alpha * g;    u = gradient-alpha * g + momentum * v (nesterov), or v
+        p = (1 - alpha * weight-decay) * p - alpha * sqrt(max(1, rows / columns)) * orthogonalize(u)
+
+    in one call of the library.  Parameters are tensors [rows, columns], a row to an output, or [matrices, rows, columns], as those of
+    experts are; vectors are for another optimizer.  What lies between the products is kept from step to step, and what was too small
+    for a larger matrix is kept too: a recorded graph may still write to it."""
+    backend: Backend
+    optimizer: dict
+    _workspaces: list = dataclasses.field(default_factory=list)
+
+    def batch_update(self, optimizer_parameters=None) -> "Muon":
+        return self
+
+    def _workspace(self, need: int):
+        have = self._workspaces[-1].ecount() if self._workspaces else 0
+        if not self._workspaces or have < need:
+            self._workspaces.append(self.backend.stream.get_device().allocate_device_buffer(max(1, need, 2 * have), "byte"))
+        return self._workspaces[-1]
+
+    def compute_parameters(self, state: dict, gradient_alpha, offset: int, gradient, parameters) -> None:
+        name, o, stream = "muon", self.optimizer, self.backend.stream
+        shape = _matrices(name, "parameters", parameters)[:3]
+        p = _packed_matrices(name, "parameters", parameters, shape)
+        g = _packed_matrices(name, "gradient", gradient, shape) if hasattr(gradient, "buffer") else gradient
+        v = _buffer(state["momentum-vals"])
+        _ensure_datatype(self.backend.datatype, g, p, v)
+        n = shape[0] * shape[1] * shape[2]
+        if g.ecount() < n or p.ecount() < n:
+            raise ValueError(f"{name}: parameters of shape {list(shape)} and a gradient of {g.ecount()} elements")
+        if any(x.device is not p.device for x in (g, v)):
+            raise ValueError(f"{name}: buffers are not all on the same device")
+        steps_of = _steps_of(o["coefficients"], o["steps"])
+        workspace = self._workspace(stream.orthogonalize_workspace(*shape, self.backend.datatype))
+        stream.muon_step(o["alpha"], o["momentum"], o["nesterov"], o["weight-decay"], gradient_alpha, steps_of, o["epsilon"], g, p,
+                         v.sub_buffer(offset, n), *shape, workspace)
+
+
 def clip_gradients(backend: Backend, gradients, max_norm, norm_and_factor, outputs=None, in_place: bool = True) -> None:
     """The norm over all ``gradients`` (buffers or dense tensors of the backend's datatype) and their clipping, ahead of
     ``compute_parameters``: with norm = sqrt(sum of all squares),
@@ -209,4 +334,6 @@ def create_optimizer(backend: Backend, optimizer: dict):
         return Adadelta(backend, optimizer)
     if kind == "sgd":
         return SGD(backend, optimizer)
+    if kind == "muon":
+        return Muon(backend, optimizer)
     raise KeyError(f"No optimizer {kind!r} for backend {backend.type!r}")

@@ -692,6 +692,40 @@ int ct_adadelta_step(void* stream, int dtype, double decay, double epsilon, void
                      void* dx_sq_accum, double gradient_alpha, const void* gradient,
                      void* parameters, int64_t n);
 
+/* Matrices made orthogonal by Newton-Schulz products; no counterpart in the reference.  With X = input / (|input| + epsilon),
+ * |.| the root of the sum of all squares, each of `steps` steps takes, with its three of the coefficients (a HOST array
+ * [steps][3], read before the call returns),
+ *   A = X X^T,   X = (a I + b A + c A A) X       (X^T X, and from the right, where there are more rows than columns)
+ * and then output = alpha * X + beta * output.  A step maps a singular value s to s (a + b s^2 + c s^4) and leaves the
+ * singular vectors.
+ * `count` matrices [rows, columns], each of its own, row-major with a column stride, a stride from matrix to matrix.  output may
+ * be input itself, with the same strides; other overlaps are refused.
+ * workspace: device memory, aligned to 16 bytes, apart from all operands, that the call may write to until it has run on the
+ * stream; calls that overlap in time need one each.  ct_orthogonalize_workspace gives the bytes with which all launches fill the
+ * chip; with fewer, down to those that it gives for one matrix, the matrices take turns.
+ * Each side is 2^21 at most, a matrix below 2^31 elements, 1 <= steps <= 64; coefficients that let a singular value grow
+ * beyond 2^40 are refused.  The squares are summed in double.  An infinity or a NaN makes its matrix NaN, its matrix only.
+ * Float: sums are float ones of products of two halves to an element; what is below 2^-39 of the largest singular value that the
+ * coefficients allow is 0 there.  dtype is CT_F32 or CT_F64. */
+int ct_orthogonalize_workspace(int64_t count, int64_t rows, int64_t columns, int dtype, int64_t* bytes);
+int ct_orthogonalize(void* stream, void* output, int64_t output_colstride, int64_t output_stride,
+                     double alpha, const void* input, int64_t input_colstride, int64_t input_stride,
+                     double beta, int64_t count, int64_t rows, int64_t columns,
+                     const double* coefficients, int steps, double epsilon, void* workspace,
+                     int64_t workspace_bytes, int dtype);
+
+/* The optimizer step for matrices that is made of it:
+ *   momentum_vals = momentum * momentum_vals + gradient_alpha * gradient
+ *   u             = gradient_alpha * gradient + momentum * momentum_vals if nesterov, else momentum_vals
+ *   parameters    = (1 - alpha * weight_decay) * parameters
+ *                   - alpha * sqrt(max(1, rows / columns)) * (u made orthogonal as above)
+ * of `count` matrices [rows, columns], all packed.  The buffers do not overlap one another. */
+int ct_muon_step(void* stream, int dtype, double alpha, double momentum, int nesterov,
+                 double weight_decay, double gradient_alpha, const double* coefficients, int steps,
+                 double epsilon, const void* gradient, void* parameters, void* momentum_vals,
+                 int64_t count, int64_t rows, int64_t columns, void* workspace,
+                 int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif
