@@ -92,6 +92,28 @@
          (->ptr b) (long b-row-count) (long b-col-count) (long b-colstride) (when b-index (->ptr b-index))
          (->ptr offsets) (long n-groups) (long row-count) (double beta) (dtype-code c)))
 
+(defn gated-gemm!
+  "inner[i] = f(gate) * up with [gate up] = a[index[i]] * transpose(b_e), kept in pre unless that is nil; without offsets one
+  group of all rows.  Activations are :logistic, :tanh, :relu, :swish and :gelu."
+  [stream inner inner-colstride pre pre-colstride activation a a-row-count a-col-count a-colstride index b hidden b-colstride
+   b-stride offsets n-groups row-count]
+  (select-device! stream)
+  (call! "ct_gated_gemm" (:handle stream) (->ptr inner) (long inner-colstride) (when pre (->ptr pre)) (long pre-colstride)
+         (op-code ffi/gate-op->code activation) (->ptr a) (long a-row-count) (long a-col-count) (long a-colstride)
+         (when index (->ptr index)) (->ptr b) (long hidden) (long b-colstride) (long b-stride)
+         (when offsets (->ptr offsets)) (long n-groups) (long row-count) (dtype-code inner)))
+
+(defn gated-gemm-gradient!
+  "pre-gradient[i] = [d * up * f'(gate)  d * f(gate)], d = a[i] * b_e; and inner[i] = f(gate) * up unless that is nil."
+  [stream pre-gradient pre-gradient-colstride inner inner-colstride activation a a-col-count a-colstride b hidden b-colstride
+   b-stride pre pre-colstride offsets n-groups row-count]
+  (select-device! stream)
+  (call! "ct_gated_gemm_gradient" (:handle stream) (->ptr pre-gradient) (long pre-gradient-colstride)
+         (when inner (->ptr inner)) (long inner-colstride) (op-code ffi/gate-op->code activation)
+         (->ptr a) (long a-col-count) (long a-colstride) (->ptr b) (long hidden) (long b-colstride) (long b-stride)
+         (->ptr pre) (long pre-colstride) (when offsets (->ptr offsets)) (long n-groups) (long row-count)
+         (dtype-code pre-gradient)))
+
 (defn combine-experts!
   "output[t] = sum over j of weights[t, j] * rows[slots[t, j]]."
   [stream output output-colstride rows row-count rows-colstride weights slots n n-chosen width]

@@ -53,6 +53,7 @@
 (def ternary-op->code {:select 0})
 (def reduce-op->code {:max 0 :min 1 :sum 2 :mean 3 :magnitude 4 :magnitude-squared 5})
 (def activation-op->code {:logistic 0 :tanh 1 :relu 2})
+(def gate-op->code {:logistic 0 :tanh 1 :relu 2 :swish 3 :gelu 4})
 (def norm-kind->code {:none 0 :rms 1 :layer 2})
 (def pool-op->code {:max 0 :avg 1 :avg-exc-pad 2})
 (def copy-kind {:host->device 0 :device->host 1 :device->device 2})

@@ -1,8 +1,9 @@
-"""Residual blocks with experts: the operators that a feed-forward block of experts with norms around it is trained and
-served with, in the manner of the tensor API (:mod:`cortex_amd.tensor`), and a layer that runs them together
-(:class:`ExpertBlock`).  No counterpart in the reference.
+"""Residual feed-forward blocks, dense and with experts: the operators that such a block with norms around it is trained and
+served with, in the manner of the tensor API (:mod:`cortex_amd.tensor`), and layers that run them together
+(:class:`GatedBlock`, :class:`ExpertBlock`).  No counterpart in the reference.
 
     output, normalized = norm_residual(block's result, residual)    the norms after a block and before the next one
+    gated_gemm                                                      both first projections of rows, and f(gate) * up
     route_experts(normalized x router)                              the experts of each token, and rows in their order
     grouped_gemm                                                    products of rows with their expert's matrix
     combine_experts                                                 the weighted sum of a token's rows
@@ -389,6 +390,113 @@ def grouped_gemm_weights(C: Tensor, alpha, A: Tensor, B: Tensor, beta, offsets: 
     return C
 
 
+# ---------------------------------------------------------------- gated products
+
+GATES = tuple(capi.GATE_OPS)
+
+
+def _gate(name: str, activation) -> None:
+    if activation not in capi.GATE_OPS:
+        raise TensorError(f"{name}: unrecognized activation {activation!r}: one of {GATES}")
+
+
+def _weights(name: str, what: str, t: Tensor, offsets):
+    """As _matrices, of one matrix where there are no groups."""
+    if offsets is not None:
+        return _matrices(name, what, t)
+    if len(t.dimensions["shape"]) != 2:
+        raise TensorError(f"{name}: {what} must be a matrix where there are no offsets")
+    return (1, *_rows(name, what, t), 0)
+
+
+def gated_gemm(inner: Tensor, pre: Tensor, A: Tensor, B: Tensor, offsets: Tensor = None, index: Tensor = None, *,
+               activation: str = "swish") -> Tensor:
+    """inner[i] = f(gate) * up with [gate up] = A[index[i]] * transpose(B), B [2 * hidden, width] the gate's projection above the
+    other's; with ``offsets`` B is [groups, 2 * hidden, width] and a row's is that of its group, as in :func:`grouped_gemm`.  ``pre``
+    [rows, 2 * hidden] takes [gate up], which :func:`gated_gemm_gradient` needs; None where there is no backward pass.  ``activation`` is
+    one of "logistic", "tanh", "relu", "swish" and "gelu"."""
+    name = "gated-gemm"
+    _gate(name, activation)
+    grouped = offsets is not None
+    found = _operands("mmmgii" if grouped else "mmmmii", (inner, pre, A, B, offsets, index))
+    if found is not None:
+        rows, hidden, stride, pre_rows, pre_columns, pre_stride, a_rows, a_columns, a_stride = found[:9]
+        groups, b_rows, b_columns, b_row_stride, b_stride = found[9:14] if grouped else (1, *found[9:12], 0)
+        of_offsets, of_index = found[14:17] if grouped else None, found[-3:]
+        if ((b_rows, b_columns) == (2 * hidden, a_columns) and (pre is None or (pre_rows, pre_columns) == (rows, 2 * hidden)) and
+                (not grouped or of_offsets == (1, groups + 1, groups + 1)) and (of_index == (1, rows, rows) if index is not None else a_rows == rows)):
+            check_stream().gated_gemm(inner.buffer, stride, _buffer(pre), pre_stride, activation, A.buffer, a_rows, a_columns, a_stride,
+                                      _buffer(index), B.buffer, hidden, b_row_stride, b_stride, _buffer(offsets), groups, rows)
+            return inner
+    _needed(name, inner=inner, A=A, B=B)
+    _floating(name, inner, pre, A, B)
+    _indexes(name, inner, offsets=offsets, index=index)
+    rows, hidden, stride = _rows(name, "inner", inner)
+    a_rows, a_columns, a_stride = _rows(name, "A", A)
+    groups, b_rows, b_columns, b_row_stride, b_stride = _weights(name, "B", B, offsets)
+    if (b_rows, b_columns) != (2 * hidden, a_columns):
+        raise TensorError(f"{name}: {a_columns} columns of A, {b_rows} by {b_columns} of B and {hidden} of inner do not go together")
+    pre_stride = 0
+    if pre is not None:
+        pre_rows, pre_columns, pre_stride = _rows(name, "pre", pre)
+        if (pre_rows, pre_columns) != (rows, 2 * hidden):
+            raise TensorError(f"{name}: pre must be {rows} by {2 * hidden}, got {list(pre.shape())}")
+    if offsets is not None:
+        _packed(name, "offsets", offsets, [groups + 1])
+    if index is not None:
+        _packed(name, "index", index, [rows])
+    elif a_rows != rows:
+        raise TensorError(f"{name}: A has {a_rows} rows, inner {rows}")
+    check_stream().gated_gemm(inner.buffer, stride, _buffer(pre), pre_stride, activation, A.buffer, a_rows, a_columns, a_stride, _buffer(index),
+                              B.buffer, hidden, b_row_stride, b_stride, _buffer(offsets), groups, rows)
+    return inner
+
+
+def gated_gemm_gradient(pre_gradient: Tensor, inner: Tensor, output_gradient: Tensor, B: Tensor, pre: Tensor, offsets: Tensor = None, *,
+                        activation: str = "swish") -> Tensor:
+    """What the backward pass of a gated block begins with.  From the gradient of the rows inner[i] * transpose(B), B [width, hidden] the
+    projection back (or [groups, width, hidden]), with d = output-gradient[i] * B:
+
+        pre-gradient[i] = [d * up * f'(gate)   d * f(gate)],    [gate up] = pre[i]
+
+    and, unless it is None, inner[i] = f(gate) * up once more.  ``pre_gradient`` may be ``pre`` itself.  The gradients of the first
+    products' operands are products of ``pre_gradient`` (gemm, or grouped_gemm and grouped_gemm_weights)."""
+    name = "gated-gemm-gradient"
+    _gate(name, activation)
+    grouped = offsets is not None
+    found = _operands("mmmmgi" if grouped else "mmmmmi", (pre_gradient, inner, output_gradient, pre, B, offsets))
+    if found is not None:
+        rows, columns, stride, inner_rows, inner_columns, inner_stride, a_rows, width, a_stride, pre_rows, pre_columns, pre_stride = found[:12]
+        groups, b_rows, hidden, b_row_stride, b_stride = found[12:17] if grouped else (1, *found[12:15], 0)
+        if ((rows, columns) == (pre_rows, pre_columns) == (a_rows, 2 * hidden) and b_rows == width and
+                (inner is None or (inner_rows, inner_columns) == (rows, hidden)) and (not grouped or found[17:] == (1, groups + 1, groups + 1))):
+            check_stream().gated_gemm_gradient(pre_gradient.buffer, stride, _buffer(inner), inner_stride, activation, output_gradient.buffer, width,
+                                               a_stride, B.buffer, hidden, b_row_stride, b_stride, pre.buffer, pre_stride, _buffer(offsets), groups,
+                                               rows)
+            return pre_gradient
+    _needed(name, pre_gradient=pre_gradient, output_gradient=output_gradient, B=B, pre=pre)
+    _floating(name, pre_gradient, inner, output_gradient, B, pre)
+    _indexes(name, pre_gradient, offsets=offsets)
+    rows, columns, stride = _rows(name, "pre gradient", pre_gradient)
+    a_rows, width, a_stride = _rows(name, "output gradient", output_gradient)
+    pre_rows, pre_columns, pre_stride = _rows(name, "pre", pre)
+    groups, b_rows, hidden, b_row_stride, b_stride = _weights(name, "B", B, offsets)
+    if b_rows != width:
+        raise TensorError(f"{name}: {width} columns of the output's gradient and {b_rows} by {hidden} of B do not go together")
+    if (rows, columns) != (pre_rows, pre_columns) or (rows, columns) != (a_rows, 2 * hidden):
+        raise TensorError(f"{name}: pre and its gradient must be {a_rows} by {2 * hidden}, got {list(pre.shape())} and {list(pre_gradient.shape())}")
+    inner_stride = 0
+    if inner is not None:
+        inner_rows, inner_columns, inner_stride = _rows(name, "inner", inner)
+        if (inner_rows, inner_columns) != (rows, hidden):
+            raise TensorError(f"{name}: inner must be {rows} by {hidden}, got {list(inner.shape())}")
+    if offsets is not None:
+        _packed(name, "offsets", offsets, [groups + 1])
+    check_stream().gated_gemm_gradient(pre_gradient.buffer, stride, _buffer(inner), inner_stride, activation, output_gradient.buffer, width, a_stride,
+                                       B.buffer, hidden, b_row_stride, b_stride, pre.buffer, pre_stride, _buffer(offsets), groups, rows)
+    return pre_gradient
+
+
 # ---------------------------------------------------------------- a token's results
 
 def combine_experts(output: Tensor, rows: Tensor, weights: Tensor, slots: Tensor) -> Tensor:
@@ -461,7 +569,55 @@ def combine_experts_gradient(rows_gradient: Tensor, weights_gradient: Tensor, ou
                                             _buffer(rows), count, rows_stride, _buffer(weights), slots.buffer, n, n_chosen, width)
 
 
-# ---------------------------------------------------------------- the layer
+# ---------------------------------------------------------------- the layers
+
+def _norms(parameters, which):
+    return {k: v[which] for k, v in parameters.items() if k in _OF_COLUMNS + ("gate",) and v.get(which) is not None}
+
+
+class GatedBlock:
+    """A residual gated feed-forward block, as it stands between two others:
+
+        x = N_pre(residual)                             (what entered: norm_residual of the block before, or of this one)
+        y = second * (f(gate) * up),  [gate up] = first * x
+        output, normalized = norm_residual(y, residual)
+
+    in the manner of :class:`ExpertBlock`: ``parameters`` is a dict of {"buffer", "gradient"} tensors, "first" [2 * hidden, width] with the
+    gate's projection above the other's, "second" [width, hidden] and those of the norms.  Gradients are overwritten.  With ``training``
+    false there is no backward pass, and what it would need is not kept."""
+
+    def __init__(self, tokens: int, width: int, hidden: int, descriptor: dict = None, datatype: str = None, activation: str = "swish",
+                 training: bool = True):
+        _gate("gated-block", activation)
+        self.descriptor = descriptor or norm_descriptor()
+        self.activation = activation
+        new = lambda shape: ct.new_tensor(shape, datatype=datatype)
+        self.inner, self.combined = new([tokens, hidden]), new([tokens, width])
+        self.statistics, self.pre, self.combined_gradient = ((new([4, tokens]), new([tokens, 2 * hidden]), new([tokens, width])) if training
+                                                             else (None, None, None))
+
+    def forward(self, parameters: dict, x: Tensor, residual: Tensor, output: Tensor, normalized: Tensor):
+        gated_gemm(self.inner, self.pre, x, parameters["first"]["buffer"], activation=self.activation)
+        ct.gemm(self.combined, False, True, 1.0, self.inner, parameters["second"]["buffer"], 0.0)
+        return norm_residual(output, normalized, self.statistics, self.combined, residual, _norms(parameters, "buffer"), self.descriptor)
+
+    def backward(self, parameters: dict, x: Tensor, output: Tensor, x_gradient: Tensor, residual_gradient: Tensor,
+                 output_gradient: Tensor, normalized_gradient: Tensor):
+        """The gradients of x and of the residual and of every parameter that has one, from those of the results, once to a forward pass:
+        what that kept is overwritten.  A parameter whose "gradient" is None or absent is held as it is."""
+        if self.pre is None:
+            raise TensorError("gated-block: there is no backward pass of a block that is not for training")
+        first, second = (parameters[k].get("gradient") for k in ("first", "second"))
+        norm_residual_gradient(self.combined_gradient, residual_gradient, _norms(parameters, "gradient"), output_gradient,
+                               normalized_gradient, self.combined, output, self.statistics, _norms(parameters, "buffer"), self.descriptor)
+        if second is not None:
+            ct.gemm(second, True, False, 1.0, self.combined_gradient, self.inner, 0.0)
+        gated_gemm_gradient(self.pre, None, self.combined_gradient, parameters["second"]["buffer"], self.pre, activation=self.activation)
+        if first is not None:
+            ct.gemm(first, True, False, 1.0, self.pre, x, 0.0)
+        ct.gemm(x_gradient, False, False, 1.0, self.pre, parameters["first"]["buffer"], 0.0)
+        return x_gradient, residual_gradient
+
 
 class ExpertBlock:
     """A residual feed-forward block of experts, as it stands between two others:
@@ -472,12 +628,18 @@ class ExpertBlock:
 
     in the manner of :mod:`cortex_amd.nn_layers`: ``parameters`` is a dict of {"buffer", "gradient"} tensors, "router"
     [experts, width], "first" [experts, hidden, width], "second" [experts, width, hidden] and those of the norms
-    ("post-scale", "pre-scale", ..., "gate").  Gradients are overwritten, one block to a batch."""
+    ("post-scale", "pre-scale", ..., "gate").  Gradients are overwritten, one block to a batch.
+
+    With ``gated``, one of :data:`GATES`, the experts are gated: "first" is [experts, 2 * hidden, width], the gates' projection above the
+    others', and the inner rows are f(gate) * up in place of the relu; a backward pass then overwrites what the forward pass kept."""
 
     def __init__(self, tokens: int, width: int, hidden: int, n_experts: int, n_chosen: int, descriptor: dict = None,
-                 datatype: str = None, renormalize: bool = True):
+                 datatype: str = None, renormalize: bool = True, gated: str = None):
+        if gated is not None:
+            _gate("expert-block", gated)
         self.descriptor = descriptor or norm_descriptor()
         self.renormalize = renormalize
+        self.gated = gated
         rows = tokens * n_chosen
         new = lambda shape, kind=datatype: ct.new_tensor(shape, datatype=kind)
         self.logits, self.logits_gradient = new([tokens, n_experts]), new([tokens, n_experts])
@@ -485,23 +647,24 @@ class ExpertBlock:
         self.experts, self.slots = new([tokens, n_chosen], "int"), new([tokens, n_chosen], "int")
         self.offsets, self.tokens = new([n_experts + 1], "int"), new([rows], "int")
         # a row to each assignment, in order of experts
-        self.inner, self.inner_gradient = new([rows, hidden]), new([rows, hidden])
+        self.inner = new([rows, hidden])
+        self.pre, self.inner_gradient = (None, new([rows, hidden])) if gated is None else (new([rows, 2 * hidden]), None)
         self.outer, self.outer_gradient = new([rows, width]), new([rows, width])
         self.combined, self.combined_gradient = new([tokens, width]), new([tokens, width])
         self.statistics = new([4, tokens])
-
-    def _norms(self, parameters, which):
-        return {k: v[which] for k, v in parameters.items() if k in _OF_COLUMNS + ("gate",) and v.get(which) is not None}
 
     def forward(self, parameters: dict, x: Tensor, residual: Tensor, output: Tensor, normalized: Tensor):
         p = {k: v["buffer"] for k, v in parameters.items()}
         ct.gemm(self.logits, False, True, 1.0, x, p["router"], 0.0)
         route_experts(self.experts, self.weights, self.offsets, self.tokens, self.slots, self.logits, renormalize=self.renormalize)
-        grouped_gemm(self.inner, True, 1.0, x, p["first"], 0.0, self.offsets, index=self.tokens)
-        ct.binary_op(self.inner, 1.0, self.inner, 1.0, 0, "max")
+        if self.gated is not None:
+            gated_gemm(self.inner, self.pre, x, p["first"], self.offsets, self.tokens, activation=self.gated)
+        else:
+            grouped_gemm(self.inner, True, 1.0, x, p["first"], 0.0, self.offsets, index=self.tokens)
+            ct.binary_op(self.inner, 1.0, self.inner, 1.0, 0, "max")
         grouped_gemm(self.outer, True, 1.0, self.inner, p["second"], 0.0, self.offsets)
         combine_experts(self.combined, self.outer, self.weights, self.slots)
-        return norm_residual(output, normalized, self.statistics, self.combined, residual, self._norms(parameters, "buffer"),
+        return norm_residual(output, normalized, self.statistics, self.combined, residual, _norms(parameters, "buffer"),
                              self.descriptor)
 
     def backward(self, parameters: dict, x: Tensor, output: Tensor, x_gradient: Tensor, residual_gradient: Tensor,
@@ -510,19 +673,22 @@ class ExpertBlock:
         "gradient" is None or absent is held as it is: nothing is formed for it alone."""
         p = {k: v["buffer"] for k, v in parameters.items()}
         router, first, second = (parameters[k].get("gradient") for k in ("router", "first", "second"))
-        norm_residual_gradient(self.combined_gradient, residual_gradient, self._norms(parameters, "gradient"), output_gradient,
-                               normalized_gradient, self.combined, output, self.statistics, self._norms(parameters, "buffer"),
+        norm_residual_gradient(self.combined_gradient, residual_gradient, _norms(parameters, "gradient"), output_gradient,
+                               normalized_gradient, self.combined, output, self.statistics, _norms(parameters, "buffer"),
                                self.descriptor)
         combine_experts_gradient(self.outer_gradient, self.weights_gradient, self.combined_gradient, self.outer, self.weights,
                                  self.slots)
         if second is not None:
             grouped_gemm_weights(second, 1.0, self.outer_gradient, self.inner, 0.0, self.offsets)
-        grouped_gemm(self.inner_gradient, False, 1.0, self.outer_gradient, p["second"], 0.0, self.offsets)
-        ct.activation_gradient(self.inner_gradient, self.inner_gradient, self.inner, "relu")
+        if self.gated is not None:
+            inner_gradient = gated_gemm_gradient(self.pre, None, self.outer_gradient, p["second"], self.pre, self.offsets, activation=self.gated)
+        else:
+            inner_gradient = grouped_gemm(self.inner_gradient, False, 1.0, self.outer_gradient, p["second"], 0.0, self.offsets)
+            ct.activation_gradient(inner_gradient, inner_gradient, self.inner, "relu")
         if first is not None:
-            grouped_gemm_weights(first, 1.0, self.inner_gradient, x, 0.0, self.offsets, b_index=self.tokens)
+            grouped_gemm_weights(first, 1.0, inner_gradient, x, 0.0, self.offsets, b_index=self.tokens)
         # the gradient of x: of its rows among the experts, and of the router's
-        grouped_gemm(self.outer_gradient, False, 1.0, self.inner_gradient, p["first"], 0.0, self.offsets)
+        grouped_gemm(self.outer_gradient, False, 1.0, inner_gradient, p["first"], 0.0, self.offsets)
         combine_experts(x_gradient, self.outer_gradient, None, self.slots)
         route_experts_gradient(self.logits_gradient, self.weights_gradient, self.weights, self.experts, self.logits,
                                renormalize=self.renormalize)

@@ -33,6 +33,7 @@ ACTIVATION_OPS = {"logistic": 0, "tanh": 1, "relu": 2}
 DISTRIBUTIONS = {"gaussian": 0, "flat": 1}
 POOL_OPS = {"max": 0, "avg": 1, "avg-exc-pad": 2}
 NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
+GATE_OPS = {"logistic": 0, "tanh": 1, "relu": 2, "swish": 3, "gelu": 4}
 REDUCE_OPS = {"max": 0, "min": 1, "sum": 2, "mean": 3, "magnitude": 4, "magnitude-squared": 5}
 
 COPY_H2D, COPY_D2H, COPY_D2D = 0, 1, 2
@@ -177,6 +178,8 @@ PROTOTYPES = {
     "ct_route_experts_gradient": [_P, _P, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I],
     "ct_grouped_gemm": [_P, _P, _L, _I, _D, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _D, _I],
     "ct_grouped_gemm_weights": [_P, _P, _L, _L, _D, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _L, _L, _D, _I],
+    "ct_gated_gemm": [_P, _P, _L, _P, _L, _I, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _I],
+    "ct_gated_gemm_gradient": [_P, _P, _L, _P, _L, _I, _P, _L, _L, _P, _L, _L, _L, _P, _L, _P, _L, _L, _I],
     "ct_combine_experts": [_P, _P, _L, _P, _L, _L, _P, _P, _L, _L, _L, _I],
     "ct_combine_experts_gradient": [_P, _P, _L, _P, _P, _L, _P, _L, _L, _P, _P, _L, _L, _L, _I],
     "ct_clip_gradients": [_P, _P, _P, _P, _L, _D, _P, _I],

@@ -369,7 +369,8 @@ Entry g_entries[] = {
     CT_ENTRY(ct_batch_normalize_gradients_spatial), CT_ENTRY(ct_gemm), CT_ENTRY(ct_gemv), CT_ENTRY(ct_rand),
     CT_ENTRY(ct_dropout_bernoulli_mask), CT_ENTRY(ct_adam_step), CT_ENTRY(ct_adadelta_step), CT_ENTRY(ct_lrn_forward),
     CT_ENTRY(ct_lrn_backward), CT_ENTRY(ct_norm_residual), CT_ENTRY(ct_norm_residual_gradient), CT_ENTRY(ct_route_experts),
-    CT_ENTRY(ct_route_experts_gradient), CT_ENTRY(ct_grouped_gemm), CT_ENTRY(ct_grouped_gemm_weights), CT_ENTRY(ct_combine_experts),
+    CT_ENTRY(ct_route_experts_gradient), CT_ENTRY(ct_grouped_gemm), CT_ENTRY(ct_grouped_gemm_weights), CT_ENTRY(ct_gated_gemm),
+    CT_ENTRY(ct_gated_gemm_gradient), CT_ENTRY(ct_combine_experts),
     CT_ENTRY(ct_combine_experts_gradient), CT_ENTRY(ct_clip_gradients)};
 PyObject* g_index;     // name -> index of an entry whose address is known
 PyObject* g_library;   // the library that the addresses are of

@@ -551,6 +551,18 @@ class HipStream:
                   int(b_colstride), _ptr(b_index), offsets.ptr, int(n_groups), int(row_count), float(beta),
                   capi.DTYPE_CODES[c.datatype])
 
+    def gated_gemm(self, inner, inner_colstride, pre, pre_colstride, activation, a, a_row_count, a_col_count, a_colstride, index, b, hidden,
+                   b_colstride, b_stride, offsets, n_groups, row_count) -> None:
+        capi.call("ct_gated_gemm", self.handle, inner.ptr, int(inner_colstride), _ptr(pre), int(pre_colstride), capi.GATE_OPS[activation], a.ptr,
+                  int(a_row_count), int(a_col_count), int(a_colstride), _ptr(index), b.ptr, int(hidden), int(b_colstride), int(b_stride),
+                  _ptr(offsets), int(n_groups), int(row_count), capi.DTYPE_CODES[inner.datatype])
+
+    def gated_gemm_gradient(self, pre_gradient, pre_gradient_colstride, inner, inner_colstride, activation, a, a_col_count, a_colstride, b,
+                            hidden, b_colstride, b_stride, pre, pre_colstride, offsets, n_groups, row_count) -> None:
+        capi.call("ct_gated_gemm_gradient", self.handle, pre_gradient.ptr, int(pre_gradient_colstride), _ptr(inner), int(inner_colstride),
+                  capi.GATE_OPS[activation], a.ptr, int(a_col_count), int(a_colstride), b.ptr, int(hidden), int(b_colstride), int(b_stride), pre.ptr,
+                  int(pre_colstride), _ptr(offsets), int(n_groups), int(row_count), capi.DTYPE_CODES[pre_gradient.datatype])
+
     def combine_experts(self, output, output_colstride, rows, row_count, rows_colstride, weights, slots, n, n_chosen, width) -> None:
         capi.call("ct_combine_experts", self.handle, output.ptr, int(output_colstride), rows.ptr, int(row_count), int(rows_colstride),
                   _ptr(weights), slots.ptr, int(n), int(n_chosen), int(width), capi.DTYPE_CODES[output.datatype])

@@ -648,6 +648,37 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
                             int64_t b_colstride, const int32_t* b_index, const int32_t* offsets,
                             int64_t n_groups, int64_t row_count, double beta, int dtype);
 
+/* The first products of a gated feed-forward block and what follows them, in one pass.  With f the activation, for every row i
+ *   [gate up] = a[index[i]] * transpose(b_e),   inner[i] = f(gate) * up,   pre[i] = [gate up]
+ * b_e = b + e * b_stride [2 * hidden, a_col_count]: the gate's projection above the other's, of the group e that the row belongs
+ * to, as in ct_grouped_gemm; offsets NULL: one group of all rows.  inner [row_count, hidden]; pre [row_count, 2 * hidden] is what
+ * ct_gated_gemm_gradient needs (NULL: it is not stored).  An index outside a is a row of zeros.  No result overlaps an operand or the other.
+ * Sums and scratch memory are those of ct_grouped_gemm.  f is evaluated in the tensor's type.  */
+typedef enum ct_gate_t {
+  CT_GATE_LOGISTIC = 0, /* 1 / (1 + exp(-x)) */
+  CT_GATE_TANH = 1,
+  CT_GATE_RELU = 2,
+  CT_GATE_SWISH = 3, /* x / (1 + exp(-x)) */
+  CT_GATE_GELU = 4   /* x times the normal distribution's share below x */
+} ct_gate_t;
+int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre, int64_t pre_colstride,
+                  int activation, const void* a, int64_t a_row_count, int64_t a_col_count,
+                  int64_t a_colstride, const int32_t* index, const void* b, int64_t hidden,
+                  int64_t b_colstride, int64_t b_stride, const int32_t* offsets, int64_t n_groups,
+                  int64_t row_count, int dtype);
+
+/* What its backward pass begins with, from the gradient a [row_count, a_col_count] of the rows inner[i] * transpose(b_e), b_e
+ * [a_col_count, hidden] the projection back: with d = a[i] * b_e
+ *   pre_gradient[i] = [d * up * f'(gate)   d * f(gate)]
+ * and, unless it is NULL, inner[i] = f(gate) * up once more (for a caller that has not kept it).  pre_gradient may be pre itself,
+ * with the same stride; other overlaps are refused.  The gradients of the first products' operands are plain products of
+ * pre_gradient (ct_gemm; ct_grouped_gemm, ct_grouped_gemm_weights).  f' of the maximum with 0 is 0 at 0. */
+int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradient_colstride, void* inner,
+                           int64_t inner_colstride, int activation, const void* a, int64_t a_col_count,
+                           int64_t a_colstride, const void* b, int64_t hidden, int64_t b_colstride,
+                           int64_t b_stride, const void* pre, int64_t pre_colstride,
+                           const int32_t* offsets, int64_t n_groups, int64_t row_count, int dtype);
+
 /* output[t] = sum over j of weights[t, j] * rows[slots[t, j]], slots outside [0, row_count) left out; weights NULL: 1.
  * rows [row_count, width], output [n, width], weights and slots [n, n_chosen] packed, n_chosen <= 32.  Sums run in the order of j,
  * in the tensor's type.  output overlaps no operand. */
