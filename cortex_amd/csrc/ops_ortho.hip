@@ -83,7 +83,7 @@ struct StartArgs {
   bool nesterov;
 };
 
-constexpr uint32_t kParts = 256;
+constexpr uint32_t kParts = 1024;
 
 // What is made orthogonal: the matrix, the momentum, or what it will be after another such gradient.
 template <class T>
@@ -136,7 +136,13 @@ __global__ void __launch_bounds__(256) start_norm_kernel(const StartArgs a, uint
 }
 
 __device__ __forceinline__ double inverse_norm(const StartArgs& a, uint32_t matrix, uint32_t parts, double* lds) {
-  const double x = threadIdx.x < parts ? a.partial[(int64_t)matrix * kParts + threadIdx.x] : 0.0;
+  double x = 0.0;
+#pragma unroll
+  for (uint32_t i = 0; i < kParts / 256; ++i) {
+    const uint32_t at = i * 256 + threadIdx.x;
+    const double y = a.partial[(int64_t)matrix * kParts + min(at, parts - 1)];
+    x += at < parts ? y : 0.0;
+  }
   return 1.0 / (sqrt(sum_of_block(x, lds)) + a.epsilon);
 }
 
@@ -146,15 +152,17 @@ __global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, ui
   __shared__ double lds[4];
   __shared__ uint32_t cells[64][65];
   const uint32_t matrix = blockIdx.z, row0 = blockIdx.y * 64, column0 = blockIdx.x * 64;
-  const double factor = inverse_norm(a, matrix, parts, lds) * scale;
   const int64_t base = (int64_t)matrix * a.stride;
-  const uint32_t c = threadIdx.x % 64;
+  const uint32_t c = threadIdx.x % 64, column = min(column0 + c, a.columns - 1);
+  float values[16];   // on their way while the norm is added up: no branch that lanes take apart
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    values[i] = start_value<float>(a, base + (int64_t)min(row0 + i * 4 + threadIdx.x / 64, a.rows - 1) * a.ld + column);
+  const double factor = inverse_norm(a, matrix, parts, lds) * scale;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint32_t r = i * 4 + threadIdx.x / 64;
-    float x = 0.f;
-    if (row0 + r < a.rows && column0 + c < a.columns)
-      x = (float)((double)start_value<float>(a, base + (int64_t)(row0 + r) * a.ld + column0 + c) * factor);
+    const float x = row0 + r < a.rows && column0 + c < a.columns ? (float)((double)values[i] * factor) : 0.f;
     _Float16 hi, lo;
     split_pair(x, &hi, &lo);
     cells[r][c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
@@ -214,88 +222,137 @@ struct PairArgs {
   float alpha, beta;
 };
 
-template <int S> struct PairShape;
-template <> struct PairShape<64> { static constexpr int kM = 2, kN = 2; };
-template <> struct PairShape<128> { static constexpr int kM = 2, kN = 2; };
-template <> struct PairShape<256> { static constexpr int kM = 2, kN = 4; };
+// Tiles of S x S by WM x WN waves, loads kAhead runs ahead.
+template <int S_, int WM_, int WN_, int kAhead_>
+struct PairTile {
+  static constexpr int S = S_, WM = WM_, WN = WN_, kAhead = kAhead_, T = 64 * WM * WN, MT = S / WM / 32, NT = S / WN / 32;
+};
+using Tile256 = PairTile<256, 2, 4, 1>;
+using Tile128 = PairTile<128, 2, 2, 1>;
+using Tile64 = PairTile<64, 2, 2, 2>;
 
-template <int S, Product kProduct>
-__global__ void __launch_bounds__(64 * PairShape<S>::kM * PairShape<S>::kN, 2) pair_kernel(const PairArgs a) {
-  constexpr int WM = PairShape<S>::kM, WN = PairShape<S>::kN, MT = S / WM / 32, NT = S / WN / 32;
+// Results of a wave's 32 x 32 cells go to memory in whole lines: by way of an image in LDS, rows of 32 with both pieces in a word,
+// from which eight lanes take a run of a row, or of a column.  (Stored from the registers a line of 128 bytes took 16 instructions of a few
+// bytes each: 16 us to a block of 256 x 256.)
+// Orders what the lanes of a wave write to LDS and read there.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr uint32_t kImagePitch = 36, kImageWords = 32 * kImagePitch;
+
+__device__ __forceinline__ void store_lines(const uint32_t* image, uint32_t lane, bool turned, char* to, uint32_t row0, uint32_t rows, uint32_t runs,
+                                            uint32_t run) {
+  if (run >= runs) return;
+  const uint32_t high = lane >> 2 & 1, k = lane % 4 * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t r = i * 8 + lane / 8;
+    uint32_t w[8];
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = image[(k + e) * kImagePitch + r];
+    } else {
+      const pair_u32x4 x = *reinterpret_cast<const pair_u32x4*>(image + r * kImagePitch + k), y = *reinterpret_cast<const pair_u32x4*>(image + r * kImagePitch + k + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = x[e];
+        w[e + 4] = y[e];
+      }
+    }
+    pair_u32x4 line;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) line[e] = high ? w[2 * e] >> 16 | (w[2 * e + 1] & 0xffff0000u) : (w[2 * e] & 0xffff) | w[2 * e + 1] << 16;
+    if (row0 + r < rows) *reinterpret_cast<pair_u32x4*>(to + ((int64_t)(row0 + r) * runs + run) * kPairRunBytes + lane % 8 * 16) = line;
+  }
+}
+
+template <class Tile, Product kProduct>
+__global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
+  constexpr int S = Tile::S, WM = Tile::WM, WN = Tile::WN, MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(S, S)];
+  static_assert(WM * WN * kImageWords * 4 <= pair_tile_lds(S, S), "an image to a wave");
   TilePlace at;
   if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const uint32_t row0 = at.m_tile * S, column0 = at.n_tile * S, row_bytes = a.runs * kPairRunBytes;
   const char* left = a.left + at.matrix * a.left_stride;
   pair_f32x16 sum[MT][NT];
-  pair_tile<S, S, WM, WN>(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
-                          a.n - 1 - column0, row_bytes, 0, a.runs, lds, tid, sum);
-  const uint32_t wave_m = row0 + wave / WN * (MT * 32) + 4 * (lane >> 5), wave_n = column0 + wave % WN * (NT * 32) + (lane & 31);
+  pair_tile<S, S, WM, WN, Tile::kAhead>(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
+                                        a.n - 1 - column0, row_bytes, a.runs, lds, tid, sum);
+  const uint32_t wave_m = row0 + wave / WN * (MT * 32), wave_n = column0 + wave % WN * (NT * 32), c = lane & 31, half = lane >> 5;
   if constexpr (kProduct == kLast) {
     float* out = a.out + at.matrix * a.out_stride;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const uint32_t n = wave_n + u * 32;
+      const uint32_t n = wave_n + u * 32 + c;
       if (n >= a.n) continue;
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
+        float* const cells = out + (int64_t)(wave_m + t * 32 + 4 * half) * a.ldo + n;
+        const uint32_t rows = a.m - min(wave_m + t * 32 + 4 * half, a.m);
+        float before[16];   // all on their way before the first is stored
+        if (a.beta != 0.f) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8u * (r / 4) + r % 4 < rows) before[r] = cells[(int64_t)(8 * (r / 4) + r % 4) * a.ldo];
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const uint32_t m = wave_m + t * 32 + 8 * (r / 4) + r % 4;
-          if (m >= a.m) continue;
-          float& cell = out[(int64_t)m * a.ldo + n];
           const float value = a.alpha * (sum[t][u][r] * a.unscale);
-          cell = a.beta == 0.f ? value : value + a.beta * cell;
+          if (8u * (r / 4) + r % 4 < rows) cells[(int64_t)(8 * (r / 4) + r % 4) * a.ldo] = a.beta == 0.f ? value : value + a.beta * before[r];
         }
+      }
     }
   } else {
     // k along the columns of these results, and along the rows
     const uint32_t runs_n = (a.n + kPairRun - 1) / kPairRun, runs_m = (a.m + kPairRun - 1) / kPairRun;
     char* by_rows = a.by_rows + at.matrix * a.rows_stride;
     char* by_columns = is_symmetric(kProduct) ? by_rows : a.by_columns + at.matrix * a.columns_stride;
-    const bool diagonal = is_symmetric(kProduct) && at.m_tile == at.n_tile;
+    uint32_t* image = reinterpret_cast<uint32_t*>(lds) + wave * kImageWords;
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
+        const uint32_t m0 = wave_m + t * 32, n0 = wave_n + u * 32;
+        if (m0 >= a.m || n0 >= a.n) continue;
+        if constexpr (kProduct == kSquare) {   // A's lines as they are, 144 bytes apart
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t n = wave_n + u * 32, m = wave_m + t * 32 + 8 * q;
-          const int64_t turned = ((int64_t)n * runs_m + m / 32) * kPairRunBytes + m % 32 * 2;   // (n, m .. m + 3)
-          float x[4];
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t r = i * 8 + lane / 8;
+            *reinterpret_cast<pair_u32x4*>(image + r * kImagePitch + lane % 8 * 4) =
+                *reinterpret_cast<const pair_u32x4*>(left + ((int64_t)min(m0 + r, a.m - 1) * runs_n + n0 / 32) * kPairRunBytes + lane % 8 * 16);
+          }
+          wave_fence();
+        }
+        float x[16];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = sum[t][u][4 * q + e] * a.unscale;
+        for (int r = 0; r < 16; ++r) {
+          x[r] = sum[t][u][r] * a.unscale;
           if constexpr (kProduct == kSquare) {
-            if (n < a.n && m < runs_m * kPairRun) {
-              const f16x4 hi = *reinterpret_cast<const f16x4*>(left + turned), lo = *reinterpret_cast<const f16x4*>(left + turned + 64);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[e] = a.c * x[e] + a.b * (((float)hi[e] + (float)lo[e]) * a.a_unscale) + (m + e == n ? a.a : 0.f);
-            }
-          }
-          f16x4 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            _Float16 h, l;
-            split_pair(m + e < a.m && n < a.n ? x[e] * a.scale : 0.f, &h, &l);
-            hi[e] = h;
-            lo[e] = l;
-          }
-          if (n < a.n && m < runs_m * kPairRun) {
-            *reinterpret_cast<f16x4*>(by_columns + turned) = hi;
-            *reinterpret_cast<f16x4*>(by_columns + turned + 64) = lo;
-          }
-          if (!diagonal && n < runs_n * kPairRun) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (m + e >= a.m) continue;
-              char* p = by_rows + ((int64_t)(m + e) * runs_n + n / 32) * kPairRunBytes + n % 32 * 2;
-              *reinterpret_cast<_Float16*>(p) = hi[e];
-              *reinterpret_cast<_Float16*>(p + 64) = lo[e];
-            }
+            const uint32_t row = 8 * (r / 4) + 4 * half + r % 4;
+            const char* cell = reinterpret_cast<const char*>(image + row * kImagePitch) + c * 2;
+            _Float16 hi, lo;
+            __builtin_memcpy(&hi, cell, 2);
+            __builtin_memcpy(&lo, cell + 64, 2);
+            x[r] = a.c * x[r] + a.b * (((float)hi + (float)lo) * a.a_unscale) + (m0 + row == n0 + c ? a.a : 0.f);
           }
         }
+        wave_fence();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t row = 8 * (r / 4) + 4 * half + r % 4;
+          _Float16 hi, lo;
+          split_pair(m0 + row < a.m && n0 + c < a.n ? x[r] * a.scale : 0.f, &hi, &lo);
+          image[row * kImagePitch + c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+        }
+        wave_fence();
+        store_lines(image, lane, false, by_rows, m0, a.m, runs_n, n0 / 32);
+        if (!is_symmetric(kProduct) || at.m_tile != at.n_tile) store_lines(image, lane, true, by_columns, n0, a.n, runs_m, m0 / 32);
+        wave_fence();
+      }
   }
 }
 
@@ -403,19 +460,34 @@ int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetr
 
 constexpr int64_t kUnits = 256;
 
-int64_t pair_side(int64_t count, int64_t m, int64_t n, int64_t runs, bool symmetric) {
-  if (tiles_of(count, m, n, 256, symmetric) >= kUnits) return 256;
-  return tiles_of(count, m, n, 128, symmetric) >= kUnits ? 128 : 64;
+// Microseconds of `tiles` tiles over `runs` runs of 32 k.  Small tiles are bound by what the L2 caches give (13 TB/s), a block to a unit by
+// latency; of 128 a side two blocks share a unit; large ones are bound by the matrix cores, whose clock is higher while some of them
+// rest.  Us of 64, 128 and 256 a side: X X^T of 1024 x 1024 15, 33, 77; 2048 x 2048 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199;
+// 4096 x 8192 720, 527, 471; B X of them 16, 33, 77; 70, 63, 130; 440, 331, 296; 1000, 738, 651.  Within 15 % of all 60 times of which
+// these are a part.
+double time_of_64(int64_t tiles, int64_t runs) { return 5.0 + 0.31 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
+double time_of_128(int64_t tiles, int64_t runs) {
+  const int64_t full = tiles / (2 * kUnits), rest = tiles % (2 * kUnits);
+  return 7.0 * (double)(full + (rest > 0)) + (double)runs * (1.5 * (double)full + (rest == 0 ? 0.0 : rest <= kUnits ? 0.8 : 1.45));
+}
+double time_of_256(int64_t tiles, int64_t runs) {
+  const int64_t full = tiles / kUnits, rest = tiles % kUnits;
+  return 14.0 * (double)(full + (rest > 0)) + (double)runs * (2.5 * (double)full + (rest > 0 ? 1.75 + 0.75 * (double)rest / kUnits : 0.0));
+}
+
+template <class Tile, Product kProduct>
+void launch_tile(hipStream_t s, PairArgs a, int64_t count) {
+  a.order = order_of(count, a.m, a.n, Tile::S, is_symmetric(kProduct));
+  hipLaunchKernelGGL((pair_kernel<Tile, kProduct>), grid_of(a.order), dim3(Tile::T), 0, s, a);
 }
 
 template <Product kProduct>
-void launch_pair(hipStream_t s, PairArgs a, int64_t count) {
-  constexpr bool kSymmetric = is_symmetric(kProduct);
-  const int64_t side = pair_side(count, a.m, a.n, a.runs, kSymmetric);
-  a.order = order_of(count, a.m, a.n, side, kSymmetric);
-  if (side == 256) hipLaunchKernelGGL((pair_kernel<256, kProduct>), grid_of(a.order), dim3(512), 0, s, a);
-  else if (side == 128) hipLaunchKernelGGL((pair_kernel<128, kProduct>), grid_of(a.order), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((pair_kernel<64, kProduct>), grid_of(a.order), dim3(256), 0, s, a);
+void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
+  auto tiles = [&](int64_t side) { return tiles_of(count, a.m, a.n, side, is_symmetric(kProduct)); };
+  const double small = time_of_64(tiles(64), a.runs), medium = time_of_128(tiles(128), a.runs), large = time_of_256(tiles(256), a.runs);
+  if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
+  else if (medium <= large) launch_tile<Tile128, kProduct>(s, a, count);
+  else launch_tile<Tile256, kProduct>(s, a, count);
 }
 
 template <Product kProduct>
@@ -484,7 +556,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
   char* const gram = turned[1] + at_once * l.turned;
   char* const factor = gram + at_once * l.square;
   double* const partial = reinterpret_cast<double*>(factor + at_once * l.square);
-  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 2048));
+  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 4096));
   const uint64_t each = (uint64_t)ceil_div(cells, parts);
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);
@@ -570,7 +642,7 @@ int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once
   double* const gram = reinterpret_cast<double*>(base + 2 * at_once * l.x);
   double* const factor = reinterpret_cast<double*>(base + 2 * at_once * l.x + at_once * l.square);
   double* const partial = reinterpret_cast<double*>(base + 2 * at_once * (l.x + l.square));
-  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 2048));
+  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 4096));
   const uint64_t each = (uint64_t)ceil_div(cells, parts);
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);

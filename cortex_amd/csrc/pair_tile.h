@@ -33,14 +33,16 @@ __device__ __forceinline__ void split_pair(float x, _Float16* hi, _Float16* lo) 
 
 constexpr int pair_tile_lds(int bm, int bn) { return 2 * (bm + bn) * kPairRunBytes; }
 
-// The sums of runs first .. first + runs - 1 (of k) of BM rows of `a` with BN rows of `b`, over WM x WN waves of 64 lanes: a lane's
+// The sums over all runs of k (at least one) of BM rows of `a` with BN rows of `b`, over WM x WN waves of 64 lanes: a lane's
 // results of 32 x 32 cells, [.][.][r] row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.  Rows beyond the last ones repeat them.  All
-// of a block's waves call it, each group of them with an LDS of its own and as many runs.
+// of a block's waves call it.
 //
-// Chunks of 16 bytes of a row are permuted by the row's number, so that eight rows' reads of one chunk cover the banks once.
-template <int BM, int BN, int WM, int WN, int MT = BM / WM / 32, int NT = BN / WN / 32>
-__device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const char* b, uint32_t last_b, uint32_t row_bytes, uint32_t first,
-                                          uint32_t runs, char* lds, uint32_t tid, pair_f32x16 (&sum)[MT][NT]) {
+// Chunks of 16 bytes of a row are permuted by half the row's number, so that sixteen rows' reads of one chunk cover the banks once.  A
+// fragment is read a product or two ahead of its use into the registers of the one that was used last, and a run's loads are kAhead runs
+// ahead of their way into LDS.
+template <int BM, int BN, int WM, int WN, int kAhead, int MT = BM / WM / 32, int NT = BN / WN / 32>
+__device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const char* b, uint32_t last_b, uint32_t row_bytes, uint32_t runs,
+                                          char* lds, uint32_t tid, pair_f32x16 (&sum)[MT][NT]) {
   constexpr int T = 64 * WM * WN, UA = BM * 8 / T, UB = BN * 8 / T, U = UA + UB, kBuffer = (BM + BN) * kPairRunBytes;
   static_assert(UA * T == BM * 8 && UB * T == BN * 8 && T % 64 == 0, "lanes share the tiles evenly");
   const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -51,58 +53,114 @@ __device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const 
     for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[t][u][r] = 0.f;
-  if (runs == 0) return;
   uint32_t offset[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const uint32_t r = min(((i < UA ? i : i - UA) * T + tid) / 8, i < UA ? last_a : last_b);
     offset[i] = r * row_bytes + tid % 8 * 16;
   }
-  const uint32_t put = tid / 8 * kPairRunBytes + ((tid ^ tid / 8) & 7) * 16;
-  pair_u32x4 raw[U];
-  auto load = [&](uint32_t run) {
-    const int64_t at = (int64_t)(first + min(run, runs - 1)) * kPairRunBytes;
+  const uint32_t put = tid / 8 * kPairRunBytes + ((tid ^ tid / 16) & 7) * 16;
+  pair_u32x4 raw[kAhead][U];
+  auto load = [&](uint32_t run, int slot) {   // a run behind the last one is not used
+    const int64_t at = (int64_t)min(run, runs - 1) * kPairRunBytes;
 #pragma unroll
-    for (int i = 0; i < U; ++i) raw[i] = *reinterpret_cast<const pair_u32x4*>((i < UA ? a : b) + at + offset[i]);
+    for (int i = 0; i < U; ++i) raw[slot][i] = *reinterpret_cast<const pair_u32x4*>((i < UA ? a : b) + at + offset[i]);
   };
-  auto stage = [&](uint32_t buffer) {
+  auto stage = [&](uint32_t buffer, int slot) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      *reinterpret_cast<pair_u32x4*>(lds + buffer * kBuffer + (i < UA ? 0 : BM * kPairRunBytes) + (i < UA ? i : i - UA) * (T / 8 * kPairRunBytes) + put) = raw[i];
+      *reinterpret_cast<pair_u32x4*>(lds + buffer * kBuffer + (i < UA ? 0 : BM * kPairRunBytes) + (i < UA ? i : i - UA) * (T / 8 * kPairRunBytes) + put) = raw[slot][i];
   };
-  // piece p of 16 k of a run, of 32 rows
-  auto fetch = [&](uint32_t buffer, uint32_t base, uint32_t r, int part, int p) {
+  // [][0] leading pieces, [][1] others; a wave of one product has registers for both halves of a run
+  constexpr bool kBoth = MT * NT == 1;
+  f16x8 left[kBoth ? 2 : 1][2][MT], right[kBoth ? 2 : 1][2][NT];
+  auto fetch_left = [&](uint32_t buffer, int part, int p) {
     const uint32_t chunk = p * 4 + part * 2 + half;
-    return *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + base + r * kPairRunBytes + ((chunk ^ r) & 7) * 16);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+      left[kBoth ? part : 0][p][t] = *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + (wave_m + t * 32 + row) * kPairRunBytes + ((chunk ^ row / 2) & 7) * 16);
   };
-  auto multiply = [&](uint32_t buffer, int part) {
-    f16x8 left[MT][2], right[NT][2];
+  auto fetch_right = [&](uint32_t buffer, int part, int p) {
+    const uint32_t chunk = p * 4 + part * 2 + half;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+      right[kBoth ? part : 0][p][u] = *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + (BM + wave_n + u * 32 + row) * kPairRunBytes + ((chunk ^ row / 2) & 7) * 16);
+  };
+  auto multiply = [&](int part, int l, int r) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+        sum[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[kBoth ? part : 0][l][t], right[kBoth ? part : 0][r][u], sum[t][u], 0, 0, 0);
+  };
+  auto fetch = [&](uint32_t buffer, int part) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-#pragma unroll
-      for (int u = 0; u < NT; ++u) right[u][p] = fetch(buffer, BM * kPairRunBytes, wave_n + u * 32 + row, part, p);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) left[t][p] = fetch(buffer, 0, wave_m + t * 32 + row, part, p);
+      fetch_left(buffer, part, p);
+      fetch_right(buffer, part, p);
     }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)   // the smaller products first
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-          sum[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[t][i == 0], right[u][i == 1], sum[t][u], 0, 0, 0);
   };
-  load(0);
-  stage(0);
-  load(1);
+  auto multiply_all = [&](int part) {
+    multiply(part, 1, 0);
+    multiply(part, 0, 0);
+    multiply(part, 0, 1);
+  };
+  // run 0 in LDS, runs 1 .. kAhead on their way
+  load(0, 0);
+  stage(0, 0);
+#pragma unroll
+  for (int i = 1; i <= kAhead; ++i) load(i, i % kAhead);
   __syncthreads();
-  for (uint32_t run = 0; run < runs; ++run) {
-    const uint32_t buffer = run & 1;
-    multiply(buffer, 0);
-    stage(buffer ^ 1);
-    load(run + 2);
-    multiply(buffer, 1);
+  if constexpr (kBoth) {
+    fetch(0, 0);
+  } else {
+    fetch_left(0, 0, 1);
+    fetch_right(0, 0, 0);
+  }
+  auto step = [&](uint32_t run, uint32_t buffer, int slot) {
+    if constexpr (kBoth) {
+      fetch(buffer, 1);
+      stage(buffer ^ 1, slot);
+      load(run + 1 + kAhead, slot);
+      multiply_all(0);
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(buffer ^ 1, 0);
+      multiply_all(1);
+      __builtin_amdgcn_sched_barrier(0);
+      return;
+    }
+    fetch_left(buffer, 0, 0);
+    fetch_right(buffer, 0, 1);
+    multiply(0, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_left(buffer, 1, 1);
+    stage(buffer ^ 1, slot);
+    multiply(0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_right(buffer, 1, 0);
+    load(run + 1 + kAhead, slot);
+    multiply(0, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_left(buffer, 1, 0);
+    fetch_right(buffer, 1, 1);
+    multiply(1, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_left(buffer ^ 1, 0, 1);
+    multiply(1, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_right(buffer ^ 1, 0, 0);
+    multiply(1, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int kTurn = kAhead % 2 ? 2 * kAhead : kAhead;
+  for (uint32_t run = 0; run < runs; run += kTurn) {
+#pragma unroll
+    for (int i = 0; i < kTurn; ++i)
+      if (i == 0 || run + i < runs) step(run + i, i & 1, (i + 1) % kAhead);
   }
 }
 
