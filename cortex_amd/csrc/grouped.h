@@ -81,6 +81,7 @@ constexpr uint32_t kBand = 8, kRun = 16;
 struct GroupedPlan {
   uint32_t m_tiles, n_tiles, units, parts, run_shift;   // m_tiles: as many as there can be; units: of all parts
   uint32_t first;                                       // unit of this launch
+  uint32_t band;                                        // rows of tiles of a band
   FastDiv part_fd, band_fd;
 };
 
@@ -95,9 +96,9 @@ __device__ __forceinline__ bool place_of(const GroupedPlan& p, TilePlace* out) {
   uint32_t band, rest;
   p.part_fd.divmod(unit, out->part, unit);
   p.band_fd.divmod(unit, band, rest);
-  const uint32_t rows = min(kBand, p.m_tiles - band * kBand);
+  const uint32_t rows = min(p.band, p.m_tiles - band * p.band);
   out->n_tile = rest / rows;
-  out->m_tile = band * kBand + rest - out->n_tile * rows;
+  out->m_tile = band * p.band + rest - out->n_tile * rows;
   return true;
 }
 
@@ -251,9 +252,11 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t kMostUnits = int64_t(1) << 21, kMostTiles = (int64_t(1) << 31) - 1;
 static_assert(kMostUnits % (kXcds * kRun) == 0, "a launch ends with a round of runs");
 
-// Calls `launch(grid, plan)` for launches that together have a block for every unit.
+// Calls `launch(grid, plan)` for launches that together have a block for every unit.  Bands of one row of tiles leave the blocks
+// without a tile for the end: between the others they would leave every other unit of the chip without work (16 rows by 8192 gates and
+// ups of 4096: 82 us, 54 of 12 rows).
 template <class F>
-void for_launches(int64_t m_tiles, int64_t n_tiles, int64_t parts, F launch) {
+void for_launches(int64_t m_tiles, int64_t n_tiles, int64_t parts, F launch, uint32_t band = kBand) {
   GroupedPlan p;
   p.m_tiles = (uint32_t)m_tiles;
   p.n_tiles = (uint32_t)n_tiles;
@@ -262,7 +265,8 @@ void for_launches(int64_t m_tiles, int64_t n_tiles, int64_t parts, F launch) {
   p.run_shift = 0;
   while ((uint32_t(2) << p.run_shift) <= std::min(kRun, p.units / kXcds)) ++p.run_shift;
   p.part_fd = FastDiv((uint32_t)(m_tiles * n_tiles));
-  p.band_fd = FastDiv((uint32_t)(kBand * n_tiles));
+  p.band = band;
+  p.band_fd = FastDiv((uint32_t)(band * n_tiles));
   const int64_t round = (int64_t)kXcds << p.run_shift;
   for (int64_t first = 0; first < p.units; first += kMostUnits) {
     p.first = (uint32_t)first;
@@ -315,10 +319,6 @@ inline double time_of_medium(int64_t blocks, int64_t k_tiles) {
   return 3.3 + 1.3 * (double)shared + (double)k_tiles * (0.31 * (double)(full + (rest > 0)) + 0.33 * (double)shared);
 }
 inline double time_of_large(int64_t blocks, int64_t k_tiles) { return 1.8 + (double)ceil_div(blocks, 256) * (3.7 + 1.19 * (double)k_tiles); }
-// Of the kernel for a few rows, blocks of 64 and of 16 columns.
-inline double time_of_thin64(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, kUnits) * (0.5 + 0.28 * (double)k_tiles); }
-inline double time_of_thin16(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, 2 * kUnits) * (0.5 + 0.22 * (double)k_tiles); }
-
 struct Choice {
   int64_t height, width, parts;
   double us;
@@ -362,9 +362,6 @@ inline void consider_double_parts(Choice* best, int64_t blocks32, int64_t blocks
   }
 }
 
-// Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
-// from 1024 on eight or sixteen are as fast or faster.
-constexpr int64_t kFewK = 768;
 constexpr int64_t kMostSplitLd = int64_t(1) << 22, kMostWeightsLd = int64_t(1) << 30;
 
 constexpr int64_t kMostExtent = (int64_t(1) << 31) - 1;

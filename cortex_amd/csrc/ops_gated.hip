@@ -86,6 +86,49 @@ __device__ __forceinline__ void finish_gradient(const GatedArgs& a, int64_t row,
   if (a.inner) static_cast<T*>(a.inner)[row * a.ld_inner + column] = value * up;
 }
 
+// The row of a lane's r-th cell in a tile of 32 x 32, behind its first one's.
+__device__ __forceinline__ constexpr uint32_t row_at(int r) { return 8 * (r / 4) + r % 4; }
+
+// A lane's cells of a column, `rows` rows of them there.  Addresses are the first cell's and uniform multiples of the stride; all that is
+// read is on its way before the first result is stored, for that may be where it was read.
+__device__ __forceinline__ void finish_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&gate)[16], const float (&up)[16]) {
+  float* const inner = static_cast<float*>(a.inner) + row * a.ld_inner + column;
+  float* const pre = static_cast<float*>(a.pre) + row * a.ld_pre + column;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (row_at(r) >= rows) continue;
+    float value, slope;
+    activate(a.activation, gate[r], &value, &slope);
+    inner[row_at(r) * a.ld_inner] = value * up[r];
+    if (a.pre) {
+      pre[row_at(r) * a.ld_pre] = gate[r];
+      pre[row_at(r) * a.ld_pre + a.g.n] = up[r];
+    }
+  }
+}
+
+__device__ __forceinline__ void finish_gradient_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&d)[16]) {
+  const float* const read = static_cast<const float*>(a.pre_read) + row * a.ld_pre_read + column;
+  float* const pre = static_cast<float*>(a.pre) + row * a.ld_pre + column;
+  float* const inner = static_cast<float*>(a.inner) + row * a.ld_inner + column;
+  float gate[16], up[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int64_t at = min(row_at(r), rows - 1) * a.ld_pre_read;
+    gate[r] = read[at];
+    up[r] = read[at + a.g.n];
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (row_at(r) >= rows) continue;
+    float value, slope;
+    activate(a.activation, gate[r], &value, &slope);
+    pre[row_at(r) * a.ld_pre] = d[r] * up[r] * slope;
+    pre[row_at(r) * a.ld_pre + a.g.n] = d[r] * value;
+    if (a.inner) inner[row_at(r) * a.ld_inner] = value * up[r];
+  }
+}
+
 // Sums of a part of k, [part][row][gate up], or [part][row][column] of a gradient.
 template <class T>
 __device__ __forceinline__ void keep_pair(const GatedArgs& a, uint32_t part, int64_t row, uint32_t column, T gate, T up) {
@@ -177,15 +220,20 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_split_kernel(const Gate
     const uint32_t column = col0 + (wave % WN * (NT / 2) + u / 2) * 32 + (lane & 31);
     if (column >= a.g.n) continue;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t m = row0 + (wave / WN * MT + t) * 32 + 4 * half;
+      if (m >= g.rows) continue;
+      float up[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t m = row0 + (wave / WN * MT + t) * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        if (m >= g.rows) continue;
-        const float gate = result[t][u][r], up = NT == 1 ? ups[(t * 16 + r) * 64] : result[t][NT == 1 ? 0 : u + 1][r];
-        if (a.g.c) keep_pair(a, at.part, (int64_t)g.first + m, column, gate, up);
-        else finish(a, (int64_t)g.first + m, column, gate, up);
+      for (int r = 0; r < 16; ++r) up[r] = NT == 1 ? ups[(t * 16 + r) * 64] : result[t][NT == 1 ? 0 : u + 1][r];
+      if (!a.g.c) {
+        finish_column(a, (int64_t)g.first + m, column, g.rows - m, result[t][u], up);
+        continue;
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (m + row_at(r) < g.rows) keep_pair(a, at.part, (int64_t)g.first + m + row_at(r), column, result[t][u][r], up[r]);
+    }
   }
 }
 
@@ -206,15 +254,19 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_gradient_split_kernel(c
     const uint32_t column = col0 + wave % WN * (NT * 32) + u * 32 + (lane & 31);
     if (column >= a.g.n) continue;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t m = row0 + (wave / WN * MT + t) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-        if (m >= g.rows) continue;
-        const int64_t row = (int64_t)g.first + m;
-        if (a.g.c) static_cast<float*>(a.g.c)[at.part * a.g.c_split + row * a.g.ldc + column] = result[t][u][r];
-        else finish_gradient(a, row, column, result[t][u][r]);
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t m = row0 + (wave / WN * MT + t) * 32 + 4 * (lane >> 5);
+      if (m >= g.rows) continue;
+      const int64_t row = (int64_t)g.first + m;
+      if (!a.g.c) {
+        finish_gradient_column(a, row, column, g.rows - m, result[t][u]);
+        continue;
       }
+      float* const to = static_cast<float*>(a.g.c) + at.part * a.g.c_split + row * a.g.ldc + column;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (m + row_at(r) < g.rows) to[row_at(r) * a.g.ldc] = result[t][u][r];
+    }
   }
 }
 
@@ -355,6 +407,20 @@ struct Shape {
   int64_t blocks(int64_t height, int64_t width) const { return row_tiles(height) * ceil_div(stored, width); }
 };
 
+// Microseconds of the kernels for a few rows, 64 or 16 sums of a row to a block: the weights at 5.6 TB/s if 200 units read them, half of
+// that again for each further tile of rows; the float instructions at 110 TFLOP/s, mostly meanwhile; the rows, which each block reads,
+// at 16 TB/s.  Us of 16 and of 64: one row, 4096 by 8192 gates and ups, 48 and 53; sixteen 68 and 54; 16 rows, 1024 by 4096, 10.5 and 12;
+// 32, 2048 by 4096, 32 and 22; one, 1024 by 2816, 8 and 12.
+double time_of_few(const Shape& s, int64_t width) {
+  const double blocks = (double)s.blocks(16, width), tiles = (double)s.row_tiles(16) / (double)s.groups, units = std::min(1.0, blocks / (width == 64 ? 200 : 256));
+  const double read = (double)(4 * s.groups * s.k * s.stored) * (0.5 + 0.5 * tiles) / (5.6e6 * (width == 64 ? units : 1.0));
+  const double products = (double)(32 * s.row_tiles(16) * s.k * s.stored) / (110e6 * units);
+  return (width == 64 ? 4.5 : 3.5) + std::max(read, products) + 0.3 * std::min(read, products) + blocks * (double)(64 * s.k) / 16e6 +
+         1.5 * (double)((s.blocks(16, width) - 1) / (4 * kUnits));
+}
+// From these many k on a block has sixteen waves, of eight: 51 and 57 us at 4096 k; below 1024 the launch of sixteen takes longer.
+constexpr uint32_t kFewK16 = 1024, kFewK64 = 2049;
+
 template <class T, bool kGradient, class Launch>
 int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool split, Launch launch) {
   const int64_t cells = shape.rows * shape.stored, pair = kGradient ? 1 : 2;
@@ -375,7 +441,7 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
       consider_double_parts(&best, shape.blocks(32, 32), shape.blocks(64, 64), shape.k, shape.k, cells, most_parts);
       return best;
     } else {
-      const double thin64 = time_of_thin64(shape.blocks(16, 64), k_tiles), thin16 = time_of_thin16(shape.blocks(16, 16), k_tiles);
+      const double thin64 = time_of_few(shape, 64), thin16 = time_of_few(shape, 16);
       Choice best{16, thin16 < thin64 ? 16 : 64, 1, std::min(thin64, thin16)};
       if (split) consider_parts(&best, shape.blocks(64, 64), shape.blocks(128, 128), k_tiles, cells, most_parts);
       return best;
@@ -384,13 +450,14 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
   Choice best = choose(kMostParts);
   const Parts<T> parts(s, best.parts, cells);
   if (parts.count() < best.parts) best = choose(1);
-  const int64_t m_tiles = shape.rows / best.height + shape.groups, n_tiles = ceil_div(shape.columns, best.width / pair);
+  const int64_t m_tiles = a.g.offsets ? shape.rows / best.height + shape.groups : ceil_div(shape.rows, best.height), n_tiles = ceil_div(shape.columns, best.width / pair);
   CT_REQUIRE(m_tiles <= kMostTiles / parts.count() / n_tiles, "%s: %lld rows of %lld columns", name, (long long)shape.rows, (long long)shape.columns);
   a.g.c = const_cast<T*>(parts.partial());
   a.g.ldc = shape.stored;
   a.g.c_split = cells;
   a.g.part = (uint32_t)(std::is_same<T, double>::value ? ceil_div(shape.k, parts.count()) : tiles_of_part(k_tiles, parts.count()) * kTileDepth);
-  launch(a, best, m_tiles, n_tiles, parts.count());
+  const uint32_t band = best.height == 16 && shape.rows <= 16 * shape.groups ? 1 : kBand;
+  launch(a, best, m_tiles, n_tiles, parts.count(), band);
   if (parts.partial()) add_up(parts.count());
   static const char* const kNames[] = {"gated_thin", "gated_medium", "gated_large", "gated_medium+gated_sum", "gated_large+gated_sum", "gated_double",
                                        "gated_double+gated_sum"};
@@ -447,23 +514,23 @@ int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre,
   args.activation = activation;
   const Shape shape{row_count, hidden, std::min(n_groups, row_count), (int64_t)args.g.k, 2 * hidden};
   if (dtype == CT_F64) {
-    return run<double, false>("ct_gated_gemm", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts) {
+    return run<double, false>("ct_gated_gemm", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
         if (best.height == 64) hipLaunchKernelGGL((gated_double_kernel<64>), grid, dim3(256), 0, s, a, plan);
         else hipLaunchKernelGGL((gated_double_kernel<32>), grid, dim3(256), 0, s, a, plan);
-      });
+      }, band);
     });
   }
-  return run<float, false>("ct_gated_gemm", s, args, shape, shape.k >= kTileDepth, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts) {
+  return run<float, false>("ct_gated_gemm", s, args, shape, shape.k >= kTileDepth, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
     for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-      const bool few = a.g.k <= kFewK;
+      const bool few = a.g.k < (best.width == 64 ? kFewK64 : kFewK16);   // k
       if (best.height == 128) hipLaunchKernelGGL((gated_split_kernel<128, 128, 4, 2>), grid, dim3(512), 0, s, a, plan);
       else if (best.height == 64) hipLaunchKernelGGL((gated_split_kernel<64, 64, 2, 2>), grid, dim3(256), 0, s, a, plan);
-      else if (best.width == 64 && few) hipLaunchKernelGGL((gated_thin_kernel<4, 4>), grid, dim3(256), 0, s, a, plan);
-      else if (best.width == 64) hipLaunchKernelGGL((gated_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
-      else if (few) hipLaunchKernelGGL((gated_thin_kernel<4, 1>), grid, dim3(256), 0, s, a, plan);
+      else if (best.width == 64 && few) hipLaunchKernelGGL((gated_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
+      else if (best.width == 64) hipLaunchKernelGGL((gated_thin_kernel<16, 4>), grid, dim3(1024), 0, s, a, plan);
+      else if (few) hipLaunchKernelGGL((gated_thin_kernel<8, 1>), grid, dim3(512), 0, s, a, plan);
       else hipLaunchKernelGGL((gated_thin_kernel<16, 1>), grid, dim3(1024), 0, s, a, plan);
-    });
+    }, band);
   });
 }
 
@@ -507,24 +574,24 @@ int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradien
   args.activation = activation;
   const Shape shape{row_count, hidden, std::min(n_groups, row_count), a_col_count, hidden};
   if (dtype == CT_F64) {
-    return run<double, true>("ct_gated_gemm_gradient", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts) {
+    return run<double, true>("ct_gated_gemm_gradient", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
         if (best.height == 64) hipLaunchKernelGGL((gated_gradient_double_kernel<64>), grid, dim3(256), 0, s, a, plan);
         else hipLaunchKernelGGL((gated_gradient_double_kernel<32>), grid, dim3(256), 0, s, a, plan);
-      });
+      }, band);
     });
   }
   const bool split = a_col_count >= kTileDepth && b_colstride <= kMostSplitLd;
-  return run<float, true>("ct_gated_gemm_gradient", s, args, shape, split, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts) {
+  return run<float, true>("ct_gated_gemm_gradient", s, args, shape, split, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
     for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-      const bool few = a.g.k <= kFewK;
+      const bool few = a.g.k < (best.width == 64 ? kFewK64 : kFewK16);   // k
       if (best.height == 128) hipLaunchKernelGGL((gated_gradient_split_kernel<128, 128, 2, 4>), grid, dim3(512), 0, s, a, plan);
       else if (best.height == 64) hipLaunchKernelGGL((gated_gradient_split_kernel<64, 64, 2, 2>), grid, dim3(256), 0, s, a, plan);
-      else if (best.width == 64 && few) hipLaunchKernelGGL((gated_gradient_thin_kernel<4, 4>), grid, dim3(256), 0, s, a, plan);
-      else if (best.width == 64) hipLaunchKernelGGL((gated_gradient_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
-      else if (few) hipLaunchKernelGGL((gated_gradient_thin_kernel<4, 1>), grid, dim3(256), 0, s, a, plan);
+      else if (best.width == 64 && few) hipLaunchKernelGGL((gated_gradient_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
+      else if (best.width == 64) hipLaunchKernelGGL((gated_gradient_thin_kernel<16, 4>), grid, dim3(1024), 0, s, a, plan);
+      else if (few) hipLaunchKernelGGL((gated_gradient_thin_kernel<8, 1>), grid, dim3(512), 0, s, a, plan);
       else hipLaunchKernelGGL((gated_gradient_thin_kernel<16, 1>), grid, dim3(1024), 0, s, a, plan);
-    });
+    }, band);
   });
 }
 

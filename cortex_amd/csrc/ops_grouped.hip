@@ -324,6 +324,14 @@ void add_up(hipStream_t s, const Parts<T>& parts, const GroupedArgs& a) {
                      (uint32_t)parts.count(), (uint32_t)parts.cells(), FastDiv(a.n), FastDiv(kWeights ? a.m : 1));
 }
 
+// Of the kernel for a few rows, blocks of 64 and of 16 columns.
+double time_of_thin64(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, kUnits) * (0.5 + 0.28 * (double)k_tiles); }
+double time_of_thin16(int64_t blocks, int64_t k_tiles) { return 3.0 + (double)ceil_div(blocks, 2 * kUnits) * (0.5 + 0.22 * (double)k_tiles); }
+
+// Up to here a block of the kernel for a few rows has four waves: 64 matrices, 768 by 768 [k][n], 12 rows each, in 30 us, against 36 with eight;
+// from 1024 on eight or sixteen are as fast or faster.
+constexpr int64_t kFewK = 768;
+
 // Of the kernels whose blocks walk over tiles: as many as one launch may have along each side.
 inline dim3 plain_grid(int64_t columns, int64_t row_tiles, int64_t groups) {
   return dim3((uint32_t)std::min(ceil_div(columns, kSide), kMostUnits), (uint32_t)std::min<int64_t>(row_tiles, 65535), (uint32_t)groups);

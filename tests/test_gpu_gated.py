@@ -149,7 +149,7 @@ def test_each_kernel_of_floats(stream):  # noqa: F811
     D, met = Owned("float"), set()
     D.u, D.type = UNIT["float"], np.float32
     for size in ((16, 640, 5000), (3, 1024, 200), (600, 256, 640), (4096, 160, 1030), (128, 4096, 96), (2048, 2048, 64), (40, 1000, 130), (2, 20, 40),
-                 (700, 64, 1100)):
+                 (700, 64, 1100), (200, 4096, 130), (512, 2048, 64), (100, 8192, 300)):
         met.update(check(D, *size, seed=1))
         D.free()
         D.kept.clear()
