@@ -16,6 +16,7 @@
 #include "common.h"
 #include "double_tile.h"
 #include "grouped.h"
+#include "pair_tile.h"
 #include "rows.h"
 #include "split_tile.h"
 
@@ -89,14 +90,15 @@ __device__ __forceinline__ void finish_gradient(const GatedArgs& a, int64_t row,
 // The row of a lane's r-th cell in a tile of 32 x 32, behind its first one's.
 __device__ __forceinline__ constexpr uint32_t row_at(int r) { return 8 * (r / 4) + r % 4; }
 
-// A lane's cells of a column, `rows` rows of them there.  Addresses are the first cell's and uniform multiples of the stride; all that is
+// A lane's cells of a column, `rows` rows of them there but for those of the bits of `skip`.  Addresses are the first cell's and uniform multiples of the stride; all that is
 // read is on its way before the first result is stored, for that may be where it was read.
-__device__ __forceinline__ void finish_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&gate)[16], const float (&up)[16]) {
+__device__ __forceinline__ void finish_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&gate)[16], const float (&up)[16],
+                                              uint32_t skip = 0) {
   float* const inner = static_cast<float*>(a.inner) + row * a.ld_inner + column;
   float* const pre = static_cast<float*>(a.pre) + row * a.ld_pre + column;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    if (row_at(r) >= rows) continue;
+    if (row_at(r) >= rows || skip >> r & 1) continue;
     float value, slope;
     activate(a.activation, gate[r], &value, &slope);
     inner[row_at(r) * a.ld_inner] = value * up[r];
@@ -107,7 +109,8 @@ __device__ __forceinline__ void finish_column(const GatedArgs& a, int64_t row, u
   }
 }
 
-__device__ __forceinline__ void finish_gradient_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&d)[16]) {
+__device__ __forceinline__ void finish_gradient_column(const GatedArgs& a, int64_t row, uint32_t column, uint32_t rows, const float (&d)[16],
+                                                       uint32_t skip = 0) {
   const float* const read = static_cast<const float*>(a.pre_read) + row * a.ld_pre_read + column;
   float* const pre = static_cast<float*>(a.pre) + row * a.ld_pre + column;
   float* const inner = static_cast<float*>(a.inner) + row * a.ld_inner + column;
@@ -120,7 +123,7 @@ __device__ __forceinline__ void finish_gradient_column(const GatedArgs& a, int64
   }
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    if (row_at(r) >= rows) continue;
+    if (row_at(r) >= rows || skip >> r & 1) continue;
     float value, slope;
     activate(a.activation, gate[r], &value, &slope);
     pre[row_at(r) * a.ld_pre] = d[r] * up[r] * slope;
@@ -267,6 +270,259 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_gradient_split_kernel(c
       for (int r = 0; r < 16; ++r)
         if (m + row_at(r) < g.rows) to[row_at(r) * a.g.ldc] = result[t][u][r];
     }
+  }
+}
+
+// ------------------------------------------------------------------ float, many rows: two halves to a float
+
+// Three products of halves in place of six of bfloat16 pieces (pair_tile.h), of operands that are split once ahead of them: rows of
+// the left one and columns of the right one have a power of two each, so that an element is held to 2^-23 of itself, or to 2^-51 of the
+// largest of its row (or column) if that is more.  The chip's power bounds both kinds: 8192 rows, 1024 k, 5632 gates and ups 340 us
+// with the splitting, with three pieces 600.  What is not finite has no power of two: rows of a NaN are NaN, and results of a row or column of infinities are
+// formed once more from the floats.
+constexpr int kAbsentRow = 1000, kRowOfNan = 1001, kRowOfInfinity = 1002;   // in the place of a row's exponent
+
+// The exponent for a row whose largest magnitude has these bits.
+__device__ __forceinline__ int exponent_for(uint32_t most) {
+  if (most > 0x7f800000u) return kRowOfNan;
+  if (most == 0x7f800000u) return kRowOfInfinity;
+  if (most == 0) return 0;
+  const int log2 = most >> 23 ? (int)(most >> 23) - 127 : 31 - __clz(most) - 149;
+  return kPairTop - log2;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+struct PiecesArgs {
+  const float* x;      // matrices of `rows` rows (or, of a right operand by columns, k of them)
+  char* pieces;
+  int* exponents;
+  uint32_t* partial;   // [matrix][part][row], by columns
+  int64_t ld, stride;
+  uint32_t rows, k, parts;
+};
+
+// Rows of k floats as pieces, a row to a wave: read once where 64 lanes hold it.
+constexpr uint32_t kRowHeld = 8;   // times eight floats to a lane
+__global__ void __launch_bounds__(256) pieces_of_rows_kernel(const PiecesArgs a) {
+  const uint32_t row = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (row >= a.rows) return;
+  const float* x = a.x + (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld;
+  const uint32_t runs = (a.k + kPairRun - 1) / kPairRun;
+  auto load = [&](uint32_t k, f32x4 (&v)[2]) {
+    if (k + 8 <= a.k) {
+      __builtin_memcpy(&v[0], x + k, 16);
+      __builtin_memcpy(&v[1], x + k + 4, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e / 4][e % 4] = k + e < a.k ? x[k + e] : 0.f;
+    }
+  };
+  auto most_of = [&](const f32x4 (&v)[2], uint32_t most) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e / 4][e % 4]));
+    return most;
+  };
+  f32x4 held[kRowHeld][2];
+  uint32_t most = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kRowHeld; ++i)
+    if (i * 512 < a.k) {
+      load(i * 512 + lane * 8, held[i]);
+      most = most_of(held[i], most);
+    }
+  for (uint32_t k = kRowHeld * 512; k < a.k; k += 512) {
+    f32x4 v[2];
+    load(k + lane * 8, v);
+    most = most_of(v, most);
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+  const int exponent = exponent_for(most);
+  const int64_t at = (int64_t)blockIdx.y * a.rows + row;
+  if (lane == 0) a.exponents[at] = exponent;
+  char* to = a.pieces + at * runs * kPairRunBytes;
+  auto store = [&](uint32_t k, const f32x4 (&v)[2]) {
+    if (k >= runs * kPairRun) return;
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 h, l;
+      split_pair_apart(exponent < kAbsentRow ? ldexpf(v[e / 4][e % 4], exponent) : 0.f, &h, &l);
+      hi[e] = h;
+      lo[e] = l;
+    }
+    char* p = to + k / kPairRun * kPairRunBytes + k % kPairRun * 2;
+    *reinterpret_cast<f16x8*>(p) = hi;
+    *reinterpret_cast<f16x8*>(p + 64) = lo;
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < kRowHeld; ++i)
+    if (i * 512 < a.k) store(i * 512 + lane * 8, held[i]);
+  for (uint32_t k = kRowHeld * 512; k < a.k; k += 512) {
+    f32x4 v[2];
+    load(k + lane * 8, v);
+    store(k + lane * 8, v);
+  }
+}
+
+// The largest magnitudes of columns, of a part of the k rows each.
+__global__ void __launch_bounds__(256) most_of_columns_kernel(const PiecesArgs a) {
+  __shared__ uint32_t found[4][64];
+  const uint32_t c = threadIdx.x % 64, column = blockIdx.x * 64 + c, each = (a.k + a.parts - 1) / a.parts, first = blockIdx.y * each;
+  const float* x = a.x + (int64_t)blockIdx.z * a.stride + min(column, a.rows - 1);
+  uint32_t most = 0;
+  for (uint32_t k0 = first + threadIdx.x / 64; k0 < min(first + each, a.k); k0 += 16) {
+    float v[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) v[e] = x[(int64_t)min(k0 + e * 4, a.k - 1) * a.ld];   // once more is no harm
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) most = max(most, magnitude(v[e]));
+  }
+  found[threadIdx.x / 64][c] = most;
+  __syncthreads();
+  if (threadIdx.x < 64 && column < a.rows)
+    a.partial[((int64_t)blockIdx.z * a.parts + blockIdx.y) * a.rows + column] = max(max(found[0][c], found[1][c]), max(found[2][c], found[3][c]));
+}
+
+// 64 columns of 64 rows as pieces, k down the columns.
+__global__ void __launch_bounds__(256) pieces_of_columns_kernel(const PiecesArgs a) {
+  __shared__ uint32_t cells[64][65];
+  __shared__ int exponents[64];
+  const uint32_t c = threadIdx.x % 64, column0 = blockIdx.x * 64, k0 = blockIdx.y * 64, column = min(column0 + c, a.rows - 1);
+  const float* x = a.x + (int64_t)blockIdx.z * a.stride + column;
+  float values[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) values[i] = x[(int64_t)min(k0 + i * 4 + threadIdx.x / 64, a.k - 1) * a.ld];
+  if (threadIdx.x < 64) {
+    uint32_t most = 0;
+    for (uint32_t part = 0; part < a.parts; ++part) most = max(most, a.partial[((int64_t)blockIdx.z * a.parts + part) * a.rows + column]);
+    exponents[c] = exponent_for(most);
+    if (blockIdx.y == 0 && column0 + c < a.rows) a.exponents[(int64_t)blockIdx.z * a.rows + column] = exponents[c];
+  }
+  __syncthreads();
+  const int exponent = exponents[c];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t k = i * 4 + threadIdx.x / 64;
+    _Float16 hi, lo;
+    split_pair_apart(k0 + k < a.k && exponent < kAbsentRow ? ldexpf(values[i], exponent) : 0.f, &hi, &lo);
+    cells[c][k] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+  }
+  __syncthreads();
+  const uint32_t runs = (a.k + kPairRun - 1) / kPairRun;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // eight k of a column to a lane
+    const uint32_t at = i * 256 + threadIdx.x, r = at / 8, k = at % 8 * 8, run = k0 / kPairRun + k / kPairRun;
+    if (column0 + r >= a.rows || run >= runs) continue;
+    pair_u32x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t v = cells[r][k + 2 * e], w = cells[r][k + 2 * e + 1];
+      hi[e] = (v & 0xffff) | w << 16;
+      lo[e] = v >> 16 | (w & 0xffff0000u);
+    }
+    char* p = a.pieces + (((int64_t)blockIdx.z * a.rows + column0 + r) * runs + run) * kPairRunBytes + k % kPairRun * 2;
+    *reinterpret_cast<pair_u32x4*>(p) = hi;
+    *reinterpret_cast<pair_u32x4*>(p + 64) = lo;
+  }
+}
+
+struct GatedPieces {
+  const char *left, *right;   // [row of a], [group][row of the weights, or column]
+  const int *left_exponents, *right_exponents;
+  uint32_t runs;
+};
+
+// A product in floats; stride: of the right operand's k.
+__device__ __forceinline__ float plain_product(const float* left, const float* right, int64_t stride, uint32_t k) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (uint32_t i = 0; i < k; ++i) sum += left[i] * right[i * stride];
+  return sum;
+}
+
+template <int BM, int BN, int WM, int WN, bool kGradient>
+__global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const GatedArgs a, const GatedPieces pieces, const GroupedPlan p) {
+  constexpr int T = 64 * WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, kColumns = kGradient ? BN : BN / 2;
+  static_assert(kGradient || NT % 2 == 0, "gates beside their ups");
+  __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(BM, BN)];
+  __shared__ int exponents[BM + BN];
+  TilePlace at;
+  Group g;
+  if (!place_of(p, &at) || !find_group(a.g, at.m_tile, BM, &g)) return;
+  const uint32_t row0 = g.tile * BM, col0 = at.n_tile * kColumns, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row_bytes = (int64_t)pieces.runs * kPairRunBytes, right0 = (int64_t)g.index * (kGradient ? a.g.n : 2 * (int64_t)a.g.n);
+  auto left_row = [&](uint32_t r) {   // of a; one outside it is absent
+    const uint32_t row = g.first + min(row0 + r, g.rows - 1);
+    return a.g.index_a ? (uint32_t)a.g.index_a[row] : row;
+  };
+  auto right_row = [&](uint32_t r) {
+    const uint32_t column = min(col0 + (kGradient ? r : r / 64 * 32 + r % 32), a.g.n - 1);
+    return kGradient || r / 32 % 2 == 0 ? column : a.g.n + column;
+  };
+  bool found = false;
+  for (uint32_t i = tid; i < BM + BN; i += T) {
+    if (i < BM) {
+      const uint32_t row = left_row(i);
+      exponents[i] = row < a.g.a_rows ? pieces.left_exponents[row] : kAbsentRow;
+    } else {
+      exponents[i] = pieces.right_exponents[right0 + right_row(i - BM)];
+    }
+    found |= exponents[i] >= kAbsentRow;
+  }
+  found = __syncthreads_or(found);
+  const PairRows<BM, BN, T> source(
+      [&](uint32_t r) {
+        const uint32_t row = left_row(r);
+        return pieces.left + (row < a.g.a_rows ? row : 0) * row_bytes;
+      },
+      [&](uint32_t r) { return pieces.right + (right0 + right_row(r)) * row_bytes; }, tid);
+  pair_f32x16 sum[2][MT][NT];
+  pair_tile<BM, BN, WM, WN, 1, true>(source, pieces.runs, lds, tid, sum);
+  // what has exponents
+#pragma unroll
+  for (int at_u = 0; at_u < (kGradient ? NT : NT / 2); ++at_u) {
+    const int u = kGradient ? at_u : 2 * at_u;
+    const uint32_t n = (wave % WN * NT + u) * 32 + (lane & 31), column = col0 + (wave % WN * (kGradient ? NT : NT / 2) + at_u) * 32 + (lane & 31);
+    if (column >= a.g.n) continue;
+    const int right = exponents[BM + n], right_up = kGradient ? 0 : exponents[BM + n + 32];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uint32_t m = (wave / WN * MT + t) * 32 + 4 * (lane >> 5);
+      if (row0 + m >= g.rows) continue;
+      float first[16], second[16];
+      uint32_t skip = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int left = exponents[m + row_at(r)];
+        skip |= (max(left, max(right, right_up)) >= kAbsentRow ? 1u : 0u) << r;
+        first[r] = ldexpf(sum[0][t][u][r] + sum[1][t][u][r] * (1.f / (1 << kPairApart)), -(left + right));
+        if constexpr (!kGradient) second[r] = ldexpf(sum[0][t][u + 1][r] + sum[1][t][u + 1][r] * (1.f / (1 << kPairApart)), -(left + right_up));
+      }
+      if constexpr (kGradient) finish_gradient_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, skip);
+      else finish_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, second, skip);
+    }
+  }
+  if (!found) return;
+  // what has not, a cell after the other
+  auto product = [&](uint32_t r, uint32_t n) -> float {
+    const int left = exponents[r], right = exponents[BM + n];
+    if (max(left, right) < kAbsentRow || (left != kAbsentRow && left != kRowOfNan && right != kRowOfNan)) {
+      const float* b = static_cast<const float*>(a.g.b) + (int64_t)g.index * a.g.b_stride + (int64_t)right_row(n) * (kGradient ? 1 : a.g.ldb);
+      return plain_product(static_cast<const float*>(a.g.a) + (int64_t)left_row(r) * a.g.lda, b, kGradient ? a.g.ldb : 1, a.g.k);
+    }
+    return left == kAbsentRow && right < kAbsentRow ? 0.f : __builtin_nanf("");   // zeros by what is not finite, too
+  };
+#pragma unroll 1
+  for (uint32_t i = tid; i < BM * kColumns; i += T) {
+    const uint32_t r = i / kColumns, c = i % kColumns, n = kGradient ? c : c / 32 * 64 + c % 32;
+    if (row0 + r >= g.rows || col0 + c >= a.g.n) continue;
+    const int most = max(exponents[r], max(exponents[BM + n], kGradient ? 0 : exponents[BM + n + (kGradient ? 0 : 32)]));
+    if (most < kAbsentRow) continue;
+    const int64_t row = (int64_t)g.first + row0 + r;
+    if constexpr (kGradient) finish_gradient(a, row, col0 + c, product(r, n));
+    else finish(a, row, col0 + c, product(r, n), product(r, n + 32));
   }
 }
 
@@ -421,6 +677,55 @@ double time_of_few(const Shape& s, int64_t width) {
 // From these many k on a block has sixteen waves, of eight: 51 and 57 us at 4096 k; below 1024 the launch of sixteen takes longer.
 constexpr uint32_t kFewK16 = 1024, kFewK64 = 2049;
 
+int64_t aligned(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
+
+// Two blocks of four waves to a unit: one's results go to memory beside the other's products (a gradient's product of 8192 rows, 2816 by
+// 1024, 255 us, in tiles of 256 by 128 of eight waves 270).
+constexpr int kPairM = 128, kPairN = 128, kPairWavesM = 2, kPairWavesN = 2;
+
+// Microseconds beyond the products' for a round of blocks, whose results' bytes bound it: with three pieces, and with two halves.
+constexpr double end_of_round(bool pairs, bool gradient) { return pairs ? (gradient ? 36.0 : 10.0) : (gradient ? 25.0 : 12.0); }
+
+// Microseconds with two halves to a float: the splitting at 3.5 TB/s, rounds of blocks, two to a unit or in the last one by themselves.
+double time_of_pairs(const Shape& s, int64_t left_rows, bool gradient) {
+  const int64_t right = s.groups * s.stored, blocks = s.blocks(kPairM, kPairN), full = blocks / (2 * kUnits), rest = blocks % (2 * kUnits);
+  const double split = (double)s.k * (8.0 * (double)left_rows + (gradient ? 12.0 : 8.0) * (double)right) / 3.5e6;
+  const double end = end_of_round(true, gradient), runs = (double)ceil_div(s.k, kPairRun);
+  return 10.0 + split + (double)full * (end + 1.38 * runs) + (rest == 0 ? 0.0 : rest <= kUnits ? 0.6 * end + 0.8 * runs : end + 1.38 * runs);
+}
+
+// Whether scratch was there, and the launches have been made.
+template <bool kGradient>
+bool run_pairs(hipStream_t s, const GatedArgs& a, const Shape& shape, int64_t left_rows, int64_t all_groups) {
+  const int64_t runs = ceil_div(shape.k, kPairRun), right_rows = all_groups * shape.stored, parts = std::min<int64_t>(32, ceil_div(shape.k, 64));
+  const int64_t left_bytes = aligned(left_rows * runs * kPairRunBytes), right_bytes = aligned(right_rows * runs * kPairRunBytes);
+  const int64_t partial_bytes = kGradient ? aligned(right_rows * parts * 4) : 0;
+  const ProductScratch scratch(s, (size_t)(left_bytes + right_bytes + aligned(left_rows * 4) + aligned(right_rows * 4) + partial_bytes));
+  char* const base = static_cast<char*>(scratch.get());
+  if (!base) return false;
+  char* const right = base + left_bytes;
+  int* const left_exponents = reinterpret_cast<int*>(right + right_bytes);
+  int* const right_exponents = left_exponents + aligned(left_rows * 4) / 4;
+  PiecesArgs of_left{static_cast<const float*>(a.g.a), base, left_exponents, nullptr, a.g.lda, 0, (uint32_t)left_rows, (uint32_t)shape.k, 0};
+  hipLaunchKernelGGL(pieces_of_rows_kernel, dim3((uint32_t)ceil_div(left_rows, 4)), dim3(256), 0, s, of_left);
+  PiecesArgs of_right{static_cast<const float*>(a.g.b), right, right_exponents, reinterpret_cast<uint32_t*>(right_exponents + aligned(right_rows * 4) / 4),
+                      a.g.ldb, a.g.b_stride, (uint32_t)shape.stored, (uint32_t)shape.k, (uint32_t)parts};
+  const uint32_t groups = (uint32_t)all_groups;
+  if constexpr (kGradient) {
+    const uint32_t columns = (uint32_t)ceil_div(shape.stored, 64);
+    hipLaunchKernelGGL(most_of_columns_kernel, dim3(columns, (uint32_t)parts, groups), dim3(256), 0, s, of_right);
+    hipLaunchKernelGGL(pieces_of_columns_kernel, dim3(columns, (uint32_t)ceil_div(shape.k, 64), groups), dim3(256), 0, s, of_right);
+  } else {
+    hipLaunchKernelGGL(pieces_of_rows_kernel, dim3((uint32_t)ceil_div(shape.stored, 4), groups), dim3(256), 0, s, of_right);
+  }
+  const GatedPieces pieces{base, right, left_exponents, right_exponents, (uint32_t)runs};
+  const int64_t m_tiles = a.g.offsets ? shape.rows / kPairM + shape.groups : ceil_div(shape.rows, kPairM), n_tiles = ceil_div(shape.stored, kPairN);
+  for_launches(m_tiles, n_tiles, 1, [&](dim3 grid, const GroupedPlan& plan) {
+    hipLaunchKernelGGL((gated_pair_kernel<kPairM, kPairN, kPairWavesM, kPairWavesN, kGradient>), grid, dim3(64 * kPairWavesM * kPairWavesN), 0, s, a, pieces, plan);
+  });
+  return true;
+}
+
 template <class T, bool kGradient, class Launch>
 int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool split, Launch launch) {
   const int64_t cells = shape.rows * shape.stored, pair = kGradient ? 1 : 2;
@@ -448,6 +753,15 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
     }
   };
   Choice best = choose(kMostParts);
+  if constexpr (std::is_same<T, float>::value) {
+    const int64_t left_rows = a.g.a_rows;
+    double us = best.us;
+    if (best.height == 128) us += end_of_round(false, kGradient) * (double)ceil_div(shape.blocks(128, 128) * best.parts, kUnits);
+    if (shape.k >= kPairRun && time_of_pairs(shape, left_rows, kGradient) < us && run_pairs<kGradient>(s, a, shape, left_rows, a.g.groups)) {
+      note_kernel(kGradient ? "gated_gradient_pairs" : "gated_pairs");
+      return after_launch(s);
+    }
+  }
   const Parts<T> parts(s, best.parts, cells);
   if (parts.count() < best.parts) best = choose(1);
   const int64_t m_tiles = a.g.offsets ? shape.rows / best.height + shape.groups : ceil_div(shape.rows, best.height), n_tiles = ceil_div(shape.columns, best.width / pair);

@@ -278,9 +278,11 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const uint32_t row0 = at.m_tile * S, column0 = at.n_tile * S, row_bytes = a.runs * kPairRunBytes;
   const char* left = a.left + at.matrix * a.left_stride;
-  pair_f32x16 sum[MT][NT];
-  pair_tile<S, S, WM, WN, Tile::kAhead>(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
-                                        a.n - 1 - column0, row_bytes, a.runs, lds, tid, sum);
+  pair_f32x16 sums[1][MT][NT];
+  const PairMatrices<S, S, Tile::T> source(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
+                                           a.n - 1 - column0, row_bytes, tid);
+  pair_tile<S, S, WM, WN, Tile::kAhead, false>(source, a.runs, lds, tid, sums);
+  pair_f32x16 (&sum)[MT][NT] = sums[0];
   const uint32_t wave_m = row0 + wave / WN * (MT * 32), wave_n = column0 + wave % WN * (NT * 32), c = lane & 31, half = lane >> 5;
   if constexpr (kProduct == kLast) {
     float* out = a.out + at.matrix * a.out_stride;

@@ -31,40 +31,73 @@ __device__ __forceinline__ void split_pair(float x, _Float16* hi, _Float16* lo) 
   *lo = (_Float16)(x - (float)*hi);
 }
 
+// Of matrices without a known bound a row has a power of two of its own, which takes its largest element below 2^15, and the other
+// pieces are 2^kPairApart times as large as they are, so that they are no denormals before the element is 2^-28 of its row's largest:
+// what is below 2^-51 of that is zero.  Their products are summed apart.
+constexpr int kPairApart = 11;
+__device__ __forceinline__ void split_pair_apart(float x, _Float16* hi, _Float16* lo) {
+  *hi = (_Float16)x;
+  *lo = (_Float16)((x - (float)*hi) * (float)(1 << kPairApart));
+}
+
 constexpr int pair_tile_lds(int bm, int bn) { return 2 * (bm + bn) * kPairRunBytes; }
 
-// The sums over all runs of k (at least one) of BM rows of `a` with BN rows of `b`, over WM x WN waves of 64 lanes: a lane's
-// results of 32 x 32 cells, [.][.][r] row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.  Rows beyond the last ones repeat them.  All
-// of a block's waves call it.
+// Rows of two matrices of pieces, those beyond the last ones repeated: where they begin and how far apart rows are.
+template <int BM, int BN, int T>
+struct PairMatrices {
+  static constexpr int UA = BM * 8 / T, U = UA + BN * 8 / T;
+  const char *a, *b;
+  uint32_t offset[U];
+  __device__ __forceinline__ PairMatrices(const char* a, uint32_t last_a, const char* b, uint32_t last_b, uint32_t row_bytes, uint32_t tid) : a(a), b(b) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) offset[i] = min(((i < UA ? i : i - UA) * T + tid) / 8, i < UA ? last_a : last_b) * row_bytes + tid % 8 * 16;
+  }
+  __device__ __forceinline__ pair_u32x4 load(int i, uint32_t run) const {
+    return *reinterpret_cast<const pair_u32x4*>((i < UA ? a : b) + (int64_t)run * kPairRunBytes + offset[i]);
+  }
+};
+
+// Rows that lie anywhere: `left(r)` and `right(r)` say where those of the tile begin.
+template <int BM, int BN, int T>
+struct PairRows {
+  static constexpr int UA = BM * 8 / T, U = UA + BN * 8 / T;
+  const char* row[U];
+  template <class Left, class Right>
+  __device__ __forceinline__ PairRows(Left left, Right right, uint32_t tid) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) row[i] = (i < UA ? left((i * T + tid) / 8) : right(((i - UA) * T + tid) / 8)) + tid % 8 * 16;
+  }
+  __device__ __forceinline__ pair_u32x4 load(int i, uint32_t run) const {
+    return *reinterpret_cast<const pair_u32x4*>(row[i] + (int64_t)run * kPairRunBytes);
+  }
+};
+
+// The sums over all runs of k (at least one) of BM rows of the source's left matrix with BN rows of its right one, over WM x WN waves of 64 lanes:
+// a lane's results of 32 x 32 cells, [.][.][.][r] row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.  All of a block's waves call it.
+// kApart: the products of the leading pieces in sum[0], those of one leading piece in sum[1]; else all of them in sum[0].
 //
 // Chunks of 16 bytes of a row are permuted by half the row's number, so that sixteen rows' reads of one chunk cover the banks once.  A
 // fragment is read a product or two ahead of its use into the registers of the one that was used last, and a run's loads are kAhead runs
 // ahead of their way into LDS.
-template <int BM, int BN, int WM, int WN, int kAhead, int MT = BM / WM / 32, int NT = BN / WN / 32>
-__device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const char* b, uint32_t last_b, uint32_t row_bytes, uint32_t runs,
-                                          char* lds, uint32_t tid, pair_f32x16 (&sum)[MT][NT]) {
-  constexpr int T = 64 * WM * WN, UA = BM * 8 / T, UB = BN * 8 / T, U = UA + UB, kBuffer = (BM + BN) * kPairRunBytes;
-  static_assert(UA * T == BM * 8 && UB * T == BN * 8 && T % 64 == 0, "lanes share the tiles evenly");
+template <int BM, int BN, int WM, int WN, int kAhead, bool kApart, class Source, int MT = BM / WM / 32, int NT = BN / WN / 32>
+__device__ __forceinline__ void pair_tile(const Source& source, uint32_t runs, char* lds, uint32_t tid, pair_f32x16 (&sum)[kApart ? 2 : 1][MT][NT]) {
+  constexpr int T = 64 * WM * WN, UA = Source::UA, U = Source::U, kBuffer = (BM + BN) * kPairRunBytes;
+  static_assert(UA * T == BM * 8 && (U - UA) * T == BN * 8 && T % 128 == 0, "lanes share the tiles evenly");
   const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t wave_m = wave / WN * (MT * 32), wave_n = wave % WN * (NT * 32), row = lane & 31, half = lane >> 5;
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int s = 0; s < (kApart ? 2 : 1); ++s)
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum[t][u][r] = 0.f;
-  uint32_t offset[U];
+      for (int u = 0; u < NT; ++u)
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const uint32_t r = min(((i < UA ? i : i - UA) * T + tid) / 8, i < UA ? last_a : last_b);
-    offset[i] = r * row_bytes + tid % 8 * 16;
-  }
+        for (int r = 0; r < 16; ++r) sum[s][t][u][r] = 0.f;
   const uint32_t put = tid / 8 * kPairRunBytes + ((tid ^ tid / 16) & 7) * 16;
   pair_u32x4 raw[kAhead][U];
   auto load = [&](uint32_t run, int slot) {   // a run behind the last one is not used
-    const int64_t at = (int64_t)min(run, runs - 1) * kPairRunBytes;
 #pragma unroll
-    for (int i = 0; i < U; ++i) raw[slot][i] = *reinterpret_cast<const pair_u32x4*>((i < UA ? a : b) + at + offset[i]);
+    for (int i = 0; i < U; ++i) raw[slot][i] = source.load(i, min(run, runs - 1));
   };
   auto stage = [&](uint32_t buffer, int slot) {
 #pragma unroll
@@ -84,14 +117,17 @@ __device__ __forceinline__ void pair_tile(const char* a, uint32_t last_a, const 
     const uint32_t chunk = p * 4 + part * 2 + half;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
-      right[kBoth ? part : 0][p][u] = *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + (BM + wave_n + u * 32 + row) * kPairRunBytes + ((chunk ^ row / 2) & 7) * 16);
+      right[kBoth ? part : 0][p][u] =
+          *reinterpret_cast<const f16x8*>(lds + buffer * kBuffer + (BM + wave_n + u * 32 + row) * kPairRunBytes + ((chunk ^ row / 2) & 7) * 16);
   };
   auto multiply = [&](int part, int l, int r) {
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
-        sum[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[kBoth ? part : 0][l][t], right[kBoth ? part : 0][r][u], sum[t][u], 0, 0, 0);
+      for (int u = 0; u < NT; ++u) {
+        pair_f32x16& to = sum[kApart ? l | r : 0][t][u];
+        to = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[kBoth ? part : 0][l][t], right[kBoth ? part : 0][r][u], to, 0, 0, 0);
+      }
   };
   auto fetch = [&](uint32_t buffer, int part) {
 #pragma unroll

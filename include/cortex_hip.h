@@ -653,7 +653,10 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
  * b_e = b + e * b_stride [2 * hidden, a_col_count]: the gate's projection above the other's, of the group e that the row belongs
  * to, as in ct_grouped_gemm; offsets NULL: one group of all rows.  inner [row_count, hidden]; pre [row_count, 2 * hidden] is what
  * ct_gated_gemm_gradient needs (NULL: it is not stored).  An index outside a is a row of zeros.  No result overlaps an operand or the other.
- * Sums and scratch memory are those of ct_grouped_gemm.  f is evaluated in the tensor's type.  */
+ * Sums and scratch memory are those of ct_grouped_gemm; but float products of many rows are formed of two halves to a float, each row of
+ * a and of b_e with a power of two of its own: an element is held to 2^-23 of itself, or to 2^-51 of the largest of its row, whichever is
+ * more, and sums are float ones.  They take scratch memory for the pieces, 4 bytes to an element of a and b, up to 256 MiB, and are
+ * formed as ct_grouped_gemm's beyond that.  f is evaluated in the tensor's type. */
 typedef enum ct_gate_t {
   CT_GATE_LOGISTIC = 0, /* 1 / (1 + exp(-x)) */
   CT_GATE_TANH = 1,
@@ -671,7 +674,8 @@ int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre,
  * [a_col_count, hidden] the projection back: with d = a[i] * b_e
  *   pre_gradient[i] = [d * up * f'(gate)   d * f(gate)]
  * and, unless it is NULL, inner[i] = f(gate) * up once more (for a caller that has not kept it).  pre_gradient may be pre itself,
- * with the same stride; other overlaps are refused.  The gradients of the first products' operands are plain products of
+ * with the same stride; other overlaps are refused.  Sums and scratch memory as above, a power of two to each row of a and column
+ * of b_e.  The gradients of the first products' operands are plain products of
  * pre_gradient (ct_gemm; ct_grouped_gemm, ct_grouped_gemm_weights).  f' of the maximum with 0 is 0 at 0. */
 int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradient_colstride, void* inner,
                            int64_t inner_colstride, int activation, const void* a, int64_t a_col_count,

@@ -149,12 +149,94 @@ def test_each_kernel_of_floats(stream):  # noqa: F811
     D, met = Owned("float"), set()
     D.u, D.type = UNIT["float"], np.float32
     for size in ((16, 640, 5000), (3, 1024, 200), (600, 256, 640), (4096, 160, 1030), (128, 4096, 96), (2048, 2048, 64), (40, 1000, 130), (2, 20, 40),
-                 (700, 64, 1100), (200, 4096, 130), (512, 2048, 64), (100, 8192, 300)):
+                 (700, 64, 1100), (200, 4096, 130), (512, 2048, 64), (100, 8192, 300), (3000, 1000, 2300), (2048, 512, 1024, 8), (2048, 512, 2048, 8)):
         met.update(check(D, *size, seed=1))
         D.free()
         D.kept.clear()
     assert met >= {"gated_thin", "gated_gradient_thin", "gated_medium", "gated_gradient_medium", "gated_large", "gated_gradient_large",
-                   "gated_medium+gated_sum", "gated_gradient_medium+gated_sum"}, met
+                   "gated_medium+gated_sum", "gated_gradient_medium+gated_sum", "gated_pairs", "gated_gradient_pairs"}, met
+
+
+def test_many_rows_of_floats_by_group(stream):  # noqa: F811
+    """Groups of uneven sizes, rows by index and rows of no group, with two halves to a float."""
+    D = Owned("float")
+    D.u, D.type = UNIT["float"], np.float32
+    for kwargs in ({}, {"indexed": True, "kind": "gaps"}, {"pad": 3, "activation": "gelu"}):
+        assert check(D, 5000, 1000, 2300, 3, seed=1, **kwargs) == ["gated_pairs", "gated_gradient_pairs"]
+        D.free()
+        D.kept.clear()
+
+
+def test_rows_of_any_magnitude(stream):  # noqa: F811
+    """With two halves to a float each row and column has its power of two: magnitudes from the smallest to the largest ones, rows of zeros,
+    and elements far below the largest of their row, whose products are held to the float sum's bar."""
+    D = Owned("float")
+    rng = np.random.default_rng(7)
+    rows, width, hidden = 3000, 1000, 2300
+    x = rng.standard_normal((rows, width)).astype(np.float32)
+    weights = (rng.standard_normal((2 * hidden, width)) / math.sqrt(width)).astype(np.float32)
+    x *= np.exp2(rng.integers(-60, 30, rows)).astype(np.float32)[:, None]
+    x[5], x[6, 1:], x[7] = 0, 0, np.float32(1e-42)
+    x[:, 17] *= np.float32(2.0 ** 12)            # one channel far above the others, whose weights are small
+    weights[:, 17] *= np.float32(2.0 ** -12)
+    weights *= np.exp2(rng.integers(-30, 30, 2 * hidden)).astype(np.float32)[:, None]
+    inner, pre = D.tensor(np.zeros((rows, hidden))), D.tensor(np.zeros((rows, 2 * hidden)))
+    blocks.gated_gemm(inner, pre, D.tensor(x), D.tensor(weights), activation="relu")
+    assert capi.last_kernel() == "gated_pairs"
+    x, weights = x.astype(np.float64), weights.astype(np.float64)
+    close(read(pre), x @ weights.T, (width + 4) * UNIT["float"] * (abs(x) @ abs(weights).T) + 2.0 ** -149, 1.0)
+    d = (rng.standard_normal((rows, 1000)) * np.exp2(rng.integers(-40, 40, rows))[:, None]).astype(np.float32)
+    back = (rng.standard_normal((1000, hidden)) * np.exp2(rng.integers(-40, 40, hidden))[None]).astype(np.float32)
+    ones = D.tensor(np.ones((rows, 2 * hidden)))
+    blocks.gated_gemm_gradient(ones, None, D.tensor(d), D.tensor(back), ones, activation="relu")
+    assert capi.last_kernel() == "gated_gradient_pairs"
+    d, back = d.astype(np.float64), back.astype(np.float64)
+    want, bar = d @ back, (1004 + 32) * UNIT["float"] * (abs(d) @ abs(back)) + 2.0 ** -149
+    got = read(ones)
+    close(got[:, :hidden], want, bar, 1.0)
+    close(got[:, hidden:], want, bar, 1.0)
+    D.free()
+
+
+def test_what_is_not_finite_with_two_halves_to_a_float(stream):  # noqa: F811
+    """In rows and columns of both operands; absent rows by all of these."""
+    D = Owned("float")
+    rng = np.random.default_rng(8)
+    rows, width, hidden = 3000, 1000, 2300
+    x = rng.standard_normal((rows, width)).astype(np.float32)
+    weights = rng.standard_normal((2 * hidden, width)).astype(np.float32)
+    x[3, 5], x[300, 7], x[301, 8], x[302, 9] = np.nan, np.inf, -np.inf, np.inf
+    x[302, 10] = -np.inf
+    weights[20, 3], weights[hidden + 40, 4], weights[50, 7] = np.inf, np.nan, 0.0
+    index = np.arange(rows)
+    index[[8, 2999]] = -1, rows
+    inner, pre = D.tensor(np.zeros((rows, hidden))), D.tensor(np.zeros((rows, 2 * hidden)))
+    blocks.gated_gemm(inner, pre, D.tensor(x), D.tensor(weights[None]), D.tensor([0, rows], "int"), D.tensor(index, "int"), activation="relu")
+    assert capi.last_kernel() == "gated_pairs"
+    taken = x.copy()
+    taken[[8, 2999]] = 0
+    with np.errstate(invalid="ignore"):
+        want = taken.astype(np.float64) @ weights.astype(np.float64).T
+    got = read(pre)
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+    rest = np.where(np.isfinite(taken), taken, 0).astype(np.float64)
+    scale = (width + 4) * UNIT["float"] * (abs(rest) @ abs(np.where(np.isfinite(weights), weights, 0)).T.astype(np.float64))
+    assert np.all(abs(got - want)[fine] <= scale[fine])
+    gate, up = got[:, :hidden], got[:, hidden:]
+    with np.errstate(invalid="ignore"):
+        assert np.array_equal(read(inner), np.maximum(gate, 0) * up, equal_nan=True)
+    d, back = x, rng.standard_normal((width, hidden)).astype(np.float32)
+    back[3, 30], back[4, 31] = -np.inf, np.nan
+    ones = D.tensor(np.ones((rows, 2 * hidden)))
+    blocks.gated_gemm_gradient(ones, None, D.tensor(d), D.tensor(back), ones, activation="relu")
+    assert capi.last_kernel() == "gated_gradient_pairs"
+    with np.errstate(invalid="ignore"):
+        want = d.astype(np.float64) @ back.astype(np.float64)
+    got = read(ones)[:, :hidden]
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+    D.free()
 
 
 def test_long_sums_of_doubles(stream):  # noqa: F811
