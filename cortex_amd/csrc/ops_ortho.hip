@@ -46,8 +46,7 @@ struct TilePlace {
 };
 
 template <bool kSymmetric>
-__device__ __forceinline__ bool place_of(const TileOrder& o, TilePlace* p) {
-  const uint32_t unit = unit_of_block(blockIdx.x, o.units);
+__device__ __forceinline__ bool place_of_unit(const TileOrder& o, uint32_t unit, TilePlace* p) {
   if (unit >= o.units) return false;
   uint32_t tile, band, rest;
   o.tiles_fd.divmod(unit, p->matrix, tile);
@@ -64,6 +63,11 @@ __device__ __forceinline__ bool place_of(const TileOrder& o, TilePlace* p) {
     p->m_tile = band * kBand + rest - p->n_tile * rows;
   }
   return true;
+}
+
+template <bool kSymmetric>
+__device__ __forceinline__ bool place_of(const TileOrder& o, TilePlace* p) {
+  return place_of_unit<kSymmetric>(o, unit_of_block(blockIdx.x, o.units), p);
 }
 
 enum Product { kGram, kSquare, kUpdate, kLast };
@@ -358,6 +362,159 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
   }
 }
 
+// Products too small to fill the chip with such tiles: a block owns 32 x 32, its W waves take every W-th of the runs first .. end - 1 each,
+// straight from memory into the operands of v_mfma_f32_16x16x32_f16, whose 16 rows of a piece of a run are 16 times 64 bytes.  Nothing is
+// left out of the products.  The sums of all waves, added in their order: cell i of a lane's, of cells_at(i).
+typedef float pair_f32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kSmallSide = 32, kSmallCells = kSmallSide * kSmallSide;
+
+template <int W>
+__device__ __forceinline__ void small_sums(const char* left, uint32_t last_left, const char* right, uint32_t last_right, int64_t row_bytes, uint32_t first,
+                                           uint32_t end, float (&partial)[W][kSmallCells]) {
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const char *l[2], *r[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    l[t] = left + min(t * 16 + lane % 16, last_left) * row_bytes + lane / 16 * 16;
+    r[t] = right + min(t * 16 + lane % 16, last_right) * row_bytes + lane / 16 * 16;
+  }
+  f16x8 x[2][2][2], y[2][2][2];   // of two runs; [][rows][piece]
+  auto load = [&](uint32_t run, int slot) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        x[slot][t][p] = *reinterpret_cast<const f16x8*>(l[t] + (int64_t)run * kPairRunBytes + p * 64);
+        y[slot][t][p] = *reinterpret_cast<const f16x8*>(r[t] + (int64_t)run * kPairRunBytes + p * 64);
+      }
+  };
+  pair_f32x4 sum[2][2] = {};
+  auto multiply = [&](int slot) {
+#pragma unroll
+    for (int i = 3; i >= 0; --i)   // the smaller products first
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sum[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[slot][t][i / 2], y[slot][u][i % 2], sum[t][u], 0, 0, 0);
+  };
+  const uint32_t mine = first + wave;
+  if (mine < end) load(mine, 0);
+  for (uint32_t run = mine; run < end; run += 2 * W) {
+    if (run + W < end) load(run + W, 1);
+    multiply(0);
+    if (run + W >= end) break;
+    if (run + 2 * W < end) load(run + 2 * W, 0);
+    multiply(1);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) partial[wave][(t * 16 + lane / 16 * 4 + e) * kSmallSide + u * 16 + lane % 16] = sum[t][u][e];
+  __syncthreads();
+}
+
+// A cell's result: to the image, or where it is for.
+template <Product kProduct>
+__device__ __forceinline__ void finish_small(const PairArgs& a, const TilePlace& at, uint32_t cell, float x, uint32_t* image) {
+  const uint32_t row = cell / kSmallSide, column = cell % kSmallSide, m = at.m_tile * kSmallSide + row, n = at.n_tile * kSmallSide + column;
+  x *= a.unscale;
+  if constexpr (kProduct == kLast) {
+    if (m >= a.m || n >= a.n) return;
+    float& to = a.out[at.matrix * a.out_stride + (int64_t)m * a.ldo + n];
+    to = a.beta == 0.f ? a.alpha * x : a.alpha * x + a.beta * to;
+  } else {
+    if constexpr (kProduct == kSquare) {
+      const char* p = a.left + at.matrix * a.left_stride + ((int64_t)min(m, a.m - 1) * a.runs + at.n_tile) * kPairRunBytes + column * 2;
+      _Float16 hi, lo;
+      __builtin_memcpy(&hi, p, 2);
+      __builtin_memcpy(&lo, p + 64, 2);
+      x = a.c * x + a.b * (((float)hi + (float)lo) * a.a_unscale) + (m == n ? a.a : 0.f);
+    }
+    _Float16 hi, lo;
+    split_pair(m < a.m && n < a.n ? x * a.scale : 0.f, &hi, &lo);
+    image[row * kImagePitch + column] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+  }
+}
+
+// Two waves store the image.
+template <Product kProduct>
+__device__ __forceinline__ void store_small(const PairArgs& a, const TilePlace& at, const uint32_t* image) {
+  const uint32_t runs_n = (a.n + kPairRun - 1) / kPairRun, runs_m = (a.m + kPairRun - 1) / kPairRun, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  __syncthreads();
+  if (wave == 0) store_lines(image, lane, false, a.by_rows + at.matrix * a.rows_stride, at.m_tile * kSmallSide, a.m, runs_n, at.n_tile);
+  if (wave == 1 && (!is_symmetric(kProduct) || at.m_tile != at.n_tile))
+    store_lines(image, lane, true, is_symmetric(kProduct) ? a.by_rows + at.matrix * a.rows_stride : a.by_columns + at.matrix * a.columns_stride,
+                at.n_tile * kSmallSide, a.n, runs_m, at.m_tile);
+}
+
+template <int W, Product kProduct>
+__global__ void __launch_bounds__(64 * W, 4) pair_small_kernel(const PairArgs a) {
+  __shared__ float partial[W][kSmallCells];
+  __shared__ __attribute__((aligned(16))) uint32_t image[kImageWords];
+  TilePlace at;
+  if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
+  const int64_t row_bytes = (int64_t)a.runs * kPairRunBytes;
+  const uint32_t row0 = at.m_tile * kSmallSide, column0 = at.n_tile * kSmallSide;
+  small_sums<W>(a.left + at.matrix * a.left_stride + row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + column0 * row_bytes,
+                a.n - 1 - column0, row_bytes, 0, a.runs, partial);
+#pragma unroll
+  for (uint32_t i = threadIdx.x; i < kSmallCells; i += 64 * W) {
+    float x = partial[0][i];
+#pragma unroll
+    for (int w = 1; w < W; ++w) x += partial[w][i];
+    finish_small<kProduct>(a, at, i, x, image);
+  }
+  if constexpr (kProduct != kLast) store_small<kProduct>(a, at, image);
+}
+
+// X X^T of few rows that are long: parts of k to a block each, [matrix][tile][part], and a second launch that adds them up, in their order
+// (40 x 4000 29 us in one launch, 9 in two; thirty-two of 16 x 8000 37 and 13).
+constexpr int kPartWaves = 8;
+__global__ void __launch_bounds__(64 * kPartWaves, 4) gram_part_kernel(const PairArgs a, uint32_t part_runs, FastDiv parts_fd, float* sums, int64_t sums_stride) {
+  __shared__ float partial[kPartWaves][kSmallCells];
+  uint32_t unit, part;
+  parts_fd.divmod(blockIdx.x, unit, part);
+  TilePlace at;
+  if (!place_of_unit<true>(a.order, unit, &at)) return;
+  const int64_t row_bytes = (int64_t)a.runs * kPairRunBytes;
+  const uint32_t row0 = at.m_tile * kSmallSide, column0 = at.n_tile * kSmallSide;
+  const char* x = a.left + at.matrix * a.left_stride;
+  small_sums<kPartWaves>(x + row0 * row_bytes, a.m - 1 - row0, x + column0 * row_bytes, a.n - 1 - column0, row_bytes, part * part_runs,
+                         min((part + 1) * part_runs, a.runs), partial);
+  float* to = sums + at.matrix * sums_stride + ((int64_t)(unit - at.matrix * a.order.tiles) * parts_fd.d + part) * kSmallCells;
+#pragma unroll
+  for (uint32_t i = threadIdx.x; i < kSmallCells; i += 64 * kPartWaves) {
+    float sum = partial[0][i];
+#pragma unroll
+    for (int w = 1; w < kPartWaves; ++w) sum += partial[w][i];
+    to[i] = sum;
+  }
+}
+
+__global__ void __launch_bounds__(256) gram_join_kernel(const PairArgs a, uint32_t parts, const float* sums, int64_t sums_stride) {
+  __shared__ __attribute__((aligned(16))) uint32_t image[kImageWords];
+  TilePlace at;
+  if (!place_of_unit<true>(a.order, blockIdx.x, &at)) return;
+  const float* from = sums + at.matrix * sums_stride + (int64_t)(blockIdx.x - at.matrix * a.order.tiles) * parts * kSmallCells + threadIdx.x;
+  float x[kSmallCells / 256] = {};
+  for (uint32_t part0 = 0; part0 < parts; part0 += 8) {   // loads of eight parts on their way
+    float y[8][kSmallCells / 256];
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+#pragma unroll
+      for (uint32_t i = 0; i < kSmallCells / 256; ++i) y[p][i] = from[(int64_t)min(part0 + p, parts - 1) * kSmallCells + i * 256];
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+#pragma unroll
+      for (uint32_t i = 0; i < kSmallCells / 256; ++i) x[i] += part0 + p < parts ? y[p][i] : 0.f;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kSmallCells / 256; ++i) finish_small<kGram>(a, at, i * 256 + threadIdx.x, x[i], image);
+  store_small<kGram>(a, at, image);
+}
+
 // ------------------------------------------------------------------ double
 
 // Matrices lie as they are given, wide ([m][n], m <= n) or tall ([n][m]).
@@ -462,11 +619,12 @@ int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetr
 
 constexpr int64_t kUnits = 256;
 
-// Microseconds of `tiles` tiles over `runs` runs of 32 k.  Small tiles are bound by what the L2 caches give (13 TB/s), a block to a unit by
-// latency; of 128 a side two blocks share a unit; large ones are bound by the matrix cores, whose clock is higher while some of them
-// rest.  Us of 64, 128 and 256 a side: X X^T of 1024 x 1024 15, 33, 77; 2048 x 2048 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199;
-// 4096 x 8192 720, 527, 471; B X of them 16, 33, 77; 70, 63, 130; 440, 331, 296; 1000, 738, 651.  Within 15 % of all 60 times of which
-// these are a part.
+// Microseconds of `tiles` tiles over `runs` runs of 32 k.  Small tiles are bound by what the L2 caches give, or one to a unit by latency; of
+// 128 a side two blocks share a unit; large ones are bound by the matrix cores, whose clock is higher while some of them rest.  Us of 32,
+// 64, 128 and 256 a side: X X^T of 128 x 784 9.3, 11, 24, 46; 512 x 512 7.5, 9.4; 1024 x 1024 25, 15, 32, 76; 2048 x 2048 64 a side
+// and up 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199; 4096 x 8192 720, 527, 471; B X of 1024 x 1024 33, 16, 33, 77; of the others
+// 70, 63, 130; 440, 331, 296; 1000, 738, 651.  Within 15 % of most of the 100 times of which these are a part.
+double time_of_32(int64_t tiles, int64_t runs) { return 3.4 + 0.245 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
 double time_of_64(int64_t tiles, int64_t runs) { return 5.0 + 0.31 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
 double time_of_128(int64_t tiles, int64_t runs) {
   const int64_t full = tiles / (2 * kUnits), rest = tiles % (2 * kUnits);
@@ -477,6 +635,15 @@ double time_of_256(int64_t tiles, int64_t runs) {
   return 14.0 * (double)(full + (rest > 0)) + (double)runs * (2.5 * (double)full + (rest > 0 ? 1.75 + 0.75 * (double)rest / kUnits : 0.0));
 }
 
+double time_of_gram(int64_t count, int64_t m, int64_t runs) {
+  auto tiles = [&](int64_t side) { return tiles_of(count, m, m, side, true); };
+  return std::min({time_of_32(tiles(kSmallSide), runs), time_of_64(tiles(64), runs), time_of_128(tiles(128), runs), time_of_256(tiles(256), runs)});
+}
+// With parts of k and the launch that joins them.
+double time_of_parts(int64_t count, int64_t m, int64_t runs, int64_t parts) {
+  return time_of_32(tiles_of(count, m, m, kSmallSide, true) * parts, ceil_div(runs, parts)) + 5.0;
+}
+
 template <class Tile, Product kProduct>
 void launch_tile(hipStream_t s, PairArgs a, int64_t count) {
   a.order = order_of(count, a.m, a.n, Tile::S, is_symmetric(kProduct));
@@ -484,10 +651,33 @@ void launch_tile(hipStream_t s, PairArgs a, int64_t count) {
 }
 
 template <Product kProduct>
+void launch_small(hipStream_t s, PairArgs a, int64_t count) {
+  a.order = order_of(count, a.m, a.n, kSmallSide, is_symmetric(kProduct));
+  if (a.runs <= 4) hipLaunchKernelGGL((pair_small_kernel<4, kProduct>), grid_of(a.order), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((pair_small_kernel<8, kProduct>), grid_of(a.order), dim3(512), 0, s, a);
+}
+
+// How many parts the k of X X^T is divided into, in the room of a matrix's `bytes`: blocks for half the chip, a run to a wave at least.
+int64_t gram_parts(int64_t count, int64_t m, int64_t runs, int64_t bytes) {
+  const int64_t tiles = tiles_of(1, m, m, kSmallSide, true);
+  return std::min({2 * kUnits / (count * tiles), ceil_div(runs, kPartWaves), bytes / (tiles * (int64_t)kSmallCells * 4)});
+}
+
+void launch_gram_parts(hipStream_t s, PairArgs a, int64_t count, int64_t parts, void* room, int64_t room_bytes) {
+  a.order = order_of(count, a.m, a.n, kSmallSide, true);
+  const uint32_t part_runs = (uint32_t)ceil_div(a.runs, parts);
+  parts = ceil_div(a.runs, part_runs);
+  float* const sums = static_cast<float*>(room);
+  hipLaunchKernelGGL(gram_part_kernel, dim3((uint32_t)(a.order.units * parts)), dim3(64 * kPartWaves), 0, s, a, part_runs, FastDiv((uint32_t)parts), sums, room_bytes / 4);
+  hipLaunchKernelGGL(gram_join_kernel, dim3(a.order.units), dim3(256), 0, s, a, (uint32_t)parts, sums, room_bytes / 4);
+}
+
+template <Product kProduct>
 void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
   auto tiles = [&](int64_t side) { return tiles_of(count, a.m, a.n, side, is_symmetric(kProduct)); };
   const double small = time_of_64(tiles(64), a.runs), medium = time_of_128(tiles(128), a.runs), large = time_of_256(tiles(256), a.runs);
-  if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
+  if (time_of_32(tiles(kSmallSide), a.runs) <= std::min({small, medium, large})) launch_small<kProduct>(s, a, count);
+  else if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
   else if (medium <= large) launch_tile<Tile128, kProduct>(s, a, count);
   else launch_tile<Tile256, kProduct>(s, a, count);
 }
@@ -587,7 +777,11 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
       g.by_rows = gram;
       g.rows_stride = l.square;
       g.scale = a_scale;
-      launch_pair<kGram>(s, g, count);
+      // X by columns lies in one of two places; the other is free
+      const int64_t parts = gram_parts(count, l.m, g.runs, l.turned);
+      if (parts > 1 && time_of_parts(count, l.m, g.runs, parts) < time_of_gram(count, l.m, g.runs))
+        launch_gram_parts(s, g, count, parts, turned[(step + 1) & 1], l.turned);
+      else launch_pair<kGram>(s, g, count);
       g.left = g.right = gram;
       g.left_stride = g.right_stride = l.square;
       g.runs = (uint32_t)ceil_div(l.m, kPairRun);
