@@ -686,9 +686,9 @@ constexpr int kPairM = 128, kPairN = 128, kPairWavesM = 2, kPairWavesN = 2;
 // Microseconds beyond the products' for a round of blocks, whose results' bytes bound it: with three pieces, and with two halves.
 constexpr double end_of_round(bool pairs, bool gradient) { return pairs ? (gradient ? 36.0 : 10.0) : (gradient ? 25.0 : 12.0); }
 
-// Microseconds with two halves to a float: the splitting at 3.5 TB/s, rounds of blocks, two to a unit or in the last one by themselves.
-double time_of_pairs(const Shape& s, int64_t left_rows, bool gradient) {
-  const int64_t right = s.groups * s.stored, blocks = s.blocks(kPairM, kPairN), full = blocks / (2 * kUnits), rest = blocks % (2 * kUnits);
+// Microseconds with two halves to a float: the splitting, of all groups' weights, at 3.5 TB/s; rounds of blocks, two to a unit or in the last one by themselves.
+double time_of_pairs(const Shape& s, int64_t left_rows, int64_t all_groups, bool gradient) {
+  const int64_t right = all_groups * s.stored, blocks = s.blocks(kPairM, kPairN), full = blocks / (2 * kUnits), rest = blocks % (2 * kUnits);
   const double split = (double)s.k * (8.0 * (double)left_rows + (gradient ? 12.0 : 8.0) * (double)right) / 3.5e6;
   const double end = end_of_round(true, gradient), runs = (double)ceil_div(s.k, kPairRun);
   return 10.0 + split + (double)full * (end + 1.38 * runs) + (rest == 0 ? 0.0 : rest <= kUnits ? 0.6 * end + 0.8 * runs : end + 1.38 * runs);
@@ -757,7 +757,7 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
     const int64_t left_rows = a.g.a_rows;
     double us = best.us;
     if (best.height == 128) us += end_of_round(false, kGradient) * (double)ceil_div(shape.blocks(128, 128) * best.parts, kUnits);
-    if (shape.k >= kPairRun && time_of_pairs(shape, left_rows, kGradient) < us && run_pairs<kGradient>(s, a, shape, left_rows, a.g.groups)) {
+    if (shape.k >= kPairRun && time_of_pairs(shape, left_rows, a.g.groups, kGradient) < us && run_pairs<kGradient>(s, a, shape, left_rows, a.g.groups)) {
       note_kernel(kGradient ? "gated_gradient_pairs" : "gated_pairs");
       return after_launch(s);
     }

@@ -19,6 +19,7 @@
 
 #include "common.h"
 #include "double_tile.h"
+#include "ortho.h"
 #include "pair_tile.h"
 #include "rows.h"
 
@@ -75,27 +76,7 @@ constexpr bool is_symmetric(Product p) { return p == kGram || p == kSquare; }
 
 // ------------------------------------------------------------------ the norm, and the matrix divided by it
 
-// What a step begins with: of ct_orthogonalize a matrix x; of ct_muon_step the momentum x, which takes up the gradient.
-struct StartArgs {
-  const void* x;
-  const void* gradient;      // of a step, else null
-  void* momentum;            // x itself, of a step
-  double* partial;           // [matrix][kParts]
-  int64_t ld, stride;
-  uint32_t rows, columns;
-  double gradient_alpha, decay, epsilon;   // decay: of the momentum
-  bool nesterov;
-};
-
 constexpr uint32_t kParts = 1024;
-
-// What is made orthogonal: the matrix, the momentum, or what it will be after another such gradient.
-template <class T>
-__device__ __forceinline__ T start_value(const StartArgs& a, int64_t at) {
-  const T x = static_cast<const T*>(a.x)[at];
-  if (!a.gradient || !a.nesterov) return x;
-  return (T)a.gradient_alpha * static_cast<const T*>(a.gradient)[at] + (T)a.decay * x;
-}
 
 __device__ __forceinline__ double sum_of_block(double x, double* lds) {
 #pragma unroll
@@ -592,6 +573,7 @@ struct Layout {
     }
     partial = kParts * 8;
     matrix = (dtype == CT_F32 ? x : 0) + 2 * turned + 2 * square + partial;
+    if (dtype == CT_F32 && m <= kMostFew) matrix = std::max(matrix, aligned(few_bytes(m, n)));
   }
 };
 
@@ -753,10 +735,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);
     StartArgs start = r.start;
-    const int64_t offset = first * start.stride * 4;
-    start.x = static_cast<const char*>(start.x) + offset;
-    if (start.gradient) start.gradient = static_cast<const char*>(start.gradient) + offset;
-    if (start.momentum) start.momentum = static_cast<char*>(start.momentum) + offset;
+    start.move(first * start.stride * 4);
     start.partial = partial;
     hipLaunchKernelGGL((start_norm_kernel<float>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
                        start.ld == r.columns);
@@ -843,10 +822,7 @@ int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);
     StartArgs start = r.start;
-    const int64_t offset = first * start.stride * 8;
-    start.x = static_cast<const char*>(start.x) + offset;
-    if (start.gradient) start.gradient = static_cast<const char*>(start.gradient) + offset;
-    if (start.momentum) start.momentum = static_cast<char*>(start.momentum) + offset;
+    start.move(first * start.stride * 8);
     start.partial = partial;
     hipLaunchKernelGGL((start_norm_kernel<double>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
                        start.ld == r.columns);
@@ -906,11 +882,12 @@ int run(const char* name, hipStream_t s, Request r) {
   CT_REQUIRE(r.steps >= 1 && r.steps <= kMostSteps, "%s: %d steps, 1 to %d are taken", name, r.steps, kMostSteps);
   CT_REQUIRE(r.coefficients, "%s: null coefficients", name);
   CT_REQUIRE(r.start.epsilon >= 0, "%s: epsilon must not be negative", name);
-  double bound = 1.0;
+  double bound = 1.0, change = 1.0;   // of the largest singular value; of what X X^T is off by
   for (int step = 0; step < r.steps; ++step) {
     const double* k = r.coefficients + 3 * step;
     CT_REQUIRE(std::isfinite(k[0]) && std::isfinite(k[1]) && std::isfinite(k[2]), "%s: coefficients must be finite", name);
     const double factor = most_of_factor(k[0], k[1], k[2], bound * bound);
+    change *= std::max(1.0, factor * most_of_factor(k[0], 3 * k[1], 5 * k[2], bound * bound));   // (s (a + b s + c s^2)^2)' is that
     bound = most_of_step(k[0], k[1], k[2], bound * bound);
     CT_REQUIRE(factor <= kMostValue && bound <= kMostValue, "%s: with these coefficients singular values grow beyond 2^40", name);
   }
@@ -926,7 +903,17 @@ int run(const char* name, hipStream_t s, Request r) {
   const Run x = run_of(r.start.x, r.start.ld, r.start.stride), gradient = run_of(r.start.gradient, r.start.ld, r.start.stride);
   const Run out = run_of(r.out, r.ldo, r.out_stride);
   CT_REQUIRE(!runs_meet(work, x) && !runs_meet(work, gradient) && !runs_meet(work, out), "%s: the workspace overlaps an operand", name);
-  return r.dtype == CT_F32 ? run_float(s, r, l, at_once) : run_double(s, r, l, at_once);
+  if (r.dtype == CT_F64) return run_double(s, r, l, at_once);
+  if (l.m > kMostFew || change > kMostFewChange) return run_float(s, r, l, at_once);
+  FewMatrices few{r.start, static_cast<char*>(r.workspace), l.matrix, static_cast<float*>(r.out), r.ldo, r.out_stride, (float)r.alpha, (float)r.beta, r.coefficients,
+                  r.steps};
+  for (int64_t first = 0; first < r.count; first += at_once) {
+    ortho_few(s, few, std::min(at_once, r.count - first));
+    few.start.move(at_once * few.start.stride * 4);
+    few.out += at_once * few.out_stride;
+  }
+  note_kernel("orthogonalize_few");
+  return after_launch(s);
 }
 
 }  // namespace

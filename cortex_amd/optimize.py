@@ -192,6 +192,8 @@ def _packed_matrices(name: str, what: str, x, shape):
 
 def _steps_of(coefficients, steps: int) -> bytes:
     """Three doubles to a step: of one triple for all steps, or of one to each."""
+    if not len(coefficients):
+        raise ValueError("coefficients: none")
     triples = [tuple(map(float, c)) for c in coefficients] if hasattr(coefficients[0], "__len__") else [tuple(map(float, coefficients))] * int(steps)
     if len(triples) != int(steps) or any(len(c) != 3 for c in triples):
         raise ValueError(f"coefficients: three numbers, or three to each of {steps} steps")

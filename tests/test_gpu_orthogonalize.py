@@ -201,6 +201,42 @@ def test_coefficients(D, coefficients):
         near(read(out)[i], want, bar + 16 * D.u * np.linalg.norm(want))
 
 
+@pytest.mark.parametrize("shape", [(1, 3, 2000), (2, 2000, 3), (2, 16, 129), (3, 17, 1000), (1, 1000, 17), (2, 48, 300), (1, 300, 48), (2, 49, 70), (1, 64, 5001),
+                                   (2, 5001, 64), (5, 64, 64)], ids=str)
+def test_few_rows(D, shape):
+    """Added to what is there, rows apart."""
+    rng = np.random.default_rng(20)
+    count, rows, columns = shape
+    whole, target = rng.standard_normal((count, rows, columns + 5)), rng.standard_normal((count, rows, columns + 3))
+    whole[:, :, :columns] = gradient(rng, *shape)
+    g, out = D.tensor(whole), D.tensor(target)
+    before, values = read(out), read(g)
+    need = D.backend.stream.orthogonalize_workspace(count, rows, columns, D.backend.datatype)
+    workspace = D.backend.stream.get_device().allocate_device_buffer(need, "byte")
+    D.backend.stream.orthogonalize(optimize._buffer(out), columns + 3, rows * (columns + 3), 0.5, optimize._buffer(g), columns + 5, rows * (columns + 5), 0.25,
+                                   count, rows, columns, optimize._steps_of(COEFFICIENTS, 5), 1e-7, workspace)
+    got = read(out)
+    workspace.release()
+    assert np.array_equal(got[:, :, columns:], before[:, :, columns:])
+    for i in range(count):
+        want, bar = bar_of(values[i, :, :columns], D.u)
+        want = 0.5 * want + 0.25 * before[i, :, :columns]
+        near(got[i, :, :columns], want, 0.5 * bar + 4 * D.u * np.linalg.norm(abs(want) + abs(before[i, :, :columns])))
+
+
+@pytest.mark.parametrize("steps", [5, 6, 7, 12, 25, 64])
+@pytest.mark.parametrize("shape", [(20, 90), (90, 64), (100, 200)], ids=str)
+def test_many_steps_of_a_singular_matrix(D, shape, steps):
+    """Singular values of 0, which rounding makes others of: all stay below what the steps allow, 1.2024, and a little for rounding."""
+    rng = np.random.default_rng(21)
+    values = gradient(rng, 1, *shape)[0]
+    values[: shape[0] // 2] = values[shape[0] // 2: 2 * (shape[0] // 2)]
+    g, out = D.tensor(values), D.tensor(np.zeros(shape))
+    optimize.orthogonalize(D.backend, out, g, steps=steps)
+    got = read(out).astype(np.float64)
+    assert np.all(np.isfinite(got)) and np.linalg.svd(got, compute_uv=False).max() < 1.21
+
+
 def test_singular_values_end_near_one(D):
     rng = np.random.default_rng(10)
     g, out = D.tensor(rng.standard_normal((96, 200))), D.tensor(np.zeros((96, 200)))

@@ -116,6 +116,7 @@ def matrix(*shape, strides=None, datatype="float", device=None):
     (ValueError, "differ", matrix(3, 4), matrix(4, 3), {}), (ValueError, "contiguous", matrix(3, 4, strides=[1, 3]), matrix(3, 4), {}),
     (ValueError, "contiguous", matrix(3, 4), matrix(3, 4, strides=[3, 1]), {}), (TypeError, "datatype", matrix(3, 4, datatype="double"), matrix(3, 4), {}),
     (ValueError, "same device", matrix(3, 4, device=Device()), matrix(3, 4), {}), (ValueError, "three numbers", matrix(3, 4), matrix(3, 4), {"coefficients": (1.0, 2.0)}),
+    (ValueError, "none", matrix(3, 4), matrix(3, 4), {"coefficients": ()}),
     (ValueError, "three numbers", matrix(3, 4), matrix(3, 4), {"coefficients": [(1.0, 2.0, 3.0)] * 4})], ids=str)
 def test_tensors(error, message, output, input, kwargs):
     with pytest.raises(error, match=message):
