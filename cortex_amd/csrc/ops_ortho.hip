@@ -46,12 +46,22 @@ struct TilePlace {
   uint32_t matrix, m_tile, n_tile;
 };
 
-template <bool kSymmetric>
+// kTall: tiles of a symmetric product are 4 high by 3 wide, not square.
+template <bool kSymmetric, bool kTall = false>
 __device__ __forceinline__ bool place_of_unit(const TileOrder& o, uint32_t unit, TilePlace* p) {
   if (unit >= o.units) return false;
   uint32_t tile, band, rest;
   o.tiles_fd.divmod(unit, p->matrix, tile);
-  if constexpr (kSymmetric) {
+  if constexpr (kSymmetric && kTall) {   // of three rows of tiles the q-th have 4 q + 2, 4 q + 3 and 4 q + 4, those before them 6 q q + 3 q
+    auto before = [](uint32_t q) { return 6 * q * q + 3 * q; };
+    uint32_t q = (uint32_t)((sqrtf(24.f * (float)tile + 9.f) - 3.f) * (1.f / 12.f));   // may be one off
+    if (before(q) > tile) --q;
+    if (before(q + 1) <= tile) ++q;
+    rest = tile - before(q);
+    const uint32_t row = rest < 4 * q + 2 ? 0 : rest < 8 * q + 5 ? 1 : 2;
+    p->m_tile = 3 * q + row;
+    p->n_tile = rest - (row == 0 ? 0 : row == 1 ? 4 * q + 2 : 8 * q + 5);
+  } else if constexpr (kSymmetric) {
     uint32_t i = (uint32_t)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);   // may be one off
     if (i * (i + 1) / 2 > tile) --i;
     if ((i + 1) * (i + 2) / 2 <= tile) ++i;
@@ -66,9 +76,9 @@ __device__ __forceinline__ bool place_of_unit(const TileOrder& o, uint32_t unit,
   return true;
 }
 
-template <bool kSymmetric>
+template <bool kSymmetric, bool kTall = false>
 __device__ __forceinline__ bool place_of(const TileOrder& o, TilePlace* p) {
-  return place_of_unit<kSymmetric>(o, unit_of_block(blockIdx.x, o.units), p);
+  return place_of_unit<kSymmetric, kTall>(o, unit_of_block(blockIdx.x, o.units), p);
 }
 
 enum Product { kGram, kSquare, kUpdate, kLast };
@@ -207,14 +217,17 @@ struct PairArgs {
   float alpha, beta;
 };
 
-// Tiles of S x S by WM x WN waves, loads kAhead runs ahead.
-template <int S_, int WM_, int WN_, int kAhead_>
+// Tiles of SM x SN by WM x WN waves, loads kAhead runs ahead.
+template <int SM_, int SN_, int WM_, int WN_, int kAhead_>
 struct PairTile {
-  static constexpr int S = S_, WM = WM_, WN = WN_, kAhead = kAhead_, T = 64 * WM * WN, MT = S / WM / 32, NT = S / WN / 32;
+  static constexpr int SM = SM_, SN = SN_, WM = WM_, WN = WN_, kAhead = kAhead_, T = 64 * WM * WN, MT = SM / WM / 32, NT = SN / WN / 32;
+  static constexpr bool kTall = SM != SN;
+  static_assert(!kTall || SM * 3 == SN * 4, "what place_of_unit counts");
 };
-using Tile256 = PairTile<256, 2, 4, 1>;
-using Tile128 = PairTile<128, 2, 2, 1>;
-using Tile64 = PairTile<64, 2, 2, 2>;
+using Tile256 = PairTile<256, 256, 2, 4, 1>;
+using TileTall = PairTile<256, 192, 4, 2, 1>;
+using Tile128 = PairTile<128, 128, 2, 2, 1>;
+using Tile64 = PairTile<64, 64, 2, 2, 2>;
 
 // Results of a wave's 32 x 32 cells go to memory in whole lines: by way of an image in LDS, rows of 32 with both pieces in a word,
 // from which eight lanes take a run of a row, or of a column.  (Stored from the registers a line of 128 bytes took 16 instructions of a few
@@ -255,18 +268,19 @@ __device__ __forceinline__ void store_lines(const uint32_t* image, uint32_t lane
 
 template <class Tile, Product kProduct>
 __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
-  constexpr int S = Tile::S, WM = Tile::WM, WN = Tile::WN, MT = Tile::MT, NT = Tile::NT;
-  __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(S, S)];
-  static_assert(WM * WN * kImageWords * 4 <= pair_tile_lds(S, S), "an image to a wave");
+  constexpr int SM = Tile::SM, SN = Tile::SN, WM = Tile::WM, WN = Tile::WN, MT = Tile::MT, NT = Tile::NT;
+  __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(SM, SN)];
+  static_assert(WM * WN * kImageWords * 4 <= pair_tile_lds(SM, SN), "an image to a wave");
   TilePlace at;
-  if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
+  if (!place_of<is_symmetric(kProduct), Tile::kTall>(a.order, &at)) return;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const uint32_t row0 = at.m_tile * S, column0 = at.n_tile * S, row_bytes = a.runs * kPairRunBytes;
+  const uint32_t row0 = at.m_tile * SM, column0 = at.n_tile * SN, row_bytes = a.runs * kPairRunBytes;
+  if (Tile::kTall && column0 >= a.n) return;   // a last row of tiles may be counted longer than it is
   const char* left = a.left + at.matrix * a.left_stride;
   pair_f32x16 sums[1][MT][NT];
-  const PairMatrices<S, S, Tile::T> source(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
+  const PairMatrices<SM, SN, Tile::T> source(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
                                            a.n - 1 - column0, row_bytes, tid);
-  pair_tile<S, S, WM, WN, Tile::kAhead, false>(source, a.runs, lds, tid, sums);
+  pair_tile<SM, SN, WM, WN, Tile::kAhead, false>(source, a.runs, lds, tid, sums);
   pair_f32x16 (&sum)[MT][NT] = sums[0];
   const uint32_t wave_m = row0 + wave / WN * (MT * 32), wave_n = column0 + wave % WN * (NT * 32), c = lane & 31, half = lane >> 5;
   if constexpr (kProduct == kLast) {
@@ -304,7 +318,7 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         const uint32_t m0 = wave_m + t * 32, n0 = wave_n + u * 32;
-        if (m0 >= a.m || n0 >= a.n) continue;
+        if (m0 >= a.m || n0 >= a.n || (is_symmetric(kProduct) && m0 < n0)) continue;
         if constexpr (kProduct == kSquare) {   // A's lines as they are, 144 bytes apart
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
         }
         wave_fence();
         store_lines(image, lane, false, by_rows, m0, a.m, runs_n, n0 / 32);
-        if (!is_symmetric(kProduct) || at.m_tile != at.n_tile) store_lines(image, lane, true, by_columns, n0, a.n, runs_m, m0 / 32);
+        if (!is_symmetric(kProduct) || m0 > n0) store_lines(image, lane, true, by_columns, n0, a.n, runs_m, m0 / 32);
         wave_fence();
       }
   }
@@ -580,10 +594,20 @@ struct Layout {
 // Matrices beyond this many cells take turns: by then each launch fills the chip.
 constexpr int64_t kCellsAtOnce = int64_t(1) << 26;
 
-TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) {
+// Of a symmetric product the tiles at and below the diagonal.
+int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t height, int64_t width, bool symmetric) {
+  const int64_t mt = ceil_div(m, height), nt = ceil_div(n, width);
+  if (!symmetric) return count * mt * nt;
+  if (height == width) return count * (mt * (mt + 1) / 2);
+  const int64_t q = mt / 3, r = mt % 3;   // as place_of_unit counts them
+  return count * (6 * q * q + 3 * q + (r == 0 ? 0 : r == 1 ? 4 * q + 2 : 8 * q + 5));
+}
+int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) { return tiles_of(count, m, n, side, side, symmetric); }
+
+TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t height, int64_t width, bool symmetric) {
   TileOrder o;
-  const int64_t mt = ceil_div(m, side), nt = ceil_div(n, side), tiles = symmetric ? mt * (mt + 1) / 2 : mt * nt;
-  o.m_tiles = (uint32_t)mt;
+  const int64_t tiles = tiles_of(1, m, n, height, width, symmetric), nt = ceil_div(n, width);
+  o.m_tiles = (uint32_t)ceil_div(m, height);
   o.n_tiles = (uint32_t)nt;
   o.tiles = (uint32_t)tiles;
   o.units = (uint32_t)(count * tiles);
@@ -591,13 +615,9 @@ TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symme
   o.band_fd = FastDiv((uint32_t)(kBand * nt));
   return o;
 }
+TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) { return order_of(count, m, n, side, side, symmetric); }
 
 dim3 grid_of(const TileOrder& o) { return dim3((uint32_t)(ceil_div(o.units, kXcds) * kXcds)); }
-
-int64_t tiles_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) {
-  const int64_t mt = ceil_div(m, side), nt = ceil_div(n, side);
-  return count * (symmetric ? mt * (mt + 1) / 2 : mt * nt);
-}
 
 constexpr int64_t kUnits = 256;
 
@@ -616,10 +636,17 @@ double time_of_256(int64_t tiles, int64_t runs) {
   const int64_t full = tiles / kUnits, rest = tiles % kUnits;
   return 14.0 * (double)(full + (rest > 0)) + (double)runs * (2.5 * (double)full + (rest > 0 ? 1.75 + 0.75 * (double)rest / kUnits : 0.0));
 }
+// 256 by 192, of symmetric products: in whole calls X X^T of 4096 x 8192, 187 tiles, takes 480 us (136 of 256 a side 527), of sixteen 1024 x 2816,
+// 240 tiles, 200 (160, 223); a call of 4096 x 4096 4086 (of 128 and 256 a side 4612, 4475).
+double time_of_tall(int64_t tiles, int64_t runs) {
+  const int64_t full = tiles / kUnits, rest = tiles % kUnits;
+  return 12.0 * (double)(full + (rest > 0)) + (double)runs * (1.95 * (double)full + (rest > 0 ? 1.05 + 0.95 * (double)rest / kUnits : 0.0));
+}
 
 double time_of_gram(int64_t count, int64_t m, int64_t runs) {
   auto tiles = [&](int64_t side) { return tiles_of(count, m, m, side, true); };
-  return std::min({time_of_32(tiles(kSmallSide), runs), time_of_64(tiles(64), runs), time_of_128(tiles(128), runs), time_of_256(tiles(256), runs)});
+  return std::min({time_of_32(tiles(kSmallSide), runs), time_of_64(tiles(64), runs), time_of_128(tiles(128), runs),
+                   time_of_tall(tiles_of(count, m, m, 256, 192, true), runs), time_of_256(tiles(256), runs)});
 }
 // With parts of k and the launch that joins them.
 double time_of_parts(int64_t count, int64_t m, int64_t runs, int64_t parts) {
@@ -628,7 +655,7 @@ double time_of_parts(int64_t count, int64_t m, int64_t runs, int64_t parts) {
 
 template <class Tile, Product kProduct>
 void launch_tile(hipStream_t s, PairArgs a, int64_t count) {
-  a.order = order_of(count, a.m, a.n, Tile::S, is_symmetric(kProduct));
+  a.order = order_of(count, a.m, a.n, Tile::SM, Tile::SN, is_symmetric(kProduct));
   hipLaunchKernelGGL((pair_kernel<Tile, kProduct>), grid_of(a.order), dim3(Tile::T), 0, s, a);
 }
 
@@ -658,6 +685,10 @@ template <Product kProduct>
 void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
   auto tiles = [&](int64_t side) { return tiles_of(count, a.m, a.n, side, is_symmetric(kProduct)); };
   const double small = time_of_64(tiles(64), a.runs), medium = time_of_128(tiles(128), a.runs), large = time_of_256(tiles(256), a.runs);
+  if constexpr (is_symmetric(kProduct)) {
+    const double tall = time_of_tall(tiles_of(count, a.m, a.n, 256, 192, true), a.runs);
+    if (tall < std::min({time_of_32(tiles(kSmallSide), a.runs), small, medium, large})) return launch_tile<TileTall, kProduct>(s, a, count);
+  }
   if (time_of_32(tiles(kSmallSide), a.runs) <= std::min({small, medium, large})) launch_small<kProduct>(s, a, count);
   else if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
   else if (medium <= large) launch_tile<Tile128, kProduct>(s, a, count);

@@ -110,7 +110,7 @@ def test_every_tile(stream, as_released):  # noqa: F811
     D = Owned("float")
     backend = optimize.Backend(stream, "float")
     rng = np.random.default_rng(8)
-    for shape in ((40, 70, 200), (24, 400, 300), (20, 1100, 1030)):
+    for shape in ((40, 70, 200), (24, 400, 300), (28, 760, 1000), (20, 1100, 1030)):
         one = gradient(rng, 1, *shape[1:])
         scales = 2.0 ** rng.integers(-3, 4, shape[0])      # a power of two in front changes no bit but for epsilon
         g, out = D.tensor(one * scales[:, None, None]), D.tensor(np.zeros(shape))
