@@ -752,6 +752,8 @@ struct Request {
 };
 
 constexpr double kMostValue = 0x1p40;
+// Of floats, whose A A has values of the fourth power, before the last step; and what A is multiplied by to leave its scale is a float.
+constexpr double kMostFloat = 0x1p30;
 
 int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once) {
   const bool tall = r.rows > r.columns;
@@ -913,15 +915,17 @@ int run(const char* name, hipStream_t s, Request r) {
   CT_REQUIRE(r.steps >= 1 && r.steps <= kMostSteps, "%s: %d steps, 1 to %d are taken", name, r.steps, kMostSteps);
   CT_REQUIRE(r.coefficients, "%s: null coefficients", name);
   CT_REQUIRE(r.start.epsilon >= 0, "%s: epsilon must not be negative", name);
-  double bound = 1.0, change = 1.0;   // of the largest singular value; of what X X^T is off by
+  double bound = 1.0, before_last = 1.0, change = 1.0;   // of the largest singular value; of what X X^T is off by
   for (int step = 0; step < r.steps; ++step) {
     const double* k = r.coefficients + 3 * step;
     CT_REQUIRE(std::isfinite(k[0]) && std::isfinite(k[1]) && std::isfinite(k[2]), "%s: coefficients must be finite", name);
+    before_last = std::max(before_last, bound);
     const double factor = most_of_factor(k[0], k[1], k[2], bound * bound);
     change *= std::max(1.0, factor * most_of_factor(k[0], 3 * k[1], 5 * k[2], bound * bound));   // (s (a + b s + c s^2)^2)' is that
     bound = most_of_step(k[0], k[1], k[2], bound * bound);
     CT_REQUIRE(factor <= kMostValue && bound <= kMostValue, "%s: with these coefficients singular values grow beyond 2^40", name);
   }
+  CT_REQUIRE(r.dtype == CT_F64 || before_last <= kMostFloat, "%s: with these coefficients singular values grow beyond 2^30 before the last step", name);
   if (r.count == 0 || r.rows == 0 || r.columns == 0) return CT_OK;
   const Layout l(r.rows, r.columns, r.dtype);
   CT_REQUIRE(r.workspace && (reinterpret_cast<uintptr_t>(r.workspace) & 15) == 0, "%s: the workspace must be a buffer, aligned to 16 bytes", name);

@@ -48,6 +48,16 @@ def test_orthogonalize(message, change):
     refuses(message, "ct_orthogonalize", *orthogonalize(**change))
 
 
+@pytest.mark.parametrize("coefficients", [(2.0 ** 31, 0.0, 0.0, 1.0, 0.0, 0.0), (2.0 ** 33, 0.0, 0.0, 0.5, 0.0, 0.0, 2.0, 0.0, 0.0)], ids=str)
+def test_singular_values_whose_fourth_power_is_no_float(coefficients):
+    """A A of a singular value of 2^33 is 2^132, which a float does not hold; as the last step's result that value may be."""
+    change = {"coefficients": of(*coefficients), "steps": len(coefficients) // 3}
+    refuses("beyond 2^30 before the last step", "ct_orthogonalize", *orthogonalize(**change))
+    refuses("beyond 2^30 before the last step", "ct_muon_step", *step(**change))
+    for allowed in (orthogonalize(coefficients=of(*coefficients), steps=1, workspace=None), orthogonalize(dtype=capi.F64, workspace=None, **change)):
+        refuses("workspace must be", "ct_orthogonalize", *allowed)
+
+
 def step(**change):
     args = dict(stream=None, dtype=capi.F32, alpha=0.02, momentum=0.95, nesterov=1, weight_decay=0.0, gradient_alpha=1.0, coefficients=TRIPLES, steps=5,
                 epsilon=1e-7, gradient=A[0], parameters=A[1], momentum_vals=A[2], count=2, rows=30, columns=40, workspace=A[3], workspace_bytes=ROOM)
