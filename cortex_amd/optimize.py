@@ -222,7 +222,7 @@ def orthogonalize(backend: Backend, output, input, *, alpha=1.0, beta=0.0, steps
     if of_input[:3] != of_output[:3]:
         raise ValueError(f"{name}: output {list(output.shape())} and input {list(input.shape())} differ")
     _ensure_datatype(backend.datatype, output.buffer, input.buffer)
-    if output.buffer.device is not input.buffer.device:
+    if any(x.device is not output.buffer.device for x in (input.buffer, *([] if workspace is None else [_buffer(workspace)]))):
         raise ValueError(f"{name}: buffers are not all on the same device")
     steps_of = _steps_of(coefficients, steps)
     own = workspace is None

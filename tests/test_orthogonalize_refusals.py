@@ -144,3 +144,8 @@ def test_optimizer(error, message, gradient, parameters, momentum):
         optimizer.compute_parameters({"momentum-vals": momentum}, 1.0, 0, gradient, parameters)
     with pytest.raises(TypeError):
         optimize.create_optimizer(optimize.Backend(None, "int"), optimize.muon())
+
+
+def test_a_workspace_of_another_device():
+    with pytest.raises(ValueError, match="same device"):
+        optimize.orthogonalize(optimize.Backend(None, "float"), matrix(3, 4), matrix(3, 4), workspace=Buffer(1 << 20, "byte", Device()))
