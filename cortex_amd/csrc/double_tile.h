@@ -147,4 +147,116 @@ __device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right rig
       for (int r = 0; r < 4; ++r) store(wave_m + t * 16 + lane / 16 + 4 * r, wave_n + u * 16 + lane % 16, sum[t][u][r]);
 }
 
+// Small products: a block owns 32 x 32, its W waves take every W-th run of 16 k each, straight from memory into the matrix cores'
+// operands, the next run's loads on their way meanwhile, and leave their sums in LDS.  Nothing waits for another wave before that: five of
+// 301 x 517 times their transposes 16 us, in tiles of 32 by way of LDS 19 (with eight waves 18.6).  A lane's four k of a run are lane / 16 * 4 and those behind it; sixteen lanes' rows, or
+// columns, of t are t * 16 and those behind it.
+constexpr uint32_t kDirectSide = 32, kDirectPitch = 33, kDirectRun = 16;
+
+template <bool kByRow>
+struct DoubleDirect {
+  const double* p[2];   // a lane's row, from k 0 on, or its column
+  int64_t ld;           // of columns
+  bool present[2];
+  // `row(i)`: which one is row i of the tile's
+  template <class Row>
+  static __device__ __forceinline__ DoubleDirect rows(const double* p, int64_t ld, Row row) {
+    DoubleDirect d;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t i = row(t * 16 + threadIdx.x % 16);
+      d.present[t] = i >= 0;
+      d.p[t] = p + (i < 0 ? 0 : i) * ld;
+    }
+    d.ld = ld;
+    return d;
+  }
+  static __device__ __forceinline__ DoubleDirect columns(const double* p, int64_t ld, uint32_t left) {   // of `left` columns
+    DoubleDirect d;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      d.present[t] = true;
+      d.p[t] = p + min(t * 16 + threadIdx.x % 16, left - 1);
+    }
+    d.ld = ld;
+    return d;
+  }
+  __device__ __forceinline__ void load(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
+    const uint32_t k = k0 + threadIdx.x % 64 / 16 * 4;
+    if (kByRow && k0 + kDirectRun <= end) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const f64x2 two = *reinterpret_cast<const f64x2_at_8*>(p[t] + k + e);
+          x[t][e] = two[0];
+          x[t][e + 1] = two[1];
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[t][e] = p[t][min(k + e, end - 1) * (kByRow ? 1 : ld)];
+    }
+  }
+  __device__ __forceinline__ void mend(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
+    const uint32_t k = k0 + threadIdx.x % 64 / 16 * 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = present[t] && k + e < end ? x[t][e] : 0.0;
+  }
+};
+
+// Of `depth` k, at least one.  The waves' sums are in `partial` afterwards, for all lanes to read.
+template <int W, class Left, class Right>
+__device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, const Right& right, double (&partial)[W][kDirectSide * kDirectPitch]) {
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  double x[2][2][4], y[2][2][4];   // of two runs
+  f64x4 sum[2][2] = {};
+  auto load = [&](uint32_t k0, int slot) {
+    left.load(k0, depth, x[slot]);
+    right.load(k0, depth, y[slot]);
+  };
+  auto multiply = [&](uint32_t k0, int slot) {
+    if (k0 + kDirectRun > depth || !__all(left.present[0] && left.present[1])) {
+      asm volatile("");   // stays a branch
+      left.mend(k0, depth, x[slot]);
+      right.mend(k0, depth, y[slot]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[slot][t][e], y[slot][u][e], sum[t][u], 0, 0, 0);
+  };
+  constexpr uint32_t kStep = W * kDirectRun;
+  const uint32_t mine = wave * kDirectRun;
+  if (mine < depth) load(mine, 0);
+  for (uint32_t k0 = mine; k0 < depth; k0 += 2 * kStep) {
+    if (k0 + kStep < depth) load(k0 + kStep, 1);
+    multiply(k0, 0);
+    if (k0 + kStep >= depth) break;
+    if (k0 + 2 * kStep < depth) load(k0 + 2 * kStep, 0);
+    multiply(k0 + kStep, 1);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) partial[wave][(t * 16 + lane / 16 + 4 * r) * kDirectPitch + u * 16 + lane % 16] = sum[t][u][r];
+  __syncthreads();
+}
+
+// The sum of cell (r, n), in the order of the waves.
+template <int W>
+__device__ __forceinline__ double direct_sum(const double (&partial)[W][kDirectSide * kDirectPitch], uint32_t r, uint32_t n) {
+  double sum = partial[0][r * kDirectPitch + n];
+#pragma unroll
+  for (int w = 1; w < W; ++w) sum += partial[w][r * kDirectPitch + n];
+  return sum;
+}
+
 }  // namespace cthip

@@ -186,14 +186,14 @@ __global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, ui
   }
 }
 
-__global__ void __launch_bounds__(256) start_double_kernel(const StartArgs a, uint32_t parts, double* to, int64_t stride, FastDiv columns_fd,
-                                                           uint32_t cells) {
+__global__ void __launch_bounds__(256) start_double_kernel(const StartArgs a, uint32_t parts, double* to, int64_t stride, uint32_t ld,
+                                                           FastDiv columns_fd, uint32_t cells) {
   __shared__ double lds[4];
   const double factor = inverse_norm(a, blockIdx.y, parts, lds);
   for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < cells; i += gridDim.x * 256) {
     uint32_t row, column;
     columns_fd.divmod(i, row, column);
-    to[blockIdx.y * stride + i] = start_value<double>(a, (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld + column) * factor;
+    to[blockIdx.y * stride + (int64_t)row * ld + column] = start_value<double>(a, (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld + column) * factor;
   }
 }
 
@@ -512,7 +512,9 @@ __global__ void __launch_bounds__(256) gram_join_kernel(const PairArgs a, uint32
 
 // ------------------------------------------------------------------ double
 
-// Matrices lie as they are given, wide ([m][n], m <= n) or tall ([n][m]).
+// Matrices lie as they are given, wide ([m][n], m <= n) or tall ([n][m]), with rows 16 bytes beyond a whole number of lines of 128 bytes apart,
+// so that 64 bytes of each of sixteen rows fall on all banks of a cache alike (X X^T of 1024 x 1024 37 us; with 1024, or an odd number of
+// lines, from row to row 48).
 struct DoubleArgs {
   const double* x;
   const double* square;   // A, or B
@@ -520,12 +522,16 @@ struct DoubleArgs {
   int64_t x_stride, square_stride, out_stride, ldo;
   TileOrder order;
   uint32_t m, n;          // rows and columns of the results
-  uint32_t depth, ldx;
+  uint32_t depth, ldx, ld_square;
   double a, b, c, alpha, beta;
 };
 
-template <int S, Product kProduct, bool kTall>
+// Large products: tiles of 64 staged in LDS.
+constexpr uint32_t kDoubleSide = 64;
+
+template <Product kProduct, bool kTall>
 __global__ void __launch_bounds__(256, 2) ortho_double_kernel(const DoubleArgs a) {
+  constexpr uint32_t S = kDoubleSide;
   using Row = DoubleRow<S>;
   using Columns = DoubleColumns<S>;
   TilePlace at;
@@ -545,11 +551,11 @@ __global__ void __launch_bounds__(256, 2) ortho_double_kernel(const DoubleArgs a
       r += row0;
       n += column0;
       if (r >= a.m || n >= a.n || r < n) return;
-      if constexpr (kProduct == kSquare) sum = a.c * sum + a.b * square[(int64_t)r * a.m + n] + (r == n ? a.a : 0.0);
-      out[(int64_t)r * a.m + n] = sum;
-      out[(int64_t)n * a.m + r] = sum;
+      if constexpr (kProduct == kSquare) sum = a.c * sum + a.b * square[(int64_t)r * a.ld_square + n] + (r == n ? a.a : 0.0);
+      out[(int64_t)r * a.ldo + n] = sum;
+      out[(int64_t)n * a.ldo + r] = sum;
     };
-    if constexpr (kProduct == kSquare) double_tile<S>(a.depth, row_of(square, a.m, row0, a.m), row_of(square, a.m, column0, a.n), store);
+    if constexpr (kProduct == kSquare) double_tile<S>(a.depth, row_of(square, a.ld_square, row0, a.m), row_of(square, a.ld_square, column0, a.n), store);
     else if constexpr (kTall) double_tile<S>(a.depth, columns_of(x, a.ldx, row0, a.m), columns_of(x, a.ldx, column0, a.n), store);
     else double_tile<S>(a.depth, row_of(x, a.ldx, row0, a.m), row_of(x, a.ldx, column0, a.n), store);
   } else {
@@ -559,9 +565,119 @@ __global__ void __launch_bounds__(256, 2) ortho_double_kernel(const DoubleArgs a
       if constexpr (kProduct == kUpdate) cell = sum;
       else cell = a.beta == 0.0 ? a.alpha * sum : a.alpha * sum + a.beta * cell;
     };
-    if constexpr (kTall) double_tile<S>(a.depth, row_of(x, a.ldx, row0, a.m), row_of(square, a.depth, column0, a.n), store);
-    else double_tile<S>(a.depth, row_of(square, a.depth, row0, a.m), columns_of(x, a.ldx, column0, a.n), store);
+    if constexpr (kTall) double_tile<S>(a.depth, row_of(x, a.ldx, row0, a.m), row_of(square, a.ld_square, column0, a.n), store);
+    else double_tile<S>(a.depth, row_of(square, a.ld_square, row0, a.m), columns_of(x, a.ldx, column0, a.n), store);
   }
+}
+
+// Smaller ones: 32 x 32 by four waves, straight from memory.  X X^T of few rows that are long: parts of k to a block each, whose sums a second
+// launch adds up, in their order (64 x 8000 110 us in one launch, 13 in two).
+constexpr int kDirectWaves = 4;
+using DirectSums = double[kDirectWaves][kDirectSide * kDirectPitch];
+
+template <Product kProduct, bool kTall>
+__device__ __forceinline__ void direct_sums(const DoubleArgs& a, const TilePlace& at, uint32_t first, uint32_t depth, DirectSums& partial) {
+  using Rows = DoubleDirect<true>;
+  using Columns = DoubleDirect<false>;
+  const uint32_t row0 = at.m_tile * kDirectSide, column0 = at.n_tile * kDirectSide;
+  const double* x = a.x + at.matrix * a.x_stride;
+  const double* square = a.square + at.matrix * a.square_stride;
+  auto rows_of = [&](const double* p, uint32_t ld, uint32_t row, uint32_t rows) {
+    return Rows::rows(p + first, ld, [&](uint32_t r) { return (int64_t)min(row + r, rows - 1); });
+  };
+  auto columns_of = [&](const double* p, uint32_t ld, uint32_t column, uint32_t columns) {
+    return Columns::columns(p + (int64_t)first * ld + column, ld, columns - column);
+  };
+  if constexpr (kProduct == kSquare) double_direct(depth, rows_of(square, a.ld_square, row0, a.m), rows_of(square, a.ld_square, column0, a.n), partial);
+  else if constexpr (kProduct == kGram && kTall) double_direct(depth, columns_of(x, a.ldx, row0, a.m), columns_of(x, a.ldx, column0, a.n), partial);
+  else if constexpr (kProduct == kGram) double_direct(depth, rows_of(x, a.ldx, row0, a.m), rows_of(x, a.ldx, column0, a.n), partial);
+  else if constexpr (kTall) double_direct(depth, rows_of(x, a.ldx, row0, a.m), rows_of(square, a.ld_square, column0, a.n), partial);
+  else double_direct(depth, rows_of(square, a.ld_square, row0, a.m), columns_of(x, a.ldx, column0, a.n), partial);
+}
+
+// A block's 32 x 32 cells, four of them a lane's.
+constexpr uint32_t kDirectCells = kDirectSide * kDirectSide / (64 * kDirectWaves);
+
+// Cells at and below the diagonal, and what is above it from those.
+__device__ __forceinline__ void store_symmetric(const DoubleArgs& a, const TilePlace& at, const double (&sums)[kDirectCells], double* image) {
+  double* out = a.out + at.matrix * a.out_stride;
+  const uint32_t row0 = at.m_tile * kDirectSide, column0 = at.n_tile * kDirectSide;
+#pragma unroll
+  for (uint32_t i = 0; i < kDirectCells; ++i) {
+    const uint32_t cell = i * 64 * kDirectWaves + threadIdx.x, r = cell / kDirectSide, n = cell % kDirectSide, m = row0 + r, c = column0 + n;
+    image[r * kDirectPitch + n] = sums[i];
+    if (m < a.m && m >= c) out[(int64_t)m * a.ldo + c] = sums[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kDirectCells; ++i) {
+    const uint32_t cell = i * 64 * kDirectWaves + threadIdx.x, r = cell % kDirectSide, n = cell / kDirectSide, m = row0 + r, c = column0 + n;
+    if (m < a.m && m > c) out[(int64_t)c * a.ldo + m] = image[r * kDirectPitch + n];
+  }
+}
+
+template <Product kProduct, bool kTall>
+__global__ void __launch_bounds__(64 * kDirectWaves, 2) ortho_direct_kernel(const DoubleArgs a) {
+  __shared__ DirectSums partial;
+  TilePlace at;
+  if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
+  const uint32_t row0 = at.m_tile * kDirectSide, column0 = at.n_tile * kDirectSide;
+  double* out = a.out + at.matrix * a.out_stride;
+  // what the results are added to, on its way meanwhile
+  double before[kDirectCells], sums[kDirectCells];
+#pragma unroll
+  for (uint32_t i = 0; i < kDirectCells; ++i) {
+    const uint32_t cell = i * 64 * kDirectWaves + threadIdx.x, r = min(row0 + cell / kDirectSide, a.m - 1), n = min(column0 + cell % kDirectSide, a.n - 1);
+    if constexpr (kProduct == kSquare) before[i] = a.square[at.matrix * a.square_stride + (int64_t)r * a.ld_square + n];
+    if constexpr (kProduct == kLast) before[i] = a.beta == 0.0 ? 0.0 : out[(int64_t)r * a.ldo + n];
+  }
+  direct_sums<kProduct, kTall>(a, at, 0, a.depth, partial);
+#pragma unroll
+  for (uint32_t i = 0; i < kDirectCells; ++i) {
+    const uint32_t cell = i * 64 * kDirectWaves + threadIdx.x, r = cell / kDirectSide, n = cell % kDirectSide;
+    sums[i] = direct_sum(partial, r, n);
+    if constexpr (kProduct == kSquare) sums[i] = a.c * sums[i] + a.b * before[i] + (row0 + r == column0 + n ? a.a : 0.0);
+    if constexpr (kProduct == kLast) sums[i] = a.beta == 0.0 ? a.alpha * sums[i] : a.alpha * sums[i] + a.beta * before[i];
+    if (!is_symmetric(kProduct) && row0 + r < a.m && column0 + n < a.n) out[(int64_t)(row0 + r) * a.ldo + column0 + n] = sums[i];
+  }
+  if constexpr (is_symmetric(kProduct)) store_symmetric(a, at, sums, partial[0]);   // lanes have read their own cells
+}
+
+// [matrix][tile][part][cell]
+template <bool kTall>
+__global__ void __launch_bounds__(64 * kDirectWaves, 2) direct_part_kernel(const DoubleArgs a, uint32_t part_depth, FastDiv parts_fd, double* room, int64_t room_stride) {
+  __shared__ DirectSums partial;
+  uint32_t unit, part;
+  parts_fd.divmod(blockIdx.x, unit, part);
+  TilePlace at;
+  if (!place_of_unit<true>(a.order, unit, &at)) return;
+  direct_sums<kGram, kTall>(a, at, part * part_depth, min(part_depth, a.depth - part * part_depth), partial);
+  double* to = room + at.matrix * room_stride + ((int64_t)(unit - at.matrix * a.order.tiles) * parts_fd.d + part) * (kDirectSide * kDirectSide);
+#pragma unroll
+  for (uint32_t i = 0; i < kDirectCells; ++i) {
+    const uint32_t cell = i * 64 * kDirectWaves + threadIdx.x;
+    to[cell] = direct_sum(partial, cell / kDirectSide, cell % kDirectSide);
+  }
+}
+
+__global__ void __launch_bounds__(64 * kDirectWaves) direct_join_kernel(const DoubleArgs a, uint32_t parts, const double* room, int64_t room_stride) {
+  __shared__ double image[kDirectSide * kDirectPitch];
+  TilePlace at;
+  if (!place_of_unit<true>(a.order, blockIdx.x, &at)) return;
+  const double* from = room + at.matrix * room_stride + (int64_t)(blockIdx.x - at.matrix * a.order.tiles) * parts * (kDirectSide * kDirectSide) + threadIdx.x;
+  double sums[kDirectCells] = {};
+  for (uint32_t part0 = 0; part0 < parts; part0 += 8) {   // loads of eight parts on their way
+    double y[8][kDirectCells];
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+#pragma unroll
+      for (uint32_t i = 0; i < kDirectCells; ++i) y[p][i] = from[(int64_t)min(part0 + p, parts - 1) * (kDirectSide * kDirectSide) + i * 64 * kDirectWaves];
+#pragma unroll
+    for (uint32_t p = 0; p < 8; ++p)
+#pragma unroll
+      for (uint32_t i = 0; i < kDirectCells; ++i) sums[i] += part0 + p < parts ? y[p][i] : 0.0;
+  }
+  store_symmetric(a, at, sums, image);
 }
 
 // ------------------------------------------------------------------ the host's side
@@ -572,18 +688,23 @@ int64_t aligned(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
 constexpr int64_t kMostSide = int64_t(1) << 21, kMostCount = 65535, kMostStride = int64_t(1) << 40;
 constexpr int kMostSteps = 64;
 
+int64_t spread_rows(int64_t doubles) { return ceil_div(std::max<int64_t>(doubles - 2, 0), 16) * 16 + 2; }
+
 // Where the matrices between the products lie in the workspace: bytes of a matrix each.
 struct Layout {
   int64_t m, n;                                  // the shorter side and the longer one
   int64_t x, turned, square, partial, matrix;   // matrix: of all that belongs to one
+  int64_t ldx, ld_square;                        // of doubles
   Layout(int64_t rows, int64_t columns, int dtype) : m(std::min(rows, columns)), n(std::max(rows, columns)) {
     if (dtype == CT_F32) {
       x = aligned(m * ceil_div(n, kPairRun) * kPairRunBytes);
       turned = aligned(n * ceil_div(m, kPairRun) * kPairRunBytes);
       square = aligned(m * ceil_div(m, kPairRun) * kPairRunBytes);
     } else {
-      x = turned = aligned(m * n * 8);
-      square = aligned(m * m * 8);
+      ldx = spread_rows(columns);
+      ld_square = spread_rows(m);
+      x = turned = aligned(rows * ldx * 8);
+      square = aligned(m * ld_square * 8);
     }
     partial = kParts * 8;
     matrix = (dtype == CT_F32 ? x : 0) + 2 * turned + 2 * square + partial;
@@ -695,16 +816,43 @@ void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
   else launch_tile<Tile256, kProduct>(s, a, count);
 }
 
+// Microseconds of `tiles` tiles over `depth` k, of 64 a side by way of LDS and of 32 straight from memory.  Us of both: X X^T of 301 x 517 29
+// and 12, of five of them 30 and 16, of 1024 x 1024 53 and 37, 2000 x 2000 234 and 197, four of 1024 x 2048 239 and 202; B X of the same
+// 20 and 8, 22 and 19, 58 and 52, 312 and 359, 321 and 351.  (Tiles of 32 by way of LDS: X X^T of five 301 x 517 19, B X 22.)
+double time_of_double(int64_t tiles, int64_t depth) { return 5.0 + (double)depth * (0.012 + 0.036 * (double)ceil_div(tiles, kUnits)); }
+double time_of_direct(int64_t tiles, int64_t depth) { return 5.0 + (double)depth * 0.0117 * (double)ceil_div(tiles, kUnits); }
+
 template <Product kProduct>
 void launch_double(hipStream_t s, DoubleArgs a, int64_t count, bool tall) {
   constexpr bool kSymmetric = is_symmetric(kProduct);
-  const int64_t side = tiles_of(count, a.m, a.n, 64, kSymmetric) >= kUnits ? 64 : 32;
-  a.order = order_of(count, a.m, a.n, side, kSymmetric);
-  const dim3 grid = grid_of(a.order);
-  if (side == 64 && tall) hipLaunchKernelGGL((ortho_double_kernel<64, kProduct, true>), grid, dim3(256), 0, s, a);
-  else if (side == 64) hipLaunchKernelGGL((ortho_double_kernel<64, kProduct, false>), grid, dim3(256), 0, s, a);
-  else if (tall) hipLaunchKernelGGL((ortho_double_kernel<32, kProduct, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((ortho_double_kernel<32, kProduct, false>), grid, dim3(256), 0, s, a);
+  const int64_t large = tiles_of(count, a.m, a.n, kDoubleSide, kSymmetric), small = tiles_of(count, a.m, a.n, kDirectSide, kSymmetric);
+  if (time_of_direct(small, a.depth) <= time_of_double(large, a.depth)) {
+    a.order = order_of(count, a.m, a.n, kDirectSide, kSymmetric);
+    const dim3 grid = grid_of(a.order), block(64 * kDirectWaves);
+    if (tall) hipLaunchKernelGGL((ortho_direct_kernel<kProduct, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((ortho_direct_kernel<kProduct, false>), grid, block, 0, s, a);
+  } else {
+    a.order = order_of(count, a.m, a.n, kDoubleSide, kSymmetric);
+    const dim3 grid = grid_of(a.order);
+    if (tall) hipLaunchKernelGGL((ortho_double_kernel<kProduct, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((ortho_double_kernel<kProduct, false>), grid, dim3(256), 0, s, a);
+  }
+}
+
+// X X^T, in parts of k where there are few tiles: a block for each unit, 32 parts at most (the launch that joins them waits for each eight),
+// 64 k at least, in the room of a matrix's `bytes`.
+void launch_double_gram(hipStream_t s, DoubleArgs a, int64_t count, bool tall, void* room, int64_t bytes) {
+  const int64_t tiles = tiles_of(1, a.m, a.n, kDirectSide, true);
+  const int64_t most = std::min({kUnits / (count * tiles), ceil_div(a.depth, 64), bytes / (tiles * kDirectSide * kDirectSide * 8), (int64_t)32});
+  const int64_t part_depth = most > 1 ? ceil_div(ceil_div(a.depth, most), kDirectRun) * kDirectRun : a.depth, parts = ceil_div(a.depth, part_depth);
+  if (parts == 1 || time_of_direct(count * tiles * parts, part_depth) + 5.0 + 0.1 * (double)parts >= time_of_direct(count * tiles, a.depth))
+    return launch_double<kGram>(s, a, count, tall);
+  a.order = order_of(count, a.m, a.n, kDirectSide, true);
+  const dim3 grid((uint32_t)(a.order.units * parts)), block(64 * kDirectWaves);
+  double* const sums = static_cast<double*>(room);
+  if (tall) hipLaunchKernelGGL((direct_part_kernel<true>), grid, block, 0, s, a, (uint32_t)part_depth, FastDiv((uint32_t)parts), sums, bytes / 8);
+  else hipLaunchKernelGGL((direct_part_kernel<false>), grid, block, 0, s, a, (uint32_t)part_depth, FastDiv((uint32_t)parts), sums, bytes / 8);
+  hipLaunchKernelGGL(direct_join_kernel, dim3(a.order.units), block, 0, s, a, (uint32_t)parts, sums, bytes / 8);
 }
 
 // The largest |a + b s + c s^2| for s of 0 to `most`, and the largest |v (a + b v^2 + c v^4)| for v of 0 to the root of it.
@@ -860,19 +1008,21 @@ int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once
     hipLaunchKernelGGL((start_norm_kernel<double>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
                        start.ld == r.columns);
     hipLaunchKernelGGL(start_double_kernel, dim3((uint32_t)std::min<int64_t>(ceil_div(cells, 256), 4096), (uint32_t)count), dim3(256), 0, s, start,
-                       (uint32_t)parts, x[0], l.x / 8, FastDiv((uint32_t)r.columns), (uint32_t)cells);
+                       (uint32_t)parts, x[0], l.x / 8, (uint32_t)l.ldx, FastDiv((uint32_t)r.columns), (uint32_t)cells);
     for (int step = 0; step < r.steps; ++step) {
       const double* k = r.coefficients + 3 * step;
       DoubleArgs g{};
       g.x = x[step & 1];
       g.x_stride = l.x / 8;
-      g.ldx = (uint32_t)r.columns;
+      g.ldx = (uint32_t)l.ldx;
+      g.ld_square = (uint32_t)l.ld_square;
+      g.ldo = l.ld_square;
       g.square_stride = g.out_stride = l.square / 8;
       g.m = g.n = (uint32_t)l.m;
       g.out = gram;
       g.square = gram;
       g.depth = (uint32_t)l.n;
-      launch_double<kGram>(s, g, count, tall);
+      launch_double_gram(s, g, count, tall, x[(step + 1) & 1], l.x);
       g.out = factor;
       g.depth = (uint32_t)l.m;
       g.a = k[0];
@@ -885,7 +1035,7 @@ int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once
       if (step + 1 < r.steps) {
         g.out = x[(step + 1) & 1];
         g.out_stride = l.x / 8;
-        g.ldo = r.columns;
+        g.ldo = l.ldx;
         launch_double<kUpdate>(s, g, count, tall);
       } else {
         g.out = static_cast<double*>(r.out) + first * r.out_stride;

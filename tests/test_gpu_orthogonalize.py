@@ -123,6 +123,23 @@ def test_every_tile(stream, as_released):  # noqa: F811
         D.kept.clear()
 
 
+@pytest.mark.parametrize("shape", [(14, 500, 600), (14, 600, 500), (3, 70, 3000), (2, 3000, 70), (1, 33, 1029), (2, 1029, 20), (1, 5, 65), (1, 130, 16), (1, 1, 5000)],
+                         ids=str)
+def test_every_kernel_of_doubles(stream, as_released, shape):  # noqa: F811
+    """Tiles of 64 and of 32 for each product, and X X^T in parts of k; matrices that are powers of two apart have the same results."""
+    D = Owned("double")
+    rng = np.random.default_rng(31)
+    one = gradient(rng, 1, *shape[1:])
+    scales = 2.0 ** rng.integers(-3, 4, shape[0])
+    g, out = D.tensor(one * scales[:, None, None]), D.tensor(np.full(shape, np.nan))
+    optimize.orthogonalize(optimize.Backend(stream, "double"), out, g, steps=3, epsilon=0.0)
+    got = read(out)
+    want, bar = bar_of(one[0], UNIT["double"], steps=3, epsilon=0.0)
+    near(got[0], want, bar)
+    assert np.array_equal(got, np.broadcast_to(got[0], shape))
+    D.free()
+
+
 @pytest.mark.parametrize("rows,columns", [(37, 65), (65, 37), (1, 9), (9, 1)])
 def test_rows_apart_and_what_the_result_is_added_to(D, rows, columns):
     rng = np.random.default_rng(1)

@@ -88,7 +88,8 @@ def test_workspace():
     assert workspace(1000, 1024, 1024) == 64 * workspace(1, 1024, 1024)
     # three float matrices in two pieces, two of the shorter side; three in double there are two
     assert 12 * 1024 * 2048 + 8 * 1024 * 1024 <= workspace(1, 1024, 2048) <= 12 * 1024 * 2048 + 8 * 1024 * 1024 + (1 << 16)
-    assert 16 * 1024 * 2048 + 16 * 1024 * 1024 <= workspace(1, 1024, 2048, capi.F64) <= 16 * 1024 * 2048 + 16 * 1024 * 1024 + (1 << 16)
+    # rows of doubles are an odd number of 128 bytes apart: up to 31 doubles more to each of four times 1024 rows
+    assert 16 * 1024 * 2048 + 16 * 1024 * 1024 <= workspace(1, 1024, 2048, capi.F64) <= 16 * 1024 * 2048 + 16 * 1024 * 1024 + 4 * 1024 * 31 * 8 + (1 << 16)
     refuses("float or double", "ct_orthogonalize_workspace", 1, 2, 3, capi.I8, C.byref(C.c_int64()))
     refuses("null result", "ct_orthogonalize_workspace", 1, 2, 3, capi.F32, None)
     refuses("bad extent", "ct_orthogonalize_workspace", 1, 1 << 22, 3, capi.F32, C.byref(C.c_int64()))
