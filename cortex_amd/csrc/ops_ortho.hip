@@ -367,6 +367,9 @@ template <int W>
 __device__ __forceinline__ void small_sums(const char* left, uint32_t last_left, const char* right, uint32_t last_right, int64_t row_bytes, uint32_t first,
                                            uint32_t end, float (&partial)[W][kSmallCells]) {
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Every other row's pieces change places, so that a load's 64 bytes of each of sixteen lines fall on all banks of a cache (512 x 512 in five steps
+  // 131 -> 108 us): all four products are formed whichever comes first.
+  const int32_t first_piece = lane % 2 * 64, other_piece = 64 - first_piece;
   const char *l[2], *r[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -379,14 +382,14 @@ __device__ __forceinline__ void small_sums(const char* left, uint32_t last_left,
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        x[slot][t][p] = *reinterpret_cast<const f16x8*>(l[t] + (int64_t)run * kPairRunBytes + p * 64);
-        y[slot][t][p] = *reinterpret_cast<const f16x8*>(r[t] + (int64_t)run * kPairRunBytes + p * 64);
+        x[slot][t][p] = *reinterpret_cast<const f16x8*>(l[t] + (int64_t)run * kPairRunBytes + (p == 0 ? first_piece : other_piece));
+        y[slot][t][p] = *reinterpret_cast<const f16x8*>(r[t] + (int64_t)run * kPairRunBytes + (p == 0 ? first_piece : other_piece));
       }
   };
   pair_f32x4 sum[2][2] = {};
   auto multiply = [&](int slot) {
 #pragma unroll
-    for (int i = 3; i >= 0; --i)   // the smaller products first
+    for (int i = 3; i >= 0; --i)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(64 * W, 4) pair_small_kernel(const PairArgs a)
 }
 
 // X X^T of few rows that are long: parts of k to a block each, [matrix][tile][part], and a second launch that adds them up, in their order
-// (40 x 4000 29 us in one launch, 9 in two; thirty-two of 16 x 8000 37 and 13).
+// (200 x 8000 41 us in one launch, 13 in two).
 constexpr int kPartWaves = 8;
 __global__ void __launch_bounds__(64 * kPartWaves, 4) gram_part_kernel(const PairArgs a, uint32_t part_runs, FastDiv parts_fd, float* sums, int64_t sums_stride) {
   __shared__ float partial[kPartWaves][kSmallCells];
@@ -744,10 +747,10 @@ constexpr int64_t kUnits = 256;
 
 // Microseconds of `tiles` tiles over `runs` runs of 32 k.  Small tiles are bound by what the L2 caches give, or one to a unit by latency; of
 // 128 a side two blocks share a unit; large ones are bound by the matrix cores, whose clock is higher while some of them rest.  Us of 32,
-// 64, 128 and 256 a side: X X^T of 128 x 784 9.3, 11, 24, 46; 512 x 512 7.5, 9.4; 1024 x 1024 25, 15, 32, 76; 2048 x 2048 64 a side
-// and up 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199; 4096 x 8192 720, 527, 471; B X of 1024 x 1024 33, 16, 33, 77; of the others
+// 64, 128 and 256 a side: X X^T of 128 x 784 7.6, 12, 26, 46; 512 x 512 6.6, 9.8; 1024 x 1024 16, 15, 32, 76; 2048 x 2048 64 a side
+// and up 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199; 4096 x 8192 720, 527, 471; B X of 1024 x 1024 21, 16, 33, 77; of the others
 // 70, 63, 130; 440, 331, 296; 1000, 738, 651.  Within 15 % of most of the 100 times of which these are a part.
-double time_of_32(int64_t tiles, int64_t runs) { return 3.4 + 0.245 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
+double time_of_32(int64_t tiles, int64_t runs) { return 3.0 + (0.9 + 0.144 * (double)runs) * (double)ceil_div(tiles, kUnits); }
 double time_of_64(int64_t tiles, int64_t runs) { return 5.0 + 0.31 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
 double time_of_128(int64_t tiles, int64_t runs) {
   const int64_t full = tiles / (2 * kUnits), rest = tiles % (2 * kUnits);
