@@ -149,16 +149,20 @@ __device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right rig
 
 // Small products: a block owns 32 x 32, its W waves take every W-th run of 16 k each, straight from memory into the matrix cores'
 // operands, the next run's loads on their way meanwhile, and leave their sums in LDS.  Nothing waits for another wave before that: five of
-// 301 x 517 times their transposes 16 us, in tiles of 32 by way of LDS 19 (with eight waves 18.6).  A lane's four k of a run are lane / 16 * 4 and those behind it; sixteen lanes' rows, or
-// columns, of t are t * 16 and those behind it.
+// 301 x 517 times their transposes 16 us, in tiles of 32 by way of LDS 19 (with eight waves 18.6).  A lane's four k of a run are
+// lane / 16 * 4 and those behind it; sixteen lanes' rows, or columns, of t are t * 16 and those behind it.
 constexpr uint32_t kDirectSide = 32, kDirectPitch = 33, kDirectRun = 16;
 
-template <bool kByRow>
+template <bool kByRow, bool kTurn = false>
 struct DoubleDirect {
   const double* p[2];   // a lane's row, from k 0 on, or its column
   int64_t ld;           // of columns
   bool present[2];
-  // `row(i)`: which one is row i of the tile's
+  // Where rows are a multiple of 32 bytes apart the two loads of every other one change places: 16 bytes of each 32 of sixteen rows
+  // would else fall on half of a cache's banks (1024 x 1024 times its transpose 37 us, and 48).  What it costs (1500 x 1500 93 us, and
+  // 104) is for those that ask for it.  0 or 2.
+  uint32_t turn;
+  // `row(i)`: which one is row i of the tile's, none if it is negative
   template <class Row>
   static __device__ __forceinline__ DoubleDirect rows(const double* p, int64_t ld, Row row) {
     DoubleDirect d;
@@ -169,6 +173,7 @@ struct DoubleDirect {
       d.p[t] = p + (i < 0 ? 0 : i) * ld;
     }
     d.ld = ld;
+    d.turn = kTurn && ld % 4 == 0 ? threadIdx.x % 2 * 2 : 0;
     return d;
   }
   static __device__ __forceinline__ DoubleDirect columns(const double* p, int64_t ld, uint32_t left) {   // of `left` columns
@@ -179,6 +184,7 @@ struct DoubleDirect {
       d.p[t] = p + min(t * 16 + threadIdx.x % 16, left - 1);
     }
     d.ld = ld;
+    d.turn = 0;
     return d;
   }
   __device__ __forceinline__ void load(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
@@ -187,8 +193,8 @@ struct DoubleDirect {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const f64x2 two = *reinterpret_cast<const f64x2_at_8*>(p[t] + k + e);
+        for (uint32_t e = 0; e < 4; e += 2) {
+          const f64x2 two = *reinterpret_cast<const f64x2_at_8*>(p[t] + k + (e ^ (kTurn ? turn : 0)));
           x[t][e] = two[0];
           x[t][e + 1] = two[1];
         }
@@ -196,7 +202,7 @@ struct DoubleDirect {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = p[t][min(k + e, end - 1) * (kByRow ? 1 : ld)];
+        for (uint32_t e = 0; e < 4; ++e) x[t][e] = p[t][min(k + (e ^ (kTurn ? turn : 0)), end - 1) * (kByRow ? 1 : ld)];
     }
   }
   __device__ __forceinline__ void mend(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
@@ -204,14 +210,16 @@ struct DoubleDirect {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] = present[t] && k + e < end ? x[t][e] : 0.0;
+      for (uint32_t e = 0; e < 4; ++e) x[t][e] = present[t] && k + (e ^ (kTurn ? turn : 0)) < end ? x[t][e] : 0.0;
   }
+  __device__ __forceinline__ double at(const double (&x)[4], int e) const { return kTurn && turn ? x[e ^ 2] : x[e]; }
 };
 
 // Of `depth` k, at least one.  The waves' sums are in `partial` afterwards, for all lanes to read.
 template <int W, class Left, class Right>
 __device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, const Right& right, double (&partial)[W][kDirectSide * kDirectPitch]) {
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool all_present = __all(left.present[0] && left.present[1]);
   double x[2][2][4], y[2][2][4];   // of two runs
   f64x4 sum[2][2] = {};
   auto load = [&](uint32_t k0, int slot) {
@@ -219,7 +227,7 @@ __device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, 
     right.load(k0, depth, y[slot]);
   };
   auto multiply = [&](uint32_t k0, int slot) {
-    if (k0 + kDirectRun > depth || !__all(left.present[0] && left.present[1])) {
+    if (k0 + kDirectRun > depth || !all_present) {
       asm volatile("");   // stays a branch
       left.mend(k0, depth, x[slot]);
       right.mend(k0, depth, y[slot]);
@@ -229,7 +237,8 @@ __device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, 
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[slot][t][e], y[slot][u][e], sum[t][u], 0, 0, 0);
+        for (int u = 0; u < 2; ++u)
+          sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(left.at(x[slot][t], e), right.at(y[slot][u], e), sum[t][u], 0, 0, 0);
   };
   constexpr uint32_t kStep = W * kDirectRun;
   const uint32_t mine = wave * kDirectRun;

@@ -581,8 +581,10 @@ __global__ void __launch_bounds__(64 * W, 4) gated_gradient_thin_kernel(const Ga
 // ------------------------------------------------------------------ double
 
 // Half of a tile's S columns are gates, the other half their ups; they meet in LDS.
-template <int S>
+constexpr uint32_t kDoubleSide = 64;
+
 __global__ void __launch_bounds__(256, 2) gated_double_kernel(const GatedArgs a, const GroupedPlan p) {
+  constexpr uint32_t S = kDoubleSide;
   using Row = DoubleRow<S>;
   __shared__ double cells[S][S + 1];
   TilePlace at;
@@ -606,8 +608,8 @@ __global__ void __launch_bounds__(256, 2) gated_double_kernel(const GatedArgs a,
   }
 }
 
-template <int S>
 __global__ void __launch_bounds__(256, 2) gated_gradient_double_kernel(const GatedArgs a, const GroupedPlan p) {
+  constexpr uint32_t S = kDoubleSide;
   using Row = DoubleRow<S>;
   TilePlace at;
   Group g;
@@ -623,6 +625,61 @@ __global__ void __launch_bounds__(256, 2) gated_gradient_double_kernel(const Gat
                    if (a.g.c) static_cast<double*>(a.g.c)[at.part * a.g.c_split + to * a.g.ldc + col0 + n] = sum;
                    else finish_gradient(a, to, col0 + n, sum);
                  });
+}
+
+// Smaller products: 32 x 32 sums to a block, straight from memory (double_tile.h).
+constexpr int kDirectWaves = 4;
+
+template <bool kTurn>
+__global__ void __launch_bounds__(64 * kDirectWaves, 2) gated_direct_kernel(const GatedArgs a, const GroupedPlan p) {
+  constexpr uint32_t S = kDirectSide, kColumns = S / 2;
+  using Rows = DoubleDirect<true, kTurn>;
+  __shared__ double partial[kDirectWaves][S * kDirectPitch];
+  TilePlace at;
+  Group g;
+  if (!place_of(p, &at) || !find_group(a.g, at.m_tile, S, &g)) return;
+  const uint32_t row0 = g.tile * S, col0 = at.n_tile * kColumns, begin = at.part * a.g.part, count = min(a.g.part, a.g.k - begin);
+  const double* b = static_cast<const double*>(a.g.b) + (int64_t)g.index * a.g.b_stride;
+  const Rows left = Rows::rows(static_cast<const double*>(a.g.a) + begin, a.g.lda, [&](uint32_t r) -> int64_t {
+    const uint32_t row = g.first + min(row0 + r, g.rows - 1), from = a.g.index_a ? (uint32_t)a.g.index_a[row] : row;
+    return from < a.g.a_rows ? (int64_t)from : -1;
+  });
+  const Rows right = Rows::rows(b + begin, a.g.ldb, [&](uint32_t r) -> int64_t {
+    const uint32_t column = min(col0 + r % kColumns, a.g.n - 1);
+    return r / kColumns ? (int64_t)a.g.n + column : column;
+  });
+  double_direct(count, left, right, partial);
+#pragma unroll
+  for (uint32_t i = threadIdx.x; i < S * kColumns; i += 64 * kDirectWaves) {
+    const uint32_t m = i / kColumns, n = i % kColumns;
+    if (row0 + m >= g.rows || col0 + n >= a.g.n) continue;
+    const double gate = direct_sum(partial, m, n), up = direct_sum(partial, m, n + kColumns);
+    if (a.g.c) keep_pair(a, at.part, (int64_t)g.first + row0 + m, col0 + n, gate, up);
+    else finish(a, (int64_t)g.first + row0 + m, col0 + n, gate, up);
+  }
+}
+
+template <bool kTurn>
+__global__ void __launch_bounds__(64 * kDirectWaves, 2) gated_gradient_direct_kernel(const GatedArgs a, const GroupedPlan p) {
+  constexpr uint32_t S = kDirectSide;
+  using Rows = DoubleDirect<true, kTurn>;
+  __shared__ double partial[kDirectWaves][S * kDirectPitch];
+  TilePlace at;
+  Group g;
+  if (!place_of(p, &at) || !find_group(a.g, at.m_tile, S, &g)) return;
+  const uint32_t row0 = g.tile * S, col0 = at.n_tile * S, begin = at.part * a.g.part, count = min(a.g.part, a.g.k - begin);
+  const double* b = static_cast<const double*>(a.g.b) + (int64_t)g.index * a.g.b_stride;
+  const Rows left = Rows::rows(static_cast<const double*>(a.g.a) + begin, a.g.lda, [&](uint32_t r) { return (int64_t)g.first + min(row0 + r, g.rows - 1); });
+  double_direct(count, left, DoubleDirect<false>::columns(b + (int64_t)begin * a.g.ldb + col0, a.g.ldb, a.g.n - col0), partial);
+#pragma unroll
+  for (uint32_t i = threadIdx.x; i < S * S; i += 64 * kDirectWaves) {
+    const uint32_t r = i / S, n = i % S;
+    if (row0 + r >= g.rows || col0 + n >= a.g.n) continue;
+    const int64_t to = (int64_t)g.first + row0 + r;
+    const double sum = direct_sum(partial, r, n);
+    if (a.g.c) static_cast<double*>(a.g.c)[at.part * a.g.c_split + to * a.g.ldc + col0 + n] = sum;
+    else finish_gradient(a, to, col0 + n, sum);
+  }
 }
 
 // ------------------------------------------------------------------ the parts of k brought together
@@ -676,6 +733,16 @@ double time_of_few(const Shape& s, int64_t width) {
 }
 // From these many k on a block has sixteen waves, of eight: 51 and 57 us at 4096 k; below 1024 the launch of sixteen takes longer.
 constexpr uint32_t kFewK16 = 1024, kFewK64 = 2049;
+
+// Microseconds of tiles of doubles, of 32 a side straight from memory and of 64 by way of LDS, whose cells are finished four at a time and
+// sixteen at a time.  Us of both, forward and gradient: 509 rows, 301 by 517, 16 and 15, 23 and 31; 1000 rows, 700 by 900, 80 and 46, 74 and 57;
+// 4096, 512 by 512, 105 and 61, 95 and 63; 4096, 301 by 517, 73 and 50, 83 and 64; 200, 4096 by 64 in parts 20 and 13.  (Tiles of 32 by way of
+// LDS: 509 rows 18 and 16.)
+double time_of_direct(int64_t tiles, double k, bool gradient) { return 5.0 + (double)ceil_div(tiles, kUnits) * (0.0117 * k + (gradient ? 1.2 : 0.9)); }
+double time_of_double(int64_t tiles, double k, bool gradient) {
+  const double rounds = (double)ceil_div(tiles, kUnits);
+  return 5.0 + k * (0.015 + 0.037 * rounds) + rounds * (gradient ? 8.0 : 3.5);
+}
 
 int64_t aligned(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
 
@@ -743,7 +810,12 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
   auto choose = [&](int64_t most_parts) {
     if constexpr (std::is_same<T, double>::value) {
       Choice best{32, 32, 1, 1e12};
-      consider_double_parts(&best, shape.blocks(32, 32), shape.blocks(64, 64), shape.k, shape.k, cells, most_parts);
+      for (int64_t parts = 1; parts <= most_parts && (parts == 1 || shape.k >= parts * 64); parts *= 2) {
+        const int64_t small = shape.blocks(kDirectSide, kDirectSide) * parts, large = shape.blocks(kDoubleSide, kDoubleSide) * parts;
+        const double k = (double)shape.k / (double)parts, sum = time_of_sum(parts, cells, sizeof(double));
+        if (time_of_direct(small, k, kGradient) + sum < best.us) best = {32, 32, parts, time_of_direct(small, k, kGradient) + sum};
+        if (time_of_double(large, k, kGradient) + sum < best.us) best = {64, 64, parts, time_of_double(large, k, kGradient) + sum};
+      }
       return best;
     } else {
       const double thin64 = time_of_few(shape, 64), thin16 = time_of_few(shape, 16);
@@ -830,8 +902,9 @@ int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre,
   if (dtype == CT_F64) {
     return run<double, false>("ct_gated_gemm", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-        if (best.height == 64) hipLaunchKernelGGL((gated_double_kernel<64>), grid, dim3(256), 0, s, a, plan);
-        else hipLaunchKernelGGL((gated_double_kernel<32>), grid, dim3(256), 0, s, a, plan);
+        if (best.height == 64) hipLaunchKernelGGL(gated_double_kernel, grid, dim3(256), 0, s, a, plan);
+        else if (a.g.lda % 4 == 0 || a.g.ldb % 4 == 0) hipLaunchKernelGGL((gated_direct_kernel<true>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
+        else hipLaunchKernelGGL((gated_direct_kernel<false>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
       }, band);
     });
   }
@@ -890,8 +963,9 @@ int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradien
   if (dtype == CT_F64) {
     return run<double, true>("ct_gated_gemm_gradient", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-        if (best.height == 64) hipLaunchKernelGGL((gated_gradient_double_kernel<64>), grid, dim3(256), 0, s, a, plan);
-        else hipLaunchKernelGGL((gated_gradient_double_kernel<32>), grid, dim3(256), 0, s, a, plan);
+        if (best.height == 64) hipLaunchKernelGGL(gated_gradient_double_kernel, grid, dim3(256), 0, s, a, plan);
+        else if (a.g.lda % 4 == 0) hipLaunchKernelGGL((gated_gradient_direct_kernel<true>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
+        else hipLaunchKernelGGL((gated_gradient_direct_kernel<false>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
       }, band);
     });
   }
