@@ -33,12 +33,13 @@ __device__ __forceinline__ uint32_t unit_of_block(uint32_t b, uint32_t units) {
   return (b % kXcds) * per_die + b / kXcds;
 }
 
-// Tiles of one product in bands of kBand rows, column after column; of a symmetric one those at and below the diagonal, row
-// after row.
+// Tiles of one product in bands of some rows, column after column, so that those that run at once on a die need few rows and columns; of a
+// symmetric one those at and below the diagonal.
 constexpr uint32_t kBand = 8;
 
 struct TileOrder {
   uint32_t units, tiles, m_tiles, n_tiles;   // tiles of a matrix; units: of all of them
+  uint32_t band;                             // rows of a band, of a symmetric product of square tiles
   FastDiv tiles_fd, band_fd;
 };
 
@@ -52,21 +53,27 @@ __device__ __forceinline__ bool place_of_unit(const TileOrder& o, uint32_t unit,
   if (unit >= o.units) return false;
   uint32_t tile, band, rest;
   o.tiles_fd.divmod(unit, p->matrix, tile);
-  if constexpr (kSymmetric && kTall) {   // of three rows of tiles the q-th have 4 q + 2, 4 q + 3 and 4 q + 4, those before them 6 q q + 3 q
-    auto before = [](uint32_t q) { return 6 * q * q + 3 * q; };
-    uint32_t q = (uint32_t)((sqrtf(24.f * (float)tile + 9.f) - 3.f) * (1.f / 12.f));   // may be one off
-    if (before(q) > tile) --q;
-    if (before(q + 1) <= tile) ++q;
-    rest = tile - before(q);
-    const uint32_t row = rest < 4 * q + 2 ? 0 : rest < 8 * q + 5 ? 1 : 2;
-    p->m_tile = 3 * q + row;
-    p->n_tile = rest - (row == 0 ? 0 : row == 1 ? 4 * q + 2 : 8 * q + 5);
-  } else if constexpr (kSymmetric) {
-    uint32_t i = (uint32_t)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);   // may be one off
-    if (i * (i + 1) / 2 > tile) --i;
-    if ((i + 1) * (i + 2) / 2 <= tile) ++i;
-    p->m_tile = i;
-    p->n_tile = tile - i * (i + 1) / 2;
+  if constexpr (kSymmetric) {
+    // band b has `rows` rows of `whole` columns and what is below the diagonal beyond them; the bands before it
+    const uint32_t rows = kTall ? 3 : o.band;
+    auto before = [&](uint32_t b) { return kTall ? 6 * b * b + 3 * b : rows * b * (rows * b + 1) / 2; };
+    band = (uint32_t)(kTall ? (sqrtf(24.f * (float)tile + 9.f) - 3.f) * (1.f / 12.f) : (sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f / (float)rows);   // may be one off
+    if (before(band) > tile) --band;
+    if (before(band + 1) <= tile) ++band;
+    rest = tile - before(band);
+    const uint32_t there = min(rows, o.m_tiles - band * rows), whole = kTall ? 4 * band + 2 : band * rows + 1;
+    uint32_t row = 0, column = 0;
+    if (rest < there * whole) {
+      column = rest / there;
+      row = rest - column * there;
+    } else {   // a column has a row less than the one before it
+      rest -= there * whole;
+      column = whole;
+      for (uint32_t left = there - 1; rest >= left; --left, ++column) rest -= left;
+      row = rest + column - whole + 1;
+    }
+    p->m_tile = band * rows + row;
+    p->n_tile = column;
   } else {
     o.band_fd.divmod(tile, band, rest);
     const uint32_t rows = min(kBand, o.m_tiles - band * kBand);
@@ -737,6 +744,7 @@ TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t height, int64_t 
   o.units = (uint32_t)(count * tiles);
   o.tiles_fd = FastDiv(o.tiles);
   o.band_fd = FastDiv((uint32_t)(kBand * nt));
+  o.band = o.units <= 24 * kXcds ? kBand / 2 : kBand;
   return o;
 }
 TileOrder order_of(int64_t count, int64_t m, int64_t n, int64_t side, bool symmetric) { return order_of(count, m, n, side, side, symmetric); }
@@ -747,11 +755,15 @@ constexpr int64_t kUnits = 256;
 
 // Microseconds of `tiles` tiles over `runs` runs of 32 k.  Small tiles are bound by what the L2 caches give, or one to a unit by latency; of
 // 128 a side two blocks share a unit; large ones are bound by the matrix cores, whose clock is higher while some of them rest.  Us of 32,
-// 64, 128 and 256 a side: X X^T of 128 x 784 7.6, 12, 26, 46; 512 x 512 6.6, 9.8; 1024 x 1024 16, 15, 32, 76; 2048 x 2048 64 a side
-// and up 49, 58, 126; sixteen of 1024 x 2816 215, 204, 199; 4096 x 8192 720, 527, 471; B X of 1024 x 1024 21, 16, 33, 77; of the others
-// 70, 63, 130; 440, 331, 296; 1000, 738, 651.  Within 15 % of most of the 100 times of which these are a part.
-double time_of_32(int64_t tiles, int64_t runs) { return 3.0 + (0.9 + 0.144 * (double)runs) * (double)ceil_div(tiles, kUnits); }
-double time_of_64(int64_t tiles, int64_t runs) { return 5.0 + 0.31 * (double)runs * std::max(1.0, (double)tiles / kUnits); }
+// 64, 128 and 256 a side: X X^T of 128 x 784 7.6, 10, 26, 46; 512 x 512 5.8, 9.0; 1024 x 1024 16, 12, 32, 76; 2048 x 2048 73, 48, 58, 126;
+// sixteen of 1024 x 2816 500, 229, 207, 199; 4096 x 8192 1090, 559, 546, 471; B X of 1024 x 1024 21, 14, 33, 77; of the others from 2048 on 129,
+// 71, 64, 130; 814, 436, 331, 296; 2139, 1018, 780, 651.  Within 15 % of most of the 150 times of which these are a part.
+double time_of_32(int64_t tiles, int64_t runs, bool symmetric) {
+  return 3.0 + ((symmetric ? 0.5 : 1.2) + 0.144 * (double)runs) * (double)ceil_div(tiles, kUnits);
+}
+double time_of_64(int64_t tiles, int64_t runs) {
+  return 5.0 + (double)runs * (tiles <= kUnits ? 0.23 : std::max(0.44, 0.285 * (double)tiles / kUnits));
+}
 double time_of_128(int64_t tiles, int64_t runs) {
   const int64_t full = tiles / (2 * kUnits), rest = tiles % (2 * kUnits);
   return 7.0 * (double)(full + (rest > 0)) + (double)runs * (1.5 * (double)full + (rest == 0 ? 0.0 : rest <= kUnits ? 0.8 : 1.45));
@@ -769,12 +781,12 @@ double time_of_tall(int64_t tiles, int64_t runs) {
 
 double time_of_gram(int64_t count, int64_t m, int64_t runs) {
   auto tiles = [&](int64_t side) { return tiles_of(count, m, m, side, true); };
-  return std::min({time_of_32(tiles(kSmallSide), runs), time_of_64(tiles(64), runs), time_of_128(tiles(128), runs),
+  return std::min({time_of_32(tiles(kSmallSide), runs, true), time_of_64(tiles(64), runs), time_of_128(tiles(128), runs),
                    time_of_tall(tiles_of(count, m, m, 256, 192, true), runs), time_of_256(tiles(256), runs)});
 }
 // With parts of k and the launch that joins them.
 double time_of_parts(int64_t count, int64_t m, int64_t runs, int64_t parts) {
-  return time_of_32(tiles_of(count, m, m, kSmallSide, true) * parts, ceil_div(runs, parts)) + 5.0;
+  return time_of_32(tiles_of(count, m, m, kSmallSide, true) * parts, ceil_div(runs, parts), true) + 5.0;
 }
 
 template <class Tile, Product kProduct>
@@ -811,9 +823,9 @@ void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
   const double small = time_of_64(tiles(64), a.runs), medium = time_of_128(tiles(128), a.runs), large = time_of_256(tiles(256), a.runs);
   if constexpr (is_symmetric(kProduct)) {
     const double tall = time_of_tall(tiles_of(count, a.m, a.n, 256, 192, true), a.runs);
-    if (tall < std::min({time_of_32(tiles(kSmallSide), a.runs), small, medium, large})) return launch_tile<TileTall, kProduct>(s, a, count);
+    if (tall < std::min({time_of_32(tiles(kSmallSide), a.runs, true), small, medium, large})) return launch_tile<TileTall, kProduct>(s, a, count);
   }
-  if (time_of_32(tiles(kSmallSide), a.runs) <= std::min({small, medium, large})) launch_small<kProduct>(s, a, count);
+  if (time_of_32(tiles(kSmallSide), a.runs, is_symmetric(kProduct)) <= std::min({small, medium, large})) launch_small<kProduct>(s, a, count);
   else if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
   else if (medium <= large) launch_tile<Tile128, kProduct>(s, a, count);
   else launch_tile<Tile256, kProduct>(s, a, count);
