@@ -241,14 +241,22 @@ __device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, 
           sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(left.at(x[slot][t], e), right.at(y[slot][u], e), sum[t][u], 0, 0, 0);
   };
   constexpr uint32_t kStep = W * kDirectRun;
-  const uint32_t mine = wave * kDirectRun;
-  if (mine < depth) load(mine, 0);
-  for (uint32_t k0 = mine; k0 < depth; k0 += 2 * kStep) {
-    if (k0 + kStep < depth) load(k0 + kStep, 1);
-    multiply(k0, 0);
-    if (k0 + kStep >= depth) break;
-    if (k0 + 2 * kStep < depth) load(k0 + 2 * kStep, 0);
-    multiply(k0 + kStep, 1);
+  uint32_t k0 = wave * kDirectRun;
+  if (k0 < depth) {
+    load(k0, 0);
+    for (; k0 + 2 * kStep < depth; k0 += 2 * kStep) {   // no load behind a branch, which would be waited for at once
+      load(k0 + kStep, 1);
+      multiply(k0, 0);
+      load(k0 + 2 * kStep, 0);
+      multiply(k0 + kStep, 1);
+    }
+    if (k0 + kStep < depth) {
+      load(k0 + kStep, 1);
+      multiply(k0, 0);
+      multiply(k0 + kStep, 1);
+    } else {
+      multiply(k0, 0);
+    }
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t)

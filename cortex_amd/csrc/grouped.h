@@ -225,19 +225,26 @@ __device__ __forceinline__ void thin_sums(const float* left, bool absent, const 
       load_columns(mine, r);
     }
   }
-  for (uint32_t k0 = mine; k0 < k_end; k0 += W * BK) {
-    const uint32_t next = k0 + W * BK;
-    if (next < k_end) load_left(next, l_next);
+  auto multiply = [&](int u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e / 4][e % 4], r[u][e / 4][e % 4], sums[u], 0, 0, 0);
+  };
+  uint32_t next = mine + W * BK;
+  for (; next < k_end; next += W * BK) {   // no load behind a branch, which would be waited for at once
+    load_left(next, l_next);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e / 4][e % 4], r[u][e / 4][e % 4], sums[u], 0, 0, 0);
+      multiply(u);
       // the column's next run into the registers of this one
-      if (kB && next < k_end) load_eight(right[kB ? u : 0], next, r[u]);
+      if constexpr (kB) load_eight(right[u], next, r[u]);
     }
-    if (!kB && next < k_end) load_columns(next, r);
+    if constexpr (!kB) load_columns(next, r);
     l[0] = l_next[0];
     l[1] = l_next[1];
+  }
+  if (mine < k_end) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) multiply(u);
   }
 #pragma unroll
   for (int u = 0; u < NT; ++u)

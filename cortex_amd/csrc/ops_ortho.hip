@@ -402,14 +402,22 @@ __device__ __forceinline__ void small_sums(const char* left, uint32_t last_left,
 #pragma unroll
         for (int u = 0; u < 2; ++u) sum[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[slot][t][i / 2], y[slot][u][i % 2], sum[t][u], 0, 0, 0);
   };
-  const uint32_t mine = first + wave;
-  if (mine < end) load(mine, 0);
-  for (uint32_t run = mine; run < end; run += 2 * W) {
-    if (run + W < end) load(run + W, 1);
-    multiply(0);
-    if (run + W >= end) break;
-    if (run + 2 * W < end) load(run + 2 * W, 0);
-    multiply(1);
+  uint32_t run = first + wave;
+  if (run < end) {
+    load(run, 0);
+    for (; run + 2 * W < end; run += 2 * W) {   // no load behind a branch, which would be waited for at once
+      load(run + W, 1);
+      multiply(0);
+      load(run + 2 * W, 0);
+      multiply(1);
+    }
+    if (run + W < end) {
+      load(run + W, 1);
+      multiply(0);
+      multiply(1);
+    } else {
+      multiply(0);
+    }
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t)
