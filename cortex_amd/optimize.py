@@ -247,7 +247,8 @@ class Muon:
 
     in one call of the library.  Parameters are tensors [rows, columns], a row to an output, or [matrices, rows, columns], as those of
     experts are; vectors are for another optimizer.  What lies between the products is kept from step to step, and what was too small
-    for a larger matrix is kept too: a recorded graph may still write to it."""
+    for a larger matrix is kept too: a recorded graph may still write to it.  A step that needs more than any before it allocates, so one is
+    made before a graph of it is recorded; steps of one optimizer do not run on two streams at once."""
     backend: Backend
     optimizer: dict
     _workspaces: list = dataclasses.field(default_factory=list)
