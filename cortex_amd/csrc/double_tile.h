@@ -153,15 +153,11 @@ __device__ __forceinline__ void double_tile(uint32_t depth, Left left, Right rig
 // lane / 16 * 4 and those behind it; sixteen lanes' rows, or columns, of t are t * 16 and those behind it.
 constexpr uint32_t kDirectSide = 32, kDirectPitch = 33, kDirectRun = 16;
 
-template <bool kByRow, bool kTurn = false>
+template <bool kByRow>
 struct DoubleDirect {
   const double* p[2];   // a lane's row, from k 0 on, or its column
   int64_t ld;           // of columns
   bool present[2];
-  // Where rows are a multiple of 32 bytes apart the two loads of every other one change places: 16 bytes of each 32 of sixteen rows
-  // would else fall on half of a cache's banks (1024 x 1024 times its transpose 37 us, and 48).  What it costs (1500 x 1500 93 us, and
-  // 104) is for those that ask for it.  0 or 2.
-  uint32_t turn;
   // `row(i)`: which one is row i of the tile's, none if it is negative
   template <class Row>
   static __device__ __forceinline__ DoubleDirect rows(const double* p, int64_t ld, Row row) {
@@ -173,7 +169,6 @@ struct DoubleDirect {
       d.p[t] = p + (i < 0 ? 0 : i) * ld;
     }
     d.ld = ld;
-    d.turn = kTurn && ld % 4 == 0 ? threadIdx.x % 2 * 2 : 0;
     return d;
   }
   static __device__ __forceinline__ DoubleDirect columns(const double* p, int64_t ld, uint32_t left) {   // of `left` columns
@@ -184,7 +179,6 @@ struct DoubleDirect {
       d.p[t] = p + min(t * 16 + threadIdx.x % 16, left - 1);
     }
     d.ld = ld;
-    d.turn = 0;
     return d;
   }
   __device__ __forceinline__ void load(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
@@ -194,7 +188,7 @@ struct DoubleDirect {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (uint32_t e = 0; e < 4; e += 2) {
-          const f64x2 two = *reinterpret_cast<const f64x2_at_8*>(p[t] + k + (e ^ (kTurn ? turn : 0)));
+          const f64x2 two = *reinterpret_cast<const f64x2_at_8*>(p[t] + k + e);
           x[t][e] = two[0];
           x[t][e + 1] = two[1];
         }
@@ -202,7 +196,7 @@ struct DoubleDirect {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) x[t][e] = p[t][min(k + (e ^ (kTurn ? turn : 0)), end - 1) * (kByRow ? 1 : ld)];
+        for (uint32_t e = 0; e < 4; ++e) x[t][e] = p[t][min(k + e, end - 1) * (kByRow ? 1 : ld)];
     }
   }
   __device__ __forceinline__ void mend(uint32_t k0, uint32_t end, double (&x)[2][4]) const {
@@ -210,9 +204,8 @@ struct DoubleDirect {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[t][e] = present[t] && k + (e ^ (kTurn ? turn : 0)) < end ? x[t][e] : 0.0;
+      for (uint32_t e = 0; e < 4; ++e) x[t][e] = present[t] && k + e < end ? x[t][e] : 0.0;
   }
-  __device__ __forceinline__ double at(const double (&x)[4], int e) const { return kTurn && turn ? x[e ^ 2] : x[e]; }
 };
 
 // Of `depth` k, at least one.  The waves' sums are in `partial` afterwards, for all lanes to read.
@@ -237,8 +230,7 @@ __device__ __forceinline__ void double_direct(uint32_t depth, const Left& left, 
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(left.at(x[slot][t], e), right.at(y[slot][u], e), sum[t][u], 0, 0, 0);
+        for (int u = 0; u < 2; ++u) sum[t][u] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[slot][t][e], y[slot][u][e], sum[t][u], 0, 0, 0);
   };
   constexpr uint32_t kStep = W * kDirectRun;
   uint32_t k0 = wave * kDirectRun;

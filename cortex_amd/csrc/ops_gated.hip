@@ -630,10 +630,9 @@ __global__ void __launch_bounds__(256, 2) gated_gradient_double_kernel(const Gat
 // Smaller products: 32 x 32 sums to a block, straight from memory (double_tile.h).
 constexpr int kDirectWaves = 4;
 
-template <bool kTurn>
 __global__ void __launch_bounds__(64 * kDirectWaves, 2) gated_direct_kernel(const GatedArgs a, const GroupedPlan p) {
   constexpr uint32_t S = kDirectSide, kColumns = S / 2;
-  using Rows = DoubleDirect<true, kTurn>;
+  using Rows = DoubleDirect<true>;
   __shared__ double partial[kDirectWaves][S * kDirectPitch];
   TilePlace at;
   Group g;
@@ -659,10 +658,9 @@ __global__ void __launch_bounds__(64 * kDirectWaves, 2) gated_direct_kernel(cons
   }
 }
 
-template <bool kTurn>
 __global__ void __launch_bounds__(64 * kDirectWaves, 2) gated_gradient_direct_kernel(const GatedArgs a, const GroupedPlan p) {
   constexpr uint32_t S = kDirectSide;
-  using Rows = DoubleDirect<true, kTurn>;
+  using Rows = DoubleDirect<true>;
   __shared__ double partial[kDirectWaves][S * kDirectPitch];
   TilePlace at;
   Group g;
@@ -903,8 +901,7 @@ int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre,
     return run<double, false>("ct_gated_gemm", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
         if (best.height == 64) hipLaunchKernelGGL(gated_double_kernel, grid, dim3(256), 0, s, a, plan);
-        else if (a.g.lda % 4 == 0 || a.g.ldb % 4 == 0) hipLaunchKernelGGL((gated_direct_kernel<true>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
-        else hipLaunchKernelGGL((gated_direct_kernel<false>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
+        else hipLaunchKernelGGL(gated_direct_kernel, grid, dim3(64 * kDirectWaves), 0, s, a, plan);
       }, band);
     });
   }
@@ -964,8 +961,7 @@ int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradien
     return run<double, true>("ct_gated_gemm_gradient", s, args, shape, true, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
       for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
         if (best.height == 64) hipLaunchKernelGGL(gated_gradient_double_kernel, grid, dim3(256), 0, s, a, plan);
-        else if (a.g.lda % 4 == 0) hipLaunchKernelGGL((gated_gradient_direct_kernel<true>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
-        else hipLaunchKernelGGL((gated_gradient_direct_kernel<false>), grid, dim3(64 * kDirectWaves), 0, s, a, plan);
+        else hipLaunchKernelGGL(gated_gradient_direct_kernel, grid, dim3(64 * kDirectWaves), 0, s, a, plan);
       }, band);
     });
   }

@@ -248,6 +248,13 @@ def test_long_sums_of_doubles(stream):  # noqa: F811
     D.free()
 
 
+@pytest.mark.parametrize("size", [(2, 256, 146), (2, 352, 33), (33, 400, 64), (1, 464, 7), (17, 300, 128), (40, 255, 96)], ids=str)
+def test_sums_of_some_hundred_terms_by_few_rows(D, size):
+    """Rows whole lines and parts of lines apart, in products that take every wave several runs of k."""
+    check(D, *size, seed=5)
+    check(D, *size, activation="gelu", pad=4, seed=6)
+
+
 def test_sums_of_no_terms(D):
     """Rows without elements, and an operand without rows: gates and ups of zero."""
     for activation in blocks.GATES:
