@@ -733,9 +733,9 @@ double time_of_few(const Shape& s, int64_t width) {
 constexpr uint32_t kFewK16 = 1024, kFewK64 = 2049;
 
 // Microseconds of tiles of doubles, of 32 a side straight from memory and of 64 by way of LDS, whose cells are finished four at a time and
-// sixteen at a time.  Us of both, forward and gradient: 509 rows, 301 by 517, 16 and 15, 23 and 31; 1000 rows, 700 by 900, 80 and 46, 74 and 57;
-// 4096, 512 by 512, 105 and 61, 95 and 63; 4096, 301 by 517, 73 and 50, 83 and 64; 200, 4096 by 64 in parts 20 and 13.  (Tiles of 32 by way of
-// LDS: 509 rows 18 and 16.)
+// sixteen at a time.  Us of both, forward and gradient: 509 rows, 301 by 517, 16 and 15, 23 and 31; 1000 rows, 700 by 900, 80 and 43, 74 and 57;
+// 4096, 512 by 512, 105 and 66, 95 and 63; 4096, 301 by 517, 81 and 50, 83 and 64; 200, 4096 by 64 in parts 18 and 11.  (Tiles of 32 by way of
+// LDS: 509 rows 18 and 16; 512 rows, 512 by 512, 21 and 16, here 22 and 12.)
 double time_of_direct(int64_t tiles, double k, bool gradient) { return 5.0 + (double)ceil_div(tiles, kUnits) * (0.0117 * k + (gradient ? 1.2 : 0.9)); }
 double time_of_double(int64_t tiles, double k, bool gradient) {
   const double rounds = (double)ceil_div(tiles, kUnits);
