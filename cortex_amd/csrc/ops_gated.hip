@@ -731,6 +731,7 @@ double time_of_few(const Shape& s, int64_t width) {
 }
 // From these many k on a block has sixteen waves, of eight: 51 and 57 us at 4096 k; below 1024 the launch of sixteen takes longer.
 constexpr uint32_t kFewK16 = 1024, kFewK64 = 2049;
+constexpr bool few_waves(int64_t width, uint32_t k) { return k < (width == 64 ? kFewK64 : kFewK16); }
 
 // Microseconds of tiles of doubles, of 32 a side straight from memory and of 64 by way of LDS, whose cells are finished four at a time and
 // sixteen at a time.  Us of both, forward and gradient: 509 rows, 301 by 517, 16 and 15, 23 and 31; 1000 rows, 700 by 900, 80 and 43, 74 and 57;
@@ -843,11 +844,17 @@ int run(const char* name, hipStream_t s, GatedArgs a, const Shape& shape, bool s
   const uint32_t band = best.height == 16 && shape.rows <= 16 * shape.groups ? 1 : kBand;
   launch(a, best, m_tiles, n_tiles, parts.count(), band);
   if (parts.partial()) add_up(parts.count());
-  static const char* const kNames[] = {"gated_thin", "gated_medium", "gated_large", "gated_medium+gated_sum", "gated_large+gated_sum", "gated_double",
-                                       "gated_double+gated_sum"};
-  static const char* const kGradientNames[] = {"gated_gradient_thin", "gated_gradient_medium", "gated_gradient_large", "gated_gradient_medium+gated_sum",
-                                               "gated_gradient_large+gated_sum", "gated_gradient_double", "gated_gradient_double+gated_sum"};
-  const int kernel = std::is_same<T, double>::value ? 5 + (parts.count() > 1) : best.height == 16 ? 0 : 1 + (best.height == 128) + 2 * (parts.count() > 1);
+  static const char* const kNames[] = {"gated_thin", "gated_thin_long", "gated_thin_wide", "gated_thin_wide_long", "gated_medium", "gated_medium+gated_sum",
+                                       "gated_large", "gated_large+gated_sum", "gated_double", "gated_double+gated_sum", "gated_double_tiles",
+                                       "gated_double_tiles+gated_sum"};
+  static const char* const kGradientNames[] = {"gated_gradient_thin", "gated_gradient_thin_long", "gated_gradient_thin_wide", "gated_gradient_thin_wide_long",
+                                               "gated_gradient_medium", "gated_gradient_medium+gated_sum", "gated_gradient_large",
+                                               "gated_gradient_large+gated_sum", "gated_gradient_double", "gated_gradient_double+gated_sum",
+                                               "gated_gradient_double_tiles", "gated_gradient_double_tiles+gated_sum"};
+  const int several = parts.count() > 1;
+  const int kernel = std::is_same<T, double>::value ? (best.height == 64 ? 10 : 8) + several
+                     : best.height == 16            ? (best.width == 64 ? 2 : 0) + !few_waves(best.width, a.g.k)
+                                                    : (best.height == 128 ? 6 : 4) + several;
   note_kernel(kGradient ? kGradientNames[kernel] : kNames[kernel]);
   return after_launch(s);
 }
@@ -907,7 +914,7 @@ int ct_gated_gemm(void* stream, void* inner, int64_t inner_colstride, void* pre,
   }
   return run<float, false>("ct_gated_gemm", s, args, shape, shape.k >= kTileDepth, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
     for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-      const bool few = a.g.k < (best.width == 64 ? kFewK64 : kFewK16);   // k
+      const bool few = few_waves(best.width, a.g.k);
       if (best.height == 128) hipLaunchKernelGGL((gated_split_kernel<128, 128, 4, 2>), grid, dim3(512), 0, s, a, plan);
       else if (best.height == 64) hipLaunchKernelGGL((gated_split_kernel<64, 64, 2, 2>), grid, dim3(256), 0, s, a, plan);
       else if (best.width == 64 && few) hipLaunchKernelGGL((gated_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
@@ -968,7 +975,7 @@ int ct_gated_gemm_gradient(void* stream, void* pre_gradient, int64_t pre_gradien
   const bool split = a_col_count >= kTileDepth && b_colstride <= kMostSplitLd;
   return run<float, true>("ct_gated_gemm_gradient", s, args, shape, split, [&](const GatedArgs& a, const Choice& best, int64_t m_tiles, int64_t n_tiles, int64_t parts, uint32_t band) {
     for_launches(m_tiles, n_tiles, parts, [&](dim3 grid, const GroupedPlan& plan) {
-      const bool few = a.g.k < (best.width == 64 ? kFewK64 : kFewK16);   // k
+      const bool few = few_waves(best.width, a.g.k);
       if (best.height == 128) hipLaunchKernelGGL((gated_gradient_split_kernel<128, 128, 2, 4>), grid, dim3(512), 0, s, a, plan);
       else if (best.height == 64) hipLaunchKernelGGL((gated_gradient_split_kernel<64, 64, 2, 2>), grid, dim3(256), 0, s, a, plan);
       else if (best.width == 64 && few) hipLaunchKernelGGL((gated_gradient_thin_kernel<8, 4>), grid, dim3(512), 0, s, a, plan);
