@@ -16,6 +16,7 @@
 // columns, for one product's sums run along the rows and the other's along the columns.
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
 
 #include "common.h"
 #include "double_tile.h"
@@ -825,18 +826,19 @@ void launch_gram_parts(hipStream_t s, PairArgs a, int64_t count, int64_t parts, 
   hipLaunchKernelGGL(gram_join_kernel, dim3(a.order.units), dim3(256), 0, s, a, (uint32_t)parts, sums, room_bytes / 4);
 }
 
+// The side of the tiles taken.
 template <Product kProduct>
-void launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
+const char* launch_pair(hipStream_t s, const PairArgs& a, int64_t count) {
   auto tiles = [&](int64_t side) { return tiles_of(count, a.m, a.n, side, is_symmetric(kProduct)); };
   const double small = time_of_64(tiles(64), a.runs), medium = time_of_128(tiles(128), a.runs), large = time_of_256(tiles(256), a.runs);
   if constexpr (is_symmetric(kProduct)) {
     const double tall = time_of_tall(tiles_of(count, a.m, a.n, 256, 192, true), a.runs);
-    if (tall < std::min({time_of_32(tiles(kSmallSide), a.runs, true), small, medium, large})) return launch_tile<TileTall, kProduct>(s, a, count);
+    if (tall < std::min({time_of_32(tiles(kSmallSide), a.runs, true), small, medium, large})) return launch_tile<TileTall, kProduct>(s, a, count), "256x192";
   }
-  if (time_of_32(tiles(kSmallSide), a.runs, is_symmetric(kProduct)) <= std::min({small, medium, large})) launch_small<kProduct>(s, a, count);
-  else if (small <= medium && small <= large) launch_tile<Tile64, kProduct>(s, a, count);
-  else if (medium <= large) launch_tile<Tile128, kProduct>(s, a, count);
-  else launch_tile<Tile256, kProduct>(s, a, count);
+  if (time_of_32(tiles(kSmallSide), a.runs, is_symmetric(kProduct)) <= std::min({small, medium, large})) return launch_small<kProduct>(s, a, count), "32";
+  if (small <= medium && small <= large) return launch_tile<Tile64, kProduct>(s, a, count), "64";
+  if (medium <= large) return launch_tile<Tile128, kProduct>(s, a, count), "128";
+  return launch_tile<Tile256, kProduct>(s, a, count), "256";
 }
 
 // Microseconds of `tiles` tiles over `depth` k, of 64 a side by way of LDS and of 32 straight from memory.  Us of both: X X^T of 301 x 517 29
@@ -936,6 +938,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
   double* const partial = reinterpret_cast<double*>(factor + at_once * l.square);
   const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 4096));
   const uint64_t each = (uint64_t)ceil_div(cells, parts);
+  const char *of_gram = "", *of_square = "", *of_update = "", *of_last = "";
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);
     StartArgs start = r.start;
@@ -962,9 +965,12 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
       g.scale = a_scale;
       // X by columns lies in one of two places; the other is free
       const int64_t parts = gram_parts(count, l.m, g.runs, l.turned);
-      if (parts > 1 && time_of_parts(count, l.m, g.runs, parts) < time_of_gram(count, l.m, g.runs))
+      if (parts > 1 && time_of_parts(count, l.m, g.runs, parts) < time_of_gram(count, l.m, g.runs)) {
         launch_gram_parts(s, g, count, parts, turned[(step + 1) & 1], l.turned);
-      else launch_pair<kGram>(s, g, count);
+        of_gram = "parts";
+      } else {
+        of_gram = launch_pair<kGram>(s, g, count);
+      }
       g.left = g.right = gram;
       g.left_stride = g.right_stride = l.square;
       g.runs = (uint32_t)ceil_div(l.m, kPairRun);
@@ -975,7 +981,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
       g.b = (float)cb;
       g.c = (float)cc;
       g.a_unscale = 1.f / a_scale;
-      launch_pair<kSquare>(s, g, count);
+      of_square = launch_pair<kSquare>(s, g, count);
       const bool last = step + 1 == r.steps;
       PairArgs u{};
       u.left = factor;
@@ -992,7 +998,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
         u.by_columns = turned[(step + 1) & 1];
         u.columns_stride = l.turned;
         u.scale = next_scale;
-        launch_pair<kUpdate>(s, u, count);
+        of_update = launch_pair<kUpdate>(s, u, count);
       } else {
         if (tall) {   // the rows of the result are those of X^T
           std::swap(u.left, u.right);
@@ -1004,13 +1010,15 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
         u.out_stride = r.out_stride;
         u.alpha = (float)r.alpha;
         u.beta = (float)r.beta;
-        launch_pair<kLast>(s, u, count);
+        of_last = launch_pair<kLast>(s, u, count);
       }
       most = next;
       x_scale = next_scale;
     }
   }
-  note_kernel("orthogonalize_pair");
+  thread_local char name[96];   // the tiles of each product, of the last matrices
+  std::snprintf(name, sizeof name, "orthogonalize_pair gram %s square %s update %s result %s", of_gram, of_square, of_update, of_last);
+  note_kernel(name);
   return after_launch(s);
 }
 
