@@ -10,10 +10,16 @@
 // done between the products: a I + b A + c A A is formed from the sums as they are stored, and a product stores its results as
 // the next one reads them.
 //
-// Float.  The singular values have a bound that the coefficients give, 1 at first and the largest s (a + b s^2 + c s^4) below the
-// last bound then, and no element of a matrix is larger than its largest singular value.  So the products are those of
-// pair_tile.h, two halves to a float, with scales from these bounds, and matrices lie in pieces between them: X by rows and by
-// columns, for one product's sums run along the rows and the other's along the columns.
+// Float.  The products are those of pair_tile.h, two halves to a float, which hold an element to 2^-39 of a bound.  So that rows, or columns, far
+// below the others keep a float's bits all the same, what is multiplied has powers of two taken out.  With X = D Y, D the
+// diagonal of a power of two to each row that its norm does not exceed, and so no element of Y one,
+//   G = Y Y^T,   M = a I + (b G + c (G D) (G D)^T) D^2,   X after the step = D M Y
+// and M is what a I + b A + c A A is between rows of D Y: of an element of it what matters to its row of Y is held.  For the product
+// with M, whose sums run down the columns of Y, each column of Y has a power of two of its own too.
+//   Where these come from: a row's norm after a step is at most its norm before, which G has on its diagonal, times the largest
+// |a + b s^2 + c s^4|, and the coefficients bound the singular values, 1 at first and the largest s (a + b s^2 + c s^4) below the last bound then.
+// A column's largest element is recorded as it is stored and has a bound after the next step (StepBounds).  All of them are powers of two, so
+// they round nothing.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -149,35 +155,205 @@ __device__ __forceinline__ double inverse_norm(const StartArgs& a, uint32_t matr
   return 1.0 / (sqrt(sum_of_block(x, lds)) + a.epsilon);
 }
 
-// 64 x 64 elements as pieces, by rows and by columns.  The scale is a power of two.
-__global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, uint32_t parts, double scale, char* by_rows, char* by_columns,
+// Powers of two of the rows and columns of X on its shorter side, in the workspace: [matrix][..] each.
+struct Exponents {
+  int *rows, *columns;            // X = 2^(rows) Y, no element of a column of Y above 2^(columns)
+  double* squares;                // sums over strips of the input's rows, [matrix][strip][row]
+  uint32_t* most_columns;         // bits of the largest magnitudes in columns of Y, times 2^kPairTop
+  int64_t stride_squares;
+  uint32_t stride_rows, stride_columns, strips;
+};
+
+// k with x <= 2^k; of 0, and of a NaN, any that no power here reaches.
+template <class T>
+__device__ __forceinline__ int exponent_above(T x) {
+  int k = -2000;
+  if (x > T(0)) (void)frexp(x, &k);
+  return k;
+}
+
+constexpr uint32_t kMostStrips = 16;
+constexpr int kLeastColumn = -100;   // of columns further below the rows' largest
+
+// k with root(squares) <= 2^k.  A row of X has the exponent of its norm in the input and that of 1 / (|input| + epsilon): 2^1 at most, or 2^2 of a
+// row of norm 1, which is a quarter of that then.
+__device__ __forceinline__ int exponent_of_root(double squares) { return (exponent_above(squares * 1.0001) + 1) >> 1; }
+
+// Of a column's largest magnitude, times 2^kPairTop.
+__device__ __forceinline__ int column_of_most(uint32_t most, int growth) {
+  return min(max(exponent_above(__builtin_bit_cast(float, most)) - kPairTop + growth, kLeastColumn), 0);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// Rows and columns of the input that a block reads, 64 of the shorter side and 64 of the longer one: a lane's i-th element.  What is outside
+// repeats the last ones.
+template <bool kTall>
+struct Square64 {
+  uint32_t shorter, longer;       // where it is
+  bool inside;
+  int64_t at;                     // in the input
+  __device__ __forceinline__ Square64(const StartArgs& a, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0, uint32_t i) {
+    const uint32_t lane = threadIdx.x % 64, other = i * 4 + threadIdx.x / 64;   // lanes along the input's rows
+    shorter = m0 + (kTall ? lane : other);
+    longer = n0 + (kTall ? other : lane);
+    inside = shorter < m && longer < n;
+    shorter = min(shorter, m - 1);
+    longer = min(longer, n - 1);
+    at = blockIdx.z * a.stride + (int64_t)(kTall ? longer : shorter) * a.ld + (kTall ? shorter : longer);
+  }
+};
+
+// As start_norm_kernel, and the sums of squares of the input's rows on its shorter side: blocks of 64 of them by strips of 64 `tiles` of the longer
+// side.  Clears the words for the columns' largest.
+template <bool kTall>
+__global__ void __launch_bounds__(256) start_scan_kernel(const StartArgs a, uint32_t tiles, const Exponents e) {
+  __shared__ double lds[4], squares[4][64];
+  const uint32_t m = kTall ? a.columns : a.rows, n = kTall ? a.rows : a.columns, part = blockIdx.y * gridDim.x + blockIdx.x;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  for (uint32_t i = part * 256 + threadIdx.x; i < e.stride_columns; i += gridDim.x * gridDim.y * 256) e.most_columns[blockIdx.z * (int64_t)e.stride_columns + i] = 0;
+  const uint32_t m0 = blockIdx.y * 64, first = blockIdx.x * tiles * 64, end = min(first + tiles * 64, n);
+  double sums[kTall ? 1 : 16] = {};   // of a lane's row; of 16 rows of a wave
+  for (uint32_t n0 = first; n0 < end; n0 += 64) {
+    float x[16], g[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const Square64<kTall> at(a, m, n, m0, n0, i);
+      x[i] = static_cast<const float*>(a.x)[at.at];
+      if (a.gradient) g[i] = static_cast<const float*>(a.gradient)[at.at];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const Square64<kTall> at(a, m, n, m0, n0, i);
+      if (!at.inside) continue;
+      if (a.gradient) {
+        const float step = (float)a.gradient_alpha * g[i];
+        x[i] = (float)a.decay * x[i] + step;
+        static_cast<float*>(a.momentum)[at.at] = x[i];
+        if (a.nesterov) x[i] = step + (float)a.decay * x[i];
+      }
+      sums[kTall ? 0 : i] += (double)x[i] * (double)x[i];
+    }
+  }
+  double mine = sums[0];
+  if constexpr (kTall) {
+    squares[wave][lane] = mine;
+    __syncthreads();
+    if (wave == 0) mine = squares[0][lane] + squares[1][lane] + squares[2][lane] + squares[3][lane];
+  } else {
+    // half of the sums to the other half of the lanes at a time: row i of a wave's is lane 4 i's in the end
+#pragma unroll
+    for (int d = 32; d >= 4; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < d / 4; ++i) {
+        const bool high = lane & d;
+        const double given = high ? sums[i] : sums[i + d / 4];
+        sums[i] = (high ? sums[i + d / 4] : sums[i]) + __shfl_xor(given, d);
+      }
+    mine = sums[0];
+    mine += __shfl_xor(mine, 2);
+    mine += __shfl_xor(mine, 1);
+    if (lane % 4 == 0) squares[0][lane + wave] = mine;   // row i * 4 + wave
+    __syncthreads();
+    if (wave == 0) mine = squares[0][lane];
+  }
+  if (wave == 0 && m0 + lane < m) e.squares[blockIdx.z * e.stride_squares + (int64_t)blockIdx.x * m + m0 + lane] = mine;
+  const double total = sum_of_block(wave == 0 ? mine : 0.0, lds);
+  if (threadIdx.x == 0) a.partial[(int64_t)blockIdx.z * kParts + part] = total;
+}
+
+// The exponents of `count` rows of the input from m0 on, in LDS.
+__device__ __forceinline__ void rows_of_input(const Exponents& e, uint32_t m, uint32_t m0, uint32_t count, int* rows) {
+  for (uint32_t i = threadIdx.x; i < count; i += 256) {
+    const double* from = e.squares + blockIdx.z * e.stride_squares + min(m0 + i, m - 1);
+    double x[kMostStrips], sum = 0.0;
+#pragma unroll
+    for (uint32_t strip = 0; strip < kMostStrips; ++strip) x[strip] = from[(int64_t)min(strip, e.strips - 1) * m];
+#pragma unroll
+    for (uint32_t strip = 0; strip < kMostStrips; ++strip) sum += strip < e.strips ? x[strip] : 0.0;
+    rows[i] = exponent_of_root(sum);
+  }
+}
+
+// The largest magnitudes of the columns of Y, or up to twice those, over strips of the shorter side, kMostAcross squares of 64 at most.
+constexpr uint32_t kMostAcross = 8;
+template <bool kTall>
+__global__ void __launch_bounds__(256) start_columns_kernel(const StartArgs a, uint32_t tiles, const Exponents e) {
+  __shared__ uint32_t most[64];
+  __shared__ int rows[kMostAcross * 64];
+  const uint32_t m = kTall ? a.columns : a.rows, n = kTall ? a.rows : a.columns, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t n0 = blockIdx.y * 64, first = blockIdx.x * tiles * 64, end = min(first + tiles * 64, m);
+  if (threadIdx.x < 64) most[lane] = 0;
+  rows_of_input(e, m, first, tiles * 64, rows);
+  uint32_t found[16] = {};
+  bool ready = false;
+  for (uint32_t m0 = first; m0 < end; m0 += 64) {
+    float x[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) x[i] = start_value<float>(a, Square64<kTall>(a, m, n, m0, n0, i).at);
+    if (!ready) __syncthreads();
+    ready = true;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+      found[i] = max(found[i], magnitude(ldexpf(x[i], kPairTop - rows[Square64<kTall>(a, m, n, m0, n0, i).shorter - first])));
+  }
+  if constexpr (kTall) {
+#pragma unroll
+    for (int d = 32; d >= 4; d >>= 1)   // as start_scan_kernel's sums
+#pragma unroll
+      for (int i = 0; i < d / 4; ++i) {
+        const bool high = lane & d;
+        const uint32_t given = high ? found[i] : found[i + d / 4];
+        found[i] = max(high ? found[i + d / 4] : found[i], (uint32_t)__shfl_xor((int)given, d));
+      }
+    found[0] = max(found[0], (uint32_t)__shfl_xor((int)found[0], 2));
+    found[0] = max(found[0], (uint32_t)__shfl_xor((int)found[0], 1));
+    if (lane % 4 == 0) most[lane + wave] = found[0];
+  } else {
+#pragma unroll
+    for (uint32_t i = 1; i < 16; ++i) found[0] = max(found[0], found[i]);
+    atomicMax(&most[lane], found[0]);
+  }
+  __syncthreads();
+  if (threadIdx.x < 64 && n0 + threadIdx.x < n) atomicMax(&e.most_columns[blockIdx.z * (int64_t)e.stride_columns + n0 + threadIdx.x], most[threadIdx.x]);
+}
+
+// 64 x 64 elements as pieces, by rows of the input and by its columns, and the exponents.
+template <bool kTall>
+__global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, uint32_t parts, const Exponents e, char* by_rows, char* by_columns,
                                                            int64_t stride_rows, int64_t stride_columns) {
   __shared__ double lds[4];
   __shared__ uint32_t cells[64][65];
-  const uint32_t matrix = blockIdx.z, row0 = blockIdx.y * 64, column0 = blockIdx.x * 64;
-  const int64_t base = (int64_t)matrix * a.stride;
-  const uint32_t c = threadIdx.x % 64, column = min(column0 + c, a.columns - 1);
+  __shared__ int of_short[64], of_long[64];
+  const uint32_t matrix = blockIdx.z, row0 = blockIdx.y * 64, column0 = blockIdx.x * 64, m = kTall ? a.columns : a.rows, n = kTall ? a.rows : a.columns;
+  const uint32_t m0 = kTall ? column0 : row0, n0 = kTall ? row0 : column0;
   float values[16];   // on their way while the norm is added up: no branch that lanes take apart
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    values[i] = start_value<float>(a, base + (int64_t)min(row0 + i * 4 + threadIdx.x / 64, a.rows - 1) * a.ld + column);
-  const double factor = inverse_norm(a, matrix, parts, lds) * scale;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t r = i * 4 + threadIdx.x / 64;
-    const float x = row0 + r < a.rows && column0 + c < a.columns ? (float)((double)values[i] * factor) : 0.f;
-    _Float16 hi, lo;
-    split_pair(x, &hi, &lo);
-    cells[r][c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+  for (uint32_t i = 0; i < 16; ++i) values[i] = start_value<float>(a, Square64<kTall>(a, m, n, m0, n0, i).at);
+  const double factor = inverse_norm(a, matrix, parts, lds);
+  const int of_factor = exponent_above(factor);
+  rows_of_input(e, m, m0, 64, of_short);
+  if (threadIdx.x >= 64 && threadIdx.x < 128) {
+    const uint32_t at = n0 + threadIdx.x % 64;
+    const int64_t to = (int64_t)matrix * e.stride_columns + min(at, n - 1);
+    const int k = column_of_most(e.most_columns[to], 0);
+    of_long[threadIdx.x % 64] = k;
+    if (m0 == 0 && at < n) e.columns[to] = k;
   }
   __syncthreads();
-  // eight k of a row to a lane, both pieces: 64 rows of two runs
-  const uint32_t row_runs = (a.columns + kPairRun - 1) / kPairRun, column_runs = (a.rows + kPairRun - 1) / kPairRun;
+  if (n0 == 0 && threadIdx.x < 64 && m0 + threadIdx.x < m) e.rows[(int64_t)matrix * e.stride_rows + m0 + threadIdx.x] = of_short[threadIdx.x] + of_factor;
+  const uint32_t c = threadIdx.x % 64;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t at = i * 256 + threadIdx.x, r = at / 8, k = at % 8 * 8, run = k / 32;
-    auto put = [&](char* to, uint32_t row, uint32_t rows, uint32_t run0, uint32_t runs, bool turned) {
-      if (row >= rows || run0 + run >= runs) return;
+  for (uint32_t i = 0; i < 16; ++i) {
+    const Square64<kTall> at(a, m, n, m0, n0, i);
+    values[i] = at.inside ? (float)ldexp((double)values[i] * factor, kPairTop - of_factor - of_short[at.shorter - m0]) : 0.f;
+  }
+  // eight k of a row to a lane, both pieces: 64 rows of two runs
+  auto put = [&](char* to, uint32_t row0, uint32_t rows, uint32_t k0, uint32_t columns, bool turned) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t at = i * 256 + threadIdx.x, r = at / 8, k = at % 8 * 8, run = (k0 + k) / kPairRun, runs = (columns + kPairRun - 1) / kPairRun;
+      if (row0 + r >= rows || run >= runs) continue;
       pair_u32x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -185,12 +361,24 @@ __global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, ui
         hi[e] = (x & 0xffff) | y << 16;
         lo[e] = x >> 16 | (y & 0xffff0000u);
       }
-      char* p = to + ((int64_t)row * runs + run0 + run) * kPairRunBytes + k % 32 * 2;
+      char* p = to + ((int64_t)(row0 + r) * runs + run) * kPairRunBytes + k % 32 * 2;
       *reinterpret_cast<pair_u32x4*>(p) = hi;
       *reinterpret_cast<pair_u32x4*>(p + 64) = lo;
-    };
-    put(by_rows + matrix * stride_rows, row0 + r, a.rows, column0 / 32, row_runs, false);
-    put(by_columns + matrix * stride_columns, column0 + r, a.columns, row0 / 32, column_runs, true);
+    }
+  };
+#pragma unroll
+  for (int with_columns = 0; with_columns < 2; ++with_columns) {   // Y, and what its columns' powers of two leave of it
+    if (with_columns) __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const uint32_t r = i * 4 + threadIdx.x / 64;
+      _Float16 hi, lo;
+      split_pair(with_columns ? ldexpf(values[i], -of_long[kTall ? r : c]) : values[i], &hi, &lo);
+      cells[r][c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+    }
+    __syncthreads();
+    if ((with_columns != 0) == kTall) put(by_rows + matrix * stride_rows, row0, a.rows, column0, a.columns, false);
+    else put(by_columns + matrix * stride_columns, column0, a.columns, row0, a.rows, true);
   }
 }
 
@@ -212,18 +400,102 @@ struct PairArgs {
   int64_t left_stride, right_stride;  // between matrices, bytes
   TileOrder order;
   uint32_t m, n, runs;
-  float unscale;
+  int shift;                          // powers of two in the sums
   // results as pieces, [m][n] and [n][m]; of a symmetric product only the first
   char *by_rows, *by_columns;
   int64_t rows_stride, columns_stride;
-  float scale;
-  // of kSquare: a I + b A + c (sums), A as it is on the left
-  float a, b, c, a_unscale;
+  int store;                          // powers of two of those
+  const int *row_exponents, *column_exponents;   // of the results' rows and columns, [matrix][..]
+  uint32_t row_exponents_stride, column_exponents_stride;
+  // of kGram and kSquare: G itself, below the diagonal and in the squares of 32 on it, [matrix][m][m]
+  float* gram;
+  int64_t gram_stride;
+  float a, b, c;                      // of kSquare
+  // G's diagonal, as of kGram, and the exponents of the rows that follow from it (next_row); of kUpdate the columns' next ones and largest elements
+  uint32_t* squares;
+  int *next_rows, *next_columns;
+  const uint32_t* most;
+  uint32_t* next_most;
+  uint32_t clear;                     // of kSquare: words of next_most
+  float most_factor;
+  int most_next, least_change, growth;
   // of kLast: out = alpha * (sums) + beta * out
   float* out;
   int64_t ldo, out_stride;
   float alpha, beta;
 };
+
+// The exponent of a row after a step, from its own and its square in G.  |x'| <= |x| most_factor, and below the bound of all singular values.  It
+// falls no faster than by least_change: smaller rows are then just smaller in Y, and a column's growth has a bound.
+__device__ __forceinline__ int next_row(const PairArgs& a, uint32_t square, int exponent) {
+  const int norm = exponent_above(sqrtf(fmaxf(__builtin_bit_cast(float, square), 0.f)) * a.most_factor);
+  return max(min(exponent + norm, a.most_next), exponent + a.least_change);
+}
+
+// What a block's tile needs of exponents, a lane's row and column: read ahead of the products, and put in LDS behind them.
+struct Staged {
+  int row, column;
+  uint32_t square, most;
+};
+template <Product kProduct>
+__device__ __forceinline__ Staged staged_exponents(const PairArgs& a, const TilePlace& at, uint32_t row0, uint32_t column0) {
+  const int64_t row = (int64_t)at.matrix * a.row_exponents_stride + min(row0 + threadIdx.x, a.m - 1);
+  const int64_t column = (int64_t)at.matrix * a.column_exponents_stride + min(column0 + threadIdx.x, a.n - 1);
+  Staged s{a.row_exponents[row], a.column_exponents[column], 0, 0};
+  if constexpr (kProduct == kUpdate) {
+    s.square = a.squares[row];
+    s.most = a.most[column];
+  }
+  return s;
+}
+
+// Of kUpdate's rows by how much they change.  The first tiles of rows and columns record what follows.
+template <Product kProduct>
+__device__ __forceinline__ void put_exponents(const PairArgs& a, const TilePlace& at, uint32_t row0, uint32_t rows, uint32_t column0, uint32_t columns,
+                                              Staged s, int* of_rows, int* of_columns, int* of_next) {
+  if (threadIdx.x < rows) {
+    if constexpr (kProduct == kUpdate) {
+      const int next = next_row(a, s.square, s.row);
+      if (at.n_tile == 0 && row0 + threadIdx.x < a.m) a.next_rows[(int64_t)at.matrix * a.row_exponents_stride + row0 + threadIdx.x] = next;
+      s.row -= next;
+    }
+    of_rows[threadIdx.x] = s.row;
+  }
+  if (threadIdx.x < columns) {
+    of_columns[threadIdx.x] = s.column;
+    if constexpr (kProduct == kUpdate) {
+      const int next = column_of_most(s.most, a.growth);
+      if (at.m_tile == 0 && column0 + threadIdx.x < a.n) a.next_columns[(int64_t)at.matrix * a.column_exponents_stride + column0 + threadIdx.x] = next;
+      of_next[threadIdx.x] = next;
+    }
+  }
+}
+
+// Words that kUpdate records to, before it.
+template <Product kProduct, uint32_t kThreads>
+__device__ __forceinline__ void clear_most(const PairArgs& a) {
+  if constexpr (kProduct == kSquare) {
+    for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < a.clear; i += gridDim.x * kThreads) a.next_most[i] = 0;
+  }
+}
+
+// Two results that are stored of a cell's sum: at (row, column), and at (column, row) of what lies by columns.
+struct Stored {
+  float by_rows, by_columns;
+};
+// `gram`: G's cell.
+template <Product kProduct>
+__device__ __forceinline__ Stored results_of(const PairArgs& a, float sum, float gram, bool diagonal, int row, int column, int next) {
+  if constexpr (kProduct == kGram) {
+    return {ldexpf(sum, column + a.store), ldexpf(sum, row + a.store)};
+  } else if constexpr (kProduct == kSquare) {
+    const float x = a.c * sum + a.b * gram, i = diagonal ? a.a : 0.f;
+    return {ldexpf(ldexpf(x, 2 * column) + i, a.store), ldexpf(ldexpf(x, 2 * row) + i, a.store)};
+  } else {
+    const float x = ldexpf(sum, row + column);
+    return {x, ldexpf(x, -next)};
+  }
+}
 
 // Tiles of SM x SN by WM x WN waves, loads kAhead runs ahead.
 template <int SM_, int SN_, int WM_, int WN_, int kAhead_>
@@ -251,7 +523,7 @@ constexpr uint32_t kImagePitch = 36, kImageWords = 32 * kImagePitch;
 __device__ __forceinline__ void store_lines(const uint32_t* image, uint32_t lane, bool turned, char* to, uint32_t row0, uint32_t rows, uint32_t runs,
                                             uint32_t run) {
   if (run >= runs) return;
-  const uint32_t high = lane >> 2 & 1, k = lane % 4 * 8;
+  const uint32_t pieces = lane >> 2 & 1 ? 0x07060302u : 0x05040100u, k = lane % 4 * 8;   // both words' upper halves, or lower ones
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t r = i * 8 + lane / 8;
@@ -269,7 +541,7 @@ __device__ __forceinline__ void store_lines(const uint32_t* image, uint32_t lane
     }
     pair_u32x4 line;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) line[e] = high ? w[2 * e] >> 16 | (w[2 * e + 1] & 0xffff0000u) : (w[2 * e] & 0xffff) | w[2 * e + 1] << 16;
+    for (int e = 0; e < 4; ++e) line[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], pieces);
     if (row0 + r < rows) *reinterpret_cast<pair_u32x4*>(to + ((int64_t)(row0 + r) * runs + run) * kPairRunBytes + lane % 8 * 16) = line;
   }
 }
@@ -278,12 +550,15 @@ template <class Tile, Product kProduct>
 __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
   constexpr int SM = Tile::SM, SN = Tile::SN, WM = Tile::WM, WN = Tile::WN, MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(SM, SN)];
-  static_assert(WM * WN * kImageWords * 4 <= pair_tile_lds(SM, SN), "an image to a wave");
+  static_assert(WM * WN * kImageWords * 4 + (SM + 2 * SN) * 4 <= pair_tile_lds(SM, SN), "an image to a wave, and exponents");
+  clear_most<kProduct, Tile::T>(a);
   TilePlace at;
   if (!place_of<is_symmetric(kProduct), Tile::kTall>(a.order, &at)) return;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const uint32_t row0 = at.m_tile * SM, column0 = at.n_tile * SN, row_bytes = a.runs * kPairRunBytes;
   if (Tile::kTall && column0 >= a.n) return;   // a last row of tiles may be counted longer than it is
+  static_assert(SM <= Tile::T && SN <= Tile::T, "a row and a column to a lane");
+  const Staged staged = staged_exponents<kProduct>(a, at, row0, column0);
   const char* left = a.left + at.matrix * a.left_stride;
   pair_f32x16 sums[1][MT][NT];
   const PairMatrices<SM, SN, Tile::T> source(left + (int64_t)row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + (int64_t)column0 * row_bytes,
@@ -291,6 +566,11 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
   pair_tile<SM, SN, WM, WN, Tile::kAhead, false>(source, a.runs, lds, tid, sums);
   pair_f32x16 (&sum)[MT][NT] = sums[0];
   const uint32_t wave_m = row0 + wave / WN * (MT * 32), wave_n = column0 + wave % WN * (NT * 32), c = lane & 31, half = lane >> 5;
+  int* const of_rows = reinterpret_cast<int*>(lds) + WM * WN * kImageWords;
+  int *const of_columns = of_rows + SM, *const of_next = of_columns + SN;
+  __syncthreads();
+  put_exponents<kProduct>(a, at, row0, SM, column0, SN, staged, of_rows, of_columns, of_next);
+  __syncthreads();
   if constexpr (kProduct == kLast) {
     float* out = a.out + at.matrix * a.out_stride;
 #pragma unroll
@@ -309,7 +589,7 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float value = a.alpha * (sum[t][u][r] * a.unscale);
+          const float value = a.alpha * ldexpf(sum[t][u][r], a.shift + of_rows[wave_m - row0 + t * 32 + 4 * half + 8 * (r / 4) + r % 4] + of_columns[n - column0]);
           if (8u * (r / 4) + r % 4 < rows) cells[(int64_t)(8 * (r / 4) + r % 4) * a.ldo] = a.beta == 0.f ? value : value + a.beta * before[r];
         }
       }
@@ -320,48 +600,80 @@ __global__ void __launch_bounds__(Tile::T, 2) pair_kernel(const PairArgs a) {
     char* by_rows = a.by_rows + at.matrix * a.rows_stride;
     char* by_columns = is_symmetric(kProduct) ? by_rows : a.by_columns + at.matrix * a.columns_stride;
     uint32_t* image = reinterpret_cast<uint32_t*>(lds) + wave * kImageWords;
-    __syncthreads();
+    float* gram = a.gram + at.matrix * a.gram_stride;
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
+    for (int u = 0; u < NT; ++u) {
+      const uint32_t n0 = wave_n + u * 32;
+      const int column = of_columns[n0 - column0 + c], next = kProduct == kUpdate ? of_next[n0 - column0 + c] : 0;
+      uint32_t most = 0;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const uint32_t m0 = wave_m + t * 32, n0 = wave_n + u * 32;
+        const uint32_t m0 = wave_m + t * 32;
         if (m0 >= a.m || n0 >= a.n || (is_symmetric(kProduct) && m0 < n0)) continue;
-        if constexpr (kProduct == kSquare) {   // A's lines as they are, 144 bytes apart
+        float before[16];   // G's cells, all on their way before the first is used
+        if constexpr (kProduct == kSquare) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t r = i * 8 + lane / 8;
-            *reinterpret_cast<pair_u32x4*>(image + r * kImagePitch + lane % 8 * 4) =
-                *reinterpret_cast<const pair_u32x4*>(left + ((int64_t)min(m0 + r, a.m - 1) * runs_n + n0 / 32) * kPairRunBytes + lane % 8 * 16);
-          }
-          wave_fence();
+          for (int r = 0; r < 16; ++r)
+            before[r] = gram[(int64_t)min(m0 + 8 * (r / 4) + 4 * half + r % 4, a.m - 1) * a.m + min(n0 + c, a.n - 1)];
         }
         float x[16];
+        int of_row[16];   // read ahead: behind a condition each read would be waited for by itself
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          x[r] = sum[t][u][r] * a.unscale;
-          if constexpr (kProduct == kSquare) {
-            const uint32_t row = 8 * (r / 4) + 4 * half + r % 4;
-            const char* cell = reinterpret_cast<const char*>(image + row * kImagePitch) + c * 2;
-            _Float16 hi, lo;
-            __builtin_memcpy(&hi, cell, 2);
-            __builtin_memcpy(&lo, cell + 64, 2);
-            x[r] = a.c * x[r] + a.b * (((float)hi + (float)lo) * a.a_unscale) + (m0 + row == n0 + c ? a.a : 0.f);
+          of_row[r] = of_rows[m0 - row0 + 8 * (r / 4) + 4 * half + r % 4];
+          x[r] = ldexpf(sum[t][u][r], a.shift);
+        }
+        auto results = [&](int r) {
+          return results_of<kProduct>(a, x[r], kProduct == kSquare ? before[r] : 0.f, m0 + 8 * (r / 4) + 4 * half + r % 4 == n0 + c, of_row[r], column, next);
+        };
+        const bool whole = m0 + 32 <= a.m && n0 + 32 <= a.n;
+        auto put = [&](int r, float value) {
+          const uint32_t row = 8 * (r / 4) + 4 * half + r % 4;
+          if (!whole) value = m0 + row < a.m && n0 + c < a.n ? value : 0.f;
+          _Float16 hi, lo;
+          split_pair(value, &hi, &lo);
+          image[row * kImagePitch + c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+        };
+        if constexpr (kProduct == kGram) {
+          float* const cells = gram + (int64_t)(m0 + 4 * half) * a.m + n0 + c;
+          const uint32_t rows = n0 + c < a.n ? a.m - min(m0 + 4 * half, a.m) : 0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8u * (r / 4) + r % 4 < rows) cells[(int64_t)(8 * (r / 4) + r % 4) * a.m] = x[r];
+          if (m0 == n0 && c < a.n - n0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (8u * (r / 4) + 4 * half + r % 4 == c) a.squares[(int64_t)at.matrix * a.row_exponents_stride + n0 + c] = __builtin_bit_cast(uint32_t, x[r]);
           }
         }
-        wave_fence();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const uint32_t row = 8 * (r / 4) + 4 * half + r % 4;
-          _Float16 hi, lo;
-          split_pair(m0 + row < a.m && n0 + c < a.n ? x[r] * a.scale : 0.f, &hi, &lo);
-          image[row * kImagePitch + c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+          const float value = results(r).by_rows;
+          if constexpr (kProduct == kUpdate) most = max(most, magnitude(value));   // rows beyond the last repeat it
+          put(r, value);
         }
         wave_fence();
         store_lines(image, lane, false, by_rows, m0, a.m, runs_n, n0 / 32);
-        if (!is_symmetric(kProduct) || m0 > n0) store_lines(image, lane, true, by_columns, n0, a.n, runs_m, m0 / 32);
+        if (is_symmetric(kProduct) && m0 == n0) {
+          wave_fence();
+          continue;
+        }
+        // one image for both where they are the same, as they mostly are
+        const bool same = is_symmetric(kProduct) ? __all(of_rows[m0 - row0 + c] == column && column == __builtin_amdgcn_readfirstlane(column)) : __all(next == 0);
+        if (!same) {
+          wave_fence();
+#pragma unroll
+          for (int r = 0; r < 16; ++r) put(r, results(r).by_columns);
+          wave_fence();
+        }
+        store_lines(image, lane, true, by_columns, n0, a.n, runs_m, m0 / 32);
         wave_fence();
       }
+      if constexpr (kProduct == kUpdate) {
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+        if (half == 0 && n0 + c < a.n) atomicMax(&a.next_most[(int64_t)at.matrix * a.column_exponents_stride + n0 + c], most);
+      }
+    }
   }
 }
 
@@ -429,56 +741,109 @@ __device__ __forceinline__ void small_sums(const char* left, uint32_t last_left,
   __syncthreads();
 }
 
-// A cell's result: to the image, or where it is for.
-template <Product kProduct>
-__device__ __forceinline__ void finish_small(const PairArgs& a, const TilePlace& at, uint32_t cell, float x, uint32_t* image) {
-  const uint32_t row = cell / kSmallSide, column = cell % kSmallSide, m = at.m_tile * kSmallSide + row, n = at.n_tile * kSmallSide + column;
-  x *= a.unscale;
-  if constexpr (kProduct == kLast) {
-    if (m >= a.m || n >= a.n) return;
-    float& to = a.out[at.matrix * a.out_stride + (int64_t)m * a.ldo + n];
-    to = a.beta == 0.f ? a.alpha * x : a.alpha * x + a.beta * to;
-  } else {
-    if constexpr (kProduct == kSquare) {
-      const char* p = a.left + at.matrix * a.left_stride + ((int64_t)min(m, a.m - 1) * a.runs + at.n_tile) * kPairRunBytes + column * 2;
-      _Float16 hi, lo;
-      __builtin_memcpy(&hi, p, 2);
-      __builtin_memcpy(&lo, p + 64, 2);
-      x = a.c * x + a.b * (((float)hi + (float)lo) * a.a_unscale) + (m == n ? a.a : 0.f);
-    }
-    _Float16 hi, lo;
-    split_pair(m < a.m && n < a.n ? x * a.scale : 0.f, &hi, &lo);
-    image[row * kImagePitch + column] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
-  }
-}
+// What a block of 32 x 32 keeps: images of the results by rows and by columns, and the columns' largest elements.
+struct SmallImage {
+  uint32_t by_rows[kImageWords], by_columns[kImageWords];
+  uint32_t most[kSmallSide];
+};
 
-// Two waves store the image.
+// What a lane's cells (cell i * kThreads + threadIdx.x, all of one column) need besides their sums: read ahead of those.
+template <Product kProduct, uint32_t kThreads>
+struct SmallCells {
+  static constexpr uint32_t kCells = kSmallCells / kThreads;
+  int rows[kCells], column, next = 0;
+  uint32_t squares[kCells], most;
+  float gram[kCells];
+  __device__ __forceinline__ SmallCells(const PairArgs& a, const TilePlace& at, SmallImage& image) {
+    const uint32_t n = min(at.n_tile * kSmallSide + threadIdx.x % kSmallSide, a.n - 1);
+    const int64_t of_row = (int64_t)at.matrix * a.row_exponents_stride, of_column = (int64_t)at.matrix * a.column_exponents_stride;
+    column = a.column_exponents[of_column + n];
+    if constexpr (kProduct == kUpdate) most = a.most[of_column + n];
+#pragma unroll
+    for (uint32_t i = 0; i < kCells; ++i) {
+      const uint32_t m = min(at.m_tile * kSmallSide + (i * kThreads + threadIdx.x) / kSmallSide, a.m - 1);
+      rows[i] = a.row_exponents[of_row + m];
+      if constexpr (kProduct == kUpdate) squares[i] = a.squares[of_row + m];
+      gram[i] = kProduct == kSquare ? a.gram[at.matrix * a.gram_stride + (int64_t)m * a.m + n] : 0.f;
+    }
+    if (threadIdx.x < kSmallSide) image.most[threadIdx.x] = 0;
+  }
+  // Behind the sums: the exponents after the step, which the first tiles of rows and columns record.
+  __device__ __forceinline__ void step(const PairArgs& a, const TilePlace& at) {
+    if constexpr (kProduct == kUpdate) {
+      next = column_of_most(most, a.growth);
+      const uint32_t n = at.n_tile * kSmallSide + threadIdx.x;
+      if (at.m_tile == 0 && threadIdx.x < kSmallSide && n < a.n) a.next_columns[(int64_t)at.matrix * a.column_exponents_stride + n] = next;
+#pragma unroll
+      for (uint32_t i = 0; i < kCells; ++i) {
+        const uint32_t m = at.m_tile * kSmallSide + (i * kThreads + threadIdx.x) / kSmallSide;
+        const int next_one = next_row(a, squares[i], rows[i]);
+        if (at.n_tile == 0 && threadIdx.x % kSmallSide == 0 && m < a.m) a.next_rows[(int64_t)at.matrix * a.row_exponents_stride + m] = next_one;
+        rows[i] -= next_one;
+      }
+    }
+  }
+  // The i-th cell's result: to the images, or where it is for.
+  __device__ __forceinline__ void finish(const PairArgs& a, const TilePlace& at, uint32_t i, float x, SmallImage& image) {
+    const uint32_t cell = i * kThreads + threadIdx.x, row = cell / kSmallSide, c = cell % kSmallSide, m = at.m_tile * kSmallSide + row, n = at.n_tile * kSmallSide + c;
+    const bool inside = m < a.m && n < a.n;
+    if constexpr (kProduct == kLast) {
+      if (!inside) return;
+      x = ldexpf(x, a.shift + rows[i] + column);
+      float& to = a.out[at.matrix * a.out_stride + (int64_t)m * a.ldo + n];
+      to = a.beta == 0.f ? a.alpha * x : a.alpha * x + a.beta * to;
+    } else {
+      x = ldexpf(x, a.shift);
+      if (kProduct == kGram && inside) {
+        a.gram[at.matrix * a.gram_stride + (int64_t)m * a.m + n] = x;
+        if (m == n) a.squares[(int64_t)at.matrix * a.row_exponents_stride + m] = __builtin_bit_cast(uint32_t, x);
+      }
+      const Stored to = results_of<kProduct>(a, x, gram[i], m == n, rows[i], column, next);
+      if (kProduct == kUpdate && inside) atomicMax(&image.most[c], magnitude(to.by_rows));
+      auto put = [&](uint32_t* words, float value) {
+        _Float16 hi, lo;
+        split_pair(inside ? value : 0.f, &hi, &lo);
+        words[row * kImagePitch + c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+      };
+      put(image.by_rows, to.by_rows);
+      put(image.by_columns, to.by_columns);
+    }
+  }
+};
+
+// Two waves store the images.
 template <Product kProduct>
-__device__ __forceinline__ void store_small(const PairArgs& a, const TilePlace& at, const uint32_t* image) {
+__device__ __forceinline__ void store_small(const PairArgs& a, const TilePlace& at, const SmallImage& image) {
   const uint32_t runs_n = (a.n + kPairRun - 1) / kPairRun, runs_m = (a.m + kPairRun - 1) / kPairRun, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   __syncthreads();
-  if (wave == 0) store_lines(image, lane, false, a.by_rows + at.matrix * a.rows_stride, at.m_tile * kSmallSide, a.m, runs_n, at.n_tile);
+  if (wave == 0) store_lines(image.by_rows, lane, false, a.by_rows + at.matrix * a.rows_stride, at.m_tile * kSmallSide, a.m, runs_n, at.n_tile);
   if (wave == 1 && (!is_symmetric(kProduct) || at.m_tile != at.n_tile))
-    store_lines(image, lane, true, is_symmetric(kProduct) ? a.by_rows + at.matrix * a.rows_stride : a.by_columns + at.matrix * a.columns_stride,
+    store_lines(image.by_columns, lane, true, is_symmetric(kProduct) ? a.by_rows + at.matrix * a.rows_stride : a.by_columns + at.matrix * a.columns_stride,
                 at.n_tile * kSmallSide, a.n, runs_m, at.m_tile);
+  if (kProduct == kUpdate && wave == 2 && lane < kSmallSide && at.n_tile * kSmallSide + lane < a.n)
+    atomicMax(&a.next_most[(int64_t)at.matrix * a.column_exponents_stride + at.n_tile * kSmallSide + lane], image.most[lane]);
 }
 
 template <int W, Product kProduct>
 __global__ void __launch_bounds__(64 * W, 4) pair_small_kernel(const PairArgs a) {
   __shared__ float partial[W][kSmallCells];
-  __shared__ __attribute__((aligned(16))) uint32_t image[kImageWords];
+  __shared__ __attribute__((aligned(16))) SmallImage image;
+  clear_most<kProduct, 64 * W>(a);
   TilePlace at;
   if (!place_of<is_symmetric(kProduct)>(a.order, &at)) return;
   const int64_t row_bytes = (int64_t)a.runs * kPairRunBytes;
   const uint32_t row0 = at.m_tile * kSmallSide, column0 = at.n_tile * kSmallSide;
+  SmallCells<kProduct, 64 * W> cells(a, at, image);
   small_sums<W>(a.left + at.matrix * a.left_stride + row0 * row_bytes, a.m - 1 - row0, a.right + at.matrix * a.right_stride + column0 * row_bytes,
                 a.n - 1 - column0, row_bytes, 0, a.runs, partial);
+  cells.step(a, at);
 #pragma unroll
-  for (uint32_t i = threadIdx.x; i < kSmallCells; i += 64 * W) {
-    float x = partial[0][i];
+  for (uint32_t i = 0; i < cells.kCells; ++i) {
+    const uint32_t cell = i * 64 * W + threadIdx.x;
+    float x = partial[0][cell];
 #pragma unroll
-    for (int w = 1; w < W; ++w) x += partial[w][i];
-    finish_small<kProduct>(a, at, i, x, image);
+    for (int w = 1; w < W; ++w) x += partial[w][cell];
+    cells.finish(a, at, i, x, image);
   }
   if constexpr (kProduct != kLast) store_small<kProduct>(a, at, image);
 }
@@ -508,9 +873,10 @@ __global__ void __launch_bounds__(64 * kPartWaves, 4) gram_part_kernel(const Pai
 }
 
 __global__ void __launch_bounds__(256) gram_join_kernel(const PairArgs a, uint32_t parts, const float* sums, int64_t sums_stride) {
-  __shared__ __attribute__((aligned(16))) uint32_t image[kImageWords];
+  __shared__ __attribute__((aligned(16))) SmallImage image;
   TilePlace at;
   if (!place_of_unit<true>(a.order, blockIdx.x, &at)) return;
+  SmallCells<kGram, 256> cells(a, at, image);
   const float* from = sums + at.matrix * sums_stride + (int64_t)(blockIdx.x - at.matrix * a.order.tiles) * parts * kSmallCells + threadIdx.x;
   float x[kSmallCells / 256] = {};
   for (uint32_t part0 = 0; part0 < parts; part0 += 8) {   // loads of eight parts on their way
@@ -525,7 +891,7 @@ __global__ void __launch_bounds__(256) gram_join_kernel(const PairArgs a, uint32
       for (uint32_t i = 0; i < kSmallCells / 256; ++i) x[i] += part0 + p < parts ? y[p][i] : 0.f;
   }
 #pragma unroll
-  for (uint32_t i = 0; i < kSmallCells / 256; ++i) finish_small<kGram>(a, at, i * 256 + threadIdx.x, x[i], image);
+  for (uint32_t i = 0; i < kSmallCells / 256; ++i) cells.finish(a, at, i, x[i], image);
   store_small<kGram>(a, at, image);
 }
 
@@ -713,6 +1079,7 @@ int64_t spread_rows(int64_t doubles) { return ceil_div(std::max<int64_t>(doubles
 struct Layout {
   int64_t m, n;                                  // the shorter side and the longer one
   int64_t x, turned, square, partial, matrix;   // matrix: of all that belongs to one
+  int64_t row_words, column_words;               // of floats: words of an array with one to each row (three of these), or column (four), of the shorter side
   int64_t ldx, ld_square;                        // of doubles
   Layout(int64_t rows, int64_t columns, int dtype) : m(std::min(rows, columns)), n(std::max(rows, columns)) {
     if (dtype == CT_F32) {
@@ -726,7 +1093,9 @@ struct Layout {
       square = aligned(m * ld_square * 8);
     }
     partial = kParts * 8;
-    matrix = (dtype == CT_F32 ? x : 0) + 2 * turned + 2 * square + partial;
+    row_words = ceil_div(m, 64) * 64;
+    column_words = ceil_div(n, 64) * 64;
+    matrix = (dtype == CT_F32 ? x + 3 * row_words * 4 + 4 * column_words * 4 : 0) + 2 * turned + 2 * square + partial;
     if (dtype == CT_F32 && m <= kMostFew) matrix = std::max(matrix, aligned(few_bytes(m, n)));
   }
 };
@@ -817,6 +1186,7 @@ int64_t gram_parts(int64_t count, int64_t m, int64_t runs, int64_t bytes) {
   return std::min({2 * kUnits / (count * tiles), ceil_div(runs, kPartWaves), bytes / (tiles * (int64_t)kSmallCells * 4)});
 }
 
+// `room`: of a matrix, the others' are room_bytes apart.
 void launch_gram_parts(hipStream_t s, PairArgs a, int64_t count, int64_t parts, void* room, int64_t room_bytes) {
   a.order = order_of(count, a.m, a.n, kSmallSide, true);
   const uint32_t part_runs = (uint32_t)ceil_div(a.runs, parts);
@@ -904,12 +1274,36 @@ double most_of_step(double a, double b, double c, double most) {
   return found;
 }
 
-// The power of two that takes `bound`, and what rounding adds, to 2^kPairTop at most.
-float scale_for(double bound) {
+// k with 1.02 bound, for what rounding adds, at most 2^k.
+int exponent_of(double bound) {
   int exponent;
-  std::frexp(std::max(1.02 * bound, 0x1p-40), &exponent);   // 1.02 bound <= 2^exponent
-  return std::ldexp(1.f, kPairTop - exponent);
+  std::frexp(std::max(1.02 * bound, 0x1p-900), &exponent);
+  return exponent;
 }
+
+// A row's exponent falls by that of the largest |a + b s^2 + c s^4| less this in a step at most.
+constexpr int kMostFall = 6;
+
+// What a step of floats needs to know of its coefficients, for singular values up to `most`.
+struct StepBounds {
+  double next, factor;   // of the singular values after it, and the largest |a + b s^2 + c s^4|
+  int factor_exponent, m_exponent, growth;
+  StepBounds(double a, double b, double c, double most, int64_t m) {
+    const double squares = most * most;
+    factor = most_of_factor(a, b, c, squares);
+    next = most_of_step(a, b, c, squares);
+    factor_exponent = exponent_of(factor);
+    // |b + c s|, and root(s) |b + c s|
+    const double of_rows = std::max(std::abs(b), std::abs(b + c * squares)), of_columns = std::max(most * of_rows, 0.0), largest = std::ldexp(1.0, exponent_of(most));
+    // M = a I + (b G + c G D D G) D^2, |G D D G| <= the norms of two rows of Y, at most 1, times squares
+    m_exponent = exponent_of(std::abs(a) + largest * largest * of_rows);
+    // A row of M times a column of Y: |a| of the column's largest; and the root of the sum of the squares of D, largest * root(m) at most, times
+    // that of (the rest of M's row) / D, which is a row of Y times (b + c X^T X) X^T; both as the row's exponent falls
+    const double fall = std::ldexp(1.0, kMostFall - factor_exponent);
+    const double rest = factor > 0 ? std::max(1.0 / factor, next > 0 ? most / next : 0.0) : 0.0;
+    growth = std::max(0, exponent_of(std::abs(a) * fall + std::sqrt((double)m) * largest * of_columns * std::min(fall, rest)));
+  }
+};
 
 struct Request {
   StartArgs start;
@@ -928,81 +1322,125 @@ constexpr double kMostValue = 0x1p40;
 // Of floats, whose A A has values of the fourth power, before the last step; and what A is multiplied by to leave its scale is a float.
 constexpr double kMostFloat = 0x1p30;
 
+// The norm, the exponents of rows and columns, and Y in pieces.  Strips are as many as fill the chip, those over the longer side kMostStrips at most.
+void launch_start(hipStream_t s, const StartArgs& a, Exponents e, uint32_t count, bool tall, char* by_rows, char* by_columns, int64_t stride_rows,
+                  int64_t stride_columns) {
+  const int64_t of_rows = ceil_div(a.rows, 64), of_columns = ceil_div(a.columns, 64), shorter = tall ? of_columns : of_rows, longer = tall ? of_rows : of_columns;
+  const int64_t most = std::min<int64_t>({kMostStrips, kParts / shorter, std::max<int64_t>(1, 8 * kUnits / (count * shorter))}), tiles = ceil_div(longer, std::min(most, longer));
+  e.strips = (uint32_t)ceil_div(longer, tiles);
+  const uint32_t parts = (uint32_t)(e.strips * shorter);
+  const int64_t across = std::min<int64_t>({std::max<int64_t>(1, count * shorter * longer / (8 * kUnits)), shorter, kMostAcross});
+  const dim3 over_longer(e.strips, (uint32_t)shorter, count), over_shorter((uint32_t)ceil_div(shorter, across), (uint32_t)longer, count);
+  const dim3 all((uint32_t)of_columns, (uint32_t)of_rows, count);
+  auto launch = [&](auto is_tall) {
+    constexpr bool kTall = decltype(is_tall)::value;
+    hipLaunchKernelGGL((start_scan_kernel<kTall>), over_longer, dim3(256), 0, s, a, (uint32_t)tiles, e);
+    hipLaunchKernelGGL((start_columns_kernel<kTall>), over_shorter, dim3(256), 0, s, a, (uint32_t)across, e);
+    hipLaunchKernelGGL((start_pieces_kernel<kTall>), all, dim3(256), 0, s, a, parts, e, by_rows, by_columns, stride_rows, stride_columns);
+  };
+  if (tall) launch(std::true_type{});
+  else launch(std::false_type{});
+}
+
 int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once) {
   const bool tall = r.rows > r.columns;
   char* const base = static_cast<char*>(r.workspace);
   char* const x = base;
   char* turned[2] = {x + at_once * l.x, x + at_once * (l.x + l.turned)};
-  char* const gram = turned[1] + at_once * l.turned;
-  char* const factor = gram + at_once * l.square;
+  char* const square = turned[1] + at_once * l.turned;
+  char* const factor = square + at_once * l.square;
   double* const partial = reinterpret_cast<double*>(factor + at_once * l.square);
-  const int64_t cells = r.rows * r.columns, parts = std::min<int64_t>(kParts, ceil_div(cells, 4096));
-  const uint64_t each = (uint64_t)ceil_div(cells, parts);
+  int* const words = reinterpret_cast<int*>(partial + at_once * kParts);
+  int* of_rows[2] = {words, words + at_once * l.row_words};
+  int* of_columns[2] = {words + at_once * 2 * l.row_words, words + at_once * (2 * l.row_words + l.column_words)};
+  uint32_t* const recorded = reinterpret_cast<uint32_t*>(of_columns[1] + at_once * l.column_words);
+  const int64_t gram_bytes = aligned(l.m * l.m * 4);
   const char *of_gram = "", *of_square = "", *of_update = "", *of_last = "";
   for (int64_t first = 0; first < r.count; first += at_once) {
     const int64_t count = std::min(at_once, r.count - first);
+    uint32_t *const of_squares = recorded, *most_of[2] = {recorded + at_once * l.row_words, recorded + at_once * (l.row_words + l.column_words)};
     StartArgs start = r.start;
     start.move(first * start.stride * 4);
     start.partial = partial;
-    hipLaunchKernelGGL((start_norm_kernel<float>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
-                       start.ld == r.columns);
+    // the sums of the input's rows are where Y by columns is next
+    const Exponents exponents{of_rows[0], of_columns[0], reinterpret_cast<double*>(turned[1]), most_of[0], l.turned / 8, (uint32_t)l.row_words,
+                              (uint32_t)l.column_words, 0};
+    launch_start(s, start, exponents, (uint32_t)count, tall, tall ? turned[0] : x, tall ? x : turned[0], tall ? l.turned : l.x, tall ? l.x : l.turned);
     double most = 1.0;
-    float x_scale = scale_for(most);
-    hipLaunchKernelGGL(start_pieces_kernel, dim3((uint32_t)ceil_div(r.columns, 64), (uint32_t)ceil_div(r.rows, 64), (uint32_t)count), dim3(256), 0, s,
-                       start, (uint32_t)parts, (double)x_scale, tall ? turned[0] : x, tall ? x : turned[0], tall ? l.turned : l.x, tall ? l.x : l.turned);
     for (int step = 0; step < r.steps; ++step) {
-      const double *k = r.coefficients + 3 * step, ca = k[0], cb = k[1], cc = k[2];
-      const double most_factor = most_of_factor(ca, cb, cc, most * most), next = most_of_step(ca, cb, cc, most * most);
-      const float a_scale = scale_for(most * most), b_scale = scale_for(most_factor), next_scale = scale_for(next);
+      const double* k = r.coefficients + 3 * step;
+      const StepBounds bounds(k[0], k[1], k[2], most, l.m);
+      const int now = step & 1, next = now ^ 1, most_exponent = exponent_of(most);
+      const bool last = step + 1 == r.steps;
       PairArgs g{};
       g.left = g.right = x;
       g.left_stride = g.right_stride = l.x;
       g.m = g.n = (uint32_t)l.m;
       g.runs = (uint32_t)ceil_div(l.n, kPairRun);
-      g.unscale = 1.f / (x_scale * x_scale);
-      g.by_rows = gram;
+      g.shift = -2 * kPairTop;
+      g.by_rows = square;
       g.rows_stride = l.square;
-      g.scale = a_scale;
-      // X by columns lies in one of two places; the other is free
-      const int64_t parts = gram_parts(count, l.m, g.runs, l.turned);
+      g.store = kPairTop - most_exponent;
+      g.row_exponents = g.column_exponents = of_rows[now];
+      g.row_exponents_stride = g.column_exponents_stride = (uint32_t)l.row_words;
+      // Y by columns lies in one of two places; the other has room for G, and behind it for sums of parts of k
+      g.gram = reinterpret_cast<float*>(turned[next]);
+      g.gram_stride = l.turned / 4;
+      g.squares = of_squares;
+      const int64_t parts = gram_parts(count, l.m, g.runs, l.turned - gram_bytes);
       if (parts > 1 && time_of_parts(count, l.m, g.runs, parts) < time_of_gram(count, l.m, g.runs)) {
-        launch_gram_parts(s, g, count, parts, turned[(step + 1) & 1], l.turned);
+        launch_gram_parts(s, g, count, parts, turned[next] + gram_bytes, l.turned);
         of_gram = "parts";
       } else {
         of_gram = launch_pair<kGram>(s, g, count);
       }
-      g.left = g.right = gram;
+      g.left = g.right = square;
       g.left_stride = g.right_stride = l.square;
       g.runs = (uint32_t)ceil_div(l.m, kPairRun);
-      g.unscale = 1.f / (a_scale * a_scale);
+      g.shift = 2 * (most_exponent - kPairTop);
       g.by_rows = factor;
-      g.scale = b_scale;
-      g.a = (float)ca;
-      g.b = (float)cb;
-      g.c = (float)cc;
-      g.a_unscale = 1.f / a_scale;
+      g.store = kPairTop - bounds.m_exponent;
+      g.a = (float)k[0];
+      g.b = (float)k[1];
+      g.c = (float)k[2];
+      g.next_most = most_of[next];
+      g.clear = last ? 0 : (uint32_t)(count * l.column_words);
       of_square = launch_pair<kSquare>(s, g, count);
-      const bool last = step + 1 == r.steps;
       PairArgs u{};
       u.left = factor;
       u.left_stride = l.square;
-      u.right = turned[step & 1];
+      u.right = turned[now];
       u.right_stride = l.turned;
       u.m = (uint32_t)l.m;
       u.n = (uint32_t)l.n;
       u.runs = (uint32_t)ceil_div(l.m, kPairRun);
-      u.unscale = 1.f / (b_scale * x_scale);
+      u.row_exponents = of_rows[now];
+      u.row_exponents_stride = (uint32_t)l.row_words;
+      u.column_exponents = of_columns[now];
+      u.column_exponents_stride = (uint32_t)l.column_words;
       if (!last) {
+        u.shift = bounds.m_exponent - kPairTop;
         u.by_rows = x;
         u.rows_stride = l.x;
-        u.by_columns = turned[(step + 1) & 1];
+        u.by_columns = turned[next];
         u.columns_stride = l.turned;
-        u.scale = next_scale;
+        u.squares = of_squares;
+        u.next_rows = of_rows[next];
+        u.next_columns = of_columns[next];
+        u.most = most_of[now];
+        u.next_most = most_of[next];
+        u.most_factor = (float)(1.02 * bounds.factor);
+        u.most_next = exponent_of(bounds.next);
+        u.least_change = bounds.factor_exponent - kMostFall;
+        u.growth = bounds.growth;
         of_update = launch_pair<kUpdate>(s, u, count);
       } else {
+        u.shift = bounds.m_exponent - 2 * kPairTop;
         if (tall) {   // the rows of the result are those of X^T
           std::swap(u.left, u.right);
           std::swap(u.left_stride, u.right_stride);
+          std::swap(u.row_exponents, u.column_exponents);
+          std::swap(u.row_exponents_stride, u.column_exponents_stride);
           std::swap(u.m, u.n);
         }
         u.out = static_cast<float*>(r.out) + first * r.out_stride;
@@ -1012,8 +1450,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
         u.beta = (float)r.beta;
         of_last = launch_pair<kLast>(s, u, count);
       }
-      most = next;
-      x_scale = next_scale;
+      most = bounds.next;
     }
   }
   thread_local char name[96];   // the tiles of each product, of the last matrices

@@ -740,8 +740,10 @@ int ct_adadelta_step(void* stream, int dtype, double decay, double epsilon, void
  * chip; with fewer, down to those that it gives for one matrix, the matrices take turns.
  * Each side is 2^21 at most, a matrix below 2^31 elements, 1 <= steps <= 64; coefficients that let a singular value grow
  * beyond 2^40, of floats beyond 2^30 before the last step, are refused.  The squares are summed in double.  An infinity or a NaN makes its matrix NaN, its matrix only.
- * Float: sums are float ones of products of two halves to an element; what is below 2^-39 of the largest singular value that the
- * coefficients allow (or of 2^-40, if that is larger) is 0 there.  Of float matrices with a side of 64 or less the sums are double ones (if these steps do not make what
+ * Float: sums are float ones of products of two halves to an element, with a power of two to each row and each column taken out, so that
+ * rows and columns far below the others have results as accurate, of their own size, as products of floats give (columns on the longer side
+ * down to 2^-100 of the others).  An element that is 2^-28 or less of the largest of its row and of its column may count as 0.
+ * Of float matrices with a side of 64 or less the sums are double ones (if these steps do not make what
  * is 0 but for rounding more than 2^24 times as large).  dtype is CT_F32 or CT_F64. */
 int ct_orthogonalize_workspace(int64_t count, int64_t rows, int64_t columns, int dtype, int64_t* bytes);
 int ct_orthogonalize(void* stream, void* output, int64_t output_colstride, int64_t output_stride,

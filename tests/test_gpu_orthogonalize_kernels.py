@@ -11,7 +11,7 @@ from cortex_amd import driver as drv
 from cortex_amd import optimize
 from cortex_amd import tensor as ct
 from test_gpu_blocks import UNIT, Owned, as_released, read, stream  # noqa: F401
-from test_gpu_orthogonalize import COEFFICIENTS, MILD, bar_of, gradient, near, step64
+from test_gpu_orthogonalize import COEFFICIENTS, MILD, bar_of, gradient, near, orthogonal64, step64
 
 pytestmark = pytest.mark.gpu
 
@@ -234,3 +234,56 @@ def test_recorded_into_a_graph(as_released, shape):  # noqa: F811
         assert rt.hipGraphExecDestroy(executable) == 0 and rt.hipGraphDestroy(graph) == 0
     D.free()
     stream.release()
+
+
+def bars_of(g, u, **kwargs):
+    """As bar_of, of each row and of each column by itself."""
+    rng = np.random.default_rng(5)
+    exact = orthogonal64(g, **kwargs)
+    moved = [orthogonal64(g, noise=u, rng=rng, **kwargs) - exact for _ in range(3)]
+    return exact, [6 * np.max([np.linalg.norm(x, axis=axis) for x in moved], axis=0) for axis in (1, 0)]
+
+
+MAGNITUDES = [(1, 200, 400), (1, 400, 200), (3, 640, 700), (1, 70, 3000), (2, 3001, 70), (26, 93, 2362), (12, 1245, 715), (30, 752, 1249), (15, 957, 2155)]
+
+
+@pytest.mark.parametrize("steps", [1, 5])
+@pytest.mark.parametrize("of", ["rows", "columns", "both"])
+@pytest.mark.parametrize("shape", MAGNITUDES, ids=str)
+def test_rows_and_columns_of_unlike_magnitudes(D, shape, of, steps):
+    """Rows of outputs, or columns of features, that are seldom used: each is held to a float's bits of itself, as products of floats hold it.  With
+    the bars of the other tests, row by row and column by column; noise of the terms' magnitudes is as small as the row."""
+    rng = np.random.default_rng(41)
+    count, rows, columns = shape
+    one = rng.standard_normal((rows, columns))
+    if of != "columns":
+        one *= 2.0 ** -rng.integers(0, 40, (rows, 1))
+    if of != "rows":
+        one *= 2.0 ** -rng.integers(0, 40, (1, columns))
+    g, out = D.tensor(np.broadcast_to(one, shape)), D.tensor(np.zeros(shape))
+    optimize.orthogonalize(D.backend, out, g, steps=steps)
+    taken()
+    got = read(out)
+    want, bars = bars_of(read(g)[0], U, steps=steps)
+    assert np.all(np.isfinite(got))
+    for bar, axis in zip(bars, (1, 0)):
+        off = np.linalg.norm(got[0] - want, axis=axis) / bar
+        assert np.all(off <= 1), (("row", "column")[axis == 0], int(off.argmax()), float(off.max()))
+    assert np.array_equal(got, np.broadcast_to(got[0], shape))
+
+
+def test_magnitudes_over_the_whole_range(D):
+    """Rows from 2^100 down to the least numbers: what the largest ones leave of the others is a float, or 0."""
+    rng = np.random.default_rng(42)
+    for shape in ((130, 300), (300, 130)):
+        data = rng.standard_normal(shape)
+        short = 0 if shape[0] < shape[1] else 1
+        data *= np.expand_dims(2.0 ** np.linspace(100, -145, shape[short]), 1 - short)
+        g, out = D.tensor(data), D.tensor(np.zeros(shape))
+        optimize.orthogonalize(D.backend, out, g, epsilon=0.0)
+        taken()
+        want, bars = bars_of(read(g), U, epsilon=0.0)
+        got = read(out)
+        assert np.all(np.isfinite(got))
+        off = np.linalg.norm(got - want, axis=1 - short)
+        assert np.all(off <= bars[short] + 2.0 ** -149 * np.sqrt(max(shape)))
