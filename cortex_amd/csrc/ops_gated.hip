@@ -279,17 +279,24 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_gradient_split_kernel(c
 // the left one and columns of the right one have a power of two each, so that an element is held to 2^-23 of itself, or to 2^-51 of the
 // largest of its row (or column) if that is more.  The chip's power bounds both kinds: 8192 rows, 1024 k, 5632 gates and ups 340 us
 // with the splitting, with three pieces 600.  What is not finite has no power of two: rows of a NaN are NaN, and results of a row or column of infinities are
-// formed once more from the floats.
-constexpr int kAbsentRow = 1000, kRowOfNan = 1001, kRowOfInfinity = 1002;   // in the place of a row's exponent
+// formed once more from the floats.  So are sums that are small beside what a row or column with elements below 2^-28 of its largest may be off by
+// (the large elements meet small ones, or none): no element of a float is held to less in them than in a product of floats.
+//
+// In the place of a row's exponent: twice the exponent, one more if it has such elements.
+constexpr int kRowOfZeros = -2000, kAbsentRow = 2000, kRowOfNan = 2002, kRowOfInfinity = 2004;
 
-// The exponent for a row whose largest magnitude has these bits.
-__device__ __forceinline__ int exponent_for(uint32_t most) {
+// For a row whose largest magnitude has these bits, and the least one that is not 0.
+__device__ __forceinline__ int exponent_for(uint32_t most, uint32_t least) {
   if (most > 0x7f800000u) return kRowOfNan;
   if (most == 0x7f800000u) return kRowOfInfinity;
-  if (most == 0) return 0;
-  const int log2 = most >> 23 ? (int)(most >> 23) - 127 : 31 - __clz(most) - 149;
-  return kPairTop - log2;
+  if (most == 0) return kRowOfZeros;
+  const int log2 = most >> 23 ? (int)(most >> 23) - 127 : 31 - __clz(most) - 149, exponent = kPairTop - log2;
+  return 2 * exponent + (ldexpf(__builtin_bit_cast(float, least), exponent) < 0x1p-13f);
 }
+__device__ __forceinline__ int power_of(int exponent) { return exponent >> 1; }
+// In the scale of the pieces elements below 2^-13 are off by 2^-36 at most, and what they are multiplied by is below 2^15: a sum of k products is off by
+// 2 k 2^-21 for both operands, 2^-24 of the sums from here on.
+__device__ __forceinline__ float least_sum(uint32_t k) { return 16.f * (float)k; }
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 
@@ -297,7 +304,7 @@ struct PiecesArgs {
   const float* x;      // matrices of `rows` rows (or, of a right operand by columns, k of them)
   char* pieces;
   int* exponents;
-  uint32_t* partial;   // [matrix][part][row], by columns
+  uint32_t* partial;   // [matrix][part][largest least][row], by columns
   int64_t ld, stride;
   uint32_t rows, k, parts;
 };
@@ -318,27 +325,33 @@ __global__ void __launch_bounds__(256) pieces_of_rows_kernel(const PiecesArgs a)
       for (int e = 0; e < 8; ++e) v[e / 4][e % 4] = k + e < a.k ? x[k + e] : 0.f;
     }
   };
-  auto most_of = [&](const f32x4 (&v)[2], uint32_t most) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e / 4][e % 4]));
-    return most;
-  };
   f32x4 held[kRowHeld][2];
-  uint32_t most = 0;
+  uint32_t most = 0, least = ~0u;
+  auto look_at = [&](const f32x4 (&v)[2]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = magnitude(v[e / 4][e % 4]);
+      most = max(most, x);
+      least = min(least, x - 1);   // of 0 the largest word
+    }
+  };
 #pragma unroll
   for (uint32_t i = 0; i < kRowHeld; ++i)
     if (i * 512 < a.k) {
       load(i * 512 + lane * 8, held[i]);
-      most = most_of(held[i], most);
+      look_at(held[i]);
     }
   for (uint32_t k = kRowHeld * 512; k < a.k; k += 512) {
     f32x4 v[2];
     load(k + lane * 8, v);
-    most = most_of(v, most);
+    look_at(v);
   }
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-  const int exponent = exponent_for(most);
+  for (int d = 32; d >= 1; d >>= 1) {
+    most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    least = min(least, (uint32_t)__shfl_xor((int)least, d));
+  }
+  const int exponent = exponent_for(most, least + 1), power = power_of(exponent);
   const int64_t at = (int64_t)blockIdx.y * a.rows + row;
   if (lane == 0) a.exponents[at] = exponent;
   char* to = a.pieces + at * runs * kPairRunBytes;
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(256) pieces_of_rows_kernel(const PiecesArgs a)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       _Float16 h, l;
-      split_pair_apart(exponent < kAbsentRow ? ldexpf(v[e / 4][e % 4], exponent) : 0.f, &h, &l);
+      split_pair_apart(exponent < kAbsentRow ? ldexpf(v[e / 4][e % 4], power) : 0.f, &h, &l);
       hi[e] = h;
       lo[e] = l;
     }
@@ -366,23 +379,30 @@ __global__ void __launch_bounds__(256) pieces_of_rows_kernel(const PiecesArgs a)
   }
 }
 
-// The largest magnitudes of columns, of a part of the k rows each.
+// The largest magnitudes of columns, and the least ones that are not 0, of a part of the k rows each.
 __global__ void __launch_bounds__(256) most_of_columns_kernel(const PiecesArgs a) {
-  __shared__ uint32_t found[4][64];
+  __shared__ uint32_t found[4][2][64];
   const uint32_t c = threadIdx.x % 64, column = blockIdx.x * 64 + c, each = (a.k + a.parts - 1) / a.parts, first = blockIdx.y * each;
   const float* x = a.x + (int64_t)blockIdx.z * a.stride + min(column, a.rows - 1);
-  uint32_t most = 0;
+  uint32_t most = 0, least = ~0u;
   for (uint32_t k0 = first + threadIdx.x / 64; k0 < min(first + each, a.k); k0 += 16) {
     float v[4];
 #pragma unroll
     for (uint32_t e = 0; e < 4; ++e) v[e] = x[(int64_t)min(k0 + e * 4, a.k - 1) * a.ld];   // once more is no harm
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) most = max(most, magnitude(v[e]));
+    for (uint32_t e = 0; e < 4; ++e) {
+      most = max(most, magnitude(v[e]));
+      least = min(least, magnitude(v[e]) - 1);   // of 0 the largest word
+    }
   }
-  found[threadIdx.x / 64][c] = most;
+  found[threadIdx.x / 64][0][c] = most;
+  found[threadIdx.x / 64][1][c] = least;
   __syncthreads();
-  if (threadIdx.x < 64 && column < a.rows)
-    a.partial[((int64_t)blockIdx.z * a.parts + blockIdx.y) * a.rows + column] = max(max(found[0][c], found[1][c]), max(found[2][c], found[3][c]));
+  if (threadIdx.x < 64 && column < a.rows) {
+    uint32_t* const to = a.partial + ((int64_t)blockIdx.z * a.parts + blockIdx.y) * 2 * a.rows + column;
+    to[0] = max(max(found[0][0][c], found[1][0][c]), max(found[2][0][c], found[3][0][c]));
+    to[a.rows] = min(min(found[0][1][c], found[1][1][c]), min(found[2][1][c], found[3][1][c]));
+  }
 }
 
 // 64 columns of 64 rows as pieces, k down the columns.
@@ -395,9 +415,13 @@ __global__ void __launch_bounds__(256) pieces_of_columns_kernel(const PiecesArgs
 #pragma unroll
   for (int i = 0; i < 16; ++i) values[i] = x[(int64_t)min(k0 + i * 4 + threadIdx.x / 64, a.k - 1) * a.ld];
   if (threadIdx.x < 64) {
-    uint32_t most = 0;
-    for (uint32_t part = 0; part < a.parts; ++part) most = max(most, a.partial[((int64_t)blockIdx.z * a.parts + part) * a.rows + column]);
-    exponents[c] = exponent_for(most);
+    uint32_t most = 0, least = ~0u;
+    for (uint32_t part = 0; part < a.parts; ++part) {
+      const uint32_t* const from = a.partial + ((int64_t)blockIdx.z * a.parts + part) * 2 * a.rows + column;
+      most = max(most, from[0]);
+      least = min(least, from[a.rows]);
+    }
+    exponents[c] = exponent_for(most, least + 1);
     if (blockIdx.y == 0 && column0 + c < a.rows) a.exponents[(int64_t)blockIdx.z * a.rows + column] = exponents[c];
   }
   __syncthreads();
@@ -406,7 +430,7 @@ __global__ void __launch_bounds__(256) pieces_of_columns_kernel(const PiecesArgs
   for (int i = 0; i < 16; ++i) {
     const uint32_t k = i * 4 + threadIdx.x / 64;
     _Float16 hi, lo;
-    split_pair_apart(k0 + k < a.k && exponent < kAbsentRow ? ldexpf(values[i], exponent) : 0.f, &hi, &lo);
+    split_pair_apart(k0 + k < a.k && exponent < kAbsentRow ? ldexpf(values[i], power_of(exponent)) : 0.f, &hi, &lo);
     cells[c][k] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
   }
   __syncthreads();
@@ -434,11 +458,13 @@ struct GatedPieces {
   uint32_t runs;
 };
 
-// A product in floats; stride: of the right operand's k.
+// A product in floats by a wave; stride: of the right operand's k.
 __device__ __forceinline__ float plain_product(const float* left, const float* right, int64_t stride, uint32_t k) {
   float sum = 0.f;
-#pragma unroll 1
-  for (uint32_t i = 0; i < k; ++i) sum += left[i] * right[i * stride];
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x % 64; i < k; i += 64) sum += left[i] * right[i * stride];
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
   return sum;
 }
 
@@ -448,6 +474,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const Gated
   static_assert(kGradient || NT % 2 == 0, "gates beside their ups");
   __shared__ __attribute__((aligned(16))) char lds[pair_tile_lds(BM, BN)];
   __shared__ int exponents[BM + BN];
+  __shared__ uint32_t again[BM][kColumns / 32];   // cells whose sums are formed from the floats
   TilePlace at;
   Group g;
   if (!place_of(p, &at) || !find_group(a.g, at.m_tile, BM, &g)) return;
@@ -469,8 +496,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const Gated
     } else {
       exponents[i] = pieces.right_exponents[right0 + right_row(i - BM)];
     }
-    found |= exponents[i] >= kAbsentRow;
+    found |= exponents[i] >= kAbsentRow || exponents[i] & 1;
   }
+  for (uint32_t i = tid; i < BM * (kColumns / 32); i += T) (&again[0][0])[i] = 0;
   found = __syncthreads_or(found);
   const PairRows<BM, BN, T> source(
       [&](uint32_t r) {
@@ -481,6 +509,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const Gated
   pair_f32x16 sum[2][MT][NT];
   pair_tile<BM, BN, WM, WN, 1, true>(source, pieces.runs, lds, tid, sum);
   // what has exponents
+  const float least = least_sum(a.g.k);
 #pragma unroll
   for (int at_u = 0; at_u < (kGradient ? NT : NT / 2); ++at_u) {
     const int u = kGradient ? at_u : 2 * at_u;
@@ -496,33 +525,46 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const Gated
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int left = exponents[m + row_at(r)];
-        skip |= (max(left, max(right, right_up)) >= kAbsentRow ? 1u : 0u) << r;
-        first[r] = ldexpf(sum[0][t][u][r] + sum[1][t][u][r] * (1.f / (1 << kPairApart)), -(left + right));
-        if constexpr (!kGradient) second[r] = ldexpf(sum[0][t][u + 1][r] + sum[1][t][u + 1][r] * (1.f / (1 << kPairApart)), -(left + right_up));
+        bool skipped = false;
+        auto cell = [&](const pair_f32x16 (&parts)[2][MT][NT], int of, int right) {
+          const float x = parts[0][t][of][r] + parts[1][t][of][r] * (1.f / (1 << kPairApart));
+          if (left == kRowOfNan || right == kRowOfNan || (left == kAbsentRow && right >= kAbsentRow)) return __builtin_nanf("");   // zeros by infinities, too
+          if (left == kAbsentRow) return 0.f;
+          skipped |= max(left, right) >= kAbsentRow || (((left | right) & 1) && min(left, right) != kRowOfZeros && fabsf(x) < least);
+          return ldexpf(x, -(power_of(left) + power_of(right)));
+        };
+        first[r] = cell(sum, u, right);
+        if constexpr (!kGradient) second[r] = cell(sum, u + 1, right_up);
+        skip |= (skipped ? 1u : 0u) << r;
+      }
+      if (found) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (skip >> r & 1) atomicOr(&again[m + row_at(r)][(column - col0) / 32], 1u << (column - col0) % 32);
       }
       if constexpr (kGradient) finish_gradient_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, skip);
       else finish_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, second, skip);
     }
   }
   if (!found) return;
-  // what has not, a cell after the other
+  // rows and columns of infinities, and what is small beside what it may be off by: a cell to a wave
+  __syncthreads();
   auto product = [&](uint32_t r, uint32_t n) -> float {
-    const int left = exponents[r], right = exponents[BM + n];
-    if (max(left, right) < kAbsentRow || (left != kAbsentRow && left != kRowOfNan && right != kRowOfNan)) {
-      const float* b = static_cast<const float*>(a.g.b) + (int64_t)g.index * a.g.b_stride + (int64_t)right_row(n) * (kGradient ? 1 : a.g.ldb);
-      return plain_product(static_cast<const float*>(a.g.a) + (int64_t)left_row(r) * a.g.lda, b, kGradient ? a.g.ldb : 1, a.g.k);
-    }
-    return left == kAbsentRow && right < kAbsentRow ? 0.f : __builtin_nanf("");   // zeros by what is not finite, too
+    if (exponents[r] == kRowOfNan || exponents[BM + n] == kRowOfNan) return __builtin_nanf("");
+    const float* b = static_cast<const float*>(a.g.b) + (int64_t)g.index * a.g.b_stride + (int64_t)right_row(n) * (kGradient ? 1 : a.g.ldb);
+    return plain_product(static_cast<const float*>(a.g.a) + (int64_t)left_row(r) * a.g.lda, b, kGradient ? a.g.ldb : 1, a.g.k);
   };
-#pragma unroll 1
-  for (uint32_t i = tid; i < BM * kColumns; i += T) {
-    const uint32_t r = i / kColumns, c = i % kColumns, n = kGradient ? c : c / 32 * 64 + c % 32;
-    if (row0 + r >= g.rows || col0 + c >= a.g.n) continue;
-    const int most = max(exponents[r], max(exponents[BM + n], kGradient ? 0 : exponents[BM + n + (kGradient ? 0 : 32)]));
-    if (most < kAbsentRow) continue;
-    const int64_t row = (int64_t)g.first + row0 + r;
-    if constexpr (kGradient) finish_gradient(a, row, col0 + c, product(r, n));
-    else finish(a, row, col0 + c, product(r, n), product(r, n + 32));
+  for (uint32_t i = wave; i < BM * (kColumns / 32); i += WM * WN) {
+    const uint32_t r = i / (kColumns / 32), c0 = i % (kColumns / 32) * 32;
+    if (row0 + r >= g.rows) break;
+    for (uint32_t cells = __builtin_amdgcn_readfirstlane(again[r][c0 / 32]); cells; cells &= cells - 1) {
+      const uint32_t c = c0 + __builtin_ctz(cells), n = kGradient ? c : c / 32 * 64 + c % 32;
+      const int64_t row = (int64_t)g.first + row0 + r;
+      const float x = product(r, n), y = kGradient ? 0.f : product(r, n + (kGradient ? 0 : 32));
+      if (lane != 0) continue;
+      if constexpr (kGradient) finish_gradient(a, row, col0 + c, x);
+      else finish(a, row, col0 + c, x, y);
+    }
   }
 }
 
@@ -765,7 +807,7 @@ template <bool kGradient>
 bool run_pairs(hipStream_t s, const GatedArgs& a, const Shape& shape, int64_t left_rows, int64_t all_groups) {
   const int64_t runs = ceil_div(shape.k, kPairRun), right_rows = all_groups * shape.stored, parts = std::min<int64_t>(32, ceil_div(shape.k, 64));
   const int64_t left_bytes = aligned(left_rows * runs * kPairRunBytes), right_bytes = aligned(right_rows * runs * kPairRunBytes);
-  const int64_t partial_bytes = kGradient ? aligned(right_rows * parts * 4) : 0;
+  const int64_t partial_bytes = kGradient ? aligned(right_rows * parts * 8) : 0;
   const ProductScratch scratch(s, (size_t)(left_bytes + right_bytes + aligned(left_rows * 4) + aligned(right_rows * 4) + partial_bytes));
   char* const base = static_cast<char*>(scratch.get());
   if (!base) return false;

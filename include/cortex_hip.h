@@ -655,7 +655,7 @@ int ct_grouped_gemm_weights(void* stream, void* c, int64_t c_colstride, int64_t 
  * ct_gated_gemm_gradient needs (NULL: it is not stored).  An index outside a is a row of zeros.  No result overlaps an operand or the other.
  * Sums and scratch memory are those of ct_grouped_gemm; but float products of many rows are formed of two halves to a float, each row of
  * a and of b_e with a power of two of its own: an element is held to 2^-23 of itself, or to 2^-51 of the largest of its row, whichever is
- * more, and sums are float ones.  They take scratch memory for the pieces, 4 bytes to an element of a and b, up to 256 MiB, and are
+ * more; sums that are small beside the latter are formed once more from the floats.  Sums are float ones.  They take scratch memory for the pieces, 4 bytes to an element of a and b, up to 256 MiB, and are
  * formed as ct_grouped_gemm's beyond that.  f is evaluated in the tensor's type. */
 typedef enum ct_gate_t {
   CT_GATE_LOGISTIC = 0, /* 1 / (1 + exp(-x)) */

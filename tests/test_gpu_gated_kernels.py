@@ -6,7 +6,7 @@ import pytest
 
 from cortex_amd import blocks
 from cortex_amd import capi
-from test_gpu_blocks import NUMPY, UNIT, Owned, read, stream  # noqa: F401
+from test_gpu_blocks import NUMPY, UNIT, Owned, close, read, stream  # noqa: F401
 from test_gpu_gated import check
 
 pytestmark = pytest.mark.gpu
@@ -86,4 +86,53 @@ def test_floats_beyond_the_range_of_halves(stream, rows, hidden, kernel):  # noq
     blocks.gated_gemm(inner, pre, D.tensor(x), D.tensor(weights), activation="relu")
     assert capi.last_kernel() == kernel
     assert np.all(read(pre) == 32.0) and np.all(read(inner) == 1024.0)
+    D.free()
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_large_elements_that_meet_none(stream, grouped):  # noqa: F811
+    """Rows of both operands with one element 2^40 above the others, which meets a zero or an element as far below: what the others come to is
+    held to the bar of a float sum.  Rows of zeros, absent rows, and tiles without such rows beside them; in place, too."""
+    D = owned("float")
+    rng = np.random.default_rng(17)
+    rows, width, hidden = 3000, 1000, 2300
+    x = rng.standard_normal((rows, width)).astype(np.float32)
+    weights = (rng.standard_normal((2 * hidden, width)) / 32).astype(np.float32)
+    x[100:1400, 0] *= np.float32(2.0 ** 40)
+    weights[:, 0] *= np.where(np.arange(2 * hidden) % 3 == 0, 0, np.float32(2.0 ** -40)).astype(np.float32)
+    weights[500:520, 1] *= np.float32(2.0 ** 45)
+    x[:, 1] = 0
+    x[7], x[1200], weights[3], weights[hidden + 600] = 0, 0, 0, 0
+    index = np.arange(rows)
+    index[[8, 700, 2999]] = -1, rows, rows + 5
+    inner, pre = D.tensor(np.zeros((rows, hidden))), D.tensor(np.zeros((rows, 2 * hidden)))
+    if grouped:
+        blocks.gated_gemm(inner, pre, D.tensor(x), D.tensor(np.stack([weights, -weights])), D.tensor([0, 1300, rows], "int"), D.tensor(index, "int"),
+                          activation="relu")
+    else:
+        blocks.gated_gemm(inner, pre, D.tensor(x), D.tensor(weights), activation="relu")
+    assert capi.last_kernel() == "gated_pairs"
+    taken = x.astype(np.float64)
+    if grouped:
+        taken[[8, 700, 2999]] = 0
+        taken[1300:] *= -1
+    w = weights.astype(np.float64)
+    got = read(pre)
+    close(got, taken @ w.T, (width + 4) * D.u * (abs(taken) @ abs(w).T) + 2.0 ** -149, 1.0)
+    assert np.array_equal(read(inner), np.maximum(got[:, :hidden], 0) * got[:, hidden:])
+    d = rng.standard_normal((rows, width)).astype(np.float32)
+    back = rng.standard_normal((width, hidden)).astype(np.float32)
+    d[50:900, 3] *= np.float32(2.0 ** 41)
+    back[3] = np.where(np.arange(hidden) % 4 == 0, 0, back[3] * np.float32(2.0 ** -41))
+    back[11, 40:70] *= np.float32(2.0 ** 44)
+    d[:, 11], d[77], back[:, 55] = 0, 0, 0
+    ones = D.tensor(np.ones((rows, 2 * hidden)))
+    args = (D.tensor(back),) if not grouped else (D.tensor(np.stack([back, back])),)
+    blocks.gated_gemm_gradient(ones, None, D.tensor(d), *args, ones, *((D.tensor([0, 1700, rows], "int"),) if grouped else ()), activation="relu")
+    assert capi.last_kernel() == "gated_gradient_pairs"
+    d, back = d.astype(np.float64), back.astype(np.float64)
+    want, bar = d @ back, (width + 4) * D.u * (abs(d) @ abs(back)) + 2.0 ** -149
+    got = read(ones)
+    close(got[:, :hidden], want, bar, 1.0)
+    close(got[:, hidden:], want, bar, 1.0)
     D.free()
