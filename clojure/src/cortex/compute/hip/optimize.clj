@@ -10,9 +10,10 @@
               the parameter buffer's offset inside the flat optimizer state (adam.clj:132-133)
     Adadelta  both accumulators addressed at the parameter offset (AdadeltaOptimizer.java:42-43)
     SGD       four tensor calls (sgd.clj:16-40), so the :cuda method's body serves unchanged
-    Muon      no counterpart in the reference: the momentum of a matrix made orthogonal by Newton-Schulz products
+    Muon      no counterpart in the reference: the momentum of a matrix made orthogonal by Newton-Schulz products; what is no matrix,
+              biases for instance, takes another optimizer's step
   UNEXERCISED (no JVM in the build image)."
-  (:require [cortex.optimize :refer [PGradientOptimizer create-optimizer]]
+  (:require [cortex.optimize :refer [PGradientOptimizer batch-update compute-parameters! create-optimizer]]
             [cortex.optimize.sgd]
             [cortex.compute.math :as math]
             [cortex.compute.driver :as drv]
@@ -118,33 +119,48 @@
            coefficients (int (count triples)) (double epsilon) (->ptr workspace) (long (dtype/ecount workspace))
            (ffi/dtype-code output))))
 
-(defrecord HipMuon [backend optimizer workspaces]
+(defn- steps->triples
+  "Three coefficients to each of the steps: of one triple for all of them, or of one to each."
+  [steps coefficients]
+  (let [triples (if (number? (first coefficients)) (repeat steps coefficients) coefficients)]
+    (when-not (and (= (long steps) (count triples)) (every? #(= 3 (count %)) triples))
+      (throw (ex-info "Muon: three coefficients, or three to each step" {:steps steps :coefficients coefficients})))
+    triples))
+
+(def ^:private default-vectors {:type :adam :alpha 0.001 :beta1 0.9 :beta2 0.999 :epsilon 1e-8})
+
+;; A network hands all of its parameters to one optimizer.  Those that are no matrices take the step of `vectors`, another optimizer, whose
+;; state lies beside :momentum-vals (of Adam :m and :v).
+(defrecord HipMuon [backend optimizer vectors workspaces]
   PGradientOptimizer
-  (batch-update [this _] this)
-  (compute-parameters! [this {:keys [momentum-vals]} gradient-alpha offset gradient parameters]
-    (let [{:keys [alpha momentum nesterov steps coefficients epsilon weight-decay]} optimizer
-          datatype (dtype/get-datatype backend)
-          stream (compute-backend/get-stream)
-          [rows columns :as shape] (m/shape parameters)
-          triples (triples->native (repeat steps coefficients))]
-      (when-not (= 2 (count shape))
-        (throw (ex-info "Muon is for matrices" {:shape shape})))
-      (ensure-datatype datatype gradient parameters momentum-vals)
-      (select-device! stream)
-      (let [need (orthogonalize-workspace datatype 1 rows columns)
-            ;; kept, the smaller ones too: a recorded graph may still write to them
-            workspace (or (first (filter #(>= (long (dtype/ecount %)) need) @workspaces))
-                          (let [fresh (drv/allocate-device-buffer need :byte)]
-                            (swap! workspaces conj fresh)
-                            fresh))]
-        (call! "ct_muon_step" (:handle stream) (int (ffi/datatype->code datatype)) (double alpha) (double momentum)
-               (ffi/bool->int nesterov) (double weight-decay) (double gradient-alpha) triples (int steps) (double epsilon)
-               (->ptr (->buffer gradient)) (->ptr (->buffer parameters)) (->ptr (->buffer momentum-vals (long offset)))
-               (long 1) (long rows) (long columns) (->ptr workspace) (long (dtype/ecount workspace)))))))
+  (batch-update [this optimizer-parameters]
+    (update this :vectors #(batch-update % optimizer-parameters)))
+  (compute-parameters! [this {:keys [momentum-vals] :as state} gradient-alpha offset gradient parameters]
+    (let [shape (vec (m/shape parameters))]
+      (if-not (<= 2 (count shape) 3)
+        (compute-parameters! vectors state gradient-alpha offset gradient parameters)
+        (let [{:keys [alpha momentum nesterov steps coefficients epsilon weight-decay]} optimizer
+              datatype (dtype/get-datatype backend)
+              stream (compute-backend/get-stream)
+              [n-matrices rows columns] (if (= 3 (count shape)) shape (into [1] shape))
+              triples (triples->native (steps->triples steps coefficients))]
+          (ensure-datatype datatype gradient parameters momentum-vals)
+          (select-device! stream)
+          (let [need (orthogonalize-workspace datatype n-matrices rows columns)
+                ;; kept, the smaller ones too: a recorded graph may still write to them
+                workspace (or (first (filter #(>= (long (dtype/ecount %)) need) @workspaces))
+                              (let [fresh (drv/allocate-device-buffer need :byte)]
+                                (swap! workspaces conj fresh)
+                                fresh))]
+            (call! "ct_muon_step" (:handle stream) (int (ffi/datatype->code datatype)) (double alpha) (double momentum)
+                   (ffi/bool->int nesterov) (double weight-decay) (double gradient-alpha) triples (int steps) (double epsilon)
+                   (->ptr (->buffer gradient)) (->ptr (->buffer parameters)) (->ptr (->buffer momentum-vals (long offset)))
+                   (long n-matrices) (long rows) (long columns) (->ptr workspace) (long (dtype/ecount workspace)))))))))
 
 (defmethod create-optimizer [:hip :muon]
   [backend optimizer]
   (->HipMuon backend (merge {:alpha 0.02 :momentum 0.95 :nesterov true :steps 5 :coefficients [3.4445 -4.7750 2.0315]
                              :epsilon 1e-7 :weight-decay 0.0}
                             optimizer)
+             (create-optimizer backend (merge default-vectors (:vectors optimizer)))
              (atom [])))
