@@ -258,7 +258,11 @@ int ct_memory_info(size_t* free_bytes, size_t* total_bytes) {
 int ct_malloc(void** ptr, size_t bytes) {
   CT_REQUIRE(ptr != nullptr, "ct_malloc: null output");
   *ptr = nullptr;
-  CT_HIP(hipMalloc(ptr, bytes ? bytes : 1));
+  const hipError_t e = hipMalloc(ptr, bytes ? bytes : 1);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();   // said here: the next launch's check is not to find it
+    return set_error(CT_ERR_HIP, "hipMalloc(ptr, bytes ? bytes : 1) failed: %s", hipGetErrorString(e));
+  }
   return CT_OK;
 }
 

@@ -238,6 +238,9 @@ def orthogonalize(backend: Backend, output, input, *, alpha=1.0, beta=0.0, steps
             workspace.release()
 
 
+_MOST_GROWTH = 64 << 20
+
+
 @dataclasses.dataclass
 class Muon:
     """Momentum for matrices, made orthogonal before it is taken off the parameters: of a matrix [rows, columns]
@@ -252,14 +255,30 @@ class Muon:
     backend: Backend
     optimizer: dict
     _workspaces: list = dataclasses.field(default_factory=list)
+    _refused: int = None     # bytes that there was no memory for
 
     def batch_update(self, optimizer_parameters=None) -> "Muon":
         return self
 
-    def _workspace(self, need: int):
-        have = self._workspaces[-1].ecount() if self._workspaces else 0
-        if not self._workspaces or have < need:
-            self._workspaces.append(self.backend.stream.get_device().allocate_device_buffer(max(1, need, 2 * have), "byte"))
+    def _workspace(self, *shape):
+        """A buffer for a step of such matrices, kept.  Small ones grow by twice at least, so that there are few; where there is no memory for as
+        much as fills the chip, what one matrix takes serves, and the matrices take turns."""
+        stream, have = self.backend.stream, self._workspaces[-1].ecount() if self._workspaces else 0
+        need = max(1, stream.orthogonalize_workspace(*shape, self.backend.datatype))
+        if have >= need:
+            return self._workspaces[-1]
+        least = max(1, stream.orthogonalize_workspace(min(shape[0], 1), *shape[1:], self.backend.datatype))
+        sizes = [n for n in (max(need, min(2 * have, _MOST_GROWTH)), need) if n < (self._refused or n + 1)]
+        for size in dict.fromkeys([*sizes, least]):
+            if size <= have:
+                break
+            try:
+                self._workspaces.append(stream.get_device().allocate_device_buffer(size, "byte"))
+                break
+            except capi.CortexHipError as e:
+                if size == least or "out of memory" not in e.message:
+                    raise
+                self._refused = size     # asked for once: each further step would wait for the same answer
         return self._workspaces[-1]
 
     def compute_parameters(self, state: dict, gradient_alpha, offset: int, gradient, parameters) -> None:
@@ -275,7 +294,7 @@ class Muon:
         if any(x.device is not p.device for x in (g, v)):
             raise ValueError(f"{name}: buffers are not all on the same device")
         steps_of = _steps_of(o["coefficients"], o["steps"])
-        workspace = self._workspace(stream.orthogonalize_workspace(*shape, self.backend.datatype))
+        workspace = self._workspace(*shape)
         stream.muon_step(o["alpha"], o["momentum"], o["nesterov"], o["weight-decay"], gradient_alpha, steps_of, o["epsilon"], g, p,
                          v.sub_buffer(offset, n), *shape, workspace)
 

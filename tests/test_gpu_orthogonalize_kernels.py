@@ -287,3 +287,33 @@ def test_magnitudes_over_the_whole_range(D):
         assert np.all(np.isfinite(got))
         off = np.linalg.norm(got - want, axis=1 - short)
         assert np.all(off <= bars[short] + 2.0 ** -149 * np.sqrt(max(shape)))
+
+
+def test_memory_that_is_refused(D):
+    """A step whose workspace there is no memory for takes a smaller one, and neither it nor what follows reports the refusal."""
+    device, shape = D.backend.stream.get_device(), (6, 90, 70)
+    one = D.backend.stream.orthogonalize_workspace(1, *shape[1:], "float")
+
+    class Little:
+        def allocate_device_buffer(self, n, datatype):
+            return device.allocate_device_buffer(n if n <= one else 1 << 50, datatype)
+
+    class Stream:
+        def __getattr__(self, name):
+            return getattr(D.backend.stream, name)
+
+        def get_device(self):
+            return Little()
+
+    results = []
+    for stream in (D.backend.stream, Stream()):
+        data = [np.asarray(gradient(np.random.default_rng(i), *shape), np.float32) for i in range(3)]
+        g, p, v = map(D.tensor, data)
+        optimizer = optimize.create_optimizer(optimize.Backend(stream, "float"), optimize.muon())
+        for _ in range(2):
+            optimizer.compute_parameters({"momentum-vals": v}, 1.0, 0, g, p)
+        results.append((read(p), read(v)))
+        assert [w.ecount() for w in optimizer._workspaces] == [one if stream is not D.backend.stream else 6 * one]
+    assert np.array_equal(results[0][1], results[1][1])
+    for i in range(shape[0]):     # other tiles: sums in another order, 150 half steps of a float cover twice the bar of either
+        assert np.linalg.norm(results[0][0][i] - results[1][0][i]) <= 150 * U * np.linalg.norm(results[0][0][i])
