@@ -110,14 +110,18 @@ __device__ __forceinline__ double sum_of_block(double x, double* lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-// The sums of squares of parts of a matrix, in double; of a step, the momentum before them.  One read of what there is, a write of the
-// momentum: bound by memory.
-template <class T>
+// The sums of squares of parts of a matrix of doubles; of a step, the momentum before them.  One read of what there is, a write of the
+// momentum: bound by memory.  Squares of doubles may be no doubles: those of what is beyond 2^480, and below 2^-480, are summed apart, of
+// 2^-600 and of 2^600 as much, [matrix][these three][part].
+constexpr double kLargeDouble = 0x1p480, kSmallDouble = 0x1p-480;
+constexpr int kDoubleShift = 600;
+
 __global__ void __launch_bounds__(256) start_norm_kernel(const StartArgs a, uint32_t parts, uint64_t each, bool dense) {
+  using T = double;
   __shared__ double lds[4];
   const int64_t base = (int64_t)blockIdx.y * a.stride;
   const uint64_t cells = (uint64_t)a.rows * a.columns, first = blockIdx.x * each, end = min(first + each, cells);
-  double sum = 0.0;
+  double sum = 0.0, large = 0.0, small = 0.0;
   for (uint64_t i0 = first + threadIdx.x; i0 < end; i0 += 4 * 256) {
     T x[4], g[4];
     int64_t at[4];
@@ -137,11 +141,58 @@ __global__ void __launch_bounds__(256) start_norm_kernel(const StartArgs a, uint
         static_cast<T*>(a.momentum)[at[e]] = x[e];
         if (a.nesterov) x[e] = step + (T)a.decay * x[e];
       }
-      sum += (double)x[e] * (double)x[e];
+      const double size = fabs(x[e]);
+      if (size >= kLargeDouble) {
+        const double y = ldexp(x[e], -kDoubleShift);
+        large += y * y;
+      } else if (size < kSmallDouble) {
+        const double y = ldexp(x[e], kDoubleShift);
+        small += y * y;
+      } else {
+        sum += x[e] * x[e];
+      }
     }
   }
+  double* const to = a.partial + (int64_t)blockIdx.y * 3 * kParts + blockIdx.x;
   const double total = sum_of_block(sum, lds);
-  if (threadIdx.x == 0) a.partial[(int64_t)blockIdx.y * kParts + blockIdx.x] = total;
+  if (threadIdx.x == 0) to[0] = total;
+  __syncthreads();
+  const double total_large = sum_of_block(large, lds);
+  if (threadIdx.x == 0) to[kParts] = total_large;
+  __syncthreads();
+  const double total_small = sum_of_block(small, lds);
+  if (threadIdx.x == 0) to[2 * kParts] = total_small;
+}
+
+// 1 / (|X| + epsilon) is factor * 2^power.
+struct InverseNorm {
+  double factor;
+  int power;
+};
+__device__ __forceinline__ InverseNorm inverse_norm_of_doubles(const StartArgs& a, uint32_t matrix, uint32_t parts, double* lds) {
+  double x[3] = {};
+#pragma unroll
+  for (uint32_t b = 0; b < 3; ++b)
+#pragma unroll
+    for (uint32_t i = 0; i < kParts / 256; ++i) {
+      const uint32_t at = i * 256 + threadIdx.x;
+      const double y = a.partial[((int64_t)matrix * 3 + b) * kParts + min(at, parts - 1)];
+      x[b] += at < parts ? y : 0.0;
+    }
+  const bool any_large = __syncthreads_or(x[1] != 0.0), any_small = __syncthreads_or(x[2] != 0.0);
+  double sum = sum_of_block(x[0], lds);
+  if (any_large) {
+    __syncthreads();
+    sum = sum_of_block(x[1], lds) + ldexp(sum, -2 * kDoubleShift);
+    return {1.0 / (sqrt(sum) + ldexp(a.epsilon, -kDoubleShift)), -kDoubleShift};
+  }
+  if (any_small) {
+    __syncthreads();
+    const double small = sum_of_block(x[2], lds);
+    if (sum == 0.0) return {1.0 / (sqrt(small) + ldexp(a.epsilon, kDoubleShift)), kDoubleShift};
+    sum += ldexp(small, -2 * kDoubleShift);
+  }
+  return {1.0 / (sqrt(sum) + a.epsilon), 0};
 }
 
 __device__ __forceinline__ double inverse_norm(const StartArgs& a, uint32_t matrix, uint32_t parts, double* lds) {
@@ -385,11 +436,11 @@ __global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, ui
 __global__ void __launch_bounds__(256) start_double_kernel(const StartArgs a, uint32_t parts, double* to, int64_t stride, uint32_t ld,
                                                            FastDiv columns_fd, uint32_t cells) {
   __shared__ double lds[4];
-  const double factor = inverse_norm(a, blockIdx.y, parts, lds);
+  const InverseNorm inverse = inverse_norm_of_doubles(a, blockIdx.y, parts, lds);
   for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < cells; i += gridDim.x * 256) {
     uint32_t row, column;
     columns_fd.divmod(i, row, column);
-    to[blockIdx.y * stride + (int64_t)row * ld + column] = start_value<double>(a, (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld + column) * factor;
+    to[blockIdx.y * stride + (int64_t)row * ld + column] = ldexp(start_value<double>(a, (int64_t)blockIdx.y * a.stride + (int64_t)row * a.ld + column), inverse.power) * inverse.factor;
   }
 }
 
@@ -1092,7 +1143,7 @@ struct Layout {
       x = turned = aligned(rows * ldx * 8);
       square = aligned(m * ld_square * 8);
     }
-    partial = kParts * 8;
+    partial = (dtype == CT_F32 ? 1 : 3) * kParts * 8;
     row_words = ceil_div(m, 64) * 64;
     column_words = ceil_div(n, 64) * 64;
     matrix = (dtype == CT_F32 ? x + 3 * row_words * 4 + 4 * column_words * 4 : 0) + 2 * turned + 2 * square + partial;
@@ -1473,7 +1524,7 @@ int run_double(hipStream_t s, const Request& r, const Layout& l, int64_t at_once
     StartArgs start = r.start;
     start.move(first * start.stride * 8);
     start.partial = partial;
-    hipLaunchKernelGGL((start_norm_kernel<double>), dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
+    hipLaunchKernelGGL(start_norm_kernel, dim3((uint32_t)parts, (uint32_t)count), dim3(256), 0, s, start, (uint32_t)parts, each,
                        start.ld == r.columns);
     hipLaunchKernelGGL(start_double_kernel, dim3((uint32_t)std::min<int64_t>(ceil_div(cells, 256), 4096), (uint32_t)count), dim3(256), 0, s, start,
                        (uint32_t)parts, x[0], l.x / 8, (uint32_t)l.ldx, FastDiv((uint32_t)r.columns), (uint32_t)cells);

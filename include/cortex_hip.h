@@ -739,7 +739,8 @@ int ct_adadelta_step(void* stream, int dtype, double decay, double epsilon, void
  * stream; calls that overlap in time need one each.  ct_orthogonalize_workspace gives the bytes with which all launches fill the
  * chip; with fewer, down to those that it gives for one matrix, the matrices take turns.
  * Each side is 2^21 at most, a matrix below 2^31 elements, 1 <= steps <= 64; coefficients that let a singular value grow
- * beyond 2^40, of floats beyond 2^30 before the last step, are refused.  The squares are summed in double.  An infinity or a NaN makes its matrix NaN, its matrix only.
+ * beyond 2^40, of floats beyond 2^30 before the last step, are refused.  The squares are summed in double, so that none of any number overflows or vanishes.
+ * An infinity or a NaN makes its matrix NaN, its matrix only.
  * Float: sums are float ones of products of two halves to an element, with a power of two to each row and each column taken out, so that
  * rows and columns far below the others have results as accurate, of their own size, as products of floats give (columns on the longer side
  * down to 2^-100 of the others).  An element that is 2^-28 or less of the largest of its row and of its column may count as 0.

@@ -317,3 +317,31 @@ def test_memory_that_is_refused(D):
     assert np.array_equal(results[0][1], results[1][1])
     for i in range(shape[0]):     # other tiles: sums in another order, 150 half steps of a float cover twice the bar of either
         assert np.linalg.norm(results[0][0][i] - results[1][0][i]) <= 150 * U * np.linalg.norm(results[0][0][i])
+
+
+@pytest.mark.parametrize("shape", [(48, 40), (130, 300), (3, 3000)], ids=str)
+def test_doubles_whose_squares_are_none(stream, shape):  # noqa: F811
+    """The norm of matrices of which squares overflow, or vanish: powers of two apart they have the same results."""
+    D = Owned("double")
+    backend = optimize.Backend(stream, "double")
+    rng = np.random.default_rng(52)
+    data = gradient(rng, 1, *shape)[0]
+    want, bar = bar_of(data, UNIT["double"], epsilon=0.0)
+    out = D.tensor(np.zeros(shape))
+    for exponent in (-980, -600, -490, 490, 600, 1015):
+        optimize.orthogonalize(backend, out, D.tensor(np.ldexp(data, exponent)), epsilon=0.0)
+        near(read(out), want, bar, exponent)
+    # some of each kind: the large ones' norm, to which the others still belong
+    for exponent in (-480, 475, 480, 485):
+        mixed = data * 2.0 ** rng.integers(-12, 13, shape[0])[:, None]
+        want, bar = bar_of(mixed, UNIT["double"], epsilon=0.0)
+        optimize.orthogonalize(backend, out, D.tensor(np.ldexp(mixed, exponent)), epsilon=0.0)
+        near(read(out), want, bar, exponent)
+    # epsilon is added to the norm as it is
+    for exponent in (-500, 500):
+        optimize.orthogonalize(backend, out, D.tensor(np.ldexp(data, exponent)), epsilon=float(np.ldexp(np.linalg.norm(data), exponent)))
+        want, bar = bar_of(data, UNIT["double"], epsilon=np.linalg.norm(data))
+        near(read(out), want, bar, ("epsilon", exponent))
+    optimize.orthogonalize(backend, out, D.tensor(np.ldexp(data, -1000)))     # 1e-7 beside which the norm is nothing
+    assert np.all(abs(read(out)) <= 1e-290)
+    D.free()
