@@ -209,6 +209,7 @@ __device__ __forceinline__ double inverse_norm(const StartArgs& a, uint32_t matr
 // Powers of two of the rows and columns of X on its shorter side, in the workspace: [matrix][..] each.
 struct Exponents {
   int *rows, *columns;            // X = 2^(rows) Y, no element of a column of Y above 2^(columns)
+  int* rows_of_input;             // rows' without that of 1 / (|input| + epsilon)
   double* squares;                // sums over strips of the input's rows, [matrix][strip][row]
   uint32_t* most_columns;         // bits of the largest magnitudes in columns of Y, times 2^kPairTop
   int64_t stride_squares;
@@ -313,8 +314,8 @@ __global__ void __launch_bounds__(256) start_scan_kernel(const StartArgs a, uint
   if (threadIdx.x == 0) a.partial[(int64_t)blockIdx.z * kParts + part] = total;
 }
 
-// The exponents of `count` rows of the input from m0 on, in LDS.
-__device__ __forceinline__ void rows_of_input(const Exponents& e, uint32_t m, uint32_t m0, uint32_t count, int* rows) {
+// The exponents of `count` rows of the input from m0 on, in LDS, and for the next launch.
+__device__ __forceinline__ void rows_of_input(const Exponents& e, uint32_t m, uint32_t m0, uint32_t count, int* rows, bool keep) {
   for (uint32_t i = threadIdx.x; i < count; i += 256) {
     const double* from = e.squares + blockIdx.z * e.stride_squares + min(m0 + i, m - 1);
     double x[kMostStrips], sum = 0.0;
@@ -323,6 +324,7 @@ __device__ __forceinline__ void rows_of_input(const Exponents& e, uint32_t m, ui
 #pragma unroll
     for (uint32_t strip = 0; strip < kMostStrips; ++strip) sum += strip < e.strips ? x[strip] : 0.0;
     rows[i] = exponent_of_root(sum);
+    if (keep && m0 + i < m) e.rows_of_input[blockIdx.z * (int64_t)e.stride_rows + m0 + i] = rows[i];
   }
 }
 
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(256) start_columns_kernel(const StartArgs a, u
   const uint32_t m = kTall ? a.columns : a.rows, n = kTall ? a.rows : a.columns, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const uint32_t n0 = blockIdx.y * 64, first = blockIdx.x * tiles * 64, end = min(first + tiles * 64, m);
   if (threadIdx.x < 64) most[lane] = 0;
-  rows_of_input(e, m, first, tiles * 64, rows);
+  rows_of_input(e, m, first, tiles * 64, rows, blockIdx.y == 0);
   uint32_t found[16] = {};
   bool ready = false;
   for (uint32_t m0 = first; m0 < end; m0 += 64) {
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(256) start_pieces_kernel(const StartArgs a, ui
   for (uint32_t i = 0; i < 16; ++i) values[i] = start_value<float>(a, Square64<kTall>(a, m, n, m0, n0, i).at);
   const double factor = inverse_norm(a, matrix, parts, lds);
   const int of_factor = exponent_above(factor);
-  rows_of_input(e, m, m0, 64, of_short);
+  if (threadIdx.x < 64) of_short[threadIdx.x] = e.rows_of_input[(int64_t)matrix * e.stride_rows + min(m0 + threadIdx.x, m - 1)];
   if (threadIdx.x >= 64 && threadIdx.x < 128) {
     const uint32_t at = n0 + threadIdx.x % 64;
     const int64_t to = (int64_t)matrix * e.stride_columns + min(at, n - 1);
@@ -1370,17 +1372,19 @@ struct Request {
 };
 
 constexpr double kMostValue = 0x1p40;
-// Of floats, whose A A has values of the fourth power, before the last step; and what A is multiplied by to leave its scale is a float.
+// Of floats before the last step: M has the squares of these values, times what b and c are to a, and is made of floats.
 constexpr double kMostFloat = 0x1p30;
 
-// The norm, the exponents of rows and columns, and Y in pieces.  Strips are as many as fill the chip, those over the longer side kMostStrips at most.
+// The norm, the exponents of rows and columns, and Y in pieces.  Strips over the longer side are as many as fill the chip, kMostStrips at most; those over the
+// shorter one as long as leaves four blocks to a unit, for each block adds up its rows' squares first (sixteen of 2816 x 1024: 112 us, with eight blocks
+// 132, with 32 153).
 void launch_start(hipStream_t s, const StartArgs& a, Exponents e, uint32_t count, bool tall, char* by_rows, char* by_columns, int64_t stride_rows,
                   int64_t stride_columns) {
   const int64_t of_rows = ceil_div(a.rows, 64), of_columns = ceil_div(a.columns, 64), shorter = tall ? of_columns : of_rows, longer = tall ? of_rows : of_columns;
   const int64_t most = std::min<int64_t>({kMostStrips, kParts / shorter, std::max<int64_t>(1, 8 * kUnits / (count * shorter))}), tiles = ceil_div(longer, std::min(most, longer));
   e.strips = (uint32_t)ceil_div(longer, tiles);
   const uint32_t parts = (uint32_t)(e.strips * shorter);
-  const int64_t across = std::min<int64_t>({std::max<int64_t>(1, count * shorter * longer / (8 * kUnits)), shorter, kMostAcross});
+  const int64_t across = std::min<int64_t>({std::max<int64_t>(1, count * shorter * longer / (4 * kUnits)), shorter, kMostAcross});
   const dim3 over_longer(e.strips, (uint32_t)shorter, count), over_shorter((uint32_t)ceil_div(shorter, across), (uint32_t)longer, count);
   const dim3 all((uint32_t)of_columns, (uint32_t)of_rows, count);
   auto launch = [&](auto is_tall) {
@@ -1414,7 +1418,7 @@ int run_float(hipStream_t s, const Request& r, const Layout& l, int64_t at_once)
     start.move(first * start.stride * 4);
     start.partial = partial;
     // the sums of the input's rows are where Y by columns is next
-    const Exponents exponents{of_rows[0], of_columns[0], reinterpret_cast<double*>(turned[1]), most_of[0], l.turned / 8, (uint32_t)l.row_words,
+    const Exponents exponents{of_rows[0], of_columns[0], of_rows[1], reinterpret_cast<double*>(turned[1]), most_of[0], l.turned / 8, (uint32_t)l.row_words,
                               (uint32_t)l.column_words, 0};
     launch_start(s, start, exponents, (uint32_t)count, tall, tall ? turned[0] : x, tall ? x : turned[0], tall ? l.turned : l.x, tall ? l.x : l.turned);
     double most = 1.0;
