@@ -522,25 +522,32 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gated_pair_kernel(const Gated
       if (row0 + m >= g.rows) continue;
       float first[16], second[16];
       uint32_t skip = 0;
+      auto sum_of = [&](int of, int r) { return sum[0][t][of][r] + sum[1][t][of][r] * (1.f / (1 << kPairApart)); };
+      if (!found) {   // as mostly: nothing to look for
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int left = exponents[m + row_at(r)];
-        bool skipped = false;
-        auto cell = [&](const pair_f32x16 (&parts)[2][MT][NT], int of, int right) {
-          const float x = parts[0][t][of][r] + parts[1][t][of][r] * (1.f / (1 << kPairApart));
-          if (left == kRowOfNan || right == kRowOfNan || (left == kAbsentRow && right >= kAbsentRow)) return __builtin_nanf("");   // zeros by infinities, too
-          if (left == kAbsentRow) return 0.f;
-          skipped |= max(left, right) >= kAbsentRow || (((left | right) & 1) && min(left, right) != kRowOfZeros && fabsf(x) < least);
-          return ldexpf(x, -(power_of(left) + power_of(right)));
-        };
-        first[r] = cell(sum, u, right);
-        if constexpr (!kGradient) second[r] = cell(sum, u + 1, right_up);
-        skip |= (skipped ? 1u : 0u) << r;
-      }
-      if (found) {
+        for (int r = 0; r < 16; ++r) {
+          const int left = power_of(exponents[m + row_at(r)]);
+          first[r] = ldexpf(sum_of(u, r), -(left + power_of(right)));
+          if constexpr (!kGradient) second[r] = ldexpf(sum_of(u + 1, r), -(left + power_of(right_up)));
+        }
+      } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (skip >> r & 1) atomicOr(&again[m + row_at(r)][(column - col0) / 32], 1u << (column - col0) % 32);
+        for (int r = 0; r < 16; ++r) {
+          const int left = exponents[m + row_at(r)];
+          bool skipped = false;
+          auto cell = [&](int of, int right) {
+            const float x = sum_of(of, r);
+            if (left == kRowOfNan || right == kRowOfNan || (left == kAbsentRow && right >= kAbsentRow)) return __builtin_nanf("");   // zeros by infinities, too
+            if (left == kAbsentRow) return 0.f;
+            skipped |= max(left, right) >= kAbsentRow || (((left | right) & 1) && min(left, right) != kRowOfZeros && fabsf(x) < least);
+            return ldexpf(x, -(power_of(left) + power_of(right)));
+          };
+          first[r] = cell(u, right);
+          if constexpr (!kGradient) second[r] = cell(u + 1, right_up);
+          if (!skipped) continue;
+          skip |= 1u << r;
+          atomicOr(&again[m + row_at(r)][(column - col0) / 32], 1u << (column - col0) % 32);
+        }
       }
       if constexpr (kGradient) finish_gradient_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, skip);
       else finish_column(a, (int64_t)g.first + row0 + m, column, g.rows - row0 - m, first, second, skip);
