@@ -8,7 +8,7 @@
 // usual steps.  So A, the steps and Q X are in double, and coefficients and steps by which it would grow to a float's last bit
 // are not taken here (kMostFewChange).  For matrices of doubles there is no such wider type, and none of this.
 //
-// Bound by latency: 4 x 9 takes 16.5 us, 64 x 64 54, 64 x 8000 81 (65 x 65, in the products of halves, 71).  Of 64 rows 40 us are the steps,
+// Bound by latency: 4 x 9 takes 17 us, 64 x 64 54, 64 x 8000 74 (65 x 65, in the products of halves, 81).  Of 64 rows 40 us are the steps,
 // which one unit makes.  The products are v_mfma_f64_16x16x4_f64: of a lane's operands the row (or column) is lane % 16 and k lane / 16, of
 // its results the rows lane / 16 + 4 r and the column lane % 16.
 #include <algorithm>
