@@ -1346,15 +1346,14 @@ struct StepBounds {
     factor = most_of_factor(a, b, c, squares);
     next = most_of_step(a, b, c, squares);
     factor_exponent = exponent_of(factor);
-    // |b + c s|, and root(s) |b + c s|
-    const double of_rows = std::max(std::abs(b), std::abs(b + c * squares)), of_columns = std::max(most * of_rows, 0.0), largest = std::ldexp(1.0, exponent_of(most));
-    // M = a I + (b G + c G D D G) D^2, |G D D G| <= the norms of two rows of Y, at most 1, times squares
-    m_exponent = exponent_of(std::abs(a) + largest * largest * of_rows);
-    // A row of M times a column of Y: |a| of the column's largest; and the root of the sum of the squares of D, largest * root(m) at most, times
-    // that of (the rest of M's row) / D, which is a row of Y times (b + c X^T X) X^T; both as the row's exponent falls
+    // b G + c G D D G is Y (b I + c X^T X) Y^T, and D is at most `largest`
+    const double inner = std::max(std::abs(b), std::abs(b + c * squares)), largest = std::ldexp(1.0, exponent_of(most));
+    m_exponent = exponent_of(std::abs(a) + largest * largest * inner);
+    // A row of M times a column of Y, against the column's largest, as the row's exponent falls: |a|; and the root of the sum of the squares of D, at most
+    // root(m) * largest, times that of (the rest of M's row) / D, which is a row of Y times (b I + c X^T X) X^T
     const double fall = std::ldexp(1.0, kMostFall - factor_exponent);
-    const double rest = factor > 0 ? std::max(1.0 / factor, next > 0 ? most / next : 0.0) : 0.0;
-    growth = std::max(0, exponent_of(std::abs(a) * fall + std::sqrt((double)m) * largest * of_columns * std::min(fall, rest)));
+    const double of_norm = factor > 0 ? std::max(1.0 / factor, next > 0 ? most / next : 0.0) : 0.0;   // |y| as it falls: |x| / |x'|'s bound
+    growth = std::max(0, exponent_of(std::abs(a) * fall + std::sqrt((double)m) * largest * most * inner * std::min(fall, of_norm)));
   }
 };
 
